@@ -447,6 +447,75 @@ om_status om_attention_bwd_flash(om_ctx *ctx, const float *q, const float *k, co
                                  const float *mask, int mask_batched, const float *o, int ld_o, const float *stats,
                                  const float *g, int ld_g, float *dq, float *dk, float *dv, int ld_d, int B, int H,
                                  int L, int d, float scale, int acc);
+/* ---------------------------------------------------------------------------------------------- rotary positions */
+/* Rotary positions: pair i < rot / 2 of each head's first `rot` values turns by the angle pos * f_i,
+ *   y_a = amp (x_a cos - x_b sin),  y_b = amp (x_b cos + x_a sin),
+ * with (a, b) = (i, i + rot / 2) (OM_ROPE_HALF) or (2 i, 2 i + 1) (OM_ROPE_INTERLEAVED); a head's other values pass
+ * through. f_i = base^(-2 i / rot), changed by `scaling` for contexts longer than the trained one:
+ *   OM_ROPE_PLAIN   f_i as it is;
+ *   OM_ROPE_LINEAR  f_i / factor;
+ *   OM_ROPE_NTK     the base becomes base * factor^(rot / (rot - 2)) (rot > 2), which divides the slowest pair's f by factor;
+ *   OM_ROPE_BANDS   with turns = f_i * trained / (2 pi), the turns pair i makes in the trained context, and keep =
+ *                   clamp((turns - low) / (high - low), 0, 1): f_i * (keep + (1 - keep) / factor).
+ * amp multiplies the turned values (1 for none). The f_i are formed on the host in double, an angle's turns and their
+ * fractional part in double on the device, so positions up to 2^31 - 1 keep their angle within 4e-7. No counterpart in
+ * the reference, whose models learn their positions. */
+enum { OM_ROPE_HALF = 0, OM_ROPE_INTERLEAVED = 1 };
+enum { OM_ROPE_PLAIN = 0, OM_ROPE_LINEAR = 1, OM_ROPE_NTK = 2, OM_ROPE_BANDS = 3 };
+typedef struct {
+    int32_t layout, scaling, rot; /* rot even, 2 .. d */
+    float amplitude;
+    double base, factor, trained, low, high; /* base > 1; factor >= 1 unless plain; the rest for bands: trained > 0, low < high */
+} om_rope;
+/* y [rows, heads * d] (rows ld_y apart) = x (rows ld_x apart) turned. pos is a device array of `rows` positions (any
+ * int32, negative ones too) or NULL: row r then stands at pos0 + r % seq. y may be x itself with the same stride
+ * (the q and k columns of a packed projection turned in place, as one call over their heads together), else the two
+ * must not overlap. rows or heads may be 0. */
+om_status om_rope_fwd(om_ctx *ctx, const float *x, int ld_x, const int32_t *pos, int pos0, float *y, int ld_y,
+                      int rows, int seq, int heads, int d, const om_rope *rope);
+/* Its backward: dx (+)= the gradient g turned back (the transposed rotation, times amp; untouched values pass). dx may
+ * be g itself with the same stride when acc is 0. */
+om_status om_rope_bwd(om_ctx *ctx, const float *g, int ld_g, const int32_t *pos, int pos0, float *dx, int ld_dx,
+                      int rows, int seq, int heads, int d, const om_rope *rope, int acc);
+
+/* ---------------------------------------------------------------------------------------------- scored attention */
+/* Softmax attention whose scores follow a rule, over grouped heads: query head h reads key/value head
+ * h / (heads / kv_heads). q, o, g, dq are [B, lq, heads, d] (rows ld_q, ld_o, ld_g, ld_dq floats apart), k, v, dk, dv
+ * [B, lk, kv_heads, d] (rows ld_kv / ld_dkv apart), so the column blocks of a packed q|k|v projection are used in
+ * place. Query t stands at position i = t + lk - lq (the queries are the last lq of lk positions), key j at j:
+ *   x = scale * (q . k);  cap > 0: x = cap * tanh(x / cap);  slopes: x -= slopes[head] * |i - j|;
+ *   p = softmax of x over the keys the query sees, o = sum of p v.
+ * Query i of batch b sees key j when all that is given holds:
+ *   j <= i with causal, and |i - j| < window with window > 0; both waived for j < prefix[b] (prefix given);
+ *   q_doc[b][t] == k_doc[b][j] >= 0 with documents (both or neither; a negative id is padding, which sees nothing and
+ *   is seen by nothing).
+ * A query that sees nothing gives o = 0 and no gradient. What a query does not see has no effect on it, infinities and
+ * NaN included; its visible values follow IEEE rules. */
+typedef struct {
+    int32_t heads, kv_heads;
+    float scale;          /* 0 or NaN: 1 / sqrt(d) */
+    float cap;            /* 0: none */
+    int32_t causal;       /* 0 or 1 */
+    int32_t window;       /* 0: none */
+    const float *slopes;  /* device [heads], or NULL */
+    const int32_t *q_doc; /* device [B, lq], or NULL */
+    const int32_t *k_doc; /* device [B, lk], or NULL */
+    const int32_t *prefix; /* device [B], or NULL */
+} om_attention_scores;
+/* d from 1 to 256; B, lq and lk may be 0. stats (2 * B * heads * lq floats, or NULL when no backward follows) receives
+ * each row's reference exponent in log2 units and the inverse row sum, [B, heads, lq] each. Where rows or keys are few
+ * the keys are split over workgroups and joined in a second launch. Context scratch holds the split operands. No
+ * counterpart in the reference, whose Attention takes an additive mask tensor and equal heads (Ops.Layers.cs:746-807). */
+om_status om_attention_fwd_scored(om_ctx *ctx, const float *q, int ld_q, const float *k, const float *v, int ld_kv,
+                                  float *o, int ld_o, float *stats, int B, int lq, int lk, int d,
+                                  const om_attention_scores *scores);
+/* Its backward from the forward's o and stats: dq, dk, dv (any may be NULL), written, or added to when acc is set;
+ * dk and dv are the sums over a key head's query heads, in a fixed order. */
+om_status om_attention_bwd_scored(om_ctx *ctx, const float *q, int ld_q, const float *k, const float *v, int ld_kv,
+                                  const float *o, int ld_o, const float *stats, const float *g, int ld_g, float *dq,
+                                  int ld_dq, float *dk, float *dv, int ld_dkv, int B, int lq, int lk, int d,
+                                  const om_attention_scores *scores, int acc);
+
 /* ---------------------------------------------------------------------------------------------- convolution, pooling */
 /* Ops.Conv2d, groups 1, square stride/padding (Ops.Layers.cs:279-336; Conv.cs:54) as implicit GEMM on MFMA, and
  * ConvBackward (BackwardNn.cs:317-402): dx = col2im(W^T g) as an implicit GEMM over g, dw = g im2col(x) with a

@@ -105,6 +105,10 @@ _OM_SIGS = {
     "om_attention_bwd_ld": [vp, vp, vp, vp, ci, vp, vp, ci, vp, vp, vp, ci, vp, ci, ci, ci, ci, ci, f32, ci],
     "om_attention_fwd_fused": [vp, vp, vp, vp, ci, vp, ci, vp, ci, ci, ci, ci, ci, f32],
     "om_attention_bwd_fused": [vp, vp, vp, vp, ci, vp, ci, vp, ci, vp, vp, vp, ci, ci, ci, ci, ci, f32, ci],
+    "om_rope_fwd": [vp, vp, ci, vp, ci, vp, ci, ci, ci, ci, ci, vp],
+    "om_rope_bwd": [vp, vp, ci, vp, ci, vp, ci, ci, ci, ci, ci, vp, ci],
+    "om_attention_fwd_scored": [vp, vp, ci, vp, vp, ci, vp, ci, vp, ci, ci, ci, ci, vp],
+    "om_attention_bwd_scored": [vp, vp, ci, vp, vp, ci, vp, ci, vp, vp, ci, vp, ci, vp, vp, ci, ci, ci, ci, ci, vp, ci],
     "om_conv2d_fwd": [vp, vp, vp, vp, vp] + [ci] * 9,
     "om_conv2d_relu_fwd": [vp, vp, vp, vp, vp] + [ci] * 9,
     "om_conv2d_bwd": [vp, vp, vp, vp, vp, vp, vp] + [ci] * 9 + [ci, ci],
@@ -200,6 +204,16 @@ class om_linear_dw(C.Structure):
 
 class om_column_sum(C.Structure):
     _fields_ = [("part", vp), ("out", vp), ("chunks", i32), ("cols", i32), ("acc", i32)]
+
+
+class om_rope(C.Structure):
+    _fields_ = [("layout", i32), ("scaling", i32), ("rot", i32), ("amplitude", f32), ("base", C.c_double),
+                ("factor", C.c_double), ("trained", C.c_double), ("low", C.c_double), ("high", C.c_double)]
+
+
+class om_attention_scores(C.Structure):
+    _fields_ = [("heads", i32), ("kv_heads", i32), ("scale", f32), ("cap", f32), ("causal", i32), ("window", i32),
+                ("slopes", vp), ("q_doc", vp), ("k_doc", vp), ("prefix", vp)]
 
 
 class omt_scale(C.Structure):

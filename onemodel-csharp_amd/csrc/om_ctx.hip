@@ -32,6 +32,12 @@ om_status check_hip(om_ctx *ctx, hipError_t e, const char *what) {
     return fail(ctx, e == hipErrorOutOfMemory ? OM_E_OOM : OM_E_DEVICE, "%s: %s", what, hipGetErrorString(e));
 }
 
+om_status use_device(om_ctx *ctx) {
+    int now = -1;
+    if (hipGetDevice(&now) == hipSuccess && now == ctx->device) return OM_OK;
+    return check_hip(ctx, hipSetDevice(ctx->device), "hipSetDevice");
+}
+
 om_status refuse_in_capture(om_ctx *ctx, const char *what) {
     if (!ctx->cap) return OM_OK;
     return fail(ctx, OM_E_STATE, "%s: not possible inside a step-graph capture (it would wait for the device or read "
@@ -45,10 +51,12 @@ static om_status grow(om_ctx *ctx, float *&buf, uint64_t &have, uint64_t bytes, 
     }
     // Growth synchronises the stream, which a capture cannot hold; a step run once outside the capture has grown it.
     if (om_status s = refuse_in_capture(ctx, "context scratch growth")) return s;
-    // No kernel may still use the old buffer.
+    if (om_status d = use_device(ctx)) return d;
+    // No kernel may still use the old buffer, nor a captured graph that is launched again later.
     om_status s = check_hip(ctx, hipStreamSynchronize(ctx->stream), "scratch sync");
     if (s) return s;
-    if (buf) (void)hipFree(buf);
+    if (buf && ctx->captured) ctx->outgrown.push_back(buf);
+    else if (buf) (void)hipFree(buf);
     buf = nullptr;
     have = 0;
     uint64_t want = bytes < (64ull << 20) ? (64ull << 20) : bytes + (bytes >> 2);
@@ -148,6 +156,7 @@ om_status om_ctx_destroy(om_ctx *ctx) {
         for (auto &s : r.slabs) (void)hipFree(s.base);
     if (ctx->scratch) (void)hipFree(ctx->scratch);
     if (ctx->scratch2) (void)hipFree(ctx->scratch2);
+    for (float *b : ctx->outgrown) (void)hipFree(b);
     for (hipEvent_t e : ctx->probe_ev) (void)hipEventDestroy(e);
     (void)hipStreamDestroy(ctx->stream);
     delete ctx;
@@ -417,6 +426,7 @@ om_status om_graph_capture_begin(om_ctx *ctx) {
         return om::check_hip(ctx, e, "om_graph_capture_begin");
     }
     ctx->cap = g;
+    ctx->captured = true;
     hipLaunchKernelGGL(k_step_begin, dim3(1), dim3(64), 0, ctx->stream, (const om_step_block *)g->host, g->dev,
                        (uint64_t *)(g->host + sizeof(om_step_block)));
     om_status s = OM_LAUNCH_CHECK(ctx, "om_graph_capture_begin");

@@ -55,6 +55,10 @@ struct om_ctx {
     // (claimed by its first allocation-free call, released by om_ctx_destroy; -1 while it holds none).
     void *noalloc_scratch = nullptr;
     int noalloc_slot = -1;
+    // Scratch buffers outgrown after a step graph was captured on this context: the graph's launches still hold their
+    // addresses, so they live until om_ctx_destroy.
+    bool captured = false;
+    std::vector<float *> outgrown;
     // How the GELU epilogues of products evaluate erf and exp (om_ctx_set_gelu).
     int gelu_mode = OM_GELU_FAST;
     int num_cus = 256;
@@ -149,6 +153,8 @@ inline const char *tuning_env(const char *name) {
 }
 // OM_E_STATE with a message when a step graph is being captured on ctx's stream (for calls a graph cannot hold).
 om_status refuse_in_capture(om_ctx *ctx, const char *what);
+// Makes the context's device the current one for the launches and allocations that follow, if it is not.
+om_status use_device(om_ctx *ctx);
 // The launch timing probe around one call: probe_begin records the start event and returns the call's slot (-1 when
 // the probe is off, full or the stream is being captured); probe_end records the end event of that slot.
 int probe_begin(om_ctx *ctx);
