@@ -407,6 +407,14 @@ void by_width(int d, bool vec, F f) {
     else w(std::integral_constant<int, 4>());
 }
 
+void join(om_ctx *ctx, const Rule &u, const Ptrs &p, int nsplit, const float *part) {
+    const int64_t values = (int64_t)u.B * u.Hk * u.G * u.lq * u.d;
+    hipLaunchKernelGGL(k_scored_join, dim3((unsigned)((values + 255) / 256)), dim3(256), 0, ctx->stream, u, p, nsplit, part);
+}
+
+// The matrix kernels take 32 rows at a time.
+bool by_matrix(const Rule &u) { return u.d <= 128 && (int64_t)u.G * u.lq >= 32 && u.lk >= 1; }
+
 om_status fwd_by_rows(om_ctx *ctx, const Rule &u, const Ptrs &p) {
     const bool vec = u.d % 4 == 0 && p.ldq % 4 == 0 && p.ldkv % 4 == 0 && al16(p.q) && al16(p.k) && al16(p.v);
     const int rows = u.G * u.lq;
@@ -435,9 +443,7 @@ om_status fwd_by_rows(om_ctx *ctx, const Rule &u, const Ptrs &p) {
             }
             hipLaunchKernelGGL((k_scored_fwd_rows<NC, R, V>), dim3((unsigned)(wgs * ns)), dim3(256), 0, ctx->stream, u, p,
                                (int)blocks, (int)ns, per, part);
-            if (ns > 1)
-                hipLaunchKernelGGL(k_scored_join, dim3((unsigned)((all * u.d + 255) / 256)), dim3(256), 0, ctx->stream, u, p,
-                                   (int)ns, part);
+            if (ns > 1) join(ctx, u, p, (int)ns, part);
         };
         if (NC >= 4 || rows == 1) launch(std::integral_constant<int, 1>());
         else if (NC == 2 || rows <= 3) launch(std::integral_constant<int, 3>());
@@ -489,7 +495,13 @@ om_status om_attention_fwd_scored(om_ctx *ctx, const float *q, int ld_q, const f
     if (B == 0 || lq == 0) return OM_OK;
     OM_REQUIRE(ctx, q && o && ((k && v) || lk == 0), "%s: NULL q/k/v/o", what);
     if (om_status s = om::use_device(ctx)) return s;
-    return fwd_by_rows(ctx, u, p);
+    if (!by_matrix(u)) return fwd_by_rows(ctx, u, p);
+    int joins;
+    float *part;
+    if (om_status s = fwd_by_matrix(ctx, u, p, &joins, &part)) return s;
+    if (joins == 1) return OM_OK;
+    join(ctx, u, p, joins, part);
+    return OM_LAUNCH_CHECK(ctx, what);
 }
 
 om_status om_attention_bwd_scored(om_ctx *ctx, const float *q, int ld_q, const float *k, const float *v, int ld_kv,

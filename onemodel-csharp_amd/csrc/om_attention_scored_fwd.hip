@@ -1,0 +1,499 @@
+// Scored attention's forward on the matrix cores (operands: om_attention_scored_mm.hpp).
+//
+// A workgroup takes 128 rows of one key head's group (a wavefront 32: its lanes' queries) and walks the visible keys in
+// steps of KT. S^T = K Q^T leaves a query's scores in its lane's registers; they become weights E = 2^(x - m) there, are
+// split, and are the operand of O^T += V^T E^T as they stand. K and V come split from scratch, straight into LDS, two
+// stages, one barrier a step. The running maximum m moves only when some lane's maximum grows by more than 2^2: E then
+// stays below 2^14 with its 2^12 of headroom, and the accumulators are left alone in most steps.
+#include "om_attention_scored_split.hpp"
+
+namespace {
+
+using namespace osc;
+
+constexpr float kInf = __builtin_inff();
+constexpr int kRows = 128;      // rows of a workgroup
+constexpr float kLift = 12.0f;  // weights are kept as 2^kLift times themselves, so that their split's m is normal fp16
+constexpr float kSlack = 2.0f;  // how far a maximum may outgrow m before m moves
+constexpr int kListed = 1024;   // blocks of keys whose step data stands in LDS
+
+template <int DP, bool VEC>
+__global__ void __launch_bounds__(256) k_scored_split_kv(Rule u, Ptrs p, SplitOut ko, SplitOut vo, int nt) {
+    OM_LDS_POISON();
+    __shared__ __attribute__((aligned(16))) char lds[DP * 256];
+    __shared__ uint32_t sh[32];
+    const int items = u.B * u.Hk * nt;
+    const int which = blockIdx.x / items, at = blockIdx.x - which * items;
+    const int t = at % nt, bh = at / nt;
+    split_keys<DP, VEC>(u, which ? p.v : p.k, p.ldkv, bh / u.Hk, bh % u.Hk, t, at, which ? vo : ko, lds, sh);
+}
+
+// One row by plain fp32 sums over the keys lo .. hi, by one wavefront: 16 lanes to a key, four keys at a time. For rows
+// whose operands the split cannot hold.
+template <int DP>
+__device__ __forceinline__ void plain_row(const Rule &u, const Ptrs &p, int b, int hk, int rr, int lo, int hi, int split, int nsplit,
+                                       float *part) {
+    constexpr int NC = (DP + 63) / 64;
+    const int lane = threadIdx.x & 63, l16 = lane & 15, st = lane >> 4, d = u.d;
+    const int pre = u.prefix ? u.prefix[b] : 0;
+    const Row row = row_of(u, hk, rr);
+    const int64_t tok = (int64_t)b * u.lq + row.t;
+    const int doc = u.qd ? u.qd[tok] : 0, pos = row.t + u.off;
+    const float slope = u.slopes ? u.slopes[row.h] * kLog2e : 0.0f;
+    floatx4 q[NC], acc[NC];
+    float m = -kInf, l = 0.0f;
+#pragma unroll
+    for (int n = 0; n < NC; n++) {
+        q[n] = load4<false>(p.q + tok * p.ldq + (int64_t)row.h * d, 64 * n + 4 * l16, d);
+        acc[n] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+    const int64_t base = (int64_t)b * u.lk;
+    for (int j = lo + st; j <= hi; j += 4) {
+        const int gap = pos - j;
+        if (doc < 0 || (u.kd && u.kd[base + j] != doc) || !in_reach(u, gap, j, pre)) continue;
+        const float *kr = p.k + (base + j) * p.ldkv + (int64_t)hk * d, *vr = p.v + (base + j) * p.ldkv + (int64_t)hk * d;
+        float s = 0.0f, th;
+#pragma unroll
+        for (int n = 0; n < NC; n++) {
+            const floatx4 k = load4<false>(kr, 64 * n + 4 * l16, d);
+#pragma unroll
+            for (int e = 0; e < 4; e++) s = __builtin_fmaf(q[n][e], k[e], s);
+        }
+        float x = score(u, row_sum(s), th);
+        if (u.slopes) x = __builtin_fmaf(-slope, (float)(gap < 0 ? -gap : gap), x);
+        const float top = x > m ? x : m, mu = top == -kInf ? 0.0f : top, alpha = exp2_hw(m - mu), e1 = exp2_hw(x - mu);
+        m = top;
+        l = l * alpha + e1;
+#pragma unroll
+        for (int n = 0; n < NC; n++) {
+            const floatx4 v = load4<false>(vr, 64 * n + 4 * l16, d);
+#pragma unroll
+            for (int e = 0; e < 4; e++) acc[n][e] = __builtin_fmaf(e1, v[e], acc[n][e] * alpha);
+        }
+    }
+    // join the four streams
+    float top = m;
+    for (int o = 16; o < 64; o += 16) {
+        const float x = __shfl(m, (lane + o) & 63, 64);
+        top = x > top ? x : top;
+    }
+    const float mu = top == -kInf ? 0.0f : top, w = exp2_hw(m - mu);
+    auto joined = [&](float v) {
+        float s = 0.0f;
+        for (int o = 0; o < 4; o++) s += __shfl(v * w, l16 + 16 * o, 64);
+        return s;
+    };
+    const float sum = joined(l);
+    const int64_t rows = (int64_t)u.G * u.lq, all = (int64_t)u.B * u.Hk * rows, at = ((int64_t)b * u.Hk + hk) * rows + rr;
+    const float rl = sum == 0.0f ? 0.0f : 1.0f / sum;
+#pragma unroll
+    for (int n = 0; n < NC; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float a = joined(acc[n][e]);
+            const int c = 64 * n + 4 * l16 + e;
+            if (st == 0 && c < d) {
+                if (part) part[((int64_t)split * all + at) * d + c] = a;
+                else p.out[tok * p.ldo + (int64_t)row.h * d + c] = sum == 0.0f ? 0.0f : a * rl;
+            }
+        }
+    if (lane == 0) {
+        if (part) {
+            float *ms = part + (int64_t)nsplit * all * d + (int64_t)split * all + at;
+            ms[0] = mu;
+            ms[(int64_t)nsplit * all] = sum;
+        } else if (p.stats) {
+            const int64_t sr = stat_at(u, b, row);
+            p.stats[sr] = mu;
+            p.stats[all + sr] = rl;
+        }
+    }
+}
+
+struct FwdArgs {
+    const char *kn, *vt;      // K in rows form, V in columns form
+    const Stats *ks, *vs;     // their blocks' statistics
+    int nt;                   // blocks of 64 keys of a head
+    int blocks;               // workgroups along a head's rows
+    int nsplit, per;          // splits of the keys, blocks of 64 keys in each
+    float *part;              // the splits' sums (om_attention_scored.hip joins them), NULL for one split
+    int vec;                  // q's rows are 16-byte aligned
+};
+
+template <int DP, int KT>
+__global__ void __launch_bounds__(256, 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArgs a) {
+    OM_LDS_POISON();
+    constexpr int S = DP / 16, NB = KT / 32, ND = DP / 32;
+    constexpr int HALF = KT * DP * 4, STAGE = 2 * HALF;  // K's planes, then V's
+    __shared__ __attribute__((aligned(16))) char sh[256 + 2 * STAGE];  // no stage at LDS address 0
+    __shared__ float kscale[kListed];
+    __shared__ signed char vstep[kListed];  // exponent of V's scale less the largest, in steps of 4
+    __shared__ unsigned char visit[kListed];  // bit 0: some row may see the block, bit 1: documents need a look
+    __shared__ uint32_t red[4][5];
+    int rb, item;
+    on_one_xcd(a.blocks * a.nsplit, rb, item);
+    const int split = rb % a.nsplit;
+    rb = a.blocks - 1 - rb / a.nsplit;  // the longest rows of a causal rule first
+    const int b = item / u.Hk, hk = item - b * u.Hk, rows = u.G * u.lq;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
+    const int pre = u.prefix ? u.prefix[b] : 0;
+    const int first = rb * kRows, last = min(first + kRows, rows) - 1;
+    const int rr = first + 32 * w + (lane & 31);
+    const Row row = row_of(u, hk, min(rr, rows - 1));
+    const int64_t tok = (int64_t)b * u.lq + row.t;
+    const int pos = row.t + u.off, doc = u.qd ? u.qd[tok] : 0;
+    const float slope = u.slopes ? u.slopes[row.h] * kLog2e : 0.0f;
+
+    // The row's query, scaled and split: d = 16 s + 8 g + e.
+    u32x4 qh[S], qm[S];
+    int eq;
+    bool bad;
+    {
+        const float *qr = p.q + tok * p.ldq + (int64_t)row.h * u.d;
+        float x[S][8];
+        uint32_t top = 0;
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+            if (a.vec) {
+                const floatx4 lo = load4<true>(qr, 16 * s + 8 * g, u.d), hi = load4<true>(qr, 16 * s + 8 * g + 4, u.d);
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[s][e] = lo[e], x[s][4 + e] = hi[e];
+            } else {
+                const floatx4 lo = load4<false>(qr, 16 * s + 8 * g, u.d), hi = load4<false>(qr, 16 * s + 8 * g + 4, u.d);
+#pragma unroll
+                for (int e = 0; e < 4; e++) x[s][e] = lo[e], x[s][4 + e] = hi[e];
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                if (doc < 0) x[s][e] = 0.0f;
+                top = max(top, __float_as_uint(x[s][e]) & 0x7FFFFFFFu);
+            }
+        }
+        const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
+        top = max(both[0], both[1]);
+        bad = !in_range(top);
+        eq = bad || !top ? 0 : scale_exp(top);
+        const float sc = u.scale < 0.0f ? -pow2(-eq) : pow2(-eq);
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[s][e] *= sc;
+            split8(x[s], qh[s], qm[s]);
+        }
+    }
+
+    // The blocks of keys this workgroup can see, and what their split found.
+    int lo, hi;
+    const int i0 = first / u.G + u.off, i1 = last / u.G + u.off;
+    key_range(u, i0, i1, pre, lo, hi);
+    lo = max(lo, split * a.per * kBlock);
+    hi = (int)min((int64_t)hi, (int64_t)(split + 1) * a.per * kBlock - 1);
+    const int t0 = lo / kBlock, t1 = hi < lo ? t0 - 1 : hi / kBlock;
+    uint32_t ktop = 0, vtop = 0, vlow = 0xFFFFFFFFu;
+    int qlo = doc < 0 ? INT32_MAX : doc, qhi = doc;
+    const int64_t kt0 = (int64_t)item * a.nt;
+    for (int t = t0 + (int)threadIdx.x; t <= t1; t += 256) {
+        ktop = max(ktop, a.ks[kt0 + t].top);
+        vtop = max(vtop, a.vs[kt0 + t].top);
+        vlow = min(vlow, a.vs[kt0 + t].low);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        ktop = max(ktop, (uint32_t)__shfl_xor((int)ktop, o, 64));
+        vtop = max(vtop, (uint32_t)__shfl_xor((int)vtop, o, 64));
+        vlow = min(vlow, (uint32_t)__shfl_xor((int)vlow, o, 64));
+        qlo = min(qlo, __shfl_xor(qlo, o, 64));
+        qhi = max(qhi, __shfl_xor(qhi, o, 64));
+    }
+    if (lane == 0) {
+        red[w][0] = ktop;
+        red[w][1] = vtop;
+        red[w][2] = vlow;
+        red[w][3] = (uint32_t)qlo;
+        red[w][4] = (uint32_t)qhi;
+    }
+    bad = __syncthreads_or(bad);
+    const bool some_padded = __syncthreads_or(doc < 0);  // such a row sees nothing, whatever the others see
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        ktop = max(ktop, red[i][0]);
+        vtop = max(vtop, red[i][1]);
+        vlow = min(vlow, red[i][2]);
+        qlo = min(qlo, (int)red[i][3]);
+        qhi = max(qhi, (int)red[i][4]);
+    }
+    bad = bad || ktop > kMostBits || vtop > kMostBits || (vtop && (vtop >> 23) - (vlow >> 23) > 16);
+    if (__builtin_amdgcn_readfirstlane(bad)) {
+        for (int r = first + 32 * w; r <= min(last, first + 32 * w + 31); r++)
+            plain_row<DP>(u, p, b, hk, r, lo, hi, split, a.nsplit, a.part);
+        return;
+    }
+    const int ev = vtop ? scale_exp(vtop) : 0;
+    auto looked = [&](int t, float &sc, int &step) -> int {
+        const Stats ks = a.ks[kt0 + t];
+        sc = ks.scale;
+        step = ((int)(__float_as_uint(a.vs[kt0 + t].scale) >> 23) - 127 - ev) / 4;
+        if (a.vs[kt0 + t].top == 0) step = 0;  // a block of zeros
+        const int j0 = t * kBlock, j1 = j0 + kBlock - 1;
+        int see = 1;
+        if (j0 >= pre) see = !(u.causal && j0 > i1) && !(u.window && (i0 - j1 >= u.window || j0 - i1 >= u.window));
+        if (u.qd) {
+            if (ks.doc_hi < qlo || ks.doc_lo > qhi) see = 0;
+            if (some_padded || ks.doc_lo < 0 || ks.doc_lo != ks.doc_hi || qlo != qhi || ks.doc_lo != qlo) see |= 2;
+        }
+        return see;
+    };
+    for (int t = t0 + (int)threadIdx.x; t <= t1 && t < t0 + kListed; t += 256) {
+        float sc;
+        int step;
+        const int see = looked(t, sc, step);
+        kscale[t - t0] = sc;
+        vstep[t - t0] = (signed char)step;
+        visit[t - t0] = (unsigned char)see;
+    }
+    __syncthreads();
+
+    const int steps = (t1 - t0 + 1) * (kBlock / KT);
+    auto next = [&](int it) {  // the next step with a key that some row may see
+        for (it++; it < steps; it++) {
+            const int t = it * KT / kBlock;
+            if (t0 * kBlock + it * KT > hi) return steps;
+            if (t >= kListed || (visit[t] & 1)) return it;
+        }
+        return steps;
+    };
+    const char *kn = a.kn + (kt0 + t0) * plane_bytes(DP, 1), *vt = a.vt + (kt0 + t0) * plane_bytes(DP, 1);
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)(sh + 256);
+    auto stage = [&](int it, int buf) {
+        constexpr int PER = HALF / 4096;  // KB of each operand per wavefront
+        const char *ka = kn + (int64_t)it * HALF + lane * 16, *va = vt + (int64_t)it * HALF + lane * 16;
+        const uint32_t to = lds0 + (uint32_t)(buf * STAGE);
+#pragma unroll
+        for (int i = 0; i < PER; i++) load_to_lds(ka + (4 * i + w) * 1024, to + (uint32_t)(4 * i + w) * 1024u);
+#pragma unroll
+        for (int i = 0; i < PER; i++) load_to_lds(va + (4 * i + w) * 1024, to + HALF + (uint32_t)(4 * i + w) * 1024u);
+    };
+
+    floatx16 acc[ND];
+#pragma unroll
+    for (int n = 0; n < ND; n++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) acc[n][e] = 0.0f;
+    float m = -kInf, l = 0.0f;
+    const int wi0 = min(first + 32 * w, last) / u.G + u.off, wi1 = min(first + 32 * w + 31, last) / u.G + u.off;
+    const bool live = first + 32 * w <= last;
+    const float cq = __builtin_fabsf(u.cl2) * pow2(eq), icq = __builtin_fabsf(u.icap) * pow2(eq);
+
+    int it = next(-1), buf = 0;
+    if (it < steps) stage(it, 0);
+    while (it < steps) {
+        wait_loads();
+        __syncthreads();  // this step has landed, and every wavefront is done with the other stage
+        const int nx = next(it);
+        if (nx < steps) stage(nx, buf ^ 1);
+        const int j0 = t0 * kBlock + it * KT, j1 = j0 + KT - 1, ti = it * KT / kBlock;
+        float ksc;
+        int vst, see;
+        if (ti < kListed) {
+            ksc = kscale[ti];
+            vst = vstep[ti];
+            see = visit[ti];
+        } else {
+            see = looked(t0 + ti, ksc, vst);
+        }
+        // what the wavefront's 32 rows see of the step
+        const bool none = !live || (j0 >= pre && ((u.causal && j0 > wi1) ||
+                                                  (u.window && (wi0 - j1 >= u.window || j0 - wi1 >= u.window))));
+        const bool whole = j1 < u.lk && !(see & 2) &&
+                           (j1 < pre || ((!u.causal || j1 <= wi0) && (!u.window || (wi1 - j0 < u.window && j1 - wi0 < u.window))));
+        if (!none) {
+            const char *kf = sh + 256 + buf * STAGE + lane * 16, *vf = kf + HALF;
+            floatx16 x[NB];
+#pragma unroll
+            for (int n = 0; n < NB; n++) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) x[n][e] = 0.0f;
+#pragma unroll
+                for (int s = 0; s < S; s++) {
+                    const u32x4 kh = *reinterpret_cast<const u32x4 *>(kf + ((n * S + s) * 2) * 1024);
+                    const u32x4 km = *reinterpret_cast<const u32x4 *>(kf + ((n * S + s) * 2 + 1) * 1024);
+                    x[n] = mma3(kh, km, qh[s], qm[s], x[n]);
+                }
+            }
+            // x * f is the score in log2 units
+            float f = cq * ksc;
+            if (u.icap != 0.0f) {
+                const float ic = icq * ksc;
+                float big = 0.0f;
+#pragma unroll
+                for (int n = 0; n < NB; n++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) big = fmaxf(big, __builtin_fabsf(x[n][e]));
+                if (__any(big * ic >= kTanhSmall)) {
+#pragma unroll
+                    for (int n = 0; n < NB; n++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) x[n][e] = tanh_any(x[n][e] * ic);
+                } else {
+#pragma unroll
+                    for (int n = 0; n < NB; n++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) x[n][e] = tanh_small(x[n][e] * ic);
+                }
+                f = u.capl2;
+            }
+            if (u.slopes) {
+                const float gap0 = (float)(pos - j0 - 4 * g);
+#pragma unroll
+                for (int n = 0; n < NB; n++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const float gap = gap0 - (float)(32 * n + 8 * (e >> 2) + (e & 3));
+                        x[n][e] = __builtin_fmaf(-slope, __builtin_fabsf(gap), x[n][e] * f);
+                    }
+                f = 1.0f;
+            }
+            if (!whole) {
+                const int j = j0 + 4 * g;
+#pragma unroll
+                for (int n = 0; n < NB; n++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        const int jj = j + 32 * n + 8 * (e >> 2) + (e & 3);
+                        bool ok = jj < u.lk && in_reach(u, pos - jj, jj, pre);
+                        if (see & 2) ok = ok && doc >= 0 && u.kd[(int64_t)b * u.lk + min(jj, u.lk - 1)] == doc;
+                        x[n][e] = ok ? x[n][e] : -kInf;
+                    }
+            }
+            float top = -kInf;
+#pragma unroll
+            for (int n = 0; n < NB; n++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) top = fmaxf(top, x[n][e]);
+            top = pair_max(top) * f;
+            if (__any(top > m + kSlack)) {
+                const float mn = fmaxf(m, top), al = mn == -kInf ? 1.0f : exp2_hw(m - mn);
+                m = mn;
+                l *= al;
+#pragma unroll
+                for (int n = 0; n < ND; n++) acc[n] *= al;
+            }
+            const float lift = kLift + 4.0f * (float)vst, mu = (m == -kInf ? 0.0f : -m) + lift;
+            float sum = 0.0f;
+#pragma unroll
+            for (int n = 0; n < NB; n++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    x[n][e] = exp2_hw(__builtin_fmaf(x[n][e], f, mu));
+                    sum += x[n][e];
+                }
+            l = __builtin_fmaf(sum, pow2(-4 * vst), l);
+#pragma unroll
+            for (int n = 0; n < NB; n++)
+#pragma unroll
+                for (int s = 0; s < 2; s++) {
+                    float e8[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) e8[e] = x[n][8 * s + e];
+                    u32x4 ph, pm;
+                    split8(e8, ph, pm);
+#pragma unroll
+                    for (int c = 0; c < ND; c++) {
+                        const char *at = vf + (((2 * n + s) * ND + c) * 2) * 1024;
+                        acc[c] = mma3(*reinterpret_cast<const u32x4 *>(at), *reinterpret_cast<const u32x4 *>(at + 1024), ph, pm,
+                                      acc[c]);
+                    }
+                }
+        }
+        it = nx;
+        buf ^= 1;
+    }
+
+    l = pair_sum(l);
+    if (rr > last) return;
+    const int64_t all = (int64_t)u.B * u.Hk * rows, at = (int64_t)item * rows + rr;
+    const float mu = m == -kInf ? 0.0f : m, rl = l == 0.0f ? 0.0f : 1.0f / l, unlift = pow2(-(int)kLift);
+    const float wgt = a.part ? pow2(ev) * unlift : pow2(ev) * rl;
+    float *to = a.part ? a.part + ((int64_t)split * all + at) * u.d : p.out + tok * p.ldo + (int64_t)row.h * u.d;
+#pragma unroll
+    for (int n = 0; n < ND; n++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const int c = 32 * n + 8 * q + 4 * g;
+            floatx4 v = floatx4{acc[n][4 * q], acc[n][4 * q + 1], acc[n][4 * q + 2], acc[n][4 * q + 3]} * wgt;
+            if (l == 0.0f) v = floatx4{0.f, 0.f, 0.f, 0.f};
+            if (c + 3 < u.d && (((uintptr_t)(to + c)) & 15) == 0) {
+                *reinterpret_cast<floatx4 *>(to + c) = v;
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (c + e < u.d) to[c + e] = v[e];
+            }
+        }
+    if (g == 0) {
+        if (a.part) {
+            float *ms = a.part + (int64_t)a.nsplit * all * u.d + (int64_t)split * all + at;
+            ms[0] = mu;
+            ms[(int64_t)a.nsplit * all] = l * unlift;
+        } else if (p.stats) {
+            const int64_t sr = stat_at(u, b, row);
+            p.stats[sr] = mu;
+            p.stats[all + sr] = l == 0.0f ? 0.0f : rl * pow2((int)kLift);
+        }
+    }
+}
+
+}  // namespace
+
+namespace osc {
+
+// The forward by the matrix cores, d up to 128; *joins gets the number of splits left to join (1: none) and *part where
+// they lie.
+om_status fwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p, int *joins, float **part) {
+    const int nt = (u.lk + kBlock - 1) / kBlock, rows = u.G * u.lq, blocks = (rows + kRows - 1) / kRows;
+    const int64_t items = (int64_t)u.B * u.Hk, wgs = items * blocks, all = items * rows;
+    const int dp = u.d <= 32 ? 32 : u.d <= 64 ? 64 : u.d <= 96 ? 96 : 128;
+    // Split the keys while the chip has fewer than two workgroups per CU, in pieces of at least four blocks.
+    int64_t ns = wgs >= 2 * ctx->num_cus ? 1 : 2 * ctx->num_cus / wgs;
+    ns = ns > nt / 4 ? nt / 4 : ns;
+    ns = ns < 1 ? 1 : ns;
+    const int per = (int)((nt + ns - 1) / ns);
+    ns = (nt + per - 1) / per;
+    OM_REQUIRE(ctx, wgs * ns <= INT32_MAX && 2 * items * nt <= INT32_MAX, "om_attention_fwd_scored: too many row blocks");
+    const int64_t plane = plane_bytes(dp, items * nt), stats = items * nt * (int64_t)sizeof(Stats);
+    const int64_t join = ns > 1 ? (int64_t)sizeof(float) * ns * all * (u.d + 2) : 0;
+    float *scr;
+    if (om_status s = om::scratch2(ctx, (uint64_t)(2 * plane + 2 * stats + join), &scr)) return s;
+    char *base = reinterpret_cast<char *>(scr);
+    FwdArgs a = {};
+    a.kn = base;
+    a.vt = base + plane;
+    a.ks = reinterpret_cast<Stats *>(base + 2 * plane);
+    a.vs = a.ks + items * nt;
+    a.nt = nt;
+    a.blocks = blocks;
+    a.nsplit = (int)ns;
+    a.per = per;
+    a.part = ns > 1 ? reinterpret_cast<float *>(base + 2 * plane + 2 * stats) : nullptr;
+    auto al16 = [](const void *x) { return ((uintptr_t)x & 15) == 0; };
+    a.vec = u.d % 4 == 0 && p.ldq % 4 == 0 && al16(p.q);
+    const bool vec = u.d % 4 == 0 && p.ldkv % 4 == 0 && al16(p.k) && al16(p.v);
+    const SplitOut ko = {base, nullptr, const_cast<Stats *>(a.ks)}, vo = {nullptr, base + plane, const_cast<Stats *>(a.vs)};
+    auto go = [&](auto dpc, auto ktc) {
+        constexpr int DP = decltype(dpc)::value, KT = decltype(ktc)::value;
+        auto split = [&](auto kern) {
+            hipLaunchKernelGGL(kern, dim3((unsigned)(2 * items * nt)), dim3(256), 0, ctx->stream, u, p, ko, vo, nt);
+        };
+        vec ? split(k_scored_split_kv<DP, true>) : split(k_scored_split_kv<DP, false>);
+        hipLaunchKernelGGL((k_scored_fwd_mm<DP, KT>), dim3((unsigned)(wgs * ns)), dim3(256), 0, ctx->stream, u, p, a);
+    };
+    if (dp == 32) go(std::integral_constant<int, 32>(), std::integral_constant<int, 64>());
+    else if (dp == 64) go(std::integral_constant<int, 64>(), std::integral_constant<int, 64>());
+    else if (dp == 96) go(std::integral_constant<int, 96>(), std::integral_constant<int, 32>());
+    else go(std::integral_constant<int, 128>(), std::integral_constant<int, 32>());
+    *joins = (int)ns;
+    *part = a.part;
+    return OM_LAUNCH_CHECK(ctx, "om_attention_fwd_scored");
+}
+
+}  // namespace osc

@@ -1,0 +1,118 @@
+// Scored attention on the matrix cores: the operand form that the forward and backward kernels share.
+//
+// fp32 products as three fp16 products. A block of 64 rows of an operand is scaled by a power of two that brings its
+// largest value to 2^10 .. 2^14 and split into x = h + m + r, h and m fp16 (11 + 11 significand bits, |r| below 2^-22 |x|,
+// or 2^-35 of the block's largest value where m is subnormal); a product keeps hh, hm, mh. The dropped terms are together
+// about 2^-23 of |x||y|, so a sum of products keeps fp32's accuracy, at a third of the fp16 matrix rate (840 TFLOP/s
+// where v_mfma_f32_16x16x4_f32 has 157 and the six-term bf16 split of om_split.hpp 419), and a split takes two vector
+// operations a value where the bf16 one takes six. What fp16's range does not hold is found beforehand (Stats): a block
+// with an infinity, a NaN or a magnitude outside 2^-40 .. 2^40, or rows whose largest values are more than 2^16 apart.
+// A workgroup that would use such a block computes its rows by plain fp32 sums instead (om_attention_scored.hip).
+//
+// Operands lie in scratch in fragment order: v_mfma_f32_32x32x16_f16 takes, from lane l, eight values of row l % 32 at
+// contraction indices of group g = l / 32, and a fragment of 64 lanes x 16 bytes is 1 KB of consecutive memory, so
+// staging is a straight copy into LDS and a fragment read is one conflict-free ds_read_b128.
+//   rows form (sums over d):    [block of 64 rows][32 rows][16 d][plane][lane][8], d = 16 s + 8 g + e;
+//   columns form (sums over rows): [block of 64 rows][16 rows][32 d][plane][lane][8], lane % 32 the d, and element e of group
+//     g row 16 s + 8 (e / 4) + 4 g + e % 4: the order in which a 32 x 32 result's registers hold its rows, so that a
+//     block of weights goes from one product's result straight into the next one's operand.
+#pragma once
+
+#include "om_attention_scored.hpp"
+
+namespace osc {
+
+typedef _Float16 half2 __attribute__((ext_vector_type(2)));
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kBlock = 64;  // rows of an operand that share a scale
+
+// What the split found in a block: the largest magnitude (bits; at or above infinity's if the split cannot hold the block),
+// the smallest nonzero row maximum (bits), 2^e of its scale, and the range of its document ids.
+struct Stats {
+    uint32_t top, low;
+    float scale;
+    int32_t doc_lo, doc_hi;
+    int32_t pad[3];
+};
+constexpr uint32_t kInfBits = 0x7F800000u;
+constexpr uint32_t kMostBits = (127u + 40) << 23, kLeastBits = (127u - 40) << 23;  // 2^40, 2^-40
+
+__device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
+// The exponent e of a scale 2^-e that brings `top` (bits of a magnitude in range) to 2^10 .. 2^14; steps of 2^4, so that
+// neighbouring blocks mostly share it.
+__device__ __forceinline__ int scale_exp(uint32_t top) {
+    const int e = (int)(top >> 23) - 127 - 13;
+    return (e + 3) & ~3;
+}
+__device__ __forceinline__ bool in_range(uint32_t top) { return top == 0 || (top >= kLeastBits && top <= kMostBits); }
+
+// Two values split into packed fp16 pairs.
+__device__ __forceinline__ void split2(float a, float b, uint32_t &h, uint32_t &m) {
+    const half2 hh = {(_Float16)a, (_Float16)b};
+    h = __builtin_bit_cast(uint32_t, hh);
+    const half2 mm = {(_Float16)__builtin_fmaf((float)hh[0], -1.0f, a), (_Float16)__builtin_fmaf((float)hh[1], -1.0f, b)};
+    m = __builtin_bit_cast(uint32_t, mm);
+}
+// Eight values as one lane's part of a fragment.
+__device__ __forceinline__ void split8(const float *x, u32x4 &h, u32x4 &m) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        uint32_t a, b;
+        split2(x[2 * i], x[2 * i + 1], a, b);
+        h[i] = a;
+        m[i] = b;
+    }
+}
+__device__ __forceinline__ floatx16 mma(u32x4 a, u32x4 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(half8, a), __builtin_bit_cast(half8, b), c, 0, 0, 0);
+}
+// One step of 16 terms: a's rows are the result's registers (8 q + 4 g + r in register 4 q + r), b's its lanes.
+__device__ __forceinline__ floatx16 mma3(u32x4 ah, u32x4 am, u32x4 bh, u32x4 bm, floatx16 c) {
+    c = mma(am, bh, c);
+    c = mma(ah, bm, c);
+    return mma(ah, bh, c);
+}
+
+// The other half-wavefront's value beside this one's: (lanes 0-31's, lanes 32-63's) of the lane's pair.
+__device__ __forceinline__ void both_halves(float v, float &lo, float &hi) {
+    const auto p = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    lo = __uint_as_float(p[0]);
+    hi = __uint_as_float(p[1]);
+}
+__device__ __forceinline__ float pair_max(float v) {
+    float a, b;
+    both_halves(v, a, b);
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float pair_sum(float v) {
+    float a, b;
+    both_halves(v, a, b);
+    return a + b;
+}
+
+// 16 bytes per lane from `src` (this lane's address) to LDS at byte address lds + 16 * lane, without registers. m0 holds
+// the address for this one instruction only; nothing else in these kernels reads it. The caller waits (wait_loads) before
+// the barrier after which the data is read.
+__device__ __forceinline__ void load_to_lds(const void *src, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// Bytes of one operand's two planes for `blocks` blocks of 64 rows.
+inline __host__ __device__ int64_t plane_bytes(int dp, int64_t blocks) { return blocks * kBlock * dp * 4; }
+
+// Workgroup id -> (block, item) with the blocks of one item on one XCD (ids are dealt round-robin over the 8 XCDs, each
+// with its own L2).
+__device__ __forceinline__ void on_one_xcd(int nb, int &blk, int &item) {
+    int lin = blockIdx.x;
+    const int total = gridDim.x;
+    if ((total & 7) == 0) lin = (lin & 7) * (total >> 3) + (lin >> 3);
+    blk = lin % nb;
+    item = lin / nb;
+}
+
+}  // namespace osc

@@ -1,0 +1,154 @@
+// The pass that splits operands for the scored attention's matrix kernels (om_attention_scored_mm.hpp): one workgroup per
+// block of 64 rows of a head, four rows x four values a thread. Bound: HBM, 4 bytes read and 4 or 8 written per value.
+#pragma once
+
+#include "om_attention_scored_mm.hpp"
+
+namespace osc {
+
+struct SplitOut {
+    char *rows, *cols;  // either may be NULL
+    Stats *stats;
+};
+
+// This thread's share of a block: values 64 n + 4 (tid % 16) .. + 3 of rows 4 (tid / 16) + i.
+template <int DP>
+struct Share {
+    static constexpr int NCH = (DP + 63) / 64;
+    floatx4 x[4][NCH];
+    template <bool VEC>
+    __device__ __forceinline__ void load(int i, const float *row, bool there, int d) {
+#pragma unroll
+        for (int n = 0; n < NCH; n++) {
+            const int c = 64 * n + 4 * (threadIdx.x & 15);
+            x[i][n] = there && c < DP ? load4<VEC>(row, c, d) : floatx4{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+    // Largest magnitude of row i as bits (infinities and NaN above every finite one), the same in the row's 16 lanes.
+    __device__ __forceinline__ uint32_t row_top(int i) const {
+        uint32_t t = 0;
+#pragma unroll
+        for (int n = 0; n < NCH; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) t = max(t, __float_as_uint(x[i][n][e]) & 0x7FFFFFFFu);
+        auto step = [&](auto ctrl) {
+            t = max(t, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)t, decltype(ctrl)::value, 0xf, 0xf, true));
+        };
+        step(std::integral_constant<int, 0x128>());
+        step(std::integral_constant<int, 0x124>());
+        step(std::integral_constant<int, 0x122>());
+        step(std::integral_constant<int, 0x121>());
+        return t;
+    }
+    __device__ __forceinline__ void scale(int i, float w) {
+#pragma unroll
+        for (int n = 0; n < NCH; n++) x[i][n] *= w;
+    }
+};
+
+// The block's top and low from its rows' maxima; every thread gets both. Uses 32 words of LDS.
+__device__ __forceinline__ void block_top(const uint32_t (&row)[4], uint32_t &top, uint32_t &low, uint32_t *sh) {
+    uint32_t t = 0, l = 0xFFFFFFFFu;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        t = max(t, row[i]);
+        l = row[i] ? min(l, row[i]) : l;
+    }
+    __syncthreads();
+    if ((threadIdx.x & 15) == 0) {
+        sh[threadIdx.x >> 4] = t;
+        sh[16 + (threadIdx.x >> 4)] = l;
+    }
+    __syncthreads();
+    top = sh[0];
+    low = sh[16];
+#pragma unroll
+    for (int i = 1; i < 16; i++) {
+        top = max(top, sh[i]);
+        low = min(low, sh[16 + i]);
+    }
+}
+
+// Writes the block's two planes in rows or columns form: through LDS (DP * 256 bytes), so that memory gets whole lines.
+template <int DP, bool COLS>
+__device__ __forceinline__ void put_block(const Share<DP> &s, char *out, char *lds) {
+    constexpr int NCH = Share<DP>::NCH;
+    const int rq = threadIdx.x >> 4;
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < NCH; n++) {
+        const int c = 64 * n + 4 * (threadIdx.x & 15);
+        if (c >= DP) continue;
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            uint32_t h0, m0, h1, m1;
+            char *to;
+            if constexpr (COLS) {  // four rows of value c + i
+                split2(s.x[0][n][i], s.x[1][n][i], h0, m0);
+                split2(s.x[2][n][i], s.x[3][n][i], h1, m1);
+                const int v = c + i;
+                to = lds + (((rq >> 2) * (DP / 32) + (v >> 5)) * 2) * 1024 + ((rq & 1) * 32 + (v & 31)) * 16 + ((rq >> 1) & 1) * 8;
+            } else {  // four values of row 4 rq + i
+                split2(s.x[i][n][0], s.x[i][n][1], h0, m0);
+                split2(s.x[i][n][2], s.x[i][n][3], h1, m1);
+                const int row = 4 * rq + i;
+                to = lds + (((row >> 5) * (DP / 16) + (c >> 4)) * 2) * 1024 + (((c >> 3) & 1) * 32 + (row & 31)) * 16 + ((c >> 2) & 1) * 8;
+            }
+            *reinterpret_cast<u32x2 *>(to) = u32x2{h0, h1};
+            *reinterpret_cast<u32x2 *>(to + 1024) = u32x2{m0, m1};
+        }
+    }
+    __syncthreads();
+    for (int f = threadIdx.x; f < DP * 16; f += 256)
+        *reinterpret_cast<u32x4 *>(out + 16 * f) = *reinterpret_cast<const u32x4 *>(lds + 16 * f);
+}
+
+// Block t of the keys of (b, hk): K or V (src) scaled by one power of two, in the forms asked for. Keys of padding
+// documents become zeros, so that nothing they hold reaches a product.
+template <int DP, bool VEC>
+__device__ __forceinline__ void split_keys(const Rule &u, const float *src, int64_t ld, int b, int hk, int t, int64_t at,
+                                           const SplitOut &o, char *lds, uint32_t *sh) {
+    Share<DP> s;
+    uint32_t top4[4], top, low;
+    int dlo = INT32_MAX, dhi = -1;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int j = t * kBlock + 4 * (threadIdx.x >> 4) + i;
+        const int64_t tok = (int64_t)b * u.lk + min(j, u.lk - 1);
+        const int doc = j >= u.lk ? -1 : u.kd ? u.kd[tok] : 0;
+        s.template load<VEC>(i, src + tok * ld + (int64_t)hk * u.d, doc >= 0, u.d);
+        top4[i] = s.row_top(i);
+        dhi = max(dhi, doc);
+        dlo = min(dlo, j >= u.lk ? INT32_MAX : doc);
+    }
+    block_top(top4, top, low, sh);
+    const bool ok = in_range(top);
+    const int e = ok && top ? scale_exp(top) : 0;
+    const float w = pow2(-e);
+#pragma unroll
+    for (int i = 0; i < 4; i++) s.scale(i, w);
+    if (o.rows) put_block<DP, false>(s, o.rows + at * plane_bytes(DP, 1), lds);
+    if (o.cols) put_block<DP, true>(s, o.cols + at * plane_bytes(DP, 1), lds);
+    // the block's document range
+    __syncthreads();
+    if ((threadIdx.x & 15) == 0) {
+        sh[threadIdx.x >> 4] = (uint32_t)dlo;
+        sh[16 + (threadIdx.x >> 4)] = (uint32_t)dhi;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 16; i++) {
+            dlo = min(dlo, (int)sh[i]);
+            dhi = max(dhi, (int)sh[16 + i]);
+        }
+        Stats st = {};
+        st.top = ok ? top : 0xFFFFFFFFu;
+        st.low = low;
+        st.scale = pow2(e);
+        st.doc_lo = dlo;
+        st.doc_hi = dhi;
+        o.stats[at] = st;
+    }
+}
+
+}  // namespace osc
