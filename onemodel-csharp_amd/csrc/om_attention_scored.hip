@@ -538,7 +538,7 @@ om_status om_attention_bwd_scored(om_ctx *ctx, const float *q, int ld_q, const f
     OM_REQUIRE(ctx, (q && o && g && stats) || lq == 0, "%s: NULL q/o/stats/g", what);
     OM_REQUIRE(ctx, (k && v) || lk == 0, "%s: NULL k/v", what);
     if (om_status s = om::use_device(ctx)) return s;
-    return bwd_by_rows(ctx, u, p);
+    return by_matrix(u) ? bwd_by_matrix(ctx, u, p) : bwd_by_rows(ctx, u, p);
 }
 
 }  // extern "C"

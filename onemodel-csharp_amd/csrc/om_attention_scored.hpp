@@ -133,5 +133,7 @@ __device__ __forceinline__ int64_t stat_at(const Rule &u, int b, const Row &r) {
 // The forward by the matrix cores (om_attention_scored_fwd.hip), d up to 128; *joins gets the number of key splits left to
 // join (1: none) and *part their sums.
 om_status fwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p, int *joins, float **part);
+// The backward by the matrix cores (om_attention_scored_bwd.hip), d up to 128.
+om_status bwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p);
 
 }  // namespace osc

@@ -1,0 +1,896 @@
+// Scored attention's backward on the matrix cores (operands: om_attention_scored_mm.hpp).
+//
+// With E = 2^(x - m) from the saved m, re the exponent of a row's gradient and w = 2^re / l:
+//   D = E (g 2^-re . v - delta 2^-re) (1 - tanh^2),
+//   dv_j = sum_i E_ij (g_i / l_i),  dk_j = scale sum_i D_ij (w_i q_i),  dq_i = scale w_i sum_j D_ij k_j:
+// each operand's rows carry the row's own factor, so that weights of 1 / length and gradients of any size keep their bits in
+// fp16 pairs.
+//
+// Two roles share a launch (their tails fill each other's): a workgroup of 128 keys holds K and V fragments and walks the rows
+// of the key head's whole group, scores with a key in each lane; one of 128 rows holds Q and G and walks the keys, with a
+// query in each lane. Either way a block of scores leaves the matrix unit in the order in which it is the next product's
+// operand. Recomputing the scores for the second role costs two products of seven; partial dq from the first role would
+// cost rows * keys / 32 values of traffic, more than that from about 2000 keys on, and atomics would lose the fixed order.
+#include "om_attention_scored_split.hpp"
+
+namespace {
+
+using namespace osc;
+
+constexpr int kKeys = 128;   // keys (or rows) of a workgroup
+constexpr int kStep = 32;    // rows (or keys) of a step
+constexpr int kListed = 512; // blocks whose step data stands in LDS
+constexpr int kLift = 12;    // E is kept as 2^12 E for dv's operand
+
+struct BwdArgs {
+    const char *kn, *kt, *vn;        // K in both forms, V in rows form
+    const char *qn, *gn, *g2, *q2;   // RowsOut
+    RowVals v;
+    const Stats *ks, *vs;
+    const RowStats *rs;
+    int nt, nr;                      // blocks of 64 keys and rows of a head
+    int kblocks, rblocks;            // workgroups along them
+    int nsplit, per;                 // splits of the rows for dk and dv, blocks of 64 rows in each
+    int first_rows;                  // workgroups of the first role
+    float *part;                     // [split][B Hk][lk][2][d] (dk, dv), NULL for one split
+};
+
+template <int DP, bool VEC>
+__global__ void __launch_bounds__(256) k_scored_split_bwd(Rule u, Ptrs p, SplitOut ko, SplitOut vo, RowsOut ro, int nt, int nr) {
+    OM_LDS_POISON();
+    __shared__ __attribute__((aligned(16))) char lds[DP * 256];
+    __shared__ uint32_t sh[32];
+    const int keys = u.B * u.Hk * nt;
+    int i = blockIdx.x;
+    if (i < 2 * keys) {
+        const int at = i % keys, bh = at / nt;
+        const bool v = i >= keys;
+        split_keys<DP, VEC>(u, v ? p.v : p.k, p.ldkv, bh / u.Hk, bh % u.Hk, at % nt, at, v ? vo : ko, lds, sh);
+    } else {
+        i -= 2 * keys;
+        const int bh = i / nr;
+        split_rows<DP, VEC>(u, p, bh / u.Hk, bh % u.Hk, i % nr, i, ro, lds, sh);
+    }
+}
+
+// What a row and a key make of each other by plain sums: p in *pr, d loss / d (q . k) / scale in *ds. 16 lanes hold the
+// vectors.
+template <int NC>
+struct Pair {
+    floatx4 q[NC], g[NC];
+    float m, rl, delta, slope;
+    int pos, doc;
+    int64_t tok;
+    int h;
+    __device__ __forceinline__ void row(const Rule &u, const Ptrs &p, int b, int hk, int rr, int l16) {
+        const Row r = row_of(u, hk, rr);
+        tok = (int64_t)b * u.lq + r.t;
+        h = r.h;
+        const int64_t sr = stat_at(u, b, r), all = (int64_t)u.B * u.Hk * u.G * u.lq;
+        float dot = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NC; n++) {
+            const int c = 64 * n + 4 * l16;
+            q[n] = load4<false>(p.q + tok * p.ldq + (int64_t)h * u.d, c, u.d);
+            g[n] = load4<false>(p.g + tok * p.ldg + (int64_t)h * u.d, c, u.d);
+            const floatx4 o = load4<false>(p.o + tok * p.ldo + (int64_t)h * u.d, c, u.d);
+#pragma unroll
+            for (int e = 0; e < 4; e++) dot = __builtin_fmaf(g[n][e], o[e], dot);
+        }
+        delta = row_sum(dot);
+        m = p.st[sr];
+        rl = p.st[all + sr];
+        pos = r.t + u.off;
+        doc = rl == 0.0f ? -1 : u.qd ? u.qd[tok] : 0;
+        slope = u.slopes ? u.slopes[h] * kLog2e : 0.0f;
+    }
+    __device__ __forceinline__ bool sees(const Rule &u, int j, int kd, int pre) const {
+        return doc >= 0 && doc == kd && in_reach(u, pos - j, j, pre);
+    }
+    __device__ __forceinline__ void grads(const Rule &u, const floatx4 (&k)[NC], const floatx4 (&v)[NC], int j, float &pr,
+                                          float &ds) const {
+        float s = 0.0f, dp = 0.0f, th;
+#pragma unroll
+        for (int n = 0; n < NC; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                s = __builtin_fmaf(q[n][e], k[n][e], s);
+                dp = __builtin_fmaf(g[n][e], v[n][e], dp);
+            }
+        float x = score(u, row_sum(s), th);
+        const int gap = pos - j;
+        if (u.slopes) x = __builtin_fmaf(-slope, (float)(gap < 0 ? -gap : gap), x);
+        pr = exp2_hw(x - m) * rl;
+        ds = pr * (row_sum(dp) - delta) * (1.0f - th * th);
+    }
+};
+// Sum of the four streams' values, the same in each.
+__device__ __forceinline__ float join4(float v) {
+    const int l16 = threadIdx.x & 15;
+    float s = 0.0f;
+    for (int o = 0; o < 4; o++) s += __shfl(v, l16 + 16 * o, 64);
+    return s;
+}
+
+// dq of one row by one wavefront.
+template <int DP>
+__device__ __forceinline__ void plain_dq(const Rule &u, const Ptrs &p, int b, int hk, int rr, int lo, int hi, int pre) {
+    constexpr int NC = (DP + 63) / 64;
+    const int lane = threadIdx.x & 63, l16 = lane & 15, st = lane >> 4;
+    Pair<NC> r;
+    r.row(u, p, b, hk, rr, l16);
+    floatx4 dq[NC], k[NC], v[NC];
+#pragma unroll
+    for (int n = 0; n < NC; n++) dq[n] = floatx4{0.f, 0.f, 0.f, 0.f};
+    const int64_t base = (int64_t)b * u.lk;
+    for (int j = lo + st; j <= hi; j += 4) {
+        if (!r.sees(u, j, u.kd ? u.kd[base + j] : 0, pre)) continue;
+#pragma unroll
+        for (int n = 0; n < NC; n++) {
+            k[n] = load4<false>(p.k + (base + j) * p.ldkv + (int64_t)hk * u.d, 64 * n + 4 * l16, u.d);
+            v[n] = load4<false>(p.v + (base + j) * p.ldkv + (int64_t)hk * u.d, 64 * n + 4 * l16, u.d);
+        }
+        float pr, ds;
+        r.grads(u, k, v, j, pr, ds);
+#pragma unroll
+        for (int n = 0; n < NC; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) dq[n][e] = __builtin_fmaf(ds, k[n][e], dq[n][e]);
+    }
+    float *to = p.dq + r.tok * p.lddq + (int64_t)r.h * u.d;
+#pragma unroll
+    for (int n = 0; n < NC; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float s = join4(dq[n][e]) * u.scale;
+            const int c = 64 * n + 4 * l16 + e;
+            if (st == 0 && c < u.d) to[c] = p.acc ? to[c] + s : s;
+        }
+}
+
+// dk and dv of one key over rows r0 .. r1 - 1 by one wavefront; `pk` (dk) and `pv` (dv) are where they go.
+template <int DP>
+__device__ __forceinline__ void plain_dkv(const Rule &u, const Ptrs &p, int b, int hk, int j, int r0, int r1, int pre, float *pk,
+                                          float *pv, int acc) {
+    constexpr int NC = (DP + 63) / 64;
+    const int lane = threadIdx.x & 63, l16 = lane & 15, st = lane >> 4;
+    const int64_t key = (int64_t)b * u.lk + j;
+    floatx4 dk[NC], dv[NC], k[NC], v[NC];
+#pragma unroll
+    for (int n = 0; n < NC; n++) {
+        k[n] = load4<false>(p.k + key * p.ldkv + (int64_t)hk * u.d, 64 * n + 4 * l16, u.d);
+        v[n] = load4<false>(p.v + key * p.ldkv + (int64_t)hk * u.d, 64 * n + 4 * l16, u.d);
+        dk[n] = dv[n] = floatx4{0.f, 0.f, 0.f, 0.f};
+    }
+    const int kd = u.kd ? u.kd[key] : 0;
+    for (int rr = r0 + st; rr < r1; rr += 4) {
+        Pair<NC> r;
+        r.row(u, p, b, hk, rr, l16);
+        if (!r.sees(u, j, kd, pre)) continue;
+        float pr, ds;
+        r.grads(u, k, v, j, pr, ds);
+#pragma unroll
+        for (int n = 0; n < NC; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                dv[n][e] = __builtin_fmaf(pr, r.g[n][e], dv[n][e]);
+                dk[n][e] = __builtin_fmaf(ds, r.q[n][e], dk[n][e]);
+            }
+    }
+#pragma unroll
+    for (int n = 0; n < NC; n++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const float sk = join4(dk[n][e]) * u.scale, sv = join4(dv[n][e]);
+            const int c = 64 * n + 4 * l16 + e;
+            if (st == 0 && c < u.d) {
+                if (pk) pk[c] = acc ? pk[c] + sk : sk;
+                if (pv) pv[c] = acc ? pv[c] + sv : sv;
+            }
+        }
+}
+
+// D is split at a scale of its lane's own, a running 2^s like a softmax's maximum: a lane's sums all belong to one row (or
+// key), so they move with it when a block's largest |D| outgrows 2^15 of it. What a row with small values or a key with small
+// weights adds up then keeps its bits whatever its neighbours hold.
+constexpr int kNoScale = -100;
+__device__ __forceinline__ float ldexp_hw(float x, int e) { return __builtin_amdgcn_ldexpf(x, e); }
+// The scale's exponent after a block whose largest magnitude is `top`.
+__device__ __forceinline__ int grown(float top, int s) {
+    const int e = (int)((__float_as_uint(top) >> 23) & 255) - 127;
+    return e - s > 14 ? e - 10 : s;
+}
+
+// Four consecutive values of a result row, added to or written.
+__device__ __forceinline__ void put4(float *to, int c, int d, floatx4 v, int acc) {
+    if (c + 3 < d && (((uintptr_t)(to + c)) & 15) == 0) {
+        floatx4 *t = reinterpret_cast<floatx4 *>(to + c);
+        *t = acc ? *t + v : v;
+    } else {
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+            if (c + e < d) to[c + e] = acc ? to[c + e] + v[e] : v[e];
+    }
+}
+
+// Whether some of positions i0 .. i1 may see some of keys j0 .. j1, documents aside.
+__device__ __forceinline__ bool may_see(const Rule &u, int i0, int i1, int j0, int j1, int pre) {
+    return j0 < pre || (!(u.causal && j0 > i1) && !(u.window && (i0 - j1 >= u.window || j0 - i1 >= u.window)));
+}
+// Whether all of positions i0 .. i1 see all of keys j0 .. j1, documents aside.
+__device__ __forceinline__ bool all_see(const Rule &u, int i0, int i1, int j0, int j1, int pre) {
+    return j1 < pre || ((!u.causal || j1 <= i0) && (!u.window || (i1 - j0 < u.window && j1 - i0 < u.window)));
+}
+
+// ---------------------------------------------------------------------------------------------------- dk and dv
+// The step data of a block of rows: its scales and whether it is visited.
+struct RowStep {
+    float q, g2, q2;
+    int see;
+};
+template <int DP>
+__device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const BwdArgs &a, int i, char *sh) {
+    constexpr int S = DP / 16, ND = DP / 32, HALF = kStep * DP * 4, STAGE = 4 * HALF;
+    __shared__ float lq_[kListed], lg2[kListed], lq2[kListed];
+    __shared__ unsigned char lsee[kListed];
+    __shared__ __attribute__((aligned(16))) float rv[2][4][kStep];  // m, delta, position, slope of the step's rows
+    __shared__ int rdoc[2][kStep];
+    __shared__ uint32_t red[4][4];
+    const int kb = i % a.kblocks, split = (i / a.kblocks) % a.nsplit, item = i / (a.kblocks * a.nsplit);
+    const int b = item / u.Hk, hk = item - b * u.Hk, rows = u.G * u.lq;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
+    const int pre = u.prefix ? u.prefix[b] : 0;
+    const int first = kb * kKeys, last = min(first + kKeys, u.lk) - 1;
+    const int j = first + 32 * w + (lane & 31);
+    const bool live = first + 32 * w <= last;
+    const int kd = j <= last ? (u.kd ? u.kd[(int64_t)b * u.lk + j] : 0) : -1;
+    const int64_t kt0 = (int64_t)item * a.nt, rt0 = (int64_t)item * a.nr;
+    // the wavefront's block of keys (a wavefront past the last key repeats it and stores nothing)
+    const int t = min((first + 32 * w) / kBlock, a.nt - 1);
+    const Stats ks = a.ks[kt0 + t], vs = a.vs[kt0 + t];
+    const int tb = min(first / kBlock + 1, a.nt - 1);
+    const Stats v0 = a.vs[kt0 + first / kBlock], v1 = a.vs[kt0 + tb], k0 = a.ks[kt0 + first / kBlock], k1 = a.ks[kt0 + tb];
+    bool bad = max(max(v0.top, v1.top), max(k0.top, k1.top)) > kMostBits;
+    const float vref = fmaxf(v0.top ? v0.scale : 0.0f, v1.top ? v1.scale : 0.0f) > 0.0f
+                           ? fmaxf(v0.top ? v0.scale : 0.0f, v1.top ? v1.scale : 0.0f) : 1.0f;
+    const int kdlo = min(k0.doc_lo, k1.doc_lo), kdhi = max(k0.doc_hi, k1.doc_hi);
+    // the blocks of rows that may see them
+    int plo, phi;
+    pos_range(u, first, last, pre, plo, phi);
+    int r0 = max((plo - u.off) * u.G, split * a.per * kBlock);
+    int r1 = min((phi - u.off + 1) * u.G, (int)min((int64_t)rows, (int64_t)(split + 1) * a.per * kBlock));  // one past
+    if (phi < plo) r1 = r0;
+    const int t0 = r0 / kBlock, t1 = r1 <= r0 ? t0 - 1 : (r1 - 1) / kBlock;
+    uint32_t gt = 0, gl = 0xFFFFFFFFu, qt = 0, ql = 0xFFFFFFFFu;
+    auto looked = [&](int rt, RowStep &st) {
+        const RowStats r = a.rs[rt0 + rt];
+        st.q = r.q;
+        st.g2 = r.g2;
+        st.q2 = r.q2;
+        const int f = rt * kBlock, l = min(f + kBlock, rows) - 1;
+        st.see = may_see(u, f / u.G + u.off, l / u.G + u.off, first, last, pre);
+        if (u.qd) {
+            if (r.doc_hi < kdlo || r.doc_lo > kdhi || r.doc_hi < 0) st.see = 0;
+            if (r.doc_lo != r.doc_hi || kdlo != kdhi || r.doc_lo != kdlo || kdlo < 0) st.see |= 2;
+        }
+        if (r.g2_top == 0 && r.q2_top == 0) st.see = 0;  // rows without gradient
+        return r;
+    };
+    for (int rt = t0 + (int)threadIdx.x; rt <= t1; rt += 256) {
+        RowStep st;
+        const RowStats r = looked(rt, st);
+        bad = bad || r.bad;
+        gt = max(gt, r.g2_top);
+        qt = max(qt, r.q2_top);
+        if (r.g2_top) gl = min(gl, r.g2_top);
+        if (r.q2_top) ql = min(ql, r.q2_top);
+        if (rt - t0 < kListed) {
+            lq_[rt - t0] = st.q;
+            lg2[rt - t0] = st.g2;
+            lq2[rt - t0] = st.q2;
+            lsee[rt - t0] = (unsigned char)st.see;
+        }
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        gt = max(gt, (uint32_t)__shfl_xor((int)gt, o, 64));
+        qt = max(qt, (uint32_t)__shfl_xor((int)qt, o, 64));
+        gl = min(gl, (uint32_t)__shfl_xor((int)gl, o, 64));
+        ql = min(ql, (uint32_t)__shfl_xor((int)ql, o, 64));
+    }
+    if (lane == 0) {
+        red[w][0] = gt;
+        red[w][1] = qt;
+        red[w][2] = gl;
+        red[w][3] = ql;
+    }
+    bad = __syncthreads_or(bad);
+#pragma unroll
+    for (int n = 0; n < 4; n++) {
+        gt = max(gt, red[n][0]);
+        qt = max(qt, red[n][1]);
+        gl = min(gl, red[n][2]);
+        ql = min(ql, red[n][3]);
+    }
+    // the accumulators move between the blocks' scales: keep the largest move inside fp32
+    bad = bad || (gt && (gt >> 23) - (gl >> 23) > 60) || (qt && (qt >> 23) - (ql >> 23) > 60);
+    auto dest = [&](int n, int jj) -> float * {  // dk (0) or dv (1) of key jj
+        if (a.part) return a.part + (((int64_t)split * u.B * u.Hk + item) * u.lk + jj) * 2 * u.d + n * u.d;
+        float *base = n ? p.dv : p.dk;
+        return base ? base + ((int64_t)b * u.lk + jj) * p.lddkv + (int64_t)hk * u.d : nullptr;
+    };
+    const int acc = a.part ? 0 : p.acc;
+    if (__builtin_amdgcn_readfirstlane(bad)) {
+        for (int jj = first + 32 * w; jj <= min(last, first + 32 * w + 31); jj++)
+            plain_dkv<DP>(u, p, b, hk, jj, r0, r1, pre, dest(0, jj), dest(1, jj), acc);
+        return;
+    }
+    // K and V fragments of the wavefront's keys
+    u32x4 kh[S], km[S], vh[S], vm[S];
+    {
+        const int half = ((first + 32 * w) / 32) & 1;
+        const char *kf = a.kn + (kt0 + t) * plane_bytes(DP, 1) + half * HALF + lane * 16;
+        const char *vf = a.vn + (kt0 + t) * plane_bytes(DP, 1) + half * HALF + lane * 16;
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+            kh[s] = *reinterpret_cast<const u32x4 *>(kf + (2 * s) * 1024);
+            km[s] = *reinterpret_cast<const u32x4 *>(kf + (2 * s + 1) * 1024);
+            vh[s] = *reinterpret_cast<const u32x4 *>(vf + (2 * s) * 1024);
+            vm[s] = *reinterpret_cast<const u32x4 *>(vf + (2 * s + 1) * 1024);
+        }
+    }
+    floatx16 dk[ND], dv[ND];
+#pragma unroll
+    for (int n = 0; n < ND; n++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) dk[n][e] = dv[n][e] = 0.0f;
+    float g2cur = 1.0f, q2cur = 1.0f;
+    const float A = vs.scale / vref, Bd = 1.0f / vref;
+    int sd = kNoScale;  // dk's sums are in units of 2^sd
+    const int steps = (t1 - t0 + 1) * 2;
+    auto next = [&](int it) {
+        for (it++; it < steps; it++) {
+            const int f = t0 * kBlock + it * kStep;
+            if (f >= r1) return steps;
+            if (f + kStep <= r0) continue;
+            if ((it >> 1) >= kListed || (lsee[it >> 1] & 1)) return it;
+        }
+        return steps;
+    };
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)(sh + 256);
+    auto stage = [&](int it, int buf) {
+        const int64_t off = (rt0 + t0) * plane_bytes(DP, 1) + (int64_t)it * HALF + lane * 16;
+        const uint32_t to = lds0 + (uint32_t)(buf * STAGE);
+        constexpr int PER = HALF / 4096;
+        auto one = [&](const char *src, int n) {
+#pragma unroll
+            for (int q = 0; q < PER; q++) load_to_lds(src + off + (4 * q + w) * 1024, to + (uint32_t)(n * HALF + (4 * q + w) * 1024));
+        };
+        one(a.qn, 0);
+        one(a.gn, 1);
+        one(a.g2, 2);
+        one(a.q2, 3);
+    };
+    // this thread's value of the step's rows: m, delta, position, slope by wavefront pairs; documents by the last threads
+    auto row_value = [&](int it) -> float {
+        const int which = threadIdx.x >> 5, rr = t0 * kBlock + it * kStep + (threadIdx.x & 31);
+        const int64_t at = rt0 * kBlock + rr;
+        if (which == 0) return a.v.m[at];
+        if (which == 1) return a.v.delta[at] * Bd;
+        const Row row = row_of(u, hk, min(rr, rows - 1));
+        if (which == 2) return __int_as_float(row.t + u.off);
+        if (which == 3) return u.slopes ? u.slopes[row.h] * kLog2e : 0.0f;
+        if (which == 4) return __int_as_float(u.qd ? u.qd[(int64_t)b * u.lq + row.t] : 0);
+        return 0.0f;
+    };
+    auto keep = [&](float v, int buf) {
+        const int which = threadIdx.x >> 5, r = threadIdx.x & 31;
+        if (which < 4) rv[buf][which][r] = v;
+        else if (which == 4) rdoc[buf][r] = __float_as_int(v);
+    };
+    int it = next(-1), buf = 0;
+    if (it < steps) {
+        stage(it, 0);
+        keep(row_value(it), 0);
+    }
+    while (it < steps) {
+        wait_loads();
+        __syncthreads();
+        const int nx = next(it);
+        float nv = 0.0f;
+        if (nx < steps) {
+            stage(nx, buf ^ 1);
+            nv = row_value(nx);
+        }
+        RowStep st;
+        if ((it >> 1) < kListed) {
+            st.q = lq_[it >> 1];
+            st.g2 = lg2[it >> 1];
+            st.q2 = lq2[it >> 1];
+            st.see = lsee[it >> 1];
+        } else {
+            looked(t0 + (it >> 1), st);
+        }
+        const int f0 = t0 * kBlock + it * kStep, f1 = min(f0 + kStep, rows) - 1;
+        const int i0 = f0 / u.G + u.off, i1 = f1 / u.G + u.off;
+        const int j0 = first + 32 * w, j1 = min(j0 + 31, last);
+        if (live && may_see(u, i0, i1, j0, j1, pre)) {
+            if (st.g2 != g2cur) {
+                const float c = g2cur / st.g2;
+#pragma unroll
+                for (int n = 0; n < ND; n++) dv[n] *= c;
+                g2cur = st.g2;
+            }
+            if (st.q2 != q2cur) {
+                const float c = q2cur / st.q2;
+#pragma unroll
+                for (int n = 0; n < ND; n++) dk[n] *= c;
+                q2cur = st.q2;
+            }
+            const char *qf = sh + 256 + buf * STAGE + lane * 16, *gf = qf + HALF, *g2f = gf + HALF, *q2f = g2f + HALF;
+            floatx16 x, dp;
+#pragma unroll
+            for (int e = 0; e < 16; e++) x[e] = dp[e] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < S; s++) {
+                x = mma3(*reinterpret_cast<const u32x4 *>(qf + (2 * s) * 1024),
+                         *reinterpret_cast<const u32x4 *>(qf + (2 * s + 1) * 1024), kh[s], km[s], x);
+                dp = mma3(*reinterpret_cast<const u32x4 *>(gf + (2 * s) * 1024),
+                          *reinterpret_cast<const u32x4 *>(gf + (2 * s + 1) * 1024), vh[s], vm[s], dp);
+            }
+            const float cs = st.q * ks.scale;
+            const bool whole = !(st.see & 2) && all_see(u, i0, i1, j0, j1, pre);
+            if (u.icap != 0.0f) {
+                const float ic = u.icap * cs;
+                float big = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 16; e++) big = fmaxf(big, __builtin_fabsf(x[e]));
+                const bool small = !__any(big * __builtin_fabsf(ic) >= kTanhSmall);
+#pragma unroll
+                for (int e = 0; e < 16; e++) x[e] *= ic;
+                if (small) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) x[e] = tanh_small(x[e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) x[e] = tanh_any(x[e]);
+                }
+            }
+            const float fx = u.icap != 0.0f ? u.capl2 : u.cl2 * cs;
+            float top = 0.0f;
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const floatx4 m4 = *reinterpret_cast<const floatx4 *>(&rv[buf][0][8 * q + 4 * g]);
+                const floatx4 d4 = *reinterpret_cast<const floatx4 *>(&rv[buf][1][8 * q + 4 * g]);
+                floatx4 y;
+#pragma unroll
+                for (int r = 0; r < 4; r++) y[r] = __builtin_fmaf(x[4 * q + r], fx, (float)kLift - m4[r]);
+                if (u.slopes || !whole) {
+                    const floatx4 p4 = *reinterpret_cast<const floatx4 *>(&rv[buf][2][8 * q + 4 * g]);
+                    if (u.slopes) {
+                        const floatx4 s4 = *reinterpret_cast<const floatx4 *>(&rv[buf][3][8 * q + 4 * g]);
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const int gap = __float_as_int(p4[r]) - j;
+                            y[r] = __builtin_fmaf(-s4[r], __builtin_fabsf((float)gap), y[r]);
+                        }
+                    }
+                    if (!whole) {
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            bool ok = in_reach(u, __float_as_int(p4[r]) - j, j, pre);
+                            if (st.see & 2) {
+                                const int qd = rdoc[buf][8 * q + 4 * g + r];
+                                ok = ok && qd >= 0 && qd == kd;
+                            }
+                            y[r] = ok ? y[r] : -3e38f;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int e = 4 * q + r;
+                    const float ex = exp2_hw(y[r]);
+                    float ds = ex * __builtin_fmaf(dp[e], A, -d4[r]);
+                    if (u.icap != 0.0f) ds *= __builtin_fmaf(-x[e], x[e], 1.0f);
+                    dp[e] = ds;
+                    x[e] = ex;
+                    top = fmaxf(top, __builtin_fabsf(ds));
+                }
+            }
+            top = pair_max(top);
+            const int sn = grown(top, sd);
+            if (__any(sn != sd)) {
+                const int by = sd - sn;
+#pragma unroll
+                for (int n = 0; n < ND; n++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) dk[n][e] = ldexp_hw(dk[n][e], by);
+                sd = sn;
+            }
+            const float fd = pow2(-sd);
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                float e8[8];
+                u32x4 ph, pm, dh, dm;
+#pragma unroll
+                for (int e = 0; e < 8; e++) e8[e] = x[8 * s + e];
+                split8(e8, ph, pm);
+#pragma unroll
+                for (int e = 0; e < 8; e++) e8[e] = dp[8 * s + e] * fd;
+                split8(e8, dh, dm);
+#pragma unroll
+                for (int c = 0; c < ND; c++) {
+                    const int at = ((s * ND + c) * 2) * 1024;
+                    dv[c] = mma3(*reinterpret_cast<const u32x4 *>(g2f + at), *reinterpret_cast<const u32x4 *>(g2f + at + 1024), ph,
+                                 pm, dv[c]);
+                    dk[c] = mma3(*reinterpret_cast<const u32x4 *>(q2f + at), *reinterpret_cast<const u32x4 *>(q2f + at + 1024), dh,
+                                 dm, dk[c]);
+                }
+            }
+        }
+        if (nx < steps) keep(nv, buf ^ 1);
+        it = nx;
+        buf ^= 1;
+    }
+    if (j > last) return;
+    const float fv = g2cur * pow2(-kLift), fk = q2cur * vref * pow2(-kLift) * u.scale;
+    float *tk = dest(0, j), *tv = dest(1, j);
+#pragma unroll
+    for (int n = 0; n < ND; n++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const int c = 32 * n + 8 * q + 4 * g;
+            const floatx4 xk = floatx4{ldexp_hw(dk[n][4 * q], sd), ldexp_hw(dk[n][4 * q + 1], sd),
+                                       ldexp_hw(dk[n][4 * q + 2], sd), ldexp_hw(dk[n][4 * q + 3], sd)} * fk;
+            const floatx4 xv = floatx4{dv[n][4 * q], dv[n][4 * q + 1], dv[n][4 * q + 2], dv[n][4 * q + 3]} * fv;
+            if (tk) put4(tk, c, u.d, xk, acc);
+            if (tv) put4(tv, c, u.d, xv, acc);
+        }
+}
+
+// ------------------------------------------------------------------------------------------------------------ dq
+template <int DP>
+__device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const BwdArgs &a, int i, char *sh) {
+    constexpr int S = DP / 16, ND = DP / 32, HALF = kStep * DP * 4, STAGE = 3 * HALF;
+    __shared__ float lk_[kListed], lv_[kListed];
+    __shared__ signed char lstep[kListed];
+    __shared__ unsigned char lsee[kListed];
+    __shared__ uint32_t red[4][6];
+    const int rb = a.rblocks - 1 - i % a.rblocks, item = i / a.rblocks;  // the longest rows of a causal rule first
+    const int b = item / u.Hk, hk = item - b * u.Hk, rows = u.G * u.lq;
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
+    const int pre = u.prefix ? u.prefix[b] : 0;
+    const int first = rb * kKeys, last = min(first + kKeys, rows) - 1;
+    const int rr = first + 32 * w + (lane & 31);
+    const Row row = row_of(u, hk, min(rr, rows - 1));
+    const int64_t tok = (int64_t)b * u.lq + row.t;
+    const int pos = row.t + u.off, doc = u.qd ? u.qd[tok] : 0;
+    const float slope = u.slopes ? u.slopes[row.h] * kLog2e : 0.0f;
+    const bool live = first + 32 * w <= last;
+    const int64_t kt0 = (int64_t)item * a.nt, rt0 = (int64_t)item * a.nr;
+    const int rt = min((first + 32 * w) / kBlock, a.nr - 1);
+    const RowStats rs = a.rs[rt0 + rt];
+    const RowStats ra = a.rs[rt0 + first / kBlock], rz = a.rs[rt0 + min(first / kBlock + 1, a.nr - 1)];
+    bool bad = ra.bad || rz.bad;
+    const int qlo = min(ra.doc_lo, rz.doc_lo), qhi = max(ra.doc_hi, rz.doc_hi);
+    int lo, hi;
+    const int i0 = first / u.G + u.off, i1 = last / u.G + u.off;
+    key_range(u, i0, i1, pre, lo, hi);
+    const int t0 = lo / kBlock, t1 = hi < lo ? t0 - 1 : hi / kBlock;
+    uint32_t kt = 0, vt = 0, kl = 0xFFFFFFFFu;
+    for (int t = t0 + (int)threadIdx.x; t <= t1; t += 256) {
+        kt = max(kt, a.ks[kt0 + t].top);
+        kl = min(kl, a.ks[kt0 + t].low);
+        vt = max(vt, a.vs[kt0 + t].top);
+    }
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        kt = max(kt, (uint32_t)__shfl_xor((int)kt, o, 64));
+        vt = max(vt, (uint32_t)__shfl_xor((int)vt, o, 64));
+        kl = min(kl, (uint32_t)__shfl_xor((int)kl, o, 64));
+    }
+    if (lane == 0) {
+        red[w][0] = kt;
+        red[w][1] = vt;
+        red[w][2] = kl;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int n = 0; n < 4; n++) {
+        kt = max(kt, red[n][0]);
+        vt = max(vt, red[n][1]);
+        kl = min(kl, red[n][2]);
+    }
+    bad = bad || kt > kMostBits || vt > kMostBits || !even_rows(kt, kl);
+    if (__builtin_amdgcn_readfirstlane(bad)) {
+        for (int r = first + 32 * w; r <= min(last, first + 32 * w + 31); r++) plain_dq<DP>(u, p, b, hk, r, lo, hi, pre);
+        return;
+    }
+    const int ek = kt ? scale_exp(kt) : 0, ev = vt ? scale_exp(vt) : 0;
+    const bool some_padded = qlo < 0;
+    auto looked = [&](int t, float &sk, float &sv, int &step) -> int {
+        const Stats ks = a.ks[kt0 + t], vs = a.vs[kt0 + t];
+        sk = ks.scale;
+        sv = vs.top ? vs.scale * pow2(-ev) : 1.0f;
+        step = ks.top ? ((int)(__float_as_uint(ks.scale) >> 23) - 127 - ek) / 4 : 0;
+        const int j0 = t * kBlock, j1 = j0 + kBlock - 1;
+        int see = may_see(u, i0, i1, j0, j1, pre);
+        if (u.qd) {
+            if (ks.doc_hi < 0 || ks.doc_hi < qlo || ks.doc_lo > qhi) see = 0;
+            if (some_padded || ks.doc_lo < 0 || ks.doc_lo != ks.doc_hi || qlo != qhi || ks.doc_lo != qlo) see |= 2;
+        }
+        return see;
+    };
+    for (int t = t0 + (int)threadIdx.x; t <= t1 && t < t0 + kListed; t += 256) {
+        float sk, sv;
+        int step;
+        const int see = looked(t, sk, sv, step);
+        lk_[t - t0] = sk;
+        lv_[t - t0] = sv;
+        lstep[t - t0] = (signed char)step;
+        lsee[t - t0] = (unsigned char)see;
+    }
+    __syncthreads();
+    // Q and G fragments of the wavefront's rows, and their values
+    u32x4 qh[S], qm[S], gh[S], gm[S];
+    {
+        const int half = ((first + 32 * w) / 32) & 1;
+        const char *qf = a.qn + (rt0 + rt) * plane_bytes(DP, 1) + half * HALF + lane * 16;
+        const char *gf = a.gn + (rt0 + rt) * plane_bytes(DP, 1) + half * HALF + lane * 16;
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+            qh[s] = *reinterpret_cast<const u32x4 *>(qf + (2 * s) * 1024);
+            qm[s] = *reinterpret_cast<const u32x4 *>(qf + (2 * s + 1) * 1024);
+            gh[s] = *reinterpret_cast<const u32x4 *>(gf + (2 * s) * 1024);
+            gm[s] = *reinterpret_cast<const u32x4 *>(gf + (2 * s + 1) * 1024);
+        }
+    }
+    const int64_t at = rt0 * kBlock + min(rr, a.nr * kBlock - 1);
+    const float m = a.v.m[at], delta = a.v.delta[at] * pow2(-ev), wr = a.v.w[at];
+    floatx16 dq[ND];
+    int sd = kNoScale;  // dq's sums are in units of 2^sd
+#pragma unroll
+    for (int n = 0; n < ND; n++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) dq[n][e] = 0.0f;
+    const int wi0 = min(first + 32 * w, last) / u.G + u.off, wi1 = min(first + 32 * w + 31, last) / u.G + u.off;
+    const int steps = (t1 - t0 + 1) * 2;
+    auto next = [&](int it) {
+        for (it++; it < steps; it++) {
+            if (t0 * kBlock + it * kStep > hi) return steps;
+            if ((it >> 1) >= kListed || (lsee[it >> 1] & 1)) return it;
+        }
+        return steps;
+    };
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)(sh + 256);
+    auto stage = [&](int it, int buf) {
+        const int64_t off = (kt0 + t0) * plane_bytes(DP, 1) + (int64_t)it * HALF + lane * 16;
+        const uint32_t to = lds0 + (uint32_t)(buf * STAGE);
+        constexpr int PER = HALF / 4096;
+        auto one = [&](const char *src, int n) {
+#pragma unroll
+            for (int q = 0; q < PER; q++) load_to_lds(src + off + (4 * q + w) * 1024, to + (uint32_t)(n * HALF + (4 * q + w) * 1024));
+        };
+        one(a.kn, 0);
+        one(a.vn, 1);
+        one(a.kt, 2);
+    };
+    int it = next(-1), buf = 0;
+    if (it < steps) stage(it, 0);
+    while (it < steps) {
+        wait_loads();
+        __syncthreads();
+        const int nx = next(it);
+        if (nx < steps) stage(nx, buf ^ 1);
+        float sk, sv;
+        int step, see;
+        if ((it >> 1) < kListed) {
+            sk = lk_[it >> 1];
+            sv = lv_[it >> 1];
+            step = lstep[it >> 1];
+            see = lsee[it >> 1];
+        } else {
+            see = looked(t0 + (it >> 1), sk, sv, step);
+        }
+        const int j0 = t0 * kBlock + it * kStep, j1 = j0 + kStep - 1;
+        if (live && may_see(u, wi0, wi1, j0, j1, pre)) {
+            const char *kf = sh + 256 + buf * STAGE + lane * 16, *vf = kf + HALF, *ktf = vf + HALF;
+            floatx16 x, dp;
+#pragma unroll
+            for (int e = 0; e < 16; e++) x[e] = dp[e] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < S; s++) {
+                x = mma3(*reinterpret_cast<const u32x4 *>(kf + (2 * s) * 1024),
+                         *reinterpret_cast<const u32x4 *>(kf + (2 * s + 1) * 1024), qh[s], qm[s], x);
+                dp = mma3(*reinterpret_cast<const u32x4 *>(vf + (2 * s) * 1024),
+                          *reinterpret_cast<const u32x4 *>(vf + (2 * s + 1) * 1024), gh[s], gm[s], dp);
+            }
+            const float cs = rs.q * sk;
+            const bool whole = j1 < u.lk && !(see & 2) && all_see(u, wi0, wi1, j0, j1, pre);
+            if (u.icap != 0.0f) {
+                const float ic = u.icap * cs;
+                float big = 0.0f;
+#pragma unroll
+                for (int e = 0; e < 16; e++) big = fmaxf(big, __builtin_fabsf(x[e]));
+                const bool small = !__any(big * __builtin_fabsf(ic) >= kTanhSmall);
+#pragma unroll
+                for (int e = 0; e < 16; e++) x[e] *= ic;
+                if (small) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) x[e] = tanh_small(x[e]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) x[e] = tanh_any(x[e]);
+                }
+            }
+            const float fx = u.icap != 0.0f ? u.capl2 : u.cl2 * cs, mu = 4.0f * (float)step - m;
+            const float gap0 = (float)(pos - j0 - 4 * g);
+            float top = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                float y = __builtin_fmaf(x[e], fx, mu);
+                const int o = 8 * (e >> 2) + (e & 3);
+                if (u.slopes) y = __builtin_fmaf(-slope, __builtin_fabsf(gap0 - (float)o), y);
+                if (!whole) {
+                    const int jj = j0 + 4 * g + o;
+                    bool ok = jj < u.lk && in_reach(u, pos - jj, jj, pre);
+                    if (see & 2) ok = ok && doc >= 0 && u.kd[(int64_t)b * u.lk + min(jj, u.lk - 1)] == doc;
+                    y = ok ? y : -3e38f;
+                }
+                float ds = exp2_hw(y) * __builtin_fmaf(dp[e], sv, -delta);
+                if (u.icap != 0.0f) ds *= __builtin_fmaf(-x[e], x[e], 1.0f);
+                dp[e] = ds;
+                top = fmaxf(top, __builtin_fabsf(ds));
+            }
+            top = pair_max(top);
+            const int sn = grown(top, sd);
+            if (__any(sn != sd)) {
+                const int by = sd - sn;
+#pragma unroll
+                for (int n = 0; n < ND; n++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) dq[n][e] = ldexp_hw(dq[n][e], by);
+                sd = sn;
+            }
+            const float fd = pow2(-sd);
+#pragma unroll
+            for (int s = 0; s < 2; s++) {
+                float e8[8];
+                u32x4 dh, dm;
+#pragma unroll
+                for (int e = 0; e < 8; e++) e8[e] = dp[8 * s + e] * fd;
+                split8(e8, dh, dm);
+#pragma unroll
+                for (int c = 0; c < ND; c++) {
+                    const char *f = ktf + ((s * ND + c) * 2) * 1024;
+                    dq[c] = mma3(*reinterpret_cast<const u32x4 *>(f), *reinterpret_cast<const u32x4 *>(f + 1024), dh, dm, dq[c]);
+                }
+            }
+        }
+        it = nx;
+        buf ^= 1;
+    }
+    if (rr > last) return;
+    const float f = u.scale * pow2(ek) * pow2(ev);
+    float *to = p.dq + tok * p.lddq + (int64_t)row.h * u.d;
+#pragma unroll
+    for (int n = 0; n < ND; n++)
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            const floatx4 v = floatx4{ldexp_hw(dq[n][4 * q], sd), ldexp_hw(dq[n][4 * q + 1], sd),
+                                      ldexp_hw(dq[n][4 * q + 2], sd), ldexp_hw(dq[n][4 * q + 3], sd)} * f * wr;
+            put4(to, 32 * n + 8 * q + 4 * g, u.d, v, p.acc);
+        }
+}
+
+template <int DP>
+__global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) k_scored_bwd_mm(Rule u, Ptrs p, BwdArgs a) {
+    OM_LDS_POISON();
+    __shared__ __attribute__((aligned(16))) char sh[256 + 2 * 4 * kStep * DP * 4];  // no stage at LDS address 0
+    int lin = blockIdx.x;
+    // ids are dealt round-robin over the 8 XCDs: the workgroups of one head stay on one
+    if (lin < a.first_rows) {
+        if ((a.first_rows & 7) == 0) lin = (lin & 7) * (a.first_rows >> 3) + (lin >> 3);
+        keys_role<DP>(u, p, a, lin, sh);
+    } else {
+        const int total = gridDim.x - a.first_rows;
+        lin -= a.first_rows;
+        if ((total & 7) == 0) lin = (lin & 7) * (total >> 3) + (lin >> 3);
+        rows_role<DP>(u, p, a, lin, sh);
+    }
+}
+
+// dk and dv from the splits' sums, in split order; a thread per value.
+__global__ void __launch_bounds__(256) k_scored_join_dkv(Rule u, Ptrs p, int nsplit, const float *__restrict__ part) {
+    OM_LDS_POISON();
+    const int64_t each = (int64_t)u.B * u.Hk * u.lk * 2 * u.d, f = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (f >= each) return;
+    float s = 0.0f;
+    for (int n = 0; n < nsplit; n++) s += part[n * each + f];
+    const int c = (int)(f % u.d), which = (int)(f / u.d % 2);
+    const int64_t key = f / (2 * u.d), item = key / u.lk;
+    float *base = which ? p.dv : p.dk;
+    if (!base) return;
+    float *to = base + ((item / u.Hk) * u.lk + key % u.lk) * p.lddkv + (item % u.Hk) * u.d + c;
+    *to = p.acc ? *to + s : s;
+}
+
+}  // namespace
+
+namespace osc {
+
+om_status bwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p) {
+    const char *what = "om_attention_bwd_scored";
+    const int64_t items = (int64_t)u.B * u.Hk, rows = (int64_t)u.G * u.lq;
+    const int dp = u.d <= 32 ? 32 : u.d <= 64 ? 64 : u.d <= 96 ? 96 : 128;
+    BwdArgs a = {};
+    a.nt = (u.lk + kBlock - 1) / kBlock;
+    a.nr = (int)((rows + kBlock - 1) / kBlock);
+    a.kblocks = (u.lk + kKeys - 1) / kKeys;
+    a.rblocks = (int)((rows + kKeys - 1) / kKeys);
+    const bool keys = p.dk || p.dv;
+    // Split the rows of dk and dv while those workgroups leave CUs idle, in pieces of at least eight blocks.
+    int64_t ns = 1, wk = items * a.kblocks;
+    if (wk < 2 * ctx->num_cus) ns = 2 * ctx->num_cus / wk;
+    ns = ns > a.nr / 8 ? a.nr / 8 : ns;
+    ns = ns < 1 ? 1 : ns;
+    a.per = (int)((a.nr + ns - 1) / ns);
+    a.nsplit = (int)((a.nr + a.per - 1) / a.per);
+    wk = keys ? wk * a.nsplit : 0;
+    const int64_t wr = p.dq ? items * a.rblocks : 0, jobs = items * (2 * (int64_t)a.nt + a.nr);
+    OM_REQUIRE(ctx, wk + wr <= INT32_MAX && jobs <= INT32_MAX, "%s: too many row blocks", what);
+    a.first_rows = (int)wk;
+    const int64_t kp = plane_bytes(dp, items * a.nt), rp = plane_bytes(dp, items * a.nr);
+    const int64_t vals = items * a.nr * kBlock * (int64_t)sizeof(float);
+    const int64_t part = keys && a.nsplit > 1 ? (int64_t)sizeof(float) * a.nsplit * items * u.lk * 2 * u.d : 0;
+    const int64_t stats = 2 * items * a.nt * (int64_t)sizeof(Stats) + items * a.nr * (int64_t)sizeof(RowStats);
+    float *scr;
+    if (om_status s = om::scratch2(ctx, (uint64_t)(3 * kp + 4 * rp + 3 * vals + stats + part), &scr)) return s;
+    char *at = reinterpret_cast<char *>(scr);
+    auto take = [&](int64_t bytes) {
+        char *x = at;
+        at += bytes;
+        return x;
+    };
+    SplitOut ko = {}, vo = {};
+    RowsOut ro = {};
+    a.kn = ko.rows = take(kp);
+    a.kt = ko.cols = take(kp);
+    a.vn = vo.rows = take(kp);
+    a.qn = ro.q = take(rp);
+    a.gn = ro.g = take(rp);
+    a.g2 = ro.g2 = take(rp);
+    a.q2 = ro.q2 = take(rp);
+    ro.v.m = reinterpret_cast<float *>(take(vals));
+    ro.v.delta = reinterpret_cast<float *>(take(vals));
+    ro.v.w = reinterpret_cast<float *>(take(vals));
+    a.v = ro.v;
+    a.ks = ko.stats = reinterpret_cast<Stats *>(take(items * a.nt * (int64_t)sizeof(Stats)));
+    a.vs = vo.stats = reinterpret_cast<Stats *>(take(items * a.nt * (int64_t)sizeof(Stats)));
+    a.rs = ro.stats = reinterpret_cast<RowStats *>(take(items * a.nr * (int64_t)sizeof(RowStats)));
+    a.part = part ? reinterpret_cast<float *>(take(part)) : nullptr;
+    auto al16 = [](const void *x) { return ((uintptr_t)x & 15) == 0; };
+    const bool vec = u.d % 4 == 0 && p.ldq % 4 == 0 && p.ldkv % 4 == 0 && p.ldo % 4 == 0 && p.ldg % 4 == 0 && al16(p.q) &&
+                     al16(p.k) && al16(p.v) && al16(p.o) && al16(p.g);
+    auto go = [&](auto dpc) {
+        constexpr int DP = decltype(dpc)::value;
+        auto split = [&](auto kern) {
+            hipLaunchKernelGGL(kern, dim3((unsigned)jobs), dim3(256), 0, ctx->stream, u, p, ko, vo, ro, a.nt, a.nr);
+        };
+        vec ? split(k_scored_split_bwd<DP, true>) : split(k_scored_split_bwd<DP, false>);
+        hipLaunchKernelGGL(k_scored_bwd_mm<DP>, dim3((unsigned)(wk + wr)), dim3(256), 0, ctx->stream, u, p, a);
+    };
+    if (dp == 32) go(std::integral_constant<int, 32>());
+    else if (dp == 64) go(std::integral_constant<int, 64>());
+    else if (dp == 96) go(std::integral_constant<int, 96>());
+    else go(std::integral_constant<int, 128>());
+    if (part) {
+        const int64_t values = items * u.lk * 2 * u.d;
+        hipLaunchKernelGGL(k_scored_join_dkv, dim3((unsigned)((values + 255) / 256)), dim3(256), 0, ctx->stream, u, p, a.nsplit,
+                           a.part);
+    }
+    return OM_LAUNCH_CHECK(ctx, what);
+}
+
+}  // namespace osc

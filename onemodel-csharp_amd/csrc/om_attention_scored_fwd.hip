@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(256, 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArg
         qlo = min(qlo, (int)red[i][3]);
         qhi = max(qhi, (int)red[i][4]);
     }
-    bad = bad || ktop > kMostBits || vtop > kMostBits || (vtop && (vtop >> 23) - (vlow >> 23) > 16);
+    bad = bad || ktop > kMostBits || vtop > kMostBits || !even_rows(vtop, vlow);
     if (__builtin_amdgcn_readfirstlane(bad)) {
         for (int r = first + 32 * w; r <= min(last, first + 32 * w + 31); r++)
             plain_row<DP>(u, p, b, hk, r, lo, hi, split, a.nsplit, a.part);

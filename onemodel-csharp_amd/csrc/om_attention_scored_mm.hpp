@@ -1,12 +1,12 @@
 // Scored attention on the matrix cores: the operand form that the forward and backward kernels share.
 //
 // fp32 products as three fp16 products. A block of 64 rows of an operand is scaled by a power of two that brings its
-// largest value to 2^10 .. 2^14 and split into x = h + m + r, h and m fp16 (11 + 11 significand bits, |r| below 2^-22 |x|,
-// or 2^-35 of the block's largest value where m is subnormal); a product keeps hh, hm, mh. The dropped terms are together
+// largest value to 2^11 .. 2^15 and split into x = h + m + r, h and m fp16 (11 + 11 significand bits, |r| below 2^-22 |x|,
+// or 2^-36 of the block's largest value where m is subnormal); a product keeps hh, hm, mh. The dropped terms are together
 // about 2^-23 of |x||y|, so a sum of products keeps fp32's accuracy, at a third of the fp16 matrix rate (840 TFLOP/s
 // where v_mfma_f32_16x16x4_f32 has 157 and the six-term bf16 split of om_split.hpp 419), and a split takes two vector
 // operations a value where the bf16 one takes six. What fp16's range does not hold is found beforehand (Stats): a block
-// with an infinity, a NaN or a magnitude outside 2^-40 .. 2^40, or rows whose largest values are more than 2^16 apart.
+// with an infinity, a NaN or a magnitude outside 2^-40 .. 2^40, or rows whose largest values are more than 2^14 apart.
 // A workgroup that would use such a block computes its rows by plain fp32 sums instead (om_attention_scored.hip).
 //
 // Operands lie in scratch in fragment order: v_mfma_f32_32x32x16_f16 takes, from lane l, eight values of row l % 32 at
@@ -42,13 +42,16 @@ constexpr uint32_t kInfBits = 0x7F800000u;
 constexpr uint32_t kMostBits = (127u + 40) << 23, kLeastBits = (127u - 40) << 23;  // 2^40, 2^-40
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
-// The exponent e of a scale 2^-e that brings `top` (bits of a magnitude in range) to 2^10 .. 2^14; steps of 2^4, so that
+// The exponent e of a scale 2^-e that brings `top` (bits of a magnitude in range) to 2^11 .. 2^15; steps of 2^4, so that
 // neighbouring blocks mostly share it.
 __device__ __forceinline__ int scale_exp(uint32_t top) {
-    const int e = (int)(top >> 23) - 127 - 13;
+    const int e = (int)(top >> 23) - 127 - 14;
     return (e + 3) & ~3;
 }
 __device__ __forceinline__ bool in_range(uint32_t top) { return top == 0 || (top >= kLeastBits && top <= kMostBits); }
+// Whether the smallest nonzero row maximum is within 2^14 of the largest: every row then keeps its 22 bits but the last one
+// or two.
+__device__ __forceinline__ bool even_rows(uint32_t top, uint32_t low) { return top == 0 || (top >> 23) - (low >> 23) <= 14; }
 
 // Two values split into packed fp16 pairs.
 __device__ __forceinline__ void split2(float a, float b, uint32_t &h, uint32_t &m) {

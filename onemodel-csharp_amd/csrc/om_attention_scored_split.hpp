@@ -122,7 +122,7 @@ __device__ __forceinline__ void split_keys(const Rule &u, const float *src, int6
         dlo = min(dlo, j >= u.lk ? INT32_MAX : doc);
     }
     block_top(top4, top, low, sh);
-    const bool ok = in_range(top);
+    const bool ok = in_range(top) && even_rows(top, low);
     const int e = ok && top ? scale_exp(top) : 0;
     const float w = pow2(-e);
 #pragma unroll
@@ -145,6 +145,142 @@ __device__ __forceinline__ void split_keys(const Rule &u, const float *src, int6
         st.top = ok ? top : 0xFFFFFFFFu;
         st.low = low;
         st.scale = pow2(e);
+        st.doc_lo = dlo;
+        st.doc_hi = dhi;
+        o.stats[at] = st;
+    }
+}
+
+// What the backward keeps of a row (a query of one head), [B Hk][rows padded to blocks] each.
+struct RowVals {
+    float *m;      // the forward's reference exponent; 3e38 for a row that has nothing to give (its weights become 0)
+    float *delta;  // g . o times 2^-re, re the exponent of g's row scale
+    float *w;      // 2^re / l: what the row's sums are multiplied with at the end; 0 for a row without gradient
+};
+// Its blocks of 64 rows.
+struct RowStats {
+    float q, g2, q2;       // scales 2^e of q, of g / l and of q w
+    uint32_t g2_top, q2_top;  // largest magnitudes (bits) of the latter two
+    uint32_t bad;          // the split cannot hold the block
+    int32_t doc_lo, doc_hi;
+};
+struct RowsOut {
+    char *q, *g;    // rows form: q by one scale per block, g by one per row
+    char *g2, *q2;  // columns form: g / l (for dv) and q w (for dk)
+    RowVals v;
+    RowStats *stats;
+};
+constexpr uint32_t kWideMost = (127u + 100) << 23, kWideLeast = (127u - 100) << 23;
+constexpr float kNoRow = 3e38f;
+
+// Block t of the rows of (b, hk) for the backward.
+template <int DP, bool VEC>
+__device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, int hk, int t, int64_t at, const RowsOut &o,
+                                           char *lds, uint32_t *sh) {
+    constexpr int NCH = Share<DP>::NCH;
+    const int rows = u.G * u.lq;
+    const int64_t all = (int64_t)u.B * u.Hk * rows;
+    Share<DP> s, g;
+    float rl[4], w[4], delta[4], m[4];
+    uint32_t qt[4], gt[4];
+    int dlo = INT32_MAX, dhi = INT32_MIN;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int rr = t * kBlock + 4 * (threadIdx.x >> 4) + i;
+        const bool there = rr < rows;
+        const Row row = row_of(u, hk, min(rr, rows - 1));
+        const int64_t tok = (int64_t)b * u.lq + row.t, sr = stat_at(u, b, row);
+        m[i] = p.st[sr];
+        rl[i] = there ? p.st[all + sr] : 0.0f;
+        const bool on = rl[i] != 0.0f;
+        if (there) {
+            const int doc = u.qd ? u.qd[tok] : 0;
+            dlo = min(dlo, doc);
+            dhi = max(dhi, doc);
+        }
+        s.template load<VEC>(i, p.q + tok * p.ldq + (int64_t)row.h * u.d, on, u.d);
+        g.template load<VEC>(i, p.g + tok * p.ldg + (int64_t)row.h * u.d, on, u.d);
+        Share<DP> ov;
+        ov.template load<VEC>(0, p.o + tok * p.ldo + (int64_t)row.h * u.d, on, u.d);
+        float dot = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NCH; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) dot = __builtin_fmaf(g.x[i][n][e], ov.x[0][n][e], dot);
+        dot = row_sum(dot);
+        qt[i] = s.row_top(i);
+        gt[i] = g.row_top(i);
+        const bool fine = gt[i] == 0 || (gt[i] >= kWideLeast && gt[i] <= kWideMost);
+        const int re = fine && gt[i] ? scale_exp(gt[i]) : 0;
+        // a row that gives nothing, and one that the split cannot hold, keep finite stand-ins
+        w[i] = gt[i] && fine ? rl[i] * pow2(re) : 0.0f;
+        delta[i] = fine ? dot * pow2(-re) : 0.0f;
+        bad = bad || !fine || (on && !(__builtin_fabsf(m[i]) < 1e30f && rl[i] > 0.0f && rl[i] < 1e30f && __builtin_fabsf(dot) < 1e38f));
+        if (!on) m[i] = kNoRow;
+        if ((threadIdx.x & 15) == 0) {
+            const int64_t r = at * kBlock + 4 * (threadIdx.x >> 4) + i;
+            o.v.m[r] = m[i];
+            o.v.delta[r] = delta[i];
+            o.v.w[r] = w[i];
+        }
+    }
+    RowStats st = {};
+    uint32_t top, low;
+    // q, one scale
+    block_top(qt, top, low, sh);
+    const bool qok = in_range(top);
+    bad = bad || !qok;
+    const int eq = qok && top ? scale_exp(top) : 0;
+    st.q = pow2(eq);
+    Share<DP> x;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+#pragma unroll
+        for (int n = 0; n < NCH; n++) x.x[i][n] = s.x[i][n] * pow2(-eq);
+    }
+    put_block<DP, false>(x, o.q + at * plane_bytes(DP, 1), lds);
+    // g, a scale for each row
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const bool fine = gt[i] >= kWideLeast && gt[i] <= kWideMost;
+        const float sc = fine ? pow2(-scale_exp(gt[i])) : 0.0f;
+#pragma unroll
+        for (int n = 0; n < NCH; n++) x.x[i][n] = g.x[i][n] * sc;
+    }
+    put_block<DP, false>(x, o.g + at * plane_bytes(DP, 1), lds);
+    // g / l and q w, one scale each
+    uint32_t t4[4];
+    auto cols = [&](Share<DP> &y, const float (&f)[4], char *out, float &scale, uint32_t &kept) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            y.scale(i, f[i]);
+            t4[i] = y.row_top(i);
+        }
+        block_top(t4, top, low, sh);
+        const bool ok = top == 0 || (top >= kWideLeast && top <= kWideMost && even_rows(top, low));
+        bad = bad || !ok;
+        const int e = ok && top ? scale_exp(top) : 0;
+        scale = pow2(e);
+        kept = top;
+#pragma unroll
+        for (int i = 0; i < 4; i++) y.scale(i, pow2(-e));
+        put_block<DP, true>(y, out + at * plane_bytes(DP, 1), lds);
+    };
+    cols(g, rl, o.g2, st.g2, st.g2_top);
+    cols(s, w, o.q2, st.q2, st.q2_top);
+    bad = __syncthreads_or(bad);
+    if ((threadIdx.x & 15) == 0) {
+        sh[threadIdx.x >> 4] = (uint32_t)dlo;
+        sh[16 + (threadIdx.x >> 4)] = (uint32_t)dhi;
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 16; i++) {
+            dlo = min(dlo, (int)sh[i]);
+            dhi = max(dhi, (int)sh[16 + i]);
+        }
+        st.bad = bad;
         st.doc_lo = dlo;
         st.doc_hi = dhi;
         o.stats[at] = st;
