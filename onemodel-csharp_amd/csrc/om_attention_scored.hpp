@@ -56,6 +56,36 @@ __device__ __forceinline__ bool in_reach(const Rule &u, int gap, int j, int pre)
     if (u.causal && gap < 0) return false;
     return u.window == 0 || (gap < u.window && gap > -u.window);
 }
+// The rule for one query as an interval of keys and a prefix, so that a score's test is two or three integer operations
+// without a branch: key j is seen when j - lo < n (unsigned) or j < pre, documents aside. Nothing for a padded query.
+struct Reach {
+    int lo;
+    uint32_t n;
+    int pre;
+    __device__ __forceinline__ bool has(int j) const { return ((uint32_t)(j - lo) < n) | (j < pre); }
+};
+__device__ __forceinline__ Reach keys_seen(const Rule &u, int pos, int doc, int pre) {
+    int lo = 0, hi = u.lk - 1;
+    if (u.causal) hi = min(hi, pos);
+    if (u.window) {
+        lo = max(lo, pos - u.window + 1);
+        hi = min(hi, pos + u.window - 1);
+    }
+    const bool on = doc >= 0;
+    return Reach{lo, on && hi >= lo ? (uint32_t)(hi - lo + 1) : 0u, on ? min(pre, u.lk) : 0};
+}
+// The same for one key: the positions that see it.
+__device__ __forceinline__ Reach rows_seeing(const Rule &u, int j, int doc, int pre) {
+    int lo = u.off, hi = u.lk - 1;
+    if (j >= pre) {
+        if (u.causal) lo = max(lo, j);
+        if (u.window) {
+            lo = max(lo, j - u.window + 1);
+            hi = min(hi, j + u.window - 1);
+        }
+    }
+    return Reach{lo, doc >= 0 && hi >= lo ? (uint32_t)(hi - lo + 1) : 0u, INT32_MIN};
+}
 // The hull [lo, hi] of the keys that queries at positions i0 .. i1 can see.
 __device__ __forceinline__ void key_range(const Rule &u, int i0, int i1, int pre, int &lo, int &hi) {
     lo = 0;

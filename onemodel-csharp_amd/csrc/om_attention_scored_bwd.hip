@@ -39,7 +39,7 @@ template <int DP, bool VEC>
 __global__ void __launch_bounds__(256) k_scored_split_bwd(Rule u, Ptrs p, SplitOut ko, SplitOut vo, RowsOut ro, int nt, int nr) {
     OM_LDS_POISON();
     __shared__ __attribute__((aligned(16))) char lds[DP * 256];
-    __shared__ uint32_t sh[32];
+    __shared__ uint32_t sh[48];
     const int keys = u.B * u.Hk * nt;
     int i = blockIdx.x;
     if (i < 2 * keys) {
@@ -226,16 +226,38 @@ __device__ __forceinline__ bool all_see(const Rule &u, int i0, int i1, int j0, i
 // The step data of a block of rows: its scales and whether it is visited.
 struct RowStep {
     float q, g2, q2;
-    int see;
+    int see, dlo, dhi;
+};
+// Either role's tables in LDS, by blocks of the other side: scales, whether the block is visited, its documents; and the
+// step's rows' m, delta, position and slope (or the step's keys' documents).
+struct KeysTables {
+    float rv[2][4][kStep];
+    int doc[2][kStep];
+    float q[kListed], g2[kListed], q2[kListed];
+    int lo[kListed], hi[kListed];
+    uint32_t red[4][5];
+    unsigned char see[kListed];
+};
+struct RowsTables {
+    int doc[2][kStep];
+    float k[kListed], v[kListed];
+    int lo[kListed], hi[kListed];
+    uint32_t red[4][3];
+    signed char step[kListed];
+    unsigned char see[kListed];
 };
 template <int DP>
-__device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const BwdArgs &a, int i, char *sh) {
+__device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const BwdArgs &a, int i, char *sh, KeysTables &t_) {
     constexpr int S = DP / 16, ND = DP / 32, HALF = kStep * DP * 4, STAGE = 4 * HALF;
-    __shared__ float lq_[kListed], lg2[kListed], lq2[kListed];
-    __shared__ unsigned char lsee[kListed];
-    __shared__ __attribute__((aligned(16))) float rv[2][4][kStep];  // m, delta, position, slope of the step's rows
-    __shared__ int rdoc[2][kStep];
-    __shared__ uint32_t red[4][4];
+    auto &lq_ = t_.q;
+    auto &lg2 = t_.g2;
+    auto &lq2 = t_.q2;
+    auto &lsee = t_.see;
+    auto &llo = t_.lo;
+    auto &lhi = t_.hi;
+    auto &rv = t_.rv;
+    auto &rdoc = t_.doc;
+    auto &red = t_.red;
     const int kb = i % a.kblocks, split = (i / a.kblocks) % a.nsplit, item = i / (a.kblocks * a.nsplit);
     const int b = item / u.Hk, hk = item - b * u.Hk, rows = u.G * u.lq;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
@@ -254,6 +276,15 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
     const float vref = fmaxf(v0.top ? v0.scale : 0.0f, v1.top ? v1.scale : 0.0f) > 0.0f
                            ? fmaxf(v0.top ? v0.scale : 0.0f, v1.top ? v1.scale : 0.0f) : 1.0f;
     const int kdlo = min(k0.doc_lo, k1.doc_lo), kdhi = max(k0.doc_hi, k1.doc_hi);
+    // documents of the wavefront's own keys (those past the last one aside)
+    int wlo = j <= last ? kd : INT32_MAX, whi = j <= last ? kd : INT32_MIN;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        wlo = min(wlo, __shfl_xor(wlo, o, 64));
+        whi = max(whi, __shfl_xor(whi, o, 64));
+    }
+    wlo = __builtin_amdgcn_readfirstlane(wlo);
+    whi = __builtin_amdgcn_readfirstlane(whi);
     // the blocks of rows that may see them
     int plo, phi;
     pos_range(u, first, last, pre, plo, phi);
@@ -269,10 +300,9 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
         st.q2 = r.q2;
         const int f = rt * kBlock, l = min(f + kBlock, rows) - 1;
         st.see = may_see(u, f / u.G + u.off, l / u.G + u.off, first, last, pre);
-        if (u.qd) {
-            if (r.doc_hi < kdlo || r.doc_lo > kdhi || r.doc_hi < 0) st.see = 0;
-            if (r.doc_lo != r.doc_hi || kdlo != kdhi || r.doc_lo != kdlo || kdlo < 0) st.see |= 2;
-        }
+        st.dlo = r.doc_lo;
+        st.dhi = r.doc_hi;
+        if (u.qd && (r.doc_hi < kdlo || r.doc_lo > kdhi || r.doc_hi < 0)) st.see = 0;
         if (r.g2_top == 0 && r.q2_top == 0) st.see = 0;  // rows without gradient
         return r;
     };
@@ -289,6 +319,8 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
             lg2[rt - t0] = st.g2;
             lq2[rt - t0] = st.q2;
             lsee[rt - t0] = (unsigned char)st.see;
+            llo[rt - t0] = st.dlo;
+            lhi[rt - t0] = st.dhi;
         }
     }
 #pragma unroll
@@ -298,19 +330,22 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
         gl = min(gl, (uint32_t)__shfl_xor((int)gl, o, 64));
         ql = min(ql, (uint32_t)__shfl_xor((int)ql, o, 64));
     }
+    const uint32_t wave_bad = __any(bad) ? 1 : 0;
     if (lane == 0) {
         red[w][0] = gt;
         red[w][1] = qt;
         red[w][2] = gl;
         red[w][3] = ql;
+        red[w][4] = wave_bad;
     }
-    bad = __syncthreads_or(bad);
+    __syncthreads();
 #pragma unroll
     for (int n = 0; n < 4; n++) {
         gt = max(gt, red[n][0]);
         qt = max(qt, red[n][1]);
         gl = min(gl, red[n][2]);
         ql = min(ql, red[n][3]);
+        bad = bad || red[n][4];
     }
     // the accumulators move between the blocks' scales: keep the largest move inside fp32
     bad = bad || (gt && (gt >> 23) - (gl >> 23) > 60) || (qt && (qt >> 23) - (ql >> 23) > 60);
@@ -339,6 +374,7 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
             vm[s] = *reinterpret_cast<const u32x4 *>(vf + (2 * s + 1) * 1024);
         }
     }
+    const Reach reach = rows_seeing(u, j, kd, pre);
     floatx16 dk[ND], dv[ND];
 #pragma unroll
     for (int n = 0; n < ND; n++)
@@ -353,7 +389,7 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
             const int f = t0 * kBlock + it * kStep;
             if (f >= r1) return steps;
             if (f + kStep <= r0) continue;
-            if ((it >> 1) >= kListed || (lsee[it >> 1] & 1)) return it;
+            if ((it >> 1) >= kListed || lsee[it >> 1]) return it;
         }
         return steps;
     };
@@ -407,14 +443,15 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
             st.q = lq_[it >> 1];
             st.g2 = lg2[it >> 1];
             st.q2 = lq2[it >> 1];
-            st.see = lsee[it >> 1];
+            st.dlo = __builtin_amdgcn_readfirstlane(llo[it >> 1]);
+            st.dhi = __builtin_amdgcn_readfirstlane(lhi[it >> 1]);
         } else {
             looked(t0 + (it >> 1), st);
         }
         const int f0 = t0 * kBlock + it * kStep, f1 = min(f0 + kStep, rows) - 1;
         const int i0 = f0 / u.G + u.off, i1 = f1 / u.G + u.off;
         const int j0 = first + 32 * w, j1 = min(j0 + 31, last);
-        if (live && may_see(u, i0, i1, j0, j1, pre)) {
+        if (live && !(u.qd && (whi < 0 || st.dhi < wlo || st.dlo > whi)) && may_see(u, i0, i1, j0, j1, pre)) {
             if (st.g2 != g2cur) {
                 const float c = g2cur / st.g2;
 #pragma unroll
@@ -439,7 +476,8 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
                           *reinterpret_cast<const u32x4 *>(gf + (2 * s + 1) * 1024), vh[s], vm[s], dp);
             }
             const float cs = st.q * ks.scale;
-            const bool whole = !(st.see & 2) && all_see(u, i0, i1, j0, j1, pre);
+            const bool one = !u.qd || (wlo == whi && st.dlo == st.dhi && st.dlo == wlo && wlo >= 0);
+            const bool whole = one && all_see(u, i0, i1, j0, j1, pre);
             if (u.icap != 0.0f) {
                 const float ic = u.icap * cs;
                 float big = 0.0f;
@@ -466,25 +504,17 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
 #pragma unroll
                 for (int r = 0; r < 4; r++) y[r] = __builtin_fmaf(x[4 * q + r], fx, (float)kLift - m4[r]);
                 if (u.slopes || !whole) {
-                    const floatx4 p4 = *reinterpret_cast<const floatx4 *>(&rv[buf][2][8 * q + 4 * g]);
+                    const intx4 p4 = *reinterpret_cast<const intx4 *>(&rv[buf][2][8 * q + 4 * g]);
                     if (u.slopes) {
                         const floatx4 s4 = *reinterpret_cast<const floatx4 *>(&rv[buf][3][8 * q + 4 * g]);
 #pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            const int gap = __float_as_int(p4[r]) - j;
-                            y[r] = __builtin_fmaf(-s4[r], __builtin_fabsf((float)gap), y[r]);
-                        }
+                        for (int r = 0; r < 4; r++) y[r] = __builtin_fmaf(-s4[r], __builtin_fabsf((float)(p4[r] - j)), y[r]);
                     }
                     if (!whole) {
+                        intx4 qd = {kd, kd, kd, kd};
+                        if (!one) qd = *reinterpret_cast<const intx4 *>(&rdoc[buf][8 * q + 4 * g]);
 #pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            bool ok = in_reach(u, __float_as_int(p4[r]) - j, j, pre);
-                            if (st.see & 2) {
-                                const int qd = rdoc[buf][8 * q + 4 * g + r];
-                                ok = ok && qd >= 0 && qd == kd;
-                            }
-                            y[r] = ok ? y[r] : -3e38f;
-                        }
+                        for (int r = 0; r < 4; r++) y[r] = reach.has(p4[r]) & (qd[r] == kd) ? y[r] : -3e38f;
                     }
                 }
 #pragma unroll
@@ -551,12 +581,16 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
 
 // ------------------------------------------------------------------------------------------------------------ dq
 template <int DP>
-__device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const BwdArgs &a, int i, char *sh) {
+__device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const BwdArgs &a, int i, char *sh, RowsTables &t_) {
     constexpr int S = DP / 16, ND = DP / 32, HALF = kStep * DP * 4, STAGE = 3 * HALF;
-    __shared__ float lk_[kListed], lv_[kListed];
-    __shared__ signed char lstep[kListed];
-    __shared__ unsigned char lsee[kListed];
-    __shared__ uint32_t red[4][6];
+    auto &lk_ = t_.k;
+    auto &lv_ = t_.v;
+    auto &lstep = t_.step;
+    auto &lsee = t_.see;
+    auto &llo = t_.lo;
+    auto &lhi = t_.hi;
+    auto &kdoc = t_.doc;
+    auto &red = t_.red;
     const int rb = a.rblocks - 1 - i % a.rblocks, item = i / a.rblocks;  // the longest rows of a causal rule first
     const int b = item / u.Hk, hk = item - b * u.Hk, rows = u.G * u.lq;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
@@ -608,24 +642,32 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
         return;
     }
     const int ek = kt ? scale_exp(kt) : 0, ev = vt ? scale_exp(vt) : 0;
-    const bool some_padded = qlo < 0;
-    auto looked = [&](int t, float &sk, float &sv, int &step) -> int {
+    int wlo = doc, whi = doc;  // documents of the wavefront's rows
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        wlo = min(wlo, __shfl_xor(wlo, o, 64));
+        whi = max(whi, __shfl_xor(whi, o, 64));
+    }
+    wlo = __builtin_amdgcn_readfirstlane(wlo);
+    whi = __builtin_amdgcn_readfirstlane(whi);
+    auto looked = [&](int t, float &sk, float &sv, int &step, int &dlo, int &dhi) -> int {
         const Stats ks = a.ks[kt0 + t], vs = a.vs[kt0 + t];
         sk = ks.scale;
         sv = vs.top ? vs.scale * pow2(-ev) : 1.0f;
         step = ks.top ? ((int)(__float_as_uint(ks.scale) >> 23) - 127 - ek) / 4 : 0;
         const int j0 = t * kBlock, j1 = j0 + kBlock - 1;
         int see = may_see(u, i0, i1, j0, j1, pre);
-        if (u.qd) {
-            if (ks.doc_hi < 0 || ks.doc_hi < qlo || ks.doc_lo > qhi) see = 0;
-            if (some_padded || ks.doc_lo < 0 || ks.doc_lo != ks.doc_hi || qlo != qhi || ks.doc_lo != qlo) see |= 2;
-        }
+        dlo = ks.doc_lo;
+        dhi = ks.doc_hi;
+        if (u.qd && (dhi < 0 || dhi < qlo || dlo > qhi)) see = 0;
         return see;
     };
     for (int t = t0 + (int)threadIdx.x; t <= t1 && t < t0 + kListed; t += 256) {
         float sk, sv;
-        int step;
-        const int see = looked(t, sk, sv, step);
+        int step, dlo, dhi;
+        const int see = looked(t, sk, sv, step, dlo, dhi);
+        llo[t - t0] = dlo;
+        lhi[t - t0] = dhi;
         lk_[t - t0] = sk;
         lv_[t - t0] = sv;
         lstep[t - t0] = (signed char)step;
@@ -648,6 +690,7 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
     }
     const int64_t at = rt0 * kBlock + min(rr, a.nr * kBlock - 1);
     const float m = a.v.m[at], delta = a.v.delta[at] * pow2(-ev), wr = a.v.w[at];
+    const Reach reach = keys_seen(u, pos, doc, pre);
     floatx16 dq[ND];
     int sd = kNoScale;  // dq's sums are in units of 2^sd
 #pragma unroll
@@ -659,7 +702,7 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
     auto next = [&](int it) {
         for (it++; it < steps; it++) {
             if (t0 * kBlock + it * kStep > hi) return steps;
-            if ((it >> 1) >= kListed || (lsee[it >> 1] & 1)) return it;
+            if ((it >> 1) >= kListed || lsee[it >> 1]) return it;
         }
         return steps;
     };
@@ -676,25 +719,37 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
         one(a.vn, 1);
         one(a.kt, 2);
     };
+    auto key_doc = [&](int it) -> int {  // of the step's key threadIdx.x
+        const int j = t0 * kBlock + it * kStep + (int)threadIdx.x;
+        return u.kd && threadIdx.x < kStep && j < u.lk ? u.kd[(int64_t)b * u.lk + j] : -1;
+    };
     int it = next(-1), buf = 0;
-    if (it < steps) stage(it, 0);
+    if (it < steps) {
+        stage(it, 0);
+        if (u.kd && threadIdx.x < kStep) kdoc[0][threadIdx.x] = key_doc(it);
+    }
     while (it < steps) {
         wait_loads();
         __syncthreads();
         const int nx = next(it);
-        if (nx < steps) stage(nx, buf ^ 1);
+        int nd = -1;
+        if (nx < steps) {
+            stage(nx, buf ^ 1);
+            nd = key_doc(nx);
+        }
         float sk, sv;
-        int step, see;
+        int step, dlo, dhi;
         if ((it >> 1) < kListed) {
             sk = lk_[it >> 1];
             sv = lv_[it >> 1];
             step = lstep[it >> 1];
-            see = lsee[it >> 1];
+            dlo = __builtin_amdgcn_readfirstlane(llo[it >> 1]);
+            dhi = __builtin_amdgcn_readfirstlane(lhi[it >> 1]);
         } else {
-            see = looked(t0 + (it >> 1), sk, sv, step);
+            looked(t0 + (it >> 1), sk, sv, step, dlo, dhi);
         }
         const int j0 = t0 * kBlock + it * kStep, j1 = j0 + kStep - 1;
-        if (live && may_see(u, wi0, wi1, j0, j1, pre)) {
+        if (live && !(u.qd && (whi < 0 || dhi < wlo || dlo > whi)) && may_see(u, wi0, wi1, j0, j1, pre)) {
             const char *kf = sh + 256 + buf * STAGE + lane * 16, *vf = kf + HALF, *ktf = vf + HALF;
             floatx16 x, dp;
 #pragma unroll
@@ -707,7 +762,8 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
                           *reinterpret_cast<const u32x4 *>(vf + (2 * s + 1) * 1024), gh[s], gm[s], dp);
             }
             const float cs = rs.q * sk;
-            const bool whole = j1 < u.lk && !(see & 2) && all_see(u, wi0, wi1, j0, j1, pre);
+            const bool one = !u.qd || (wlo == whi && dlo == dhi && dlo == wlo && dlo >= 0);
+            const bool whole = j1 < u.lk && one && all_see(u, wi0, wi1, j0, j1, pre);
             if (u.icap != 0.0f) {
                 const float ic = u.icap * cs;
                 float big = 0.0f;
@@ -732,12 +788,7 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
                 float y = __builtin_fmaf(x[e], fx, mu);
                 const int o = 8 * (e >> 2) + (e & 3);
                 if (u.slopes) y = __builtin_fmaf(-slope, __builtin_fabsf(gap0 - (float)o), y);
-                if (!whole) {
-                    const int jj = j0 + 4 * g + o;
-                    bool ok = jj < u.lk && in_reach(u, pos - jj, jj, pre);
-                    if (see & 2) ok = ok && doc >= 0 && u.kd[(int64_t)b * u.lk + min(jj, u.lk - 1)] == doc;
-                    y = ok ? y : -3e38f;
-                }
+                if (!whole) y = reach.has(j0 + 4 * g + o) & (one || kdoc[buf][4 * g + o] == doc) ? y : -3e38f;
                 float ds = exp2_hw(y) * __builtin_fmaf(dp[e], sv, -delta);
                 if (u.icap != 0.0f) ds *= __builtin_fmaf(-x[e], x[e], 1.0f);
                 dp[e] = ds;
@@ -768,6 +819,7 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
                 }
             }
         }
+        if (u.kd && nx < steps && threadIdx.x < kStep) kdoc[buf ^ 1][threadIdx.x] = nd;
         it = nx;
         buf ^= 1;
     }
@@ -788,16 +840,20 @@ template <int DP>
 __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) k_scored_bwd_mm(Rule u, Ptrs p, BwdArgs a) {
     OM_LDS_POISON();
     __shared__ __attribute__((aligned(16))) char sh[256 + 2 * 4 * kStep * DP * 4];  // no stage at LDS address 0
+    __shared__ __attribute__((aligned(16))) union {
+        KeysTables k;
+        RowsTables r;
+    } t;
     int lin = blockIdx.x;
     // ids are dealt round-robin over the 8 XCDs: the workgroups of one head stay on one
     if (lin < a.first_rows) {
         if ((a.first_rows & 7) == 0) lin = (lin & 7) * (a.first_rows >> 3) + (lin >> 3);
-        keys_role<DP>(u, p, a, lin, sh);
+        keys_role<DP>(u, p, a, lin, sh, t.k);
     } else {
         const int total = gridDim.x - a.first_rows;
         lin -= a.first_rows;
         if ((total & 7) == 0) lin = (lin & 7) * (total >> 3) + (lin >> 3);
-        rows_role<DP>(u, p, a, lin, sh);
+        rows_role<DP>(u, p, a, lin, sh, t.r);
     }
 }
 

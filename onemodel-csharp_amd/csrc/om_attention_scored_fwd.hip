@@ -15,13 +15,13 @@ constexpr float kInf = __builtin_inff();
 constexpr int kRows = 128;      // rows of a workgroup
 constexpr float kLift = 12.0f;  // weights are kept as 2^kLift times themselves, so that their split's m is normal fp16
 constexpr float kSlack = 2.0f;  // how far a maximum may outgrow m before m moves
-constexpr int kListed = 1024;   // blocks of keys whose step data stands in LDS
+constexpr int kListed = 512;    // blocks of keys whose step data stands in LDS
 
 template <int DP, bool VEC>
 __global__ void __launch_bounds__(256) k_scored_split_kv(Rule u, Ptrs p, SplitOut ko, SplitOut vo, int nt) {
     OM_LDS_POISON();
     __shared__ __attribute__((aligned(16))) char lds[DP * 256];
-    __shared__ uint32_t sh[32];
+    __shared__ uint32_t sh[48];
     const int items = u.B * u.Hk * nt;
     const int which = blockIdx.x / items, at = blockIdx.x - which * items;
     const int t = at % nt, bh = at / nt;
@@ -128,8 +128,10 @@ __global__ void __launch_bounds__(256, 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArg
     __shared__ __attribute__((aligned(16))) char sh[256 + 2 * STAGE];  // no stage at LDS address 0
     __shared__ float kscale[kListed];
     __shared__ signed char vstep[kListed];  // exponent of V's scale less the largest, in steps of 4
-    __shared__ unsigned char visit[kListed];  // bit 0: some row may see the block, bit 1: documents need a look
-    __shared__ uint32_t red[4][5];
+    __shared__ unsigned char visit[kListed];  // whether some row may see the block
+    __shared__ int docs_lo[kListed], docs_hi[kListed];
+    __shared__ __attribute__((aligned(16))) int kdoc[2][KT];  // documents of the step's keys
+    __shared__ uint32_t red[4][6];
     int rb, item;
     on_one_xcd(a.blocks * a.nsplit, rb, item);
     const int split = rb % a.nsplit;
@@ -205,15 +207,19 @@ __global__ void __launch_bounds__(256, 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArg
         qlo = min(qlo, __shfl_xor(qlo, o, 64));
         qhi = max(qhi, __shfl_xor(qhi, o, 64));
     }
+    const uint32_t wave_bad = __any(bad) ? 1 : 0;
     if (lane == 0) {
         red[w][0] = ktop;
         red[w][1] = vtop;
         red[w][2] = vlow;
         red[w][3] = (uint32_t)qlo;
         red[w][4] = (uint32_t)qhi;
+        red[w][5] = wave_bad;
     }
-    bad = __syncthreads_or(bad);
-    const bool some_padded = __syncthreads_or(doc < 0);  // such a row sees nothing, whatever the others see
+    // documents of the wavefront's rows; a padded row sees nothing, whatever the others see
+    const int wqlo = __builtin_amdgcn_readfirstlane(qlo), wqhi = __builtin_amdgcn_readfirstlane(qhi);
+    const bool one_doc = wqlo == wqhi && !__any(doc < 0);
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         ktop = max(ktop, red[i][0]);
@@ -221,6 +227,7 @@ __global__ void __launch_bounds__(256, 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArg
         vlow = min(vlow, red[i][2]);
         qlo = min(qlo, (int)red[i][3]);
         qhi = max(qhi, (int)red[i][4]);
+        bad = bad || red[i][5];
     }
     bad = bad || ktop > kMostBits || vtop > kMostBits || !even_rows(vtop, vlow);
     if (__builtin_amdgcn_readfirstlane(bad)) {
@@ -229,24 +236,25 @@ __global__ void __launch_bounds__(256, 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArg
         return;
     }
     const int ev = vtop ? scale_exp(vtop) : 0;
-    auto looked = [&](int t, float &sc, int &step) -> int {
+    auto looked = [&](int t, float &sc, int &step, int &dlo, int &dhi) -> int {
         const Stats ks = a.ks[kt0 + t];
         sc = ks.scale;
+        dlo = ks.doc_lo;
+        dhi = ks.doc_hi;
         step = ((int)(__float_as_uint(a.vs[kt0 + t].scale) >> 23) - 127 - ev) / 4;
         if (a.vs[kt0 + t].top == 0) step = 0;  // a block of zeros
         const int j0 = t * kBlock, j1 = j0 + kBlock - 1;
         int see = 1;
         if (j0 >= pre) see = !(u.causal && j0 > i1) && !(u.window && (i0 - j1 >= u.window || j0 - i1 >= u.window));
-        if (u.qd) {
-            if (ks.doc_hi < qlo || ks.doc_lo > qhi) see = 0;
-            if (some_padded || ks.doc_lo < 0 || ks.doc_lo != ks.doc_hi || qlo != qhi || ks.doc_lo != qlo) see |= 2;
-        }
+        if (u.qd && (dhi < qlo || dlo > qhi)) see = 0;
         return see;
     };
     for (int t = t0 + (int)threadIdx.x; t <= t1 && t < t0 + kListed; t += 256) {
         float sc;
-        int step;
-        const int see = looked(t, sc, step);
+        int step, dlo, dhi;
+        const int see = looked(t, sc, step, dlo, dhi);
+        docs_lo[t - t0] = dlo;
+        docs_hi[t - t0] = dhi;
         kscale[t - t0] = sc;
         vstep[t - t0] = (signed char)step;
         visit[t - t0] = (unsigned char)see;
@@ -258,7 +266,7 @@ __global__ void __launch_bounds__(256, 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArg
         for (it++; it < steps; it++) {
             const int t = it * KT / kBlock;
             if (t0 * kBlock + it * KT > hi) return steps;
-            if (t >= kListed || (visit[t] & 1)) return it;
+            if (t >= kListed || visit[t]) return it;
         }
         return steps;
     };
@@ -274,6 +282,7 @@ __global__ void __launch_bounds__(256, 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArg
         for (int i = 0; i < PER; i++) load_to_lds(va + (4 * i + w) * 1024, to + HALF + (uint32_t)(4 * i + w) * 1024u);
     };
 
+    const Reach reach = keys_seen(u, pos, doc, pre);
     floatx16 acc[ND];
 #pragma unroll
     for (int n = 0; n < ND; n++)
@@ -284,27 +293,40 @@ __global__ void __launch_bounds__(256, 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArg
     const bool live = first + 32 * w <= last;
     const float cq = __builtin_fabsf(u.cl2) * pow2(eq), icq = __builtin_fabsf(u.icap) * pow2(eq);
 
+    auto key_doc = [&](int it) -> int {  // of the step's key threadIdx.x
+        const int j = t0 * kBlock + it * KT + (int)threadIdx.x;
+        return u.kd && threadIdx.x < KT && j < u.lk ? u.kd[(int64_t)b * u.lk + j] : -1;
+    };
     int it = next(-1), buf = 0;
-    if (it < steps) stage(it, 0);
+    if (it < steps) {
+        stage(it, 0);
+        if (u.kd && threadIdx.x < KT) kdoc[0][threadIdx.x] = key_doc(it);
+    }
     while (it < steps) {
         wait_loads();
         __syncthreads();  // this step has landed, and every wavefront is done with the other stage
         const int nx = next(it);
-        if (nx < steps) stage(nx, buf ^ 1);
+        int nd = -1;
+        if (nx < steps) {
+            stage(nx, buf ^ 1);
+            nd = key_doc(nx);
+        }
         const int j0 = t0 * kBlock + it * KT, j1 = j0 + KT - 1, ti = it * KT / kBlock;
         float ksc;
-        int vst, see;
+        int vst, dlo, dhi;
         if (ti < kListed) {
             ksc = kscale[ti];
             vst = vstep[ti];
-            see = visit[ti];
+            dlo = __builtin_amdgcn_readfirstlane(docs_lo[ti]);
+            dhi = __builtin_amdgcn_readfirstlane(docs_hi[ti]);
         } else {
-            see = looked(t0 + ti, ksc, vst);
+            looked(t0 + ti, ksc, vst, dlo, dhi);
         }
         // what the wavefront's 32 rows see of the step
-        const bool none = !live || (j0 >= pre && ((u.causal && j0 > wi1) ||
+        const bool none = !live || (u.qd && (dhi < wqlo || dlo > wqhi)) || (j0 >= pre && ((u.causal && j0 > wi1) ||
                                                   (u.window && (wi0 - j1 >= u.window || j0 - wi1 >= u.window))));
-        const bool whole = j1 < u.lk && !(see & 2) &&
+        const bool one = !u.qd || (one_doc && dlo == dhi && dlo == wqlo && dlo >= 0);
+        const bool whole = j1 < u.lk && one &&
                            (j1 < pre || ((!u.causal || j1 <= wi0) && (!u.window || (wi1 - j0 < u.window && j1 - wi0 < u.window))));
         if (!none) {
             const char *kf = sh + 256 + buf * STAGE + lane * 16, *vf = kf + HALF;
@@ -354,15 +376,18 @@ __global__ void __launch_bounds__(256, 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArg
                 f = 1.0f;
             }
             if (!whole) {
-                const int j = j0 + 4 * g;
 #pragma unroll
                 for (int n = 0; n < NB; n++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const int jj = j + 32 * n + 8 * (e >> 2) + (e & 3);
-                        bool ok = jj < u.lk && in_reach(u, pos - jj, jj, pre);
-                        if (see & 2) ok = ok && doc >= 0 && u.kd[(int64_t)b * u.lk + min(jj, u.lk - 1)] == doc;
-                        x[n][e] = ok ? x[n][e] : -kInf;
+                    for (int q = 0; q < 4; q++) {
+                        const int k0 = 32 * n + 8 * q + 4 * g;
+                        intx4 kd = {doc, doc, doc, doc};
+                        if (!one) kd = *reinterpret_cast<const intx4 *>(&kdoc[buf][k0]);
+#pragma unroll
+                        for (int r = 0; r < 4; r++) {
+                            const bool ok = reach.has(j0 + k0 + r) & (kd[r] == doc);
+                            x[n][4 * q + r] = ok ? x[n][4 * q + r] : -kInf;
+                        }
                     }
             }
             float top = -kInf;
@@ -405,6 +430,7 @@ __global__ void __launch_bounds__(256, 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArg
                     }
                 }
         }
+        if (u.kd && nx < steps && threadIdx.x < KT) kdoc[buf ^ 1][threadIdx.x] = nd;
         it = nx;
         buf ^= 1;
     }

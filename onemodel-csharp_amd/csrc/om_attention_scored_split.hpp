@@ -46,7 +46,7 @@ struct Share {
     }
 };
 
-// The block's top and low from its rows' maxima; every thread gets both. Uses 32 words of LDS.
+// The block's top and low from its rows' maxima; every thread gets both. Uses 32 words of `sh`.
 __device__ __forceinline__ void block_top(const uint32_t (&row)[4], uint32_t &top, uint32_t &low, uint32_t *sh) {
     uint32_t t = 0, l = 0xFFFFFFFFu;
 #pragma unroll
@@ -269,18 +269,20 @@ __device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, 
     };
     cols(g, rl, o.g2, st.g2, st.g2_top);
     cols(s, w, o.q2, st.q2, st.q2_top);
-    bad = __syncthreads_or(bad);
+    __syncthreads();
+    const bool wave_bad = __any(bad);
     if ((threadIdx.x & 15) == 0) {
         sh[threadIdx.x >> 4] = (uint32_t)dlo;
         sh[16 + (threadIdx.x >> 4)] = (uint32_t)dhi;
+        sh[32 + (threadIdx.x >> 4)] = wave_bad;
     }
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int i = 0; i < 16; i++) {
             dlo = min(dlo, (int)sh[i]);
             dhi = max(dhi, (int)sh[16 + i]);
+            st.bad |= sh[32 + i];
         }
-        st.bad = bad;
         st.doc_lo = dlo;
         st.doc_hi = dhi;
         o.stats[at] = st;
