@@ -171,50 +171,60 @@ __global__ void __launch_bounds__(256) k_scored_fwd_rows(Rule u, Ptrs p, int blo
     fwd_rows<NC, R, VEC>(u, p, i / u.Hk, i % u.Hk, rb * R, split, nsplit, per, part);
 }
 
-// Joins the splits: o = sum_s 2^(m_s - m) a_s / sum_s 2^(m_s - m) l_s, in split order. A wavefront per row: its lanes hold
-// a split's weight each, then a value each of the row, so that a row's loads are independent of one another (a thread per
-// value, which waits for every split in turn, took 33 us for 96 rows of 32 splits; this takes 5).
+// Joins the splits: o = sum_s 2^(m_s - m) a_s / sum_s 2^(m_s - m) l_s, in split order; a thread per four values (or one,
+// where d is no multiple of four). The loads of kAtOnce splits are issued together: a loop that waits for every split in
+// turn took 33 us for 96 rows of 32 splits.
+constexpr int kAtOnce = 8;
+template <int W>
 __global__ void __launch_bounds__(256) k_scored_join(Rule u, Ptrs p, int nsplit, const float *__restrict__ part) {
     OM_LDS_POISON();
-    const int rows = u.G * u.lq, d = u.d, lane = threadIdx.x & 63;
-    const int64_t all = (int64_t)u.B * u.Hk * rows, at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (at >= all) return;
+    typedef float vec __attribute__((ext_vector_type(W), aligned(4)));
+    const int rows = u.G * u.lq, d = u.d, per = d / W;
+    const int64_t all = (int64_t)u.B * u.Hk * rows, f = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (f >= all * per) return;
+    const int64_t at = f / per;
+    const int c = (int)(f - at * per) * W;
     const float *ms = part + (int64_t)nsplit * all * d + at, *ls = ms + (int64_t)nsplit * all;
-    // a split without a visible key has l = 0 and stands at 0: its maximum must not count
-    float top = -kInf;
-    for (int s0 = 0; s0 < nsplit; s0 += 64) {
-        const int s = s0 + lane;
-        if (s < nsplit && ls[s * all] != 0.0f) top = fmaxf(top, ms[s * all]);
-    }
-    top = omd::wave_max(top);
-    const float mu = top == -kInf ? 0.0f : top;
-    float sum = 0.0f, a[4] = {0.f, 0.f, 0.f, 0.f};  // d up to 256: values lane, lane + 64, ...
-    for (int s0 = 0; s0 < nsplit; s0 += 64) {
-        const int n = min(64, nsplit - s0);
-        float w = 0.0f, l = 0.0f;
-        if (lane < n) {
-            l = ls[(s0 + lane) * all];
-            w = l != 0.0f ? exp2_hw(ms[(s0 + lane) * all] - mu) : 0.0f;
-        }
-        for (int s = 0; s < n; s++) {
-            const float ws = __shfl(w, s, 64), lw = __shfl(l, s, 64);
-            if (lw == 0.0f) continue;  // nothing was written to the split's sums that counts
-            sum = __builtin_fmaf(ws, lw, sum);
-            const float *from = part + ((int64_t)(s0 + s) * all + at) * d;
+    float mu = -kInf, sum = 0.0f;  // of the splits so far
+    vec a;
 #pragma unroll
-            for (int c = 0; c < 4; c++)
-                if (lane + 64 * c < d) a[c] = __builtin_fmaf(ws, from[lane + 64 * c], a[c]);
+    for (int e = 0; e < W; e++) a[e] = 0.0f;
+    for (int s0 = 0; s0 < nsplit; s0 += kAtOnce) {
+        float m[kAtOnce], l[kAtOnce];
+        vec x[kAtOnce];
+#pragma unroll
+        for (int i = 0; i < kAtOnce; i++) {
+            const int64_t s = min(s0 + i, nsplit - 1);
+            m[i] = ms[s * all];
+            l[i] = s0 + i < nsplit ? ls[s * all] : 0.0f;
+            x[i] = *reinterpret_cast<const vec *>(part + (s * all + at) * d + c);
+        }
+        // a split without a visible key has l = 0 and stands at 0: it must not count
+        float top = mu;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; i++) top = l[i] != 0.0f && m[i] > top ? m[i] : top;
+        const float old = top == -kInf ? 1.0f : exp2_hw(mu - top);
+        mu = top;
+        sum *= old;
+        a *= old;
+#pragma unroll
+        for (int i = 0; i < kAtOnce; i++) {
+            const float w = exp2_hw(m[i] - (top == -kInf ? 0.0f : top));
+            sum = l[i] != 0.0f ? __builtin_fmaf(w, l[i], sum) : sum;
+#pragma unroll
+            for (int e = 0; e < W; e++) a[e] = l[i] != 0.0f ? __builtin_fmaf(w, x[i][e], a[e]) : a[e];
         }
     }
+    if (mu == -kInf) mu = 0.0f;
     const int64_t bh = at / rows;
     const int b = (int)(bh / u.Hk);
     const Row row = row_of(u, (int)(bh % u.Hk), (int)(at - bh * rows));
     const float rl = sum == 0.0f ? 0.0f : 1.0f / sum;
-    float *to = p.out + ((int64_t)b * u.lq + row.t) * p.ldo + (int64_t)row.h * d;
+    vec o;
 #pragma unroll
-    for (int c = 0; c < 4; c++)
-        if (lane + 64 * c < d) to[lane + 64 * c] = sum == 0.0f ? 0.0f : a[c] * rl;
-    if (lane == 0 && p.stats) {
+    for (int e = 0; e < W; e++) o[e] = sum == 0.0f ? 0.0f : a[e] * rl;
+    *reinterpret_cast<vec *>(p.out + ((int64_t)b * u.lq + row.t) * p.ldo + (int64_t)row.h * d + c) = o;
+    if (c == 0 && p.stats) {
         const int64_t sr = stat_at(u, b, row);
         p.stats[sr] = mu;
         p.stats[all + sr] = rl;
@@ -422,8 +432,11 @@ void by_width(int d, bool vec, F f) {
 }
 
 void join(om_ctx *ctx, const Rule &u, const Ptrs &p, int nsplit, const float *part) {
-    const int64_t rows = (int64_t)u.B * u.Hk * u.G * u.lq;
-    hipLaunchKernelGGL(k_scored_join, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, ctx->stream, u, p, nsplit, part);
+    auto go = [&](auto kern, int w) {
+        const int64_t values = (int64_t)u.B * u.Hk * u.G * u.lq * (u.d / w);
+        hipLaunchKernelGGL(kern, dim3((unsigned)((values + 255) / 256)), dim3(256), 0, ctx->stream, u, p, nsplit, part);
+    };
+    u.d % 4 == 0 ? go(k_scored_join<4>, 4) : go(k_scored_join<1>, 1);
 }
 
 // The matrix kernels take 32 rows at a time.

@@ -19,13 +19,13 @@ using namespace osc;
 
 constexpr int kKeys = 128;   // keys (or rows) of a workgroup
 constexpr int kStep = 32;    // rows (or keys) of a step
-constexpr int kListed = 512; // blocks whose step data stands in LDS
+constexpr int kListed = 256; // blocks whose step data stands in LDS
 constexpr int kLift = 12;    // E is kept as 2^12 E for dv's operand
 
 struct BwdArgs {
     const char *kn, *kt, *vn;        // K in both forms, V in rows form
     const char *qn, *gn, *g2, *q2;   // RowsOut
-    RowVals v;
+    const float *v;
     const Stats *ks, *vs;
     const RowStats *rs;
     int nt, nr;                      // blocks of 64 keys and rows of a head
@@ -228,18 +228,14 @@ struct RowStep {
     float q, g2, q2;
     int see, dlo, dhi;
 };
-// Either role's tables in LDS, by blocks of the other side: scales, whether the block is visited, its documents; and the
-// step's rows' m, delta, position and slope (or the step's keys' documents).
+// Either role's tables in LDS, by blocks of the other side: scales, whether the block is visited, its documents.
 struct KeysTables {
-    float rv[2][4][kStep];
-    int doc[2][kStep];
     float q[kListed], g2[kListed], q2[kListed];
     int lo[kListed], hi[kListed];
     uint32_t red[4][5];
     unsigned char see[kListed];
 };
 struct RowsTables {
-    int doc[2][kStep];
     float k[kListed], v[kListed];
     int lo[kListed], hi[kListed];
     uint32_t red[4][3];
@@ -248,15 +244,13 @@ struct RowsTables {
 };
 template <int DP>
 __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const BwdArgs &a, int i, char *sh, KeysTables &t_) {
-    constexpr int S = DP / 16, ND = DP / 32, HALF = kStep * DP * 4, STAGE = 4 * HALF;
+    constexpr int S = DP / 16, ND = DP / 32, HALF = kStep * DP * 4, STAGE = 4 * HALF + 1024;  // the rows' record last
     auto &lq_ = t_.q;
     auto &lg2 = t_.g2;
     auto &lq2 = t_.q2;
     auto &lsee = t_.see;
     auto &llo = t_.lo;
     auto &lhi = t_.hi;
-    auto &rv = t_.rv;
-    auto &rdoc = t_.doc;
     auto &red = t_.red;
     const int kb = i % a.kblocks, split = (i / a.kblocks) % a.nsplit, item = i / (a.kblocks * a.nsplit);
     const int b = item / u.Hk, hk = item - b * u.Hk, rows = u.G * u.lq;
@@ -273,18 +267,13 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
     const int tb = min(first / kBlock + 1, a.nt - 1);
     const Stats v0 = a.vs[kt0 + first / kBlock], v1 = a.vs[kt0 + tb], k0 = a.ks[kt0 + first / kBlock], k1 = a.ks[kt0 + tb];
     bool bad = max(max(v0.top, v1.top), max(k0.top, k1.top)) > kMostBits;
-    const float vref = fmaxf(v0.top ? v0.scale : 0.0f, v1.top ? v1.scale : 0.0f) > 0.0f
-                           ? fmaxf(v0.top ? v0.scale : 0.0f, v1.top ? v1.scale : 0.0f) : 1.0f;
     const int kdlo = min(k0.doc_lo, k1.doc_lo), kdhi = max(k0.doc_hi, k1.doc_hi);
     // documents of the wavefront's own keys (those past the last one aside)
-    int wlo = j <= last ? kd : INT32_MAX, whi = j <= last ? kd : INT32_MIN;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        wlo = min(wlo, __shfl_xor(wlo, o, 64));
-        whi = max(whi, __shfl_xor(whi, o, 64));
+    int wlo = 0, whi = 0;
+    if (u.qd) {
+        wlo = __builtin_amdgcn_readfirstlane(wave_imin(j <= last ? kd : INT32_MAX));
+        whi = __builtin_amdgcn_readfirstlane(wave_imax(j <= last ? kd : INT32_MIN));
     }
-    wlo = __builtin_amdgcn_readfirstlane(wlo);
-    whi = __builtin_amdgcn_readfirstlane(whi);
     // the blocks of rows that may see them
     int plo, phi;
     pos_range(u, first, last, pre, plo, phi);
@@ -293,8 +282,7 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
     if (phi < plo) r1 = r0;
     const int t0 = r0 / kBlock, t1 = r1 <= r0 ? t0 - 1 : (r1 - 1) / kBlock;
     uint32_t gt = 0, gl = 0xFFFFFFFFu, qt = 0, ql = 0xFFFFFFFFu;
-    auto looked = [&](int rt, RowStep &st) {
-        const RowStats r = a.rs[rt0 + rt];
+    auto looked = [&](int rt, const RowStats &r, RowStep &st) {
         st.q = r.q;
         st.g2 = r.g2;
         st.q2 = r.q2;
@@ -304,11 +292,11 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
         st.dhi = r.doc_hi;
         if (u.qd && (r.doc_hi < kdlo || r.doc_lo > kdhi || r.doc_hi < 0)) st.see = 0;
         if (r.g2_top == 0 && r.q2_top == 0) st.see = 0;  // rows without gradient
-        return r;
     };
     for (int rt = t0 + (int)threadIdx.x; rt <= t1; rt += 256) {
         RowStep st;
-        const RowStats r = looked(rt, st);
+        const RowStats r = a.rs[rt0 + rt];
+        looked(rt, r, st);
         bad = bad || r.bad;
         gt = max(gt, r.g2_top);
         qt = max(qt, r.q2_top);
@@ -323,13 +311,10 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
             lhi[rt - t0] = st.dhi;
         }
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        gt = max(gt, (uint32_t)__shfl_xor((int)gt, o, 64));
-        qt = max(qt, (uint32_t)__shfl_xor((int)qt, o, 64));
-        gl = min(gl, (uint32_t)__shfl_xor((int)gl, o, 64));
-        ql = min(ql, (uint32_t)__shfl_xor((int)ql, o, 64));
-    }
+    gt = wave_umax(gt);
+    qt = wave_umax(qt);
+    gl = wave_umin(gl);
+    ql = wave_umin(ql);
     const uint32_t wave_bad = __any(bad) ? 1 : 0;
     if (lane == 0) {
         red[w][0] = gt;
@@ -381,7 +366,6 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
 #pragma unroll
         for (int e = 0; e < 16; e++) dk[n][e] = dv[n][e] = 0.0f;
     float g2cur = 1.0f, q2cur = 1.0f;
-    const float A = vs.scale / vref, Bd = 1.0f / vref;
     int sd = kNoScale;  // dk's sums are in units of 2^sd
     const int steps = (t1 - t0 + 1) * 2;
     auto next = [&](int it) {
@@ -406,38 +390,14 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
         one(a.gn, 1);
         one(a.g2, 2);
         one(a.q2, 3);
-    };
-    // this thread's value of the step's rows: m, delta, position, slope by wavefront pairs; documents by the last threads
-    auto row_value = [&](int it) -> float {
-        const int which = threadIdx.x >> 5, rr = t0 * kBlock + it * kStep + (threadIdx.x & 31);
-        const int64_t at = rt0 * kBlock + rr;
-        if (which == 0) return a.v.m[at];
-        if (which == 1) return a.v.delta[at] * Bd;
-        const Row row = row_of(u, hk, min(rr, rows - 1));
-        if (which == 2) return __int_as_float(row.t + u.off);
-        if (which == 3) return u.slopes ? u.slopes[row.h] * kLog2e : 0.0f;
-        if (which == 4) return __int_as_float(u.qd ? u.qd[(int64_t)b * u.lq + row.t] : 0);
-        return 0.0f;
-    };
-    auto keep = [&](float v, int buf) {
-        const int which = threadIdx.x >> 5, r = threadIdx.x & 31;
-        if (which < 4) rv[buf][which][r] = v;
-        else if (which == 4) rdoc[buf][r] = __float_as_int(v);
+        if (w == 0) load_to_lds(a.v + row_value((rt0 + t0) * kBlock + (int64_t)it * kStep, 0) + 4 * lane, to + 4 * HALF);
     };
     int it = next(-1), buf = 0;
-    if (it < steps) {
-        stage(it, 0);
-        keep(row_value(it), 0);
-    }
+    if (it < steps) stage(it, 0);
     while (it < steps) {
-        wait_loads();
-        __syncthreads();
+        land<0>();
         const int nx = next(it);
-        float nv = 0.0f;
-        if (nx < steps) {
-            stage(nx, buf ^ 1);
-            nv = row_value(nx);
-        }
+        if (nx < steps) stage(nx, buf ^ 1);
         RowStep st;
         if ((it >> 1) < kListed) {
             st.q = lq_[it >> 1];
@@ -446,7 +406,7 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
             st.dlo = __builtin_amdgcn_readfirstlane(llo[it >> 1]);
             st.dhi = __builtin_amdgcn_readfirstlane(lhi[it >> 1]);
         } else {
-            looked(t0 + (it >> 1), st);
+            looked(t0 + (it >> 1), a.rs[rt0 + t0 + (it >> 1)], st);
         }
         const int f0 = t0 * kBlock + it * kStep, f1 = min(f0 + kStep, rows) - 1;
         const int i0 = f0 / u.G + u.off, i1 = f1 / u.G + u.off;
@@ -465,6 +425,7 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
                 q2cur = st.q2;
             }
             const char *qf = sh + 256 + buf * STAGE + lane * 16, *gf = qf + HALF, *g2f = gf + HALF, *q2f = g2f + HALF;
+            const float *rv = reinterpret_cast<const float *>(sh + 256 + buf * STAGE + 4 * HALF) + 4 * g;
             floatx16 x, dp;
 #pragma unroll
             for (int e = 0; e < 16; e++) x[e] = dp[e] = 0.0f;
@@ -498,30 +459,30 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
             float top = 0.0f;
 #pragma unroll
             for (int q = 0; q < 4; q++) {
-                const floatx4 m4 = *reinterpret_cast<const floatx4 *>(&rv[buf][0][8 * q + 4 * g]);
-                const floatx4 d4 = *reinterpret_cast<const floatx4 *>(&rv[buf][1][8 * q + 4 * g]);
+                const floatx4 m4 = *reinterpret_cast<const floatx4 *>(rv + 32 * kRowM + 8 * q);
+                const floatx4 d4 = *reinterpret_cast<const floatx4 *>(rv + 32 * kRowDelta + 8 * q);
                 floatx4 y;
 #pragma unroll
                 for (int r = 0; r < 4; r++) y[r] = __builtin_fmaf(x[4 * q + r], fx, (float)kLift - m4[r]);
                 if (u.slopes || !whole) {
-                    const intx4 p4 = *reinterpret_cast<const intx4 *>(&rv[buf][2][8 * q + 4 * g]);
+                    const intx4 p4 = *reinterpret_cast<const intx4 *>(rv + 32 * kRowPos + 8 * q);
                     if (u.slopes) {
-                        const floatx4 s4 = *reinterpret_cast<const floatx4 *>(&rv[buf][3][8 * q + 4 * g]);
+                        const floatx4 s4 = *reinterpret_cast<const floatx4 *>(rv + 32 * kRowSlope + 8 * q);
 #pragma unroll
                         for (int r = 0; r < 4; r++) y[r] = __builtin_fmaf(-s4[r], __builtin_fabsf((float)(p4[r] - j)), y[r]);
                     }
                     if (!whole) {
                         intx4 qd = {kd, kd, kd, kd};
-                        if (!one) qd = *reinterpret_cast<const intx4 *>(&rdoc[buf][8 * q + 4 * g]);
+                        if (!one) qd = *reinterpret_cast<const intx4 *>(rv + 32 * kRowDoc + 8 * q);
 #pragma unroll
-                        for (int r = 0; r < 4; r++) y[r] = reach.has(p4[r]) & (qd[r] == kd) ? y[r] : -3e38f;
+                        for (int r = 0; r < 4; r++) y[r] = (reach.has(p4[r]) & (qd[r] == kd)) ? y[r] : -3e38f;
                     }
                 }
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const int e = 4 * q + r;
                     const float ex = exp2_hw(y[r]);
-                    float ds = ex * __builtin_fmaf(dp[e], A, -d4[r]);
+                    float ds = ex * __builtin_fmaf(dp[e], vs.scale, -d4[r]);
                     if (u.icap != 0.0f) ds *= __builtin_fmaf(-x[e], x[e], 1.0f);
                     dp[e] = ds;
                     x[e] = ex;
@@ -559,12 +520,11 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
                 }
             }
         }
-        if (nx < steps) keep(nv, buf ^ 1);
         it = nx;
         buf ^= 1;
     }
     if (j > last) return;
-    const float fv = g2cur * pow2(-kLift), fk = q2cur * vref * pow2(-kLift) * u.scale;
+    const float fv = g2cur * pow2(-kLift), fk = q2cur * pow2(-kLift) * u.scale;
     float *tk = dest(0, j), *tv = dest(1, j);
 #pragma unroll
     for (int n = 0; n < ND; n++)
@@ -582,14 +542,13 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
 // ------------------------------------------------------------------------------------------------------------ dq
 template <int DP>
 __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const BwdArgs &a, int i, char *sh, RowsTables &t_) {
-    constexpr int S = DP / 16, ND = DP / 32, HALF = kStep * DP * 4, STAGE = 3 * HALF;
+    constexpr int S = DP / 16, ND = DP / 32, HALF = kStep * DP * 4, STAGE = 3 * HALF + 128;  // the keys' documents last
     auto &lk_ = t_.k;
     auto &lv_ = t_.v;
     auto &lstep = t_.step;
     auto &lsee = t_.see;
     auto &llo = t_.lo;
     auto &lhi = t_.hi;
-    auto &kdoc = t_.doc;
     auto &red = t_.red;
     const int rb = a.rblocks - 1 - i % a.rblocks, item = i / a.rblocks;  // the longest rows of a causal rule first
     const int b = item / u.Hk, hk = item - b * u.Hk, rows = u.G * u.lq;
@@ -613,17 +572,17 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
     key_range(u, i0, i1, pre, lo, hi);
     const int t0 = lo / kBlock, t1 = hi < lo ? t0 - 1 : hi / kBlock;
     uint32_t kt = 0, vt = 0, kl = 0xFFFFFFFFu;
-    for (int t = t0 + (int)threadIdx.x; t <= t1; t += 256) {
-        kt = max(kt, a.ks[kt0 + t].top);
-        kl = min(kl, a.ks[kt0 + t].low);
-        vt = max(vt, a.vs[kt0 + t].top);
+    Stats mk = {}, mv = {};  // the thread's first
+    for (int t = t0 + (int)threadIdx.x, n = 0; t <= t1; t += 256, n++) {
+        const Stats sk = a.ks[kt0 + t], sv = a.vs[kt0 + t];
+        if (n == 0) mk = sk, mv = sv;
+        kt = max(kt, sk.top);
+        kl = min(kl, sk.low);
+        vt = max(vt, sv.top);
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        kt = max(kt, (uint32_t)__shfl_xor((int)kt, o, 64));
-        vt = max(vt, (uint32_t)__shfl_xor((int)vt, o, 64));
-        kl = min(kl, (uint32_t)__shfl_xor((int)kl, o, 64));
-    }
+    kt = wave_umax(kt);
+    vt = wave_umax(vt);
+    kl = wave_umin(kl);
     if (lane == 0) {
         red[w][0] = kt;
         red[w][1] = vt;
@@ -641,37 +600,32 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
         for (int r = first + 32 * w; r <= min(last, first + 32 * w + 31); r++) plain_dq<DP>(u, p, b, hk, r, lo, hi, pre);
         return;
     }
-    const int ek = kt ? scale_exp(kt) : 0, ev = vt ? scale_exp(vt) : 0;
-    int wlo = doc, whi = doc;  // documents of the wavefront's rows
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        wlo = min(wlo, __shfl_xor(wlo, o, 64));
-        whi = max(whi, __shfl_xor(whi, o, 64));
+    const int ek = kt ? scale_exp(kt) : 0;
+    int wlo = 0, whi = 0;  // documents of the wavefront's rows
+    if (u.qd) {
+        wlo = __builtin_amdgcn_readfirstlane(wave_imin(doc));
+        whi = __builtin_amdgcn_readfirstlane(wave_imax(doc));
     }
-    wlo = __builtin_amdgcn_readfirstlane(wlo);
-    whi = __builtin_amdgcn_readfirstlane(whi);
-    auto looked = [&](int t, float &sk, float &sv, int &step, int &dlo, int &dhi) -> int {
-        const Stats ks = a.ks[kt0 + t], vs = a.vs[kt0 + t];
+    auto looked = [&](int t, const Stats &ks, const Stats &vs, float &sk, float &sv, int &step) -> int {
         sk = ks.scale;
-        sv = vs.top ? vs.scale * pow2(-ev) : 1.0f;
+        sv = vs.scale;
         step = ks.top ? ((int)(__float_as_uint(ks.scale) >> 23) - 127 - ek) / 4 : 0;
         const int j0 = t * kBlock, j1 = j0 + kBlock - 1;
         int see = may_see(u, i0, i1, j0, j1, pre);
-        dlo = ks.doc_lo;
-        dhi = ks.doc_hi;
-        if (u.qd && (dhi < 0 || dhi < qlo || dlo > qhi)) see = 0;
+        if (u.qd && (ks.doc_hi < 0 || ks.doc_hi < qlo || ks.doc_lo > qhi)) see = 0;
         return see;
     };
-    for (int t = t0 + (int)threadIdx.x; t <= t1 && t < t0 + kListed; t += 256) {
+    if (t0 + (int)threadIdx.x <= t1) {
+        static_assert(kListed == 256, "a thread's first block is its entry");
         float sk, sv;
-        int step, dlo, dhi;
-        const int see = looked(t, sk, sv, step, dlo, dhi);
-        llo[t - t0] = dlo;
-        lhi[t - t0] = dhi;
-        lk_[t - t0] = sk;
-        lv_[t - t0] = sv;
-        lstep[t - t0] = (signed char)step;
-        lsee[t - t0] = (unsigned char)see;
+        int step;
+        const int see = looked(t0 + threadIdx.x, mk, mv, sk, sv, step);
+        llo[threadIdx.x] = mk.doc_lo;
+        lhi[threadIdx.x] = mk.doc_hi;
+        lk_[threadIdx.x] = sk;
+        lv_[threadIdx.x] = sv;
+        lstep[threadIdx.x] = (signed char)step;
+        lsee[threadIdx.x] = (unsigned char)see;
     }
     __syncthreads();
     // Q and G fragments of the wavefront's rows, and their values
@@ -689,7 +643,7 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
         }
     }
     const int64_t at = rt0 * kBlock + min(rr, a.nr * kBlock - 1);
-    const float m = a.v.m[at], delta = a.v.delta[at] * pow2(-ev), wr = a.v.w[at];
+    const float m = a.v[row_value(at, kRowM)], delta = a.v[row_value(at, kRowDelta)], wr = a.v[row_value(at, kRowW)];
     const Reach reach = keys_seen(u, pos, doc, pre);
     floatx16 dq[ND];
     int sd = kNoScale;  // dq's sums are in units of 2^sd
@@ -718,25 +672,15 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
         one(a.kn, 0);
         one(a.vn, 1);
         one(a.kt, 2);
-    };
-    auto key_doc = [&](int it) -> int {  // of the step's key threadIdx.x
-        const int j = t0 * kBlock + it * kStep + (int)threadIdx.x;
-        return u.kd && threadIdx.x < kStep && j < u.lk ? u.kd[(int64_t)b * u.lk + j] : -1;
+        if (u.kd && threadIdx.x < kStep)
+            load_to_lds4(u.kd + (int64_t)b * u.lk + min(t0 * kBlock + it * kStep + lane, u.lk - 1), to + 3 * HALF);
     };
     int it = next(-1), buf = 0;
-    if (it < steps) {
-        stage(it, 0);
-        if (u.kd && threadIdx.x < kStep) kdoc[0][threadIdx.x] = key_doc(it);
-    }
+    if (it < steps) stage(it, 0);
     while (it < steps) {
-        wait_loads();
-        __syncthreads();
+        land<0>();
         const int nx = next(it);
-        int nd = -1;
-        if (nx < steps) {
-            stage(nx, buf ^ 1);
-            nd = key_doc(nx);
-        }
+        if (nx < steps) stage(nx, buf ^ 1);
         float sk, sv;
         int step, dlo, dhi;
         if ((it >> 1) < kListed) {
@@ -746,11 +690,15 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
             dlo = __builtin_amdgcn_readfirstlane(llo[it >> 1]);
             dhi = __builtin_amdgcn_readfirstlane(lhi[it >> 1]);
         } else {
-            looked(t0 + (it >> 1), sk, sv, step, dlo, dhi);
+            const Stats ks = a.ks[kt0 + t0 + (it >> 1)];
+            looked(t0 + (it >> 1), ks, a.vs[kt0 + t0 + (it >> 1)], sk, sv, step);
+            dlo = ks.doc_lo;
+            dhi = ks.doc_hi;
         }
         const int j0 = t0 * kBlock + it * kStep, j1 = j0 + kStep - 1;
         if (live && !(u.qd && (whi < 0 || dhi < wlo || dlo > whi)) && may_see(u, wi0, wi1, j0, j1, pre)) {
             const char *kf = sh + 256 + buf * STAGE + lane * 16, *vf = kf + HALF, *ktf = vf + HALF;
+            const int *kdoc = reinterpret_cast<const int *>(sh + 256 + buf * STAGE + 3 * HALF) + 4 * g;
             floatx16 x, dp;
 #pragma unroll
             for (int e = 0; e < 16; e++) x[e] = dp[e] = 0.0f;
@@ -788,7 +736,7 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
                 float y = __builtin_fmaf(x[e], fx, mu);
                 const int o = 8 * (e >> 2) + (e & 3);
                 if (u.slopes) y = __builtin_fmaf(-slope, __builtin_fabsf(gap0 - (float)o), y);
-                if (!whole) y = reach.has(j0 + 4 * g + o) & (one || kdoc[buf][4 * g + o] == doc) ? y : -3e38f;
+                if (!whole) y = (reach.has(j0 + 4 * g + o) & (one || kdoc[o] == doc)) ? y : -3e38f;
                 float ds = exp2_hw(y) * __builtin_fmaf(dp[e], sv, -delta);
                 if (u.icap != 0.0f) ds *= __builtin_fmaf(-x[e], x[e], 1.0f);
                 dp[e] = ds;
@@ -819,12 +767,11 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
                 }
             }
         }
-        if (u.kd && nx < steps && threadIdx.x < kStep) kdoc[buf ^ 1][threadIdx.x] = nd;
         it = nx;
         buf ^= 1;
     }
     if (rr > last) return;
-    const float f = u.scale * pow2(ek) * pow2(ev);
+    const float f = u.scale * pow2(ek);
     float *to = p.dq + tok * p.lddq + (int64_t)row.h * u.d;
 #pragma unroll
     for (int n = 0; n < ND; n++)
@@ -839,7 +786,7 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
 template <int DP>
 __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) k_scored_bwd_mm(Rule u, Ptrs p, BwdArgs a) {
     OM_LDS_POISON();
-    __shared__ __attribute__((aligned(16))) char sh[256 + 2 * 4 * kStep * DP * 4];  // no stage at LDS address 0
+    __shared__ __attribute__((aligned(16))) char sh[256 + 2 * (4 * kStep * DP * 4 + 1024)];  // no stage at LDS address 0
     __shared__ __attribute__((aligned(16))) union {
         KeysTables k;
         RowsTables r;
@@ -898,11 +845,11 @@ om_status bwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p) {
     OM_REQUIRE(ctx, wk + wr <= INT32_MAX && jobs <= INT32_MAX, "%s: too many row blocks", what);
     a.first_rows = (int)wk;
     const int64_t kp = plane_bytes(dp, items * a.nt), rp = plane_bytes(dp, items * a.nr);
-    const int64_t vals = items * a.nr * kBlock * (int64_t)sizeof(float);
+    const int64_t vals = items * a.nr * kBlock * kRowValues * (int64_t)sizeof(float);
     const int64_t part = keys && a.nsplit > 1 ? (int64_t)sizeof(float) * a.nsplit * items * u.lk * 2 * u.d : 0;
     const int64_t stats = 2 * items * a.nt * (int64_t)sizeof(Stats) + items * a.nr * (int64_t)sizeof(RowStats);
     float *scr;
-    if (om_status s = om::scratch2(ctx, (uint64_t)(3 * kp + 4 * rp + 3 * vals + stats + part), &scr)) return s;
+    if (om_status s = om::scratch2(ctx, (uint64_t)(3 * kp + 4 * rp + vals + stats + part), &scr)) return s;
     char *at = reinterpret_cast<char *>(scr);
     auto take = [&](int64_t bytes) {
         char *x = at;
@@ -918,10 +865,7 @@ om_status bwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p) {
     a.gn = ro.g = take(rp);
     a.g2 = ro.g2 = take(rp);
     a.q2 = ro.q2 = take(rp);
-    ro.v.m = reinterpret_cast<float *>(take(vals));
-    ro.v.delta = reinterpret_cast<float *>(take(vals));
-    ro.v.w = reinterpret_cast<float *>(take(vals));
-    a.v = ro.v;
+    a.v = ro.v = reinterpret_cast<float *>(take(vals));
     a.ks = ko.stats = reinterpret_cast<Stats *>(take(items * a.nt * (int64_t)sizeof(Stats)));
     a.vs = vo.stats = reinterpret_cast<Stats *>(take(items * a.nt * (int64_t)sizeof(Stats)));
     a.rs = ro.stats = reinterpret_cast<RowStats *>(take(items * a.nr * (int64_t)sizeof(RowStats)));

@@ -1,9 +1,9 @@
 // Scored attention's forward on the matrix cores (operands: om_attention_scored_mm.hpp).
 //
 // A workgroup takes 128 rows of one key head's group (a wavefront 32: its lanes' queries) and walks the visible keys in
-// steps of KT. S^T = K Q^T leaves a query's scores in its lane's registers; they become weights E = 2^(x - m) there, are
-// split, and are the operand of O^T += V^T E^T as they stand. K and V come split from scratch, straight into LDS, two
-// stages, one barrier a step. The running maximum m moves only when some lane's maximum grows by more than 2^2: E then
+// steps of 32. S^T = K Q^T leaves a query's scores in its lane's registers; they become weights E = 2^(x - m) there, are
+// split, and are the operand of O^T += V^T E^T as they stand. K and V come split from scratch, straight into LDS, a
+// ring of steps, one barrier each. The running maximum m moves only when some lane's maximum grows by more than 2^2: E then
 // stays below 2^14 with its 2^12 of headroom, and the accumulators are left alone in most steps.
 #include "om_attention_scored_split.hpp"
 
@@ -15,7 +15,7 @@ constexpr float kInf = __builtin_inff();
 constexpr int kRows = 128;      // rows of a workgroup
 constexpr float kLift = 12.0f;  // weights are kept as 2^kLift times themselves, so that their split's m is normal fp16
 constexpr float kSlack = 2.0f;  // how far a maximum may outgrow m before m moves
-constexpr int kListed = 512;    // blocks of keys whose step data stands in LDS
+constexpr int kListed = 256;    // blocks of keys whose step data stands in LDS
 
 template <int DP, bool VEC>
 __global__ void __launch_bounds__(256) k_scored_split_kv(Rule u, Ptrs p, SplitOut ko, SplitOut vo, int nt) {
@@ -120,17 +120,17 @@ struct FwdArgs {
     int vec;                  // q's rows are 16-byte aligned
 };
 
-template <int DP, int KT>
-__global__ void __launch_bounds__(256, 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArgs a) {
+template <int DP>
+__global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArgs a) {
     OM_LDS_POISON();
-    constexpr int S = DP / 16, NB = KT / 32, ND = DP / 32;
-    constexpr int HALF = KT * DP * 4, STAGE = 2 * HALF;  // K's planes, then V's
-    __shared__ __attribute__((aligned(16))) char sh[256 + 2 * STAGE];  // no stage at LDS address 0
+    constexpr int KT = 32, S = DP / 16, ND = DP / 32, NST = DP == 128 ? 2 : 3;  // as many stages as leave two workgroups a CU
+    constexpr int HALF = KT * DP * 4, STAGE = 2 * HALF + KT * 4;  // K's planes, V's, the keys' documents
+    constexpr int PER = 2 * (HALF / 4096);  // loads of a step per wavefront, documents aside
+    __shared__ __attribute__((aligned(16))) char sh[256 + NST * STAGE];  // no stage at LDS address 0
     __shared__ float kscale[kListed];
     __shared__ signed char vstep[kListed];  // exponent of V's scale less the largest, in steps of 4
     __shared__ unsigned char visit[kListed];  // whether some row may see the block
     __shared__ int docs_lo[kListed], docs_hi[kListed];
-    __shared__ __attribute__((aligned(16))) int kdoc[2][KT];  // documents of the step's keys
     __shared__ uint32_t red[4][6];
     int rb, item;
     on_one_xcd(a.blocks * a.nsplit, rb, item);
@@ -146,31 +146,49 @@ __global__ void __launch_bounds__(256, 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArg
     const int pos = row.t + u.off, doc = u.qd ? u.qd[tok] : 0;
     const float slope = u.slopes ? u.slopes[row.h] * kLog2e : 0.0f;
 
-    // The row's query, scaled and split: d = 16 s + 8 g + e.
+    // The row's query: d = 16 s + 8 g + e.
+    float x0[S][8];
+    {
+        const float *qr = p.q + tok * p.ldq + (int64_t)row.h * u.d;
+#pragma unroll
+        for (int s = 0; s < S; s++) {
+            const floatx4 lo = a.vec ? load4<true>(qr, 16 * s + 8 * g, u.d) : load4<false>(qr, 16 * s + 8 * g, u.d);
+            const floatx4 hi = a.vec ? load4<true>(qr, 16 * s + 8 * g + 4, u.d) : load4<false>(qr, 16 * s + 8 * g + 4, u.d);
+#pragma unroll
+            for (int e = 0; e < 4; e++) x0[s][e] = lo[e], x0[s][4 + e] = hi[e];
+        }
+    }
+
+    // The blocks of keys this workgroup can see, and what their split found; a thread keeps the first round's.
+    int lo, hi;
+    const int i0 = first / u.G + u.off, i1 = last / u.G + u.off;
+    key_range(u, i0, i1, pre, lo, hi);
+    lo = max(lo, split * a.per * kBlock);
+    hi = (int)min((int64_t)hi, (int64_t)(split + 1) * a.per * kBlock - 1);
+    const int t0 = lo / kBlock, t1 = hi < lo ? t0 - 1 : hi / kBlock;
+    uint32_t ktop = 0, vtop = 0, vlow = 0xFFFFFFFFu;
+    const int64_t kt0 = (int64_t)item * a.nt;
+    Stats mk = {}, mv = {};
+    for (int t = t0 + (int)threadIdx.x, n = 0; t <= t1; t += 256, n++) {
+        const Stats sk = a.ks[kt0 + t], sv = a.vs[kt0 + t];
+        if (n == 0) mk = sk, mv = sv;
+        ktop = max(ktop, sk.top);
+        vtop = max(vtop, sv.top);
+        vlow = min(vlow, sv.low);
+    }
+    // The query, scaled and split.
     u32x4 qh[S], qm[S];
     int eq;
     bool bad;
     {
-        const float *qr = p.q + tok * p.ldq + (int64_t)row.h * u.d;
-        float x[S][8];
         uint32_t top = 0;
 #pragma unroll
-        for (int s = 0; s < S; s++) {
-            if (a.vec) {
-                const floatx4 lo = load4<true>(qr, 16 * s + 8 * g, u.d), hi = load4<true>(qr, 16 * s + 8 * g + 4, u.d);
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[s][e] = lo[e], x[s][4 + e] = hi[e];
-            } else {
-                const floatx4 lo = load4<false>(qr, 16 * s + 8 * g, u.d), hi = load4<false>(qr, 16 * s + 8 * g + 4, u.d);
-#pragma unroll
-                for (int e = 0; e < 4; e++) x[s][e] = lo[e], x[s][4 + e] = hi[e];
-            }
+        for (int s = 0; s < S; s++)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                if (doc < 0) x[s][e] = 0.0f;
-                top = max(top, __float_as_uint(x[s][e]) & 0x7FFFFFFFu);
+                if (doc < 0) x0[s][e] = 0.0f;
+                top = max(top, __float_as_uint(x0[s][e]) & 0x7FFFFFFFu);
             }
-        }
         const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
         top = max(both[0], both[1]);
         bad = !in_range(top);
@@ -179,47 +197,32 @@ __global__ void __launch_bounds__(256, 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArg
 #pragma unroll
         for (int s = 0; s < S; s++) {
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[s][e] *= sc;
-            split8(x[s], qh[s], qm[s]);
+            for (int e = 0; e < 8; e++) x0[s][e] *= sc;
+            split8(x0[s], qh[s], qm[s]);
         }
     }
-
-    // The blocks of keys this workgroup can see, and what their split found.
-    int lo, hi;
-    const int i0 = first / u.G + u.off, i1 = last / u.G + u.off;
-    key_range(u, i0, i1, pre, lo, hi);
-    lo = max(lo, split * a.per * kBlock);
-    hi = (int)min((int64_t)hi, (int64_t)(split + 1) * a.per * kBlock - 1);
-    const int t0 = lo / kBlock, t1 = hi < lo ? t0 - 1 : hi / kBlock;
-    uint32_t ktop = 0, vtop = 0, vlow = 0xFFFFFFFFu;
-    int qlo = doc < 0 ? INT32_MAX : doc, qhi = doc;
-    const int64_t kt0 = (int64_t)item * a.nt;
-    for (int t = t0 + (int)threadIdx.x; t <= t1; t += 256) {
-        ktop = max(ktop, a.ks[kt0 + t].top);
-        vtop = max(vtop, a.vs[kt0 + t].top);
-        vlow = min(vlow, a.vs[kt0 + t].low);
-    }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        ktop = max(ktop, (uint32_t)__shfl_xor((int)ktop, o, 64));
-        vtop = max(vtop, (uint32_t)__shfl_xor((int)vtop, o, 64));
-        vlow = min(vlow, (uint32_t)__shfl_xor((int)vlow, o, 64));
-        qlo = min(qlo, __shfl_xor(qlo, o, 64));
-        qhi = max(qhi, __shfl_xor(qhi, o, 64));
+    ktop = wave_umax(ktop);
+    vtop = wave_umax(vtop);
+    vlow = wave_umin(vlow);
+    // documents of the wavefront's rows; a padded row sees nothing, whatever the others see
+    int wqlo = 0, wqhi = 0;
+    bool one_doc = true;
+    if (u.qd) {
+        wqlo = __builtin_amdgcn_readfirstlane(wave_imin(doc < 0 ? INT32_MAX : doc));
+        wqhi = __builtin_amdgcn_readfirstlane(wave_imax(doc));
+        one_doc = wqlo == wqhi && !__any(doc < 0);
     }
     const uint32_t wave_bad = __any(bad) ? 1 : 0;
     if (lane == 0) {
         red[w][0] = ktop;
         red[w][1] = vtop;
         red[w][2] = vlow;
-        red[w][3] = (uint32_t)qlo;
-        red[w][4] = (uint32_t)qhi;
+        red[w][3] = (uint32_t)wqlo;
+        red[w][4] = (uint32_t)wqhi;
         red[w][5] = wave_bad;
     }
-    // documents of the wavefront's rows; a padded row sees nothing, whatever the others see
-    const int wqlo = __builtin_amdgcn_readfirstlane(qlo), wqhi = __builtin_amdgcn_readfirstlane(qhi);
-    const bool one_doc = wqlo == wqhi && !__any(doc < 0);
     __syncthreads();
+    int qlo = wqlo, qhi = wqhi;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         ktop = max(ktop, red[i][0]);
@@ -236,28 +239,25 @@ __global__ void __launch_bounds__(256, 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArg
         return;
     }
     const int ev = vtop ? scale_exp(vtop) : 0;
-    auto looked = [&](int t, float &sc, int &step, int &dlo, int &dhi) -> int {
-        const Stats ks = a.ks[kt0 + t];
+    auto looked = [&](int t, const Stats &ks, const Stats &vs, float &sc, int &step) -> int {
         sc = ks.scale;
-        dlo = ks.doc_lo;
-        dhi = ks.doc_hi;
-        step = ((int)(__float_as_uint(a.vs[kt0 + t].scale) >> 23) - 127 - ev) / 4;
-        if (a.vs[kt0 + t].top == 0) step = 0;  // a block of zeros
+        step = vs.top ? ((int)(__float_as_uint(vs.scale) >> 23) - 127 - ev) / 4 : 0;  // 0 for a block of zeros
         const int j0 = t * kBlock, j1 = j0 + kBlock - 1;
         int see = 1;
         if (j0 >= pre) see = !(u.causal && j0 > i1) && !(u.window && (i0 - j1 >= u.window || j0 - i1 >= u.window));
-        if (u.qd && (dhi < qlo || dlo > qhi)) see = 0;
+        if (u.qd && (ks.doc_hi < qlo || ks.doc_lo > qhi)) see = 0;
         return see;
     };
-    for (int t = t0 + (int)threadIdx.x; t <= t1 && t < t0 + kListed; t += 256) {
+    if (t0 + (int)threadIdx.x <= t1) {
+        static_assert(kListed == 256, "a thread's first block is its entry");
         float sc;
-        int step, dlo, dhi;
-        const int see = looked(t, sc, step, dlo, dhi);
-        docs_lo[t - t0] = dlo;
-        docs_hi[t - t0] = dhi;
-        kscale[t - t0] = sc;
-        vstep[t - t0] = (signed char)step;
-        visit[t - t0] = (unsigned char)see;
+        int step;
+        const int see = looked(t0 + threadIdx.x, mk, mv, sc, step);
+        docs_lo[threadIdx.x] = mk.doc_lo;
+        docs_hi[threadIdx.x] = mk.doc_hi;
+        kscale[threadIdx.x] = sc;
+        vstep[threadIdx.x] = (signed char)step;
+        visit[threadIdx.x] = (unsigned char)see;
     }
     __syncthreads();
 
@@ -272,14 +272,15 @@ __global__ void __launch_bounds__(256, 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArg
     };
     const char *kn = a.kn + (kt0 + t0) * plane_bytes(DP, 1), *vt = a.vt + (kt0 + t0) * plane_bytes(DP, 1);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)(sh + 256);
-    auto stage = [&](int it, int buf) {
-        constexpr int PER = HALF / 4096;  // KB of each operand per wavefront
+    auto stage = [&](int it, int slot) {
         const char *ka = kn + (int64_t)it * HALF + lane * 16, *va = vt + (int64_t)it * HALF + lane * 16;
-        const uint32_t to = lds0 + (uint32_t)(buf * STAGE);
+        const uint32_t to = lds0 + (uint32_t)(slot * STAGE);
 #pragma unroll
-        for (int i = 0; i < PER; i++) load_to_lds(ka + (4 * i + w) * 1024, to + (uint32_t)(4 * i + w) * 1024u);
+        for (int i = 0; i < PER / 2; i++) load_to_lds(ka + (4 * i + w) * 1024, to + (uint32_t)(4 * i + w) * 1024u);
 #pragma unroll
-        for (int i = 0; i < PER; i++) load_to_lds(va + (4 * i + w) * 1024, to + HALF + (uint32_t)(4 * i + w) * 1024u);
+        for (int i = 0; i < PER / 2; i++) load_to_lds(va + (4 * i + w) * 1024, to + HALF + (uint32_t)(4 * i + w) * 1024u);
+        if (u.kd && lane >> 3 == w)  // eight of the step's keys each
+            load_to_lds4(u.kd + (int64_t)b * u.lk + min(t0 * kBlock + it * KT + lane, u.lk - 1), to + 2 * HALF);
     };
 
     const Reach reach = keys_seen(u, pos, doc, pre);
@@ -293,24 +294,17 @@ __global__ void __launch_bounds__(256, 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArg
     const bool live = first + 32 * w <= last;
     const float cq = __builtin_fabsf(u.cl2) * pow2(eq), icq = __builtin_fabsf(u.icap) * pow2(eq);
 
-    auto key_doc = [&](int it) -> int {  // of the step's key threadIdx.x
-        const int j = t0 * kBlock + it * KT + (int)threadIdx.x;
-        return u.kd && threadIdx.x < KT && j < u.lk ? u.kd[(int64_t)b * u.lk + j] : -1;
-    };
-    int it = next(-1), buf = 0;
-    if (it < steps) {
-        stage(it, 0);
-        if (u.kd && threadIdx.x < KT) kdoc[0][threadIdx.x] = key_doc(it);
-    }
+    int it = next(-1), nx = it < steps ? next(it) : steps, slot = 0;
+    if (it < steps) stage(it, 0);
+    if (NST == 3 && nx < steps) stage(nx, 1);
     while (it < steps) {
-        wait_loads();
-        __syncthreads();  // this step has landed, and every wavefront is done with the other stage
-        const int nx = next(it);
-        int nd = -1;
-        if (nx < steps) {
-            stage(nx, buf ^ 1);
-            nd = key_doc(nx);
-        }
+        // this step has landed (with three stages the next is in flight), and every wavefront is done with the one before
+        if (NST == 2 || nx >= steps) land<0>();
+        else if (u.kd) land<PER + 1>();
+        else land<PER>();
+        const int nn = nx < steps ? next(nx) : steps;
+        if (NST == 3 && nn < steps) stage(nn, slot == 0 ? 2 : slot - 1);
+        if (NST == 2 && nx < steps) stage(nx, slot ^ 1);
         const int j0 = t0 * kBlock + it * KT, j1 = j0 + KT - 1, ti = it * KT / kBlock;
         float ksc;
         int vst, dlo, dhi;
@@ -320,7 +314,10 @@ __global__ void __launch_bounds__(256, 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArg
             dlo = __builtin_amdgcn_readfirstlane(docs_lo[ti]);
             dhi = __builtin_amdgcn_readfirstlane(docs_hi[ti]);
         } else {
-            looked(t0 + ti, ksc, vst, dlo, dhi);
+            const Stats ks = a.ks[kt0 + t0 + ti];
+            looked(t0 + ti, ks, a.vs[kt0 + t0 + ti], ksc, vst);
+            dlo = ks.doc_lo;
+            dhi = ks.doc_hi;
         }
         // what the wavefront's 32 rows see of the step
         const bool none = !live || (u.qd && (dhi < wqlo || dlo > wqhi)) || (j0 >= pre && ((u.causal && j0 > wi1) ||
@@ -329,18 +326,16 @@ __global__ void __launch_bounds__(256, 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArg
         const bool whole = j1 < u.lk && one &&
                            (j1 < pre || ((!u.causal || j1 <= wi0) && (!u.window || (wi1 - j0 < u.window && j1 - wi0 < u.window))));
         if (!none) {
-            const char *kf = sh + 256 + buf * STAGE + lane * 16, *vf = kf + HALF;
-            floatx16 x[NB];
+            const char *kf = sh + 256 + slot * STAGE + lane * 16, *vf = kf + HALF;
+            const int *kdoc = reinterpret_cast<const int *>(sh + 256 + slot * STAGE + 2 * HALF);
+            floatx16 x;
 #pragma unroll
-            for (int n = 0; n < NB; n++) {
+            for (int e = 0; e < 16; e++) x[e] = 0.0f;
 #pragma unroll
-                for (int e = 0; e < 16; e++) x[n][e] = 0.0f;
-#pragma unroll
-                for (int s = 0; s < S; s++) {
-                    const u32x4 kh = *reinterpret_cast<const u32x4 *>(kf + ((n * S + s) * 2) * 1024);
-                    const u32x4 km = *reinterpret_cast<const u32x4 *>(kf + ((n * S + s) * 2 + 1) * 1024);
-                    x[n] = mma3(kh, km, qh[s], qm[s], x[n]);
-                }
+            for (int s = 0; s < S; s++) {
+                const u32x4 kh = *reinterpret_cast<const u32x4 *>(kf + (2 * s) * 1024);
+                const u32x4 km = *reinterpret_cast<const u32x4 *>(kf + (2 * s + 1) * 1024);
+                x = mma3(kh, km, qh[s], qm[s], x);
             }
             // x * f is the score in log2 units
             float f = cq * ksc;
@@ -348,53 +343,40 @@ __global__ void __launch_bounds__(256, 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArg
                 const float ic = icq * ksc;
                 float big = 0.0f;
 #pragma unroll
-                for (int n = 0; n < NB; n++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) big = fmaxf(big, __builtin_fabsf(x[n][e]));
+                for (int e = 0; e < 16; e++) big = fmaxf(big, __builtin_fabsf(x[e]));
                 if (__any(big * ic >= kTanhSmall)) {
 #pragma unroll
-                    for (int n = 0; n < NB; n++)
-#pragma unroll
-                        for (int e = 0; e < 16; e++) x[n][e] = tanh_any(x[n][e] * ic);
+                    for (int e = 0; e < 16; e++) x[e] = tanh_any(x[e] * ic);
                 } else {
 #pragma unroll
-                    for (int n = 0; n < NB; n++)
-#pragma unroll
-                        for (int e = 0; e < 16; e++) x[n][e] = tanh_small(x[n][e] * ic);
+                    for (int e = 0; e < 16; e++) x[e] = tanh_small(x[e] * ic);
                 }
                 f = u.capl2;
             }
             if (u.slopes) {
                 const float gap0 = (float)(pos - j0 - 4 * g);
 #pragma unroll
-                for (int n = 0; n < NB; n++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
-                        const float gap = gap0 - (float)(32 * n + 8 * (e >> 2) + (e & 3));
-                        x[n][e] = __builtin_fmaf(-slope, __builtin_fabsf(gap), x[n][e] * f);
-                    }
+                for (int e = 0; e < 16; e++) {
+                    const float gap = gap0 - (float)(8 * (e >> 2) + (e & 3));
+                    x[e] = __builtin_fmaf(-slope, __builtin_fabsf(gap), x[e] * f);
+                }
                 f = 1.0f;
             }
             if (!whole) {
 #pragma unroll
-                for (int n = 0; n < NB; n++)
+                for (int q = 0; q < 4; q++) {
+                    intx4 kd = {doc, doc, doc, doc};
+                    if (!one) kd = *reinterpret_cast<const intx4 *>(kdoc + 8 * q + 4 * g);
 #pragma unroll
-                    for (int q = 0; q < 4; q++) {
-                        const int k0 = 32 * n + 8 * q + 4 * g;
-                        intx4 kd = {doc, doc, doc, doc};
-                        if (!one) kd = *reinterpret_cast<const intx4 *>(&kdoc[buf][k0]);
-#pragma unroll
-                        for (int r = 0; r < 4; r++) {
-                            const bool ok = reach.has(j0 + k0 + r) & (kd[r] == doc);
-                            x[n][4 * q + r] = ok ? x[n][4 * q + r] : -kInf;
-                        }
+                    for (int r = 0; r < 4; r++) {
+                        const bool ok = reach.has(j0 + 8 * q + 4 * g + r) & (kd[r] == doc);
+                        x[4 * q + r] = ok ? x[4 * q + r] : -kInf;
                     }
+                }
             }
             float top = -kInf;
 #pragma unroll
-            for (int n = 0; n < NB; n++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) top = fmaxf(top, x[n][e]);
+            for (int e = 0; e < 16; e++) top = fmaxf(top, x[e]);
             top = pair_max(top) * f;
             if (__any(top > m + kSlack)) {
                 const float mn = fmaxf(m, top), al = mn == -kInf ? 1.0f : exp2_hw(m - mn);
@@ -406,33 +388,28 @@ __global__ void __launch_bounds__(256, 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArg
             const float lift = kLift + 4.0f * (float)vst, mu = (m == -kInf ? 0.0f : -m) + lift;
             float sum = 0.0f;
 #pragma unroll
-            for (int n = 0; n < NB; n++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    x[n][e] = exp2_hw(__builtin_fmaf(x[n][e], f, mu));
-                    sum += x[n][e];
-                }
+            for (int e = 0; e < 16; e++) {
+                x[e] = exp2_hw(__builtin_fmaf(x[e], f, mu));
+                sum += x[e];
+            }
             l = __builtin_fmaf(sum, pow2(-4 * vst), l);
 #pragma unroll
-            for (int n = 0; n < NB; n++)
+            for (int s = 0; s < 2; s++) {
+                float e8[8];
 #pragma unroll
-                for (int s = 0; s < 2; s++) {
-                    float e8[8];
+                for (int e = 0; e < 8; e++) e8[e] = x[8 * s + e];
+                u32x4 ph, pm;
+                split8(e8, ph, pm);
 #pragma unroll
-                    for (int e = 0; e < 8; e++) e8[e] = x[n][8 * s + e];
-                    u32x4 ph, pm;
-                    split8(e8, ph, pm);
-#pragma unroll
-                    for (int c = 0; c < ND; c++) {
-                        const char *at = vf + (((2 * n + s) * ND + c) * 2) * 1024;
-                        acc[c] = mma3(*reinterpret_cast<const u32x4 *>(at), *reinterpret_cast<const u32x4 *>(at + 1024), ph, pm,
-                                      acc[c]);
-                    }
+                for (int c = 0; c < ND; c++) {
+                    const char *at = vf + ((s * ND + c) * 2) * 1024;
+                    acc[c] = mma3(*reinterpret_cast<const u32x4 *>(at), *reinterpret_cast<const u32x4 *>(at + 1024), ph, pm, acc[c]);
                 }
+            }
         }
-        if (u.kd && nx < steps && threadIdx.x < KT) kdoc[buf ^ 1][threadIdx.x] = nd;
         it = nx;
-        buf ^= 1;
+        nx = nn;
+        slot = slot == NST - 1 ? 0 : slot + 1;
     }
 
     l = pair_sum(l);
@@ -505,18 +482,18 @@ om_status fwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p, int *joins, f
     a.vec = u.d % 4 == 0 && p.ldq % 4 == 0 && al16(p.q);
     const bool vec = u.d % 4 == 0 && p.ldkv % 4 == 0 && al16(p.k) && al16(p.v);
     const SplitOut ko = {base, nullptr, const_cast<Stats *>(a.ks)}, vo = {nullptr, base + plane, const_cast<Stats *>(a.vs)};
-    auto go = [&](auto dpc, auto ktc) {
-        constexpr int DP = decltype(dpc)::value, KT = decltype(ktc)::value;
+    auto go = [&](auto dpc) {
+        constexpr int DP = decltype(dpc)::value;
         auto split = [&](auto kern) {
             hipLaunchKernelGGL(kern, dim3((unsigned)(2 * items * nt)), dim3(256), 0, ctx->stream, u, p, ko, vo, nt);
         };
         vec ? split(k_scored_split_kv<DP, true>) : split(k_scored_split_kv<DP, false>);
-        hipLaunchKernelGGL((k_scored_fwd_mm<DP, KT>), dim3((unsigned)(wgs * ns)), dim3(256), 0, ctx->stream, u, p, a);
+        hipLaunchKernelGGL(k_scored_fwd_mm<DP>, dim3((unsigned)(wgs * ns)), dim3(256), 0, ctx->stream, u, p, a);
     };
-    if (dp == 32) go(std::integral_constant<int, 32>(), std::integral_constant<int, 64>());
-    else if (dp == 64) go(std::integral_constant<int, 64>(), std::integral_constant<int, 64>());
-    else if (dp == 96) go(std::integral_constant<int, 96>(), std::integral_constant<int, 32>());
-    else go(std::integral_constant<int, 128>(), std::integral_constant<int, 32>());
+    if (dp == 32) go(std::integral_constant<int, 32>());
+    else if (dp == 64) go(std::integral_constant<int, 64>());
+    else if (dp == 96) go(std::integral_constant<int, 96>());
+    else go(std::integral_constant<int, 128>());
     *joins = (int)ns;
     *part = a.part;
     return OM_LAUNCH_CHECK(ctx, "om_attention_fwd_scored");

@@ -98,13 +98,40 @@ __device__ __forceinline__ float pair_sum(float v) {
     return a + b;
 }
 
-// 16 bytes per lane from `src` (this lane's address) to LDS at byte address lds + 16 * lane, without registers. m0 holds
-// the address for this one instruction only; nothing else in these kernels reads it. The caller waits (wait_loads) before
-// the barrier after which the data is read.
+// Largest of a value over the wavefront's 64 lanes, in every lane: four rotations inside a row of 16, then the rows' swaps.
+__device__ __forceinline__ uint32_t wave_umax(uint32_t v) {
+    auto turn = [&](auto ctrl) {
+        v = max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, decltype(ctrl)::value, 0xf, 0xf, true));
+    };
+    turn(std::integral_constant<int, 0x128>());
+    turn(std::integral_constant<int, 0x124>());
+    turn(std::integral_constant<int, 0x122>());
+    turn(std::integral_constant<int, 0x121>());
+    const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(p[0], p[1]);
+    const auto q = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max(q[0], q[1]);
+}
+__device__ __forceinline__ uint32_t wave_umin(uint32_t v) { return ~wave_umax(~v); }
+// The same for signed values.
+__device__ __forceinline__ int wave_imax(int v) { return (int)(wave_umax((uint32_t)v ^ 0x80000000u) ^ 0x80000000u); }
+__device__ __forceinline__ int wave_imin(int v) { return ~wave_imax(~v); }
+
+// 16 (or 4) bytes per lane from `src` (this lane's address) to LDS at byte address lds + 16 (4) * lane, without registers. m0
+// holds the address for this one instruction only; nothing else in these kernels reads it. Loads land in the order of
+// their issue; land<N>() waits until at most this wavefront's last N are in flight and its own LDS reads are done, then
+// meets the others.
 __device__ __forceinline__ void load_to_lds(const void *src, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
 }
-__device__ __forceinline__ void wait_loads() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void load_to_lds4(const void *src, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
+}
+template <int N>
+__device__ __forceinline__ void land() {
+    static_assert(N <= 63, "vmcnt holds at most 63");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
 
 // Bytes of one operand's two planes for `blocks` blocks of 64 rows.
 inline __host__ __device__ int64_t plane_bytes(int dp, int64_t blocks) { return blocks * kBlock * dp * 4; }

@@ -151,13 +151,18 @@ __device__ __forceinline__ void split_keys(const Rule &u, const float *src, int6
     }
 }
 
-// What the backward keeps of a row (a query of one head), [B Hk][rows padded to blocks] each.
-struct RowVals {
-    float *m;      // the forward's reference exponent; 3e38 for a row that has nothing to give (its weights become 0)
-    float *delta;  // g . o times 2^-re, re the exponent of g's row scale
-    float *w;      // 2^re / l: what the row's sums are multiplied with at the end; 0 for a row without gradient
+// What the backward keeps of its rows (queries of one head): a record of 1 KB per 32 rows, a value of all 32 after another.
+enum {
+    kRowM,      // the forward's reference exponent; kNoRow for a row that has nothing to give (its weights become 0)
+    kRowDelta,  // g . o times 2^-re, re the exponent of g's row scale
+    kRowPos,    // position (int)
+    kRowSlope,  // slope of its head, in log2 units
+    kRowDoc,    // document (int)
+    kRowW,      // 2^re / l: what the row's sums are multiplied with at the end; 0 for a row without gradient
+    kRowValues = 8
 };
-// Its blocks of 64 rows.
+__host__ __device__ __forceinline__ int64_t row_value(int64_t row, int which) { return (row >> 5) * (32 * kRowValues) + which * 32 + (row & 31); }
+// A block of 64 rows.
 struct RowStats {
     float q, g2, q2;       // scales 2^e of q, of g / l and of q w
     uint32_t g2_top, q2_top;  // largest magnitudes (bits) of the latter two
@@ -167,7 +172,7 @@ struct RowStats {
 struct RowsOut {
     char *q, *g;    // rows form: q by one scale per block, g by one per row
     char *g2, *q2;  // columns form: g / l (for dv) and q w (for dk)
-    RowVals v;
+    float *v;       // row_value
     RowStats *stats;
 };
 constexpr uint32_t kWideMost = (127u + 100) << 23, kWideLeast = (127u - 100) << 23;
@@ -220,9 +225,12 @@ __device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, 
         if (!on) m[i] = kNoRow;
         if ((threadIdx.x & 15) == 0) {
             const int64_t r = at * kBlock + 4 * (threadIdx.x >> 4) + i;
-            o.v.m[r] = m[i];
-            o.v.delta[r] = delta[i];
-            o.v.w[r] = w[i];
+            o.v[row_value(r, kRowM)] = m[i];
+            o.v[row_value(r, kRowDelta)] = delta[i];
+            o.v[row_value(r, kRowPos)] = __int_as_float(row.t + u.off);
+            o.v[row_value(r, kRowSlope)] = u.slopes ? u.slopes[row.h] * kLog2e : 0.0f;
+            o.v[row_value(r, kRowDoc)] = __int_as_float(u.qd ? u.qd[tok] : 0);
+            o.v[row_value(r, kRowW)] = w[i];
         }
     }
     RowStats st = {};
