@@ -20,7 +20,6 @@ using namespace osc;
 constexpr int kKeys = 128;   // keys (or rows) of a workgroup
 constexpr int kStep = 32;    // rows (or keys) of a step
 constexpr int kListed = 256; // blocks whose step data stands in LDS
-constexpr int kLift = 12;    // E is kept as 2^12 E for dv's operand
 
 struct BwdArgs {
     const char *kn, *kt, *vn;        // K in both forms, V in rows form
@@ -403,8 +402,8 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
             st.q = lq_[it >> 1];
             st.g2 = lg2[it >> 1];
             st.q2 = lq2[it >> 1];
-            st.dlo = __builtin_amdgcn_readfirstlane(llo[it >> 1]);
-            st.dhi = __builtin_amdgcn_readfirstlane(lhi[it >> 1]);
+            st.dlo = u.qd ? __builtin_amdgcn_readfirstlane(llo[it >> 1]) : 0;
+            st.dhi = u.qd ? __builtin_amdgcn_readfirstlane(lhi[it >> 1]) : 0;
         } else {
             looked(t0 + (it >> 1), a.rs[rt0 + t0 + (it >> 1)], st);
         }
@@ -463,7 +462,7 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
                 const floatx4 d4 = *reinterpret_cast<const floatx4 *>(rv + 32 * kRowDelta + 8 * q);
                 floatx4 y;
 #pragma unroll
-                for (int r = 0; r < 4; r++) y[r] = __builtin_fmaf(x[4 * q + r], fx, (float)kLift - m4[r]);
+                for (int r = 0; r < 4; r++) y[r] = __builtin_fmaf(x[4 * q + r], fx, m4[r]);
                 if (u.slopes || !whole) {
                     const intx4 p4 = *reinterpret_cast<const intx4 *>(rv + 32 * kRowPos + 8 * q);
                     if (u.slopes) {
@@ -653,10 +652,11 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
         for (int e = 0; e < 16; e++) dq[n][e] = 0.0f;
     const int wi0 = min(first + 32 * w, last) / u.G + u.off, wi1 = min(first + 32 * w + 31, last) / u.G + u.off;
     const int steps = (t1 - t0 + 1) * 2;
+    const bool dense = !u.qd && !(u.window && pre > 0);  // no gaps in what is seen
     auto next = [&](int it) {
         for (it++; it < steps; it++) {
             if (t0 * kBlock + it * kStep > hi) return steps;
-            if ((it >> 1) >= kListed || lsee[it >> 1]) return it;
+            if (dense || (it >> 1) >= kListed || lsee[it >> 1]) return it;
         }
         return steps;
     };
@@ -687,8 +687,8 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
             sk = lk_[it >> 1];
             sv = lv_[it >> 1];
             step = lstep[it >> 1];
-            dlo = __builtin_amdgcn_readfirstlane(llo[it >> 1]);
-            dhi = __builtin_amdgcn_readfirstlane(lhi[it >> 1]);
+            dlo = u.qd ? __builtin_amdgcn_readfirstlane(llo[it >> 1]) : 0;
+            dhi = u.qd ? __builtin_amdgcn_readfirstlane(lhi[it >> 1]) : 0;
         } else {
             const Stats ks = a.ks[kt0 + t0 + (it >> 1)];
             looked(t0 + (it >> 1), ks, a.vs[kt0 + t0 + (it >> 1)], sk, sv, step);
@@ -728,7 +728,7 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
                     for (int e = 0; e < 16; e++) x[e] = tanh_any(x[e]);
                 }
             }
-            const float fx = u.icap != 0.0f ? u.capl2 : u.cl2 * cs, mu = 4.0f * (float)step - m;
+            const float fx = u.icap != 0.0f ? u.capl2 : u.cl2 * cs, mu = 4.0f * (float)step + m;
             const float gap0 = (float)(pos - j0 - 4 * g);
             float top = 0.0f;
 #pragma unroll
@@ -771,7 +771,7 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
         buf ^= 1;
     }
     if (rr > last) return;
-    const float f = u.scale * pow2(ek);
+    const float f = u.scale * pow2(ek - kLift);
     float *to = p.dq + tok * p.lddq + (int64_t)row.h * u.d;
 #pragma unroll
     for (int n = 0; n < ND; n++)

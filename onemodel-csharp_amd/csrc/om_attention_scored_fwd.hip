@@ -13,7 +13,6 @@ using namespace osc;
 
 constexpr float kInf = __builtin_inff();
 constexpr int kRows = 128;      // rows of a workgroup
-constexpr float kLift = 12.0f;  // weights are kept as 2^kLift times themselves, so that their split's m is normal fp16
 constexpr float kSlack = 2.0f;  // how far a maximum may outgrow m before m moves
 constexpr int kListed = 256;    // blocks of keys whose step data stands in LDS
 
@@ -262,11 +261,12 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
     __syncthreads();
 
     const int steps = (t1 - t0 + 1) * (kBlock / KT);
+    const bool dense = !u.qd && !(u.window && pre > 0);  // no gaps in what is seen
     auto next = [&](int it) {  // the next step with a key that some row may see
         for (it++; it < steps; it++) {
             const int t = it * KT / kBlock;
             if (t0 * kBlock + it * KT > hi) return steps;
-            if (t >= kListed || visit[t]) return it;
+            if (dense || t >= kListed || visit[t]) return it;
         }
         return steps;
     };
@@ -311,8 +311,8 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
         if (ti < kListed) {
             ksc = kscale[ti];
             vst = vstep[ti];
-            dlo = __builtin_amdgcn_readfirstlane(docs_lo[ti]);
-            dhi = __builtin_amdgcn_readfirstlane(docs_hi[ti]);
+            dlo = u.qd ? __builtin_amdgcn_readfirstlane(docs_lo[ti]) : 0;
+            dhi = u.qd ? __builtin_amdgcn_readfirstlane(docs_hi[ti]) : 0;
         } else {
             const Stats ks = a.ks[kt0 + t0 + ti];
             looked(t0 + ti, ks, a.vs[kt0 + t0 + ti], ksc, vst);
@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
 #pragma unroll
                 for (int n = 0; n < ND; n++) acc[n] *= al;
             }
-            const float lift = kLift + 4.0f * (float)vst, mu = (m == -kInf ? 0.0f : -m) + lift;
+            const float lift = (float)kLift + 4.0f * (float)vst, mu = (m == -kInf ? 0.0f : -m) + lift;
             float sum = 0.0f;
 #pragma unroll
             for (int e = 0; e < 16; e++) {
@@ -415,7 +415,7 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
     l = pair_sum(l);
     if (rr > last) return;
     const int64_t all = (int64_t)u.B * u.Hk * rows, at = (int64_t)item * rows + rr;
-    const float mu = m == -kInf ? 0.0f : m, rl = l == 0.0f ? 0.0f : 1.0f / l, unlift = pow2(-(int)kLift);
+    const float mu = m == -kInf ? 0.0f : m, rl = l == 0.0f ? 0.0f : 1.0f / l, unlift = pow2(-kLift);
     const float wgt = a.part ? pow2(ev) * unlift : pow2(ev) * rl;
     float *to = a.part ? a.part + ((int64_t)split * all + at) * u.d : p.out + tok * p.ldo + (int64_t)row.h * u.d;
 #pragma unroll
@@ -441,7 +441,7 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
         } else if (p.stats) {
             const int64_t sr = stat_at(u, b, row);
             p.stats[sr] = mu;
-            p.stats[all + sr] = l == 0.0f ? 0.0f : rl * pow2((int)kLift);
+            p.stats[all + sr] = l == 0.0f ? 0.0f : rl * pow2(kLift);
         }
     }
 }
@@ -456,8 +456,10 @@ om_status fwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p, int *joins, f
     const int nt = (u.lk + kBlock - 1) / kBlock, rows = u.G * u.lq, blocks = (rows + kRows - 1) / kRows;
     const int64_t items = (int64_t)u.B * u.Hk, wgs = items * blocks, all = items * rows;
     const int dp = u.d <= 32 ? 32 : u.d <= 64 ? 64 : u.d <= 96 ? 96 : 128;
-    // Split the keys while the chip has fewer than two workgroups per CU, in pieces of at least four blocks.
-    int64_t ns = wgs >= 2 * ctx->num_cus ? 1 : 2 * ctx->num_cus / wgs;
+    // Split the keys into pieces of at least four blocks until there are twice the workgroups that the chip holds at once
+    // (their lengths differ under a causal rule, and the short ones fill up behind the long ones).
+    const int64_t want = 2 * (dp == 32 ? 4 : dp == 64 ? 3 : 2) * (int64_t)ctx->num_cus;
+    int64_t ns = wgs >= want ? 1 : want / wgs;
     ns = ns > nt / 4 ? nt / 4 : ns;
     ns = ns < 1 ? 1 : ns;
     const int per = (int)((nt + ns - 1) / ns);

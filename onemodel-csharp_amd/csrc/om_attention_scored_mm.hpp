@@ -54,11 +54,17 @@ __device__ __forceinline__ bool in_range(uint32_t top) { return top == 0 || (top
 // or two.
 __device__ __forceinline__ bool even_rows(uint32_t top, uint32_t low) { return top == 0 || (top >> 23) - (low >> 23) <= 14; }
 
-// Two values split into packed fp16 pairs.
+// Two values split into packed fp16 pairs: a packed conversion, the two remainders with the halves taken as they lie
+// (v_fma_mix_f32 reads either half of a register as fp16), a packed conversion. Left to itself the compiler converts each
+// value a second time to get its half alone: eight instructions where four do.
 __device__ __forceinline__ void split2(float a, float b, uint32_t &h, uint32_t &m) {
     const half2 hh = {(_Float16)a, (_Float16)b};
     h = __builtin_bit_cast(uint32_t, hh);
-    const half2 mm = {(_Float16)__builtin_fmaf((float)hh[0], -1.0f, a), (_Float16)__builtin_fmaf((float)hh[1], -1.0f, b)};
+    asm("" : "+v"(h));
+    float ra, rb;
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(ra) : "v"(h), "v"(a));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rb) : "v"(h), "v"(b));
+    const half2 mm = {(_Float16)ra, (_Float16)rb};
     m = __builtin_bit_cast(uint32_t, mm);
 }
 // Eight values as one lane's part of a fragment.

@@ -153,7 +153,7 @@ __device__ __forceinline__ void split_keys(const Rule &u, const float *src, int6
 
 // What the backward keeps of its rows (queries of one head): a record of 1 KB per 32 rows, a value of all 32 after another.
 enum {
-    kRowM,      // the forward's reference exponent; kNoRow for a row that has nothing to give (its weights become 0)
+    kRowM,      // kLift less the forward's reference exponent; -kNoRow for a row that has nothing to give (its weights become 0)
     kRowDelta,  // g . o times 2^-re, re the exponent of g's row scale
     kRowPos,    // position (int)
     kRowSlope,  // slope of its head, in log2 units
@@ -177,6 +177,7 @@ struct RowsOut {
 };
 constexpr uint32_t kWideMost = (127u + 100) << 23, kWideLeast = (127u - 100) << 23;
 constexpr float kNoRow = 3e38f;
+constexpr int kLift = 12;  // weights are kept as 2^kLift times themselves, so that their split's second half is normal fp16
 
 // Block t of the rows of (b, hk) for the backward.
 template <int DP, bool VEC>
@@ -222,7 +223,7 @@ __device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, 
         w[i] = gt[i] && fine ? rl[i] * pow2(re) : 0.0f;
         delta[i] = fine ? dot * pow2(-re) : 0.0f;
         bad = bad || !fine || (on && !(__builtin_fabsf(m[i]) < 1e30f && rl[i] > 0.0f && rl[i] < 1e30f && __builtin_fabsf(dot) < 1e38f));
-        if (!on) m[i] = kNoRow;
+        m[i] = on ? (float)kLift - m[i] : -kNoRow;
         if ((threadIdx.x & 15) == 0) {
             const int64_t r = at * kBlock + 4 * (threadIdx.x >> 4) + i;
             o.v[row_value(r, kRowM)] = m[i];
