@@ -29,8 +29,8 @@ struct BwdArgs {
     const RowStats *rs;
     int nt, nr;                      // blocks of 64 keys and rows of a head
     int kblocks, rblocks;            // workgroups along them
-    int nsplit, per;                 // splits of the rows for dk and dv, blocks of 64 rows in each
-    int first_rows;                  // workgroups of the first role
+    int nsplit;                      // splits of each block of keys' rows for dk and dv
+    int keys_wgs;                    // workgroups of the first role
     float *part;                     // [split][B Hk][lk][2][d] (dk, dv), NULL for one split
 };
 
@@ -251,7 +251,8 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
     auto &llo = t_.lo;
     auto &lhi = t_.hi;
     auto &red = t_.red;
-    const int kb = i % a.kblocks, split = (i / a.kblocks) % a.nsplit, item = i / (a.kblocks * a.nsplit);
+    const Place pl = place_of(i, u.B * u.Hk);
+    const int item = pl.item, split = pl.block % a.nsplit, kb = pl.block / a.nsplit;
     const int b = item / u.Hk, hk = item - b * u.Hk, rows = u.G * u.lq;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
     const int pre = u.prefix ? u.prefix[b] : 0;
@@ -276,10 +277,12 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
     // the blocks of rows that may see them
     int plo, phi;
     pos_range(u, first, last, pre, plo, phi);
-    int r0 = max((plo - u.off) * u.G, split * a.per * kBlock);
-    int r1 = min((phi - u.off + 1) * u.G, (int)min((int64_t)rows, (int64_t)(split + 1) * a.per * kBlock));  // one past
-    if (phi < plo) r1 = r0;
-    const int t0 = r0 / kBlock, t1 = r1 <= r0 ? t0 - 1 : (r1 - 1) / kBlock;
+    int r0 = (plo - u.off) * u.G, r1 = phi < plo ? r0 : (phi - u.off + 1) * u.G;  // one past the last
+    // this split's share of them, in blocks: equal shares
+    const int c0 = r0 / kBlock, c1 = r1 <= r0 ? c0 - 1 : (r1 - 1) / kBlock, per = (c1 - c0 + a.nsplit) / a.nsplit;
+    const int t0 = c0 + split * per, t1 = min(c1, t0 + per - 1);
+    r0 = max(r0, t0 * kBlock);
+    r1 = max(r0, min(r1, (t1 + 1) * kBlock));
     uint32_t gt = 0, gl = 0xFFFFFFFFu, qt = 0, ql = 0xFFFFFFFFu;
     auto looked = [&](int rt, const RowStats &r, RowStep &st) {
         st.q = r.q;
@@ -549,7 +552,8 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
     auto &llo = t_.lo;
     auto &lhi = t_.hi;
     auto &red = t_.red;
-    const int rb = a.rblocks - 1 - i % a.rblocks, item = i / a.rblocks;  // the longest rows of a causal rule first
+    const Place pl = place_of(i, u.B * u.Hk);
+    const int item = pl.item, rb = a.rblocks - 1 - pl.block;
     const int b = item / u.Hk, hk = item - b * u.Hk, rows = u.G * u.lq;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
     const int pre = u.prefix ? u.prefix[b] : 0;
@@ -791,17 +795,11 @@ __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) k_scored_bwd_mm(Rule u,
         KeysTables k;
         RowsTables r;
     } t;
-    int lin = blockIdx.x;
-    // ids are dealt round-robin over the 8 XCDs: the workgroups of one head stay on one
-    if (lin < a.first_rows) {
-        if ((a.first_rows & 7) == 0) lin = (lin & 7) * (a.first_rows >> 3) + (lin >> 3);
-        keys_role<DP>(u, p, a, lin, sh, t.k);
-    } else {
-        const int total = gridDim.x - a.first_rows;
-        lin -= a.first_rows;
-        if ((total & 7) == 0) lin = (lin & 7) * (total >> 3) + (lin >> 3);
-        rows_role<DP>(u, p, a, lin, sh, t.r);
-    }
+    // The roles' workgroups in proportion, each in its order of falling work: the longest of both start first.
+    const int64_t id = blockIdx.x, all = gridDim.x;
+    const int k = (int)(id * a.keys_wgs / all);
+    if ((int)((id + 1) * a.keys_wgs / all) > k) keys_role<DP>(u, p, a, k, sh, t.k);
+    else rows_role<DP>(u, p, a, (int)id - k, sh, t.r);
 }
 
 // dk and dv from the splits' sums, in split order; a thread per value.
@@ -838,12 +836,11 @@ om_status bwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p) {
     if (wk < 2 * ctx->num_cus) ns = 2 * ctx->num_cus / wk;
     ns = ns > a.nr / 8 ? a.nr / 8 : ns;
     ns = ns < 1 ? 1 : ns;
-    a.per = (int)((a.nr + ns - 1) / ns);
-    a.nsplit = (int)((a.nr + a.per - 1) / a.per);
+    a.nsplit = (int)ns;
     wk = keys ? wk * a.nsplit : 0;
     const int64_t wr = p.dq ? items * a.rblocks : 0, jobs = items * (2 * (int64_t)a.nt + a.nr);
     OM_REQUIRE(ctx, wk + wr <= INT32_MAX && jobs <= INT32_MAX, "%s: too many row blocks", what);
-    a.first_rows = (int)wk;
+    a.keys_wgs = (int)wk;
     const int64_t kp = plane_bytes(dp, items * a.nt), rp = plane_bytes(dp, items * a.nr);
     const int64_t vals = items * a.nr * kBlock * kRowValues * (int64_t)sizeof(float);
     const int64_t part = keys && a.nsplit > 1 ? (int64_t)sizeof(float) * a.nsplit * items * u.lk * 2 * u.d : 0;

@@ -114,7 +114,7 @@ struct FwdArgs {
     const Stats *ks, *vs;     // their blocks' statistics
     int nt;                   // blocks of 64 keys of a head
     int blocks;               // workgroups along a head's rows
-    int nsplit, per;          // splits of the keys, blocks of 64 keys in each
+    int nsplit;               // splits of each block of rows' keys
     float *part;              // the splits' sums (om_attention_scored.hip joins them), NULL for one split
     int vec;                  // q's rows are 16-byte aligned
 };
@@ -131,10 +131,8 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
     __shared__ unsigned char visit[kListed];  // whether some row may see the block
     __shared__ int docs_lo[kListed], docs_hi[kListed];
     __shared__ uint32_t red[4][6];
-    int rb, item;
-    on_one_xcd(a.blocks * a.nsplit, rb, item);
-    const int split = rb % a.nsplit;
-    rb = a.blocks - 1 - rb / a.nsplit;  // the longest rows of a causal rule first
+    const Place at = place_of(blockIdx.x, u.B * u.Hk);
+    const int item = at.item, split = at.block % a.nsplit, rb = a.blocks - 1 - at.block / a.nsplit;
     const int b = item / u.Hk, hk = item - b * u.Hk, rows = u.G * u.lq;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
     const int pre = u.prefix ? u.prefix[b] : 0;
@@ -162,9 +160,11 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
     int lo, hi;
     const int i0 = first / u.G + u.off, i1 = last / u.G + u.off;
     key_range(u, i0, i1, pre, lo, hi);
-    lo = max(lo, split * a.per * kBlock);
-    hi = (int)min((int64_t)hi, (int64_t)(split + 1) * a.per * kBlock - 1);
-    const int t0 = lo / kBlock, t1 = hi < lo ? t0 - 1 : hi / kBlock;
+    // this split's share of them, in blocks: equal shares, so that a block of rows is as many equal pieces
+    const int c0 = lo / kBlock, c1 = hi < lo ? c0 - 1 : hi / kBlock, per = (c1 - c0 + a.nsplit) / a.nsplit;
+    const int t0 = c0 + split * per, t1 = min(c1, t0 + per - 1);
+    lo = max(lo, t0 * kBlock);
+    hi = min(hi, t1 * kBlock + kBlock - 1);
     uint32_t ktop = 0, vtop = 0, vlow = 0xFFFFFFFFu;
     const int64_t kt0 = (int64_t)item * a.nt;
     Stats mk = {}, mv = {};
@@ -414,10 +414,10 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
 
     l = pair_sum(l);
     if (rr > last) return;
-    const int64_t all = (int64_t)u.B * u.Hk * rows, at = (int64_t)item * rows + rr;
+    const int64_t all = (int64_t)u.B * u.Hk * rows, out = (int64_t)item * rows + rr;
     const float mu = m == -kInf ? 0.0f : m, rl = l == 0.0f ? 0.0f : 1.0f / l, unlift = pow2(-kLift);
     const float wgt = a.part ? pow2(ev) * unlift : pow2(ev) * rl;
-    float *to = a.part ? a.part + ((int64_t)split * all + at) * u.d : p.out + tok * p.ldo + (int64_t)row.h * u.d;
+    float *to = a.part ? a.part + ((int64_t)split * all + out) * u.d : p.out + tok * p.ldo + (int64_t)row.h * u.d;
 #pragma unroll
     for (int n = 0; n < ND; n++)
 #pragma unroll
@@ -435,7 +435,7 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
         }
     if (g == 0) {
         if (a.part) {
-            float *ms = a.part + (int64_t)a.nsplit * all * u.d + (int64_t)split * all + at;
+            float *ms = a.part + (int64_t)a.nsplit * all * u.d + (int64_t)split * all + out;
             ms[0] = mu;
             ms[(int64_t)a.nsplit * all] = l * unlift;
         } else if (p.stats) {
@@ -462,8 +462,6 @@ om_status fwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p, int *joins, f
     int64_t ns = wgs >= want ? 1 : want / wgs;
     ns = ns > nt / 4 ? nt / 4 : ns;
     ns = ns < 1 ? 1 : ns;
-    const int per = (int)((nt + ns - 1) / ns);
-    ns = (nt + per - 1) / per;
     OM_REQUIRE(ctx, wgs * ns <= INT32_MAX && 2 * items * nt <= INT32_MAX, "om_attention_fwd_scored: too many row blocks");
     const int64_t plane = plane_bytes(dp, items * nt), stats = items * nt * (int64_t)sizeof(Stats);
     const int64_t join = ns > 1 ? (int64_t)sizeof(float) * ns * all * (u.d + 2) : 0;
@@ -478,7 +476,6 @@ om_status fwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p, int *joins, f
     a.nt = nt;
     a.blocks = blocks;
     a.nsplit = (int)ns;
-    a.per = per;
     a.part = ns > 1 ? reinterpret_cast<float *>(base + 2 * plane + 2 * stats) : nullptr;
     auto al16 = [](const void *x) { return ((uintptr_t)x & 15) == 0; };
     a.vec = u.d % 4 == 0 && p.ldq % 4 == 0 && al16(p.q);
