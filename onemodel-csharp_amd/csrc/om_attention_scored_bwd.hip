@@ -24,7 +24,7 @@ constexpr int kListed = 256; // blocks whose step data stands in LDS
 struct BwdArgs {
     const char *kn, *kt, *vn;        // K in both forms, V in rows form
     const char *qn, *gn, *g2, *q2;   // RowsOut
-    const float *v;
+    const float *v, *keys;           // the rows' records and the steps' words of the keys
     const Stats *ks, *vs;
     const RowStats *rs;
     int nt, nr;                      // blocks of 64 keys and rows of a head
@@ -212,45 +212,17 @@ __device__ __forceinline__ void put4(float *to, int c, int d, floatx4 v, int acc
     }
 }
 
-// Whether some of positions i0 .. i1 may see some of keys j0 .. j1, documents aside.
-__device__ __forceinline__ bool may_see(const Rule &u, int i0, int i1, int j0, int j1, int pre) {
-    return j0 < pre || (!(u.causal && j0 > i1) && !(u.window && (i0 - j1 >= u.window || j0 - i1 >= u.window)));
-}
-// Whether all of positions i0 .. i1 see all of keys j0 .. j1, documents aside.
-__device__ __forceinline__ bool all_see(const Rule &u, int i0, int i1, int j0, int j1, int pre) {
-    return j1 < pre || ((!u.causal || j1 <= i0) && (!u.window || (i1 - j0 < u.window && j1 - i0 < u.window)));
-}
-
 // ---------------------------------------------------------------------------------------------------- dk and dv
-// The step data of a block of rows: its scales and whether it is visited.
-struct RowStep {
-    float q, g2, q2;
-    int see, dlo, dhi;
-};
-// Either role's tables in LDS, by blocks of the other side: scales, whether the block is visited, its documents.
-struct KeysTables {
-    float q[kListed], g2[kListed], q2[kListed];
-    int lo[kListed], hi[kListed];
+// Either role's tables in LDS, by blocks of the other side: whether the block is visited (documents).
+struct Tables {
     uint32_t red[4][5];
     unsigned char see[kListed];
 };
-struct RowsTables {
-    float k[kListed], v[kListed];
-    int lo[kListed], hi[kListed];
-    uint32_t red[4][3];
-    signed char step[kListed];
-    unsigned char see[kListed];
-};
-template <int DP>
-__device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const BwdArgs &a, int i, char *sh, KeysTables &t_) {
+template <int DP, int PARTS>
+__device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const BwdArgs &a, int i, char *sh, Tables &tab) {
+    constexpr bool DOCS = PARTS & kDocs, CAP = PARTS & kCap, SLOPES = PARTS & kSlopes;
     constexpr int S = DP / 16, ND = DP / 32, HALF = kStep * DP * 4, STAGE = 4 * HALF + 1024;  // the rows' record last
-    auto &lq_ = t_.q;
-    auto &lg2 = t_.g2;
-    auto &lq2 = t_.q2;
-    auto &lsee = t_.see;
-    auto &llo = t_.lo;
-    auto &lhi = t_.hi;
-    auto &red = t_.red;
+    auto &red = tab.red;
     const Place pl = place_of(i, u.B * u.Hk);
     const int item = pl.item, split = pl.block % a.nsplit, kb = pl.block / a.nsplit;
     const int b = item / u.Hk, hk = item - b * u.Hk, rows = u.G * u.lq;
@@ -259,7 +231,7 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
     const int first = kb * kKeys, last = min(first + kKeys, u.lk) - 1;
     const int j = first + 32 * w + (lane & 31);
     const bool live = first + 32 * w <= last;
-    const int kd = j <= last ? (u.kd ? u.kd[(int64_t)b * u.lk + j] : 0) : -1;
+    const int kd = j <= last ? (DOCS ? u.kd[(int64_t)b * u.lk + j] : 0) : -1;
     const int64_t kt0 = (int64_t)item * a.nt, rt0 = (int64_t)item * a.nr;
     // the wavefront's block of keys (a wavefront past the last key repeats it and stores nothing)
     const int t = min((first + 32 * w) / kBlock, a.nt - 1);
@@ -270,7 +242,7 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
     const int kdlo = min(k0.doc_lo, k1.doc_lo), kdhi = max(k0.doc_hi, k1.doc_hi);
     // documents of the wavefront's own keys (those past the last one aside)
     int wlo = 0, whi = 0;
-    if (u.qd) {
+    if (DOCS) {
         wlo = __builtin_amdgcn_readfirstlane(wave_imin(j <= last ? kd : INT32_MAX));
         whi = __builtin_amdgcn_readfirstlane(wave_imax(j <= last ? kd : INT32_MIN));
     }
@@ -284,34 +256,19 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
     r0 = max(r0, t0 * kBlock);
     r1 = max(r0, min(r1, (t1 + 1) * kBlock));
     uint32_t gt = 0, gl = 0xFFFFFFFFu, qt = 0, ql = 0xFFFFFFFFu;
-    auto looked = [&](int rt, const RowStats &r, RowStep &st) {
-        st.q = r.q;
-        st.g2 = r.g2;
-        st.q2 = r.q2;
-        const int f = rt * kBlock, l = min(f + kBlock, rows) - 1;
-        st.see = may_see(u, f / u.G + u.off, l / u.G + u.off, first, last, pre);
-        st.dlo = r.doc_lo;
-        st.dhi = r.doc_hi;
-        if (u.qd && (r.doc_hi < kdlo || r.doc_lo > kdhi || r.doc_hi < 0)) st.see = 0;
-        if (r.g2_top == 0 && r.q2_top == 0) st.see = 0;  // rows without gradient
-    };
-    for (int rt = t0 + (int)threadIdx.x; rt <= t1; rt += 256) {
-        RowStep st;
+    RowStats mine = {};  // the thread's first
+    for (int rt = t0 + (int)threadIdx.x, n = 0; rt <= t1; rt += 256, n++) {
         const RowStats r = a.rs[rt0 + rt];
-        looked(rt, r, st);
+        if (n == 0) mine = r;
         bad = bad || r.bad;
         gt = max(gt, r.g2_top);
         qt = max(qt, r.q2_top);
         if (r.g2_top) gl = min(gl, r.g2_top);
         if (r.q2_top) ql = min(ql, r.q2_top);
-        if (rt - t0 < kListed) {
-            lq_[rt - t0] = st.q;
-            lg2[rt - t0] = st.g2;
-            lq2[rt - t0] = st.q2;
-            lsee[rt - t0] = (unsigned char)st.see;
-            llo[rt - t0] = st.dlo;
-            lhi[rt - t0] = st.dhi;
-        }
+    }
+    if (DOCS && t0 + (int)threadIdx.x <= t1) {
+        static_assert(kListed == 256, "a thread's first block is its entry");
+        tab.see[threadIdx.x] = mine.doc_hi >= max(kdlo, 0) && mine.doc_lo <= kdhi && (mine.g2_top || mine.q2_top);
     }
     gt = wave_umax(gt);
     qt = wave_umax(qt);
@@ -369,16 +326,14 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
         for (int e = 0; e < 16; e++) dk[n][e] = dv[n][e] = 0.0f;
     float g2cur = 1.0f, q2cur = 1.0f;
     int sd = kNoScale;  // dk's sums are in units of 2^sd
-    const int steps = (t1 - t0 + 1) * 2;
+    const int base = t0 * kBlock, steps = r1 <= r0 ? 0 : (r1 - 1 - base) / kStep + 1;
     auto next = [&](int it) {
-        for (it++; it < steps; it++) {
-            const int f = t0 * kBlock + it * kStep;
-            if (f >= r1) return steps;
-            if (f + kStep <= r0) continue;
-            if ((it >> 1) >= kListed || lsee[it >> 1]) return it;
-        }
-        return steps;
+        it++;
+        if (DOCS)
+            while (it < steps && it / 2 < kListed && !tab.see[it / 2]) it++;
+        return it < steps ? it : steps;
     };
+    const RowBand band(u, first + 32 * w, min(first + 32 * w + 31, last), pre);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)(sh + 256);
     auto stage = [&](int it, int buf) {
         const int64_t off = (rt0 + t0) * plane_bytes(DP, 1) + (int64_t)it * HALF + lane * 16;
@@ -394,40 +349,38 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
         one(a.q2, 3);
         if (w == 0) load_to_lds(a.v + row_value((rt0 + t0) * kBlock + (int64_t)it * kStep, 0) + 4 * lane, to + 4 * HALF);
     };
-    int it = next(-1), buf = 0;
+    int it = next((r0 - base) / kStep - 1), buf = 0;
     if (it < steps) stage(it, 0);
     while (it < steps) {
         land<0>();
         const int nx = next(it);
         if (nx < steps) stage(nx, buf ^ 1);
-        RowStep st;
-        if ((it >> 1) < kListed) {
-            st.q = lq_[it >> 1];
-            st.g2 = lg2[it >> 1];
-            st.q2 = lq2[it >> 1];
-            st.dlo = u.qd ? __builtin_amdgcn_readfirstlane(llo[it >> 1]) : 0;
-            st.dhi = u.qd ? __builtin_amdgcn_readfirstlane(lhi[it >> 1]) : 0;
-        } else {
-            looked(t0 + (it >> 1), a.rs[rt0 + t0 + (it >> 1)], st);
+        const int f0 = base + it * kStep, f1 = f0 + kStep - 1;
+        const char *qf = sh + 256 + buf * STAGE + lane * 16, *gf = qf + HALF, *g2f = gf + HALF, *q2f = g2f + HALF;
+        const float *rec = reinterpret_cast<const float *>(sh + 256 + buf * STAGE + 4 * HALF), *rv = rec + 4 * g;
+        const float *blk = rec + 32 * kRowBlock;
+        bool some = live & band.some(f0, f1), one = true;
+        if (DOCS) {
+            const int dlo = __builtin_amdgcn_readfirstlane(__float_as_int(blk[3]));
+            const int dhi = __builtin_amdgcn_readfirstlane(__float_as_int(blk[4]));
+            some = some & (whi >= 0) & (dhi >= wlo) & (dlo <= whi);
+            one = (wlo == whi) & (dlo == dhi) & (dlo == wlo) & (wlo >= 0);
         }
-        const int f0 = t0 * kBlock + it * kStep, f1 = min(f0 + kStep, rows) - 1;
-        const int i0 = f0 / u.G + u.off, i1 = f1 / u.G + u.off;
-        const int j0 = first + 32 * w, j1 = min(j0 + 31, last);
-        if (live && !(u.qd && (whi < 0 || st.dhi < wlo || st.dlo > whi)) && may_see(u, i0, i1, j0, j1, pre)) {
-            if (st.g2 != g2cur) {
-                const float c = g2cur / st.g2;
+        if (some) {
+            const float sq = blk[0], sg2 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(blk[1]))),
+                        sq2 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(blk[2])));
+            if (sg2 != g2cur) {
+                const float c = g2cur / sg2;
 #pragma unroll
                 for (int n = 0; n < ND; n++) dv[n] *= c;
-                g2cur = st.g2;
+                g2cur = sg2;
             }
-            if (st.q2 != q2cur) {
-                const float c = q2cur / st.q2;
+            if (sq2 != q2cur) {
+                const float c = q2cur / sq2;
 #pragma unroll
                 for (int n = 0; n < ND; n++) dk[n] *= c;
-                q2cur = st.q2;
+                q2cur = sq2;
             }
-            const char *qf = sh + 256 + buf * STAGE + lane * 16, *gf = qf + HALF, *g2f = gf + HALF, *q2f = g2f + HALF;
-            const float *rv = reinterpret_cast<const float *>(sh + 256 + buf * STAGE + 4 * HALF) + 4 * g;
             floatx16 x, dp;
 #pragma unroll
             for (int e = 0; e < 16; e++) x[e] = dp[e] = 0.0f;
@@ -438,10 +391,9 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
                 dp = mma3(*reinterpret_cast<const u32x4 *>(gf + (2 * s) * 1024),
                           *reinterpret_cast<const u32x4 *>(gf + (2 * s + 1) * 1024), vh[s], vm[s], dp);
             }
-            const float cs = st.q * ks.scale;
-            const bool one = !u.qd || (wlo == whi && st.dlo == st.dhi && st.dlo == wlo && wlo >= 0);
-            const bool whole = one && all_see(u, i0, i1, j0, j1, pre);
-            if (u.icap != 0.0f) {
+            const float cs = sq * ks.scale;
+            const bool whole = band.all(f0, f1) & one;
+            if (CAP) {
                 const float ic = u.icap * cs;
                 float big = 0.0f;
 #pragma unroll
@@ -457,7 +409,7 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
                     for (int e = 0; e < 16; e++) x[e] = tanh_any(x[e]);
                 }
             }
-            const float fx = u.icap != 0.0f ? u.capl2 : u.cl2 * cs;
+            const float fx = CAP ? u.capl2 : u.cl2 * cs;
             float top = 0.0f;
 #pragma unroll
             for (int q = 0; q < 4; q++) {
@@ -466,16 +418,16 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
                 floatx4 y;
 #pragma unroll
                 for (int r = 0; r < 4; r++) y[r] = __builtin_fmaf(x[4 * q + r], fx, m4[r]);
-                if (u.slopes || !whole) {
+                if (SLOPES || !whole) {
                     const intx4 p4 = *reinterpret_cast<const intx4 *>(rv + 32 * kRowPos + 8 * q);
-                    if (u.slopes) {
+                    if (SLOPES) {
                         const floatx4 s4 = *reinterpret_cast<const floatx4 *>(rv + 32 * kRowSlope + 8 * q);
 #pragma unroll
                         for (int r = 0; r < 4; r++) y[r] = __builtin_fmaf(-s4[r], __builtin_fabsf((float)(p4[r] - j)), y[r]);
                     }
                     if (!whole) {
                         intx4 qd = {kd, kd, kd, kd};
-                        if (!one) qd = *reinterpret_cast<const intx4 *>(rv + 32 * kRowDoc + 8 * q);
+                        if (DOCS) qd = *reinterpret_cast<const intx4 *>(rv + 32 * kRowDoc + 8 * q);
 #pragma unroll
                         for (int r = 0; r < 4; r++) y[r] = (reach.has(p4[r]) & (qd[r] == kd)) ? y[r] : -3e38f;
                     }
@@ -485,7 +437,7 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
                     const int e = 4 * q + r;
                     const float ex = exp2_hw(y[r]);
                     float ds = ex * __builtin_fmaf(dp[e], vs.scale, -d4[r]);
-                    if (u.icap != 0.0f) ds *= __builtin_fmaf(-x[e], x[e], 1.0f);
+                    if (CAP) ds *= __builtin_fmaf(-x[e], x[e], 1.0f);
                     dp[e] = ds;
                     x[e] = ex;
                     top = fmaxf(top, __builtin_fabsf(ds));
@@ -542,16 +494,11 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
 }
 
 // ------------------------------------------------------------------------------------------------------------ dq
-template <int DP>
-__device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const BwdArgs &a, int i, char *sh, RowsTables &t_) {
-    constexpr int S = DP / 16, ND = DP / 32, HALF = kStep * DP * 4, STAGE = 3 * HALF + 128;  // the keys' documents last
-    auto &lk_ = t_.k;
-    auto &lv_ = t_.v;
-    auto &lstep = t_.step;
-    auto &lsee = t_.see;
-    auto &llo = t_.lo;
-    auto &lhi = t_.hi;
-    auto &red = t_.red;
+template <int DP, int PARTS>
+__device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const BwdArgs &a, int i, char *sh, Tables &tab) {
+    constexpr bool DOCS = PARTS & kDocs, CAP = PARTS & kCap, SLOPES = PARTS & kSlopes;
+    constexpr int S = DP / 16, ND = DP / 32, HALF = kStep * DP * 4, STAGE = 3 * HALF + 4 * kKeyWords;  // the step's words last
+    auto &red = tab.red;
     const Place pl = place_of(i, u.B * u.Hk);
     const int item = pl.item, rb = a.rblocks - 1 - pl.block;
     const int b = item / u.Hk, hk = item - b * u.Hk, rows = u.G * u.lq;
@@ -561,8 +508,8 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
     const int rr = first + 32 * w + (lane & 31);
     const Row row = row_of(u, hk, min(rr, rows - 1));
     const int64_t tok = (int64_t)b * u.lq + row.t;
-    const int pos = row.t + u.off, doc = u.qd ? u.qd[tok] : 0;
-    const float slope = u.slopes ? u.slopes[row.h] * kLog2e : 0.0f;
+    const int pos = row.t + u.off, doc = DOCS ? u.qd[tok] : 0;
+    const float slope = SLOPES ? u.slopes[row.h] * kLog2e : 0.0f;
     const bool live = first + 32 * w <= last;
     const int64_t kt0 = (int64_t)item * a.nt, rt0 = (int64_t)item * a.nr;
     const int rt = min((first + 32 * w) / kBlock, a.nr - 1);
@@ -605,32 +552,17 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
     }
     const int ek = kt ? scale_exp(kt) : 0;
     int wlo = 0, whi = 0;  // documents of the wavefront's rows
-    if (u.qd) {
+    if (DOCS) {
         wlo = __builtin_amdgcn_readfirstlane(wave_imin(doc));
         whi = __builtin_amdgcn_readfirstlane(wave_imax(doc));
     }
-    auto looked = [&](int t, const Stats &ks, const Stats &vs, float &sk, float &sv, int &step) -> int {
-        sk = ks.scale;
-        sv = vs.scale;
-        step = ks.top ? ((int)(__float_as_uint(ks.scale) >> 23) - 127 - ek) / 4 : 0;
-        const int j0 = t * kBlock, j1 = j0 + kBlock - 1;
-        int see = may_see(u, i0, i1, j0, j1, pre);
-        if (u.qd && (ks.doc_hi < 0 || ks.doc_hi < qlo || ks.doc_lo > qhi)) see = 0;
-        return see;
-    };
-    if (t0 + (int)threadIdx.x <= t1) {
-        static_assert(kListed == 256, "a thread's first block is its entry");
-        float sk, sv;
-        int step;
-        const int see = looked(t0 + threadIdx.x, mk, mv, sk, sv, step);
-        llo[threadIdx.x] = mk.doc_lo;
-        lhi[threadIdx.x] = mk.doc_hi;
-        lk_[threadIdx.x] = sk;
-        lv_[threadIdx.x] = sv;
-        lstep[threadIdx.x] = (signed char)step;
-        lsee[threadIdx.x] = (unsigned char)see;
+    if (DOCS) {
+        if (t0 + (int)threadIdx.x <= t1) {
+            static_assert(kListed == 256, "a thread's first block is its entry");
+            tab.see[threadIdx.x] = mk.doc_hi >= max(qlo, 0) && mk.doc_lo <= qhi;
+        }
+        __syncthreads();
     }
-    __syncthreads();
     // Q and G fragments of the wavefront's rows, and their values
     u32x4 qh[S], qm[S], gh[S], gm[S];
     {
@@ -655,14 +587,15 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
 #pragma unroll
         for (int e = 0; e < 16; e++) dq[n][e] = 0.0f;
     const int wi0 = min(first + 32 * w, last) / u.G + u.off, wi1 = min(first + 32 * w + 31, last) / u.G + u.off;
-    const int steps = (t1 - t0 + 1) * 2;
-    const bool dense = !u.qd && !(u.window && pre > 0);  // no gaps in what is seen
+    const int base = t0 * kBlock, steps = hi < lo ? 0 : (hi - base) / kStep + 1;
+    const Band whole_wg(u, i0, i1, pre), mine(u, wi0, wi1, pre);
     auto next = [&](int it) {
-        for (it++; it < steps; it++) {
-            if (t0 * kBlock + it * kStep > hi) return steps;
-            if (dense || (it >> 1) >= kListed || lsee[it >> 1]) return it;
-        }
-        return steps;
+        it++;
+        const int j0 = base + it * kStep;  // a window leaves a gap behind a prefix
+        if ((j0 >= whole_wg.pre) & (j0 + kStep <= whole_wg.some0)) it = (whole_wg.some0 - base) / kStep;
+        if (DOCS)
+            while (it < steps && it / 2 < kListed && !tab.see[it / 2]) it++;
+        return it < steps ? it : steps;
     };
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)(sh + 256);
     auto stage = [&](int it, int buf) {
@@ -676,8 +609,7 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
         one(a.kn, 0);
         one(a.vn, 1);
         one(a.kt, 2);
-        if (u.kd && threadIdx.x < kStep)
-            load_to_lds4(u.kd + (int64_t)b * u.lk + min(t0 * kBlock + it * kStep + lane, u.lk - 1), to + 3 * HALF);
+        if (w == 0) load_to_lds4(a.keys + (2 * (kt0 + t0) + it) * kKeyWords + lane, to + 3 * HALF);
     };
     int it = next(-1), buf = 0;
     if (it < steps) stage(it, 0);
@@ -685,24 +617,19 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
         land<0>();
         const int nx = next(it);
         if (nx < steps) stage(nx, buf ^ 1);
-        float sk, sv;
-        int step, dlo, dhi;
-        if ((it >> 1) < kListed) {
-            sk = lk_[it >> 1];
-            sv = lv_[it >> 1];
-            step = lstep[it >> 1];
-            dlo = u.qd ? __builtin_amdgcn_readfirstlane(llo[it >> 1]) : 0;
-            dhi = u.qd ? __builtin_amdgcn_readfirstlane(lhi[it >> 1]) : 0;
-        } else {
-            const Stats ks = a.ks[kt0 + t0 + (it >> 1)];
-            looked(t0 + (it >> 1), ks, a.vs[kt0 + t0 + (it >> 1)], sk, sv, step);
-            dlo = ks.doc_lo;
-            dhi = ks.doc_hi;
+        const int j0 = base + it * kStep, j1 = j0 + kStep - 1;
+        const char *kf = sh + 256 + buf * STAGE + lane * 16, *vf = kf + HALF, *ktf = vf + HALF;
+        const int *words = reinterpret_cast<const int *>(sh + 256 + buf * STAGE + 3 * HALF);
+        bool some = live & mine.some(j0, j1), one = true;
+        if (DOCS) {
+            const int dlo = __builtin_amdgcn_readfirstlane(words[kKeyDocLo]), dhi = __builtin_amdgcn_readfirstlane(words[kKeyDocHi]);
+            some = some & (whi >= 0) & (dhi >= wlo) & (dlo <= whi);
+            one = (wlo == whi) & (dlo == dhi) & (dlo == wlo) & (wlo >= 0);
         }
-        const int j0 = t0 * kBlock + it * kStep, j1 = j0 + kStep - 1;
-        if (live && !(u.qd && (whi < 0 || dhi < wlo || dlo > whi)) && may_see(u, wi0, wi1, j0, j1, pre)) {
-            const char *kf = sh + 256 + buf * STAGE + lane * 16, *vf = kf + HALF, *ktf = vf + HALF;
-            const int *kdoc = reinterpret_cast<const int *>(sh + 256 + buf * STAGE + 3 * HALF) + 4 * g;
+        if (some) {
+            const float sk = __int_as_float(words[kKeyScaleK]), sv = __int_as_float(words[kKeyScaleV]);
+            // K's exponent less the largest; a block of zeros may say anything
+            const int step = min(max((words[kKeyScaleK] >> 23) - 127 - ek, -32), 0);
             floatx16 x, dp;
 #pragma unroll
             for (int e = 0; e < 16; e++) x[e] = dp[e] = 0.0f;
@@ -714,9 +641,8 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
                           *reinterpret_cast<const u32x4 *>(vf + (2 * s + 1) * 1024), gh[s], gm[s], dp);
             }
             const float cs = rs.q * sk;
-            const bool one = !u.qd || (wlo == whi && dlo == dhi && dlo == wlo && dlo >= 0);
-            const bool whole = j1 < u.lk && one && all_see(u, wi0, wi1, j0, j1, pre);
-            if (u.icap != 0.0f) {
+            const bool whole = mine.all(j0, j1) & one;
+            if (CAP) {
                 const float ic = u.icap * cs;
                 float big = 0.0f;
 #pragma unroll
@@ -732,17 +658,17 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
                     for (int e = 0; e < 16; e++) x[e] = tanh_any(x[e]);
                 }
             }
-            const float fx = u.icap != 0.0f ? u.capl2 : u.cl2 * cs, mu = 4.0f * (float)step + m;
+            const float fx = CAP ? u.capl2 : u.cl2 * cs, mu = (float)step + m;
             const float gap0 = (float)(pos - j0 - 4 * g);
             float top = 0.0f;
 #pragma unroll
             for (int e = 0; e < 16; e++) {
                 float y = __builtin_fmaf(x[e], fx, mu);
                 const int o = 8 * (e >> 2) + (e & 3);
-                if (u.slopes) y = __builtin_fmaf(-slope, __builtin_fabsf(gap0 - (float)o), y);
-                if (!whole) y = (reach.has(j0 + 4 * g + o) & (one || kdoc[o] == doc)) ? y : -3e38f;
+                if (SLOPES) y = __builtin_fmaf(-slope, __builtin_fabsf(gap0 - (float)o), y);
+                if (!whole) y = (reach.has(j0 + 4 * g + o) & (!DOCS || words[kKeyDoc + 4 * g + o] == doc)) ? y : -3e38f;
                 float ds = exp2_hw(y) * __builtin_fmaf(dp[e], sv, -delta);
-                if (u.icap != 0.0f) ds *= __builtin_fmaf(-x[e], x[e], 1.0f);
+                if (CAP) ds *= __builtin_fmaf(-x[e], x[e], 1.0f);
                 dp[e] = ds;
                 top = fmaxf(top, __builtin_fabsf(ds));
             }
@@ -787,19 +713,16 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
         }
 }
 
-template <int DP>
+template <int DP, int PARTS>
 __global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) k_scored_bwd_mm(Rule u, Ptrs p, BwdArgs a) {
     OM_LDS_POISON();
     __shared__ __attribute__((aligned(16))) char sh[256 + 2 * (4 * kStep * DP * 4 + 1024)];  // no stage at LDS address 0
-    __shared__ __attribute__((aligned(16))) union {
-        KeysTables k;
-        RowsTables r;
-    } t;
+    __shared__ Tables tab;
     // The roles' workgroups in proportion, each in its order of falling work: the longest of both start first.
     const int64_t id = blockIdx.x, all = gridDim.x;
     const int k = (int)(id * a.keys_wgs / all);
-    if ((int)((id + 1) * a.keys_wgs / all) > k) keys_role<DP>(u, p, a, k, sh, t.k);
-    else rows_role<DP>(u, p, a, (int)id - k, sh, t.r);
+    if ((int)((id + 1) * a.keys_wgs / all) > k) keys_role<DP, PARTS>(u, p, a, k, sh, tab);
+    else rows_role<DP, PARTS>(u, p, a, (int)id - k, sh, tab);
 }
 
 // dk and dv from the splits' sums, in split order; a thread per value.
@@ -843,10 +766,11 @@ om_status bwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p) {
     a.keys_wgs = (int)wk;
     const int64_t kp = plane_bytes(dp, items * a.nt), rp = plane_bytes(dp, items * a.nr);
     const int64_t vals = items * a.nr * kBlock * kRowValues * (int64_t)sizeof(float);
+    const int64_t words = 2 * items * a.nt * kKeyWords * (int64_t)sizeof(float);
     const int64_t part = keys && a.nsplit > 1 ? (int64_t)sizeof(float) * a.nsplit * items * u.lk * 2 * u.d : 0;
     const int64_t stats = 2 * items * a.nt * (int64_t)sizeof(Stats) + items * a.nr * (int64_t)sizeof(RowStats);
     float *scr;
-    if (om_status s = om::scratch2(ctx, (uint64_t)(3 * kp + 4 * rp + vals + stats + part), &scr)) return s;
+    if (om_status s = om::scratch2(ctx, (uint64_t)(3 * kp + 4 * rp + vals + words + stats + part), &scr)) return s;
     char *at = reinterpret_cast<char *>(scr);
     auto take = [&](int64_t bytes) {
         char *x = at;
@@ -863,6 +787,9 @@ om_status bwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p) {
     a.g2 = ro.g2 = take(rp);
     a.q2 = ro.q2 = take(rp);
     a.v = ro.v = reinterpret_cast<float *>(take(vals));
+    float *kw = reinterpret_cast<float *>(take(words));
+    a.keys = ko.keys = vo.keys = kw;
+    vo.is_v = true;
     a.ks = ko.stats = reinterpret_cast<Stats *>(take(items * a.nt * (int64_t)sizeof(Stats)));
     a.vs = vo.stats = reinterpret_cast<Stats *>(take(items * a.nt * (int64_t)sizeof(Stats)));
     a.rs = ro.stats = reinterpret_cast<RowStats *>(take(items * a.nr * (int64_t)sizeof(RowStats)));
@@ -870,18 +797,17 @@ om_status bwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p) {
     auto al16 = [](const void *x) { return ((uintptr_t)x & 15) == 0; };
     const bool vec = u.d % 4 == 0 && p.ldq % 4 == 0 && p.ldkv % 4 == 0 && p.ldo % 4 == 0 && p.ldg % 4 == 0 && al16(p.q) &&
                      al16(p.k) && al16(p.v) && al16(p.o) && al16(p.g);
-    auto go = [&](auto dpc) {
+    by_depth(u.d, [&](auto dpc) {
         constexpr int DP = decltype(dpc)::value;
         auto split = [&](auto kern) {
             hipLaunchKernelGGL(kern, dim3((unsigned)jobs), dim3(256), 0, ctx->stream, u, p, ko, vo, ro, a.nt, a.nr);
         };
         vec ? split(k_scored_split_bwd<DP, true>) : split(k_scored_split_bwd<DP, false>);
-        hipLaunchKernelGGL(k_scored_bwd_mm<DP>, dim3((unsigned)(wk + wr)), dim3(256), 0, ctx->stream, u, p, a);
-    };
-    if (dp == 32) go(std::integral_constant<int, 32>());
-    else if (dp == 64) go(std::integral_constant<int, 64>());
-    else if (dp == 96) go(std::integral_constant<int, 96>());
-    else go(std::integral_constant<int, 128>());
+        by_parts(parts_of(u), [&](auto pc) {
+            hipLaunchKernelGGL((k_scored_bwd_mm<DP, decltype(pc)::value>), dim3((unsigned)(wk + wr)), dim3(256), 0, ctx->stream, u,
+                               p, a);
+        });
+    });
     if (part) {
         const int64_t values = items * u.lk * 2 * u.d;
         hipLaunchKernelGGL(k_scored_join_dkv, dim3((unsigned)((values + 255) / 256)), dim3(256), 0, ctx->stream, u, p, a.nsplit,

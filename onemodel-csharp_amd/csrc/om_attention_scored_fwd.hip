@@ -14,7 +14,7 @@ using namespace osc;
 constexpr float kInf = __builtin_inff();
 constexpr int kRows = 128;      // rows of a workgroup
 constexpr float kSlack = 2.0f;  // how far a maximum may outgrow m before m moves
-constexpr int kListed = 256;    // blocks of keys whose step data stands in LDS
+constexpr int kListed = 256;    // blocks of keys whose documents' look stands in LDS
 
 template <int DP, bool VEC>
 __global__ void __launch_bounds__(256) k_scored_split_kv(Rule u, Ptrs p, SplitOut ko, SplitOut vo, int nt) {
@@ -112,6 +112,7 @@ __device__ __forceinline__ void plain_row(const Rule &u, const Ptrs &p, int b, i
 struct FwdArgs {
     const char *kn, *vt;      // K in rows form, V in columns form
     const Stats *ks, *vs;     // their blocks' statistics
+    const float *keys;        // the steps' words
     int nt;                   // blocks of 64 keys of a head
     int blocks;               // workgroups along a head's rows
     int nsplit;               // splits of each block of rows' keys
@@ -119,17 +120,15 @@ struct FwdArgs {
     int vec;                  // q's rows are 16-byte aligned
 };
 
-template <int DP>
+template <int DP, int PARTS>
 __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored_fwd_mm(Rule u, Ptrs p, FwdArgs a) {
     OM_LDS_POISON();
+    constexpr bool DOCS = PARTS & kDocs, CAP = PARTS & kCap, SLOPES = PARTS & kSlopes;
     constexpr int KT = 32, S = DP / 16, ND = DP / 32, NST = DP == 128 ? 2 : 3;  // as many stages as leave two workgroups a CU
-    constexpr int HALF = KT * DP * 4, STAGE = 2 * HALF + KT * 4;  // K's planes, V's, the keys' documents
-    constexpr int PER = 2 * (HALF / 4096);  // loads of a step per wavefront, documents aside
+    constexpr int HALF = KT * DP * 4, STAGE = 2 * HALF + 4 * kKeyWords;  // K's planes, V's, the step's words
+    constexpr int PER = 2 * (HALF / 4096) + 1;  // loads of a step per wavefront
     __shared__ __attribute__((aligned(16))) char sh[256 + NST * STAGE];  // no stage at LDS address 0
-    __shared__ float kscale[kListed];
-    __shared__ signed char vstep[kListed];  // exponent of V's scale less the largest, in steps of 4
-    __shared__ unsigned char visit[kListed];  // whether some row may see the block
-    __shared__ int docs_lo[kListed], docs_hi[kListed];
+    __shared__ unsigned char visit[DOCS ? kListed : 1];  // whether some row may see the block
     __shared__ uint32_t red[4][6];
     const Place at = place_of(blockIdx.x, u.B * u.Hk);
     const int item = at.item, split = at.block % a.nsplit, rb = a.blocks - 1 - at.block / a.nsplit;
@@ -140,8 +139,8 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
     const int rr = first + 32 * w + (lane & 31);
     const Row row = row_of(u, hk, min(rr, rows - 1));
     const int64_t tok = (int64_t)b * u.lq + row.t;
-    const int pos = row.t + u.off, doc = u.qd ? u.qd[tok] : 0;
-    const float slope = u.slopes ? u.slopes[row.h] * kLog2e : 0.0f;
+    const int pos = row.t + u.off, doc = DOCS ? u.qd[tok] : 0;
+    const float slope = SLOPES ? u.slopes[row.h] * kLog2e : 0.0f;
 
     // The row's query: d = 16 s + 8 g + e.
     float x0[S][8];
@@ -206,7 +205,7 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
     // documents of the wavefront's rows; a padded row sees nothing, whatever the others see
     int wqlo = 0, wqhi = 0;
     bool one_doc = true;
-    if (u.qd) {
+    if (DOCS) {
         wqlo = __builtin_amdgcn_readfirstlane(wave_imin(doc < 0 ? INT32_MAX : doc));
         wqhi = __builtin_amdgcn_readfirstlane(wave_imax(doc));
         one_doc = wqlo == wqhi && !__any(doc < 0);
@@ -238,37 +237,24 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
         return;
     }
     const int ev = vtop ? scale_exp(vtop) : 0;
-    auto looked = [&](int t, const Stats &ks, const Stats &vs, float &sc, int &step) -> int {
-        sc = ks.scale;
-        step = vs.top ? ((int)(__float_as_uint(vs.scale) >> 23) - 127 - ev) / 4 : 0;  // 0 for a block of zeros
-        const int j0 = t * kBlock, j1 = j0 + kBlock - 1;
-        int see = 1;
-        if (j0 >= pre) see = !(u.causal && j0 > i1) && !(u.window && (i0 - j1 >= u.window || j0 - i1 >= u.window));
-        if (u.qd && (ks.doc_hi < qlo || ks.doc_lo > qhi)) see = 0;
-        return see;
-    };
-    if (t0 + (int)threadIdx.x <= t1) {
-        static_assert(kListed == 256, "a thread's first block is its entry");
-        float sc;
-        int step;
-        const int see = looked(t0 + threadIdx.x, mk, mv, sc, step);
-        docs_lo[threadIdx.x] = mk.doc_lo;
-        docs_hi[threadIdx.x] = mk.doc_hi;
-        kscale[threadIdx.x] = sc;
-        vstep[threadIdx.x] = (signed char)step;
-        visit[threadIdx.x] = (unsigned char)see;
-    }
-    __syncthreads();
-
-    const int steps = (t1 - t0 + 1) * (kBlock / KT);
-    const bool dense = !u.qd && !(u.window && pre > 0);  // no gaps in what is seen
-    auto next = [&](int it) {  // the next step with a key that some row may see
-        for (it++; it < steps; it++) {
-            const int t = it * KT / kBlock;
-            if (t0 * kBlock + it * KT > hi) return steps;
-            if (dense || t >= kListed || visit[t]) return it;
+    if (DOCS) {
+        if (t0 + (int)threadIdx.x <= t1) {
+            static_assert(kListed == 256, "a thread's first block is its entry");
+            visit[threadIdx.x] = !(mk.doc_hi < qlo || mk.doc_lo > qhi);
         }
-        return steps;
+        __syncthreads();
+    }
+
+    const int base = t0 * kBlock, steps = hi < lo ? 0 : (hi - base) / KT + 1;
+    const Band whole_wg(u, i0, i1, pre);
+    auto next = [&](int it) {  // the next step with a key that some row may see
+        it++;
+        // a window leaves a gap behind a prefix
+        const int j0 = base + it * KT;
+        if ((j0 >= whole_wg.pre) & (j0 + KT <= whole_wg.some0)) it = (whole_wg.some0 - base) / KT;
+        if (DOCS)
+            while (it < steps && it / 2 < kListed && !visit[it / 2]) it++;
+        return it < steps ? it : steps;
     };
     const char *kn = a.kn + (kt0 + t0) * plane_bytes(DP, 1), *vt = a.vt + (kt0 + t0) * plane_bytes(DP, 1);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)(sh + 256);
@@ -279,8 +265,8 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
         for (int i = 0; i < PER / 2; i++) load_to_lds(ka + (4 * i + w) * 1024, to + (uint32_t)(4 * i + w) * 1024u);
 #pragma unroll
         for (int i = 0; i < PER / 2; i++) load_to_lds(va + (4 * i + w) * 1024, to + HALF + (uint32_t)(4 * i + w) * 1024u);
-        if (u.kd && lane >> 3 == w)  // eight of the step's keys each
-            load_to_lds4(u.kd + (int64_t)b * u.lk + min(t0 * kBlock + it * KT + lane, u.lk - 1), to + 2 * HALF);
+        if (lane >> 4 == w)  // a quarter of the step's words each
+            load_to_lds4(a.keys + (2 * (kt0 + t0) + it) * kKeyWords + lane, to + 2 * HALF);
     };
 
     const Reach reach = keys_seen(u, pos, doc, pre);
@@ -292,6 +278,7 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
     float m = -kInf, l = 0.0f;
     const int wi0 = min(first + 32 * w, last) / u.G + u.off, wi1 = min(first + 32 * w + 31, last) / u.G + u.off;
     const bool live = first + 32 * w <= last;
+    const Band mine(u, wi0, wi1, pre);
     const float cq = __builtin_fabsf(u.cl2) * pow2(eq), icq = __builtin_fabsf(u.icap) * pow2(eq);
 
     int it = next(-1), nx = it < steps ? next(it) : steps, slot = 0;
@@ -300,34 +287,24 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
     while (it < steps) {
         // this step has landed (with three stages the next is in flight), and every wavefront is done with the one before
         if (NST == 2 || nx >= steps) land<0>();
-        else if (u.kd) land<PER + 1>();
         else land<PER>();
         const int nn = nx < steps ? next(nx) : steps;
         if (NST == 3 && nn < steps) stage(nn, slot == 0 ? 2 : slot - 1);
         if (NST == 2 && nx < steps) stage(nx, slot ^ 1);
-        const int j0 = t0 * kBlock + it * KT, j1 = j0 + KT - 1, ti = it * KT / kBlock;
-        float ksc;
-        int vst, dlo, dhi;
-        if (ti < kListed) {
-            ksc = kscale[ti];
-            vst = vstep[ti];
-            dlo = u.qd ? __builtin_amdgcn_readfirstlane(docs_lo[ti]) : 0;
-            dhi = u.qd ? __builtin_amdgcn_readfirstlane(docs_hi[ti]) : 0;
-        } else {
-            const Stats ks = a.ks[kt0 + t0 + ti];
-            looked(t0 + ti, ks, a.vs[kt0 + t0 + ti], ksc, vst);
-            dlo = ks.doc_lo;
-            dhi = ks.doc_hi;
-        }
+        const int j0 = base + it * KT, j1 = j0 + KT - 1;
+        const char *kf = sh + 256 + slot * STAGE + lane * 16, *vf = kf + HALF;
+        const int *words = reinterpret_cast<const int *>(sh + 256 + slot * STAGE + 2 * HALF);
         // what the wavefront's 32 rows see of the step
-        const bool none = !live || (u.qd && (dhi < wqlo || dlo > wqhi)) || (j0 >= pre && ((u.causal && j0 > wi1) ||
-                                                  (u.window && (wi0 - j1 >= u.window || j0 - wi1 >= u.window))));
-        const bool one = !u.qd || (one_doc && dlo == dhi && dlo == wqlo && dlo >= 0);
-        const bool whole = j1 < u.lk && one &&
-                           (j1 < pre || ((!u.causal || j1 <= wi0) && (!u.window || (wi1 - j0 < u.window && j1 - wi0 < u.window))));
-        if (!none) {
-            const char *kf = sh + 256 + slot * STAGE + lane * 16, *vf = kf + HALF;
-            const int *kdoc = reinterpret_cast<const int *>(sh + 256 + slot * STAGE + 2 * HALF);
+        bool some = live & mine.some(j0, j1), one = true;
+        if (DOCS) {
+            const int dlo = __builtin_amdgcn_readfirstlane(words[kKeyDocLo]), dhi = __builtin_amdgcn_readfirstlane(words[kKeyDocHi]);
+            some = some & (dhi >= wqlo) & (dlo <= wqhi);
+            one = one_doc & (dlo == dhi) & (dlo == wqlo) & (dlo >= 0);
+        }
+        if (some) {
+            const float ksc = __int_as_float(words[kKeyScaleK]);
+            // V's exponent less the largest, in steps of 4; a block of zeros may say anything
+            const int vst = min(max(((words[kKeyScaleV] >> 23) - 127 - ev) >> 2, -8), 0);
             floatx16 x;
 #pragma unroll
             for (int e = 0; e < 16; e++) x[e] = 0.0f;
@@ -339,7 +316,7 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
             }
             // x * f is the score in log2 units
             float f = cq * ksc;
-            if (u.icap != 0.0f) {
+            if (CAP) {
                 const float ic = icq * ksc;
                 float big = 0.0f;
 #pragma unroll
@@ -351,9 +328,9 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
 #pragma unroll
                     for (int e = 0; e < 16; e++) x[e] = tanh_small(x[e] * ic);
                 }
-                f = u.capl2;
+            f = u.capl2;
             }
-            if (u.slopes) {
+            if (SLOPES) {
                 const float gap0 = (float)(pos - j0 - 4 * g);
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
@@ -362,11 +339,11 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
                 }
                 f = 1.0f;
             }
-            if (!whole) {
+            if (!(mine.all(j0, j1) & one)) {
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
                     intx4 kd = {doc, doc, doc, doc};
-                    if (!one) kd = *reinterpret_cast<const intx4 *>(kdoc + 8 * q + 4 * g);
+                    if (DOCS) kd = *reinterpret_cast<const intx4 *>(words + kKeyDoc + 8 * q + 4 * g);
 #pragma unroll
                     for (int r = 0; r < 4; r++) {
                         const bool ok = reach.has(j0 + 8 * q + 4 * g + r) & (kd[r] == doc);
@@ -464,9 +441,10 @@ om_status fwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p, int *joins, f
     ns = ns < 1 ? 1 : ns;
     OM_REQUIRE(ctx, wgs * ns <= INT32_MAX && 2 * items * nt <= INT32_MAX, "om_attention_fwd_scored: too many row blocks");
     const int64_t plane = plane_bytes(dp, items * nt), stats = items * nt * (int64_t)sizeof(Stats);
+    const int64_t words = 2 * items * nt * kKeyWords * (int64_t)sizeof(float);
     const int64_t join = ns > 1 ? (int64_t)sizeof(float) * ns * all * (u.d + 2) : 0;
     float *scr;
-    if (om_status s = om::scratch2(ctx, (uint64_t)(2 * plane + 2 * stats + join), &scr)) return s;
+    if (om_status s = om::scratch2(ctx, (uint64_t)(2 * plane + 2 * stats + words + join), &scr)) return s;
     char *base = reinterpret_cast<char *>(scr);
     FwdArgs a = {};
     a.kn = base;
@@ -476,23 +454,25 @@ om_status fwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p, int *joins, f
     a.nt = nt;
     a.blocks = blocks;
     a.nsplit = (int)ns;
-    a.part = ns > 1 ? reinterpret_cast<float *>(base + 2 * plane + 2 * stats) : nullptr;
+    float *keys = reinterpret_cast<float *>(base + 2 * plane + 2 * stats);
+    a.keys = keys;
+    a.part = ns > 1 ? reinterpret_cast<float *>(base + 2 * plane + 2 * stats + words) : nullptr;
     auto al16 = [](const void *x) { return ((uintptr_t)x & 15) == 0; };
     a.vec = u.d % 4 == 0 && p.ldq % 4 == 0 && al16(p.q);
     const bool vec = u.d % 4 == 0 && p.ldkv % 4 == 0 && al16(p.k) && al16(p.v);
-    const SplitOut ko = {base, nullptr, const_cast<Stats *>(a.ks)}, vo = {nullptr, base + plane, const_cast<Stats *>(a.vs)};
-    auto go = [&](auto dpc) {
+    const SplitOut ko = {base, nullptr, const_cast<Stats *>(a.ks), keys, false};
+    const SplitOut vo = {nullptr, base + plane, const_cast<Stats *>(a.vs), keys, true};
+    by_depth(u.d, [&](auto dpc) {
         constexpr int DP = decltype(dpc)::value;
         auto split = [&](auto kern) {
             hipLaunchKernelGGL(kern, dim3((unsigned)(2 * items * nt)), dim3(256), 0, ctx->stream, u, p, ko, vo, nt);
         };
         vec ? split(k_scored_split_kv<DP, true>) : split(k_scored_split_kv<DP, false>);
-        hipLaunchKernelGGL(k_scored_fwd_mm<DP>, dim3((unsigned)(wgs * ns)), dim3(256), 0, ctx->stream, u, p, a);
-    };
-    if (dp == 32) go(std::integral_constant<int, 32>());
-    else if (dp == 64) go(std::integral_constant<int, 64>());
-    else if (dp == 96) go(std::integral_constant<int, 96>());
-    else go(std::integral_constant<int, 128>());
+        by_parts(parts_of(u), [&](auto pc) {
+            hipLaunchKernelGGL((k_scored_fwd_mm<DP, decltype(pc)::value>), dim3((unsigned)(wgs * ns)), dim3(256), 0, ctx->stream, u,
+                               p, a);
+        });
+    });
     *joins = (int)ns;
     *part = a.part;
     return OM_LAUNCH_CHECK(ctx, "om_attention_fwd_scored");

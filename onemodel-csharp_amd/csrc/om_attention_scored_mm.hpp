@@ -39,6 +39,8 @@ struct Stats {
     int32_t doc_lo, doc_hi;
     int32_t pad[3];
 };
+// What a step of 32 keys carries along with its operands, staged with them: 64 words.
+enum { kKeyDoc = 0, kKeyScaleK = 32, kKeyScaleV, kKeyDocLo, kKeyDocHi, kKeyWords = 64 };
 constexpr uint32_t kInfBits = 0x7F800000u;
 constexpr uint32_t kMostBits = (127u + 40) << 23, kLeastBits = (127u - 40) << 23;  // 2^40, 2^-40
 
@@ -141,6 +143,82 @@ __device__ __forceinline__ void land() {
 
 // Bytes of one operand's two planes for `blocks` blocks of 64 rows.
 inline __host__ __device__ int64_t plane_bytes(int dp, int64_t blocks) { return blocks * kBlock * dp * 4; }
+
+// Which of the rule's parts a kernel is compiled for; the others cost it nothing, not a branch in its loop.
+enum { kDocs = 1, kCap = 2, kSlopes = 4 };
+inline int parts_of(const Rule &u) { return (u.qd ? kDocs : 0) | (u.icap != 0.0f ? kCap : 0) | (u.slopes ? kSlopes : 0); }
+template <typename F>
+void by_parts(int parts, F f) {
+    switch (parts) {
+    case 0: return f(std::integral_constant<int, 0>());
+    case 1: return f(std::integral_constant<int, 1>());
+    case 2: return f(std::integral_constant<int, 2>());
+    case 3: return f(std::integral_constant<int, 3>());
+    case 4: return f(std::integral_constant<int, 4>());
+    case 5: return f(std::integral_constant<int, 5>());
+    case 6: return f(std::integral_constant<int, 6>());
+    default: return f(std::integral_constant<int, 7>());
+    }
+}
+template <typename F>
+void by_depth(int d, F f) {
+    if (d <= 32) f(std::integral_constant<int, 32>());
+    else if (d <= 64) f(std::integral_constant<int, 64>());
+    else if (d <= 96) f(std::integral_constant<int, 96>());
+    else f(std::integral_constant<int, 128>());
+}
+
+// What positions i0 .. i1 see of the keys, documents aside, as intervals: all of them see `all0 .. all1`, some may see
+// `some0 .. some1`; and all see the keys below pre.
+struct Band {
+    int all0, all1, some0, some1, pre;
+    __device__ __forceinline__ Band(const Rule &u, int i0, int i1, int prefix) {
+        all0 = some0 = 0;
+        all1 = some1 = u.lk - 1;
+        if (u.causal) {
+            all1 = min(all1, i0);
+            some1 = min(some1, i1);
+        }
+        if (u.window) {
+            all0 = max(0, i1 - u.window + 1);
+            some0 = max(0, i0 - u.window + 1);
+            all1 = min(all1, i0 + u.window - 1);
+            some1 = min(some1, i1 + u.window - 1);
+        }
+        pre = min(prefix, u.lk);
+    }
+    // bitwise throughout: a chain of scalar branches costs more than the arithmetic it saves
+    __device__ __forceinline__ bool all(int j0, int j1) const { return ((j0 >= all0) & (j1 <= all1)) | (j1 < pre); }
+    __device__ __forceinline__ bool some(int j0, int j1) const { return ((j0 <= some1) & (j1 >= some0)) | (j0 < pre); }
+};
+
+// The same from the keys' side, in rows of the group: rows all0 .. all1 see all of keys j0 .. j1, rows some0 .. some1 some.
+struct RowBand {
+    int all0, all1, some0, some1;
+    __device__ __forceinline__ RowBand(const Rule &u, int j0, int j1, int prefix) {
+        int a0 = u.off, a1 = INT32_MAX, s0 = u.off, s1 = INT32_MAX;  // positions
+        if (j1 >= prefix) {
+            if (u.causal) a0 = max(a0, j1);
+            if (u.window) {
+                a0 = max(a0, j1 - u.window + 1);
+                a1 = j0 + u.window - 1;
+            }
+        }
+        if (j0 >= prefix) {
+            if (u.causal) s0 = max(s0, j0);
+            if (u.window) {
+                s0 = max(s0, j0 - u.window + 1);
+                s1 = j1 + u.window - 1;
+            }
+        }
+        all0 = (a0 - u.off) * u.G;
+        some0 = (s0 - u.off) * u.G;
+        all1 = a1 >= u.lk - 1 ? INT32_MAX : (a1 - u.off + 1) * u.G - 1;
+        some1 = s1 >= u.lk - 1 ? INT32_MAX : (s1 - u.off + 1) * u.G - 1;
+    }
+    __device__ __forceinline__ bool all(int r0, int r1) const { return (r0 >= all0) & (r1 <= all1); }
+    __device__ __forceinline__ bool some(int r0, int r1) const { return (r1 >= some0) & (r0 <= some1); }
+};
 
 // Workgroup id -> item and block. Ids are dealt round-robin over the 8 XCDs, each with its own L2, so the items come
 // innermost: an XCD then works on few heads' operands (one in eight of them where their number is a multiple of eight), an

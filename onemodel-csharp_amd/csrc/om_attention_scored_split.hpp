@@ -9,6 +9,8 @@ namespace osc {
 struct SplitOut {
     char *rows, *cols;  // either may be NULL
     Stats *stats;
+    float *keys;  // the steps' words (kKeyWords for each 32 keys); K writes the documents too
+    bool is_v;
 };
 
 // This thread's share of a block: values 64 n + 4 (tid % 16) .. + 3 of rows 4 (tid / 16) + i.
@@ -149,6 +151,26 @@ __device__ __forceinline__ void split_keys(const Rule &u, const float *src, int6
         st.doc_hi = dhi;
         o.stats[at] = st;
     }
+    __syncthreads();
+    // the words of the block's two steps
+    if (threadIdx.x < 2 * kKeyWords) {
+        const int half = threadIdx.x / kKeyWords, n = threadIdx.x % kKeyWords;
+        float *to = o.keys + (2 * at + half) * kKeyWords;
+        if (o.is_v) {
+            if (n == kKeyScaleV) to[n] = pow2(e);
+        } else if (n < 32) {
+            const int j = t * kBlock + 32 * half + n;
+            to[n] = __int_as_float(j >= u.lk ? -1 : u.kd ? u.kd[(int64_t)b * u.lk + j] : 0);
+        } else if (n == kKeyScaleK) {
+            to[n] = pow2(e);
+        } else if (n == kKeyDocLo || n == kKeyDocHi) {
+            for (int i = 0; i < 16; i++) {
+                dlo = min(dlo, (int)sh[i]);
+                dhi = max(dhi, (int)sh[16 + i]);
+            }
+            to[n] = __int_as_float(n == kKeyDocLo ? dlo : dhi);
+        }
+    }
 }
 
 // What the backward keeps of its rows (queries of one head): a record of 1 KB per 32 rows, a value of all 32 after another.
@@ -159,6 +181,7 @@ enum {
     kRowSlope,  // slope of its head, in log2 units
     kRowDoc,    // document (int)
     kRowW,      // 2^re / l: what the row's sums are multiplied with at the end; 0 for a row without gradient
+    kRowBlock,  // of the rows' block of 64: its scales of q, g / l and q w, its documents' range
     kRowValues = 8
 };
 __host__ __device__ __forceinline__ int64_t row_value(int64_t row, int which) { return (row >> 5) * (32 * kRowValues) + which * 32 + (row & 31); }
@@ -295,6 +318,14 @@ __device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, 
         st.doc_lo = dlo;
         st.doc_hi = dhi;
         o.stats[at] = st;
+        for (int half = 0; half < 2; half++) {
+            float *to = o.v + row_value(at * kBlock + 32 * half, kRowBlock);
+            to[0] = st.q;
+            to[1] = st.g2;
+            to[2] = st.q2;
+            to[3] = __int_as_float(dlo);
+            to[4] = __int_as_float(dhi);
+        }
     }
 }
 
