@@ -11,13 +11,21 @@
 // query in each lane. Either way a block of scores leaves the matrix unit in the order in which it is the next product's
 // operand. Recomputing the scores for the second role costs two products of seven; partial dq from the first role would
 // cost rows * keys / 32 values of traffic, more than that from about 2000 keys on, and atomics would lose the fixed order.
+#include <algorithm>
+
 #include "om_attention_scored_split.hpp"
 
 namespace {
 
 using namespace osc;
 
-constexpr int kKeys = 128;   // keys (or rows) of a workgroup
+constexpr int kKeys = 128;   // keys of a workgroup of the first role
+// Wavefronts of a workgroup. Up to 64 values a head, four: each holds 32 keys' dk and dv, two or three workgroups a CU. Above,
+// both and the fragments of K and V take more than half a SIMD's registers, and one wavefront a SIMD is left. Up to 96, eight
+// share the stages instead: four hold K and dv and form the scores and the weights, four hold V and dk of the same keys, form
+// g . v meanwhile, and take the weights over through LDS (777 rows of 80 values, prefix: 108 -> 95 us). At 128 that spills
+// registers and is no faster than four (8192 rows in a window of 1024: 1157 us against 1152).
+constexpr int waves_of(int dp) { return dp == 96 ? 8 : 4; }
 constexpr int kStep = 32;    // rows (or keys) of a step
 constexpr int kListed = 256; // blocks whose step data stands in LDS
 
@@ -30,7 +38,8 @@ struct BwdArgs {
     int nt, nr;                      // blocks of 64 keys and rows of a head
     int kblocks, rblocks;            // workgroups along them
     int nsplit;                      // splits of each block of keys' rows for dk and dv
-    int keys_wgs;                    // workgroups of the first role
+    int keys_wgs, rows_wgs;          // workgroups of the roles
+    int kperiod, rperiod;            // where the roles' sweeps begin: at multiples, in blocks of rows and in steps of keys
     float *part;                     // [split][B Hk][lk][2][d] (dk, dv), NULL for one split
 };
 
@@ -215,26 +224,27 @@ __device__ __forceinline__ void put4(float *to, int c, int d, floatx4 v, int acc
 // ---------------------------------------------------------------------------------------------------- dk and dv
 // Either role's tables in LDS, by blocks of the other side: whether the block is visited (documents).
 struct Tables {
-    uint32_t red[4][5];
+    uint32_t red[8][5];
     unsigned char see[kListed];
 };
 template <int DP, int PARTS>
 __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const BwdArgs &a, int i, char *sh, Tables &tab) {
     constexpr bool DOCS = PARTS & kDocs, CAP = PARTS & kCap, SLOPES = PARTS & kSlopes;
-    constexpr int S = DP / 16, ND = DP / 32, HALF = kStep * DP * 4, STAGE = 4 * HALF + 1024;  // the rows' record last
+    constexpr int NW = waves_of(DP), S = DP / 16, ND = DP / 32, HALF = kStep * DP * 4, STAGE = 4 * HALF + 1024;  // the rows' record last
     auto &red = tab.red;
     const Place pl = place_of(i, u.B * u.Hk);
     const int item = pl.item, split = pl.block % a.nsplit, kb = pl.block / a.nsplit;
-    const int b = item / u.Hk, hk = item - b * u.Hk, rows = u.G * u.lq;
+    const int b = item / u.Hk, hk = item - b * u.Hk;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
     const int pre = u.prefix ? u.prefix[b] : 0;
     const int first = kb * kKeys, last = min(first + kKeys, u.lk) - 1;
-    const int j = first + 32 * w + (lane & 31);
-    const bool live = first + 32 * w <= last;
+    const int own = first + 32 * (w & 3);  // the wavefront's keys; the second four of eight have those of the first
+    const int j = own + (lane & 31);
+    const bool live = own <= last;
     const int kd = j <= last ? (DOCS ? u.kd[(int64_t)b * u.lk + j] : 0) : -1;
     const int64_t kt0 = (int64_t)item * a.nt, rt0 = (int64_t)item * a.nr;
     // the wavefront's block of keys (a wavefront past the last key repeats it and stores nothing)
-    const int t = min((first + 32 * w) / kBlock, a.nt - 1);
+    const int t = min(own / kBlock, a.nt - 1);
     const Stats ks = a.ks[kt0 + t], vs = a.vs[kt0 + t];
     const int tb = min(first / kBlock + 1, a.nt - 1);
     const Stats v0 = a.vs[kt0 + first / kBlock], v1 = a.vs[kt0 + tb], k0 = a.ks[kt0 + first / kBlock], k1 = a.ks[kt0 + tb];
@@ -250,14 +260,10 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
     int plo, phi;
     pos_range(u, first, last, pre, plo, phi);
     int r0 = (plo - u.off) * u.G, r1 = phi < plo ? r0 : (phi - u.off + 1) * u.G;  // one past the last
-    // this split's share of them, in blocks: equal shares
-    const int c0 = r0 / kBlock, c1 = r1 <= r0 ? c0 - 1 : (r1 - 1) / kBlock, per = (c1 - c0 + a.nsplit) / a.nsplit;
-    const int t0 = c0 + split * per, t1 = min(c1, t0 + per - 1);
-    r0 = max(r0, t0 * kBlock);
-    r1 = max(r0, min(r1, (t1 + 1) * kBlock));
+    const int t0 = r0 / kBlock, t1 = r1 <= r0 ? t0 - 1 : (r1 - 1) / kBlock;
     uint32_t gt = 0, gl = 0xFFFFFFFFu, qt = 0, ql = 0xFFFFFFFFu;
     RowStats mine = {};  // the thread's first
-    for (int rt = t0 + (int)threadIdx.x, n = 0; rt <= t1; rt += 256, n++) {
+    for (int rt = t0 + (int)threadIdx.x, n = 0; rt <= t1; rt += 64 * NW, n++) {
         const RowStats r = a.rs[rt0 + rt];
         if (n == 0) mine = r;
         bad = bad || r.bad;
@@ -266,7 +272,7 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
         if (r.g2_top) gl = min(gl, r.g2_top);
         if (r.q2_top) ql = min(ql, r.q2_top);
     }
-    if (DOCS && t0 + (int)threadIdx.x <= t1) {
+    if (DOCS && threadIdx.x < kListed && t0 + (int)threadIdx.x <= t1) {
         static_assert(kListed == 256, "a thread's first block is its entry");
         tab.see[threadIdx.x] = mine.doc_hi >= max(kdlo, 0) && mine.doc_lo <= kdhi && (mine.g2_top || mine.q2_top);
     }
@@ -284,7 +290,7 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
     }
     __syncthreads();
 #pragma unroll
-    for (int n = 0; n < 4; n++) {
+    for (int n = 0; n < NW; n++) {
         gt = max(gt, red[n][0]);
         qt = max(qt, red[n][1]);
         gl = min(gl, red[n][2]);
@@ -300,48 +306,77 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
     };
     const int acc = a.part ? 0 : p.acc;
     if (__builtin_amdgcn_readfirstlane(bad)) {
-        for (int jj = first + 32 * w; jj <= min(last, first + 32 * w + 31); jj++)
+        constexpr int EACH = kKeys / NW;
+        const int per = (t1 - t0 + a.nsplit) / a.nsplit * kBlock, s0 = t0 * kBlock + split * per;  // the split's equal share
+        r1 = max(r0, min(r1, s0 + per));
+        r0 = min(max(r0, s0), r1);
+        for (int jj = first + EACH * w; jj <= min(last, first + EACH * w + EACH - 1); jj++)
             plain_dkv<DP>(u, p, b, hk, jj, r0, r1, pre, dest(0, jj), dest(1, jj), acc);
         return;
     }
     // K and V fragments of the wavefront's keys
-    u32x4 kh[S], km[S], vh[S], vm[S];
+    u32x4 kh[S], km[S], vh[NW == 4 ? S : 1], vm[NW == 4 ? S : 1];  // the second four of eight have V's in kh, km
     {
-        const int half = ((first + 32 * w) / 32) & 1;
+        const int half = (own / 32) & 1;
         const char *kf = a.kn + (kt0 + t) * plane_bytes(DP, 1) + half * HALF + lane * 16;
         const char *vf = a.vn + (kt0 + t) * plane_bytes(DP, 1) + half * HALF + lane * 16;
 #pragma unroll
         for (int s = 0; s < S; s++) {
-            kh[s] = *reinterpret_cast<const u32x4 *>(kf + (2 * s) * 1024);
-            km[s] = *reinterpret_cast<const u32x4 *>(kf + (2 * s + 1) * 1024);
-            vh[s] = *reinterpret_cast<const u32x4 *>(vf + (2 * s) * 1024);
-            vm[s] = *reinterpret_cast<const u32x4 *>(vf + (2 * s + 1) * 1024);
+            const char *f = NW == 8 && w >= 4 ? vf : kf;
+            kh[s] = *reinterpret_cast<const u32x4 *>(f + (2 * s) * 1024);
+            km[s] = *reinterpret_cast<const u32x4 *>(f + (2 * s + 1) * 1024);
+            if constexpr (NW == 4) {
+                vh[s] = *reinterpret_cast<const u32x4 *>(vf + (2 * s) * 1024);
+                vm[s] = *reinterpret_cast<const u32x4 *>(vf + (2 * s + 1) * 1024);
+            }
         }
     }
     const Reach reach = rows_seeing(u, j, kd, pre);
+    // sums of dk and dv; of eight wavefronts each has one of them, in `dk`
     floatx16 dk[ND], dv[ND];
 #pragma unroll
     for (int n = 0; n < ND; n++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) dk[n][e] = dv[n][e] = 0.0f;
+        for (int e = 0; e < 16; e++) {
+            dk[n][e] = 0.0f;
+            dv[n][e] = 0.0f;
+        }
     float g2cur = 1.0f, q2cur = 1.0f;
     int sd = kNoScale;  // dk's sums are in units of 2^sd
-    const int base = t0 * kBlock, steps = r1 <= r0 ? 0 : (r1 - 1 - base) / kStep + 1;
-    auto next = [&](int it) {
-        it++;
-        if (DOCS)
-            while (it < steps && it / 2 < kListed && !tab.see[it / 2]) it++;
-        return it < steps ? it : steps;
+    // The split has every nsplit-th block. They are taken downwards, and from a multiple of `period` blocks on, round the
+    // range's ends: workgroups of other keys that run meanwhile then read the same blocks, under a causal rule from the last
+    // row on, in a window at the same remainder, and find them in their XCD's L2. (Each from its own first row, a window of
+    // 1024 at 8192 rows of 4 heads of 128 missed L2 in two of three reads and was bound by that.)
+    const int base = t0 * kBlock, nb = t1 - t0 + 1, first_step = (r0 - base) / kStep, last_step = r1 <= r0 ? -1 : (r1 - 1 - base) / kStep;
+    const int cut = max((t1 + 1) / a.kperiod * a.kperiod - t0, 0);
+    auto top = [&](int bl) { return 2 * (bl - (t0 + bl - split + a.nsplit) % a.nsplit) + 1; };  // the split's last step up to block bl
+    int stop = 0;
+    bool more = cut > 0;
+    auto settle = [&](int it) {  // the first step from `it` on that is the split's to take; -1 behind the last
+        while (true) {
+            if (it < stop) {
+                if (!more) return -1;
+                more = false;
+                it = top(nb - 1);
+                stop = 2 * cut;
+            } else if ((it > last_step) | (it < first_step) || (DOCS && it / 2 < kListed && !tab.see[it / 2])) {
+                it = it & 1 ? it - 1 : it + 1 - 2 * a.nsplit;
+            } else {
+                return it;
+            }
+        }
     };
-    const RowBand band(u, first + 32 * w, min(first + 32 * w + 31, last), pre);
+    auto next = [&](int it) { return settle(it & 1 ? it - 1 : it + 1 - 2 * a.nsplit); };
+    const RowBand band(u, own, min(own + 31, last), pre);
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)(sh + 256);
     auto stage = [&](int it, int buf) {
         const int64_t off = (rt0 + t0) * plane_bytes(DP, 1) + (int64_t)it * HALF + lane * 16;
         const uint32_t to = lds0 + (uint32_t)(buf * STAGE);
-        constexpr int PER = HALF / 4096;
         auto one = [&](const char *src, int n) {
 #pragma unroll
-            for (int q = 0; q < PER; q++) load_to_lds(src + off + (4 * q + w) * 1024, to + (uint32_t)(n * HALF + (4 * q + w) * 1024));
+            for (int q = 0; q < HALF / 1024; q += NW)
+                if (HALF / 1024 % NW == 0 || q + w < HALF / 1024)
+                    load_to_lds(src + off + (q + w) * 1024, to + (uint32_t)(n * HALF + (q + w) * 1024));
         };
         one(a.qn, 0);
         one(a.gn, 1);
@@ -349,12 +384,12 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
         one(a.q2, 3);
         if (w == 0) load_to_lds(a.v + row_value((rt0 + t0) * kBlock + (int64_t)it * kStep, 0) + 4 * lane, to + 4 * HALF);
     };
-    int it = next((r0 - base) / kStep - 1), buf = 0;
-    if (it < steps) stage(it, 0);
-    while (it < steps) {
+    int it = settle(top((more ? cut : nb) - 1)), buf = 0;
+    if (it >= 0) stage(it, 0);
+    while (it >= 0) {
         land<0>();
         const int nx = next(it);
-        if (nx < steps) stage(nx, buf ^ 1);
+        if (nx >= 0) stage(nx, buf ^ 1);
         const int f0 = base + it * kStep, f1 = f0 + kStep - 1;
         const char *qf = sh + 256 + buf * STAGE + lane * 16, *gf = qf + HALF, *g2f = gf + HALF, *q2f = g2f + HALF;
         const float *rec = reinterpret_cast<const float *>(sh + 256 + buf * STAGE + 4 * HALF), *rv = rec + 4 * g;
@@ -366,31 +401,26 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
             some = some & (whi >= 0) & (dhi >= wlo) & (dlo <= whi);
             one = (wlo == whi) & (dlo == dhi) & (dlo == wlo) & (wlo >= 0);
         }
-        if (some) {
-            const float sq = blk[0], sg2 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(blk[1]))),
-                        sq2 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(blk[2])));
-            if (sg2 != g2cur) {
-                const float c = g2cur / sg2;
+        floatx16 x, dp;
+        const float sq = blk[0], sg2 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(blk[1]))),
+                    sq2 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(blk[2])));
+        auto move = [&](floatx16(&sum)[ND], float &cur, float to) {  // sums to another block's scale
+            if (to == cur) return;
+            const float c = cur / to;
 #pragma unroll
-                for (int n = 0; n < ND; n++) dv[n] *= c;
-                g2cur = sg2;
-            }
-            if (sq2 != q2cur) {
-                const float c = q2cur / sq2;
+            for (int n = 0; n < ND; n++) sum[n] *= c;
+            cur = to;
+        };
+        auto products = [&](floatx16 &out, const char *f, const u32x4 *fh, const u32x4 *fm) {
 #pragma unroll
-                for (int n = 0; n < ND; n++) dk[n] *= c;
-                q2cur = sq2;
-            }
-            floatx16 x, dp;
+            for (int e = 0; e < 16; e++) out[e] = 0.0f;
 #pragma unroll
-            for (int e = 0; e < 16; e++) x[e] = dp[e] = 0.0f;
-#pragma unroll
-            for (int s = 0; s < S; s++) {
-                x = mma3(*reinterpret_cast<const u32x4 *>(qf + (2 * s) * 1024),
-                         *reinterpret_cast<const u32x4 *>(qf + (2 * s + 1) * 1024), kh[s], km[s], x);
-                dp = mma3(*reinterpret_cast<const u32x4 *>(gf + (2 * s) * 1024),
-                          *reinterpret_cast<const u32x4 *>(gf + (2 * s + 1) * 1024), vh[s], vm[s], dp);
-            }
+            for (int s = 0; s < S; s++)
+                out = mma3(*reinterpret_cast<const u32x4 *>(f + (2 * s) * 1024),
+                           *reinterpret_cast<const u32x4 *>(f + (2 * s + 1) * 1024), fh[s], fm[s], out);
+        };
+        // x from raw products to weights E; `keep(e, w)` gets E (1 - tanh^2)
+        auto weights = [&](auto keep) {
             const float cs = sq * ks.scale;
             const bool whole = band.all(f0, f1) & one;
             if (CAP) {
@@ -410,11 +440,9 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
                 }
             }
             const float fx = CAP ? u.capl2 : u.cl2 * cs;
-            float top = 0.0f;
 #pragma unroll
             for (int q = 0; q < 4; q++) {
                 const floatx4 m4 = *reinterpret_cast<const floatx4 *>(rv + 32 * kRowM + 8 * q);
-                const floatx4 d4 = *reinterpret_cast<const floatx4 *>(rv + 32 * kRowDelta + 8 * q);
                 floatx4 y;
 #pragma unroll
                 for (int r = 0; r < 4; r++) y[r] = __builtin_fmaf(x[4 * q + r], fx, m4[r]);
@@ -435,12 +463,23 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const int e = 4 * q + r;
-                    const float ex = exp2_hw(y[r]);
-                    float ds = ex * __builtin_fmaf(dp[e], vs.scale, -d4[r]);
-                    if (CAP) ds *= __builtin_fmaf(-x[e], x[e], 1.0f);
-                    dp[e] = ds;
+                    const float ex = exp2_hw(y[r]), th = x[e];
                     x[e] = ex;
-                    top = fmaxf(top, __builtin_fabsf(ds));
+                    keep(e, CAP ? ex * __builtin_fmaf(-th, th, 1.0f) : ex);
+                }
+            }
+        };
+        // dp from g . v to D, given E (1 - tanh^2); dk's sums to its scale; what D is multiplied with before it is split
+        auto gradient = [&](const floatx16 &e1) -> float {
+            float top = 0.0f;
+#pragma unroll
+            for (int q = 0; q < 4; q++) {
+                const floatx4 d4 = *reinterpret_cast<const floatx4 *>(rv + 32 * kRowDelta + 8 * q);
+#pragma unroll
+                for (int r = 0; r < 4; r++) {
+                    const int e = 4 * q + r;
+                    dp[e] = e1[e] * __builtin_fmaf(dp[e], vs.scale, -d4[r]);
+                    top = fmaxf(top, __builtin_fabsf(dp[e]));
                 }
             }
             top = pair_max(top);
@@ -453,25 +492,64 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
                     for (int e = 0; e < 16; e++) dk[n][e] = ldexp_hw(dk[n][e], by);
                 sd = sn;
             }
-            const float fd = pow2(-sd);
+            return pow2(-sd);
+        };
+        auto add_half = [&](floatx16(&sum)[ND], const char *f, const floatx16 &v, float by, int s) {  // 16 of the step's rows
+            float e8[8];
+            u32x4 h, m;
 #pragma unroll
-            for (int s = 0; s < 2; s++) {
-                float e8[8];
-                u32x4 ph, pm, dh, dm;
+            for (int e = 0; e < 8; e++) e8[e] = v[8 * s + e] * by;
+            split8(e8, h, m);
 #pragma unroll
-                for (int e = 0; e < 8; e++) e8[e] = x[8 * s + e];
-                split8(e8, ph, pm);
+            for (int c = 0; c < ND; c++) {
+                const char *at = f + ((s * ND + c) * 2) * 1024;
+                sum[c] = mma3(*reinterpret_cast<const u32x4 *>(at), *reinterpret_cast<const u32x4 *>(at + 1024), h, m, sum[c]);
+            }
+        };
+        if constexpr (NW == 4) {
+            if (some) {
+                move(dv, g2cur, sg2);
+                move(dk, q2cur, sq2);
+                products(x, qf, kh, km);
+                products(dp, gf, vh, vm);
+                floatx16 e1;
+                weights([&](int e, float v) { e1[e] = v; });
+                const float fd = gradient(e1);
 #pragma unroll
-                for (int e = 0; e < 8; e++) e8[e] = dp[8 * s + e] * fd;
-                split8(e8, dh, dm);
-#pragma unroll
-                for (int c = 0; c < ND; c++) {
-                    const int at = ((s * ND + c) * 2) * 1024;
-                    dv[c] = mma3(*reinterpret_cast<const u32x4 *>(g2f + at), *reinterpret_cast<const u32x4 *>(g2f + at + 1024), ph,
-                                 pm, dv[c]);
-                    dk[c] = mma3(*reinterpret_cast<const u32x4 *>(q2f + at), *reinterpret_cast<const u32x4 *>(q2f + at + 1024), dh,
-                                 dm, dk[c]);
+                for (int s = 0; s < 2; s++) {
+                    add_half(dv, g2f, x, 1.0f, s);
+                    add_half(dk, q2f, dp, fd, s);
                 }
+            }
+        } else {
+            // a wavefront's and its partner's registers hold the same rows and key: the weights pass lane by lane
+            floatx4 *pass = reinterpret_cast<floatx4 *>(sh + 256 + 2 * STAGE + (w & 3) * 4096) + lane;
+            if (some && w < 4) {
+                products(x, qf, kh, km);
+                floatx4 e4;
+                weights([&](int e, float v) {
+                    e4[e & 3] = v;
+                    if ((e & 3) == 3) pass[64 * (e >> 2)] = e4;
+                });
+            } else if (some) {
+                products(dp, gf, kh, km);
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+            if (some && w < 4) {
+                move(dk, g2cur, sg2);
+#pragma unroll
+                for (int s = 0; s < 2; s++) add_half(dk, g2f, x, 1.0f, s);
+            } else if (some) {
+                move(dk, q2cur, sq2);
+#pragma unroll
+                for (int q = 0; q < 4; q++) {
+                    const floatx4 e4 = pass[64 * q];
+#pragma unroll
+                    for (int r = 0; r < 4; r++) x[4 * q + r] = e4[r];
+                }
+                const float fd = gradient(x);
+#pragma unroll
+                for (int s = 0; s < 2; s++) add_half(dk, q2f, dp, fd, s);
             }
         }
         it = nx;
@@ -479,17 +557,23 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
     }
     if (j > last) return;
     const float fv = g2cur * pow2(-kLift), fk = q2cur * pow2(-kLift) * u.scale;
-    float *tk = dest(0, j), *tv = dest(1, j);
+    const bool has_v = NW == 4 || w < 4, has_k = NW == 4 || w >= 4;
+    float *tk = has_k ? dest(0, j) : nullptr, *tv = has_v ? dest(1, j) : nullptr;
 #pragma unroll
     for (int n = 0; n < ND; n++)
 #pragma unroll
         for (int q = 0; q < 4; q++) {
             const int c = 32 * n + 8 * q + 4 * g;
-            const floatx4 xk = floatx4{ldexp_hw(dk[n][4 * q], sd), ldexp_hw(dk[n][4 * q + 1], sd),
-                                       ldexp_hw(dk[n][4 * q + 2], sd), ldexp_hw(dk[n][4 * q + 3], sd)} * fk;
-            const floatx4 xv = floatx4{dv[n][4 * q], dv[n][4 * q + 1], dv[n][4 * q + 2], dv[n][4 * q + 3]} * fv;
-            if (tk) put4(tk, c, u.d, xk, acc);
-            if (tv) put4(tv, c, u.d, xv, acc);
+            const floatx16 &sv = dv[n];
+            const floatx4 xk = floatx4{dk[n][4 * q], dk[n][4 * q + 1], dk[n][4 * q + 2], dk[n][4 * q + 3]};
+            const floatx4 xv = NW == 4 ? floatx4{sv[4 * q], sv[4 * q + 1], sv[4 * q + 2], sv[4 * q + 3]} : xk;
+            if (tk) {
+                floatx4 y;
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = ldexp_hw(xk[e], sd) * fk;
+                put4(tk, c, u.d, y, acc);
+            }
+            if (tv) put4(tv, c, u.d, xv * fv, acc);
         }
 }
 
@@ -497,33 +581,39 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
 template <int DP, int PARTS>
 __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const BwdArgs &a, int i, char *sh, Tables &tab) {
     constexpr bool DOCS = PARTS & kDocs, CAP = PARTS & kCap, SLOPES = PARTS & kSlopes;
-    constexpr int S = DP / 16, ND = DP / 32, HALF = kStep * DP * 4, STAGE = 3 * HALF + 4 * kKeyWords;  // the step's words last
+    constexpr int NW = waves_of(DP), ROWS = 32 * NW, S = DP / 16, ND = DP / 32, HALF = kStep * DP * 4, STAGE = 3 * HALF + 4 * kKeyWords;  // the step's words last
     auto &red = tab.red;
     const Place pl = place_of(i, u.B * u.Hk);
     const int item = pl.item, rb = a.rblocks - 1 - pl.block;
     const int b = item / u.Hk, hk = item - b * u.Hk, rows = u.G * u.lq;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
     const int pre = u.prefix ? u.prefix[b] : 0;
-    const int first = rb * kKeys, last = min(first + kKeys, rows) - 1;
-    const int rr = first + 32 * w + (lane & 31);
+    const int first = rb * ROWS, last = min(first + ROWS, rows) - 1;
+    const int own = first + 32 * w, rr = own + (lane & 31);
     const Row row = row_of(u, hk, min(rr, rows - 1));
     const int64_t tok = (int64_t)b * u.lq + row.t;
     const int pos = row.t + u.off, doc = DOCS ? u.qd[tok] : 0;
     const float slope = SLOPES ? u.slopes[row.h] * kLog2e : 0.0f;
-    const bool live = first + 32 * w <= last;
+    const bool live = own <= last;
     const int64_t kt0 = (int64_t)item * a.nt, rt0 = (int64_t)item * a.nr;
-    const int rt = min((first + 32 * w) / kBlock, a.nr - 1);
+    const int rt = min(own / kBlock, a.nr - 1);
     const RowStats rs = a.rs[rt0 + rt];
-    const RowStats ra = a.rs[rt0 + first / kBlock], rz = a.rs[rt0 + min(first / kBlock + 1, a.nr - 1)];
-    bool bad = ra.bad || rz.bad;
-    const int qlo = min(ra.doc_lo, rz.doc_lo), qhi = max(ra.doc_hi, rz.doc_hi);
+    bool bad = false;
+    int qlo = INT32_MAX, qhi = INT32_MIN;
+#pragma unroll
+    for (int n = 0; n < ROWS / kBlock; n++) {
+        const RowStats r = a.rs[rt0 + min(first / kBlock + n, a.nr - 1)];
+        bad = bad || r.bad;
+        qlo = min(qlo, r.doc_lo);
+        qhi = max(qhi, r.doc_hi);
+    }
     int lo, hi;
     const int i0 = first / u.G + u.off, i1 = last / u.G + u.off;
     key_range(u, i0, i1, pre, lo, hi);
     const int t0 = lo / kBlock, t1 = hi < lo ? t0 - 1 : hi / kBlock;
     uint32_t kt = 0, vt = 0, kl = 0xFFFFFFFFu;
     Stats mk = {}, mv = {};  // the thread's first
-    for (int t = t0 + (int)threadIdx.x, n = 0; t <= t1; t += 256, n++) {
+    for (int t = t0 + (int)threadIdx.x, n = 0; t <= t1; t += 64 * NW, n++) {
         const Stats sk = a.ks[kt0 + t], sv = a.vs[kt0 + t];
         if (n == 0) mk = sk, mv = sv;
         kt = max(kt, sk.top);
@@ -540,14 +630,14 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
     }
     __syncthreads();
 #pragma unroll
-    for (int n = 0; n < 4; n++) {
+    for (int n = 0; n < NW; n++) {
         kt = max(kt, red[n][0]);
         vt = max(vt, red[n][1]);
         kl = min(kl, red[n][2]);
     }
     bad = bad || kt > kMostBits || vt > kMostBits || !even_rows(kt, kl);
     if (__builtin_amdgcn_readfirstlane(bad)) {
-        for (int r = first + 32 * w; r <= min(last, first + 32 * w + 31); r++) plain_dq<DP>(u, p, b, hk, r, lo, hi, pre);
+        for (int r = own; r <= min(last, own + 31); r++) plain_dq<DP>(u, p, b, hk, r, lo, hi, pre);
         return;
     }
     const int ek = kt ? scale_exp(kt) : 0;
@@ -557,7 +647,7 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
         whi = __builtin_amdgcn_readfirstlane(wave_imax(doc));
     }
     if (DOCS) {
-        if (t0 + (int)threadIdx.x <= t1) {
+        if (threadIdx.x < kListed && t0 + (int)threadIdx.x <= t1) {
             static_assert(kListed == 256, "a thread's first block is its entry");
             tab.see[threadIdx.x] = mk.doc_hi >= max(qlo, 0) && mk.doc_lo <= qhi;
         }
@@ -566,7 +656,7 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
     // Q and G fragments of the wavefront's rows, and their values
     u32x4 qh[S], qm[S], gh[S], gm[S];
     {
-        const int half = ((first + 32 * w) / 32) & 1;
+        const int half = own / 32 & 1;
         const char *qf = a.qn + (rt0 + rt) * plane_bytes(DP, 1) + half * HALF + lane * 16;
         const char *gf = a.gn + (rt0 + rt) * plane_bytes(DP, 1) + half * HALF + lane * 16;
 #pragma unroll
@@ -586,37 +676,51 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
     for (int n = 0; n < ND; n++)
 #pragma unroll
         for (int e = 0; e < 16; e++) dq[n][e] = 0.0f;
-    const int wi0 = min(first + 32 * w, last) / u.G + u.off, wi1 = min(first + 32 * w + 31, last) / u.G + u.off;
+    const int wi0 = min(own, last) / u.G + u.off, wi1 = min(own + 31, last) / u.G + u.off;
     const int base = t0 * kBlock, steps = hi < lo ? 0 : (hi - base) / kStep + 1;
     const Band whole_wg(u, i0, i1, pre), mine(u, wi0, wi1, pre);
-    auto next = [&](int it) {
-        it++;
-        const int j0 = base + it * kStep;  // a window leaves a gap behind a prefix
-        if ((j0 >= whole_wg.pre) & (j0 + kStep <= whole_wg.some0)) it = (whole_wg.some0 - base) / kStep;
-        if (DOCS)
-            while (it < steps && it / 2 < kListed && !tab.see[it / 2]) it++;
-        return it < steps ? it : steps;
+    // Keys upwards, in a window from a multiple of `period` steps on and round the range's end: see the keys' role.
+    const int abs0 = base / kStep, up = (abs0 + a.rperiod - 1) / a.rperiod * a.rperiod - abs0, cut = up < steps ? up : 0;
+    int stop = steps;
+    bool more = cut > 0;
+    auto settle = [&](int it) {  // the first step from `it` on to take; -1 behind the last
+        while (true) {
+            const int j0 = base + it * kStep;
+            if (it >= stop) {
+                if (!more) return -1;
+                more = false;
+                it = 0;
+                stop = cut;
+            } else if ((j0 >= whole_wg.pre) & (j0 + kStep <= whole_wg.some0)) {  // a window leaves a gap behind a prefix
+                it = (whole_wg.some0 - base) / kStep;
+            } else if (DOCS && it / 2 < kListed && !tab.see[it / 2]) {
+                it++;
+            } else {
+                return it;
+            }
+        }
     };
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) void *)(sh + 256);
     auto stage = [&](int it, int buf) {
         const int64_t off = (kt0 + t0) * plane_bytes(DP, 1) + (int64_t)it * HALF + lane * 16;
         const uint32_t to = lds0 + (uint32_t)(buf * STAGE);
-        constexpr int PER = HALF / 4096;
         auto one = [&](const char *src, int n) {
 #pragma unroll
-            for (int q = 0; q < PER; q++) load_to_lds(src + off + (4 * q + w) * 1024, to + (uint32_t)(n * HALF + (4 * q + w) * 1024));
+            for (int q = 0; q < HALF / 1024; q += NW)
+                if (HALF / 1024 % NW == 0 || q + w < HALF / 1024)
+                    load_to_lds(src + off + (q + w) * 1024, to + (uint32_t)(n * HALF + (q + w) * 1024));
         };
         one(a.kn, 0);
         one(a.vn, 1);
         one(a.kt, 2);
         if (w == 0) load_to_lds4(a.keys + (2 * (kt0 + t0) + it) * kKeyWords + lane, to + 3 * HALF);
     };
-    int it = next(-1), buf = 0;
-    if (it < steps) stage(it, 0);
-    while (it < steps) {
+    int it = settle(cut), buf = 0;
+    if (it >= 0) stage(it, 0);
+    while (it >= 0) {
         land<0>();
-        const int nx = next(it);
-        if (nx < steps) stage(nx, buf ^ 1);
+        const int nx = settle(it + 1);
+        if (nx >= 0) stage(nx, buf ^ 1);
         const int j0 = base + it * kStep, j1 = j0 + kStep - 1;
         const char *kf = sh + 256 + buf * STAGE + lane * 16, *vf = kf + HALF, *ktf = vf + HALF;
         const int *words = reinterpret_cast<const int *>(sh + 256 + buf * STAGE + 3 * HALF);
@@ -626,20 +730,20 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
             some = some & (whi >= 0) & (dhi >= wlo) & (dlo <= whi);
             one = (wlo == whi) & (dlo == dhi) & (dlo == wlo) & (wlo >= 0);
         }
-        if (some) {
-            const float sk = __int_as_float(words[kKeyScaleK]), sv = __int_as_float(words[kKeyScaleV]);
+        const float sk = __int_as_float(words[kKeyScaleK]), sv = __int_as_float(words[kKeyScaleV]);
+        floatx16 x, dp;
+        auto products = [&](floatx16 &out, const char *f, const u32x4 *fh, const u32x4 *fm) {
+#pragma unroll
+            for (int e = 0; e < 16; e++) out[e] = 0.0f;
+#pragma unroll
+            for (int s = 0; s < S; s++)
+                out = mma3(*reinterpret_cast<const u32x4 *>(f + (2 * s) * 1024),
+                           *reinterpret_cast<const u32x4 *>(f + (2 * s + 1) * 1024), fh[s], fm[s], out);
+        };
+        // x from raw products to the weights E (1 - tanh^2)
+        auto weights = [&]() {
             // K's exponent less the largest; a block of zeros may say anything
             const int step = min(max((words[kKeyScaleK] >> 23) - 127 - ek, -32), 0);
-            floatx16 x, dp;
-#pragma unroll
-            for (int e = 0; e < 16; e++) x[e] = dp[e] = 0.0f;
-#pragma unroll
-            for (int s = 0; s < S; s++) {
-                x = mma3(*reinterpret_cast<const u32x4 *>(kf + (2 * s) * 1024),
-                         *reinterpret_cast<const u32x4 *>(kf + (2 * s + 1) * 1024), qh[s], qm[s], x);
-                dp = mma3(*reinterpret_cast<const u32x4 *>(vf + (2 * s) * 1024),
-                          *reinterpret_cast<const u32x4 *>(vf + (2 * s + 1) * 1024), gh[s], gm[s], dp);
-            }
             const float cs = rs.q * sk;
             const bool whole = mine.all(j0, j1) & one;
             if (CAP) {
@@ -660,20 +764,17 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
             }
             const float fx = CAP ? u.capl2 : u.cl2 * cs, mu = (float)step + m;
             const float gap0 = (float)(pos - j0 - 4 * g);
-            float top = 0.0f;
 #pragma unroll
             for (int e = 0; e < 16; e++) {
                 float y = __builtin_fmaf(x[e], fx, mu);
                 const int o = 8 * (e >> 2) + (e & 3);
                 if (SLOPES) y = __builtin_fmaf(-slope, __builtin_fabsf(gap0 - (float)o), y);
                 if (!whole) y = (reach.has(j0 + 4 * g + o) & (!DOCS || words[kKeyDoc + 4 * g + o] == doc)) ? y : -3e38f;
-                float ds = exp2_hw(y) * __builtin_fmaf(dp[e], sv, -delta);
-                if (CAP) ds *= __builtin_fmaf(-x[e], x[e], 1.0f);
-                dp[e] = ds;
-                top = fmaxf(top, __builtin_fabsf(ds));
+                const float ex = exp2_hw(y);
+                x[e] = CAP ? ex * __builtin_fmaf(-x[e], x[e], 1.0f) : ex;
             }
-            top = pair_max(top);
-            const int sn = grown(top, sd);
+        };
+        auto rescale = [&](int sn) {  // dq's sums to units of 2^sn
             if (__any(sn != sd)) {
                 const int by = sd - sn;
 #pragma unroll
@@ -682,20 +783,36 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
                     for (int e = 0; e < 16; e++) dq[n][e] = ldexp_hw(dq[n][e], by);
                 sd = sn;
             }
-            const float fd = pow2(-sd);
+        };
+        auto gradient = [&]() {  // dp from g . v to D
+            float top = 0.0f;
 #pragma unroll
-            for (int s = 0; s < 2; s++) {
-                float e8[8];
-                u32x4 dh, dm;
-#pragma unroll
-                for (int e = 0; e < 8; e++) e8[e] = dp[8 * s + e] * fd;
-                split8(e8, dh, dm);
-#pragma unroll
-                for (int c = 0; c < ND; c++) {
-                    const char *f = ktf + ((s * ND + c) * 2) * 1024;
-                    dq[c] = mma3(*reinterpret_cast<const u32x4 *>(f), *reinterpret_cast<const u32x4 *>(f + 1024), dh, dm, dq[c]);
-                }
+            for (int e = 0; e < 16; e++) {
+                dp[e] = x[e] * __builtin_fmaf(dp[e], sv, -delta);
+                top = fmaxf(top, __builtin_fabsf(dp[e]));
             }
+            rescale(grown(pair_max(top), sd));
+        };
+        auto add_half = [&](int s) {  // 16 of the step's keys
+            const float fd = pow2(-sd);
+            float e8[8];
+            u32x4 dh, dm;
+#pragma unroll
+            for (int e = 0; e < 8; e++) e8[e] = dp[8 * s + e] * fd;
+            split8(e8, dh, dm);
+#pragma unroll
+            for (int c = 0; c < ND; c++) {
+                const char *f = ktf + ((s * ND + c) * 2) * 1024;
+                dq[c] = mma3(*reinterpret_cast<const u32x4 *>(f), *reinterpret_cast<const u32x4 *>(f + 1024), dh, dm, dq[c]);
+            }
+        };
+        if (some) {
+            products(x, kf, qh, qm);
+            products(dp, vf, gh, gm);
+            weights();
+            gradient();
+#pragma unroll
+            for (int s = 0; s < 2; s++) add_half(s);
         }
         it = nx;
         buf ^= 1;
@@ -714,15 +831,19 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
 }
 
 template <int DP, int PARTS>
-__global__ void __launch_bounds__(256, DP <= 64 ? 2 : 1) k_scored_bwd_mm(Rule u, Ptrs p, BwdArgs a) {
+__global__ void __launch_bounds__(64 * waves_of(DP), DP == 128 ? 1 : 2) k_scored_bwd_mm(Rule u, Ptrs p, BwdArgs a) {
     OM_LDS_POISON();
-    __shared__ __attribute__((aligned(16))) char sh[256 + 2 * (4 * kStep * DP * 4 + 1024)];  // no stage at LDS address 0
+    __shared__ __attribute__((aligned(16))) char sh[256 + 2 * (4 * kStep * DP * 4 + 1024) + (waves_of(DP) == 8 ? 16384 : 0)];
     __shared__ Tables tab;
-    // The roles' workgroups in proportion, each in its order of falling work: the longest of both start first.
-    const int64_t id = blockIdx.x, all = gridDim.x;
-    const int k = (int)(id * a.keys_wgs / all);
-    if ((int)((id + 1) * a.keys_wgs / all) > k) keys_role<DP, PARTS>(u, p, a, k, sh, tab);
-    else rows_role<DP, PARTS>(u, p, a, (int)id - k, sh, tab);
+    // The roles' workgroups in proportion, each in its order of falling work: the longest of both start first. Eight ids a
+    // turn, one on each XCD, so that a role's index keeps its remainder by eight and an XCD its items.
+    const int64_t id = blockIdx.x >> 3, all = gridDim.x >> 3, kg = (a.keys_wgs + 7) / 8;
+    const int k = (int)(id * kg / all), x = blockIdx.x & 7;
+    if ((int)((id + 1) * kg / all) > k) {
+        if (8 * k + x < a.keys_wgs) keys_role<DP, PARTS>(u, p, a, 8 * k + x, sh, tab);
+    } else if (8 * ((int)id - k) + x < a.rows_wgs) {
+        rows_role<DP, PARTS>(u, p, a, 8 * ((int)id - k) + x, sh, tab);
+    }
 }
 
 // dk and dv from the splits' sums, in split order; a thread per value.
@@ -752,7 +873,8 @@ om_status bwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p) {
     a.nt = (u.lk + kBlock - 1) / kBlock;
     a.nr = (int)((rows + kBlock - 1) / kBlock);
     a.kblocks = (u.lk + kKeys - 1) / kKeys;
-    a.rblocks = (int)((rows + kKeys - 1) / kKeys);
+    const int rows_wg = 32 * waves_of(dp);
+    a.rblocks = (int)((rows + rows_wg - 1) / rows_wg);
     const bool keys = p.dk || p.dv;
     // Split the rows of dk and dv while those workgroups leave CUs idle, in pieces of at least eight blocks.
     int64_t ns = 1, wk = items * a.kblocks;
@@ -762,8 +884,13 @@ om_status bwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p) {
     a.nsplit = (int)ns;
     wk = keys ? wk * a.nsplit : 0;
     const int64_t wr = p.dq ? items * a.rblocks : 0, jobs = items * (2 * (int64_t)a.nt + a.nr);
-    OM_REQUIRE(ctx, wk + wr <= INT32_MAX && jobs <= INT32_MAX, "%s: too many row blocks", what);
+    OM_REQUIRE(ctx, wk + wr <= INT32_MAX - 64 && jobs <= INT32_MAX, "%s: too many row blocks", what);
     a.keys_wgs = (int)wk;
+    a.rows_wgs = (int)wr;
+    // a window's whole range: of rows that see a workgroup's keys, in blocks a split; of keys that its rows see, in steps
+    const int64_t sides = u.causal ? 1 : 2, none = INT32_MAX / 2;
+    a.kperiod = (int)(u.window ? std::min(none, (sides * u.window + kKeys) * u.G / kBlock + 1) : none);
+    a.rperiod = (int)(u.window ? std::min(none, (sides * u.window + rows_wg / u.G) / kStep + 2) : none);
     const int64_t kp = plane_bytes(dp, items * a.nt), rp = plane_bytes(dp, items * a.nr);
     const int64_t vals = items * a.nr * kBlock * kRowValues * (int64_t)sizeof(float);
     const int64_t words = 2 * items * a.nt * kKeyWords * (int64_t)sizeof(float);
@@ -804,8 +931,8 @@ om_status bwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p) {
         };
         vec ? split(k_scored_split_bwd<DP, true>) : split(k_scored_split_bwd<DP, false>);
         by_parts(parts_of(u), [&](auto pc) {
-            hipLaunchKernelGGL((k_scored_bwd_mm<DP, decltype(pc)::value>), dim3((unsigned)(wk + wr)), dim3(256), 0, ctx->stream, u,
-                               p, a);
+            hipLaunchKernelGGL((k_scored_bwd_mm<DP, decltype(pc)::value>), dim3((unsigned)(8 * ((wk + 7) / 8 + (wr + 7) / 8))), dim3(64 * waves_of(DP)), 0,
+                               ctx->stream, u, p, a);
         });
     });
     if (part) {

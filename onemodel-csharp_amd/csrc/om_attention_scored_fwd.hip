@@ -5,6 +5,9 @@
 // split, and are the operand of O^T += V^T E^T as they stand. K and V come split from scratch, straight into LDS, a
 // ring of steps, one barrier each. The running maximum m moves only when some lane's maximum grows by more than 2^2: E then
 // stays below 2^14 with its 2^12 of headroom, and the accumulators are left alone in most steps.
+#include <algorithm>
+#include <cmath>
+
 #include "om_attention_scored_split.hpp"
 
 namespace {
@@ -429,16 +432,39 @@ namespace osc {
 
 // The forward by the matrix cores, d up to 128; *joins gets the number of splits left to join (1: none) and *part where
 // they lie.
+// Into how many pieces to split each row block's keys: the number whose time is least by what was measured of the parts. A
+// workgroup takes 5 us before its first step of 32 keys; a step of 64 values a head takes 1.2 us alone on its CU and 0.25 us
+// more for each neighbour there, in proportion for other widths; pieces are joined at 4 TB/s after another launch. Work that
+// differs from block to block (a causal rule over many rows) fills the chip up to the longest piece, even work goes in rounds.
+// 500 rows behind 4096 keys, 2 x 12 heads of 64: one round of 8 pieces 58 us with its join, two of 16 69 us. 512 x 512 in
+// documents, 8 x 12 heads: whole rows 33 us, 2 pieces 42 us with their join.
+static int64_t pieces(const om_ctx *ctx, const Rule &u, int dp, int64_t wgs, int64_t rows) {
+    const int64_t most = std::min<int64_t>((u.lk + kBlock - 1) / kBlock / 4, 64);
+    const double cus = ctx->num_cus, occ = dp == 32 ? 4 : dp == 64 ? 3 : 2, wide = dp / 64.0;
+    const double seen = u.window ? std::min<double>(u.lk, (u.causal ? 1.0 : 2.0) * u.window + kRows / u.G) : u.lk;
+    const double longest = seen / 32;
+    const bool uneven = u.causal && !u.window && 2 * (int64_t)u.lq > u.lk;
+    const double mean = uneven ? longest * (1.0 - 0.5 * u.lq / u.lk) : longest;
+    int64_t best = 1;
+    double least = 0.0;
+    for (int64_t ns = 1; ns <= std::max<int64_t>(most, 1); ns++) {
+        const double n = (double)wgs * ns, there = std::min(occ, std::ceil(n / cus));
+        const double step = (1.2 + 0.25 * (there - 1.0)) * wide, one = 5.0 + step * longest / ns;
+        double us = uneven ? std::max(one, n / (occ * cus) * (5.0 + step * mean / ns)) : std::ceil(n / (occ * cus)) * one;
+        if (ns > 1) us += 4.0 + 2.0 * ns * rows * (u.d + 2) * sizeof(float) / 4e6;
+        if (ns == 1 || us < least) {
+            best = ns;
+            least = us;
+        }
+    }
+    return best;
+}
+
 om_status fwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p, int *joins, float **part) {
     const int nt = (u.lk + kBlock - 1) / kBlock, rows = u.G * u.lq, blocks = (rows + kRows - 1) / kRows;
     const int64_t items = (int64_t)u.B * u.Hk, wgs = items * blocks, all = items * rows;
     const int dp = u.d <= 32 ? 32 : u.d <= 64 ? 64 : u.d <= 96 ? 96 : 128;
-    // Split the keys into pieces of at least four blocks until there are twice the workgroups that the chip holds at once
-    // (their lengths differ under a causal rule, and the short ones fill up behind the long ones).
-    const int64_t want = 2 * (dp == 32 ? 4 : dp == 64 ? 3 : 2) * (int64_t)ctx->num_cus;
-    int64_t ns = wgs >= want ? 1 : want / wgs;
-    ns = ns > nt / 4 ? nt / 4 : ns;
-    ns = ns < 1 ? 1 : ns;
+    const int64_t ns = pieces(ctx, u, dp, wgs, all);
     OM_REQUIRE(ctx, wgs * ns <= INT32_MAX && 2 * items * nt <= INT32_MAX, "om_attention_fwd_scored: too many row blocks");
     const int64_t plane = plane_bytes(dp, items * nt), stats = items * nt * (int64_t)sizeof(Stats);
     const int64_t words = 2 * items * nt * kKeyWords * (int64_t)sizeof(float);
