@@ -48,16 +48,16 @@ __global__ void __launch_bounds__(256) k_scored_split_bwd(Rule u, Ptrs p, SplitO
     OM_LDS_POISON();
     __shared__ __attribute__((aligned(16))) char lds[DP * 256];
     __shared__ uint32_t sh[48];
-    const int keys = u.B * u.Hk * nt;
+    const int keys = u.B * u.Hk * nt, rows = u.B * u.Hk * nr;
     int i = blockIdx.x;
-    if (i < 2 * keys) {
+    if (i < rows) {  // the longer jobs first
+        const int bh = i / nr;
+        split_rows<DP, VEC>(u, p, bh / u.Hk, bh % u.Hk, i % nr, i, ro, lds, sh);
+    } else {
+        i -= rows;
         const int at = i % keys, bh = at / nt;
         const bool v = i >= keys;
         split_keys<DP, VEC>(u, v ? p.v : p.k, p.ldkv, bh / u.Hk, bh % u.Hk, at % nt, at, v ? vo : ko, lds, sh);
-    } else {
-        i -= 2 * keys;
-        const int bh = i / nr;
-        split_rows<DP, VEC>(u, p, bh / u.Hk, bh % u.Hk, i % nr, i, ro, lds, sh);
     }
 }
 

@@ -19,12 +19,19 @@ struct Share {
     static constexpr int NCH = (DP + 63) / 64;
     floatx4 x[4][NCH];
     template <bool VEC>
-    __device__ __forceinline__ void load(int i, const float *row, bool there, int d) {
+    __device__ __forceinline__ void load(int i, const float *row, int d) {
 #pragma unroll
         for (int n = 0; n < NCH; n++) {
             const int c = 64 * n + 4 * (threadIdx.x & 15);
-            x[i][n] = there && c < DP ? load4<VEC>(row, c, d) : floatx4{0.f, 0.f, 0.f, 0.f};
+            x[i][n] = c < DP ? load4<VEC>(row, c, d) : floatx4{0.f, 0.f, 0.f, 0.f};
         }
+    }
+    // Zeros in place of a row that does not count, whatever it holds: once it is here, so that the loads wait for nothing.
+    __device__ __forceinline__ void keep(int i, bool on) {
+#pragma unroll
+        for (int n = 0; n < NCH; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[i][n][e] = on ? x[i][n][e] : 0.0f;
     }
     // Largest magnitude of row i as bits (infinities and NaN above every finite one), the same in the row's 16 lanes.
     __device__ __forceinline__ uint32_t row_top(int i) const {
@@ -112,16 +119,21 @@ __device__ __forceinline__ void split_keys(const Rule &u, const float *src, int6
                                            const SplitOut &o, char *lds, uint32_t *sh) {
     Share<DP> s;
     uint32_t top4[4], top, low;
-    int dlo = INT32_MAX, dhi = -1;
+    int dlo = INT32_MAX, dhi = -1, doc[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int j = t * kBlock + 4 * (threadIdx.x >> 4) + i;
         const int64_t tok = (int64_t)b * u.lk + min(j, u.lk - 1);
-        const int doc = j >= u.lk ? -1 : u.kd ? u.kd[tok] : 0;
-        s.template load<VEC>(i, src + tok * ld + (int64_t)hk * u.d, doc >= 0, u.d);
+        doc[i] = u.kd ? u.kd[tok] : 0;
+        s.template load<VEC>(i, src + tok * ld + (int64_t)hk * u.d, u.d);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const bool there = t * kBlock + 4 * (int)(threadIdx.x >> 4) + i < u.lk;
+        s.keep(i, there && doc[i] >= 0);
         top4[i] = s.row_top(i);
-        dhi = max(dhi, doc);
-        dlo = min(dlo, j >= u.lk ? INT32_MAX : doc);
+        dhi = max(dhi, there ? doc[i] : -1);
+        dlo = min(dlo, there ? doc[i] : INT32_MAX);
     }
     block_top(top4, top, low, sh);
     const bool ok = in_range(top) && even_rows(top, low);
@@ -209,34 +221,41 @@ __device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, 
     constexpr int NCH = Share<DP>::NCH;
     const int rows = u.G * u.lq;
     const int64_t all = (int64_t)u.B * u.Hk * rows;
-    Share<DP> s, g;
+    Share<DP> s, g, ov;
     float rl[4], w[4], delta[4], m[4];
     uint32_t qt[4], gt[4];
-    int dlo = INT32_MAX, dhi = INT32_MIN;
+    int dlo = INT32_MAX, dhi = INT32_MIN, doc[4];
     bool bad = false;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const Row row = row_of(u, hk, min(t * kBlock + 4 * (int)(threadIdx.x >> 4) + i, rows - 1));
+        const int64_t tok = (int64_t)b * u.lq + row.t, sr = stat_at(u, b, row);
+        m[i] = p.st[sr];
+        rl[i] = p.st[all + sr];
+        doc[i] = u.qd ? u.qd[tok] : 0;
+        s.template load<VEC>(i, p.q + tok * p.ldq + (int64_t)row.h * u.d, u.d);
+        g.template load<VEC>(i, p.g + tok * p.ldg + (int64_t)row.h * u.d, u.d);
+        ov.template load<VEC>(i, p.o + tok * p.ldo + (int64_t)row.h * u.d, u.d);
+    }
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const int rr = t * kBlock + 4 * (threadIdx.x >> 4) + i;
         const bool there = rr < rows;
         const Row row = row_of(u, hk, min(rr, rows - 1));
-        const int64_t tok = (int64_t)b * u.lq + row.t, sr = stat_at(u, b, row);
-        m[i] = p.st[sr];
-        rl[i] = there ? p.st[all + sr] : 0.0f;
+        if (!there) rl[i] = 0.0f;
         const bool on = rl[i] != 0.0f;
         if (there) {
-            const int doc = u.qd ? u.qd[tok] : 0;
-            dlo = min(dlo, doc);
-            dhi = max(dhi, doc);
+            dlo = min(dlo, doc[i]);
+            dhi = max(dhi, doc[i]);
         }
-        s.template load<VEC>(i, p.q + tok * p.ldq + (int64_t)row.h * u.d, on, u.d);
-        g.template load<VEC>(i, p.g + tok * p.ldg + (int64_t)row.h * u.d, on, u.d);
-        Share<DP> ov;
-        ov.template load<VEC>(0, p.o + tok * p.ldo + (int64_t)row.h * u.d, on, u.d);
+        s.keep(i, on);
+        g.keep(i, on);
+        ov.keep(i, on);
         float dot = 0.0f;
 #pragma unroll
         for (int n = 0; n < NCH; n++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) dot = __builtin_fmaf(g.x[i][n][e], ov.x[0][n][e], dot);
+            for (int e = 0; e < 4; e++) dot = __builtin_fmaf(g.x[i][n][e], ov.x[i][n][e], dot);
         dot = row_sum(dot);
         qt[i] = s.row_top(i);
         gt[i] = g.row_top(i);
@@ -253,7 +272,7 @@ __device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, 
             o.v[row_value(r, kRowDelta)] = delta[i];
             o.v[row_value(r, kRowPos)] = __int_as_float(row.t + u.off);
             o.v[row_value(r, kRowSlope)] = u.slopes ? u.slopes[row.h] * kLog2e : 0.0f;
-            o.v[row_value(r, kRowDoc)] = __int_as_float(u.qd ? u.qd[tok] : 0);
+            o.v[row_value(r, kRowDoc)] = __int_as_float(doc[i]);
             o.v[row_value(r, kRowW)] = w[i];
         }
     }
