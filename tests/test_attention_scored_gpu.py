@@ -491,3 +491,103 @@ def test_decoder_attention_as_a_user_runs_it(dev):
     near(dev.get(O), o.reshape(rows, -1))
     back = R.rope(np.concatenate([dq.reshape(rows, H, d), dk.reshape(rows, Hk, d)], 1), pos, 32, "half", f, back=True)
     near(dev.get(DX), np.concatenate([back, dv.reshape(rows, Hk, d)], 1).reshape(rows, w))
+
+
+PARTS = {
+    "plain": {},
+    "documents": dict(docs=1),
+    "cap": dict(cap=6.0),
+    "slopes": dict(slopes=True),
+    "documents-cap": dict(docs=1, cap=6.0),
+    "documents-slopes": dict(docs=1, slopes=True),
+    "cap-slopes": dict(cap=6.0, slopes=True),
+    "all": dict(docs=1, cap=6.0, slopes=True),
+}
+
+
+@pytest.mark.parametrize("d", [30, 64, 72, 104, 128])
+@pytest.mark.parametrize("part", PARTS, ids=PARTS.keys())
+def test_every_part_at_every_width(dev, part, d):
+    kw = dict(PARTS[part])
+    lq, lk = 90, 170
+    if kw.pop("docs", 0):
+        kw.update(qdoc=docs(1, lq, 5, 2), kdoc=docs(1, lk, 6, 2))
+    both(Case(dev, 1, 4, 2, lq, lk, d, seed=31, causal=1, **kw))
+
+
+@pytest.mark.parametrize("kw", [dict(causal=1, window=100), dict(window=70), dict(causal=1, window=50, prefix=[120]),
+                                dict(causal=1, window=257, prefix=[3]), dict(causal=1, window=1), dict(causal=1, window=64, slopes=True)],
+                         ids=str)
+@pytest.mark.parametrize("s", [(1, 2, 1, 700, 700, 64), (1, 4, 1, 330, 901, 128), (1, 3, 3, 901, 330, 40), (1, 4, 1, 512, 512, 80)],
+                         ids=str)
+def test_windows_over_many_blocks(dev, s, kw):
+    both(Case(dev, *s, seed=32, **kw))
+
+
+@pytest.mark.parametrize("lens", [(40, 16700), (16700, 40)], ids=str)
+def test_more_blocks_than_are_listed(dev, lens):
+    """Documents over more than 256 blocks of one side: those past the list are visited and masked key by key."""
+    lq, lk = lens
+    both(Case(dev, 1, 1, 1, lq, lk, 32, seed=33, qdoc=docs(1, lq, 7, 3), kdoc=docs(1, lk, 8, 3)))
+
+
+@pytest.mark.parametrize("s", [(1, 4, 1, 300, 700, 64), (1, 4, 1, 300, 700, 96), (1, 8, 2, 300, 700, 128)], ids=str)
+def test_accumulation_and_outputs_left_out_with_pieces(dev, s):
+    """Sizes whose rows and keys are cut into pieces that a further launch joins."""
+    c = Case(dev, *s, seed=34, causal=1, cap=9.0)
+    want = c.reference()
+    near(c.forward(), want[0])
+    for got, ref, fl in zip(c.backward(acc=1, start=2.0), want[1:], (*c.floor(), 0.0)):
+        near(got, ref + 2.0, floor=fl)
+    for i in range(3):
+        got = c.backward(want=[int(n == i) for n in range(3)])
+        near(got[i], want[1 + i], floor=(*c.floor(), 0.0)[i])
+        assert all((got[n] == 5.0).all() for n in range(3) if n != i)
+
+
+@pytest.mark.parametrize("s", [(1, 4, 1, 300, 300, 32), (1, 4, 1, 300, 300, 96), (1, 4, 2, 600, 600, 128)], ids=str)
+@pytest.mark.parametrize("ratio", [1e5, 1e12])
+def test_values_of_very_different_size_at_every_width(dev, s, ratio):
+    """As test_rows_of_very_different_size, in shared heads and over pieces; the larger ratio is summed row by row."""
+    L = s[3]
+    ids = (np.arange(L)[None] >= 150).astype(np.int32)
+    c = Case(dev, *s, seed=35, causal=1, cap=12.0, qdoc=ids, kdoc=ids)
+    c.v[:, 150:] *= np.float32(ratio)
+    c.g[:, 150:] *= np.float32(1.0 / ratio)
+    want = c.reference()
+    for g, w, n in zip([c.forward()] + c.backward(), want, ("o", "dq", "dk", "dv")):
+        for part in (slice(0, 150), slice(150, L)):
+            near(g[:, part], w[:, part], what=(n, part))
+
+
+@pytest.mark.parametrize("where", ["q", "k", "v", "g"])
+def test_one_infinity_leaves_other_heads_alone(dev, where):
+    """A value that the matrix products cannot hold sends its own head's rows to the plain sums, no other head's."""
+    a = Case(dev, 1, 4, 2, 200, 200, 96, seed=36, causal=1)
+    b = Case(dev, 1, 4, 2, 200, 200, 96, seed=36, causal=1)
+    getattr(b, where)[0, 100, 0, 5] = np.inf
+    want = a.reference()
+    for g, w in zip([b.forward()] + b.backward(), want):
+        n = g.shape[2] // 2  # the second key head and its query heads
+        near(g[:, :, n:], w[:, :, n:], floor=max(a.floor()))
+        assert np.isfinite(g[:, :, n:]).all()
+
+
+def _drawn(n):
+    r = rng_of(37, n)
+    Hk, G, d = int(r.integers(1, 4)), int(r.integers(1, 5)), int(r.choice([8, 24, 32, 48, 64, 80, 96, 112, 128]))
+    lq, lk = (int(np.exp(r.uniform(np.log(8), np.log(600)))) for _ in range(2))
+    kw = dict(causal=int(r.integers(2)), cap=float(r.choice([0.0, 3.0, 30.0])), slopes=bool(r.integers(2)),
+              window=int(r.choice([0, 0, 5, 60, 300])))
+    if r.integers(2):
+        kw["prefix"] = [int(r.integers(0, lk + 20))]
+    if r.integers(2):
+        kw.update(qdoc=docs(1, lq, n, 3), kdoc=docs(1, lk, n + 1, 3))
+    return (1, Hk * G, Hk, lq, lk, d), kw
+
+
+@pytest.mark.parametrize("n", range(30))
+def test_drawn_rules(dev, n):
+    s, kw = _drawn(n)
+    print(s, {k: v for k, v in kw.items() if "doc" not in k}, flush=True)
+    both(Case(dev, *s, seed=n, **kw))
