@@ -439,8 +439,15 @@ void join(om_ctx *ctx, const Rule &u, const Ptrs &p, int nsplit, const float *pa
     u.d % 4 == 0 ? go(k_scored_join<4>, 4) : go(k_scored_join<1>, 1);
 }
 
-// The matrix kernels take 32 rows at a time.
-bool by_matrix(const Rule &u) { return u.d <= 128 && (int64_t)u.G * u.lq >= 32 && u.lk >= 1; }
+// The matrix kernels run where there is work enough: below, their splitting pass and half-filled tiles cost more than the row
+// kernels' whole call; and fewer than eight rows would leave most of a tile empty. In us, forward / backward, by rows
+// against by matrix: 4 heads of 31 | 32 rows, 512 keys of 64 values (64 thousand pairs) 14 / 34, 21 / 41; 4096 keys (half a
+// million) 42 / 297, 25 / 50; 96 heads of 64 keys (196 thousand) 19 / 22, 13 / 20; at 128 values 24 heads of 512 keys (380
+// thousand) 32 / 64, 33 / 72; of 4096 keys 173 / 485, 61 / 179.
+bool by_matrix(const Rule &u) {
+    const int64_t rows = (int64_t)u.G * u.lq;
+    return u.d <= 128 && rows >= 8 && rows * u.lk * u.B * u.Hk >= 1024 * (int64_t)((u.d + 31) / 32 * 32);
+}
 
 om_status fwd_by_rows(om_ctx *ctx, const Rule &u, const Ptrs &p) {
     const bool vec = u.d % 4 == 0 && p.ldq % 4 == 0 && p.ldkv % 4 == 0 && al16(p.q) && al16(p.k) && al16(p.v);

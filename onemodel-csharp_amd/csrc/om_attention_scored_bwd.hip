@@ -37,10 +37,11 @@ struct BwdArgs {
     const RowStats *rs;
     int nt, nr;                      // blocks of 64 keys and rows of a head
     int kblocks, rblocks;            // workgroups along them
-    int nsplit;                      // splits of each block of keys' rows for dk and dv
+    int nsplit, qsplit;              // splits of each block of keys' rows for dk and dv, of each block of rows' keys for dq
     int keys_wgs, rows_wgs;          // workgroups of the roles
     int kperiod, rperiod;            // where the roles' sweeps begin: at multiples, in blocks of rows and in steps of keys
     float *part;                     // [split][B Hk][lk][2][d] (dk, dv), NULL for one split
+    float *qpart;                    // [split][B Hk][G lq][d] (dq), NULL for one split
 };
 
 template <int DP, bool VEC>
@@ -120,9 +121,10 @@ __device__ __forceinline__ float join4(float v) {
     return s;
 }
 
-// dq of one row by one wavefront.
+// dq of one row over keys lo .. hi by one wavefront, to `to`.
 template <int DP>
-__device__ __forceinline__ void plain_dq(const Rule &u, const Ptrs &p, int b, int hk, int rr, int lo, int hi, int pre) {
+__device__ __forceinline__ void plain_dq(const Rule &u, const Ptrs &p, int b, int hk, int rr, int lo, int hi, int pre, float *to,
+                                         int acc) {
     constexpr int NC = (DP + 63) / 64;
     const int lane = threadIdx.x & 63, l16 = lane & 15, st = lane >> 4;
     Pair<NC> r;
@@ -145,14 +147,13 @@ __device__ __forceinline__ void plain_dq(const Rule &u, const Ptrs &p, int b, in
 #pragma unroll
             for (int e = 0; e < 4; e++) dq[n][e] = __builtin_fmaf(ds, k[n][e], dq[n][e]);
     }
-    float *to = p.dq + r.tok * p.lddq + (int64_t)r.h * u.d;
 #pragma unroll
     for (int n = 0; n < NC; n++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
             const float s = join4(dq[n][e]) * u.scale;
             const int c = 64 * n + 4 * l16 + e;
-            if (st == 0 && c < u.d) to[c] = p.acc ? to[c] + s : s;
+            if (st == 0 && c < u.d) to[c] = acc ? to[c] + s : s;
         }
 }
 
@@ -584,7 +585,7 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
     constexpr int NW = waves_of(DP), ROWS = 32 * NW, S = DP / 16, ND = DP / 32, HALF = kStep * DP * 4, STAGE = 3 * HALF + 4 * kKeyWords;  // the step's words last
     auto &red = tab.red;
     const Place pl = place_of(i, u.B * u.Hk);
-    const int item = pl.item, rb = a.rblocks - 1 - pl.block;
+    const int item = pl.item, split = pl.block % a.qsplit, rb = a.rblocks - 1 - pl.block / a.qsplit;
     const int b = item / u.Hk, hk = item - b * u.Hk, rows = u.G * u.lq;
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), g = lane >> 5;
     const int pre = u.prefix ? u.prefix[b] : 0;
@@ -610,7 +611,16 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
     int lo, hi;
     const int i0 = first / u.G + u.off, i1 = last / u.G + u.off;
     key_range(u, i0, i1, pre, lo, hi);
-    const int t0 = lo / kBlock, t1 = hi < lo ? t0 - 1 : hi / kBlock;
+    // the split's equal share of the blocks
+    const int c0 = lo / kBlock, c1 = hi < lo ? c0 - 1 : hi / kBlock, per = (c1 - c0 + a.qsplit) / a.qsplit;
+    const int t0 = c0 + split * per, t1 = min(c1, t0 + per - 1);
+    lo = max(lo, t0 * kBlock);
+    hi = min(hi, t1 * kBlock + kBlock - 1);
+    auto dest = [&](int r, const Row &to) {  // dq of row r
+        return a.qpart ? a.qpart + (((int64_t)split * u.B * u.Hk + item) * rows + r) * u.d
+                       : p.dq + ((int64_t)b * u.lq + to.t) * p.lddq + (int64_t)to.h * u.d;
+    };
+    const int acc = a.qpart ? 0 : p.acc;
     uint32_t kt = 0, vt = 0, kl = 0xFFFFFFFFu;
     Stats mk = {}, mv = {};  // the thread's first
     for (int t = t0 + (int)threadIdx.x, n = 0; t <= t1; t += 64 * NW, n++) {
@@ -637,7 +647,7 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
     }
     bad = bad || kt > kMostBits || vt > kMostBits || !even_rows(kt, kl);
     if (__builtin_amdgcn_readfirstlane(bad)) {
-        for (int r = own; r <= min(last, own + 31); r++) plain_dq<DP>(u, p, b, hk, r, lo, hi, pre);
+        for (int r = own; r <= min(last, own + 31); r++) plain_dq<DP>(u, p, b, hk, r, lo, hi, pre, dest(r, row_of(u, hk, r)), acc);
         return;
     }
     const int ek = kt ? scale_exp(kt) : 0;
@@ -819,14 +829,14 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
     }
     if (rr > last) return;
     const float f = u.scale * pow2(ek - kLift);
-    float *to = p.dq + tok * p.lddq + (int64_t)row.h * u.d;
+    float *to = dest(rr, row);
 #pragma unroll
     for (int n = 0; n < ND; n++)
 #pragma unroll
         for (int q = 0; q < 4; q++) {
             const floatx4 v = floatx4{ldexp_hw(dq[n][4 * q], sd), ldexp_hw(dq[n][4 * q + 1], sd),
                                       ldexp_hw(dq[n][4 * q + 2], sd), ldexp_hw(dq[n][4 * q + 3], sd)} * f * wr;
-            put4(to, 32 * n + 8 * q + 4 * g, u.d, v, p.acc);
+            put4(to, 32 * n + 8 * q + 4 * g, u.d, v, acc);
         }
 }
 
@@ -846,19 +856,32 @@ __global__ void __launch_bounds__(64 * waves_of(DP), DP == 128 ? 1 : 2) k_scored
     }
 }
 
-// dk and dv from the splits' sums, in split order; a thread per value.
-__global__ void __launch_bounds__(256) k_scored_join_dkv(Rule u, Ptrs p, int nsplit, const float *__restrict__ part) {
+// dk and dv, then dq, from their splits' sums, in split order; a thread per value.
+__global__ void __launch_bounds__(256) k_scored_join_bwd(Rule u, Ptrs p, int64_t dkv, int nsplit, const float *__restrict__ part,
+                                                         int64_t dq, int qsplit, const float *__restrict__ qpart) {
     OM_LDS_POISON();
-    const int64_t each = (int64_t)u.B * u.Hk * u.lk * 2 * u.d, f = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (f >= each) return;
+    int64_t f = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (f >= dkv + dq) return;
+    const bool q = f >= dkv;
+    const int64_t each = q ? dq : dkv;
+    const float *from = q ? qpart : part;
+    const int n = q ? qsplit : nsplit;
+    if (q) f -= dkv;
     float s = 0.0f;
-    for (int n = 0; n < nsplit; n++) s += part[n * each + f];
-    const int c = (int)(f % u.d), which = (int)(f / u.d % 2);
-    const int64_t key = f / (2 * u.d), item = key / u.lk;
-    float *base = which ? p.dv : p.dk;
-    if (!base) return;
-    float *to = base + ((item / u.Hk) * u.lk + key % u.lk) * p.lddkv + (item % u.Hk) * u.d + c;
-    *to = p.acc ? *to + s : s;
+    for (int i = 0; i < n; i++) s += from[i * each + f];
+    const int c = (int)(f % u.d);
+    float *to;
+    if (q) {
+        const int64_t r = f / u.d, rows = (int64_t)u.G * u.lq, item = r / rows;
+        const Row row = row_of(u, (int)(item % u.Hk), (int)(r - item * rows));
+        to = p.dq + ((item / u.Hk) * u.lq + row.t) * p.lddq + (int64_t)row.h * u.d;
+    } else {
+        const int64_t key = f / (2 * u.d), item = key / u.lk;
+        to = f / u.d % 2 ? p.dv : p.dk;
+        if (!to) return;
+        to += ((item / u.Hk) * u.lk + key % u.lk) * p.lddkv + (item % u.Hk) * u.d;
+    }
+    to[c] = p.acc ? to[c] + s : s;
 }
 
 }  // namespace
@@ -883,7 +906,14 @@ om_status bwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p) {
     ns = ns < 1 ? 1 : ns;
     a.nsplit = (int)ns;
     wk = keys ? wk * a.nsplit : 0;
-    const int64_t wr = p.dq ? items * a.rblocks : 0, jobs = items * (2 * (int64_t)a.nt + a.nr);
+    // The keys of dq alike: 32 rows of 4 heads over 4096 keys of 64 values, 225 us whole.
+    int64_t qs = 1, wr = items * a.rblocks;
+    if (wr < 2 * ctx->num_cus) qs = 2 * ctx->num_cus / wr;
+    qs = qs > a.nt / 8 ? a.nt / 8 : qs;
+    qs = qs < 1 ? 1 : qs;
+    a.qsplit = (int)qs;
+    wr = p.dq ? wr * a.qsplit : 0;
+    const int64_t jobs = items * (2 * (int64_t)a.nt + a.nr);
     OM_REQUIRE(ctx, wk + wr <= INT32_MAX - 64 && jobs <= INT32_MAX, "%s: too many row blocks", what);
     a.keys_wgs = (int)wk;
     a.rows_wgs = (int)wr;
@@ -894,10 +924,11 @@ om_status bwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p) {
     const int64_t kp = plane_bytes(dp, items * a.nt), rp = plane_bytes(dp, items * a.nr);
     const int64_t vals = items * a.nr * kBlock * kRowValues * (int64_t)sizeof(float);
     const int64_t words = 2 * items * a.nt * kKeyWords * (int64_t)sizeof(float);
+    const int64_t qpart = p.dq && a.qsplit > 1 ? (int64_t)sizeof(float) * a.qsplit * items * rows * u.d : 0;
     const int64_t part = keys && a.nsplit > 1 ? (int64_t)sizeof(float) * a.nsplit * items * u.lk * 2 * u.d : 0;
     const int64_t stats = 2 * items * a.nt * (int64_t)sizeof(Stats) + items * a.nr * (int64_t)sizeof(RowStats);
     float *scr;
-    if (om_status s = om::scratch2(ctx, (uint64_t)(3 * kp + 4 * rp + vals + words + stats + part), &scr)) return s;
+    if (om_status s = om::scratch2(ctx, (uint64_t)(3 * kp + 4 * rp + vals + words + stats + part + qpart), &scr)) return s;
     char *at = reinterpret_cast<char *>(scr);
     auto take = [&](int64_t bytes) {
         char *x = at;
@@ -921,6 +952,7 @@ om_status bwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p) {
     a.vs = vo.stats = reinterpret_cast<Stats *>(take(items * a.nt * (int64_t)sizeof(Stats)));
     a.rs = ro.stats = reinterpret_cast<RowStats *>(take(items * a.nr * (int64_t)sizeof(RowStats)));
     a.part = part ? reinterpret_cast<float *>(take(part)) : nullptr;
+    a.qpart = qpart ? reinterpret_cast<float *>(take(qpart)) : nullptr;
     auto al16 = [](const void *x) { return ((uintptr_t)x & 15) == 0; };
     const bool vec = u.d % 4 == 0 && p.ldq % 4 == 0 && p.ldkv % 4 == 0 && p.ldo % 4 == 0 && p.ldg % 4 == 0 && al16(p.q) &&
                      al16(p.k) && al16(p.v) && al16(p.o) && al16(p.g);
@@ -935,10 +967,10 @@ om_status bwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p) {
                                ctx->stream, u, p, a);
         });
     });
-    if (part) {
-        const int64_t values = items * u.lk * 2 * u.d;
-        hipLaunchKernelGGL(k_scored_join_dkv, dim3((unsigned)((values + 255) / 256)), dim3(256), 0, ctx->stream, u, p, a.nsplit,
-                           a.part);
+    if (part || qpart) {
+        const int64_t dkv = part ? items * u.lk * 2 * u.d : 0, dq = qpart ? items * rows * u.d : 0;
+        hipLaunchKernelGGL(k_scored_join_bwd, dim3((unsigned)((dkv + dq + 255) / 256)), dim3(256), 0, ctx->stream, u, p, dkv,
+                           a.nsplit, a.part, dq, a.qsplit, a.qpart);
     }
     return OM_LAUNCH_CHECK(ctx, what);
 }
