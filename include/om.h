@@ -504,13 +504,18 @@ typedef struct {
 } om_attention_scores;
 /* d from 1 to 256; B, lq and lk may be 0. stats (2 * B * heads * lq floats, or NULL when no backward follows) receives
  * each row's reference exponent in log2 units and the inverse row sum, [B, heads, lq] each. Where rows or keys are few
- * the keys are split over workgroups and joined in a second launch. Context scratch holds the split operands. No
- * counterpart in the reference, whose Attention takes an additive mask tensor and equal heads (Ops.Layers.cs:746-807). */
+ * the keys are split over workgroups and joined in a second launch. Larger calls with d up to 128 run on the matrix cores
+ * from operands split into fp16 pairs (22 bits), with context scratch for those; where a block of 64 rows of an operand
+ * holds an infinity, a NaN or magnitudes that pairs cannot (outside 2^-40 .. 2^40, or rows further apart than 2^14), the
+ * workgroups that use it take plain fp32 sums, many times slower. Results are the same bits for the same call. o and stats
+ * must not overlap an input or each other. No counterpart in the reference, whose Attention takes an additive mask tensor
+ * and equal heads (Ops.Layers.cs:746-807). */
 om_status om_attention_fwd_scored(om_ctx *ctx, const float *q, int ld_q, const float *k, const float *v, int ld_kv,
                                   float *o, int ld_o, float *stats, int B, int lq, int lk, int d,
                                   const om_attention_scores *scores);
 /* Its backward from the forward's o and stats: dq, dk, dv (any may be NULL), written, or added to when acc is set;
- * dk and dv are the sums over a key head's query heads, in a fixed order. */
+ * dk and dv are the sums over a key head's query heads, in a fixed order. They must not overlap an input or each other
+ * (columns of one packed buffer are fine). The rule has to be the forward's. */
 om_status om_attention_bwd_scored(om_ctx *ctx, const float *q, int ld_q, const float *k, const float *v, int ld_kv,
                                   const float *o, int ld_o, const float *stats, const float *g, int ld_g, float *dq,
                                   int ld_dq, float *dk, float *dv, int ld_dkv, int B, int lq, int lk, int d,

@@ -8,8 +8,8 @@
 // A workgroup holds R rows (or R keys) in registers and streams the keys (or rows) past them: 16 lanes share a streamed
 // row, four values each per 64, so that 16 streams of rows run side by side in a workgroup and every load is 16 bytes;
 // a product is four multiply-adds a lane and a sum over the 16 lanes in four DPP additions. The streams are joined
-// through LDS in a fixed order. With few rows the pass over K and V is bound by memory; with many it is bound by the
-// vector unit.
+// through LDS in a fixed order. With few rows the pass over K and V is bound by memory (8 x 4 key heads, three rows each over 4096
+// keys of 64 values: 67 MB in 24.5 us with the join, 2.7 TB/s); with many it is bound by the vector unit.
 #include <cmath>
 
 #include "om_attention_scored.hpp"
@@ -440,13 +440,14 @@ void join(om_ctx *ctx, const Rule &u, const Ptrs &p, int nsplit, const float *pa
 }
 
 // The matrix kernels run where there is work enough: below, their splitting pass and half-filled tiles cost more than the row
-// kernels' whole call; and fewer than eight rows would leave most of a tile empty. In us, forward / backward, by rows
-// against by matrix: 4 heads of 31 | 32 rows, 512 keys of 64 values (64 thousand pairs) 14 / 34, 21 / 41; 4096 keys (half a
-// million) 42 / 297, 25 / 50; 96 heads of 64 keys (196 thousand) 19 / 22, 13 / 20; at 128 values 24 heads of 512 keys (380
-// thousand) 32 / 64, 33 / 72; of 4096 keys 173 / 485, 61 / 179.
-bool by_matrix(const Rule &u) {
+// kernels' whole call. In us, forward / backward, by rows against by matrix: 4 heads of 31 | 32 rows, 512 keys of 64 values (64
+// thousand pairs) 14 / 34, 21 / 41; 4096 keys (half a million) 42 / 297, 25 / 50; 96 heads of 64 keys (196 thousand) 19 / 22,
+// 13 / 20; at 128 values 24 heads of 512 keys (380 thousand) 32 / 64, 33 / 72; of 4096 keys 173 / 485, 61 / 179. A forward of
+// less than eight rows leaves most of a tile empty and runs faster by rows, 7 rows as above in 20 us; a backward does not,
+// whose keys the row kernels do not split: 252 us.
+bool by_matrix(const Rule &u, int least) {
     const int64_t rows = (int64_t)u.G * u.lq;
-    return u.d <= 128 && rows >= 8 && rows * u.lk * u.B * u.Hk >= 1024 * (int64_t)((u.d + 31) / 32 * 32);
+    return u.d <= 128 && rows >= least && rows * u.lk * u.B * u.Hk >= 1024 * (int64_t)((u.d + 31) / 32 * 32);
 }
 
 om_status fwd_by_rows(om_ctx *ctx, const Rule &u, const Ptrs &p) {
@@ -479,9 +480,10 @@ om_status fwd_by_rows(om_ctx *ctx, const Rule &u, const Ptrs &p) {
                                (int)blocks, (int)ns, per, part);
             if (ns > 1) join(ctx, u, p, (int)ns, part);
         };
+        // Three rows a pass over K and V: 4096 keys of 64 values, 16 x 12 heads, 7 rows in 227 us where six a pass take 311
+        // (their registers leave half the wavefronts), 3 rows in 82 us; one row alone in 76 us where three a pass take 82.
         if (NC >= 4 || rows == 1) launch(std::integral_constant<int, 1>());
-        else if (NC == 2 || rows <= 3) launch(std::integral_constant<int, 3>());
-        else launch(std::integral_constant<int, 6>());
+        else launch(std::integral_constant<int, 3>());
     });
     return status ? status : OM_LAUNCH_CHECK(ctx, "om_attention_fwd_scored");
 }
@@ -529,7 +531,7 @@ om_status om_attention_fwd_scored(om_ctx *ctx, const float *q, int ld_q, const f
     if (B == 0 || lq == 0) return OM_OK;
     OM_REQUIRE(ctx, q && o && ((k && v) || lk == 0), "%s: NULL q/k/v/o", what);
     if (om_status s = om::use_device(ctx)) return s;
-    if (!by_matrix(u)) return fwd_by_rows(ctx, u, p);
+    if (!by_matrix(u, 8)) return fwd_by_rows(ctx, u, p);
     int joins;
     float *part;
     if (om_status s = fwd_by_matrix(ctx, u, p, &joins, &part)) return s;
@@ -572,7 +574,7 @@ om_status om_attention_bwd_scored(om_ctx *ctx, const float *q, int ld_q, const f
     OM_REQUIRE(ctx, (q && o && g && stats) || lq == 0, "%s: NULL q/o/stats/g", what);
     OM_REQUIRE(ctx, (k && v) || lk == 0, "%s: NULL k/v", what);
     if (om_status s = om::use_device(ctx)) return s;
-    return by_matrix(u) ? bwd_by_matrix(ctx, u, p) : bwd_by_rows(ctx, u, p);
+    return by_matrix(u, 1) ? bwd_by_matrix(ctx, u, p) : bwd_by_rows(ctx, u, p);
 }
 
 }  // extern "C"

@@ -11,6 +11,9 @@
 // query in each lane. Either way a block of scores leaves the matrix unit in the order in which it is the next product's
 // operand. Recomputing the scores for the second role costs two products of seven; partial dq from the first role would
 // cost rows * keys / 32 values of traffic, more than that from about 2000 keys on, and atomics would lose the fixed order.
+//
+// Bound: as the forward. 12 heads of 64 values in 4 key heads, 4096 causal rows with a cap: 365 us (matrix unit busy 40 % of the
+// time, vector unit 58 %); 16 heads of 128 in 4, 8192 rows in a window of 1024: 1150 us (32 %, 27 %, one wavefront a SIMD).
 #include <algorithm>
 
 #include "om_attention_scored_split.hpp"
@@ -856,32 +859,37 @@ __global__ void __launch_bounds__(64 * waves_of(DP), DP == 128 ? 1 : 2) k_scored
     }
 }
 
-// dk and dv, then dq, from their splits' sums, in split order; a thread per value.
+// dk and dv (`dkv` values), then dq (`dq` values), from their splits' sums, in split order; a thread per four values (or one,
+// where d is no multiple of four).
+template <int W>
 __global__ void __launch_bounds__(256) k_scored_join_bwd(Rule u, Ptrs p, int64_t dkv, int nsplit, const float *__restrict__ part,
                                                          int64_t dq, int qsplit, const float *__restrict__ qpart) {
     OM_LDS_POISON();
-    int64_t f = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    typedef float vec __attribute__((ext_vector_type(W), aligned(4)));
+    int64_t f = ((int64_t)blockIdx.x * 256 + threadIdx.x) * W;
     if (f >= dkv + dq) return;
     const bool q = f >= dkv;
     const int64_t each = q ? dq : dkv;
     const float *from = q ? qpart : part;
     const int n = q ? qsplit : nsplit;
     if (q) f -= dkv;
-    float s = 0.0f;
-    for (int i = 0; i < n; i++) s += from[i * each + f];
-    const int c = (int)(f % u.d);
+    const int64_t row = f / u.d;  // a row's query of a head, or dk, dv of a key in turn
+    const int c = (int)(f - row * u.d);
     float *to;
     if (q) {
-        const int64_t r = f / u.d, rows = (int64_t)u.G * u.lq, item = r / rows;
-        const Row row = row_of(u, (int)(item % u.Hk), (int)(r - item * rows));
-        to = p.dq + ((item / u.Hk) * u.lq + row.t) * p.lddq + (int64_t)row.h * u.d;
+        const int64_t rows = (int64_t)u.G * u.lq, item = row / rows;
+        const Row r = row_of(u, (int)(item % u.Hk), (int)(row - item * rows));
+        to = p.dq + ((item / u.Hk) * u.lq + r.t) * p.lddq + (int64_t)r.h * u.d;
     } else {
-        const int64_t key = f / (2 * u.d), item = key / u.lk;
-        to = f / u.d % 2 ? p.dv : p.dk;
+        const int64_t key = row >> 1, item = key / u.lk;
+        to = row & 1 ? p.dv : p.dk;
         if (!to) return;
-        to += ((item / u.Hk) * u.lk + key % u.lk) * p.lddkv + (item % u.Hk) * u.d;
+        to += ((item / u.Hk) * u.lk + (key - item * u.lk)) * p.lddkv + (item % u.Hk) * u.d;
     }
-    to[c] = p.acc ? to[c] + s : s;
+    vec s = *reinterpret_cast<const vec *>(from + f);
+    for (int i = 1; i < n; i++) s += *reinterpret_cast<const vec *>(from + i * each + f);
+    vec *out = reinterpret_cast<vec *>(to + c);
+    *out = p.acc ? *out + s : s;
 }
 
 }  // namespace
@@ -899,14 +907,15 @@ om_status bwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p) {
     const int rows_wg = 32 * waves_of(dp);
     a.rblocks = (int)((rows + rows_wg - 1) / rows_wg);
     const bool keys = p.dk || p.dv;
-    // Split the rows of dk and dv while those workgroups leave CUs idle, in pieces of at least eight blocks.
+    // Split the rows of dk and dv while those workgroups leave CUs idle, in pieces of at least eight blocks (below, a
+    // workgroup's start of 5 us and the join cost what the shorter walk saves).
     int64_t ns = 1, wk = items * a.kblocks;
     if (wk < 2 * ctx->num_cus) ns = 2 * ctx->num_cus / wk;
     ns = ns > a.nr / 8 ? a.nr / 8 : ns;
     ns = ns < 1 ? 1 : ns;
     a.nsplit = (int)ns;
     wk = keys ? wk * a.nsplit : 0;
-    // The keys of dq alike: 32 rows of 4 heads over 4096 keys of 64 values, 225 us whole.
+    // The keys of dq alike: 32 rows of 4 heads over 4096 keys of 64 values, 225 us for the call whole, 50 us in pieces.
     int64_t qs = 1, wr = items * a.rblocks;
     if (wr < 2 * ctx->num_cus) qs = 2 * ctx->num_cus / wr;
     qs = qs > a.nt / 8 ? a.nt / 8 : qs;
@@ -969,8 +978,11 @@ om_status bwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p) {
     });
     if (part || qpart) {
         const int64_t dkv = part ? items * u.lk * 2 * u.d : 0, dq = qpart ? items * rows * u.d : 0;
-        hipLaunchKernelGGL(k_scored_join_bwd, dim3((unsigned)((dkv + dq + 255) / 256)), dim3(256), 0, ctx->stream, u, p, dkv,
-                           a.nsplit, a.part, dq, a.qsplit, a.qpart);
+        auto join = [&](auto kern, int w) {
+            hipLaunchKernelGGL(kern, dim3((unsigned)(((dkv + dq) / w + 255) / 256)), dim3(256), 0, ctx->stream, u, p, dkv, a.nsplit,
+                               a.part, dq, a.qsplit, a.qpart);
+        };
+        u.d % 4 == 0 ? join(k_scored_join_bwd<4>, 4) : join(k_scored_join_bwd<1>, 1);
     }
     return OM_LAUNCH_CHECK(ctx, what);
 }

@@ -5,6 +5,10 @@
 // split, and are the operand of O^T += V^T E^T as they stand. K and V come split from scratch, straight into LDS, a
 // ring of steps, one barrier each. The running maximum m moves only when some lane's maximum grows by more than 2^2: E then
 // stays below 2^14 with its 2^12 of headroom, and the accumulators are left alone in most steps.
+//
+// Bound: a wavefront's matrix instructions and its vector work (exponents, caps, masks, splits) follow each other, so a SIMD
+// runs one of them only while another wavefront is in the other; 12 heads of 64 values in 4 key heads, 4096 causal rows with
+// a cap: 113 us and 14 us for the joins, 228 TFLOP/s of fp32 products where three fp16 products for each reach about 380.
 #include <algorithm>
 #include <cmath>
 

