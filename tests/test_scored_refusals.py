@@ -14,7 +14,7 @@ MAIN = os.path.join(ROOT, "tests", "host", "scored_refusals_main.cpp")
 def test_refusals(tmp_path):
     hipcc = shutil.which("hipcc") or "/opt/rocm/bin/hipcc"
     if not (os.path.exists(hipcc) and os.path.exists(MAIN) and os.path.exists(os.path.join(LIB, "libom_hip.so"))):
-        pytest.skip("needs hipcc, the driver's source and the built library")
+        pytest.skip("needs hipcc, the test program's source and the built library")
     exe = str(tmp_path / "refusals")
     subprocess.run([hipcc, "-x", "hip", "--offload-arch=gfx950", "-std=c++17", "-O1", "-Wno-unused-result", MAIN, "-o", exe,
                     "-L", LIB, "-lom_hip", "-Wl,-rpath," + LIB], check=True, capture_output=True)
