@@ -907,17 +907,20 @@ om_status bwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p) {
     const int rows_wg = 32 * waves_of(dp);
     a.rblocks = (int)((rows + rows_wg - 1) / rows_wg);
     const bool keys = p.dk || p.dv;
-    // Split the rows of dk and dv while those workgroups leave CUs idle, in pieces of at least eight blocks (below, a
-    // workgroup's start of 5 us and the join cost what the shorter walk saves).
+    // Split the rows of dk and dv until there are eight wavefronts a CU, in pieces of at least eight blocks (below, a workgroup's
+    // start of 5 us and the join cost what the shorter walk saves). Half as many: 644 us for 488 at 4096 causal rows of 64
+    // values, 1557 for 1363 in the window of 128; half as many again: 501 and 1342; 777 rows of 80 values with twice as many:
+    // 158 for 149.
+    const int64_t want = 8 / waves_of(dp) * ctx->num_cus;
     int64_t ns = 1, wk = items * a.kblocks;
-    if (wk < 2 * ctx->num_cus) ns = 2 * ctx->num_cus / wk;
+    if (wk < want) ns = want / wk;
     ns = ns > a.nr / 8 ? a.nr / 8 : ns;
     ns = ns < 1 ? 1 : ns;
     a.nsplit = (int)ns;
     wk = keys ? wk * a.nsplit : 0;
     // The keys of dq alike: 32 rows of 4 heads over 4096 keys of 64 values, 225 us for the call whole, 50 us in pieces.
     int64_t qs = 1, wr = items * a.rblocks;
-    if (wr < 2 * ctx->num_cus) qs = 2 * ctx->num_cus / wr;
+    if (wr < want) qs = want / wr;
     qs = qs > a.nt / 8 ? a.nt / 8 : qs;
     qs = qs < 1 ? 1 : qs;
     a.qsplit = (int)qs;
