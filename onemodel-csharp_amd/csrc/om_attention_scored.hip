@@ -324,10 +324,9 @@ __device__ __forceinline__ void dkv_keys(const Rule &u, const Ptrs &p, int b, in
 #pragma unroll
         for (int n = 0; n < NC; n++) dk[r][n] = dv[r][n] = floatx4{0.f, 0.f, 0.f, 0.f};
     }
-    int lo, hi;
-    pos_range(u, j0, min(j0 + R, u.lk) - 1, pre, lo, hi);
-    const int r1 = (hi - u.off + 1) * u.G;
-    for (int rr = (lo - u.off) * u.G + st; rr < r1; rr += kStreams) {
+    int r0, r1;
+    row_range(u, j0, min(j0 + R, u.lk) - 1, pre, r0, r1);
+    for (int rr = r0 + st; rr < r1; rr += kStreams) {
         const Row row = row_of(u, hk, rr);
         const int64_t tok = (int64_t)b * u.lq + row.t, sr = stat_at(u, b, row);
         floatx4 q[NC], g[NC], o[NC];
@@ -377,7 +376,8 @@ om_status make_rule(om_ctx *ctx, const char *what, const om_attention_scores *f,
                B, lq, lk, d);
     OM_REQUIRE(ctx, f->heads >= 1 && f->kv_heads >= 1 && f->heads % f->kv_heads == 0,
                "%s: %d heads are not a multiple of %d key heads", what, f->heads, f->kv_heads);
-    // 2^30 keeps every row, key and position index, and their sums with a tile, inside 32 bits
+    // 2^30 keeps every row, key and position index, and their sums with a tile or a window, inside 32 bits (not a key's
+    // index times the group: row_range)
     constexpr int64_t kMost = 1 << 30;
     OM_REQUIRE(ctx, (int64_t)f->heads * d <= kMost && lq <= kMost && lk <= kMost && (int64_t)B * f->heads <= kMost &&
                (int64_t)B * f->heads * lq <= kMost && (int64_t)B * f->kv_heads * lk <= kMost, "%s: too many rows", what);
@@ -395,8 +395,8 @@ om_status make_rule(om_ctx *ctx, const char *what, const om_attention_scores *f,
     u.d = d;
     u.off = lk - lq;
     u.causal = f->causal;
-    // |i - j| is below lq + lk, so a window that wide is none; a narrower one cannot take a position out of 32 bits
-    u.window = f->window >= (int64_t)lq + lk ? 0 : f->window;
+    // |i - j| is below the larger length, so a window that wide is none; a narrower one cannot take a position out of 32 bits
+    u.window = f->window >= (lq > lk ? lq : lk) ? 0 : f->window;
     u.scale = f->scale == 0.0f || f->scale != f->scale ? 1.0f / sqrtf((float)d) : f->scale;
     u.cl2 = u.scale * kLog2e;
     if (f->cap > 0.0f) {

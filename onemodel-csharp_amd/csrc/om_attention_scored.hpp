@@ -13,7 +13,7 @@ constexpr float kLog2e = 1.4426950408889634f;
 // one row index covers a whole group and a block of rows shares its keys.
 struct Rule {
     int B, Hk, G, lq, lk, d, off;  // off = lk - lq: query t stands at position t + off
-    int causal, window;            // window 0: none; else below lq + lk
+    int causal, window;            // window 0: none; else below the larger of lq and lk
     float scale, cl2;              // cl2 = scale log2 e
     float icap, capl2;             // cap > 0: icap = scale / cap, capl2 = cap log2 e; else icap = 0
     const float *slopes;
@@ -51,7 +51,7 @@ __device__ __forceinline__ float score(const Rule &u, float raw, float &th) {
 }
 
 // Whether the query at position i sees key j (i - j = gap) with prefix keys `pre`, documents aside.
-__device__ __forceinline__ bool in_reach(const Rule &u, int gap, int j, int pre) {
+__host__ __device__ __forceinline__ bool in_reach(const Rule &u, int gap, int j, int pre) {
     if (j < pre) return true;
     if (u.causal && gap < 0) return false;
     return u.window == 0 || (gap < u.window && gap > -u.window);
@@ -62,9 +62,9 @@ struct Reach {
     int lo;
     uint32_t n;
     int pre;
-    __device__ __forceinline__ bool has(int j) const { return ((uint32_t)(j - lo) < n) | (j < pre); }
+    __host__ __device__ __forceinline__ bool has(int j) const { return ((uint32_t)(j - lo) < n) | (j < pre); }
 };
-__device__ __forceinline__ Reach keys_seen(const Rule &u, int pos, int doc, int pre) {
+__host__ __device__ __forceinline__ Reach keys_seen(const Rule &u, int pos, int doc, int pre) {
     int lo = 0, hi = u.lk - 1;
     if (u.causal) hi = min(hi, pos);
     if (u.window) {
@@ -75,7 +75,7 @@ __device__ __forceinline__ Reach keys_seen(const Rule &u, int pos, int doc, int 
     return Reach{lo, on && hi >= lo ? (uint32_t)(hi - lo + 1) : 0u, on ? min(pre, u.lk) : 0};
 }
 // The same for one key: the positions that see it.
-__device__ __forceinline__ Reach rows_seeing(const Rule &u, int j, int doc, int pre) {
+__host__ __device__ __forceinline__ Reach rows_seeing(const Rule &u, int j, int doc, int pre) {
     int lo = u.off, hi = u.lk - 1;
     if (j >= pre) {
         if (u.causal) lo = max(lo, j);
@@ -87,7 +87,7 @@ __device__ __forceinline__ Reach rows_seeing(const Rule &u, int j, int doc, int 
     return Reach{lo, doc >= 0 && hi >= lo ? (uint32_t)(hi - lo + 1) : 0u, INT32_MIN};
 }
 // The hull [lo, hi] of the keys that queries at positions i0 .. i1 can see.
-__device__ __forceinline__ void key_range(const Rule &u, int i0, int i1, int pre, int &lo, int &hi) {
+__host__ __device__ __forceinline__ void key_range(const Rule &u, int i0, int i1, int pre, int &lo, int &hi) {
     lo = 0;
     hi = u.lk - 1;
     if (u.causal) hi = min(hi, i1);
@@ -101,7 +101,7 @@ __device__ __forceinline__ void key_range(const Rule &u, int i0, int i1, int pre
     }
 }
 // The hull [lo, hi] of the positions that can see one of the keys j0 .. j1.
-__device__ __forceinline__ void pos_range(const Rule &u, int j0, int j1, int pre, int &lo, int &hi) {
+__host__ __device__ __forceinline__ void pos_range(const Rule &u, int j0, int j1, int pre, int &lo, int &hi) {
     lo = u.off;
     hi = u.lk - 1;
     if (j0 < pre) return;
@@ -110,6 +110,14 @@ __device__ __forceinline__ void pos_range(const Rule &u, int j0, int j1, int pre
         hi = min(hi, j1 + u.window - 1);
         if (!u.causal) lo = max(lo, j0 - u.window + 1);
     }
+}
+// The rows r0 .. r1 - 1 of the group that can see one of the keys j0 .. j1. A window may leave the hull before the first
+// query's position, by up to lk: it is cut there before the group's size multiplies it, since lk * G may pass 32 bits.
+__host__ __device__ __forceinline__ void row_range(const Rule &u, int j0, int j1, int pre, int &r0, int &r1) {
+    int lo, hi;
+    pos_range(u, j0, j1, pre, lo, hi);
+    r0 = (lo - u.off) * u.G;
+    r1 = hi < lo ? r0 : (hi - u.off + 1) * u.G;
 }
 
 // Sum over the 16 lanes of a DPP row; every lane gets the same bits (each step adds partners' equal sums).

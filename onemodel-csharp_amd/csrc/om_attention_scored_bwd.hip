@@ -261,9 +261,8 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
         whi = __builtin_amdgcn_readfirstlane(wave_imax(j <= last ? kd : INT32_MIN));
     }
     // the blocks of rows that may see them
-    int plo, phi;
-    pos_range(u, first, last, pre, plo, phi);
-    int r0 = (plo - u.off) * u.G, r1 = phi < plo ? r0 : (phi - u.off + 1) * u.G;  // one past the last
+    int r0, r1;  // r1: one past the last
+    row_range(u, first, last, pre, r0, r1);
     const int t0 = r0 / kBlock, t1 = r1 <= r0 ? t0 - 1 : (r1 - 1) / kBlock;
     uint32_t gt = 0, gl = 0xFFFFFFFFu, qt = 0, ql = 0xFFFFFFFFu;
     RowStats mine = {};  // the thread's first

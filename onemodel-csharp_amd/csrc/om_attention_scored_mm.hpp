@@ -172,7 +172,7 @@ void by_depth(int d, F f) {
 // `some0 .. some1`; and all see the keys below pre.
 struct Band {
     int all0, all1, some0, some1, pre;
-    __device__ __forceinline__ Band(const Rule &u, int i0, int i1, int prefix) {
+    __host__ __device__ __forceinline__ Band(const Rule &u, int i0, int i1, int prefix) {
         all0 = some0 = 0;
         all1 = some1 = u.lk - 1;
         if (u.causal) {
@@ -188,14 +188,14 @@ struct Band {
         pre = min(prefix, u.lk);
     }
     // bitwise throughout: a chain of scalar branches costs more than the arithmetic it saves
-    __device__ __forceinline__ bool all(int j0, int j1) const { return ((j0 >= all0) & (j1 <= all1)) | (j1 < pre); }
-    __device__ __forceinline__ bool some(int j0, int j1) const { return ((j0 <= some1) & (j1 >= some0)) | (j0 < pre); }
+    __host__ __device__ __forceinline__ bool all(int j0, int j1) const { return ((j0 >= all0) & (j1 <= all1)) | (j1 < pre); }
+    __host__ __device__ __forceinline__ bool some(int j0, int j1) const { return ((j0 <= some1) & (j1 >= some0)) | (j0 < pre); }
 };
 
 // The same from the keys' side, in rows of the group: rows all0 .. all1 see all of keys j0 .. j1, rows some0 .. some1 some.
 struct RowBand {
     int all0, all1, some0, some1;
-    __device__ __forceinline__ RowBand(const Rule &u, int j0, int j1, int prefix) {
+    __host__ __device__ __forceinline__ RowBand(const Rule &u, int j0, int j1, int prefix) {
         int a0 = u.off, a1 = INT32_MAX, s0 = u.off, s1 = INT32_MAX;  // positions
         if (j1 >= prefix) {
             if (u.causal) a0 = max(a0, j1);
@@ -211,13 +211,15 @@ struct RowBand {
                 s1 = j1 + u.window - 1;
             }
         }
-        all0 = (a0 - u.off) * u.G;
-        some0 = (s0 - u.off) * u.G;
-        all1 = a1 >= u.lk - 1 ? INT32_MAX : (a1 - u.off + 1) * u.G - 1;
-        some1 = s1 >= u.lk - 1 ? INT32_MAX : (s1 - u.off + 1) * u.G - 1;
+        // positions cut to the queries' and one more on either side: a distance of lk times G may pass 32 bits
+        auto row = [&](int pos) { return (min(max(pos, u.off - 1), u.lk) - u.off) * u.G; };
+        all0 = row(a0);
+        some0 = row(s0);
+        all1 = a1 >= u.lk - 1 ? INT32_MAX : row(a1 + 1) - 1;
+        some1 = s1 >= u.lk - 1 ? INT32_MAX : row(s1 + 1) - 1;
     }
-    __device__ __forceinline__ bool all(int r0, int r1) const { return (r0 >= all0) & (r1 <= all1); }
-    __device__ __forceinline__ bool some(int r0, int r1) const { return (r1 >= some0) & (r0 <= some1); }
+    __host__ __device__ __forceinline__ bool all(int r0, int r1) const { return (r0 >= all0) & (r1 <= all1); }
+    __host__ __device__ __forceinline__ bool some(int r0, int r1) const { return (r1 >= some0) & (r0 <= some1); }
 };
 
 // Workgroup id -> item and block. Ids are dealt round-robin over the 8 XCDs, each with its own L2, so the items come
