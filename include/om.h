@@ -506,8 +506,10 @@ typedef struct {
  * each row's reference exponent in log2 units and the inverse row sum, [B, heads, lq] each. Where rows or keys are few
  * the keys are split over workgroups and joined in a second launch. Larger calls with d up to 128 run on the matrix cores
  * from operands split into fp16 pairs (22 bits), with context scratch for those; where a block of 64 rows of an operand
- * holds an infinity, a NaN or magnitudes that pairs cannot (outside 2^-40 .. 2^40, or rows further apart than 2^14), the
- * workgroups that use it take plain fp32 sums, many times slower. Results are the same bits for the same call. o and stats
+ * holds an infinity, a NaN or magnitudes that pairs cannot (outside 2^-40 .. 2^40, or rows further apart than 2^14), or where
+ * a query's length times a key's times scale passes 709 (2^10 in log2 units: a score is held to 2^-22 of itself, and the
+ * backward's weight to as much of the score), the workgroups that use it take plain fp32 sums, many times slower. A scale
+ * (or scale / cap) outside 2^-40 .. 2^40 takes the row kernels. Results are the same bits for the same call. o and stats
  * must not overlap an input or each other. No counterpart in the reference, whose Attention takes an additive mask tensor
  * and equal heads (Ops.Layers.cs:746-807). */
 om_status om_attention_fwd_scored(om_ctx *ctx, const float *q, int ld_q, const float *k, const float *v, int ld_kv,

@@ -445,9 +445,13 @@ void join(om_ctx *ctx, const Rule &u, const Ptrs &p, int nsplit, const float *pa
 // 13 / 20; at 128 values 24 heads of 512 keys (380 thousand) 32 / 64, 33 / 72; of 4096 keys 173 / 485, 61 / 179. A forward of
 // less than eight rows leaves most of a tile empty and runs faster by rows, 7 rows as above in 20 us; a backward does not,
 // whose keys the row kernels do not split: 252 us.
+// The matrix kernels' factors, scale or scale / cap times the operands' powers of two (2^-52 .. 2^28 each), have to stay fp32
+// numbers: within 2^-40 .. 2^40 for a score that is not lost itself.
 bool by_matrix(const Rule &u, int least) {
     const int64_t rows = (int64_t)u.G * u.lq;
-    return u.d <= 128 && rows >= least && rows * u.lk * u.B * u.Hk >= 1024 * (int64_t)((u.d + 31) / 32 * 32);
+    const float s = std::fabs(u.scale), c = std::fabs(u.icap);
+    const bool fits = s >= 0x1p-40f && s <= 0x1p40f && (c == 0.0f || (c >= 0x1p-40f && c <= 0x1p40f));
+    return fits && u.d <= 128 && rows >= least && rows * u.lk * u.B * u.Hk >= 1024 * (int64_t)((u.d + 31) / 32 * 32);
 }
 
 om_status fwd_by_rows(om_ctx *ctx, const Rule &u, const Ptrs &p) {

@@ -228,7 +228,7 @@ __device__ __forceinline__ void put4(float *to, int c, int d, floatx4 v, int acc
 // ---------------------------------------------------------------------------------------------------- dk and dv
 // Either role's tables in LDS, by blocks of the other side: whether the block is visited (documents).
 struct Tables {
-    uint32_t red[8][5];
+    uint32_t red[8][6];
     unsigned char see[kListed];
 };
 template <int DP, int PARTS>
@@ -264,7 +264,7 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
     int r0, r1;  // r1: one past the last
     row_range(u, first, last, pre, r0, r1);
     const int t0 = r0 / kBlock, t1 = r1 <= r0 ? t0 - 1 : (r1 - 1) / kBlock;
-    uint32_t gt = 0, gl = 0xFFFFFFFFu, qt = 0, ql = 0xFFFFFFFFu;
+    uint32_t gt = 0, gl = 0xFFFFFFFFu, qt = 0, ql = 0xFFFFFFFFu, qnorm = 0;
     RowStats mine = {};  // the thread's first
     for (int rt = t0 + (int)threadIdx.x, n = 0; rt <= t1; rt += 64 * NW, n++) {
         const RowStats r = a.rs[rt0 + rt];
@@ -272,6 +272,7 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
         bad = bad || r.bad;
         gt = max(gt, r.g2_top);
         qt = max(qt, r.q2_top);
+        qnorm = max(qnorm, __float_as_uint(r.norm));
         if (r.g2_top) gl = min(gl, r.g2_top);
         if (r.q2_top) ql = min(ql, r.q2_top);
     }
@@ -283,6 +284,7 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
     qt = wave_umax(qt);
     gl = wave_umin(gl);
     ql = wave_umin(ql);
+    qnorm = wave_umax(qnorm);
     const uint32_t wave_bad = __any(bad) ? 1 : 0;
     if (lane == 0) {
         red[w][0] = gt;
@@ -290,6 +292,7 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
         red[w][2] = gl;
         red[w][3] = ql;
         red[w][4] = wave_bad;
+        red[w][5] = qnorm;
     }
     __syncthreads();
 #pragma unroll
@@ -299,7 +302,9 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
         gl = min(gl, red[n][2]);
         ql = min(ql, red[n][3]);
         bad = bad || red[n][4];
+        qnorm = max(qnorm, red[n][5]);
     }
+    bad = bad || !scores_fit(u, __uint_as_float(qnorm), larger(k0.norm, k1.norm));
     // the accumulators move between the blocks' scales: keep the largest move inside fp32
     bad = bad || (gt && (gt >> 23) - (gl >> 23) > 60) || (qt && (qt >> 23) - (ql >> 23) > 60);
     auto dest = [&](int n, int jj) -> float * {  // dk (0) or dv (1) of key jj
@@ -414,13 +419,14 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
             for (int n = 0; n < ND; n++) sum[n] *= c;
             cur = to;
         };
+        // scores as the forward summed them, bit for bit where the operands are
         auto products = [&](floatx16 &out, const char *f, const u32x4 *fh, const u32x4 *fm) {
 #pragma unroll
             for (int e = 0; e < 16; e++) out[e] = 0.0f;
 #pragma unroll
             for (int s = 0; s < S; s++)
-                out = mma3(*reinterpret_cast<const u32x4 *>(f + (2 * s) * 1024),
-                           *reinterpret_cast<const u32x4 *>(f + (2 * s + 1) * 1024), fh[s], fm[s], out);
+                out = mma3_t(*reinterpret_cast<const u32x4 *>(f + (2 * s) * 1024),
+                             *reinterpret_cast<const u32x4 *>(f + (2 * s + 1) * 1024), fh[s], fm[s], out);
         };
         // x from raw products to weights E; `keep(e, w)` gets E (1 - tanh^2)
         auto weights = [&](auto keep) {
@@ -602,11 +608,13 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
     const int rt = min(own / kBlock, a.nr - 1);
     const RowStats rs = a.rs[rt0 + rt];
     bool bad = false;
+    float qnorm = 0.0f;
     int qlo = INT32_MAX, qhi = INT32_MIN;
 #pragma unroll
     for (int n = 0; n < ROWS / kBlock; n++) {
         const RowStats r = a.rs[rt0 + min(first / kBlock + n, a.nr - 1)];
         bad = bad || r.bad;
+        qnorm = larger(qnorm, r.norm);
         qlo = min(qlo, r.doc_lo);
         qhi = max(qhi, r.doc_hi);
     }
@@ -623,22 +631,25 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
                        : p.dq + ((int64_t)b * u.lq + to.t) * p.lddq + (int64_t)to.h * u.d;
     };
     const int acc = a.qpart ? 0 : p.acc;
-    uint32_t kt = 0, vt = 0, kl = 0xFFFFFFFFu;
-    Stats mk = {}, mv = {};  // the thread's first
+    uint32_t kt = 0, vt = 0, kl = 0xFFFFFFFFu, knorm = 0;
+    Stats mk = {};  // the thread's first
     for (int t = t0 + (int)threadIdx.x, n = 0; t <= t1; t += 64 * NW, n++) {
         const Stats sk = a.ks[kt0 + t], sv = a.vs[kt0 + t];
-        if (n == 0) mk = sk, mv = sv;
+        if (n == 0) mk = sk;
         kt = max(kt, sk.top);
+        knorm = max(knorm, __float_as_uint(sk.norm));
         kl = min(kl, sk.low);
         vt = max(vt, sv.top);
     }
     kt = wave_umax(kt);
     vt = wave_umax(vt);
     kl = wave_umin(kl);
+    knorm = wave_umax(knorm);
     if (lane == 0) {
         red[w][0] = kt;
         red[w][1] = vt;
         red[w][2] = kl;
+        red[w][3] = knorm;
     }
     __syncthreads();
 #pragma unroll
@@ -646,8 +657,9 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
         kt = max(kt, red[n][0]);
         vt = max(vt, red[n][1]);
         kl = min(kl, red[n][2]);
+        knorm = max(knorm, red[n][3]);
     }
-    bad = bad || kt > kMostBits || vt > kMostBits || !even_rows(kt, kl);
+    bad = bad || !scores_fit(u, qnorm, __uint_as_float(knorm)) || kt > kMostBits || vt > kMostBits || !even_rows(kt, kl);
     if (__builtin_amdgcn_readfirstlane(bad)) {
         for (int r = own; r <= min(last, own + 31); r++) plain_dq<DP>(u, p, b, hk, r, lo, hi, pre, dest(r, row_of(u, hk, r)), acc);
         return;
@@ -959,11 +971,11 @@ om_status bwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p) {
     float *kw = reinterpret_cast<float *>(take(words));
     a.keys = ko.keys = vo.keys = kw;
     vo.is_v = true;
+    a.part = part ? reinterpret_cast<float *>(take(part)) : nullptr;
+    a.qpart = qpart ? reinterpret_cast<float *>(take(qpart)) : nullptr;
     a.ks = ko.stats = reinterpret_cast<Stats *>(take(items * a.nt * (int64_t)sizeof(Stats)));
     a.vs = vo.stats = reinterpret_cast<Stats *>(take(items * a.nt * (int64_t)sizeof(Stats)));
     a.rs = ro.stats = reinterpret_cast<RowStats *>(take(items * a.nr * (int64_t)sizeof(RowStats)));
-    a.part = part ? reinterpret_cast<float *>(take(part)) : nullptr;
-    a.qpart = qpart ? reinterpret_cast<float *>(take(qpart)) : nullptr;
     auto al16 = [](const void *x) { return ((uintptr_t)x & 15) == 0; };
     const bool vec = u.d % 4 == 0 && p.ldq % 4 == 0 && p.ldkv % 4 == 0 && p.ldo % 4 == 0 && p.ldg % 4 == 0 && al16(p.q) &&
                      al16(p.k) && al16(p.v) && al16(p.o) && al16(p.g);

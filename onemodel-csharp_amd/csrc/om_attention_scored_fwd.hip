@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
     constexpr int PER = 2 * (HALF / 4096) + 1;  // loads of a step per wavefront
     __shared__ __attribute__((aligned(16))) char sh[256 + NST * STAGE];  // no stage at LDS address 0
     __shared__ unsigned char visit[DOCS ? kListed : 1];  // whether some row may see the block
-    __shared__ uint32_t red[4][6];
+    __shared__ uint32_t red[4][8];
     const Place at = place_of(blockIdx.x, u.B * u.Hk);
     const int item = at.item, split = at.block % a.nsplit, rb = a.blocks - 1 - at.block / a.nsplit;
     const int b = item / u.Hk, hk = item - b * u.Hk, rows = u.G * u.lq;
@@ -171,13 +171,14 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
     const int t0 = c0 + split * per, t1 = min(c1, t0 + per - 1);
     lo = max(lo, t0 * kBlock);
     hi = min(hi, t1 * kBlock + kBlock - 1);
-    uint32_t ktop = 0, vtop = 0, vlow = 0xFFFFFFFFu;
+    uint32_t ktop = 0, vtop = 0, vlow = 0xFFFFFFFFu, knorm = 0;
     const int64_t kt0 = (int64_t)item * a.nt;
-    Stats mk = {}, mv = {};
+    Stats mk = {};
     for (int t = t0 + (int)threadIdx.x, n = 0; t <= t1; t += 256, n++) {
         const Stats sk = a.ks[kt0 + t], sv = a.vs[kt0 + t];
-        if (n == 0) mk = sk, mv = sv;
+        if (n == 0) mk = sk;
         ktop = max(ktop, sk.top);
+        knorm = max(knorm, __float_as_uint(sk.norm));
         vtop = max(vtop, sv.top);
         vlow = min(vlow, sv.low);
     }
@@ -185,15 +186,19 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
     u32x4 qh[S], qm[S];
     int eq;
     bool bad;
+    uint32_t qnorm;
     {
         uint32_t top = 0;
+        float norm = 0.0f;
 #pragma unroll
         for (int s = 0; s < S; s++)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 if (doc < 0) x0[s][e] = 0.0f;
                 top = max(top, __float_as_uint(x0[s][e]) & 0x7FFFFFFFu);
+                norm = __builtin_fmaf(x0[s][e], x0[s][e], norm);
             }
+        qnorm = __float_as_uint(pair_sum(norm));
         const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
         top = max(both[0], both[1]);
         bad = !in_range(top);
@@ -209,6 +214,8 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
     ktop = wave_umax(ktop);
     vtop = wave_umax(vtop);
     vlow = wave_umin(vlow);
+    knorm = wave_umax(knorm);
+    qnorm = wave_umax(qnorm);
     // documents of the wavefront's rows; a padded row sees nothing, whatever the others see
     int wqlo = 0, wqhi = 0;
     bool one_doc = true;
@@ -225,6 +232,8 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
         red[w][3] = (uint32_t)wqlo;
         red[w][4] = (uint32_t)wqhi;
         red[w][5] = wave_bad;
+        red[w][6] = knorm;
+        red[w][7] = qnorm;
     }
     __syncthreads();
     int qlo = wqlo, qhi = wqhi;
@@ -236,8 +245,10 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
         qlo = min(qlo, (int)red[i][3]);
         qhi = max(qhi, (int)red[i][4]);
         bad = bad || red[i][5];
+        knorm = max(knorm, red[i][6]);
+        qnorm = max(qnorm, red[i][7]);
     }
-    bad = bad || ktop > kMostBits || vtop > kMostBits || !even_rows(vtop, vlow);
+    bad = bad || !scores_fit(u, __uint_as_float(qnorm), __uint_as_float(knorm)) || ktop > kMostBits || vtop > kMostBits || !even_rows(vtop, vlow);
     if (__builtin_amdgcn_readfirstlane(bad)) {
         for (int r = first + 32 * w; r <= min(last, first + 32 * w + 31); r++)
             plain_row<DP>(u, p, b, hk, r, lo, hi, split, a.nsplit, a.part);

@@ -32,17 +32,20 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kBlock = 64;  // rows of an operand that share a scale
 
 // What the split found in a block: the largest magnitude (bits; at or above infinity's if the split cannot hold the block),
-// the smallest nonzero row maximum (bits), 2^e of its scale, and the range of its document ids.
+// the smallest nonzero row maximum (bits), 2^e of its scale, the range of its document ids, and the largest sum of a row's
+// squares.
 struct Stats {
     uint32_t top, low;
     float scale;
     int32_t doc_lo, doc_hi;
-    int32_t pad[3];
+    float norm;
 };
 // What a step of 32 keys carries along with its operands, staged with them: 64 words.
 enum { kKeyDoc = 0, kKeyScaleK = 32, kKeyScaleV, kKeyDocLo, kKeyDocHi, kKeyWords = 64 };
 constexpr uint32_t kInfBits = 0x7F800000u;
 constexpr uint32_t kMostBits = (127u + 40) << 23, kLeastBits = (127u - 40) << 23;  // 2^40, 2^-40
+
+constexpr float kMostScore = 1024.0f;  // in log2 units
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
 // The exponent e of a scale 2^-e that brings `top` (bits of a magnitude in range) to 2^11 .. 2^15; steps of 2^4, so that
@@ -55,6 +58,11 @@ __device__ __forceinline__ bool in_range(uint32_t top) { return top == 0 || (top
 // Whether the smallest nonzero row maximum is within 2^14 of the largest: every row then keeps its 22 bits but the last one
 // or two.
 __device__ __forceinline__ bool even_rows(uint32_t top, uint32_t low) { return top == 0 || (top >> 23) - (low >> 23) <= 14; }
+// Whether scores of rows and keys with these largest sums of squares stay below kMostScore (no, if one is a NaN). A cap does not
+// help: what goes into its tanh is held to 2^-36 of the largest.
+__device__ __forceinline__ bool scores_fit(const Rule &u, float q_norm, float k_norm) {
+    return __builtin_amdgcn_sqrtf(q_norm) * __builtin_amdgcn_sqrtf(k_norm) * __builtin_fabsf(u.cl2) < kMostScore;
+}
 
 // Two values split into packed fp16 pairs: a packed conversion, the two remainders with the halves taken as they lie
 // (v_fma_mix_f32 reads either half of a register as fp16), a packed conversion. Left to itself the compiler converts each
@@ -86,6 +94,12 @@ __device__ __forceinline__ floatx16 mma(u32x4 a, u32x4 b, floatx16 c) {
 __device__ __forceinline__ floatx16 mma3(u32x4 ah, u32x4 am, u32x4 bh, u32x4 bm, floatx16 c) {
     c = mma(am, bh, c);
     c = mma(ah, bm, c);
+    return mma(ah, bh, c);
+}
+// The same sum in the same order with the operands' roles exchanged: mma3_t(a, b) has the bits of mma3(b, a).
+__device__ __forceinline__ floatx16 mma3_t(u32x4 ah, u32x4 am, u32x4 bh, u32x4 bm, floatx16 c) {
+    c = mma(ah, bm, c);
+    c = mma(am, bh, c);
     return mma(ah, bh, c);
 }
 

@@ -51,33 +51,63 @@ struct Share {
         step(std::integral_constant<int, 0x121>());
         return t;
     }
+    // Sum of row i's squares, the same in the row's 16 lanes.
+    __device__ __forceinline__ float row_norm(int i) const {
+        float s = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NCH; n++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) s = __builtin_fmaf(x[i][n][e], x[i][n][e], s);
+        return row_sum(s);
+    }
     __device__ __forceinline__ void scale(int i, float w) {
 #pragma unroll
         for (int n = 0; n < NCH; n++) x[i][n] *= w;
     }
 };
 
-// The block's top and low from its rows' maxima; every thread gets both. Uses 32 words of `sh`.
-__device__ __forceinline__ void block_top(const uint32_t (&row)[4], uint32_t &top, uint32_t &low, uint32_t *sh) {
-    uint32_t t = 0, l = 0xFFFFFFFFu;
+// Largest of a value over the wavefront's four rows of 16 lanes, whose lanes hold the same.
+__device__ __forceinline__ uint32_t rows_umax(uint32_t v) {
+    const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = max(p[0], p[1]);
+    const auto q = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return max(q[0], q[1]);
+}
+// The block's top and low from its rows' maxima, and its largest `norm`; every thread gets them. Uses 12 words of `sh`.
+__device__ __forceinline__ void block_top(const uint32_t (&row)[4], uint32_t &top, uint32_t &low, float &norm, uint32_t *sh) {
+    uint32_t t = 0, l = 0xFFFFFFFFu, n = __float_as_uint(norm);  // as bits: a NaN is above all
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         t = max(t, row[i]);
         l = row[i] ? min(l, row[i]) : l;
     }
+    t = rows_umax(t);
+    l = ~rows_umax(~l);
+    n = rows_umax(n);
     __syncthreads();
-    if ((threadIdx.x & 15) == 0) {
-        sh[threadIdx.x >> 4] = t;
-        sh[16 + (threadIdx.x >> 4)] = l;
+    if ((threadIdx.x & 63) == 0) {
+        sh[threadIdx.x >> 6] = t;
+        sh[4 + (threadIdx.x >> 6)] = l;
+        sh[8 + (threadIdx.x >> 6)] = n;
     }
     __syncthreads();
     top = sh[0];
-    low = sh[16];
+    low = sh[4];
+    n = sh[8];
 #pragma unroll
-    for (int i = 1; i < 16; i++) {
+    for (int i = 1; i < 4; i++) {
         top = max(top, sh[i]);
-        low = min(low, sh[16 + i]);
+        low = min(low, sh[4 + i]);
+        n = max(n, sh[8 + i]);
     }
+    norm = __uint_as_float(n);
+}
+__device__ __forceinline__ void block_top(const uint32_t (&row)[4], uint32_t &top, uint32_t &low, uint32_t *sh) {
+    float none = 0.0f;
+    block_top(row, top, low, none, sh);
+}
+__device__ __forceinline__ float larger(float a, float b) {  // of sums of squares; a NaN is the largest
+    return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
 }
 
 // Writes the block's two planes in rows or columns form: through LDS (DP * 256 bytes), so that memory gets whole lines.
@@ -121,6 +151,7 @@ __device__ __forceinline__ void split_keys(const Rule &u, const float *src, int6
                                            const SplitOut &o, char *lds, uint32_t *sh) {
     Share<DP> s;
     uint32_t top4[4], top, low;
+    float norm = 0.0f;
     int dlo = INT32_MAX, dhi = -1, doc[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
@@ -134,10 +165,11 @@ __device__ __forceinline__ void split_keys(const Rule &u, const float *src, int6
         const bool there = t * kBlock + 4 * (int)(threadIdx.x >> 4) + i < u.lk;
         s.keep(i, there && doc[i] >= 0);
         top4[i] = s.row_top(i);
+        if (!o.is_v) norm = larger(norm, s.row_norm(i));
         dhi = max(dhi, there ? doc[i] : -1);
         dlo = min(dlo, there ? doc[i] : INT32_MAX);
     }
-    block_top(top4, top, low, sh);
+    block_top(top4, top, low, norm, sh);
     const bool ok = in_range(top) && even_rows(top, low);
     const int e = ok && top ? scale_exp(top) : 0;
     const float w = pow2(-e);
@@ -163,6 +195,7 @@ __device__ __forceinline__ void split_keys(const Rule &u, const float *src, int6
         st.scale = pow2(e);
         st.doc_lo = dlo;
         st.doc_hi = dhi;
+        st.norm = norm;
         o.stats[at] = st;
     }
     __syncthreads();
@@ -205,6 +238,7 @@ struct RowStats {
     uint32_t g2_top, q2_top;  // largest magnitudes (bits) of the latter two
     uint32_t bad;          // the split cannot hold the block
     int32_t doc_lo, doc_hi;
+    float norm;            // largest sum of the squares of a row of q
 };
 struct RowsOut {
     char *q, *g;    // rows form: q by one scale per block, g by one per row
@@ -226,6 +260,7 @@ __device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, 
     Share<DP> s, g, ov;
     float rl[4], w[4], delta[4], m[4];
     uint32_t qt[4], gt[4];
+    float norm = 0.0f;
     int dlo = INT32_MAX, dhi = INT32_MIN, doc[4];
     bool bad = false;
 #pragma unroll
@@ -260,6 +295,7 @@ __device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, 
             for (int e = 0; e < 4; e++) dot = __builtin_fmaf(g.x[i][n][e], ov.x[i][n][e], dot);
         dot = row_sum(dot);
         qt[i] = s.row_top(i);
+        norm = larger(norm, s.row_norm(i));
         gt[i] = g.row_top(i);
         const bool fine = gt[i] == 0 || (gt[i] >= kWideLeast && gt[i] <= kWideMost);
         const int re = fine && gt[i] ? scale_exp(gt[i]) : 0;
@@ -281,7 +317,8 @@ __device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, 
     RowStats st = {};
     uint32_t top, low;
     // q, one scale
-    block_top(qt, top, low, sh);
+    block_top(qt, top, low, norm, sh);
+    st.norm = norm;
     const bool qok = in_range(top);
     bad = bad || !qok;
     const int eq = qok && top ? scale_exp(top) : 0;

@@ -1,0 +1,69 @@
+"""Scored attention where values or scores leave the ordinary range, against the float64 definition.
+
+Tolerances: as in test_attention_scored_gpu.py (1e-5 of the largest value) where nothing else is said."""
+import numpy as np
+import pytest
+
+from gpu_util import Dev
+from test_attention_scored_gpu import TOL, Case, near
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def dev():
+    return Dev()
+
+
+def winners(c, size):
+    """Each query points at one key that it sees: that key's score is about size * sqrt(d), the others' a few times less."""
+    B, H, Hk, lq, lk, d = c.dims
+    for t in range(lq):
+        c.q[:, t] = np.float32(size) * np.repeat(c.k[:, (t + lk - lq) // 2], H // Hk, 1)
+
+
+@pytest.mark.parametrize("s", [(1, 4, 2, 200, 200, 64), (2, 2, 1, 60, 300, 96), (1, 2, 2, 150, 150, 128), (1, 4, 1, 90, 90, 20),
+                               (4, 4, 4, 100, 120, 32), (2, 2, 1, 160, 300, 96), (1, 4, 2, 260, 260, 128)], ids=str)
+@pytest.mark.parametrize("size", [10.0, 1e3, 1e5, 1e8])
+def test_scores_of_any_size_with_clear_winners(dev, s, size):
+    """Weights are one for the winner. A recomputed score of the matrix products is within 2^-22 of itself, and so is the
+    weight that the backward takes from it: their scores are kept below 2^10, beyond it sums round equally both ways. dq and dk
+    are nothing but what rounding leaves of g . v - g . o: 2^-20 of the sum of magnitudes, times the row or key it goes with."""
+    c = Case(dev, *s, causal=1, seed=41)
+    winners(c, size)
+    want = c.reference()
+    near(c.forward(), want[0], what="o")
+    dq, dk, dv = c.backward()
+    near(dv, want[3], TOL + min(2.0 ** 10, 2 * size * s[5] ** 0.5) * 2.0 ** -22, what="dv")
+    left = 2.0 ** -20 * np.abs(c.g).sum(3).max() * np.abs(c.v).max() * s[5] ** -0.5
+    near(dq, want[1], what="dq", floor=left * np.abs(c.k).max())
+    near(dk, want[2], what="dk", floor=left * np.abs(c.q).max() * s[3])
+
+
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+def test_queries_of_very_different_size_in_one_block(dev, cap):
+    """Every other query 2^32 times as large with a gradient as much smaller: the small ones' scores keep their bits."""
+    c = Case(dev, 1, 4, 2, 190, 190, 64, causal=1, seed=42, cap=cap)
+    c.q[:, ::2] *= np.float32(2.0 ** 32)
+    c.g[:, ::2] *= np.float32(2.0 ** -32)
+    want = c.reference()
+    o, (dq, dk, dv) = c.forward(), c.backward()
+    near(o[:, 1::2], want[0][:, 1::2], what="o")
+    near(dq[:, 1::2], want[1][:, 1::2], what="dq")
+    near(dv, want[3], what="dv")
+    near(dk, want[2], what="dk", floor=c.floor()[1] * 2.0 ** -32)  # the large queries' part: their gradients are as small
+
+
+@pytest.mark.parametrize("kw", [dict(scale=1e-43), dict(scale=-1e-20), dict(scale=1e-30, cap=1e-9), dict(cap=1e36), dict(cap=1e25, scale=1e-5),
+                                dict(scale=1e20)], ids=str)
+def test_scale_and_cap_far_from_one(dev, kw):
+    c = Case(dev, 1, 4, 2, 150, 150, 64, causal=1, seed=43, **kw)
+    if kw.get("scale") == 1e20:
+        winners(c, 1.0)
+    want = c.reference()
+    near(c.forward(), want[0], what="o")
+    dq, dk, dv = c.backward()
+    near(dv, want[3], what="dv")
+    if kw.get("scale") != 1e20:  # dq and dk are zero there: see test_scores_of_any_size_with_clear_winners
+        near(dq, want[1], what="dq", floor=c.floor()[0])
+        near(dk, want[2], what="dk", floor=c.floor()[1])
