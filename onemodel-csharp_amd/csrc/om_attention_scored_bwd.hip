@@ -613,7 +613,7 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
 #pragma unroll
     for (int n = 0; n < ROWS / kBlock; n++) {
         const RowStats r = a.rs[rt0 + min(first / kBlock + n, a.nr - 1)];
-        bad = bad || r.bad;
+        bad = bad || (r.bad & kBadRows);
         qnorm = larger(qnorm, r.norm);
         qlo = min(qlo, r.doc_lo);
         qhi = max(qhi, r.doc_hi);

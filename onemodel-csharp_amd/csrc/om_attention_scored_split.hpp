@@ -232,11 +232,13 @@ enum {
     kRowValues = 8
 };
 __host__ __device__ __forceinline__ int64_t row_value(int64_t row, int which) { return (row >> 5) * (32 * kRowValues) + which * 32 + (row & 31); }
-// A block of 64 rows.
+// A block of 64 rows. Either role needs the rows' values and the rows form; only dk and dv the columns form, whose rows may be
+// further apart by their gradients and sums.
+enum { kBadRows = 1, kBadColumns = 2 };
 struct RowStats {
     float q, g2, q2;       // scales 2^e of q, of g / l and of q w
     uint32_t g2_top, q2_top;  // largest magnitudes (bits) of the latter two
-    uint32_t bad;          // the split cannot hold the block
+    uint32_t bad;          // what the split cannot hold of the block: kBadRows, kBadColumns
     int32_t doc_lo, doc_hi;
     float norm;            // largest sum of the squares of a row of q
 };
@@ -262,7 +264,7 @@ __device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, 
     uint32_t qt[4], gt[4];
     float norm = 0.0f;
     int dlo = INT32_MAX, dhi = INT32_MIN, doc[4];
-    bool bad = false;
+    bool bad = false, bad_columns = false;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const Row row = row_of(u, hk, min(t * kBlock + 4 * (int)(threadIdx.x >> 4) + i, rows - 1));
@@ -349,7 +351,7 @@ __device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, 
         }
         block_top(t4, top, low, sh);
         const bool ok = top == 0 || (top >= kWideLeast && top <= kWideMost && even_rows(top, low));
-        bad = bad || !ok;
+        bad_columns = bad_columns || !ok;
         const int e = ok && top ? scale_exp(top) : 0;
         scale = pow2(e);
         kept = top;
@@ -360,7 +362,7 @@ __device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, 
     cols(g, rl, o.g2, st.g2, st.g2_top);
     cols(s, w, o.q2, st.q2, st.q2_top);
     __syncthreads();
-    const bool wave_bad = __any(bad);
+    const uint32_t wave_bad = (__any(bad) ? kBadRows : 0) | (__any(bad_columns) ? kBadColumns : 0);
     if ((threadIdx.x & 15) == 0) {
         sh[threadIdx.x >> 4] = (uint32_t)dlo;
         sh[16 + (threadIdx.x >> 4)] = (uint32_t)dhi;

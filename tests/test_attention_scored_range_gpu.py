@@ -67,3 +67,16 @@ def test_scale_and_cap_far_from_one(dev, kw):
     if kw.get("scale") != 1e20:  # dq and dk are zero there: see test_scores_of_any_size_with_clear_winners
         near(dq, want[1], what="dq", floor=c.floor()[0])
         near(dk, want[2], what="dk", floor=c.floor()[1])
+
+
+@pytest.mark.parametrize("s", [(1, 4, 2, 200, 200, 64), (1, 4, 4, 260, 300, 32), (1, 8, 2, 130, 140, 96), (1, 4, 2, 260, 260, 128)], ids=str)
+def test_gradient_rows_of_very_different_size(dev, s):
+    """A row's dq scales with its gradient, bit for bit by powers of two: no neighbour's size sends it to other sums."""
+    a, b = (Case(dev, *s, causal=1, cap=12.0, seed=44) for _ in range(2))
+    by = np.where(np.arange(s[3]) % 5 == 2, 20, 0)
+    b.g = np.ldexp(b.g, by[None, :, None, None]).astype(np.float32)
+    a.forward(), b.forward()
+    plain, spread, want = a.backward()[0], b.backward(), b.reference()[1:]
+    assert np.array_equal(spread[0], np.ldexp(plain, by[None, :, None, None]))
+    for got, ref, n in zip(spread, want, ("dq", "dk", "dv")):
+        near(got, ref, what=n, floor=b.floor()[0] if n == "dq" else 0.0)
