@@ -505,11 +505,14 @@ typedef struct {
 /* d from 1 to 256; B, lq and lk may be 0. stats (2 * B * heads * lq floats, or NULL when no backward follows) receives
  * each row's reference exponent in log2 units and the inverse row sum, [B, heads, lq] each. Where rows or keys are few
  * the keys are split over workgroups and joined in a second launch. Larger calls with d up to 128 run on the matrix cores
- * from operands split into fp16 pairs (22 bits), with context scratch for those; where a block of 64 rows of an operand
- * holds an infinity, a NaN or magnitudes that pairs cannot (outside 2^-40 .. 2^40, or rows further apart than 2^14), or where
- * a query's length times a key's times scale passes 709 (2^10 in log2 units: a score is held to 2^-22 of itself, and the
- * backward's weight to as much of the score), the workgroups that use it take plain fp32 sums, many times slower. A scale
- * (or scale / cap) outside 2^-40 .. 2^40 takes the row kernels. Results are the same bits for the same call. o and stats
+ * from operands split into fp16 pairs, with context scratch for those. A pair holds 22 bits, and never less than 2^-36 of the
+ * largest value in its block of 64 rows. Workgroups that would use a block which pairs do not hold take plain fp32 sums, many
+ * times slower: one with an infinity or a NaN, with a largest value outside 2^-40 .. 2^40, or with rows or columns (zero ones
+ * aside) whose largest values are further apart than 2^14 (2^18 for the columns of a single row). Rows count in k, v, g / sum
+ * and q g / sum, columns in v always and in the others where they become a gradient's. So do workgroups where a query's length
+ * times a key's times scale passes 709 (2^10 in log2 units): a score is held to 2^-22 of itself, and the backward's weight to as
+ * much of the score. A scale (or scale / cap) outside 2^-40 .. 2^40 takes the row kernels. Results are the same bits for the
+ * same call. o and stats
  * must not overlap an input or each other. No counterpart in the reference, whose Attention takes an additive mask tensor
  * and equal heads (Ops.Layers.cs:746-807). */
 om_status om_attention_fwd_scored(om_ctx *ctx, const float *q, int ld_q, const float *k, const float *v, int ld_kv,

@@ -636,7 +636,7 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
     for (int t = t0 + (int)threadIdx.x, n = 0; t <= t1; t += 64 * NW, n++) {
         const Stats sk = a.ks[kt0 + t], sv = a.vs[kt0 + t];
         if (n == 0) mk = sk;
-        kt = max(kt, sk.top);
+        kt = max(kt, sk.columns ? sk.top : 0xFFFFFFFFu);
         knorm = max(knorm, __float_as_uint(sk.norm));
         kl = min(kl, sk.low);
         vt = max(vt, sv.top);

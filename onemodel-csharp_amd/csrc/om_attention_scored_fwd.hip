@@ -490,14 +490,15 @@ om_status fwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p, int *joins, f
     FwdArgs a = {};
     a.kn = base;
     a.vt = base + plane;
-    a.ks = reinterpret_cast<Stats *>(base + 2 * plane);
+    // 16-byte stores first, the statistics last
+    float *keys = reinterpret_cast<float *>(base + 2 * plane);
+    a.keys = keys;
+    a.part = ns > 1 ? reinterpret_cast<float *>(base + 2 * plane + words) : nullptr;
+    a.ks = reinterpret_cast<Stats *>(base + 2 * plane + words + join);
     a.vs = a.ks + items * nt;
     a.nt = nt;
     a.blocks = blocks;
     a.nsplit = (int)ns;
-    float *keys = reinterpret_cast<float *>(base + 2 * plane + 2 * stats);
-    a.keys = keys;
-    a.part = ns > 1 ? reinterpret_cast<float *>(base + 2 * plane + 2 * stats + words) : nullptr;
     auto al16 = [](const void *x) { return ((uintptr_t)x & 15) == 0; };
     a.vec = u.d % 4 == 0 && p.ldq % 4 == 0 && al16(p.q);
     const bool vec = u.d % 4 == 0 && p.ldkv % 4 == 0 && al16(p.k) && al16(p.v);

@@ -32,10 +32,10 @@ typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 constexpr int kBlock = 64;  // rows of an operand that share a scale
 
 // What the split found in a block: the largest magnitude (bits; at or above infinity's if the split cannot hold the block),
-// the smallest nonzero row maximum (bits), 2^e of its scale, the range of its document ids, and the largest sum of a row's
-// squares.
+// the smallest nonzero row maximum (bits), whether its columns keep their bits too, 2^e of its scale, the range of its document
+// ids, and the largest sum of a row's squares.
 struct Stats {
-    uint32_t top, low;
+    uint32_t top, low, columns;
     float scale;
     int32_t doc_lo, doc_hi;
     float norm;

@@ -73,38 +73,88 @@ __device__ __forceinline__ uint32_t rows_umax(uint32_t v) {
     const auto q = __builtin_amdgcn_permlane32_swap(v, v, false, false);
     return max(q[0], q[1]);
 }
-// The block's top and low from its rows' maxima, and its largest `norm`; every thread gets them. Uses 12 words of `sh`.
-__device__ __forceinline__ void block_top(const uint32_t (&row)[4], uint32_t &top, uint32_t &low, float &norm, uint32_t *sh) {
-    uint32_t t = 0, l = 0xFFFFFFFFu, n = __float_as_uint(norm);  // as bits: a NaN is above all
+// Sum of a count over the same.
+__device__ __forceinline__ uint32_t rows_usum(uint32_t v) {
+    const auto p = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = p[0] + p[1];
+    const auto q = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return q[0] + q[1];
+}
+// What a block of 64 rows holds: the largest magnitude (bits), the smallest nonzero row and column maximum, its rows that are
+// not zero, and the largest of the threads' `norm`.
+struct BlockTop {
+    uint32_t top, low, column, rows;
+    float norm;
+};
+// Of a block with these row maxima; every thread gets it. COLUMNS: columns too (else they count as even), from the staging
+// buffer `lds` (16 bytes a column). Uses 16 words of `sh`.
+template <int DP, bool COLUMNS>
+__device__ __forceinline__ BlockTop block_top(const Share<DP> &s, const uint32_t (&row)[4], float norm, uint32_t *sh, char *lds) {
+    constexpr int NCH = Share<DP>::NCH;
+    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    uint32_t t = 0, l = 0xFFFFFFFFu, live = 0;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         t = max(t, row[i]);
         l = row[i] ? min(l, row[i]) : l;
+        live += row[i] ? 1 : 0;
     }
     t = rows_umax(t);
     l = ~rows_umax(~l);
-    n = rows_umax(n);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) {
-        sh[threadIdx.x >> 6] = t;
-        sh[4 + (threadIdx.x >> 6)] = l;
-        sh[8 + (threadIdx.x >> 6)] = n;
+    const uint32_t n = rows_umax(__float_as_uint(norm));  // as bits: a NaN is above all
+    live = rows_usum(live);
+    u32x4 c[NCH];
+    if constexpr (COLUMNS) {
+#pragma unroll
+        for (int k = 0; k < NCH; k++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                uint32_t m = 0;
+#pragma unroll
+                for (int i = 0; i < 4; i++) m = max(m, __float_as_uint(s.x[i][k][e]) & 0x7FFFFFFFu);
+                c[k][e] = rows_umax(m);
+            }
     }
     __syncthreads();
-    top = sh[0];
-    low = sh[4];
-    n = sh[8];
+    if (lane == 0) {
+        sh[w] = t;
+        sh[4 + w] = l;
+        sh[8 + w] = n;
+        sh[12 + w] = live;
+    }
+    uint32_t *columns = reinterpret_cast<uint32_t *>(lds);
+    if constexpr (COLUMNS) {
+#pragma unroll
+        for (int k = 0; k < NCH; k++)
+            if (lane < 16 && 64 * k + 4 * lane < DP) *reinterpret_cast<u32x4 *>(columns + w * DP + 64 * k + 4 * lane) = c[k];
+    }
+    __syncthreads();
+    BlockTop r = {sh[0], sh[4], 0xFFFFFFFFu, sh[12], 0.0f};
+    uint32_t most = sh[8];
 #pragma unroll
     for (int i = 1; i < 4; i++) {
-        top = max(top, sh[i]);
-        low = min(low, sh[4 + i]);
-        n = max(n, sh[8 + i]);
+        r.top = max(r.top, sh[i]);
+        r.low = min(r.low, sh[4 + i]);
+        most = max(most, sh[8 + i]);
+        r.rows += sh[12 + i];
     }
-    norm = __uint_as_float(n);
+    r.norm = __uint_as_float(most);
+    if constexpr (COLUMNS) {
+#pragma unroll
+        for (int k = 0; k < NCH; k++) {
+            const int at = min(64 * k + lane, DP - 1);
+            const uint32_t m = max(max(columns[at], columns[DP + at]), max(columns[2 * DP + at], columns[3 * DP + at]));
+            r.column = min(r.column, m ? m : 0xFFFFFFFFu);
+        }
+        r.column = wave_umin(r.column);
+    }
+    return r;
 }
-__device__ __forceinline__ void block_top(const uint32_t (&row)[4], uint32_t &top, uint32_t &low, uint32_t *sh) {
-    float none = 0.0f;
-    block_top(row, top, low, none, sh);
+// Whether every column that is not zero keeps its bits: its largest value within 2^14 of the block's, so held to 2^-22 of
+// itself. In a single row each column is one value, and one in 8000 of a normal's is 2^14 below the largest: there 2^18,
+// held to 2^-18.
+__device__ __forceinline__ bool even_columns(const BlockTop &b) {
+    return b.top == 0 || (b.top >> 23) - (b.column >> 23) <= (b.rows > 1 ? 14 : 18);
 }
 __device__ __forceinline__ float larger(float a, float b) {  // of sums of squares; a NaN is the largest
     return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
@@ -150,7 +200,7 @@ template <int DP, bool VEC>
 __device__ __forceinline__ void split_keys(const Rule &u, const float *src, int64_t ld, int b, int hk, int t, int64_t at,
                                            const SplitOut &o, char *lds, uint32_t *sh) {
     Share<DP> s;
-    uint32_t top4[4], top, low;
+    uint32_t top4[4];
     float norm = 0.0f;
     int dlo = INT32_MAX, dhi = -1, doc[4];
 #pragma unroll
@@ -169,9 +219,10 @@ __device__ __forceinline__ void split_keys(const Rule &u, const float *src, int6
         dhi = max(dhi, there ? doc[i] : -1);
         dlo = min(dlo, there ? doc[i] : INT32_MAX);
     }
-    block_top(top4, top, low, norm, sh);
-    const bool ok = in_range(top) && even_rows(top, low);
-    const int e = ok && top ? scale_exp(top) : 0;
+    const BlockTop bt = block_top<DP, true>(s, top4, norm, sh, lds);
+    // V's columns are a product's rows or columns either way, K's only in dq: a score bounded by kMostScore loses nothing
+    const bool even = even_columns(bt), ok = in_range(bt.top) && even_rows(bt.top, bt.low) && (even || !o.is_v);
+    const int e = ok && bt.top ? scale_exp(bt.top) : 0;
     const float w = pow2(-e);
 #pragma unroll
     for (int i = 0; i < 4; i++) s.scale(i, w);
@@ -190,12 +241,13 @@ __device__ __forceinline__ void split_keys(const Rule &u, const float *src, int6
             dhi = max(dhi, (int)sh[16 + i]);
         }
         Stats st = {};
-        st.top = ok ? top : 0xFFFFFFFFu;
-        st.low = low;
+        st.top = ok ? bt.top : 0xFFFFFFFFu;
+        st.low = bt.low;
+        st.columns = ok && even;
         st.scale = pow2(e);
         st.doc_lo = dlo;
         st.doc_hi = dhi;
-        st.norm = norm;
+        st.norm = bt.norm;
         o.stats[at] = st;
     }
     __syncthreads();
@@ -233,7 +285,7 @@ enum {
 };
 __host__ __device__ __forceinline__ int64_t row_value(int64_t row, int which) { return (row >> 5) * (32 * kRowValues) + which * 32 + (row & 31); }
 // A block of 64 rows. Either role needs the rows' values and the rows form; only dk and dv the columns form, whose rows may be
-// further apart by their gradients and sums.
+// further apart by their gradients and sums, and whose columns have to be near each other.
 enum { kBadRows = 1, kBadColumns = 2 };
 struct RowStats {
     float q, g2, q2;       // scales 2^e of q, of g / l and of q w
@@ -317,13 +369,12 @@ __device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, 
         }
     }
     RowStats st = {};
-    uint32_t top, low;
     // q, one scale
-    block_top(qt, top, low, norm, sh);
-    st.norm = norm;
-    const bool qok = in_range(top);
+    const BlockTop qb = block_top<DP, false>(s, qt, norm, sh, lds);
+    st.norm = qb.norm;
+    const bool qok = in_range(qb.top);
     bad = bad || !qok;
-    const int eq = qok && top ? scale_exp(top) : 0;
+    const int eq = qok && qb.top ? scale_exp(qb.top) : 0;
     st.q = pow2(eq);
     Share<DP> x;
 #pragma unroll
@@ -349,12 +400,12 @@ __device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, 
             y.scale(i, f[i]);
             t4[i] = y.row_top(i);
         }
-        block_top(t4, top, low, sh);
-        const bool ok = top == 0 || (top >= kWideLeast && top <= kWideMost && even_rows(top, low));
+        const BlockTop bt = block_top<DP, true>(y, t4, 0.0f, sh, lds);
+        const bool ok = bt.top == 0 || (bt.top >= kWideLeast && bt.top <= kWideMost && even_rows(bt.top, bt.low) && even_columns(bt));
         bad_columns = bad_columns || !ok;
-        const int e = ok && top ? scale_exp(top) : 0;
+        const int e = ok && bt.top ? scale_exp(bt.top) : 0;
         scale = pow2(e);
-        kept = top;
+        kept = bt.top;
 #pragma unroll
         for (int i = 0; i < 4; i++) y.scale(i, pow2(-e));
         put_block<DP, true>(y, out + at * plane_bytes(DP, 1), lds);

@@ -80,3 +80,48 @@ def test_gradient_rows_of_very_different_size(dev, s):
     assert np.array_equal(spread[0], np.ldexp(plain, by[None, :, None, None]))
     for got, ref, n in zip(spread, want, ("dq", "dk", "dv")):
         near(got, ref, what=n, floor=b.floor()[0] if n == "dq" else 0.0)
+
+
+COLUMN_SHAPES = [(1, 4, 2, 200, 200, 64), (1, 4, 4, 260, 300, 32), (1, 8, 2, 130, 140, 96), (1, 4, 2, 260, 260, 128), (1, 4, 2, 193, 193, 40)]
+
+
+@pytest.mark.parametrize("s", COLUMN_SHAPES, ids=str)
+@pytest.mark.parametrize("power", [-20, -28, -36])
+@pytest.mark.parametrize("which", ["q", "k", "v", "g"])
+def test_columns_of_very_different_size(dev, which, power, s):
+    """A column of one operand 2^power times as large: the column that it makes of an output keeps its own precision."""
+    c = Case(dev, *s, causal=1, seed=45)
+    getattr(c, which)[..., 7] *= np.float32(2.0 ** power)
+    want = c.reference()
+    got = [c.forward()] + c.backward()
+    out = {"v": 0, "k": 1, "q": 2, "g": 3}[which]
+    floors = [0.0, c.floor()[0], 0.0, 0.0]
+    near(got[out][..., 7], want[out][..., 7], what=which, floor=floors[out] * 2.0 ** power)
+    for g, w, n, f in zip(got, want, ("o", "dq", "dk", "dv"), floors):
+        near(g, w, what=n, floor=f)
+
+
+@pytest.mark.parametrize("s", COLUMN_SHAPES, ids=str)
+def test_a_small_column_of_v_beside_a_large_one_of_g(dev, s):
+    """Values and gradients whose columns' sizes cancel: g . v keeps its bits."""
+    c = Case(dev, *s, causal=1, seed=46)
+    want = c.reference()
+    c.v[..., 7] *= np.float32(2.0 ** -28)
+    c.g[..., 7] *= np.float32(2.0 ** 28)
+    near(c.forward()[..., :7], want[0][..., :7], what="o")
+    dq, dk, dv = c.backward()
+    near(dq, want[1], what="dq", floor=2.0 ** -22 * 64 * 8 * s[5] ** -0.5)  # sums of up to d products below 8, four roundings
+    near(dk, want[2], what="dk")
+    near(dv[..., :7], want[3][..., :7], what="dv")
+
+
+def test_columns_of_one_live_row(dev):
+    """A last block of one key or query: its columns are single values, and stay on the matrix cores down to 2^-18 of the largest."""
+    c = Case(dev, 1, 4, 2, 193, 193, 64, causal=1, seed=47)
+    for x in (c.q, c.k, c.v, c.g):
+        x[:, 192, :, 3] *= np.float32(2.0 ** -19)
+        x[:, 192, :, 9] = 0.0
+    want = c.reference()
+    for g, w, n, f in zip([c.forward()] + c.backward(), want, ("o", "dq", "dk", "dv"), (0.0, *c.floor(), 0.0)):
+        near(g, w, what=n, floor=f)
+    near(c.backward()[2][:, 192], want[3][:, 192], what="dv of the last key")
