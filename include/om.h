@@ -457,9 +457,9 @@ om_status om_attention_bwd_flash(om_ctx *ctx, const float *q, const float *k, co
  *   OM_ROPE_NTK     the base becomes base * factor^(rot / (rot - 2)) (rot > 2), which divides the slowest pair's f by factor;
  *   OM_ROPE_BANDS   with turns = f_i * trained / (2 pi), the turns pair i makes in the trained context, and keep =
  *                   clamp((turns - low) / (high - low), 0, 1): f_i * (keep + (1 - keep) / factor).
- * amp multiplies the turned values (1 for none). The f_i are formed on the host in double, an angle's turns and their
- * fractional part in double on the device, so positions up to 2^31 - 1 keep their angle within 4e-7. No counterpart in
- * the reference, whose models learn their positions. */
+ * amp multiplies the turned values (1 for none). The f_i are formed on the host in long double and rounded to double, an
+ * angle's turns and their fractional part are exact on the device, so every position keeps its angle within 4e-7 (2^-53 of the
+ * angle and 5e-8). No counterpart in the reference, whose models learn their positions. */
 enum { OM_ROPE_HALF = 0, OM_ROPE_INTERLEAVED = 1 };
 enum { OM_ROPE_PLAIN = 0, OM_ROPE_LINEAR = 1, OM_ROPE_NTK = 2, OM_ROPE_BANDS = 3 };
 typedef struct {

@@ -3,8 +3,10 @@
 //
 // Bound: HBM, 8 bytes per value (one read, one write) plus 4 per token. The angle costs about 45 vector instructions
 // per pair, which a CU hides eight times over under its share of the bandwidth (8 B per cycle), so nothing is tabulated
-// and every thread forms its own: turns = pos * (f_i / 2 pi) in double (relative error 2^-52, so 2^-23 of a turn at 2^31
-// turns), the fractional part exactly in double, then sine and cosine of an eighth turn by their Taylor sums in fp32.
+// and every thread forms its own: turns = pos * (f_i / 2 pi) in double with the product's rounding error beside it, the
+// fractional part exactly, then sine and cosine of an eighth turn by their Taylor sums in fp32. What is left of an angle's error
+// is f_i's one rounding, 2^-53 of the angle (2.4e-7 at 2^31), and the eighth turn's in fp32, 5e-8. (f_i as two doubles leaves
+// only the latter, but their reads cost 3 % of a long call and a third of a short one.)
 #include "om_internal.hpp"
 
 #include <cmath>
@@ -16,9 +18,10 @@ struct Turns {
     double f[kMaxPairs];  // turns per position of pair i
 };
 
-// (cos, sin)(2 pi turns), each within 1.2e-7.
-__device__ __forceinline__ void cos_sin(double turns, float &c, float &s) {
-    const double r = turns - __builtin_rint(turns);  // -1/2 .. 1/2, exact
+// (cos, sin)(2 pi pos f), each within 1.2e-7.
+__device__ __forceinline__ void cos_sin(double pos, double f, float &c, float &s) {
+    const double turns = pos * f, left = __builtin_fma(pos, f, -turns);  // the product, exactly
+    const double r = turns - __builtin_rint(turns) + left;  // -1/2 .. 1/2, the difference exact
     const double q = __builtin_rint(4.0 * r);        // quarter turns: -2 .. 2
     const float y = (float)((r - 0.25 * q) * 6.283185307179586);  // |y| <= pi / 4
     const float z = y * y;
@@ -70,7 +73,7 @@ __global__ void __launch_bounds__(256) k_rope(const float *x, int64_t ldx, const
         float c[W], s[W];
 #pragma unroll
         for (int w = 0; w < W; w++) {
-            cos_sin(ps * tr.f[p0 + w], c[w], s[w]);
+            cos_sin(ps, tr.f[p0 + w], c[w], s[w]);
             c[w] *= amp;
             s[w] *= amp * sign;
         }
@@ -130,18 +133,22 @@ om_status rope(om_ctx *ctx, const char *what, const float *x, int ldx, const int
     OM_REQUIRE(ctx, pos || (int64_t)pos0 + (seq < rows ? seq : rows) - 1 <= INT32_MAX, "%s: positions past 2^31 - 1", what);
     if (om_status s = om::use_device(ctx)) return s;
     const int rot = rp->rot;
-    const double base = rp->scaling == OM_ROPE_NTK ? rp->base * std::pow(rp->factor, rot / (rot - 2.0)) : rp->base;
+    // In the host's 64-bit significands and rounded once, each speed from the one before: 128 products are 2^-56 of it off. (A
+    // power for each took 8 us a call.)
+    typedef long double wide;
+    const wide base = rp->scaling == OM_ROPE_NTK ? rp->base * std::pow((wide)rp->factor, rot / (rot - (wide)2)) : (wide)rp->base;
+    const wide step = std::pow(base, (wide)-2 / rot);
+    wide plain = 1 / 6.283185307179586476925286766559L;
     Turns tr = {};
-    for (int i = 0; i < rot / 2; i++) {
-        double f = std::pow(base, -2.0 * i / rot);
+    for (int i = 0; i < rot / 2; i++, plain *= step) {
+        wide f = plain;
         if (rp->scaling == OM_ROPE_LINEAR) f /= rp->factor;
-        f /= 6.283185307179586;
         if (rp->scaling == OM_ROPE_BANDS) {
-            double keep = (f * rp->trained - rp->low) / (rp->high - rp->low);
-            keep = keep < 0.0 ? 0.0 : keep > 1.0 ? 1.0 : keep;
-            f *= keep + (1.0 - keep) / rp->factor;
+            wide keep = (f * rp->trained - rp->low) / ((wide)rp->high - rp->low);
+            keep = keep < 0 ? 0 : keep > 1 ? 1 : keep;
+            f *= keep + (1 - keep) / rp->factor;
         }
-        tr.f[i] = f;
+        tr.f[i] = (double)f;
     }
     const bool half = rp->layout == OM_ROPE_HALF;
     // 16-byte slots where every one starts at a multiple of 16 bytes
