@@ -139,7 +139,8 @@ om_status om_readback_wait(om_readback *r, void *dst_host, uint64_t bytes);
  * Inside a capture, calls that would wait for the device or read host memory when the graph runs fail with
  * OM_E_STATE and leave the capture unusable (abort it): om_upload, om_download, om_ctx_sync, om_sgd_step (its rate
  * and first-step flag are host values), the stager calls, a second readback object, and growth of the context's
- * scratch (run one step outside a capture first, so scratch and arena have their steady size).
+ * scratch (run one step outside a capture first, so scratch and arena have their steady size). Scratch that later calls
+ * outgrow is kept for the graphs that use it, until the context's last graph is destroyed.
  * om_graph_launch waits, if need be, until the previous launch of the same graph has read its values.
  * No counterpart in the reference, whose step runs on the CPU (TrainCase.cs:114-127). */
 typedef struct om_graph om_graph;

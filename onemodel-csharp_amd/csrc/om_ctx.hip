@@ -55,7 +55,7 @@ static om_status grow(om_ctx *ctx, float *&buf, uint64_t &have, uint64_t bytes, 
     // No kernel may still use the old buffer, nor a captured graph that is launched again later.
     om_status s = check_hip(ctx, hipStreamSynchronize(ctx->stream), "scratch sync");
     if (s) return s;
-    if (buf && ctx->captured) ctx->outgrown.push_back(buf);
+    if (buf && ctx->graphs > 0) ctx->outgrown.push_back(buf);
     else if (buf) (void)hipFree(buf);
     buf = nullptr;
     have = 0;
@@ -399,7 +399,11 @@ void free_graph(om_graph *g) {
     if (g->graph) (void)hipGraphDestroy(g->graph);
     if (g->dev) (void)hipFree(g->dev);
     if (g->host) (void)hipHostFree(g->host);
+    om_ctx *ctx = g->ctx;
     delete g;
+    if (--ctx->graphs > 0) return;
+    for (float *b : ctx->outgrown) (void)hipFree(b);  // waits for what still runs
+    ctx->outgrown.clear();
 }
 
 }  // namespace
@@ -411,6 +415,7 @@ om_status om_graph_capture_begin(om_ctx *ctx) {
     if (ctx->cap) return om::fail(ctx, OM_E_STATE, "om_graph_capture_begin: a capture is already running");
     om_graph *g = new om_graph;
     g->ctx = ctx;
+    ctx->graphs++;
     // Fine-grained (coherent) pinned memory: the first node reads what the host wrote just before the launch, and
     // the host polls the ack the node writes, with no cache in between.
     hipError_t e = hipHostMalloc((void **)&g->host, 64, hipHostMallocCoherent);
@@ -426,7 +431,6 @@ om_status om_graph_capture_begin(om_ctx *ctx) {
         return om::check_hip(ctx, e, "om_graph_capture_begin");
     }
     ctx->cap = g;
-    ctx->captured = true;
     hipLaunchKernelGGL(k_step_begin, dim3(1), dim3(64), 0, ctx->stream, (const om_step_block *)g->host, g->dev,
                        (uint64_t *)(g->host + sizeof(om_step_block)));
     om_status s = OM_LAUNCH_CHECK(ctx, "om_graph_capture_begin");

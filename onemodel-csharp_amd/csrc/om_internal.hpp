@@ -55,9 +55,9 @@ struct om_ctx {
     // (claimed by its first allocation-free call, released by om_ctx_destroy; -1 while it holds none).
     void *noalloc_scratch = nullptr;
     int noalloc_slot = -1;
-    // Scratch buffers outgrown after a step graph was captured on this context: the graph's launches still hold their
-    // addresses, so they live until om_ctx_destroy.
-    bool captured = false;
+    // Step graphs captured on this context and not destroyed yet (one being captured counts), and the scratch buffers that
+    // were outgrown meanwhile: the graphs' launches hold their addresses, so they live as long as a graph does.
+    int graphs = 0;
     std::vector<float *> outgrown;
     // How the GELU epilogues of products evaluate erf and exp (om_ctx_set_gelu).
     int gelu_mode = OM_GELU_FAST;
