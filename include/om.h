@@ -512,8 +512,8 @@ typedef struct {
  * aside) whose largest values are further apart than 2^14 (2^18 for the columns of a single row). Rows count in k, v, g / sum
  * and q g / sum, columns in v always and in the others where they become a gradient's. So do workgroups where a query's length
  * times a key's times scale passes 709 (2^10 in log2 units): a score is held to 2^-22 of itself, and the backward's weight to as
- * much of the score. A scale (or scale / cap) outside 2^-40 .. 2^40 takes the row kernels. Results are the same bits for the
- * same call. o and stats
+ * much of the score; and where a slope times lq + lk passes 2^22 in log2 units. A scale (or scale / cap) outside 2^-40 .. 2^40
+ * takes the row kernels. Results are the same bits for the same call. o and stats
  * must not overlap an input or each other. No counterpart in the reference, whose Attention takes an additive mask tensor
  * and equal heads (Ops.Layers.cs:746-807). */
 om_status om_attention_fwd_scored(om_ctx *ctx, const float *q, int ld_q, const float *k, const float *v, int ld_kv,

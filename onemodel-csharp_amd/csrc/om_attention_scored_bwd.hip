@@ -454,13 +454,13 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
                 const floatx4 m4 = *reinterpret_cast<const floatx4 *>(rv + 32 * kRowM + 8 * q);
                 floatx4 y;
 #pragma unroll
-                for (int r = 0; r < 4; r++) y[r] = __builtin_fmaf(x[4 * q + r], fx, m4[r]);
+                for (int r = 0; r < 4; r++) y[r] = SLOPES ? x[4 * q + r] * fx : __builtin_fmaf(x[4 * q + r], fx, m4[r]);
                 if (SLOPES || !whole) {
                     const intx4 p4 = *reinterpret_cast<const intx4 *>(rv + 32 * kRowPos + 8 * q);
-                    if (SLOPES) {
+                    if (SLOPES) {  // each rounding as in the forward, so that a score that is mostly bias cancels with its maximum
                         const floatx4 s4 = *reinterpret_cast<const floatx4 *>(rv + 32 * kRowSlope + 8 * q);
 #pragma unroll
-                        for (int r = 0; r < 4; r++) y[r] = __builtin_fmaf(-s4[r], __builtin_fabsf((float)(p4[r] - j)), y[r]);
+                        for (int r = 0; r < 4; r++) y[r] = __builtin_fmaf(-s4[r], __builtin_fabsf((float)(p4[r] - j)), y[r]) + m4[r];
                     }
                     if (!whole) {
                         intx4 qd = {kd, kd, kd, kd};
@@ -790,9 +790,8 @@ __device__ __forceinline__ void rows_role(const Rule &u, const Ptrs &p, const Bw
             const float gap0 = (float)(pos - j0 - 4 * g);
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-                float y = __builtin_fmaf(x[e], fx, mu);
                 const int o = 8 * (e >> 2) + (e & 3);
-                if (SLOPES) y = __builtin_fmaf(-slope, __builtin_fabsf(gap0 - (float)o), y);
+                float y = SLOPES ? __builtin_fmaf(-slope, __builtin_fabsf(gap0 - (float)o), x[e] * fx) + mu : __builtin_fmaf(x[e], fx, mu);
                 if (!whole) y = (reach.has(j0 + 4 * g + o) & (!DOCS || words[kKeyDoc + 4 * g + o] == doc)) ? y : -3e38f;
                 const float ex = exp2_hw(y);
                 x[e] = CAP ? ex * __builtin_fmaf(-x[e], x[e], 1.0f) : ex;

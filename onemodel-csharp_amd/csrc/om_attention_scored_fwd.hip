@@ -201,8 +201,8 @@ __global__ void __launch_bounds__(256, DP == 32 ? 4 : DP == 64 ? 3 : 2) k_scored
         qnorm = __float_as_uint(pair_sum(norm));
         const auto both = __builtin_amdgcn_permlane32_swap(top, top, false, false);
         top = max(both[0], both[1]);
-        bad = !in_range(top);
-        eq = bad || !top ? 0 : scale_exp(top);
+        bad = !in_range(top) || (SLOPES && !bias_fits(u, slope));
+        eq = !in_range(top) || !top ? 0 : scale_exp(top);
         const float sc = u.scale < 0.0f ? -pow2(-eq) : pow2(-eq);
 #pragma unroll
         for (int s = 0; s < S; s++) {

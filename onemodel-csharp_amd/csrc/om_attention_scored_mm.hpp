@@ -63,6 +63,10 @@ __device__ __forceinline__ bool even_rows(uint32_t top, uint32_t low) { return t
 __device__ __forceinline__ bool scores_fit(const Rule &u, float q_norm, float k_norm) {
     return __builtin_amdgcn_sqrtf(q_norm) * __builtin_amdgcn_sqrtf(k_norm) * __builtin_fabsf(u.cl2) < kMostScore;
 }
+// Whether a row's distance biases leave a score's last bits below a half: further out its weight may outgrow the 2^kLift.
+__device__ __forceinline__ bool bias_fits(const Rule &u, float slope) {
+    return __builtin_fabsf(slope) * ((float)u.lq + (float)u.lk) < 0x1p22f;
+}
 
 // Two values split into packed fp16 pairs: a packed conversion, the two remainders with the halves taken as they lie
 // (v_fma_mix_f32 reads either half of a register as fp16), a packed conversion. Left to itself the compiler converts each

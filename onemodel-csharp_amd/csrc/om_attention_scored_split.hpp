@@ -312,7 +312,7 @@ __device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, 
     const int rows = u.G * u.lq;
     const int64_t all = (int64_t)u.B * u.Hk * rows;
     Share<DP> s, g, ov;
-    float rl[4], w[4], delta[4], m[4];
+    float rl[4], w[4], delta[4], m[4], slope[4];
     uint32_t qt[4], gt[4];
     float norm = 0.0f;
     int dlo = INT32_MAX, dhi = INT32_MIN, doc[4];
@@ -324,6 +324,7 @@ __device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, 
         m[i] = p.st[sr];
         rl[i] = p.st[all + sr];
         doc[i] = u.qd ? u.qd[tok] : 0;
+        slope[i] = u.slopes ? u.slopes[row.h] * kLog2e : 0.0f;
         s.template load<VEC>(i, p.q + tok * p.ldq + (int64_t)row.h * u.d, u.d);
         g.template load<VEC>(i, p.g + tok * p.ldg + (int64_t)row.h * u.d, u.d);
         ov.template load<VEC>(i, p.o + tok * p.ldo + (int64_t)row.h * u.d, u.d);
@@ -356,14 +357,14 @@ __device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, 
         // a row that gives nothing, and one that the split cannot hold, keep finite stand-ins
         w[i] = gt[i] && fine ? rl[i] * pow2(re) : 0.0f;
         delta[i] = fine ? dot * pow2(-re) : 0.0f;
-        bad = bad || !fine || (on && !(__builtin_fabsf(m[i]) < 1e30f && rl[i] > 0.0f && rl[i] < 1e30f && __builtin_fabsf(dot) < 1e38f));
+        bad = bad || !fine || (on && !bias_fits(u, slope[i])) || (on && !(__builtin_fabsf(m[i]) < 1e30f && rl[i] > 0.0f && rl[i] < 1e30f && __builtin_fabsf(dot) < 1e38f));
         m[i] = on ? (float)kLift - m[i] : -kNoRow;
         if ((threadIdx.x & 15) == 0) {
             const int64_t r = at * kBlock + 4 * (threadIdx.x >> 4) + i;
             o.v[row_value(r, kRowM)] = m[i];
             o.v[row_value(r, kRowDelta)] = delta[i];
             o.v[row_value(r, kRowPos)] = __int_as_float(row.t + u.off);
-            o.v[row_value(r, kRowSlope)] = u.slopes ? u.slopes[row.h] * kLog2e : 0.0f;
+            o.v[row_value(r, kRowSlope)] = on ? slope[i] : 0.0f;
             o.v[row_value(r, kRowDoc)] = __int_as_float(doc[i]);
             o.v[row_value(r, kRowW)] = w[i];
         }

@@ -125,3 +125,22 @@ def test_columns_of_one_live_row(dev):
     for g, w, n, f in zip([c.forward()] + c.backward(), want, ("o", "dq", "dk", "dv"), (0.0, *c.floor(), 0.0)):
         near(g, w, what=n, floor=f)
     near(c.backward()[2][:, 192], want[3][:, 192], what="dv of the last key")
+
+
+@pytest.mark.parametrize("s", [(1, 4, 2, 200, 200, 64), (1, 4, 4, 200, 200, 32), (2, 4, 2, 200, 200, 96), (2, 4, 1, 200, 200, 128)], ids=str)
+@pytest.mark.parametrize("slopes", [(0.5, 3.0, 50.0, 800.0), (2e4, 1e6, 3e9, -40.0)], ids=str)
+def test_distance_bias_where_only_far_keys_are_seen(dev, s, slopes):
+    """Half of the queries see only the keys of the other half: their scores are all bias, the nearest key (the furthest, where a
+    slope is negative) has the weight. Rounded the same way in both directions, it is one."""
+    ids = np.repeat([[1, 0]], s[3] // 2, 1).repeat(s[0], 0)
+    c = Case(dev, *s, seed=48, slopes=True, qdoc=ids, kdoc=1 - ids)
+    c.sl[:] = slopes
+    buf = dev.put(c.sl)
+    c.keep.append(buf)
+    c.form.slopes = buf.data_ptr()
+    want = c.reference()
+    near(c.forward(), want[0], what="o")
+    dq, dk, dv = c.backward()
+    near(dv, want[3], what="dv")
+    near(dq, want[1], what="dq", floor=c.floor()[0])
+    near(dk, want[2], what="dk", floor=c.floor()[1])
