@@ -507,13 +507,14 @@ typedef struct {
  * each row's reference exponent in log2 units and the inverse row sum, [B, heads, lq] each. Where rows or keys are few
  * the keys are split over workgroups and joined in a second launch. Larger calls with d up to 128 run on the matrix cores
  * from operands split into fp16 pairs, with context scratch for those. A pair holds 22 bits, and never less than 2^-36 of the
- * largest value in its block of 64 rows. Workgroups that would use a block which pairs do not hold take plain fp32 sums, many
- * times slower: one with an infinity or a NaN, with a largest value outside 2^-40 .. 2^40, or with rows or columns (zero ones
- * aside) whose largest values are further apart than 2^14 (2^18 for the columns of a single row). Rows count in k, v, g / sum
- * and q g / sum, columns in v always and in the others where they become a gradient's. So do workgroups where a query's length
- * times a key's times scale passes 709 (2^10 in log2 units): a score is held to 2^-22 of itself, and the backward's weight to as
- * much of the score; and where a slope times lq + lk passes 2^22 in log2 units. A scale (or scale / cap) outside 2^-40 .. 2^40
- * takes the row kernels. Results are the same bits for the same call. o and stats
+ * largest value in its block of 64 rows (in its row of g, and of q in the forward). Workgroups that would use a block which
+ * pairs do not hold take plain fp32 sums, tens of times slower: one with an infinity or a NaN, with a largest value outside
+ * 2^-40 .. 2^40 (g: 2^-100 .. 2^100, and 2^60 over the row's sum), or with rows (of k, v and, for dk, q) or columns (of v, and of
+ * k, q, g for the gradient that they make) whose largest values, zero ones aside, are further apart than 2^14 (2^18 for the
+ * columns of a single row). So do workgroups where a query's length times a key's times scale passes 709 (2^10 in log2 units): a
+ * score is held to 2^-22 of itself, and the backward's weight to as much of the score; and where a slope times lq + lk passes
+ * 2^22 in log2 units. A scale (or scale / cap) outside 2^-40 .. 2^40 takes the row kernels. Results are the same bits for the
+ * same call. o and stats
  * must not overlap an input or each other. No counterpart in the reference, whose Attention takes an additive mask tensor
  * and equal heads (Ops.Layers.cs:746-807). */
 om_status om_attention_fwd_scored(om_ctx *ctx, const float *q, int ld_q, const float *k, const float *v, int ld_kv,

@@ -2,8 +2,9 @@
 //
 // With E = 2^(x - m) from the saved m, re the exponent of a row's gradient and w = 2^re / l:
 //   D = E (g 2^-re . v - delta 2^-re) (1 - tanh^2),
-//   dv_j = sum_i E_ij (g_i / l_i),  dk_j = scale sum_i D_ij (w_i q_i),  dq_i = scale w_i sum_j D_ij k_j:
-// each operand's rows carry the row's own factor, so that weights of 1 / length and gradients of any size keep their bits in
+//   dv_j = sum_i E_ij 2^ge (g_i 2^-ge / l_i),  dk_j = scale sum_i D_ij 2^ge (q_i 2^(re - ge) / l_i),  dq_i = scale w_i sum_j D_ij k_j,
+// ge the exponent of g_i / l_i: an operand's row carries the row's factor up to a power of two, the weights carry that in fp32
+// and are split at a running scale of each key's, so that weights of 1 / length and gradients of any size keep their bits in
 // fp16 pairs.
 //
 // Two roles share a launch (their tails fill each other's): a workgroup of 128 keys holds K and V fragments and walks the rows
@@ -228,7 +229,7 @@ __device__ __forceinline__ void put4(float *to, int c, int d, floatx4 v, int acc
 // ---------------------------------------------------------------------------------------------------- dk and dv
 // Either role's tables in LDS, by blocks of the other side: whether the block is visited (documents).
 struct Tables {
-    uint32_t red[8][6];
+    uint32_t red[8][4];
     unsigned char see[kListed];
 };
 template <int DP, int PARTS>
@@ -264,49 +265,41 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
     int r0, r1;  // r1: one past the last
     row_range(u, first, last, pre, r0, r1);
     const int t0 = r0 / kBlock, t1 = r1 <= r0 ? t0 - 1 : (r1 - 1) / kBlock;
-    uint32_t gt = 0, gl = 0xFFFFFFFFu, qt = 0, ql = 0xFFFFFFFFu, qnorm = 0;
+    uint32_t qt = 0, ql = 0xFFFFFFFFu, qnorm = 0;
     RowStats mine = {};  // the thread's first
     for (int rt = t0 + (int)threadIdx.x, n = 0; rt <= t1; rt += 64 * NW, n++) {
         const RowStats r = a.rs[rt0 + rt];
         if (n == 0) mine = r;
         bad = bad || r.bad;
-        gt = max(gt, r.g2_top);
         qt = max(qt, r.q2_top);
         qnorm = max(qnorm, __float_as_uint(r.norm));
-        if (r.g2_top) gl = min(gl, r.g2_top);
         if (r.q2_top) ql = min(ql, r.q2_top);
     }
     if (DOCS && threadIdx.x < kListed && t0 + (int)threadIdx.x <= t1) {
         static_assert(kListed == 256, "a thread's first block is its entry");
         tab.see[threadIdx.x] = mine.doc_hi >= max(kdlo, 0) && mine.doc_lo <= kdhi && (mine.g2_top || mine.q2_top);
     }
-    gt = wave_umax(gt);
     qt = wave_umax(qt);
-    gl = wave_umin(gl);
     ql = wave_umin(ql);
     qnorm = wave_umax(qnorm);
     const uint32_t wave_bad = __any(bad) ? 1 : 0;
     if (lane == 0) {
-        red[w][0] = gt;
-        red[w][1] = qt;
-        red[w][2] = gl;
-        red[w][3] = ql;
-        red[w][4] = wave_bad;
-        red[w][5] = qnorm;
+        red[w][0] = qt;
+        red[w][1] = ql;
+        red[w][2] = wave_bad;
+        red[w][3] = qnorm;
     }
     __syncthreads();
 #pragma unroll
     for (int n = 0; n < NW; n++) {
-        gt = max(gt, red[n][0]);
-        qt = max(qt, red[n][1]);
-        gl = min(gl, red[n][2]);
-        ql = min(ql, red[n][3]);
-        bad = bad || red[n][4];
-        qnorm = max(qnorm, red[n][5]);
+        qt = max(qt, red[n][0]);
+        ql = min(ql, red[n][1]);
+        bad = bad || red[n][2];
+        qnorm = max(qnorm, red[n][3]);
     }
     bad = bad || !scores_fit(u, __uint_as_float(qnorm), larger(k0.norm, k1.norm));
-    // the accumulators move between the blocks' scales: keep the largest move inside fp32
-    bad = bad || (gt && (gt >> 23) - (gl >> 23) > 60) || (qt && (qt >> 23) - (ql >> 23) > 60);
+    // dk's sums move between the blocks' scales: keep the largest move inside fp32
+    bad = bad || (qt && (qt >> 23) - (ql >> 23) > 60);
     auto dest = [&](int n, int jj) -> float * {  // dk (0) or dv (1) of key jj
         if (a.part) return a.part + (((int64_t)split * u.B * u.Hk + item) * u.lk + jj) * 2 * u.d + n * u.d;
         float *base = n ? p.dv : p.dk;
@@ -349,8 +342,8 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
             dk[n][e] = 0.0f;
             dv[n][e] = 0.0f;
         }
-    float g2cur = 1.0f, q2cur = 1.0f;
-    int sd = kNoScale;  // dk's sums are in units of 2^sd
+    float q2cur = 1.0f;
+    int sd = kNoScale, sv = kNoScale;  // dk's sums are in units of 2^sd q2cur, dv's in units of 2^sv
     // The split has every nsplit-th block. They are taken downwards, and from a multiple of `period` blocks on, round the
     // range's ends: workgroups of other keys that run meanwhile then read the same blocks, under a causal rule from the last
     // row on, in a window at the same remainder, and find them in their XCD's L2. (Each from its own first row, a window of
@@ -404,20 +397,31 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
         const float *blk = rec + 32 * kRowBlock;
         bool some = live & band.some(f0, f1), one = true;
         if (DOCS) {
-            const int dlo = __builtin_amdgcn_readfirstlane(__float_as_int(blk[3]));
-            const int dhi = __builtin_amdgcn_readfirstlane(__float_as_int(blk[4]));
+            const int dlo = __builtin_amdgcn_readfirstlane(__float_as_int(blk[2]));
+            const int dhi = __builtin_amdgcn_readfirstlane(__float_as_int(blk[3]));
             some = some & (whi >= 0) & (dhi >= wlo) & (dlo <= whi);
             one = (wlo == whi) & (dlo == dhi) & (dlo == wlo) & (wlo >= 0);
         }
         floatx16 x, dp;
-        const float sq = blk[0], sg2 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(blk[1]))),
-                    sq2 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(blk[2])));
-        auto move = [&](floatx16(&sum)[ND], float &cur, float to) {  // sums to another block's scale
-            if (to == cur) return;
-            const float c = cur / to;
+        const float sq = blk[0], sq2 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(blk[1])));
+        auto move = [&](float to) {  // dk's sums to another block's scale
+            if (to == q2cur) return;
+            const float c = q2cur / to;
 #pragma unroll
-            for (int n = 0; n < ND; n++) sum[n] *= c;
-            cur = to;
+            for (int n = 0; n < ND; n++) dk[n] *= c;
+            q2cur = to;
+        };
+        auto fit = [&](floatx16(&sum)[ND], int &s, float top) {  // sums to a scale that holds `top`, the lane's and its pair's largest
+            const int sn = grown(pair_max(top), s);
+            if (__any(sn != s)) {
+                const int by = s - sn;
+#pragma unroll
+                for (int n = 0; n < ND; n++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) sum[n][e] = ldexp_hw(sum[n][e], by);
+                s = sn;
+            }
+            return pow2(-s);
         };
         // scores as the forward summed them, bit for bit where the operands are
         auto products = [&](floatx16 &out, const char *f, const u32x4 *fh, const u32x4 *fm) {
@@ -428,7 +432,7 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
                 out = mma3_t(*reinterpret_cast<const u32x4 *>(f + (2 * s) * 1024),
                              *reinterpret_cast<const u32x4 *>(f + (2 * s + 1) * 1024), fh[s], fm[s], out);
         };
-        // x from raw products to weights E; `keep(e, w)` gets E (1 - tanh^2)
+        // x from raw products to weights E 2^ge; `keep(e, w)` gets them times 1 - tanh^2
         auto weights = [&](auto keep) {
             const float cs = sq * ks.scale;
             const bool whole = band.all(f0, f1) & one;
@@ -469,16 +473,17 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
                         for (int r = 0; r < 4; r++) y[r] = (reach.has(p4[r]) & (qd[r] == kd)) ? y[r] : -3e38f;
                     }
                 }
+                const floatx4 w4 = *reinterpret_cast<const floatx4 *>(rv + 32 * kRowGrad + 8 * q);
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
                     const int e = 4 * q + r;
-                    const float ex = exp2_hw(y[r]), th = x[e];
+                    const float ex = exp2_hw(y[r]) * w4[r], th = x[e];
                     x[e] = ex;
                     keep(e, CAP ? ex * __builtin_fmaf(-th, th, 1.0f) : ex);
                 }
             }
         };
-        // dp from g . v to D, given E (1 - tanh^2); dk's sums to its scale; what D is multiplied with before it is split
+        // dp from g . v to D 2^ge, given E 2^ge (1 - tanh^2); what D is multiplied with before it is split
         auto gradient = [&](const floatx16 &e1) -> float {
             float top = 0.0f;
 #pragma unroll
@@ -491,17 +496,13 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
                     top = fmaxf(top, __builtin_fabsf(dp[e]));
                 }
             }
-            top = pair_max(top);
-            const int sn = grown(top, sd);
-            if (__any(sn != sd)) {
-                const int by = sd - sn;
+            return fit(dk, sd, top);
+        };
+        auto largest = [&]() {  // of the weights, which are not negative
+            float top = 0.0f;
 #pragma unroll
-                for (int n = 0; n < ND; n++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) dk[n][e] = ldexp_hw(dk[n][e], by);
-                sd = sn;
-            }
-            return pow2(-sd);
+            for (int e = 0; e < 16; e++) top = fmaxf(top, x[e]);
+            return top;
         };
         auto add_half = [&](floatx16(&sum)[ND], const char *f, const floatx16 &v, float by, int s) {  // 16 of the step's rows
             float e8[8];
@@ -517,16 +518,15 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
         };
         if constexpr (NW == 4) {
             if (some) {
-                move(dv, g2cur, sg2);
-                move(dk, q2cur, sq2);
+                move(sq2);
                 products(x, qf, kh, km);
                 products(dp, gf, vh, vm);
                 floatx16 e1;
                 weights([&](int e, float v) { e1[e] = v; });
-                const float fd = gradient(e1);
+                const float fe = fit(dv, sv, largest()), fd = gradient(e1);
 #pragma unroll
                 for (int s = 0; s < 2; s++) {
-                    add_half(dv, g2f, x, 1.0f, s);
+                    add_half(dv, g2f, x, fe, s);
                     add_half(dk, q2f, dp, fd, s);
                 }
             }
@@ -545,11 +545,11 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
             }
             asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
             if (some && w < 4) {
-                move(dk, g2cur, sg2);
+                const float fe = fit(dk, sv, largest());
 #pragma unroll
-                for (int s = 0; s < 2; s++) add_half(dk, g2f, x, 1.0f, s);
+                for (int s = 0; s < 2; s++) add_half(dk, g2f, x, fe, s);
             } else if (some) {
-                move(dk, q2cur, sq2);
+                move(sq2);
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
                     const floatx4 e4 = pass[64 * q];
@@ -565,7 +565,7 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
         buf ^= 1;
     }
     if (j > last) return;
-    const float fv = g2cur * pow2(-kLift), fk = q2cur * pow2(-kLift) * u.scale;
+    const float fv = pow2(-kLift), fk = q2cur * pow2(-kLift) * u.scale;
     const bool has_v = NW == 4 || w < 4, has_k = NW == 4 || w >= 4;
     float *tk = has_k ? dest(0, j) : nullptr, *tv = has_v ? dest(1, j) : nullptr;
 #pragma unroll
@@ -573,16 +573,21 @@ __device__ __forceinline__ void keys_role(const Rule &u, const Ptrs &p, const Bw
 #pragma unroll
         for (int q = 0; q < 4; q++) {
             const int c = 32 * n + 8 * q + 4 * g;
-            const floatx16 &sv = dv[n];
+            const floatx16 &dvn = dv[n];
             const floatx4 xk = floatx4{dk[n][4 * q], dk[n][4 * q + 1], dk[n][4 * q + 2], dk[n][4 * q + 3]};
-            const floatx4 xv = NW == 4 ? floatx4{sv[4 * q], sv[4 * q + 1], sv[4 * q + 2], sv[4 * q + 3]} : xk;
+            const floatx4 xv = NW == 4 ? floatx4{dvn[4 * q], dvn[4 * q + 1], dvn[4 * q + 2], dvn[4 * q + 3]} : xk;
             if (tk) {
                 floatx4 y;
 #pragma unroll
                 for (int e = 0; e < 4; e++) y[e] = ldexp_hw(xk[e], sd) * fk;
                 put4(tk, c, u.d, y, acc);
             }
-            if (tv) put4(tv, c, u.d, xv * fv, acc);
+            if (tv) {
+                floatx4 y;
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = ldexp_hw(xv[e], sv) * fv;
+                put4(tv, c, u.d, y, acc);
+            }
         }
 }
 

@@ -279,29 +279,33 @@ enum {
     kRowPos,    // position (int)
     kRowSlope,  // slope of its head, in log2 units
     kRowDoc,    // document (int)
-    kRowW,      // 2^re / l: what the row's sums are multiplied with at the end; 0 for a row without gradient
-    kRowBlock,  // of the rows' block of 64: its scales of q, g / l and q w, its documents' range
+    kRowW,      // 2^re / l: what dq's sums are multiplied with at the end; 0 for a row without gradient
+    kRowBlock,  // of the rows' block of 64: its scales of q and q f, its documents' range
+    kRowGrad,   // 2^ge, ge the exponent of the row's g / l: what its weights are multiplied with for dk and dv; 0 without gradient
     kRowValues = 8
 };
 __host__ __device__ __forceinline__ int64_t row_value(int64_t row, int which) { return (row >> 5) * (32 * kRowValues) + which * 32 + (row & 31); }
-// A block of 64 rows. Either role needs the rows' values and the rows form; only dk and dv the columns form, whose rows may be
-// further apart by their gradients and sums, and whose columns have to be near each other.
+// A block of 64 rows. Either role needs the rows' values and the rows form; only dk and dv the columns form, where q's rows and
+// the columns have to be near each other. g's rows need not: each is scaled by itself there too. (At one scale a block, one row
+// in ten peaked and gradients spread as exp of a normal sent most calls to plain sums: 30 ms where 0.5 are taken, 4096 causal rows.)
 enum { kBadRows = 1, kBadColumns = 2 };
 struct RowStats {
-    float q, g2, q2;       // scales 2^e of q, of g / l and of q w
-    uint32_t g2_top, q2_top;  // largest magnitudes (bits) of the latter two
+    float q, q2;              // scales 2^e of q and of q f
+    uint32_t g2_top, q2_top;  // largest magnitudes (bits) of g 2^-ge / l and q f
     uint32_t bad;          // what the split cannot hold of the block: kBadRows, kBadColumns
     int32_t doc_lo, doc_hi;
     float norm;            // largest sum of the squares of a row of q
 };
 struct RowsOut {
     char *q, *g;    // rows form: q by one scale per block, g by one per row
-    char *g2, *q2;  // columns form: g / l (for dv) and q w (for dk)
+    char *g2, *q2;  // columns form: g / l (for dv) by one scale per row, q f (for dk) by one per block, f = 2^(re - ge) / l, 1/2 .. 2
     float *v;       // row_value
     RowStats *stats;
 };
-constexpr uint32_t kWideMost = (127u + 100) << 23, kWideLeast = (127u - 100) << 23;
+constexpr uint32_t kWideMost = (127u + 100) << 23, kWideLeast = (127u - 100) << 23, kGradMost = (127u + 60) << 23;
 constexpr float kNoRow = 3e38f;
+// The exponent e of a row's own scale 2^-e, which brings its largest magnitude to 2^14 .. 2^15.
+__device__ __forceinline__ int row_exp(uint32_t top) { return (int)(top >> 23) - 127 - 14; }
 constexpr int kLift = 12;  // weights are kept as 2^kLift times themselves, so that their split's second half is normal fp16
 
 // Block t of the rows of (b, hk) for the backward.
@@ -312,7 +316,7 @@ __device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, 
     const int rows = u.G * u.lq;
     const int64_t all = (int64_t)u.B * u.Hk * rows;
     Share<DP> s, g, ov;
-    float rl[4], w[4], delta[4], m[4], slope[4];
+    float rl[4], f[4], gd[4], delta[4], m[4], slope[4];
     uint32_t qt[4], gt[4];
     float norm = 0.0f;
     int dlo = INT32_MAX, dhi = INT32_MIN, doc[4];
@@ -353,9 +357,16 @@ __device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, 
         norm = larger(norm, s.row_norm(i));
         gt[i] = g.row_top(i);
         const bool fine = gt[i] == 0 || (gt[i] >= kWideLeast && gt[i] <= kWideMost);
-        const int re = fine && gt[i] ? scale_exp(gt[i]) : 0;
+        const int re = fine && gt[i] ? row_exp(gt[i]) : 0;
+        // weights take g / l's size, at most 2^60, so that their products with a row's g . v, below 2^63, stay fp32 numbers
+        const uint32_t lt = __float_as_uint(__uint_as_float(gt[i]) * rl[i]);
+        const bool gives = gt[i] && fine && lt >= kWideLeast && lt <= kGradMost;
+        const int ge = gives ? row_exp(lt) : 0;
+        bad_columns = bad_columns || (gt[i] && !gives);
         // a row that gives nothing, and one that the split cannot hold, keep finite stand-ins
-        w[i] = gt[i] && fine ? rl[i] * pow2(re) : 0.0f;
+        const float w = gt[i] && fine ? rl[i] * pow2(re) : 0.0f;
+        f[i] = gives ? rl[i] * pow2(re - ge) : 0.0f;
+        gd[i] = gives ? pow2(-ge) : 0.0f;
         delta[i] = fine ? dot * pow2(-re) : 0.0f;
         bad = bad || !fine || (on && !bias_fits(u, slope[i])) || (on && !(__builtin_fabsf(m[i]) < 1e30f && rl[i] > 0.0f && rl[i] < 1e30f && __builtin_fabsf(dot) < 1e38f));
         m[i] = on ? (float)kLift - m[i] : -kNoRow;
@@ -366,7 +377,8 @@ __device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, 
             o.v[row_value(r, kRowPos)] = __int_as_float(row.t + u.off);
             o.v[row_value(r, kRowSlope)] = on ? slope[i] : 0.0f;
             o.v[row_value(r, kRowDoc)] = __int_as_float(doc[i]);
-            o.v[row_value(r, kRowW)] = w[i];
+            o.v[row_value(r, kRowW)] = w;
+            o.v[row_value(r, kRowGrad)] = gives ? pow2(ge) : 0.0f;
         }
     }
     RowStats st = {};
@@ -388,31 +400,38 @@ __device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, 
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         const bool fine = gt[i] >= kWideLeast && gt[i] <= kWideMost;
-        const float sc = fine ? pow2(-scale_exp(gt[i])) : 0.0f;
+        const float sc = fine ? pow2(-row_exp(gt[i])) : 0.0f;
 #pragma unroll
         for (int n = 0; n < NCH; n++) x.x[i][n] = g.x[i][n] * sc;
     }
     put_block<DP, false>(x, o.g + at * plane_bytes(DP, 1), lds);
-    // g / l and q w, one scale each
+    // g / l, a scale for each row: their columns are looked at as they are scaled
     uint32_t t4[4];
-    auto cols = [&](Share<DP> &y, const float (&f)[4], char *out, float &scale, uint32_t &kept) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            y.scale(i, f[i]);
-            t4[i] = y.row_top(i);
-        }
-        const BlockTop bt = block_top<DP, true>(y, t4, 0.0f, sh, lds);
-        const bool ok = bt.top == 0 || (bt.top >= kWideLeast && bt.top <= kWideMost && even_rows(bt.top, bt.low) && even_columns(bt));
-        bad_columns = bad_columns || !ok;
-        const int e = ok && bt.top ? scale_exp(bt.top) : 0;
-        scale = pow2(e);
-        kept = bt.top;
+    for (int i = 0; i < 4; i++) {
+        g.scale(i, rl[i]);
+        g.scale(i, gd[i]);
+        t4[i] = g.row_top(i);
+    }
+    const BlockTop gb = block_top<DP, true>(g, t4, 0.0f, sh, lds);
+    bad_columns = bad_columns || !even_columns(gb);
+    st.g2_top = gb.top;
+    put_block<DP, true>(g, o.g2 + at * plane_bytes(DP, 1), lds);
+    // q f, one scale
 #pragma unroll
-        for (int i = 0; i < 4; i++) y.scale(i, pow2(-e));
-        put_block<DP, true>(y, out + at * plane_bytes(DP, 1), lds);
-    };
-    cols(g, rl, o.g2, st.g2, st.g2_top);
-    cols(s, w, o.q2, st.q2, st.q2_top);
+    for (int i = 0; i < 4; i++) {
+        s.scale(i, f[i]);
+        t4[i] = s.row_top(i);
+    }
+    const BlockTop fb = block_top<DP, true>(s, t4, 0.0f, sh, lds);
+    const bool fok = fb.top == 0 || (fb.top >= kWideLeast && fb.top <= kWideMost && even_rows(fb.top, fb.low) && even_columns(fb));
+    bad_columns = bad_columns || !fok;
+    const int ef = fok && fb.top ? scale_exp(fb.top) : 0;
+    st.q2 = pow2(ef);
+    st.q2_top = fb.top;
+#pragma unroll
+    for (int i = 0; i < 4; i++) s.scale(i, pow2(-ef));
+    put_block<DP, true>(s, o.q2 + at * plane_bytes(DP, 1), lds);
     __syncthreads();
     const uint32_t wave_bad = (__any(bad) ? kBadRows : 0) | (__any(bad_columns) ? kBadColumns : 0);
     if ((threadIdx.x & 15) == 0) {
@@ -433,10 +452,9 @@ __device__ __forceinline__ void split_rows(const Rule &u, const Ptrs &p, int b, 
         for (int half = 0; half < 2; half++) {
             float *to = o.v + row_value(at * kBlock + 32 * half, kRowBlock);
             to[0] = st.q;
-            to[1] = st.g2;
-            to[2] = st.q2;
-            to[3] = __int_as_float(dlo);
-            to[4] = __int_as_float(dhi);
+            to[1] = st.q2;
+            to[2] = __int_as_float(dlo);
+            to[3] = __int_as_float(dhi);
         }
     }
 }

@@ -144,3 +144,31 @@ def test_distance_bias_where_only_far_keys_are_seen(dev, s, slopes):
     near(dv, want[3], what="dv")
     near(dq, want[1], what="dq", floor=c.floor()[0])
     near(dk, want[2], what="dk", floor=c.floor()[1])
+
+
+@pytest.mark.parametrize("s", [(1, 4, 2, 200, 200, 64), (1, 4, 4, 260, 260, 32), (1, 8, 2, 140, 140, 96), (1, 4, 2, 300, 300, 128)], ids=str)
+@pytest.mark.parametrize("by", [16, 40, -40])
+def test_gradients_of_one_document_leave_the_others_bits(dev, s, by):
+    """Rows of one document with gradients 2^by times as large: dk and dv of its keys scale by it, the other document's keep their
+    bits, though rows of both share blocks."""
+    ids = (np.arange(s[3])[None] >= 100).astype(np.int32)
+    a, b = (Case(dev, *s, causal=1, cap=12.0, seed=49, qdoc=ids, kdoc=ids) for _ in range(2))
+    b.g[:, :100] = np.ldexp(b.g[:, :100], by)
+    a.forward(), b.forward()
+    for x, y in zip(a.backward(), b.backward()):
+        assert np.array_equal(y[:, 100:], x[:, 100:])
+        assert np.array_equal(y[:, :100], np.ldexp(x[:, :100], by))
+
+
+@pytest.mark.parametrize("s", [(1, 4, 2, 400, 400, 64), (1, 4, 4, 260, 300, 32), (1, 8, 2, 333, 333, 96), (1, 4, 2, 300, 300, 128)], ids=str)
+@pytest.mark.parametrize("width", [1.0, 3.0, 8.0])
+def test_peaked_and_flat_rows_with_gradients_of_many_sizes(dev, s, width):
+    """One row in ten peaked (its sum near one), the others flat, gradients log-normal over the rows."""
+    c = Case(dev, *s, causal=1, seed=50)
+    r = np.random.default_rng(50)
+    c.q *= np.where(r.random((s[0], s[3], 1, 1)) < 0.1, 6.0, 0.2).astype(np.float32)
+    c.g *= np.exp(width * r.normal(size=(s[0], s[3], 1, 1))).astype(np.float32)
+    want = c.reference()
+    near(c.forward(), want[0], what="o")
+    for g, w, n, f in zip(c.backward(), want[1:], ("dq", "dk", "dv"), (2 * c.floor()[0], 0.0, 0.0)):
+        near(g, w, what=n, floor=f)
