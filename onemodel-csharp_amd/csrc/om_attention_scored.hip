@@ -470,7 +470,7 @@ om_status fwd_by_rows(om_ctx *ctx, const Rule &u, const Ptrs &p) {
             if (ns < 1) ns = 1;
             const int per = (int)((u.lk + ns - 1) / ns);
             if (per > 0) ns = (u.lk + per - 1) / per;
-            if (wgs * ns > INT32_MAX) {
+            if (wgs * ns > most_groups(256)) {
                 status = om::fail(ctx, OM_E_ARG, "om_attention_fwd_scored: too many row blocks");
                 return;
             }
@@ -502,7 +502,7 @@ om_status bwd_by_rows(om_ctx *ctx, const Rule &u, const Ptrs &p) {
         const int64_t rows = (int64_t)u.G * u.lq, nq = p.dq ? (rows + R - 1) / R : 0;
         const int64_t nk = p.dk || p.dv ? (u.lk + R - 1) / R : 0, wgs = (nq + nk) * u.B * u.Hk;
         if (wgs == 0) return;
-        if (wgs > INT32_MAX) {
+        if (wgs > most_groups(256)) {
             status = om::fail(ctx, OM_E_ARG, "om_attention_bwd_scored: too many row blocks");
             return;
         }

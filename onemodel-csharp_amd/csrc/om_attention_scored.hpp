@@ -146,6 +146,9 @@ __device__ __forceinline__ floatx4 load4(const float *row, int c, int d) {
     }
 }
 
+// Workgroups of `threads` that one launch takes: the runtime counts its threads in 32 bits.
+constexpr int64_t most_groups(int threads) { return (int64_t)UINT32_MAX / threads; }
+
 // Everything the kernels read and write besides the rule.
 struct Ptrs {
     const float *q, *k, *v, *o, *g;

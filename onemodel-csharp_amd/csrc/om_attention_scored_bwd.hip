@@ -941,7 +941,7 @@ om_status bwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p) {
     a.qsplit = (int)qs;
     wr = p.dq ? wr * a.qsplit : 0;
     const int64_t jobs = items * (2 * (int64_t)a.nt + a.nr);
-    OM_REQUIRE(ctx, wk + wr <= INT32_MAX - 64 && jobs <= INT32_MAX, "%s: too many row blocks", what);
+    OM_REQUIRE(ctx, wk + wr + 64 <= most_groups(64 * waves_of(dp)) && jobs <= most_groups(256), "%s: too many row blocks", what);
     a.keys_wgs = (int)wk;
     a.rows_wgs = (int)wr;
     // a window's whole range: of rows that see a workgroup's keys, in blocks a split; of keys that its rows see, in steps

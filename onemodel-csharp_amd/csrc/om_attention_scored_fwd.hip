@@ -480,7 +480,7 @@ om_status fwd_by_matrix(om_ctx *ctx, const Rule &u, const Ptrs &p, int *joins, f
     const int64_t items = (int64_t)u.B * u.Hk, wgs = items * blocks, all = items * rows;
     const int dp = u.d <= 32 ? 32 : u.d <= 64 ? 64 : u.d <= 96 ? 96 : 128;
     const int64_t ns = pieces(ctx, u, dp, wgs, all);
-    OM_REQUIRE(ctx, wgs * ns <= INT32_MAX && 2 * items * nt <= INT32_MAX, "om_attention_fwd_scored: too many row blocks");
+    OM_REQUIRE(ctx, wgs * ns <= most_groups(256) && 2 * items * nt <= most_groups(256), "om_attention_fwd_scored: too many row blocks");
     const int64_t plane = plane_bytes(dp, items * nt), stats = items * nt * (int64_t)sizeof(Stats);
     const int64_t words = 2 * items * nt * kKeyWords * (int64_t)sizeof(float);
     const int64_t join = ns > 1 ? (int64_t)sizeof(float) * ns * all * (u.d + 2) : 0;
