@@ -490,8 +490,9 @@ om_status om_rope_bwd(om_ctx *ctx, const float *g, int ld_g, const int32_t *pos,
  *   j <= i with causal, and |i - j| < window with window > 0; both waived for j < prefix[b] (prefix given);
  *   q_doc[b][t] == k_doc[b][j] >= 0 with documents (both or neither; a negative id is padding, which sees nothing and
  *   is seen by nothing).
- * A query that sees nothing gives o = 0 and no gradient. What a query does not see has no effect on it, infinities and
- * NaN included; its visible values follow IEEE rules. */
+ * A query that sees nothing gives o = 0 and no gradient. What a query does not see adds nothing to it, infinities and NaN
+ * included; in a block of keys or rows that it shares, its size may decide how visible values are split or that they are summed
+ * plainly (see below), and so the last bits. Visible values follow IEEE rules. */
 typedef struct {
     int32_t heads, kv_heads;
     float scale;          /* 0 or NaN: 1 / sqrt(d) */

@@ -5,9 +5,12 @@
 // or 2^-36 of the block's largest value where m is subnormal); a product keeps hh, hm, mh. The dropped terms are together
 // about 2^-23 of |x||y|, so a sum of products keeps fp32's accuracy, at a third of the fp16 matrix rate (840 TFLOP/s
 // where v_mfma_f32_16x16x4_f32 has 157 and the six-term bf16 split of om_split.hpp 419), and a split takes two vector
-// operations a value where the bf16 one takes six. What fp16's range does not hold is found beforehand (Stats): a block
-// with an infinity, a NaN or a magnitude outside 2^-40 .. 2^40, or rows whose largest values are more than 2^14 apart.
-// A workgroup that would use such a block computes its rows by plain fp32 sums instead (om_attention_scored.hip).
+// operations a value where the bf16 one takes six. What fp16's range does not hold is found beforehand (Stats, RowStats): a
+// block with an infinity, a NaN or a largest magnitude outside 2^-40 .. 2^40, or rows or columns whose largest values are more
+// than 2^14 apart. A workgroup that would use such a block computes its rows by plain fp32 sums instead (plain_row in
+// om_attention_scored_fwd.hip, plain_dq and plain_dkv in om_attention_scored_bwd.hip), and so does one whose scores may pass
+// kMostScore: a score is held to 2^-22 of itself, so its weight to as much of the score, and past 2^24 the weights' 2^kLift is
+// lost in the rounding of their exponents. Scores are bounded by the longest row's length times the longest key's.
 //
 // Operands lie in scratch in fragment order: v_mfma_f32_32x32x16_f16 takes, from lane l, eight values of row l % 32 at
 // contraction indices of group g = l / 32, and a fragment of 64 lanes x 16 bytes is 1 KB of consecutive memory, so
@@ -42,9 +45,7 @@ struct Stats {
 };
 // What a step of 32 keys carries along with its operands, staged with them: 64 words.
 enum { kKeyDoc = 0, kKeyScaleK = 32, kKeyScaleV, kKeyDocLo, kKeyDocHi, kKeyWords = 64 };
-constexpr uint32_t kInfBits = 0x7F800000u;
 constexpr uint32_t kMostBits = (127u + 40) << 23, kLeastBits = (127u - 40) << 23;  // 2^40, 2^-40
-
 constexpr float kMostScore = 1024.0f;  // in log2 units
 
 __device__ __forceinline__ float pow2(int e) { return __int_as_float((e + 127) << 23); }
