@@ -492,7 +492,8 @@ om_status om_rope_bwd(om_ctx *ctx, const float *g, int ld_g, const int32_t *pos,
  *   is seen by nothing).
  * A query that sees nothing gives o = 0 and no gradient. What a query does not see adds nothing to it, infinities and NaN
  * included; in a block of keys or rows that it shares, its size may decide how visible values are split or that they are summed
- * plainly (see below), and so the last bits. Visible values follow IEEE rules. */
+ * plainly (see below), and so the last bits. Visible values follow IEEE rules, but that a query whose visible scores are all
+ * minus infinity counts as one that sees nothing. */
 typedef struct {
     int32_t heads, kv_heads;
     float scale;          /* 0 or NaN: 1 / sqrt(d) */
