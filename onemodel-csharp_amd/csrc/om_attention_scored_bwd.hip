@@ -13,8 +13,9 @@
 // operand. Recomputing the scores for the second role costs two products of seven; partial dq from the first role would
 // cost rows * keys / 32 values of traffic, more than that from about 2000 keys on, and atomics would lose the fixed order.
 //
-// Bound: as the forward. 12 heads of 64 values in 4 key heads, 4096 causal rows with a cap: 365 us (matrix unit busy 40 % of the
-// time, vector unit 58 %); 16 heads of 128 in 4, 8192 rows in a window of 1024: 1150 us (32 %, 27 %, one wavefront a SIMD).
+// Bound: as the forward. 12 heads of 64 values in 4 key heads, 4096 causal rows with a cap: 350 to 415 us over several runs, 382
+// in the middle (matrix unit busy 40 % of the time, vector unit 62 %); 16 heads of 128 in 4, 8192 rows in a window of 1024: 1080
+// to 1225 us (30 %, 33 %, one wavefront a SIMD).
 #include <algorithm>
 
 #include "om_attention_scored_split.hpp"
@@ -28,7 +29,7 @@ constexpr int kKeys = 128;   // keys of a workgroup of the first role
 // both and the fragments of K and V take more than half a SIMD's registers, and one wavefront a SIMD is left. Up to 96, eight
 // share the stages instead: four hold K and dv and form the scores and the weights, four hold V and dk of the same keys, form
 // g . v meanwhile, and take the weights over through LDS (777 rows of 80 values, prefix: 108 -> 95 us). At 128 that spills
-// registers and is no faster than four (8192 rows in a window of 1024: 1157 us against 1152).
+// registers and is no faster than four (8192 rows in a window of 1024, timed side by side: 1157 us against 1152).
 constexpr int waves_of(int dp) { return dp == 96 ? 8 : 4; }
 constexpr int kStep = 32;    // rows (or keys) of a step
 constexpr int kListed = 256; // blocks whose step data stands in LDS

@@ -8,7 +8,8 @@
 //
 // Bound: a wavefront's matrix instructions and its vector work (exponents, caps, masks, splits) follow each other, so a SIMD
 // runs one of them only while another wavefront is in the other; 12 heads of 64 values in 4 key heads, 4096 causal rows with
-// a cap: 113 us and 14 us for the joins, 228 TFLOP/s of fp32 products where three fp16 products for each reach about 380.
+// a cap: 107 to 123 us over several runs and 14 us for the joins, 210 to 240 TFLOP/s of fp32 products where three fp16 products
+// for each reach about 380.
 #include <algorithm>
 #include <cmath>
 
