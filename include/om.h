@@ -512,7 +512,7 @@ typedef struct {
  * largest value in its block of 64 rows (in its row of g, and of q in the forward). Workgroups that would use a block which
  * pairs do not hold take plain fp32 sums, tens of times slower: one with an infinity or a NaN, with a largest value outside
  * 2^-40 .. 2^40 (g: 2^-100 .. 2^100, and 2^60 over the row's sum), or with rows (of k, v and, for dk, q) or columns (of v, and of
- * k, q, g for the gradient that they make) whose largest values, zero ones aside, are further apart than 2^14 (2^18 for the
+ * k, q, g for the gradient that they make) whose largest values, zero ones aside, are further apart than 2^14 (2^22 for the
  * columns of a single row). So do workgroups where a query's length times a key's times scale passes 709 (2^10 in log2 units): a
  * score is held to 2^-22 of itself, and the backward's weight to as much of the score; and where a slope times lq + lk passes
  * 2^22 in log2 units. A scale (or scale / cap) outside 2^-40 .. 2^40 takes the row kernels. Results are the same bits for the

@@ -151,10 +151,10 @@ __device__ __forceinline__ BlockTop block_top(const Share<DP> &s, const uint32_t
     return r;
 }
 // Whether every column that is not zero keeps its bits: its largest value within 2^14 of the block's, so held to 2^-22 of
-// itself. In a single row each column is one value, and one in 8000 of a normal's is 2^14 below the largest: there 2^18,
-// held to 2^-18.
+// itself. In a single row, as a last block may hold, each column is one value, and of a normal's one in 8000 is 2^14 below the
+// largest, one in 2 million 2^22: there 2^22 is asked for, or every few calls would have a head that sums plainly for nothing.
 __device__ __forceinline__ bool even_columns(const BlockTop &b) {
-    return b.top == 0 || (b.top >> 23) - (b.column >> 23) <= (b.rows > 1 ? 14 : 18);
+    return b.top == 0 || (b.top >> 23) - (b.column >> 23) <= (b.rows > 1 ? 14 : 22);
 }
 __device__ __forceinline__ float larger(float a, float b) {  // of sums of squares; a NaN is the largest
     return __uint_as_float(max(__float_as_uint(a), __float_as_uint(b)));
