@@ -369,6 +369,47 @@ om_status om_layernorm_bwd_partials(om_ctx *ctx, const float *g, const float *x,
                                     const float *rstd, const float *dx_add, float *dx, int acc_dx, double *part_g,
                                     double *part_b, int rows, int cols);
 
+/* ---------------------------------------------------------------------------------------------- 8-bit tensors */
+/* Activations kept for the backward pass in a quarter of their memory, and products of tensors held that way (no
+ * counterpart in the reference, whose tape keeps fp32). A packed tensor of [rows, cols] holds, for each block of 128
+ * neighbouring values of a row, 8-bit floats (OCP e4m3) and one power of two: with e the least exponent from -127 on that
+ * brings the block's largest finite |x| / 2^e to 448 or below, a code is x / 2^e rounded to nearest, ties to even (a relative
+ * error of at most 2^-4, or 2^-10 2^e below 2^-6 2^e); infinities and NaN become NaN and leave the others alone.
+ * Layout: `rows` rows of codes of S = 128 ceil(cols / 128) bytes, zeros behind the last column, then `rows` rows of scale
+ * bytes e + 127 of T = 4 ceil(S / 512) bytes, zeros behind the last block; om_pack8_bytes gives rows * (S + T), 0 where rows
+ * or cols is not positive. Packed tensors start at multiples of 16 bytes (om_alloc's do). A block is 128 wide whatever cols
+ * is, so a narrow tensor is best viewed as a wide one first.
+ * Where an entry point says x8 its rows are packed; xt8 is the packed transpose, [cols, rows], whose blocks run along the
+ * rows of x: a product takes each operand packed along the dimension it sums over. */
+uint64_t om_pack8_bytes(int rows, int cols);
+/* x8 = x packed and xt8 = x^T packed, from one pass over x (rows of ld_x >= cols floats); either may be NULL, not both. */
+om_status om_pack8(om_ctx *ctx, const float *x, int ld_x, int rows, int cols, uint8_t *x8, uint8_t *xt8);
+/* y[r][c] (+)= the packed value (rows of ld_y >= cols floats; what stands behind a row's cols values is left alone). */
+om_status om_unpack8(om_ctx *ctx, const uint8_t *x8, float *y, int ld_y, int rows, int cols, int acc);
+/* c[m,n] (+)= a b^T (+ bias[n]) with a8 = [m, k] and b8 = [n, k] packed; bias may be NULL, c has rows of ldc >= n floats.
+ * Every product of two values is exact and sums are fp32 (on the bf16 matrix cores, which hold an 8-bit value as it is; the
+ * 8-bit instructions round their sums to about 14 bits). Values below 2^-126, which only blocks whose largest value is below
+ * 2^-109 hold, may count as zero. A Linear with all three products in 8 bits: y = om_gemm8(rows, out, in, x8, w8, b),
+ * dx = om_gemm8(rows, in, out, g8, wt8), dw = om_gemm8(out, in, rows, gt8, xt8), db = om_colsum(g). */
+om_status om_gemm8(om_ctx *ctx, int m, int n, int k, const uint8_t *a8, const uint8_t *b8, const float *bias, float *c,
+                   int ldc, int acc);
+/* om_linear_bwd with the layer's input kept as xt8, the packed transpose of x [rows, in]: dw (+)= g^T x (every product
+ * exact, sums fp32) and db (+)= fp64 column sums of g; dx (+)= g w is om_linear_bwd's. Each output may be NULL. */
+om_status om_linear_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *xt8, const float *w, float *dx, float *dw, float *db,
+                           int rows, int in, int out, int acc_dx, int acc_dw, int acc_db);
+/* om_gelu_fwd over [rows, cols] that keeps its input packed, and its backward from that: dx (+)= g * gelu'(value of x8).
+ * Both follow om_ctx_set_gelu; y may be x, dx may be g. */
+om_status om_gelu_fwd_x8(om_ctx *ctx, const float *x, float *y, uint8_t *x8, int rows, int cols);
+om_status om_gelu_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *x8, float *dx, int rows, int cols, int acc);
+/* LayerNorm that keeps its normalised rows packed: mean and 1 / sigma are formed in double and rounded to float once each
+ * (om_layernorm_fwd: float sums), xh = (x - mean) * rstd and y = xh * gamma + beta with one rounding an operation, and xh8
+ * is xh packed. The backward needs xh8 and rstd alone: with h the value of xh8 and q = g gamma, dx (+)= rstd (q - mean(q) -
+ * h mean(q h)), dgamma (+)= fp64 column sums of g h, dbeta (+)= those of g; each may be NULL. y may be x, dx may be g. */
+om_status om_layernorm_fwd_x8(om_ctx *ctx, const float *x, const float *gamma, const float *beta, float *y, uint8_t *xh8,
+                              float *rstd, int rows, int cols, float eps);
+om_status om_layernorm_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *xh8, const float *gamma, const float *rstd,
+                              float *dx, float *dgamma, float *dbeta, int rows, int cols, int acc_dx, int acc_params);
+
 /* ---------------------------------------------------------------------------------------------- softmax family */
 /* Softmax.Rows (Softmax.cs:27-133) and its backward (BackwardNn.cs:26-52). */
 om_status om_softmax_fwd(om_ctx *ctx, const float *x, float *y, int rows, int cols);

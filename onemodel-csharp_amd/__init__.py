@@ -92,6 +92,15 @@ _OM_SIGS = {
     "om_layernorm_bwd_add": [vp, vp, vp, vp, vp, vp, vp, vp, vp, vp, ci, ci, ci],
     "om_layernorm_bwd_chunks": [ci, ci],
     "om_layernorm_bwd_partials": [vp, vp, vp, vp, vp, vp, vp, vp, ci, vp, vp, ci, ci],
+    "om_pack8_bytes": [ci, ci],
+    "om_pack8": [vp, vp, ci, ci, ci, vp, vp],
+    "om_unpack8": [vp, vp, vp, ci, ci, ci, ci],
+    "om_gemm8": [vp, ci, ci, ci, vp, vp, vp, vp, ci, ci],
+    "om_linear_bwd_x8": [vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci, ci, ci],
+    "om_gelu_fwd_x8": [vp, vp, vp, vp, ci, ci],
+    "om_gelu_bwd_x8": [vp, vp, vp, vp, ci, ci, ci],
+    "om_layernorm_fwd_x8": [vp, vp, vp, vp, vp, vp, vp, ci, ci, f32],
+    "om_layernorm_bwd_x8": [vp, vp, vp, vp, vp, vp, vp, vp, ci, ci, ci, ci],
     "om_softmax_fwd": [vp, vp, vp, ci, ci],
     "om_softmax_bwd": [vp, vp, vp, vp, ci, ci, ci],
     "om_logsoftmax_fwd": [vp, vp, vp, ci, ci],
@@ -158,6 +167,7 @@ _RESTYPE = {"om_last_error": C.c_char_p, "om_ctx_stream": vp, "om_abi_version": 
             "om_adam_scalars": None,
             "om_ctc_tables_bytes": u64,
             "om_linear_small": ci,
+            "om_pack8_bytes": u64,
             "om_layernorm_bwd_chunks": ci,
             "om_stager_slot_bytes": u64}
 

@@ -1,0 +1,359 @@
+// LayerNorm that keeps its normalised rows in 8 bits (om_pack8.hpp has the format), forward and backward.
+//
+// Forward: mean and variance in 64 bits and rounded once each, so that the rows kept, xh = fl(fl(x - mean) * rstd), have bits
+// of their own whatever order a row was summed in; y = xh gamma + beta, xh8 = pack(xh). Kept are the normalised rows and not
+// x: a code is off by 2^-4 of its value, which of x would be 2^-4 of its mean as well. Backward, with h the value of xh8 and
+// q = g gamma: dx = rstd (q - mean(q) - h mean(q h)), dgamma = sum of g h, dbeta = sum of g.
+//
+// Bound: HBM, 9 bytes a value each way (x or g 4, the packed rows 1, y or dx 4). A row is read once and stays in registers:
+// one wavefront to a row of up to 1024, a workgroup to a longer one, four values a lane at a time, so that 32 lanes hold a
+// block of 128. Rows past 16384 columns (backward: 8192, whose column sums need the registers) are read again for each pass.
+#include "om_pack8.hpp"
+
+#include <type_traits>
+
+namespace {
+
+using namespace om8;
+
+// What NW wavefronts add up together: the totals in every lane, in a fixed order. `sh` holds NW values; the wavefronts meet
+// before it is written, so calls may follow each other.
+template <int NW, class T>
+__device__ __forceinline__ T row_sum(T v, T *sh) {
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    if constexpr (NW == 1) {
+        return v;
+    } else {
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) sh[threadIdx.x >> 6] = v;
+        __syncthreads();
+        T t = sh[0];
+#pragma unroll
+        for (int i = 1; i < NW; i++) t += sh[i];
+        return t;
+    }
+}
+
+__device__ __forceinline__ void put_codes(const Packed &p, int64_t row, int64_t blk, int64_t col, floatx4 xh) {
+    const int s = scale_byte(max32(finite_bits4(xh)));
+    *reinterpret_cast<uint32_t *>(p.q + row * p.ldq + col) = encode4(xh, inverse_of(s));
+    if ((threadIdx.x & 31) == 0) p.s[row * p.lds + blk] = (uint8_t)s;
+}
+
+// NW wavefronts to a row (4 / NW rows to a workgroup), NV quads of 64 NW lanes. NV = 0: any number, read again for each pass.
+template <int NW, int NV>
+__global__ void __launch_bounds__(256) k_ln8(const float *x, const float *__restrict__ gamma, const float *__restrict__ beta,
+                                             float *y, Packed p, float *__restrict__ rstd, int64_t rows, int64_t cols,
+                                             float eps) {
+    OM_LDS_POISON();
+    __shared__ double sh[4];
+    constexpr int L = 64 * NW, KEEP = NV ? NV : 1;
+    const int64_t row = (int64_t)blockIdx.x * (4 / NW) + (NW == 1 ? threadIdx.x >> 6 : 0);
+    if (row >= rows) return;  // whole rows leave; a row of more than one wavefront is its workgroup's only one
+    const int t = threadIdx.x % L;
+    const float *xr = x + row * cols;
+    const int64_t quads = p.ldq / 4;  // up to the end of the last block
+    const int nv = NV ? NV : (int)((quads + L - 1) / L);
+    floatx4 v[KEEP];
+    auto at = [&](int i) { return 4 * ((int64_t)i * L + t); };
+    auto quad = [&](int i) { return at(i) < cols ? load4(xr + at(i), cols - at(i)) : floatx4{0.0f, 0.0f, 0.0f, 0.0f}; };
+    // f(i, quad i), from registers or read again
+    auto sweep = [&](auto f) {
+        if constexpr (NV) {
+#pragma unroll
+            for (int i = 0; i < NV; i++) f(i, v[i]);
+        } else {
+            for (int i = 0; i < nv; i++) f(i, quad(i));
+        }
+    };
+    if constexpr (NV) {
+#pragma unroll
+        for (int i = 0; i < NV; i++) v[i] = quad(i);
+    }
+    double sum = 0.0;
+    sweep([&](int, floatx4 w) { sum += ((double)w[0] + (double)w[1]) + ((double)w[2] + (double)w[3]); });
+    const double mean = row_sum<NW>(sum, sh) / (double)cols;
+    double ss = 0.0;
+    sweep([&](int i, floatx4 w) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            const double d = (double)w[e] - mean;
+            ss += at(i) + e < cols ? d * d : 0.0;
+        }
+    });
+    const float r = (float)(1.0 / sqrt(row_sum<NW>(ss, sh) / (double)cols + (double)eps)), m = (float)mean;
+    if (t == 0) rstd[row] = r;
+    sweep([&](int i, floatx4 xh) {
+        const int64_t c = at(i);
+        if (c >= p.ldq) return;  // whole blocks of 32 lanes leave together
+#pragma unroll
+        for (int e = 0; e < 4; e++) xh[e] = c + e < cols ? (xh[e] - m) * r : 0.0f;
+        put_codes(p, row, c / 128, c, xh);
+        if (c < cols) {
+            const floatx4 ga = load4(gamma + c, cols - c), be = load4(beta + c, cols - c);
+            floatx4 o;
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e] = xh[e] * ga[e] + be[e];
+            store4(y + row * cols + c, cols - c, o);
+        }
+    });
+    if (const int64_t b = p.ldq / 128; t < p.lds - b) p.s[row * p.lds + b + t] = 0;
+}
+
+// A workgroup takes `chunk` rows, 4 / NW at a time; every lane keeps the fp64 sums of its own columns and leaves them as one
+// partial row of the workgroup's (added over its wavefronts through LDS in order where several share the columns).
+template <int NW, int NV, bool ACC>
+__global__ void __launch_bounds__(256) k_ln8_bwd(const float *g, Packed p, const float *__restrict__ gamma,
+                                                 const float *__restrict__ rstd, float *dx, double *part_g, double *part_b,
+                                                 int64_t rows, int64_t cols, int chunk) {
+    OM_LDS_POISON();
+    __shared__ float sh[4];
+    __shared__ double cs[NW == 1 ? 4 * 256 : 1];
+    constexpr int L = 64 * NW;
+    const int t = threadIdx.x % L, w = threadIdx.x >> 6;
+    const int64_t r0 = (int64_t)blockIdx.x * chunk, r1 = min(rows, r0 + chunk);
+    double sg[4 * NV], sb[4 * NV];
+    floatx4 ga[NV];
+    auto at = [&](int i) { return 4 * ((int64_t)i * L + t); };
+#pragma unroll
+    for (int i = 0; i < NV; i++) {
+        ga[i] = at(i) < cols ? load4(gamma + at(i), cols - at(i)) : floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int e = 0; e < 4; e++) sg[4 * i + e] = sb[4 * i + e] = 0.0;
+    }
+    for (int64_t row = r0 + (NW == 1 ? w : 0); row < r1; row += 4 / NW) {
+        const float *gr = g + row * cols;
+        floatx4 gv[NV], h[NV], old[ACC ? NV : 1];
+        uint32_t q[NV];
+        int s[NV];
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            const int64_t c = at(i);
+            const bool in = c < cols;
+            gv[i] = in ? load4(gr + c, cols - c) : floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+            q[i] = in ? *reinterpret_cast<const uint32_t *>(p.q + row * p.ldq + c) : 0u;
+            s[i] = in ? p.s[row * p.lds + c / 128] : 0;
+            if constexpr (ACC) old[i] = in && dx ? load4(dx + row * cols + c, cols - c) : floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        }
+        float s1 = 0.0f, s2 = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            h[i] = decode4(q[i], scale_of(s[i]));
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                sg[4 * i + e] = __builtin_fma((double)gv[i][e], (double)h[i][e], sg[4 * i + e]);
+                sb[4 * i + e] += (double)gv[i][e];
+                gv[i][e] *= ga[i][e];
+                s1 += gv[i][e];
+                s2 = __builtin_fmaf(gv[i][e], h[i][e], s2);
+            }
+        }
+        if (dx) {
+            const float m1 = row_sum<NW>(s1, sh) / (float)cols, m2 = row_sum<NW>(s2, sh) / (float)cols, r = rstd[row];
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+                const int64_t c = at(i);
+                if (c >= cols) break;
+                floatx4 o;
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    o[e] = r * ((gv[i][e] - m1) - h[i][e] * m2);
+                    if constexpr (ACC) o[e] = old[i][e] + o[e];
+                }
+                store4(dx + row * cols + c, cols - c, o);
+            }
+        }
+    }
+    auto leave = [&](double *part, const double (&sum)[4 * NV]) {
+        if (!part) return;
+#pragma unroll
+        for (int i = 0; i < NV; i++) {
+            if constexpr (NW == 1) {  // the four wavefronts' sums of these 256 columns
+                __syncthreads();
+#pragma unroll
+                for (int e = 0; e < 4; e++) cs[256 * w + 64 * e + t] = sum[4 * i + e];
+                __syncthreads();
+                const int64_t c = 256 * (int64_t)i + 4 * t + w;  // column of lane t's w-th value
+                if (c < cols) part[(int64_t)blockIdx.x * cols + c] =
+                    ((cs[64 * w + t] + cs[256 + 64 * w + t]) + cs[512 + 64 * w + t]) + cs[768 + 64 * w + t];
+            } else {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (at(i) + e < cols) part[(int64_t)blockIdx.x * cols + at(i) + e] = sum[4 * i + e];
+            }
+        }
+    };
+    leave(part_g, sg);
+    leave(part_b, sb);
+}
+
+// dx alone for rows of any length: both passes over the row read it again.
+template <bool ACC>
+__global__ void __launch_bounds__(256) k_ln8_dx_long(const float *g, Packed p, const float *__restrict__ gamma,
+                                                     const float *__restrict__ rstd, float *dx, int64_t cols) {
+    OM_LDS_POISON();
+    __shared__ float sh[4];
+    const int64_t row = blockIdx.x;
+    const float *gr = g + row * cols;
+    auto value = [&](int64_t c) {
+        return decode4(*reinterpret_cast<const uint32_t *>(p.q + row * p.ldq + c), scale_of(p.s[row * p.lds + c / 128]));
+    };
+    auto graded = [&](int64_t c) {
+        floatx4 q = load4(gr + c, cols - c);
+        const floatx4 ga = load4(gamma + c, cols - c);
+#pragma unroll
+        for (int e = 0; e < 4; e++) q[e] *= ga[e];
+        return q;
+    };
+    float s1 = 0.0f, s2 = 0.0f;
+    for (int64_t c = 4 * threadIdx.x; c < cols; c += 1024) {
+        const floatx4 q = graded(c), h = value(c);
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            s1 += q[e];
+            s2 = __builtin_fmaf(q[e], h[e], s2);
+        }
+    }
+    const float m1 = row_sum<4>(s1, sh) / (float)cols, m2 = row_sum<4>(s2, sh) / (float)cols, r = rstd[row];
+    for (int64_t c = 4 * threadIdx.x; c < cols; c += 1024) {
+        const floatx4 q = graded(c), h = value(c);
+        const floatx4 old = ACC ? load4(dx + row * cols + c, cols - c) : floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+        floatx4 o;
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            o[e] = r * ((q[e] - m1) - h[e] * m2);
+            if constexpr (ACC) o[e] = old[e] + o[e];
+        }
+        store4(dx + row * cols + c, cols - c, o);
+    }
+}
+// dgamma's and dbeta's partials of such rows: a workgroup adds `chunk` rows of 1024 columns.
+__global__ void __launch_bounds__(256) k_ln8_params_long(const float *__restrict__ g, Packed p, double *part_g, double *part_b,
+                                                         int64_t rows, int64_t cols, int chunk) {
+    OM_LDS_POISON();
+    const int64_t c = 1024 * (int64_t)blockIdx.y + 4 * threadIdx.x;
+    if (c >= cols) return;
+    double sg[4] = {0.0, 0.0, 0.0, 0.0}, sb[4] = {0.0, 0.0, 0.0, 0.0};
+    const int64_t r1 = min(rows, ((int64_t)blockIdx.x + 1) * chunk);
+    for (int64_t row = (int64_t)blockIdx.x * chunk; row < r1; row++) {
+        const floatx4 gv = load4(g + row * cols + c, cols - c);
+        const floatx4 h =
+            decode4(*reinterpret_cast<const uint32_t *>(p.q + row * p.ldq + c), scale_of(p.s[row * p.lds + c / 128]));
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            sg[e] = __builtin_fma((double)gv[e], (double)h[e], sg[e]);
+            sb[e] += (double)gv[e];
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+        if (c + e < cols) {
+            if (part_g) part_g[(int64_t)blockIdx.x * cols + c + e] = sg[e];
+            if (part_b) part_b[(int64_t)blockIdx.x * cols + c + e] = sb[e];
+        }
+}
+
+// out[c] (+)= the sum of part[k][c] over the chunks: 64 columns to a workgroup, its four wavefronts take every fourth chunk
+// in turn and their sums are added in order.
+__global__ void __launch_bounds__(256) k_ln8_final(const double *__restrict__ part_g, const double *__restrict__ part_b,
+                                                   float *dgamma, float *dbeta, int chunks, int64_t cols, int acc) {
+    OM_LDS_POISON();
+    __shared__ double sh[4][64];
+    const double *part = blockIdx.y ? part_b : part_g;
+    float *out = blockIdx.y ? dbeta : dgamma;
+    const int t = threadIdx.x & 63, w = threadIdx.x >> 6;
+    const int64_t c = 64 * (int64_t)blockIdx.x + t;
+    double s = 0.0;
+    if (out && c < cols)
+#pragma unroll 8
+        for (int k = w; k < chunks; k += 4) s += part[(int64_t)k * cols + c];
+    sh[w][t] = s;
+    __syncthreads();
+    if (w == 0 && out && c < cols) {
+        const float v = (float)(((sh[0][t] + sh[1][t]) + sh[2][t]) + sh[3][t]);
+        out[c] = acc ? out[c] + v : v;
+    }
+}
+
+// Columns of a row that stay in registers: the forward keeps the values alone, the backward sums beside them.
+constexpr int64_t kKeptFwd = 16384, kKeptBwd = 8192;
+template <class F>
+void by_width(int64_t cols, int64_t kept, F f) {
+    if (cols > kept) return f(std::integral_constant<int, 4>(), std::integral_constant<int, 0>());
+#define OM_LN8(NW, NV) \
+    if (cols <= 256 * NW * NV) return f(std::integral_constant<int, NW>(), std::integral_constant<int, NV>());
+    OM_LN8(1, 1) OM_LN8(1, 2) OM_LN8(1, 3) OM_LN8(1, 4) OM_LN8(4, 2) OM_LN8(4, 3) OM_LN8(4, 4) OM_LN8(4, 8) OM_LN8(4, 16)
+#undef OM_LN8
+}
+
+}  // namespace
+
+extern "C" {
+
+om_status om_layernorm_fwd_x8(om_ctx *ctx, const float *x, const float *gamma, const float *beta, float *y, uint8_t *xh8,
+                              float *rstd, int rows, int cols, float eps) {
+    OM_CHECK_CTX(ctx);
+    OM_REQUIRE(ctx, rows >= 0 && cols > 0, "om_layernorm_fwd_x8: rows=%d cols=%d", rows, cols);
+    OM_REQUIRE(ctx, aligned16(xh8), "om_layernorm_fwd_x8: packed tensors start at multiples of 16 bytes");
+    if (rows == 0) return OM_OK;
+    OM_REQUIRE(ctx, x && gamma && beta && y && xh8 && rstd, "om_layernorm_fwd_x8: NULL pointer");
+    if (om_status s = om::use_device(ctx)) return s;
+    const Packed p = packed(xh8, rows, cols);
+    by_width(cols, kKeptFwd, [&](auto nw, auto nv) {
+        constexpr int NW = decltype(nw)::value, NV = decltype(nv)::value;
+        hipLaunchKernelGGL((k_ln8<NW, NV>), dim3((unsigned)(((int64_t)rows * NW + 3) / 4)), dim3(256), 0, ctx->stream, x,
+                           gamma, beta, y, p, rstd, (int64_t)rows, (int64_t)cols, eps);
+    });
+    return OM_LAUNCH_CHECK(ctx, "om_layernorm_fwd_x8");
+}
+
+om_status om_layernorm_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *xh8, const float *gamma, const float *rstd,
+                              float *dx, float *dgamma, float *dbeta, int rows, int cols, int acc_dx, int acc_params) {
+    OM_CHECK_CTX(ctx);
+    OM_REQUIRE(ctx, rows >= 0 && cols > 0, "om_layernorm_bwd_x8: rows=%d cols=%d", rows, cols);
+    OM_REQUIRE(ctx, aligned16(xh8), "om_layernorm_bwd_x8: packed tensors start at multiples of 16 bytes");
+    OM_REQUIRE(ctx, rows == 0 || (g && xh8 && gamma && rstd), "om_layernorm_bwd_x8: NULL pointer");
+    if (!dx && !dgamma && !dbeta) return OM_OK;
+    OM_REQUIRE(ctx, cols <= 1 << 26, "om_layernorm_bwd_x8: cols=%d is more than a launch takes", cols);
+    if (om_status s = om::use_device(ctx)) return s;
+    // chunks of rows: as many as two workgroups a CU, of at least eight rows
+    int chunk = (rows + ctx->num_cus * 2 - 1) / (ctx->num_cus * 2);
+    chunk = chunk < 8 ? 8 : chunk;
+    const int chunks = rows ? (rows + chunk - 1) / chunk : 0;
+    double *pg = nullptr, *pb = nullptr;
+    if (dgamma || dbeta) {
+        float *scr;
+        if (om_status s = om::scratch(ctx, sizeof(double) * 2ull * (uint64_t)chunks * (uint64_t)cols, &scr)) return s;
+        double *base = reinterpret_cast<double *>(scr);
+        pg = dgamma ? base : nullptr;
+        pb = dbeta ? base + (uint64_t)chunks * (uint64_t)cols : nullptr;
+    }
+    const Packed p = packed(xh8, rows, cols);
+    if (rows)
+        by_width(cols, kKeptBwd, [&](auto nw, auto nv) {
+            constexpr int NW = decltype(nw)::value, NV = decltype(nv)::value;
+            if constexpr (NV && 256 * NW * NV <= kKeptBwd) {
+                auto go = [&](auto kern) {
+                    hipLaunchKernelGGL(kern, dim3((unsigned)chunks), dim3(256), 0, ctx->stream, g, p, gamma, rstd, dx, pg, pb,
+                                       (int64_t)rows, (int64_t)cols, chunk);
+                };
+                acc_dx ? go(k_ln8_bwd<NW, NV, true>) : go(k_ln8_bwd<NW, NV, false>);
+            } else if constexpr (!NV) {
+                auto go = [&](auto kern) {
+                    hipLaunchKernelGGL(kern, dim3((unsigned)rows), dim3(256), 0, ctx->stream, g, p, gamma, rstd, dx,
+                                       (int64_t)cols);
+                };
+                if (pg || pb)
+                    hipLaunchKernelGGL(k_ln8_params_long, dim3((unsigned)chunks, (unsigned)((cols + 1023) / 1024)), dim3(256),
+                                       0, ctx->stream, g, p, pg, pb, (int64_t)rows, (int64_t)cols, chunk);
+                if (dx) acc_dx ? go(k_ln8_dx_long<true>) : go(k_ln8_dx_long<false>);  // last: dx may be g
+            }
+        });
+    if (dgamma || dbeta)
+        hipLaunchKernelGGL(k_ln8_final, dim3((unsigned)(((int64_t)cols + 63) / 64), 2), dim3(256), 0, ctx->stream, pg, pb,
+                           dgamma, dbeta, chunks, (int64_t)cols, acc_params);
+    return OM_LAUNCH_CHECK(ctx, "om_layernorm_bwd_x8");
+}
+
+}  // extern "C"

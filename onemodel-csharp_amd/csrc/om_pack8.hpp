@@ -1,0 +1,92 @@
+// Tensors held in 8 bits: the layout of a packed tensor and the conversions, shared by the pack and element kernels
+// (om_pack8.hip), LayerNorm's (om_norm8.hip) and the products' (om_gemm8.hip).
+//
+// A packed tensor of [rows, cols] holds e4m3 codes, rows of stride8(cols) bytes (cols rounded up to 128, zeros behind the last
+// column), and behind them the scale bytes, rows of scales8(cols) bytes (one to a block of 128 columns, rounded up to four,
+// zeros behind the last block). A scale byte s stands for 2^(s - 127); a block takes the least s >= 0 that brings its largest
+// finite value to 448, e4m3's largest, or below. A power of two, so the division is exact and a code is the one rounding
+// (to nearest, ties to even) of its value; infinities and NaN become NaN codes.
+#pragma once
+
+#include "om_internal.hpp"
+
+namespace om8 {
+
+inline int64_t blocks8(int64_t cols) { return (cols + 127) / 128; }
+inline int64_t stride8(int64_t cols) { return blocks8(cols) * 128; }
+inline int64_t scales8(int64_t cols) { return (blocks8(cols) + 3) / 4 * 4; }
+inline uint64_t bytes8(int64_t rows, int64_t cols) { return (uint64_t)rows * (uint64_t)(stride8(cols) + scales8(cols)); }
+
+// A packed tensor's parts.
+struct Packed {
+    uint8_t *q, *s;
+    int64_t ldq, lds;
+};
+inline Packed packed(const uint8_t *p, int64_t rows, int64_t cols) {
+    uint8_t *q = const_cast<uint8_t *>(p);
+    return Packed{q, q ? q + rows * stride8(cols) : nullptr, stride8(cols), scales8(cols)};
+}
+inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
+
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));  // rows of any alignment: the hardware takes 4 bytes
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+// |x| as ordered bits, 0 where x is not finite.
+__device__ __forceinline__ uint32_t finite_bits(float x) {
+    const uint32_t u = __float_as_uint(x) & 0x7FFFFFFFu;
+    return u < 0x7F800000u ? u : 0u;
+}
+__device__ __forceinline__ uint32_t finite_bits4(floatx4 v) {
+    return max(max(finite_bits(v[0]), finite_bits(v[1])), max(finite_bits(v[2]), finite_bits(v[3])));
+}
+// The scale byte of a block from its largest value's bits. 448 = 1.75 * 2^8: the exponent less 8, one more where the
+// significand is above 1.75 (the sum carries), and 0 where that would be negative.
+__device__ __forceinline__ int scale_byte(uint32_t top) { return max((int)((top + 0x1FFFFFu) >> 23) - 8, 0); }
+// 2^(127 - s) and 2^(s - 127); s is at most 247 (top at most 2^128 (1 - 2^-24)).
+__device__ __forceinline__ float inverse_of(int s) { return __uint_as_float((uint32_t)(254 - s) << 23); }
+__device__ __forceinline__ float scale_of(int s) { return __uint_as_float(s ? (uint32_t)s << 23 : 1u << 22); }
+// Four codes. The instruction rounds to nearest even and makes NaN codes of infinities and NaN.
+__device__ __forceinline__ uint32_t encode4(floatx4 v, float inv) {
+    int w = __builtin_amdgcn_cvt_pk_fp8_f32(v[0] * inv, v[1] * inv, 0, false);
+    return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[2] * inv, v[3] * inv, w, true);
+}
+__device__ __forceinline__ floatx4 decode4(uint32_t w, float scale) {
+    const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    return floatx4{a[0] * scale, a[1] * scale, b[0] * scale, b[1] * scale};
+}
+// Largest of 32 neighbouring lanes, in all of them: four steps on the vector pipe inside 16 lanes, one across.
+__device__ __forceinline__ uint32_t max32(uint32_t v) {
+    auto dpp = [](uint32_t x, auto ctrl) {
+        return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xF, 0xF, true);
+    };
+    v = max(v, dpp(v, std::integral_constant<int, 0xB1>()));   // quad_perm [1, 0, 3, 2]
+    v = max(v, dpp(v, std::integral_constant<int, 0x4E>()));   // quad_perm [2, 3, 0, 1]
+    v = max(v, dpp(v, std::integral_constant<int, 0x141>()));  // row_half_mirror
+    v = max(v, dpp(v, std::integral_constant<int, 0x140>()));  // row_mirror
+    return max(v, (uint32_t)__shfl_xor((int)v, 16, 64));
+}
+
+// Four neighbouring values of a row that ends at `left` more values (any number), zeros behind it.
+__device__ __forceinline__ floatx4 load4(const float *p, int64_t left) {
+    if (left >= 4) {
+        const f4u v = *reinterpret_cast<const f4u *>(p);
+        return floatx4{v[0], v[1], v[2], v[3]};
+    }
+    floatx4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int e = 0; e < 3; e++)
+        if (e < left) v[e] = p[e];
+    return v;
+}
+__device__ __forceinline__ void store4(float *p, int64_t left, floatx4 v) {
+    if (left >= 4) {
+        *reinterpret_cast<f4u *>(p) = f4u{v[0], v[1], v[2], v[3]};
+        return;
+    }
+#pragma unroll
+    for (int e = 0; e < 3; e++)
+        if (e < left) p[e] = v[e];
+}
+
+}  // namespace om8
