@@ -10,6 +10,7 @@
 // 16.6 with six conversions to each).
 #include "om_pack8.hpp"
 
+#include <cmath>
 #include <type_traits>
 
 #include "om_split.hpp"
@@ -33,16 +34,25 @@ __device__ __forceinline__ u32x4 widen8(uint32_t w0, uint32_t w1, float scale) {
                  widen2(w1, scale, std::false_type()), widen2(w1, scale, std::true_type())};
 }
 
-// 16 (or 4) bytes a lane from `src` (this lane's address) to LDS at byte address lds + 16 (4) * lane, without registers. m0
-// holds the address for this one instruction only; nothing else in these kernels reads it. land() waits until all of this
-// wavefront's loads have landed and its own LDS reads are done, then meets the others.
-__device__ __forceinline__ void load_to_lds(const void *src, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
+// 16 (or 4) bytes a lane from base (uniform) + off (this lane's) to LDS at byte address lds + 16 (4) * lane, without registers. m0
+// holds the address for this one instruction only; nothing else in these kernels reads it. Loads land in the order of their
+// issue; land<N>() waits until at most this wavefront's last N are in flight and its own LDS reads are done, then meets the
+// others.
+__device__ __forceinline__ void load_to_lds(const void *base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
 }
+__device__ __forceinline__ void load_to_lds4(const void *base, uint32_t off, uint32_t lds) {
+    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
+}
+// The same with an address to each lane.
 __device__ __forceinline__ void load_to_lds4(const void *src, uint32_t lds) {
     asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
 }
-__device__ __forceinline__ void land() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void land() {
+    static_assert(N <= 63, "vmcnt holds at most 63");
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+}
 
 struct Gemm8 {
     Packed a, b;
@@ -75,38 +85,84 @@ __device__ __forceinline__ void tile_of(int tiles_m, int tiles_n, int total, int
 __device__ __forceinline__ int piece_at(int row, int piece) { return row * 128 + ((piece ^ (row >> 1)) & 7) * 16; }
 
 // A tile's operand on its way into LDS: NW wavefronts, each instruction 64 pieces (eight rows). Rows past the last one
-// load the last one again; what they give is not stored.
+// load the last one again; what they give is not stored. Offsets inside a tile stay in 32 bits (the host checks).
 template <int ROWS, int NW>
 struct Stage {
     static constexpr int PER = ROWS / 8 / NW;
     static_assert(ROWS % (8 * NW) == 0, "whole instructions to each wavefront");
-    const uint8_t *src[PER];
-    const uint8_t *sc;
+    const uint8_t *q, *s;  // of the tile's first row
+    uint32_t off[PER], soff;
     __device__ __forceinline__ Stage(const Packed &p, int r0, int rows, int wv, int lane) {
+        q = p.q + (int64_t)r0 * p.ldq;
+        s = p.s + (int64_t)r0 * p.lds;
 #pragma unroll
         for (int i = 0; i < PER; i++) {
             const int r = 8 * (wv * PER + i) + (lane >> 3), piece = (lane ^ (r >> 1)) & 7;
-            src[i] = p.q + (int64_t)min(r0 + r, rows - 1) * p.ldq + 16 * piece;
+            off[i] = (uint32_t)min(r, rows - 1 - r0) * (uint32_t)p.ldq + 16 * piece;
         }
-        sc = p.s + (int64_t)min(r0 + (wv * 64 + lane) % ROWS, rows - 1) * p.lds;
+        soff = (uint32_t)min((wv * 64 + lane) % ROWS, rows - 1 - r0) * (uint32_t)p.lds;
     }
     __device__ __forceinline__ void load(int blk, uint32_t lds, int wv) const {
 #pragma unroll
-        for (int i = 0; i < PER; i++) load_to_lds(src[i] + (int64_t)blk * 128, lds + (wv * PER + i) * 1024);
+        for (int i = 0; i < PER; i++) load_to_lds(q + (int64_t)blk * 128, off[i], lds + (wv * PER + i) * 1024);
     }
     // The scale dword that holds block blk's byte, of every row.
     __device__ __forceinline__ void load_scales(int blk, uint32_t lds, int wv) const {
-        if (wv < ROWS / 64) load_to_lds4(sc + (blk & ~3), lds + wv * 256);
+        if (wv < ROWS / 64) load_to_lds4(s + (blk & ~3), soff, lds + wv * 256);
     }
 };
 
 __device__ __forceinline__ float scale_in(uint32_t dword, int blk) { return scale_of((int)(dword >> (8 * (blk & 3))) & 255); }
 
+// One half chunk (16 k) of a wavefront's MT x NT blocks: its MFMAs from the widened operands w, and between them, in this
+// order, the conversions of the half that comes next and what `beside` has to do: the matrix pipe takes 32 cycles an MFMA,
+// the four to six instructions after it go under those. (Left to itself the compiler gathers the conversions, and the two
+// pipes take turns.)
+template <int MT, int NT, class Raw, class Scale, class Beside>
+__device__ __forceinline__ void half_chunk(floatx16 (&acc)[MT][NT], const u32x4 (&w)[MT + NT], u32x4 (&next)[MT + NT], Raw raw,
+                                           Scale scale, Beside beside) {
+    constexpr int M = MT * NT, V = 2 * (MT + NT);  // conversions in pairs
+#pragma unroll
+    for (int f = 0; f < M; f++) {
+        acc[f / NT][f % NT] = oms::mma(w[f / NT], w[MT + f % NT], acc[f / NT][f % NT]);
+        beside(f);
+#pragma unroll
+        for (int v = f * V / M; v < (f + 1) * V / M; v++) {
+            const int o = v / 2, h = v & 1;
+            const uint32_t c = raw(o, h);
+            next[o][2 * h] = widen2(c, scale(o), std::false_type());
+            next[o][2 * h + 1] = widen2(c, scale(o), std::true_type());
+        }
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
+
+// Where finished sums go: a split's own partial sums, or C with the bias (-0, which changes nothing, where there is none).
+struct Out {
+    float *base;
+    int64_t ld;
+    const float *bias;
+    bool acc;
+    __device__ __forceinline__ Out(const Gemm8 &p, int split) {
+        const bool part = p.splits > 1;
+        base = part ? p.ws + (int64_t)split * p.m * p.n : p.c;
+        ld = part ? p.n : p.ldc;
+        bias = part ? nullptr : p.bias;
+        acc = !part && p.acc;
+    }
+    __device__ __forceinline__ float bias_of(int col) const { return bias ? bias[col] : -0.0f; }
+    __device__ __forceinline__ void put(int row, int col, float v, float bias) const {
+        float *c = base + row * ld + col;
+        v = v + bias;
+        *c = acc ? *c + v : v;
+    }
+};
+
 // A workgroup of WM x WN wavefronts computes BM x BN of C in stages of 128 k, two of them in LDS: the next one's loads are
 // issued as the current one begins. A lane's 16-byte piece g + 2 j (g = lane / 32) of a row feeds two MFMAs, which so see
 // k = 32 j + 16 g + 8 t + e in place of their own order, alike for both operands.
 template <int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN) k_gemm8(Gemm8 p) {
+__global__ void __launch_bounds__(64 * WM * WN, 2) k_gemm8(Gemm8 p) {
     OM_LDS_POISON();
     constexpr int NW = WM * WN, MT = BM / WM / 32, NT = BN / WN / 32;
     constexpr int STAGE = (BM + BN) * 132, AS = BM * 128, BS = AS + BN * 128, SS = BS + BM * 4;
@@ -133,60 +189,211 @@ __global__ void __launch_bounds__(64 * WM * WN) k_gemm8(Gemm8 p) {
         for (int j = 0; j < NT; j++)
 #pragma unroll
             for (int e = 0; e < 16; e++) acc[i][j][e] = 0.0f;
-    if (b0 < b1) issue(b0, base);  // (k may be 0)
-    for (int blk = b0; blk < b1; blk++) {
-        const int at = ((blk - b0) & 1) * STAGE;
-        land();
-        if (blk + 1 < b1) issue(blk + 1, base + (STAGE - at));
-        const char *cur = sh + at;
-        float fa[MT], fb[NT];
+    // A stage is four chunks of 32 k, a chunk two halves of 16. Operands 0 .. MT - 1 are A's blocks, the others B's. A chunk's
+    // codes are read a chunk ahead, a half's are widened a half ahead. The barrier stands before a stage's last chunk, whose
+    // codes are in registers by then, so that the next stage's first ones follow without a gap and the stage just read is
+    // free for the loads of the one after the next.
+    u32x4 raw[2][MT + NT], w[2][MT + NT];
+    float sc[2][MT + NT];
+    auto row_at = [&](int o) { return o < MT ? (wm + 32 * o + l32) : BM + wn + 32 * (o - MT) + l32; };
+    auto read = [&](int h, const char *cur, int q, int o) {
+        raw[h][o] = *reinterpret_cast<const u32x4 *>(cur + piece_at(row_at(o), 2 * q + g));
+    };
+    auto read_scale = [&](const char *cur, int o) { return *reinterpret_cast<const uint32_t *>(cur + BS + 4 * row_at(o)); };
+    auto first_half = [&](int q, const char *cur, int nq) {  // reads chunk nq of `cur` meanwhile
+        half_chunk<MT, NT>(acc, w[0], w[1], [&](int o, int h) { return raw[q & 1][o][2 + h]; }, [&](int o) { return sc[0][o]; },
+                           [&](int f) {
 #pragma unroll
-        for (int i = 0; i < MT; i++) fa[i] = scale_in(*reinterpret_cast<const uint32_t *>(cur + BS + 4 * (wm + 32 * i + l32)), blk);
+                               for (int o = f * (MT + NT) / (MT * NT); o < (f + 1) * (MT + NT) / (MT * NT); o++)
+                                   read((q + 1) & 1, cur, nq, o);
+                           });
+    };
+    auto second_half = [&](int q, int s) {
+        half_chunk<MT, NT>(acc, w[1], w[0], [&](int o, int h) { return raw[(q + 1) & 1][o][h]; },
+                           [&](int o) { return sc[s][o]; }, [](int) {});
+    };
+    if (b0 < b1) {  // (k may be 0)
+        issue(b0, base);
+        land<0>();
+        if (b0 + 1 < b1) issue(b0 + 1, base + STAGE);
 #pragma unroll
-        for (int j = 0; j < NT; j++) fb[j] = scale_in(*reinterpret_cast<const uint32_t *>(cur + SS + 4 * (wn + 32 * j + l32)), blk);
+        for (int o = 0; o < MT + NT; o++) {
+            read(0, sh, 0, o);
+            sc[0][o] = sc[1][o] = scale_in(read_scale(sh, o), b0);
+            w[0][o] = widen8(raw[0][o][0], raw[0][o][1], sc[0][o]);
+        }
+        for (int blk = b0; blk < b1; blk++) {
+            const int at = ((blk - b0) & 1) * STAGE;
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            u32x4 a[MT], b[NT];
-#pragma unroll
-            for (int i = 0; i < MT; i++) a[i] = *reinterpret_cast<const u32x4 *>(cur + piece_at(wm + 32 * i + l32, 2 * q + g));
-#pragma unroll
-            for (int j = 0; j < NT; j++) b[j] = *reinterpret_cast<const u32x4 *>(cur + AS + piece_at(wn + 32 * j + l32, 2 * q + g));
-#pragma unroll
-            for (int t = 0; t < 2; t++) {
-                u32x4 wa[MT], wb[NT];
-#pragma unroll
-                for (int i = 0; i < MT; i++) wa[i] = widen8(a[i][2 * t], a[i][2 * t + 1], fa[i]);
-#pragma unroll
-                for (int j = 0; j < NT; j++) wb[j] = widen8(b[j][2 * t], b[j][2 * t + 1], fb[j]);
-#pragma unroll
-                for (int i = 0; i < MT; i++)
-#pragma unroll
-                    for (int j = 0; j < NT; j++) acc[i][j] = oms::mma(wa[i], wb[j], acc[i][j]);
+            for (int q = 0; q < 3; q++) {
+                first_half(q, sh + at, q + 1);
+                second_half(q, 0);
             }
+            if (blk + 1 < b1) {
+                land<0>();
+                if (blk + 2 < b1) issue(blk + 2, base + at);
+#pragma unroll
+                for (int o = 0; o < MT + NT; o++) sc[1][o] = scale_in(read_scale(sh + (STAGE - at), o), blk + 1);
+            }
+            first_half(3, sh + (STAGE - at), 0);  // (past the last stage what the other buffer holds, for nothing)
+            second_half(3, 1);
+#pragma unroll
+            for (int o = 0; o < MT + NT; o++) sc[0][o] = sc[1][o];
         }
     }
     // A register is one row, 32 neighbouring columns over the lanes: stores of whole 128-byte lines.
+    const Out to(p, split);
+    const bool whole = m0 + BM <= p.m;
 #pragma unroll
     for (int j = 0; j < NT; j++) {
         const int col = n0 + wn + 32 * j + l32;
         if (col >= p.n) continue;
-        const float bias = p.bias ? p.bias[col] : 0.0f;
+        const float bias = to.bias_of(col);
 #pragma unroll
-        for (int i = 0; i < MT; i++)
+        for (int i = 0; i < MT; i++) {
+            const int row = m0 + wm + 32 * i + 4 * g;
+            float *c = to.base + row * to.ld + col;
+            float old[16];
+            if (to.acc) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int r = 8 * (e >> 2) + (e & 3);
+                    if (whole || row + r < p.m) old[e] = c[r * to.ld];
+                }
+#pragma unroll
+                for (int e = 0; e < 16; e++) acc[i][j][e] = old[e] + (acc[i][j][e] + bias);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 16; e++) acc[i][j][e] += bias;
+            }
 #pragma unroll
             for (int e = 0; e < 16; e++) {
-                const int row = m0 + wm + 32 * i + 8 * (e >> 2) + 4 * g + (e & 3);
-                if (row >= p.m) continue;
-                float v = acc[i][j][e];
-                if (p.splits > 1) {
-                    p.ws[((int64_t)split * p.m + row) * p.n + col] = v;
-                    continue;
-                }
-                float *c = p.c + row * p.ldc + col;
-                if (p.bias) v = v + bias;
-                if (p.acc) v = *c + v;
-                *c = v;
+                const int r = 8 * (e >> 2) + (e & 3);
+                if (whole || row + r < p.m) c[r * to.ld] = acc[i][j][e];
             }
+        }
+    }
+}
+
+// Few tiles: the wavefronts of a workgroup share one tile of BM x BN and split k between them, four to a block of 128, so that
+// every code is widened once and a stage of KW blocks goes round without a barrier inside it. D stages stand in LDS, and
+// one more in registers. Their sums meet in LDS and are added in order.
+template <int BM, int BN, int KW, int D>
+__global__ void __launch_bounds__(256 * KW, KW < 2 ? 2 : KW) k_gemm8_few(Gemm8 p) {
+    OM_LDS_POISON();
+    static_assert(4 % KW == 0, "a stage's scale bytes lie in one dword");
+    constexpr int NW = 4 * KW, MT = BM / 32, NT = BN / 32, BLOCK = (BM + BN) * 128;
+    constexpr int SS = KW * BLOCK, STAGE = SS + (BM + BN + 63) / 64 * 256;  // a scale load fills 64 dwords
+    constexpr int LD = BN + 1, OUT = NW * BM * LD * 4;
+    constexpr int LDS = D * STAGE > OUT ? D * STAGE : OUT, PER = (BM + BN) / 32;
+    __shared__ __attribute__((aligned(16))) char sh[LDS];
+    const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kb = wv >> 2, q = wv & 3;
+    int split, tm, tn;
+    tile_of(p.tiles_m, p.tiles_n, gridDim.x, split, tm, tn);
+    const int m0 = tm * BM, n0 = tn * BN;
+    // Rows 0 .. BM - 1 of a stage's block are A's, the others B's; this wavefront loads its quarter of block kb, eight rows of
+    // one operand an instruction.
+    const uint8_t *src[PER];
+    uint32_t off[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int r0 = 8 * (q * PER + i), r = r0 + (lane >> 3), piece = (lane ^ (r >> 1)) & 7;
+        const bool a = r0 < BM;
+        const Packed &o = a ? p.a : p.b;
+        const int first = a ? m0 : n0, last = (a ? p.m : p.n) - 1 - first;
+        src[i] = o.q + (int64_t)first * o.ldq;
+        off[i] = (uint32_t)min(a ? r : r - BM, last) * (uint32_t)o.ldq + 16 * piece;
+    }
+    // scale bytes: 64 rows an instruction, A's and then B's
+    const int sr = min(wv * 64 + lane, BM + BN - 1);
+    const uint8_t *ssrc = sr < BM ? p.a.s + (int64_t)min(m0 + sr, p.m - 1) * p.a.lds
+                                  : p.b.s + (int64_t)min(n0 + sr - BM, p.n - 1) * p.b.lds;
+    const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)sh;
+    const int b0 = split * p.per, b1 = min(p.blocks, b0 + p.per), stages = (b1 - b0 + KW - 1) / KW;
+    auto issue = [&](int st) {  // past the last stage the last one again, into a slot that nothing reads
+        const uint32_t at = base + (uint32_t)(st % D) * STAGE;
+        const int blk = min(b0 + min(st, stages - 1) * KW + kb, b1 - 1);
+#pragma unroll
+        for (int i = 0; i < PER; i++) load_to_lds(src[i] + (int64_t)blk * 128, off[i], at + kb * BLOCK + (q * PER + i) * 1024);
+        if (wv * 64 < BM + BN) load_to_lds4(ssrc + (blk & ~3), at + SS + wv * 256);
+    };
+    floatx16 acc[MT][NT];
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) acc[i][j][e] = 0.0f;
+    u32x4 raw[2][MT + NT], w[2][MT + NT];
+    uint32_t dw[2][MT + NT];
+    auto row_at = [&](int o) { return o < MT ? 32 * o + l32 : BM + 32 * (o - MT) + l32; };
+    auto read = [&](int h, int st, int o) {
+        const char *cur = sh + (st % D) * STAGE;
+        dw[h][o] = *reinterpret_cast<const uint32_t *>(cur + SS + 4 * row_at(o));
+        raw[h][o] = *reinterpret_cast<const u32x4 *>(cur + kb * BLOCK + piece_at(row_at(o), 2 * q + g));
+    };
+    // Stage st from registers, the next one's codes read meanwhile, its own slot loaded anew. (Blocks past the last one hold
+    // the last one's codes, which this wavefront drops.)
+    float sc[2][MT + NT];
+    auto turn = [&](int h, int st) {
+        land<(D - 2) * PER>();
+        issue(st + D);
+#pragma unroll
+        for (int o = 0; o < MT + NT; o++) read(h ^ 1, st + 1, o);
+        const int blk = b0 + st * KW + kb;
+        if (blk < b1) {
+            half_chunk<MT, NT>(acc, w[0], w[1], [&](int o, int t) { return raw[h][o][2 + t]; }, [&](int o) { return sc[h][o]; },
+                               [](int) {});
+#pragma unroll
+            for (int o = 0; o < MT + NT; o++) sc[h ^ 1][o] = scale_in(dw[h ^ 1][o], blk + KW);
+            half_chunk<MT, NT>(acc, w[1], w[0], [&](int o, int t) { return raw[h ^ 1][o][t]; },
+                               [&](int o) { return sc[h ^ 1][o]; }, [](int) {});
+        }
+    };
+    if (stages) {
+#pragma unroll
+        for (int st = 0; st < D; st++) issue(st);
+        land<(D - 1) * PER>();
+#pragma unroll
+        for (int o = 0; o < MT + NT; o++) {
+            read(0, 0, o);
+            sc[0][o] = scale_in(dw[0][o], b0 + kb);
+            w[0][o] = widen8(raw[0][o][0], raw[0][o][1], sc[0][o]);
+        }
+        for (int st = 0; st < stages; st += 2) {
+            turn(0, st);
+            if (st + 1 < stages) turn(1, st + 1);
+        }
+    }
+    land<0>();
+    float *out = reinterpret_cast<float *>(sh);
+#pragma unroll
+    for (int i = 0; i < MT; i++)
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++)
+                out[(wv * BM + 32 * i + 8 * (e >> 2) + 4 * g + (e & 3)) * LD + 32 * j + l32] = acc[i][j][e];
+    __syncthreads();
+    const Out to(p, split);
+    constexpr int EACH = BM * BN / (64 * NW);  // values a thread
+    static_assert(BM * BN % (64 * NW) == 0 && 64 * NW % BN == 0, "whole rows to a pass of the threads");
+    const int c = threadIdx.x % BN, col = n0 + c;
+    if (col >= p.n) return;
+    const float bias = to.bias_of(col);
+    float v[EACH];
+#pragma unroll
+    for (int u = 0; u < EACH; u++) {
+        const int r = threadIdx.x / BN + u * (64 * NW / BN);
+        v[u] = out[r * LD + c];
+#pragma unroll
+        for (int w = 1; w < NW; w++) v[u] += out[(w * BM + r) * LD + c];
+    }
+#pragma unroll
+    for (int u = 0; u < EACH; u++) {
+        const int row = m0 + threadIdx.x / BN + u * (64 * NW / BN);
+        if (row < p.m) to.put(row, col, v[u], bias);
     }
 }
 
@@ -205,23 +412,73 @@ __global__ void __launch_bounds__(256) k_gemm8_join(Gemm8 p) {
     }
 }
 
+// A kernel's tile and what its workgroups take, in us, with `resident` of them on a CU at most: `fix` a round of those and
+// `each` a workgroup, and for a stage of kw blocks of k `alone` where a CU has one workgroup, `shared` a workgroup where it
+// has more. Fitted to 8019 (products) and 2674 (weight gradients) times over all kernels, splits of k from 1 to 16 and sizes
+// from 1 to 16384; of all those the choice by them is 0.8 % behind the best in the mean, 21 % at most.
+struct Tile {
+    int bm, bn, kw, resident;
+    float fix, each, alone, shared;
+};
+struct Choice {
+    int tile, splits;
+};
+// Splitting k costs a second launch that adds the parts, `join` us and `join_each` a million values.
+template <int N>
+Choice choose(const Tile (&tiles)[N], int cus, int64_t m, int64_t n, int blocks, int64_t row_bytes, float join, float join_each) {
+    Choice best = {-1, 1};
+    double least = 0.0;
+    for (int t = 0; t < N; t++) {
+        const Tile &c = tiles[t];
+        if ((c.bm > c.bn ? c.bm : c.bn) * row_bytes > INT64_C(0xFFFFFFFF)) continue;  // offsets inside a tile: 32 bits
+        for (int s : {1, 2, 3, 4, 6, 8, 12, 16}) {
+            if (s > 1 && blocks < 4 * s) break;
+            const int per = ((blocks + s - 1) / s + c.kw - 1) / c.kw * c.kw, parts = per ? (blocks + per - 1) / per : 1;
+            const double wgs = (double)((m + c.bm - 1) / c.bm) * (double)((n + c.bn - 1) / c.bn) * parts;
+            const double load = std::ceil(wgs / cus), rounds = std::ceil(load / c.resident), stages = per / c.kw;
+            double us = c.fix * rounds + c.each * load + std::fmax(c.alone * rounds, c.shared * load) * stages;
+            if (parts > 1) us += join + join_each * parts * (double)m * (double)n * 1e-6;
+            if (best.tile < 0 || us < least) {
+                least = us;
+                best = {t, s};
+            }
+        }
+    }
+    if (const char *force = om::tuning_env("OM_TILE8")) best.tile = atoi(force);
+    if (const char *force = om::tuning_env("OM_SPLITS8")) best.splits = atoi(force);
+    return best;
+}
+// Blocks of k to a split (whole stages, since a stage's scale bytes are one dword) and the splits that gives.
+inline void split_blocks(int blocks, int kw, int splits, int &per, int &parts) {
+    per = ((blocks + splits - 1) / splits + kw - 1) / kw * kw;
+    parts = blocks > per ? (blocks + per - 1) / per : 1;
+}
+
+constexpr Tile kTiles[] = {{256, 256, 1, 1, 4.86f, 0.38f, 2.255f, 0.0f},
+                           {128, 128, 1, 2, 0.0f, 2.76f, 0.852f, 0.31f},
+                           {64, 64, 1, 2, 0.24f, 2.2f, 0.305f, 0.24f},
+                           {32, 32, 1, 4, 0.55f, 0.5f, 0.18f, 0.095f},
+                           {32, 32, 2, 2, 0.0f, 1.24f, 0.256f, 0.194f}};
+
 om_status gemm8(om_ctx *ctx, const char *what, Gemm8 p) {
-    const int64_t big = (int64_t)((p.m + 255) / 256) * ((p.n + 255) / 256);
-    const int bm = big >= ctx->num_cus ? 256 : 128;
-    p.tiles_m = (p.m + bm - 1) / bm;
-    p.tiles_n = (p.n + bm - 1) / bm;
-    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-    int splits = 1;
-    if (tiles < ctx->num_cus) splits = (int)(ctx->num_cus / tiles);
-    if (splits > p.blocks) splits = p.blocks;
-    p.per = splits > 1 ? (p.blocks + splits - 1) / splits : p.blocks;
-    p.splits = splits > 1 ? (p.blocks + p.per - 1) / p.per : 1;
-    OM_REQUIRE(ctx, tiles * p.splits <= INT32_MAX, "%s: %d x %d is more than a launch takes", what, p.m, p.n);
+    const Choice ch = choose(kTiles, ctx->num_cus, p.m, p.n, p.blocks, p.a.ldq, 2.24f, 1.61f);
+    OM_REQUIRE(ctx, ch.tile >= 0, "%s: k is more than a launch takes", what);
+    const Tile &c = kTiles[ch.tile];
+    p.tiles_m = (p.m + c.bm - 1) / c.bm;
+    p.tiles_n = (p.n + c.bn - 1) / c.bn;
+    split_blocks(p.blocks, c.kw, ch.splits, p.per, p.splits);
+    const int64_t wgs = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+    OM_REQUIRE(ctx, wgs <= INT32_MAX, "%s: %d x %d is more than a launch takes", what, p.m, p.n);
     if (p.splits > 1)
         if (om_status s = om::scratch(ctx, sizeof(float) * (uint64_t)p.splits * (uint64_t)p.m * (uint64_t)p.n, &p.ws)) return s;
-    const unsigned grid = (unsigned)(tiles * p.splits);
-    if (bm == 256) hipLaunchKernelGGL((k_gemm8<256, 256, 2, 4>), dim3(grid), dim3(512), 0, ctx->stream, p);
-    else hipLaunchKernelGGL((k_gemm8<128, 128, 2, 2>), dim3(grid), dim3(256), 0, ctx->stream, p);
+    auto go = [&](auto kern, int threads) { hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(threads), 0, ctx->stream, p); };
+    switch (ch.tile) {
+        case 0: go(k_gemm8<256, 256, 2, 4>, 512); break;
+        case 1: go(k_gemm8<128, 128, 2, 2>, 256); break;
+        case 2: go(k_gemm8_few<64, 64, 1, 3>, 256); break;
+        case 3: go(k_gemm8_few<32, 32, 1, 4>, 256); break;
+        default: go(k_gemm8_few<32, 32, 2, 4>, 512); break;
+    }
     if (p.splits > 1)
         hipLaunchKernelGGL(k_gemm8_join, dim3(om::grid1d((int64_t)p.m * p.n, 256, (int64_t)ctx->num_cus * 8)), dim3(256), 0,
                            ctx->stream, p);
@@ -238,6 +495,7 @@ struct Dw8 {
     const float *g;         // [rows, m]
     Packed x;               // [n, rows]
     int rows, m, n, blocks;
+    int full;               // blocks of 128 whole rows that are loaded four columns at a time
     float *dw, *db;
     int acc_dw, acc_db;
     int splits, per;
@@ -246,96 +504,171 @@ struct Dw8 {
     int tiles_m, tiles_n;
 };
 
-__device__ __forceinline__ void split3(float x0, float x1, uint32_t &h, uint32_t &m, uint32_t &l) {
-    h = oms::pack2(x0, x1);
+// The parts of two values, in two steps: the first part and what it leaves (x), then the other two.
+__device__ __forceinline__ uint32_t split_first(float &x0, float &x1) {
+    uint32_t h = oms::pack2(x0, x1);
     asm("" : "+v"(h));  // else the compiler converts x0 a second time instead of shifting h
-    const float r0 = x0 - __uint_as_float(h << 16), r1 = x1 - __uint_as_float(h & 0xFFFF0000u);
+    x0 -= __uint_as_float(h << 16);
+    x1 -= __uint_as_float(h & 0xFFFF0000u);
+    return h;
+}
+__device__ __forceinline__ void split_rest(float r0, float r1, uint32_t &m, uint32_t &l) {
     m = oms::pack2(r0, r1);
     asm("" : "+v"(m));
     l = oms::pack2(r0 - __uint_as_float(m << 16), r1 - __uint_as_float(m & 0xFFFF0000u));
 }
 
-template <int BN, int MG>
-__global__ void __launch_bounds__(64 * MG) k_dw8(Dw8 p) {
+// A workgroup computes (32 MG) x (32 NT) of dW with MG groups of 4 KW wavefronts: wavefront (mg, kb, q) has 32 rows (columns
+// of g), all columns, and the q-th 32 k of every KW-th block of 128, so x is widened by MG wavefronts only and g is split
+// once. Both come through LDS, D stages of KW blocks and one more in registers, by loads of 16 bytes a lane (a dword a lane
+// into registers, as g's layout would have it, keeps the load path busy as long for a quarter of the data: 210 us against
+// 140 of products at 16384 x 768 x 2304). The next half's (16 k) splits and conversions stand between a half's MFMAs. At the end the wavefronts'
+// sums meet in LDS and are added in order.
+template <int NT, int MG, int KW, int D>
+__global__ void __launch_bounds__(256 * MG * KW, MG * KW < 4 ? 2 : 4) k_dw8(Dw8 p) {
     OM_LDS_POISON();
-    constexpr int BM = 32 * MG, NT = BN / 32, STAGE = BN * 132, SS = BN * 128;
-    __shared__ __attribute__((aligned(16))) char sh[2 * STAGE];
+    constexpr int NW = 4 * KW * MG, BM = 32 * MG, BN = 32 * NT, BLOCK = BN * 128, SS = KW * BLOCK;
+    constexpr int GS = SS + (BN + 63) / 64 * 256;  // a scale load fills 64 dwords
+    constexpr int STAGE = GS + NW * 4096, LD = BN + 1, OUT = NW * 32 * LD * 4, LDS = D * STAGE > OUT ? D * STAGE : OUT;
+    constexpr int PER = BN / 32 / MG, LOADS = PER + 4;
+    static_assert(BN % (32 * MG) == 0 && BN <= 64 * NW && 4 % KW == 0, "whole loads to each wavefront, scales by one of each");
+    __shared__ __attribute__((aligned(16))) char sh[LDS];
     const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
-    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mg = wv / (4 * KW), kb = wv / 4 % KW, q = wv & 3;
     int split, tm, tn;
     tile_of(p.tiles_m, p.tiles_n, gridDim.x, split, tm, tn);
-    const int m0 = tm * BM + 32 * wv, n0 = tn * BN;
-    const int b0 = split * p.per, b1 = min(p.blocks, b0 + p.per);
-    const Stage<BN, MG> sb(p.x, n0, p.n, wv, lane);
+    const int m0 = tm * BM + 32 * mg, n0 = tn * BN;
+    // blocks of 128 rows, and (in the last split) the rows behind the last that is taken as one
+    const int b0 = split * p.per, b1 = min(p.full, b0 + p.per), count = max(b1 - b0, 0), stages = (count + KW - 1) / KW;
+    const bool tail = split == p.splits - 1 && p.full < p.blocks;
+    const uint8_t *xq = p.x.q + (int64_t)n0 * p.x.ldq;
+    uint32_t off[PER];
+#pragma unroll
+    for (int i = 0; i < PER; i++) {
+        const int r = 8 * ((q * MG + mg) * PER + i) + (lane >> 3), piece = (lane ^ (r >> 1)) & 7;
+        off[i] = (uint32_t)min(r, p.n - 1 - n0) * (uint32_t)p.x.ldq + 16 * piece;
+    }
+    const uint8_t *xs = p.x.s + (int64_t)min(n0 + (wv * 64 + lane) % BN, p.n - 1) * p.x.lds;
+    // g: this wavefront's own 32 rows x 32 columns of a stage, eight rows a load, four columns a lane. Columns past the last
+    // four start there: column c then stands at c - (m - 4) of its four. (Of fewer than four columns the loads run on into
+    // the next rows, which is why the last block is not loaded so then.)
+    const int first4 = max(p.m - 4, 0), gc = min(m0 + l32, p.m - 1);
+    const uint32_t goff = 4u * ((uint32_t)(lane >> 3) * (uint32_t)p.m + (uint32_t)min(m0 + 4 * (lane & 7), first4));
+    const int gat = GS + wv * 4096 + 2048 * g + 4 * ((l32 & ~3) + min(gc - min(m0 + (l32 & ~3), first4), 3));
     const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)sh;
-    auto issue = [&](int blk, uint32_t at) {
-        sb.load(blk, at, wv);
-        sb.load_scales(blk, at + SS, wv);
+    // Loads past the last block load that one again, into slots that nothing reads.
+    auto issue = [&](int st) {
+        const uint32_t at = base + (uint32_t)(st % D) * STAGE;
+        const int blk = b0 + min(min(st, stages - 1) * KW + kb, count - 1);
+#pragma unroll
+        for (int i = 0; i < PER; i++)
+            load_to_lds(xq + (int64_t)blk * 128, off[i], at + kb * BLOCK + ((q * MG + mg) * PER + i) * 1024);
+        if (wv * 64 < BN) load_to_lds4(xs + (blk & ~3), at + SS + wv * 256);
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            load_to_lds(p.g + ((int64_t)blk * 128 + 32 * q + 8 * i) * p.m, goff, at + GS + wv * 4096 + i * 1024);
     };
-    // a wavefront past the last row of dW loads the last one; nothing of it is stored
-    const float *gp = p.g + min(m0 + l32, p.m - 1);
-    const bool sums = p.db && tn == 0;
-    double cs = 0.0;
+    float raw[2][16];
     floatx16 acc[NT];
 #pragma unroll
     for (int j = 0; j < NT; j++)
 #pragma unroll
         for (int e = 0; e < 16; e++) acc[j][e] = 0.0f;
-    float raw[16];
-    // The 16 values of g that chunk q (32 k) of block blk takes in this lane; rows past the last are zero.
-    auto fetch = [&](int blk, int q) {
-        const int64_t k0 = (int64_t)blk * 128 + 32 * q + 16 * g;
-        if ((int64_t)blk * 128 + 128 <= p.rows) {
+    const bool sums = p.db && tn == 0;
+    double cs = 0.0;
+    u32x4 xr[2][NT], wa[2][3], wb[2][NT];
+    float sc[2][NT];
+    auto read = [&](int h, int st) {
+        const char *cur = sh + (st % D) * STAGE;
 #pragma unroll
-            for (int e = 0; e < 16; e++) raw[e] = gp[(k0 + e) * p.m];
+        for (int j = 0; j < NT; j++) {
+            sc[h][j] = scale_in(*reinterpret_cast<const uint32_t *>(cur + SS + 4 * (32 * j + l32)), b0 + st * KW + kb);
+            xr[h][j] = *reinterpret_cast<const u32x4 *>(cur + kb * BLOCK + piece_at(32 * j + l32, 2 * q + g));
+        }
+#pragma unroll
+        for (int e = 0; e < 16; e++) raw[h][e] = *reinterpret_cast<const float *>(cur + gat + 128 * e);
+    };
+    // Step v of the operands of half t of the stage in set h: four pairs of g in two steps each, then the blocks of x; four to
+    // six instructions each, which go under an MFMA's 32 cycles.
+    constexpr int STEPS = 8 + NT;
+    float left[2];
+    auto prepare = [&](int t, int h, int v) {
+        if (v >= 8) {
+            wb[t][v - 8] = widen8(xr[h][v - 8][2 * t], xr[h][v - 8][2 * t + 1], sc[h][v - 8]);
+        } else if (v % 2 == 0) {
+            left[0] = raw[h][8 * t + v];
+            left[1] = raw[h][8 * t + v + 1];
+            wa[t][0][v / 2] = split_first(left[0], left[1]);
         } else {
-#pragma unroll
-            for (int e = 0; e < 16; e++) {
-                const float v = gp[min(k0 + e, (int64_t)p.rows - 1) * p.m];
-                raw[e] = k0 + e < p.rows ? v : 0.0f;
-            }
+            uint32_t m, l;
+            split_rest(left[0], left[1], m, l);
+            wa[t][1][v / 2] = m;
+            wa[t][2][v / 2] = l;
         }
     };
-    issue(b0, base);
-    fetch(b0, 0);
-    for (int blk = b0; blk < b1; blk++) {
-        const int at = ((blk - b0) & 1) * STAGE;
-        land();
-        if (blk + 1 < b1) issue(blk + 1, base + (STAGE - at));
-        const char *cur = sh + at;
-        float fb[NT];
+    auto half = [&](int t, int h) {  // half t's products; the next half is t ^ 1, of set h
 #pragma unroll
-        for (int j = 0; j < NT; j++) fb[j] = scale_in(*reinterpret_cast<const uint32_t *>(cur + SS + 4 * (32 * j + l32)), blk);
+        for (int f = 0; f < 3 * NT; f++) {
+            acc[f % NT] = oms::mma(wa[t][2 - f / NT], wb[t][f % NT], acc[f % NT]);
 #pragma unroll
-        for (int q = 0; q < 4; q++) {
-            u32x4 fa[2][3];
+            for (int v = f * STEPS / (3 * NT); v < (f + 1) * STEPS / (3 * NT); v++) prepare(t ^ 1, h, v);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    };
+    auto add_sums = [&](int h) {
+        if (sums) {  // four chains
+            double part[4] = {0.0, 0.0, 0.0, 0.0};
 #pragma unroll
-            for (int t = 0; t < 2; t++)
+            for (int e = 0; e < 16; e++) part[e & 3] += (double)raw[h][e];
+            cs += (part[0] + part[1]) + (part[2] + part[3]);
+        }
+    };
+    // Stage st from registers, the next one read meanwhile, its own slot loaded anew.
+    auto turn = [&](int h, int st) {
+        land<(D - 2) * LOADS>();
+        issue(st + D);
+        read(h ^ 1, st + 1);
+        if (st * KW + kb < count) {
+            add_sums(h);
+            half(0, h);
+            half(1, h ^ 1);
+        }
+    };
+    if (count > 0) {
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    uint32_t h, m, l;
-                    split3(raw[8 * t + 2 * e], raw[8 * t + 2 * e + 1], h, m, l);
-                    fa[t][0][e] = h;
-                    fa[t][1][e] = m;
-                    fa[t][2][e] = l;
-                }
-            if (sums) {
+        for (int st = 0; st < D; st++) issue(st);
+        land<(D - 1) * LOADS>();
+        read(0, 0);
 #pragma unroll
-                for (int e = 0; e < 16; e++) cs += (double)raw[e];
-            }
-            if (q < 3) fetch(blk, q + 1);
-            else if (blk + 1 < b1) fetch(blk + 1, 0);
+        for (int v = 0; v < STEPS; v++) prepare(0, 0, v);
+        for (int st = 0; st < stages; st += 2) {
+            turn(0, st);
+            if (st + 1 < stages) turn(1, st + 1);
+        }
+        land<0>();  // the loads past the last stage, too, before LDS is used again
+    }
+    const bool rest = tail && kb == count % KW;
+#pragma unroll 1
+    for (int blk = rest ? p.full : p.blocks; blk < p.blocks; blk++) {  // the rows behind, straight from memory
 #pragma unroll
-            for (int j = 0; j < NT; j++) {
-                const u32x4 b = *reinterpret_cast<const u32x4 *>(cur + piece_at(32 * j + l32, 2 * q + g));
+        for (int e = 0; e < 16; e++) {
+            const int k = blk * 128 + 32 * q + 16 * g + e;
+            const float v = p.g[(int64_t)min(k, p.rows - 1) * p.m + gc];
+            raw[0][e] = k < p.rows ? v : 0.0f;
+        }
 #pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    const u32x4 w = widen8(b[2 * t], b[2 * t + 1], fb[j]);
-                    acc[j] = oms::mma(fa[t][2], w, acc[j]);
-                    acc[j] = oms::mma(fa[t][1], w, acc[j]);
-                    acc[j] = oms::mma(fa[t][0], w, acc[j]);
-                }
-            }
+        for (int j = 0; j < NT; j++) {
+            const int64_t col = min(n0 + 32 * j + l32, p.n - 1);
+            xr[0][j] = *reinterpret_cast<const u32x4 *>(p.x.q + col * p.x.ldq + (int64_t)blk * 128 + 32 * q + 16 * g);
+            sc[0][j] = scale_of(p.x.s[col * p.x.lds + blk]);
+        }
+        add_sums(0);
+#pragma unroll
+        for (int t = 0; t < 2; t++) {
+#pragma unroll
+            for (int v = 0; v < STEPS; v++) prepare(t, 0, v);
+#pragma unroll
+            for (int f = 0; f < 3 * NT; f++) acc[f % NT] = oms::mma(wa[t][2 - f / NT], wb[t][f % NT], acc[f % NT]);
         }
     }
     unsigned big = 0;
@@ -343,30 +676,43 @@ __global__ void __launch_bounds__(64 * MG) k_dw8(Dw8 p) {
     for (int j = 0; j < NT; j++)
 #pragma unroll
         for (int e = 0; e < 16; e++) oms::note(acc[j][e], big);
-    if (oms::beyond(big)) {
-#pragma unroll
+    if (oms::beyond(big)) {  // this wavefront's k again, two at a time
+#pragma unroll 1
         for (int j = 0; j < NT; j++) {
             const int64_t col = min(n0 + 32 * j + l32, p.n - 1);
-            const uint8_t *xq = p.x.q + col * p.x.ldq, *xs = p.x.s + col * p.x.lds;
+            const uint8_t *cq = p.x.q + col * p.x.ldq, *cx = p.x.s + col * p.x.lds;
             floatx16 t;
 #pragma unroll
             for (int e = 0; e < 16; e++) t[e] = 0.0f;
-            const int k1 = (int)min((int64_t)b1 * 128, (int64_t)p.rows);
+            auto block = [&](int blk) {
 #pragma unroll 1
-            for (int k0 = b0 * 128; k0 < k1; k0 += 2) {
-                const int k = min(k0 + g, k1 - 1);
-                const bool in = k0 + g < k1;
-                const float x = decode4(xq[k], scale_of(xs[k / 128]))[0];
-                const float gv = gp[(int64_t)k * p.m];
-                t = __builtin_amdgcn_mfma_f32_32x32x2f32(in ? gv : 0.0f, in ? x : 0.0f, t, 0, 0, 0);
-            }
-            oms::take_beyond(acc[j], t);
+                for (int k0 = blk * 128 + 32 * q, end = min(k0 + 32, p.rows); k0 < end; k0 += 2) {
+                    const int k = min(k0 + g, p.rows - 1);
+                    const bool in = k0 + g < p.rows;
+                    const float x = decode4(cq[k], scale_of(cx[blk]))[0], gv = p.g[(int64_t)k * p.m + gc];
+                    t = __builtin_amdgcn_mfma_f32_32x32x2f32(in ? gv : 0.0f, in ? x : 0.0f, t, 0, 0, 0);
+                }
+            };
+#pragma unroll 1
+            for (int at = kb; at < count; at += KW) block(b0 + at);
+            if (rest)
+#pragma unroll 1
+                for (int blk = p.full; blk < p.blocks; blk++) block(blk);
+#pragma unroll
+            for (int i = 0; i < NT; i++)
+                if (i == j) oms::take_beyond(acc[i], t);
         }
     }
+    __syncthreads();
     if (sums) {
         cs += __shfl_xor(cs, 32, 64);
+        double *shd = reinterpret_cast<double *>(sh);
+        if (g == 0) shd[wv * 32 + l32] = cs;
+        __syncthreads();
         const int row = m0 + l32;
-        if (g == 0 && row < p.m) {
+        if (wv % (4 * KW) == 0 && g == 0 && row < p.m) {
+#pragma unroll
+            for (int i = 1; i < 4 * KW; i++) cs += shd[(wv + i) * 32 + l32];
             if (p.splits > 1) {
                 p.cs[(int64_t)split * p.m + row] = cs;
             } else {
@@ -374,21 +720,31 @@ __global__ void __launch_bounds__(64 * MG) k_dw8(Dw8 p) {
                 p.db[row] = p.acc_db ? p.db[row] + v : v;
             }
         }
+        __syncthreads();
     }
+    float *out = reinterpret_cast<float *>(sh);
 #pragma unroll
-    for (int j = 0; j < NT; j++) {
-        const int col = n0 + 32 * j + l32;
-        if (col >= p.n) continue;
+    for (int j = 0; j < NT; j++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const int row = m0 + 8 * (e >> 2) + 4 * g + (e & 3);
-            if (row >= p.m) continue;
-            if (p.splits > 1) {
-                p.ws[((int64_t)split * p.m + row) * p.n + col] = acc[j][e];
-                continue;
-            }
-            float *c = p.dw + (int64_t)row * p.n + col;
-            *c = p.acc_dw ? *c + acc[j][e] : acc[j][e];
+        for (int e = 0; e < 16; e++) out[(wv * 32 + 8 * (e >> 2) + 4 * g + (e & 3)) * LD + 32 * j + l32] = acc[j][e];
+    __syncthreads();
+    constexpr int STEP = 64 * NW / BN, EACH = BM / STEP;
+    static_assert(64 * NW % BN == 0 && BM % STEP == 0, "whole rows to a pass of the threads");
+    const int c = threadIdx.x % BN, col = n0 + c;
+    if (col >= p.n) return;
+    const bool part = p.splits > 1;
+    float *to = part ? p.ws + (int64_t)split * p.m * p.n : p.dw;
+    const bool keep = !part && p.acc_dw;
+#pragma unroll 4
+    for (int u = 0; u < EACH; u++) {
+        const int r = threadIdx.x / BN + u * STEP, row = tm * BM + r;
+        const float *s = out + (r / 32 * 4 * KW * 32 + r % 32) * LD + c;
+        float v = s[0];
+#pragma unroll
+        for (int w = 1; w < 4 * KW; w++) v += s[w * 32 * LD];
+        if (row < p.m) {
+            float *d = to + (int64_t)row * p.n + col;
+            *d = keep ? *d + v : v;
         }
     }
 }
@@ -410,26 +766,31 @@ __global__ void __launch_bounds__(256) k_dw8_join(Dw8 p) {
     }
 }
 
+constexpr Tile kTilesDw[] = {{32, 128, 1, 2, 0.0f, 2.96f, 0.795f, 0.335f},
+                             {32, 64, 1, 3, 2.14f, 0.0f, 0.454f, 0.507f},
+                             {32, 32, 1, 2, 1.06f, 0.31f, 0.527f, 0.374f}};
+
 om_status dw8(om_ctx *ctx, Dw8 p) {
-    const int64_t big = (int64_t)((p.m + 255) / 256) * ((p.n + 127) / 128);
-    const int bm = big >= ctx->num_cus ? 256 : 128;
-    p.tiles_m = (p.m + bm - 1) / bm;
-    p.tiles_n = (p.n + 127) / 128;
-    const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
-    int splits = 1;
-    if (tiles < ctx->num_cus) splits = (int)(ctx->num_cus / tiles);
-    if (splits > p.blocks) splits = p.blocks;
-    p.per = (p.blocks + splits - 1) / splits;
-    p.splits = (p.blocks + p.per - 1) / p.per;
-    OM_REQUIRE(ctx, tiles * p.splits <= INT32_MAX, "om_linear_bwd_x8: in=%d out=%d is more than a launch takes", p.n, p.m);
+    const Choice ch = choose(kTilesDw, ctx->num_cus, p.m, p.n, p.blocks, p.x.ldq, 3.45f, 1.66f);
+    OM_REQUIRE(ctx, ch.tile >= 0 && p.rows <= INT32_MAX - 255 && p.m < 1 << 26,
+               "om_linear_bwd_x8: rows=%d in=%d out=%d is more than a launch takes", p.rows, p.n, p.m);
+    const Tile &c = kTilesDw[ch.tile];
+    p.tiles_m = (p.m + c.bm - 1) / c.bm;
+    p.tiles_n = (p.n + c.bn - 1) / c.bn;
+    split_blocks(p.blocks, c.kw, ch.splits, p.per, p.splits);
+    const int64_t wgs = (int64_t)p.tiles_m * p.tiles_n * p.splits;
+    OM_REQUIRE(ctx, wgs <= INT32_MAX, "om_linear_bwd_x8: in=%d out=%d is more than a launch takes", p.n, p.m);
     if (p.splits > 1) {
         const uint64_t sums = ((uint64_t)p.splits * p.m * p.n + 1) / 2 * 2;
         if (om_status s = om::scratch(ctx, 4 * sums + 8ull * p.splits * p.m, &p.ws)) return s;
         p.cs = reinterpret_cast<double *>(p.ws + sums);
     }
-    const unsigned grid = (unsigned)(tiles * p.splits);
-    if (bm == 256) hipLaunchKernelGGL((k_dw8<128, 8>), dim3(grid), dim3(512), 0, ctx->stream, p);
-    else hipLaunchKernelGGL((k_dw8<128, 4>), dim3(grid), dim3(256), 0, ctx->stream, p);
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(256), 0, ctx->stream, p); };
+    switch (ch.tile) {
+        case 0: go(k_dw8<4, 1, 1, 2>); break;
+        case 1: go(k_dw8<2, 1, 1, 2>); break;
+        default: go(k_dw8<1, 1, 1, 3>); break;
+    }
     if (p.splits > 1)
         hipLaunchKernelGGL(k_dw8_join, dim3(om::grid1d((int64_t)p.m * p.n, 256, (int64_t)ctx->num_cus * 8)), dim3(256), 0,
                            ctx->stream, p);
@@ -475,6 +836,7 @@ om_status om_linear_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *xt8, cons
     p.g = g;
     p.x = packed(xt8, in, rows);
     p.rows = rows, p.m = out, p.n = in, p.blocks = (int)blocks8(rows);
+    p.full = out >= 4 ? rows / 128 : rows > 3 ? (rows - 3) / 128 : 0;  // four of fewer columns end up to three rows on
     p.dw = dw, p.db = db, p.acc_dw = acc_dw, p.acc_db = acc_db;
     return dw8(ctx, p);
 }

@@ -101,16 +101,20 @@ __global__ void __launch_bounds__(256) k_ln8(const float *x, const float *__rest
     if (const int64_t b = p.ldq / 128; t < p.lds - b) p.s[row * p.lds + b + t] = 0;
 }
 
-// A workgroup takes `chunk` rows, 4 / NW at a time; every lane keeps the fp64 sums of its own columns and leaves them as one
-// partial row of the workgroup's (added over its wavefronts through LDS in order where several share the columns).
+// A workgroup takes `chunk` rows: sixteen wavefronts a row each (NW = 1; eight past 512 columns, whose sums need the
+// registers), or four to a row (NW = 4). Every lane keeps the
+// fp64 sums of its own columns and leaves them as one partial row of the workgroup's (added over its wavefronts through LDS in
+// order where several share the columns).
+template <int NW, int NV>
+constexpr int kBwdThreads = NW > 1 ? 256 : NV <= 2 ? 1024 : 512;
 template <int NW, int NV, bool ACC>
-__global__ void __launch_bounds__(256) k_ln8_bwd(const float *g, Packed p, const float *__restrict__ gamma,
-                                                 const float *__restrict__ rstd, float *dx, double *part_g, double *part_b,
-                                                 int64_t rows, int64_t cols, int chunk) {
+__global__ void __launch_bounds__(kBwdThreads<NW, NV>) k_ln8_bwd(const float *g, Packed p, const float *__restrict__ gamma,
+                                                             const float *__restrict__ rstd, float *dx, double *part_g,
+                                                             double *part_b, int64_t rows, int64_t cols, int chunk) {
     OM_LDS_POISON();
+    constexpr int L = 64 * NW, WAVES = kBwdThreads<NW, NV> / 64, AT_ONCE = WAVES / NW;
     __shared__ float sh[4];
-    __shared__ double cs[NW == 1 ? 4 * 256 : 1];
-    constexpr int L = 64 * NW;
+    __shared__ double cs[NW == 1 ? WAVES * 256 : 1];
     const int t = threadIdx.x % L, w = threadIdx.x >> 6;
     const int64_t r0 = (int64_t)blockIdx.x * chunk, r1 = min(rows, r0 + chunk);
     double sg[4 * NV], sb[4 * NV];
@@ -122,7 +126,7 @@ __global__ void __launch_bounds__(256) k_ln8_bwd(const float *g, Packed p, const
 #pragma unroll
         for (int e = 0; e < 4; e++) sg[4 * i + e] = sb[4 * i + e] = 0.0;
     }
-    for (int64_t row = r0 + (NW == 1 ? w : 0); row < r1; row += 4 / NW) {
+    for (int64_t row = r0 + (NW == 1 ? w : 0); row < r1; row += AT_ONCE) {
         const float *gr = g + row * cols;
         floatx4 gv[NV], h[NV], old[ACC ? NV : 1];
         uint32_t q[NV];
@@ -167,20 +171,25 @@ __global__ void __launch_bounds__(256) k_ln8_bwd(const float *g, Packed p, const
     }
     auto leave = [&](double *part, const double (&sum)[4 * NV]) {
         if (!part) return;
+        part += (int64_t)blockIdx.x * cols;
 #pragma unroll
         for (int i = 0; i < NV; i++) {
-            if constexpr (NW == 1) {  // the four wavefronts' sums of these 256 columns
+            if constexpr (NW == 1) {  // the wavefronts' sums of these 256 columns: value e of lane t at 64 e + t
                 __syncthreads();
 #pragma unroll
                 for (int e = 0; e < 4; e++) cs[256 * w + 64 * e + t] = sum[4 * i + e];
                 __syncthreads();
-                const int64_t c = 256 * (int64_t)i + 4 * t + w;  // column of lane t's w-th value
-                if (c < cols) part[(int64_t)blockIdx.x * cols + c] =
-                    ((cs[64 * w + t] + cs[256 + 64 * w + t]) + cs[512 + 64 * w + t]) + cs[768 + 64 * w + t];
+                const int64_t c = 256 * (int64_t)i + 4 * t + w;
+                if (w < 4 && c < cols) {
+                    double v = cs[64 * w + t];
+#pragma unroll
+                    for (int k = 1; k < WAVES; k++) v += cs[256 * k + 64 * w + t];
+                    part[c] = v;
+                }
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    if (at(i) + e < cols) part[(int64_t)blockIdx.x * cols + at(i) + e] = sum[4 * i + e];
+                    if (at(i) + e < cols) part[at(i) + e] = sum[4 * i + e];
             }
         }
     };
@@ -254,24 +263,29 @@ __global__ void __launch_bounds__(256) k_ln8_params_long(const float *__restrict
         }
 }
 
-// out[c] (+)= the sum of part[k][c] over the chunks: 64 columns to a workgroup, its four wavefronts take every fourth chunk
-// in turn and their sums are added in order.
-__global__ void __launch_bounds__(256) k_ln8_final(const double *__restrict__ part_g, const double *__restrict__ part_b,
-                                                   float *dgamma, float *dbeta, int chunks, int64_t cols, int acc) {
+// out[c] (+)= the sum of part[k][c] over the chunks: 16 columns (a 128-byte line) to a workgroup, its 64 groups of 16 lanes
+// take every 64th chunk, and the groups' sums are added pairwise in a fixed order.
+__global__ void __launch_bounds__(1024) k_ln8_final(const double *__restrict__ part_g, const double *__restrict__ part_b,
+                                                    float *dgamma, float *dbeta, int chunks, int64_t cols, int acc) {
     OM_LDS_POISON();
-    __shared__ double sh[4][64];
+    __shared__ double sh[64][16];
     const double *part = blockIdx.y ? part_b : part_g;
     float *out = blockIdx.y ? dbeta : dgamma;
-    const int t = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const int64_t c = 64 * (int64_t)blockIdx.x + t;
+    if (!out) return;
+    const int t = threadIdx.x & 15, w = threadIdx.x >> 4;
+    const int64_t c = 16 * (int64_t)blockIdx.x + t;
     double s = 0.0;
-    if (out && c < cols)
-#pragma unroll 8
-        for (int k = w; k < chunks; k += 4) s += part[(int64_t)k * cols + c];
+    if (c < cols)
+#pragma unroll 4
+        for (int k = w; k < chunks; k += 64) s += part[(int64_t)k * cols + c];
     sh[w][t] = s;
-    __syncthreads();
-    if (w == 0 && out && c < cols) {
-        const float v = (float)(((sh[0][t] + sh[1][t]) + sh[2][t]) + sh[3][t]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        __syncthreads();
+        if (w < o) sh[w][t] = s = s + sh[w + o][t];
+    }
+    if (w == 0 && c < cols) {
+        const float v = (float)s;
         out[c] = acc ? out[c] + v : v;
     }
 }
@@ -317,9 +331,9 @@ om_status om_layernorm_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *xh8, c
     if (!dx && !dgamma && !dbeta) return OM_OK;
     OM_REQUIRE(ctx, cols <= 1 << 26, "om_layernorm_bwd_x8: cols=%d is more than a launch takes", cols);
     if (om_status s = om::use_device(ctx)) return s;
-    // chunks of rows: as many as two workgroups a CU, of at least eight rows
+    // chunks of rows: as many as two workgroups a CU, of at least 16 rows
     int chunk = (rows + ctx->num_cus * 2 - 1) / (ctx->num_cus * 2);
-    chunk = chunk < 8 ? 8 : chunk;
+    chunk = chunk < 16 ? 16 : chunk;
     const int chunks = rows ? (rows + chunk - 1) / chunk : 0;
     double *pg = nullptr, *pb = nullptr;
     if (dgamma || dbeta) {
@@ -335,7 +349,7 @@ om_status om_layernorm_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *xh8, c
             constexpr int NW = decltype(nw)::value, NV = decltype(nv)::value;
             if constexpr (NV && 256 * NW * NV <= kKeptBwd) {
                 auto go = [&](auto kern) {
-                    hipLaunchKernelGGL(kern, dim3((unsigned)chunks), dim3(256), 0, ctx->stream, g, p, gamma, rstd, dx, pg, pb,
+                    hipLaunchKernelGGL(kern, dim3((unsigned)chunks), dim3(kBwdThreads<NW, NV>), 0, ctx->stream, g, p, gamma, rstd, dx, pg, pb,
                                        (int64_t)rows, (int64_t)cols, chunk);
                 };
                 acc_dx ? go(k_ln8_bwd<NW, NV, true>) : go(k_ln8_bwd<NW, NV, false>);
@@ -351,7 +365,7 @@ om_status om_layernorm_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *xh8, c
             }
         });
     if (dgamma || dbeta)
-        hipLaunchKernelGGL(k_ln8_final, dim3((unsigned)(((int64_t)cols + 63) / 64), 2), dim3(256), 0, ctx->stream, pg, pb,
+        hipLaunchKernelGGL(k_ln8_final, dim3((unsigned)(((int64_t)cols + 15) / 16), 2), dim3(1024), 0, ctx->stream, pg, pb,
                            dgamma, dbeta, chunks, (int64_t)cols, acc_params);
     return OM_LAUNCH_CHECK(ctx, "om_layernorm_bwd_x8");
 }

@@ -37,9 +37,14 @@ __device__ __forceinline__ uint32_t finite_bits(float x) {
     const uint32_t u = __float_as_uint(x) & 0x7FFFFFFFu;
     return u < 0x7F800000u ? u : 0u;
 }
-__device__ __forceinline__ uint32_t finite_bits4(floatx4 v) {
-    return max(max(finite_bits(v[0]), finite_bits(v[1])), max(finite_bits(v[2]), finite_bits(v[3])));
+// The largest of four. One look for all lanes whether anything is not finite spares the common case the selections.
+__device__ __forceinline__ uint32_t top_of(float a, float b, float c, float d) {
+    auto bits = [](float x) { return __float_as_uint(x) & 0x7FFFFFFFu; };
+    uint32_t u = max(max(bits(a), bits(b)), max(bits(c), bits(d)));
+    if (__any(u >= 0x7F800000u)) u = max(max(finite_bits(a), finite_bits(b)), max(finite_bits(c), finite_bits(d)));
+    return u;
 }
+__device__ __forceinline__ uint32_t finite_bits4(floatx4 v) { return top_of(v[0], v[1], v[2], v[3]); }
 // The scale byte of a block from its largest value's bits. 448 = 1.75 * 2^8: the exponent less 8, one more where the
 // significand is above 1.75 (the sum carries), and 0 where that would be negative.
 __device__ __forceinline__ int scale_byte(uint32_t top) { return max((int)((top + 0x1FFFFFu) >> 23) - 8, 0); }
@@ -55,7 +60,7 @@ __device__ __forceinline__ floatx4 decode4(uint32_t w, float scale) {
     const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
     return floatx4{a[0] * scale, a[1] * scale, b[0] * scale, b[1] * scale};
 }
-// Largest of 32 neighbouring lanes, in all of them: four steps on the vector pipe inside 16 lanes, one across.
+// Largest of 32 neighbouring lanes, in all of them: five steps on the vector pipe, four inside 16 lanes and one across.
 __device__ __forceinline__ uint32_t max32(uint32_t v) {
     auto dpp = [](uint32_t x, auto ctrl) {
         return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xF, 0xF, true);
@@ -64,7 +69,8 @@ __device__ __forceinline__ uint32_t max32(uint32_t v) {
     v = max(v, dpp(v, std::integral_constant<int, 0x4E>()));   // quad_perm [2, 3, 0, 1]
     v = max(v, dpp(v, std::integral_constant<int, 0x141>()));  // row_half_mirror
     v = max(v, dpp(v, std::integral_constant<int, 0x140>()));  // row_mirror
-    return max(v, (uint32_t)__shfl_xor((int)v, 16, 64));
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);  // the other 16 lanes' in one of the two
+    return max(r[0], r[1]);
 }
 
 // Four neighbouring values of a row that ends at `left` more values (any number), zeros behind it.

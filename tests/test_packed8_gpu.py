@@ -243,7 +243,9 @@ def dw_case(dev, rng, rows, inp, out, g):
 
 
 DW = [(1, 1, 1), (2, 3, 5), (37, 20, 33), (127, 64, 64), (128, 128, 128), (129, 130, 257), (300, 77, 40), (1000, 384, 100),
-      (4096, 384, 1536), (2500, 512, 2100), (640, 1000, 333), (64, 2048, 2304)]
+      (4096, 384, 1536), (2500, 512, 2100), (640, 1000, 333), (64, 2048, 2304),
+      # fewer than four columns of g, and rows just past whole blocks
+      (129, 20, 1), (257, 40, 2), (384, 33, 3), (130, 7, 1), (131, 9, 2), (3, 5, 2), (512, 140, 1), (300, 50, 5), (640, 64, 70)]
 
 
 @pytest.mark.parametrize("rows,inp,out", DW)
