@@ -397,6 +397,83 @@ __global__ void __launch_bounds__(256 * KW, KW < 2 ? 2 : KW) k_gemm8_few(Gemm8 p
     }
 }
 
+// At most 16 rows of A: a workgroup computes 16 columns on v_mfma_f32_16x16x32_bf16, its NW wavefronts a share of k each.
+// Each wavefront goes through its blocks of 128 k alone, D of them on their way into its own part of LDS (whole 128-byte rows;
+// loaded straight into fragments, 64 bytes of 16 rows at a time, they take three times as long), so nothing meets before the
+// sums do. Bound: latency, then B's bytes.
+template <int NW, int D>
+__global__ void __launch_bounds__(64 * NW) k_gemm8_thin(Gemm8 p) {
+    OM_LDS_POISON();
+    typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+    constexpr int SLOT = 4096 + 256, LOADS = 5;
+    __shared__ __attribute__((aligned(16))) char sh[NW * D * SLOT];
+    const int lane = threadIdx.x & 63, row = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16;
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int per = (p.blocks + NW - 1) / NW, b0 = wv * per, b1 = min(p.blocks, b0 + per);
+    // Rows and columns past the last one are the last one again; what they give is not stored.
+    uint32_t oa[2], ob[2];
+#pragma unroll
+    for (int i = 0; i < 2; i++) {
+        const int r = 8 * i + (lane >> 3), piece = (lane ^ (r >> 1)) & 7;
+        oa[i] = (uint32_t)min(r, p.m - 1) * (uint32_t)p.a.ldq + 16 * piece;
+        ob[i] = (uint32_t)min(r, p.n - 1 - n0) * (uint32_t)p.b.ldq + 16 * piece;
+    }
+    const uint8_t *qb = p.b.q + (int64_t)n0 * p.b.ldq;
+    // scale dwords: 16 rows of A, then 16 of B, and those again
+    const uint8_t *ss = lane & 16 ? p.b.s + (int64_t)min(n0 + row, p.n - 1) * p.b.lds : p.a.s + (int64_t)min(row, p.m - 1) * p.a.lds;
+    char *mine = sh + wv * D * SLOT;
+    const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)mine;
+    auto issue = [&](int blk) {  // past the last block that one again, into a slot that nothing reads
+        const uint32_t at = base + (uint32_t)((blk - b0) % D) * SLOT;
+        const int k = min(blk, b1 - 1);
+#pragma unroll
+        for (int i = 0; i < 2; i++) {
+            load_to_lds(p.a.q + (int64_t)k * 128, oa[i], at + 1024 * i);
+            load_to_lds(qb + (int64_t)k * 128, ob[i], at + 2048 + 1024 * i);
+        }
+        load_to_lds4(ss + (k & ~3), at + 4096);
+    };
+    floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (b0 < b1) {
+#pragma unroll
+        for (int i = 0; i < D; i++) issue(b0 + i);
+        for (int blk = b0; blk < b1; blk++) {
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * LOADS) : "memory");
+            const char *cur = mine + (blk - b0) % D * SLOT;
+            u32x4 a[2], b[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                a[j] = *reinterpret_cast<const u32x4 *>(cur + piece_at(row, 4 * j + g));
+                b[j] = *reinterpret_cast<const u32x4 *>(cur + 2048 + piece_at(row, 4 * j + g));
+            }
+            const float fa = scale_in(*reinterpret_cast<const uint32_t *>(cur + 4096 + 4 * row), blk);
+            const float fb = scale_in(*reinterpret_cast<const uint32_t *>(cur + 4096 + 64 + 4 * row), blk);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read, so the slot may be loaded again
+            issue(blk + D);
+#pragma unroll
+            for (int j = 0; j < 2; j++)
+#pragma unroll
+                for (int t = 0; t < 2; t++)
+                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                        __builtin_bit_cast(bf16x8, widen8(a[j][2 * t], a[j][2 * t + 1], fa)),
+                        __builtin_bit_cast(bf16x8, widen8(b[j][2 * t], b[j][2 * t + 1], fb)), acc, 0, 0, 0);
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    float *out = reinterpret_cast<float *>(sh);
+#pragma unroll
+    for (int e = 0; e < 4; e++) out[wv * 256 + (4 * g + e) * 16 + row] = acc[e];
+    __syncthreads();
+    const int r = threadIdx.x >> 4, col = n0 + (threadIdx.x & 15);
+    if (r >= p.m || col >= p.n) return;
+    float v = out[threadIdx.x];
+#pragma unroll
+    for (int w = 1; w < NW; w++) v += out[256 * w + threadIdx.x];
+    const Out to(p, 0);
+    to.put(r, col, v, to.bias_of(col));
+}
+
 // Adds the splits' sums in order, then bias and C.
 __global__ void __launch_bounds__(256) k_gemm8_join(Gemm8 p) {
     OM_LDS_POISON();
@@ -414,11 +491,12 @@ __global__ void __launch_bounds__(256) k_gemm8_join(Gemm8 p) {
 
 // A kernel's tile and what its workgroups take, in us, with `resident` of them on a CU at most: `fix` a round of those and
 // `each` a workgroup, and for a stage of kw blocks of k `alone` where a CU has one workgroup, `shared` a workgroup where it
-// has more. Fitted to 8019 (products) and 2674 (weight gradients) times over all kernels, splits of k from 1 to 16 and sizes
-// from 1 to 16384; of all those the choice by them is 0.8 % behind the best in the mean, 21 % at most.
+// has more; with every CU busy the clock falls and the caches fill, and a stage takes `chip` a workgroup and CU. Fitted to 5815
+// (products) and 4611 (weight gradients) times over all kernels, splits of k from 1 to 16 and sizes from 1 to 16384; the
+// choice by them is 0.5 % behind the best of all those in the mean, 26 % at most.
 struct Tile {
     int bm, bn, kw, resident;
-    float fix, each, alone, shared;
+    float fix, each, alone, shared, chip;
 };
 struct Choice {
     int tile, splits;
@@ -428,15 +506,20 @@ template <int N>
 Choice choose(const Tile (&tiles)[N], int cus, int64_t m, int64_t n, int blocks, int64_t row_bytes, float join, float join_each) {
     Choice best = {-1, 1};
     double least = 0.0;
+    // comparisons of one kernel or split: a number that is none of them leaves no choice
+    const char *only_tile = om::tuning_env("OM_TILE8"), *only_splits = om::tuning_env("OM_SPLITS8");
     for (int t = 0; t < N; t++) {
         const Tile &c = tiles[t];
+        if (only_tile && atoi(only_tile) != t) continue;
         if ((c.bm > c.bn ? c.bm : c.bn) * row_bytes > INT64_C(0xFFFFFFFF)) continue;  // offsets inside a tile: 32 bits
         for (int s : {1, 2, 3, 4, 6, 8, 12, 16}) {
             if (s > 1 && blocks < 4 * s) break;
+            if (only_splits && atoi(only_splits) != s) continue;
             const int per = ((blocks + s - 1) / s + c.kw - 1) / c.kw * c.kw, parts = per ? (blocks + per - 1) / per : 1;
             const double wgs = (double)((m + c.bm - 1) / c.bm) * (double)((n + c.bn - 1) / c.bn) * parts;
             const double load = std::ceil(wgs / cus), rounds = std::ceil(load / c.resident), stages = per / c.kw;
-            double us = c.fix * rounds + c.each * load + std::fmax(c.alone * rounds, c.shared * load) * stages;
+            double us = c.fix * rounds + c.each * load +
+                        std::fmax(std::fmax(c.alone * rounds, c.shared * load), c.chip * wgs / cus) * stages;
             if (parts > 1) us += join + join_each * parts * (double)m * (double)n * 1e-6;
             if (best.tile < 0 || us < least) {
                 least = us;
@@ -444,8 +527,6 @@ Choice choose(const Tile (&tiles)[N], int cus, int64_t m, int64_t n, int blocks,
             }
         }
     }
-    if (const char *force = om::tuning_env("OM_TILE8")) best.tile = atoi(force);
-    if (const char *force = om::tuning_env("OM_SPLITS8")) best.splits = atoi(force);
     return best;
 }
 // Blocks of k to a split (whole stages, since a stage's scale bytes are one dword) and the splits that gives.
@@ -454,14 +535,21 @@ inline void split_blocks(int blocks, int kw, int splits, int &per, int &parts) {
     parts = blocks > per ? (blocks + per - 1) / per : 1;
 }
 
-constexpr Tile kTiles[] = {{256, 256, 1, 1, 4.86f, 0.38f, 2.255f, 0.0f},
-                           {128, 128, 1, 2, 0.0f, 2.76f, 0.852f, 0.31f},
-                           {64, 64, 1, 2, 0.24f, 2.2f, 0.305f, 0.24f},
-                           {32, 32, 1, 4, 0.55f, 0.5f, 0.18f, 0.095f},
-                           {32, 32, 2, 2, 0.0f, 1.24f, 0.256f, 0.194f}};
+constexpr Tile kTiles[] = {{256, 256, 1, 1, 8.0f, 0.4f, 2.27f, 0.4f, 3.2f},
+                           {128, 128, 1, 2, 0.0f, 2.0f, 0.856f, 0.45f, 0.86f},
+                           {64, 64, 1, 2, 0.53f, 1.91f, 0.305f, 0.271f, 0.264f},
+                           {32, 32, 1, 4, 0.44f, 0.48f, 0.184f, 0.102f, 0.069f},
+                           {32, 32, 2, 2, 0.0f, 1.26f, 0.246f, 0.203f, 0.201f}};
 
 om_status gemm8(om_ctx *ctx, const char *what, Gemm8 p) {
-    const Choice ch = choose(kTiles, ctx->num_cus, p.m, p.n, p.blocks, p.a.ldq, 2.24f, 1.61f);
+    // Up to 16 rows the thin kernel is the fastest (4 x 4096 x 4096: 5.6 us, the best of the others 8.2) until a wavefront has so
+    // many blocks one after the other that a split of k is worth its second launch (16 x 16 x 16384: 10.5 and 7.8 us).
+    if (p.m <= 16 && p.blocks <= 64) {
+        p.splits = 1;
+        hipLaunchKernelGGL((k_gemm8_thin<4, 4>), dim3((unsigned)(((int64_t)p.n + 15) / 16)), dim3(256), 0, ctx->stream, p);
+        return OM_LAUNCH_CHECK(ctx, what);
+    }
+    const Choice ch = choose(kTiles, ctx->num_cus, p.m, p.n, p.blocks, p.a.ldq, 2.46f, 0.89f);
     OM_REQUIRE(ctx, ch.tile >= 0, "%s: k is more than a launch takes", what);
     const Tile &c = kTiles[ch.tile];
     p.tiles_m = (p.m + c.bm - 1) / c.bm;
@@ -766,12 +854,12 @@ __global__ void __launch_bounds__(256) k_dw8_join(Dw8 p) {
     }
 }
 
-constexpr Tile kTilesDw[] = {{32, 128, 1, 2, 0.0f, 2.96f, 0.795f, 0.335f},
-                             {32, 64, 1, 3, 2.14f, 0.0f, 0.454f, 0.507f},
-                             {32, 32, 1, 2, 1.06f, 0.31f, 0.527f, 0.374f}};
+constexpr Tile kTilesDw[] = {{32, 128, 1, 2, 0.77f, 1.63f, 0.76f, 0.696f, 0.72f},
+                             {32, 64, 1, 3, 0.71f, 0.62f, 0.563f, 0.463f, 0.471f},
+                             {32, 32, 1, 2, 0.0f, 0.84f, 0.523f, 0.38f, 0.375f}};
 
 om_status dw8(om_ctx *ctx, Dw8 p) {
-    const Choice ch = choose(kTilesDw, ctx->num_cus, p.m, p.n, p.blocks, p.x.ldq, 3.45f, 1.66f);
+    const Choice ch = choose(kTilesDw, ctx->num_cus, p.m, p.n, p.blocks, p.x.ldq, 3.44f, 0.71f);
     OM_REQUIRE(ctx, ch.tile >= 0 && p.rows <= INT32_MAX - 255 && p.m < 1 << 26,
                "om_linear_bwd_x8: rows=%d in=%d out=%d is more than a launch takes", p.rows, p.n, p.m);
     const Tile &c = kTilesDw[ch.tile];

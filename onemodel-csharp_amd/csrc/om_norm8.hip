@@ -108,7 +108,7 @@ __global__ void __launch_bounds__(256) k_ln8(const float *x, const float *__rest
 template <int NW, int NV>
 constexpr int kBwdThreads = NW > 1 ? 256 : NV <= 2 ? 1024 : 512;
 template <int NW, int NV, bool ACC>
-__global__ void __launch_bounds__(kBwdThreads<NW, NV>) k_ln8_bwd(const float *g, Packed p, const float *__restrict__ gamma,
+__global__ void __launch_bounds__((kBwdThreads<NW, NV>)) k_ln8_bwd(const float *g, Packed p, const float *__restrict__ gamma,
                                                              const float *__restrict__ rstd, float *dx, double *part_g,
                                                              double *part_b, int64_t rows, int64_t cols, int chunk) {
     OM_LDS_POISON();
@@ -263,33 +263,6 @@ __global__ void __launch_bounds__(256) k_ln8_params_long(const float *__restrict
         }
 }
 
-// out[c] (+)= the sum of part[k][c] over the chunks: 16 columns (a 128-byte line) to a workgroup, its 64 groups of 16 lanes
-// take every 64th chunk, and the groups' sums are added pairwise in a fixed order.
-__global__ void __launch_bounds__(1024) k_ln8_final(const double *__restrict__ part_g, const double *__restrict__ part_b,
-                                                    float *dgamma, float *dbeta, int chunks, int64_t cols, int acc) {
-    OM_LDS_POISON();
-    __shared__ double sh[64][16];
-    const double *part = blockIdx.y ? part_b : part_g;
-    float *out = blockIdx.y ? dbeta : dgamma;
-    if (!out) return;
-    const int t = threadIdx.x & 15, w = threadIdx.x >> 4;
-    const int64_t c = 16 * (int64_t)blockIdx.x + t;
-    double s = 0.0;
-    if (c < cols)
-#pragma unroll 4
-        for (int k = w; k < chunks; k += 64) s += part[(int64_t)k * cols + c];
-    sh[w][t] = s;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        __syncthreads();
-        if (w < o) sh[w][t] = s = s + sh[w + o][t];
-    }
-    if (w == 0 && c < cols) {
-        const float v = (float)s;
-        out[c] = acc ? out[c] + v : v;
-    }
-}
-
 // Columns of a row that stay in registers: the forward keeps the values alone, the backward sums beside them.
 constexpr int64_t kKeptFwd = 16384, kKeptBwd = 8192;
 template <class F>
@@ -364,10 +337,10 @@ om_status om_layernorm_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *xh8, c
                 if (dx) acc_dx ? go(k_ln8_dx_long<true>) : go(k_ln8_dx_long<false>);  // last: dx may be g
             }
         });
-    if (dgamma || dbeta)
-        hipLaunchKernelGGL(k_ln8_final, dim3((unsigned)(((int64_t)cols + 15) / 16), 2), dim3(1024), 0, ctx->stream, pg, pb,
-                           dgamma, dbeta, chunks, (int64_t)cols, acc_params);
-    return OM_LAUNCH_CHECK(ctx, "om_layernorm_bwd_x8");
+    if (om_status s = OM_LAUNCH_CHECK(ctx, "om_layernorm_bwd_x8")) return s;
+    if (dgamma && dbeta) return om::chunk_final(ctx, pg, chunks, cols, dgamma, acc_params, pb, dbeta);
+    if (dgamma) return om::chunk_final(ctx, pg, chunks, cols, dgamma, acc_params);
+    return dbeta ? om::chunk_final(ctx, pb, chunks, cols, dbeta, acc_params) : OM_OK;
 }
 
 }  // extern "C"
