@@ -20,8 +20,7 @@ using namespace om8;
 // before it is written, so calls may follow each other.
 template <int NW, class T>
 __device__ __forceinline__ T row_sum(T v, T *sh) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+    v = wave_sum8(v);
     if constexpr (NW == 1) {
         return v;
     } else {
@@ -45,7 +44,7 @@ __device__ __forceinline__ void put_codes(const Packed &p, int64_t row, int64_t 
 template <int NW, int NV>
 __global__ void __launch_bounds__(256) k_ln8(const float *x, const float *__restrict__ gamma, const float *__restrict__ beta,
                                              float *y, Packed p, float *__restrict__ rstd, int64_t rows, int64_t cols,
-                                             float eps) {
+                                             float eps, double inv_n) {
     OM_LDS_POISON();
     __shared__ double sh[4];
     constexpr int L = 64 * NW, KEEP = NV ? NV : 1;
@@ -73,7 +72,7 @@ __global__ void __launch_bounds__(256) k_ln8(const float *x, const float *__rest
     }
     double sum = 0.0;
     sweep([&](int, floatx4 w) { sum += ((double)w[0] + (double)w[1]) + ((double)w[2] + (double)w[3]); });
-    const double mean = row_sum<NW>(sum, sh) / (double)cols;
+    const double mean = row_sum<NW>(sum, sh) * inv_n;
     double ss = 0.0;
     sweep([&](int i, floatx4 w) {
 #pragma unroll
@@ -82,7 +81,14 @@ __global__ void __launch_bounds__(256) k_ln8(const float *x, const float *__rest
             ss += at(i) + e < cols ? d * d : 0.0;
         }
     });
-    const float r = (float)(1.0 / sqrt(row_sum<NW>(ss, sh) / (double)cols + (double)eps)), m = (float)mean;
+    // 1 / sqrt by the instruction's approximation (about 2^-26) and two Newton steps, 2^-52: the float nearest to it is the
+    // exact value's but where that lies within 2^-28 of a step from a tie. (Zero and what is not finite by the division.)
+    const double var = row_sum<NW>(ss, sh) * inv_n + (double)eps;
+    double root = __builtin_amdgcn_rsq(var);
+#pragma unroll
+    for (int i = 0; i < 2; i++) root = root * __builtin_fma(-0.5 * var * root, root, 1.5);
+    if (!(var > 1e-300 && var < 1e300)) root = 1.0 / sqrt(var);
+    const float r = (float)root, m = (float)mean;
     if (t == 0) rstd[row] = r;
     sweep([&](int i, floatx4 xh) {
         const int64_t c = at(i);
@@ -290,7 +296,7 @@ om_status om_layernorm_fwd_x8(om_ctx *ctx, const float *x, const float *gamma, c
     by_width(cols, kKeptFwd, [&](auto nw, auto nv) {
         constexpr int NW = decltype(nw)::value, NV = decltype(nv)::value;
         hipLaunchKernelGGL((k_ln8<NW, NV>), dim3((unsigned)(((int64_t)rows * NW + 3) / 4)), dim3(256), 0, ctx->stream, x,
-                           gamma, beta, y, p, rstd, (int64_t)rows, (int64_t)cols, eps);
+                           gamma, beta, y, p, rstd, (int64_t)rows, (int64_t)cols, eps, 1.0 / cols);
     });
     return OM_LAUNCH_CHECK(ctx, "om_layernorm_fwd_x8");
 }

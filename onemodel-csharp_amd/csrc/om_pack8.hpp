@@ -8,6 +8,8 @@
 // (to nearest, ties to even) of its value; infinities and NaN become NaN codes.
 #pragma once
 
+#include <type_traits>
+
 #include "om_internal.hpp"
 
 namespace om8 {
@@ -60,17 +62,52 @@ __device__ __forceinline__ floatx4 decode4(uint32_t w, float scale) {
     const auto a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
     return floatx4{a[0] * scale, a[1] * scale, b[0] * scale, b[1] * scale};
 }
+// The value of another lane of the 16 (CTRL: a DPP control).
+template <int CTRL>
+__device__ __forceinline__ uint32_t lane_of16(uint32_t x) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, true);
+}
+constexpr int kSwap1 = 0xB1, kSwap2 = 0x4E, kHalfMirror = 0x141, kMirror = 0x140;  // quad_perm [1,0,3,2], [2,3,0,1]; rows of 16
 // Largest of 32 neighbouring lanes, in all of them: five steps on the vector pipe, four inside 16 lanes and one across.
 __device__ __forceinline__ uint32_t max32(uint32_t v) {
-    auto dpp = [](uint32_t x, auto ctrl) {
-        return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, 0xF, 0xF, true);
-    };
-    v = max(v, dpp(v, std::integral_constant<int, 0xB1>()));   // quad_perm [1, 0, 3, 2]
-    v = max(v, dpp(v, std::integral_constant<int, 0x4E>()));   // quad_perm [2, 3, 0, 1]
-    v = max(v, dpp(v, std::integral_constant<int, 0x141>()));  // row_half_mirror
-    v = max(v, dpp(v, std::integral_constant<int, 0x140>()));  // row_mirror
+    v = max(v, lane_of16<kSwap1>(v));
+    v = max(v, lane_of16<kSwap2>(v));
+    v = max(v, lane_of16<kHalfMirror>(v));
+    v = max(v, lane_of16<kMirror>(v));
     const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);  // the other 16 lanes' in one of the two
     return max(r[0], r[1]);
+}
+// Sum over the wavefront, in all lanes, by the same pairs (through LDS a step takes ten times as long, and a row's statistics
+// are a chain of twelve).
+__device__ __forceinline__ float wave_sum8(float v) {
+    auto add = [](float x, uint32_t o) { return x + __uint_as_float(o); };
+    v = add(v, lane_of16<kSwap1>(__float_as_uint(v)));
+    v = add(v, lane_of16<kSwap2>(__float_as_uint(v)));
+    v = add(v, lane_of16<kHalfMirror>(__float_as_uint(v)));
+    v = add(v, lane_of16<kMirror>(__float_as_uint(v)));
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+__device__ __forceinline__ double wave_sum8(double v) {
+    auto join = [](uint32_t lo, uint32_t hi) { return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo); };
+    auto step = [&](auto ctrl) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        v += join(lane_of16<decltype(ctrl)::value>((uint32_t)u), lane_of16<decltype(ctrl)::value>((uint32_t)(u >> 32)));
+    };
+    step(std::integral_constant<int, kSwap1>());
+    step(std::integral_constant<int, kSwap2>());
+    step(std::integral_constant<int, kHalfMirror>());
+    step(std::integral_constant<int, kMirror>());
+    auto across = [&](auto swap) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, v);
+        const auto lo = swap((uint32_t)u), hi = swap((uint32_t)(u >> 32));
+        v = join(lo[0], hi[0]) + join(lo[1], hi[1]);
+    };
+    across([](uint32_t x) { return __builtin_amdgcn_permlane16_swap(x, x, false, false); });
+    across([](uint32_t x) { return __builtin_amdgcn_permlane32_swap(x, x, false, false); });
+    return v;
 }
 
 // Four neighbouring values of a row that ends at `left` more values (any number), zeros behind it.
