@@ -541,22 +541,24 @@ constexpr Tile kTiles[] = {{256, 256, 1, 1, 8.0f, 0.4f, 2.27f, 0.4f, 3.2f},
                            {32, 32, 1, 4, 0.44f, 0.48f, 0.184f, 0.102f, 0.069f},
                            {32, 32, 2, 2, 0.0f, 1.26f, 0.246f, 0.203f, 0.201f}};
 
-om_status gemm8(om_ctx *ctx, const char *what, Gemm8 p) {
+om_status gemm8(om_ctx *ctx, Gemm8 p) {
     // Up to 16 rows the thin kernel is the fastest (4 x 4096 x 4096: 5.6 us, the best of the others 8.2) until a wavefront has so
     // many blocks one after the other that a split of k is worth its second launch (16 x 16 x 16384: 10.5 and 7.8 us).
     if (p.m <= 16 && p.blocks <= 64) {
+        if (om_status s = om::use_device(ctx)) return s;
         p.splits = 1;
         hipLaunchKernelGGL((k_gemm8_thin<4, 4>), dim3((unsigned)(((int64_t)p.n + 15) / 16)), dim3(256), 0, ctx->stream, p);
-        return OM_LAUNCH_CHECK(ctx, what);
+        return OM_LAUNCH_CHECK(ctx, "om_gemm8");
     }
     const Choice ch = choose(kTiles, ctx->num_cus, p.m, p.n, p.blocks, p.a.ldq, 2.46f, 0.89f);
-    OM_REQUIRE(ctx, ch.tile >= 0, "%s: k is more than a launch takes", what);
+    OM_REQUIRE(ctx, ch.tile >= 0, "om_gemm8: k is more than a launch takes");
     const Tile &c = kTiles[ch.tile];
-    p.tiles_m = (p.m + c.bm - 1) / c.bm;
-    p.tiles_n = (p.n + c.bn - 1) / c.bn;
+    p.tiles_m = (int)(((int64_t)p.m + c.bm - 1) / c.bm);
+    p.tiles_n = (int)(((int64_t)p.n + c.bn - 1) / c.bn);
     split_blocks(p.blocks, c.kw, ch.splits, p.per, p.splits);
     const int64_t wgs = (int64_t)p.tiles_m * p.tiles_n * p.splits;
-    OM_REQUIRE(ctx, wgs <= INT32_MAX, "%s: %d x %d is more than a launch takes", what, p.m, p.n);
+    OM_REQUIRE(ctx, wgs <= INT32_MAX, "om_gemm8: %d x %d is more than a launch takes", p.m, p.n);
+    if (om_status s = om::use_device(ctx)) return s;
     if (p.splits > 1)
         if (om_status s = om::scratch(ctx, sizeof(float) * (uint64_t)p.splits * (uint64_t)p.m * (uint64_t)p.n, &p.ws)) return s;
     auto go = [&](auto kern, int threads) { hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(threads), 0, ctx->stream, p); };
@@ -570,7 +572,7 @@ om_status gemm8(om_ctx *ctx, const char *what, Gemm8 p) {
     if (p.splits > 1)
         hipLaunchKernelGGL(k_gemm8_join, dim3(om::grid1d((int64_t)p.m * p.n, 256, (int64_t)ctx->num_cus * 8)), dim3(256), 0,
                            ctx->stream, p);
-    return OM_LAUNCH_CHECK(ctx, what);
+    return OM_LAUNCH_CHECK(ctx, "om_gemm8");
 }
 
 // ------------------------------------------------------------------------------------------------- weight gradient
@@ -858,23 +860,30 @@ constexpr Tile kTilesDw[] = {{32, 128, 1, 2, 0.77f, 1.63f, 0.76f, 0.696f, 0.72f}
                              {32, 64, 1, 3, 0.71f, 0.62f, 0.563f, 0.463f, 0.471f},
                              {32, 32, 1, 2, 0.0f, 0.84f, 0.523f, 0.38f, 0.375f}};
 
-om_status dw8(om_ctx *ctx, Dw8 p) {
+// Chooses the kernel for p (its tile in `tile`) and fills in the tiles and splits.
+om_status plan_dw8(om_ctx *ctx, Dw8 &p, int &tile) {
     const Choice ch = choose(kTilesDw, ctx->num_cus, p.m, p.n, p.blocks, p.x.ldq, 3.44f, 0.71f);
     OM_REQUIRE(ctx, ch.tile >= 0 && p.rows <= INT32_MAX - 255 && p.m < 1 << 26,
                "om_linear_bwd_x8: rows=%d in=%d out=%d is more than a launch takes", p.rows, p.n, p.m);
-    const Tile &c = kTilesDw[ch.tile];
-    p.tiles_m = (p.m + c.bm - 1) / c.bm;
-    p.tiles_n = (p.n + c.bn - 1) / c.bn;
+    const Tile &c = kTilesDw[tile = ch.tile];
+    p.tiles_m = (int)(((int64_t)p.m + c.bm - 1) / c.bm);
+    p.tiles_n = (int)(((int64_t)p.n + c.bn - 1) / c.bn);
     split_blocks(p.blocks, c.kw, ch.splits, p.per, p.splits);
-    const int64_t wgs = (int64_t)p.tiles_m * p.tiles_n * p.splits;
-    OM_REQUIRE(ctx, wgs <= INT32_MAX, "om_linear_bwd_x8: in=%d out=%d is more than a launch takes", p.n, p.m);
+    OM_REQUIRE(ctx, (int64_t)p.tiles_m * p.tiles_n * p.splits <= INT32_MAX,
+               "om_linear_bwd_x8: in=%d out=%d is more than a launch takes", p.n, p.m);
+    return OM_OK;
+}
+
+om_status dw8(om_ctx *ctx, Dw8 p, int tile) {
     if (p.splits > 1) {
         const uint64_t sums = ((uint64_t)p.splits * p.m * p.n + 1) / 2 * 2;
         if (om_status s = om::scratch(ctx, 4 * sums + 8ull * p.splits * p.m, &p.ws)) return s;
         p.cs = reinterpret_cast<double *>(p.ws + sums);
     }
-    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(256), 0, ctx->stream, p); };
-    switch (ch.tile) {
+    auto go = [&](auto kern) {
+        hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)p.tiles_m * p.tiles_n * p.splits)), dim3(256), 0, ctx->stream, p);
+    };
+    switch (tile) {
         case 0: go(k_dw8<4, 1, 1, 2>); break;
         case 1: go(k_dw8<2, 1, 1, 2>); break;
         default: go(k_dw8<1, 1, 1, 3>); break;
@@ -896,13 +905,12 @@ om_status om_gemm8(om_ctx *ctx, int m, int n, int k, const uint8_t *a8, const ui
     OM_REQUIRE(ctx, aligned16(a8) && aligned16(b8), "om_gemm8: packed tensors start at multiples of 16 bytes");
     if (m == 0 || n == 0) return OM_OK;
     OM_REQUIRE(ctx, c && (k == 0 || (a8 && b8)), "om_gemm8: NULL pointer");
-    if (om_status s = om::use_device(ctx)) return s;
     Gemm8 p = {};
     p.a = packed(a8, m, k);
     p.b = packed(b8, n, k);
     p.m = m, p.n = n, p.blocks = (int)blocks8(k);
     p.bias = bias, p.c = c, p.ldc = ldc, p.acc = acc;
-    return gemm8(ctx, "om_gemm8", p);
+    return gemm8(ctx, p);
 }
 
 om_status om_linear_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *xt8, const float *w, float *dx, float *dw, float *db,
@@ -911,22 +919,27 @@ om_status om_linear_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *xt8, cons
     OM_REQUIRE(ctx, rows >= 0 && in > 0 && out > 0, "om_linear_bwd_x8: rows=%d in=%d out=%d", rows, in, out);
     OM_REQUIRE(ctx, aligned16(xt8), "om_linear_bwd_x8: packed tensors start at multiples of 16 bytes");
     OM_REQUIRE(ctx, rows == 0 || (g && (!dx || w) && (!dw || xt8)), "om_linear_bwd_x8: a needed tensor is NULL");
-    if (om_status s = om::use_device(ctx)) return s;
-    if (rows > 0 && dx)
-        if (om_status s = om_linear_bwd(ctx, g, nullptr, w, dx, nullptr, nullptr, rows, in, out, acc_dx, 0, 0)) return s;
+    if (!dx && !dw && !db) return OM_OK;
     if (rows == 0) {  // empty sums
         if (dw && !acc_dw)
             if (om_status s = om_fill(ctx, dw, 0.0f, (int64_t)in * out)) return s;
         return db && !acc_db ? om_fill(ctx, db, 0.0f, out) : OM_OK;
     }
-    if (!dw) return db ? om_colsum(ctx, g, db, rows, out, acc_db) : OM_OK;
     Dw8 p = {};
-    p.g = g;
-    p.x = packed(xt8, in, rows);
-    p.rows = rows, p.m = out, p.n = in, p.blocks = (int)blocks8(rows);
-    p.full = out >= 4 ? rows / 128 : rows > 3 ? (rows - 3) / 128 : 0;  // four of fewer columns end up to three rows on
-    p.dw = dw, p.db = db, p.acc_dw = acc_dw, p.acc_db = acc_db;
-    return dw8(ctx, p);
+    int tile = 0;
+    if (dw) {
+        p.g = g;
+        p.x = packed(xt8, in, rows);
+        p.rows = rows, p.m = out, p.n = in, p.blocks = (int)blocks8(rows);
+        p.full = out >= 4 ? rows / 128 : rows > 3 ? (rows - 3) / 128 : 0;  // four of fewer columns end up to three rows on
+        p.dw = dw, p.db = db, p.acc_dw = acc_dw, p.acc_db = acc_db;
+        if (om_status s = plan_dw8(ctx, p, tile)) return s;
+    }
+    if (om_status s = om::use_device(ctx)) return s;
+    if (dx)
+        if (om_status s = om_linear_bwd(ctx, g, nullptr, w, dx, nullptr, nullptr, rows, in, out, acc_dx, 0, 0)) return s;
+    if (!dw) return db ? om_colsum(ctx, g, db, rows, out, acc_db) : OM_OK;
+    return dw8(ctx, p, tile);
 }
 
 }  // extern "C"
