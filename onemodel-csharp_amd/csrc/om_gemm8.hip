@@ -545,6 +545,7 @@ om_status gemm8(om_ctx *ctx, Gemm8 p) {
     // Up to 16 rows the thin kernel is the fastest (4 x 4096 x 4096: 5.6 us, the best of the others 8.2) until a wavefront has so
     // many blocks one after the other that a split of k is worth its second launch (16 x 16 x 16384: 10.5 and 7.8 us).
     if (p.m <= 16 && p.blocks <= 64) {
+        OM_REQUIRE(ctx, launches(((int64_t)p.n + 15) / 16, 256), "om_gemm8: n=%d is more than a launch takes", p.n);
         if (om_status s = om::use_device(ctx)) return s;
         p.splits = 1;
         hipLaunchKernelGGL((k_gemm8_thin<4, 4>), dim3((unsigned)(((int64_t)p.n + 15) / 16)), dim3(256), 0, ctx->stream, p);
@@ -557,17 +558,18 @@ om_status gemm8(om_ctx *ctx, Gemm8 p) {
     p.tiles_n = (int)(((int64_t)p.n + c.bn - 1) / c.bn);
     split_blocks(p.blocks, c.kw, ch.splits, p.per, p.splits);
     const int64_t wgs = (int64_t)p.tiles_m * p.tiles_n * p.splits;
-    OM_REQUIRE(ctx, wgs <= INT32_MAX, "om_gemm8: %d x %d is more than a launch takes", p.m, p.n);
+    const int threads = ch.tile == 0 || ch.tile == 4 ? 512 : 256;
+    OM_REQUIRE(ctx, launches(wgs, threads), "om_gemm8: %d x %d is more than a launch takes", p.m, p.n);
     if (om_status s = om::use_device(ctx)) return s;
     if (p.splits > 1)
         if (om_status s = om::scratch(ctx, sizeof(float) * (uint64_t)p.splits * (uint64_t)p.m * (uint64_t)p.n, &p.ws)) return s;
-    auto go = [&](auto kern, int threads) { hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(threads), 0, ctx->stream, p); };
+    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(threads), 0, ctx->stream, p); };
     switch (ch.tile) {
-        case 0: go(k_gemm8<256, 256, 2, 4>, 512); break;
-        case 1: go(k_gemm8<128, 128, 2, 2>, 256); break;
-        case 2: go(k_gemm8_few<64, 64, 1, 3>, 256); break;
-        case 3: go(k_gemm8_few<32, 32, 1, 4>, 256); break;
-        default: go(k_gemm8_few<32, 32, 2, 4>, 512); break;
+        case 0: go(k_gemm8<256, 256, 2, 4>); break;
+        case 1: go(k_gemm8<128, 128, 2, 2>); break;
+        case 2: go(k_gemm8_few<64, 64, 1, 3>); break;
+        case 3: go(k_gemm8_few<32, 32, 1, 4>); break;
+        default: go(k_gemm8_few<32, 32, 2, 4>); break;
     }
     if (p.splits > 1)
         hipLaunchKernelGGL(k_gemm8_join, dim3(om::grid1d((int64_t)p.m * p.n, 256, (int64_t)ctx->num_cus * 8)), dim3(256), 0,
@@ -869,7 +871,7 @@ om_status plan_dw8(om_ctx *ctx, Dw8 &p, int &tile) {
     p.tiles_m = (int)(((int64_t)p.m + c.bm - 1) / c.bm);
     p.tiles_n = (int)(((int64_t)p.n + c.bn - 1) / c.bn);
     split_blocks(p.blocks, c.kw, ch.splits, p.per, p.splits);
-    OM_REQUIRE(ctx, (int64_t)p.tiles_m * p.tiles_n * p.splits <= INT32_MAX,
+    OM_REQUIRE(ctx, launches((int64_t)p.tiles_m * p.tiles_n * p.splits, 256),
                "om_linear_bwd_x8: in=%d out=%d is more than a launch takes", p.n, p.m);
     return OM_OK;
 }

@@ -169,7 +169,7 @@ inline hipStream_t cur_stream(const om_ctx *ctx) { return ctx->stream; }
 om_status readback_target(om_ctx *ctx, om_readback *r, uint64_t bytes, char **dst, uint64_t **seq_at, uint64_t *seq,
                           const uint64_t **seq_dev);
 void readback_posted(om_readback *r, uint64_t seq, uint64_t bytes);
-// out[col] (+)= (float) sum over c < chunks of part[c * cols + col], in double, a wavefront per column; a second
+// out[col] (+)= (float) sum over c < chunks of part[c * cols + col], in double; a second
 // (part2, out2) pair of the same shape is reduced in the same launch when given.
 om_status chunk_final(om_ctx *ctx, const double *part, int chunks, int cols, float *out, int acc,
                       const double *part2 = nullptr, float *out2 = nullptr);

@@ -270,7 +270,7 @@ __global__ void __launch_bounds__(256) k_ln8_params_long(const float *__restrict
 }
 
 // Columns of a row that stay in registers: the forward keeps the values alone, the backward sums beside them.
-constexpr int64_t kKeptFwd = 16384, kKeptBwd = 8192;
+constexpr int64_t kKeptFwd = 16384, kKeptBwd = 8192, kOneWave = 1024;  // kOneWave: a wavefront to a row
 template <class F>
 void by_width(int64_t cols, int64_t kept, F f) {
     if (cols > kept) return f(std::integral_constant<int, 4>(), std::integral_constant<int, 0>());
@@ -291,6 +291,8 @@ om_status om_layernorm_fwd_x8(om_ctx *ctx, const float *x, const float *gamma, c
     OM_REQUIRE(ctx, aligned16(xh8), "om_layernorm_fwd_x8: packed tensors start at multiples of 16 bytes");
     if (rows == 0) return OM_OK;
     OM_REQUIRE(ctx, x && gamma && beta && y && xh8 && rstd, "om_layernorm_fwd_x8: NULL pointer");
+    OM_REQUIRE(ctx, launches(cols <= kOneWave ? ((int64_t)rows + 3) / 4 : rows, 256),
+               "om_layernorm_fwd_x8: %d x %d is more than a launch takes", rows, cols);
     if (om_status s = om::use_device(ctx)) return s;
     const Packed p = packed(xh8, rows, cols);
     by_width(cols, kKeptFwd, [&](auto nw, auto nv) {
@@ -308,12 +310,12 @@ om_status om_layernorm_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *xh8, c
     OM_REQUIRE(ctx, aligned16(xh8), "om_layernorm_bwd_x8: packed tensors start at multiples of 16 bytes");
     OM_REQUIRE(ctx, rows == 0 || (g && xh8 && gamma && rstd), "om_layernorm_bwd_x8: NULL pointer");
     if (!dx && !dgamma && !dbeta) return OM_OK;
-    OM_REQUIRE(ctx, cols <= 1 << 26, "om_layernorm_bwd_x8: cols=%d is more than a launch takes", cols);
+    OM_REQUIRE(ctx, cols <= 65535 * 1024 && (cols <= kKeptBwd || launches(rows, 256)),
+               "om_layernorm_bwd_x8: %d x %d is more than a launch takes", rows, cols);
     if (om_status s = om::use_device(ctx)) return s;
     // chunks of rows: as many as two workgroups a CU, of at least 16 rows
-    int chunk = (rows + ctx->num_cus * 2 - 1) / (ctx->num_cus * 2);
-    chunk = chunk < 16 ? 16 : chunk;
-    const int chunks = rows ? (rows + chunk - 1) / chunk : 0;
+    const int64_t most = 2 * (int64_t)ctx->num_cus, even = (rows + most - 1) / most;
+    const int chunk = even < 16 ? 16 : (int)even, chunks = (int)(((int64_t)rows + chunk - 1) / chunk);
     double *pg = nullptr, *pb = nullptr;
     if (dgamma || dbeta) {
         float *scr;

@@ -213,12 +213,14 @@ __global__ void __launch_bounds__(kThreads) k_gelu8_bwd(const float *g, Packed p
                     });
 }
 
-// Calls f(whether the tensor is one block wide, grid) for a walk over [rows, cols].
-constexpr int64_t kMostBlocks = INT32_MAX;
+// Workgroups of a walk over [rows, cols]; f(whether the tensor is one block wide, grid) for it.
+int64_t walk_groups(int64_t rows, int64_t blocks) {
+    const int64_t items = blocks == 1 ? (rows + 1) / 2 : rows * ((blocks + 1) / 2), per = kThreads / 64 * kUnroll;
+    return (items + per - 1) / per;
+}
 template <class F>
 void walk(int64_t rows, int64_t blocks, F f) {
-    const int64_t items = blocks == 1 ? (rows + 1) / 2 : rows * ((blocks + 1) / 2);
-    const dim3 grid(om::grid1d(items, kThreads / 64 * kUnroll, INT32_MAX));
+    const dim3 grid((unsigned)walk_groups(rows, blocks));
     blocks == 1 ? f(std::true_type(), grid) : f(std::false_type(), grid);
 }
 
@@ -236,7 +238,8 @@ om_status om_pack8(om_ctx *ctx, const float *x, int ld_x, int rows, int cols, ui
     if (rows == 0 || cols == 0) return OM_OK;
     OM_REQUIRE(ctx, x, "om_pack8: NULL x");
     const int64_t rb = blocks8(rows), cb = blocks8(cols);
-    OM_REQUIRE(ctx, (xt8 ? rb : (int64_t)rows) * cb <= kMostBlocks, "om_pack8: %d x %d is more than a launch takes", rows, cols);
+    OM_REQUIRE(ctx, xt8 ? launches(rb * cb, kTile) : launches(walk_groups(rows, cb), kThreads),
+               "om_pack8: %d x %d is more than a launch takes", rows, cols);
     if (om_status s = om::use_device(ctx)) return s;
     const Packed p = packed(x8, rows, cols), t = packed(xt8, cols, rows);
     if (!xt8)
@@ -260,7 +263,8 @@ om_status om_unpack8(om_ctx *ctx, const uint8_t *x8, float *y, int ld_y, int row
     if (rows == 0 || cols == 0) return OM_OK;
     OM_REQUIRE(ctx, x8 && y, "om_unpack8: NULL pointer");
     const int64_t cb = blocks8(cols);
-    OM_REQUIRE(ctx, rows * cb <= kMostBlocks, "om_unpack8: %d x %d is more than a launch takes", rows, cols);
+    OM_REQUIRE(ctx, launches(walk_groups(rows, cb), kThreads), "om_unpack8: %d x %d is more than a launch takes", rows,
+               cols);
     if (om_status s = om::use_device(ctx)) return s;
     const Packed p = packed(x8, rows, cols);
     walk(rows, cb, [&](auto pair, dim3 grid) {
@@ -281,7 +285,8 @@ om_status om_gelu_fwd_x8(om_ctx *ctx, const float *x, float *y, uint8_t *x8, int
     if (rows == 0 || cols == 0) return OM_OK;
     OM_REQUIRE(ctx, x && y && x8, "om_gelu_fwd_x8: NULL pointer");
     const int64_t cb = blocks8(cols);
-    OM_REQUIRE(ctx, rows * cb <= kMostBlocks, "om_gelu_fwd_x8: %d x %d is more than a launch takes", rows, cols);
+    OM_REQUIRE(ctx, launches(walk_groups(rows, cb), kThreads), "om_gelu_fwd_x8: %d x %d is more than a launch takes", rows,
+               cols);
     if (om_status s = om::use_device(ctx)) return s;
     walk(rows, cb, [&](auto pair, dim3 grid) {
         constexpr bool P = decltype(pair)::value;
@@ -301,7 +306,8 @@ om_status om_gelu_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *x8, float *
     if (rows == 0 || cols == 0) return OM_OK;
     OM_REQUIRE(ctx, g && x8 && dx, "om_gelu_bwd_x8: NULL pointer");
     const int64_t cb = blocks8(cols);
-    OM_REQUIRE(ctx, rows * cb <= kMostBlocks, "om_gelu_bwd_x8: %d x %d is more than a launch takes", rows, cols);
+    OM_REQUIRE(ctx, launches(walk_groups(rows, cb), kThreads), "om_gelu_bwd_x8: %d x %d is more than a launch takes", rows,
+               cols);
     if (om_status s = om::use_device(ctx)) return s;
     walk(rows, cb, [&](auto pair, dim3 grid) {
         constexpr bool P = decltype(pair)::value;

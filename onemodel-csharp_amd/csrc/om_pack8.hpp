@@ -28,6 +28,8 @@ inline Packed packed(const uint8_t *p, int64_t rows, int64_t cols) {
     uint8_t *q = const_cast<uint8_t *>(p);
     return Packed{q, q ? q + rows * stride8(cols) : nullptr, stride8(cols), scales8(cols)};
 }
+// A launch takes fewer than 2^32 threads.
+inline bool launches(int64_t groups, int threads) { return groups <= INT64_C(0xFFFFFFFF) / threads; }
 inline bool aligned16(const void *p) { return ((uintptr_t)p & 15) == 0; }
 
 typedef float floatx4 __attribute__((ext_vector_type(4)));

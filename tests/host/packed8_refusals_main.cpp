@@ -28,6 +28,9 @@ int main() {
     say("pack-align-t", om_pack8(&ctx, x, 8, 1, 8, nullptr, off));
     say("pack-many", om_pack8(&ctx, x, big, big, big, q, nullptr));
     say("pack-many-t", om_pack8(&ctx, x, big, big, big, nullptr, q));
+    // one column (packed 128 bytes wide), 2^28 rows: past 2^32 threads, as is the transpose of 2^29
+    say("pack-narrow", om_pack8(&ctx, x, 1, (1 << 28) + 1, 1, q, nullptr));
+    say("pack-narrow-t", om_pack8(&ctx, x, 1, 1 << 29, 1, nullptr, q));
     say("ok-pack-no-rows", om_pack8(&ctx, nullptr, 8, 0, 8, q, q));
     say("ok-pack-no-cols", om_pack8(&ctx, nullptr, 8, 8, 0, q, nullptr));
 
@@ -37,6 +40,7 @@ int main() {
     say("unpack-y", om_unpack8(&ctx, q, nullptr, 8, 1, 8, 0));
     say("unpack-align", om_unpack8(&ctx, off, x, 8, 1, 8, 0));
     say("unpack-many", om_unpack8(&ctx, q, x, big, big, big, 0));
+    say("unpack-narrow", om_unpack8(&ctx, q, x, 1, (1 << 28) + 1, 1, 0));
     say("ok-unpack-no-rows", om_unpack8(&ctx, nullptr, nullptr, 8, 0, 8, 1));
 
     say("gemm-m", om_gemm8(&ctx, -1, 4, 4, q, q, nullptr, x, 4, 0));
@@ -50,6 +54,8 @@ int main() {
     say("gemm-align-b", om_gemm8(&ctx, 4, 4, 4, q, off, nullptr, x, 4, 0));
     say("gemm-long", om_gemm8(&ctx, 40, 40, big, q, q, nullptr, x, 40, 0));
     say("gemm-wide", om_gemm8(&ctx, big, big, 1 << 20, q, q, nullptr, x, big, 0));
+    say("gemm-thin", om_gemm8(&ctx, 1, 1 << 28, 128, q, q, nullptr, x, 1 << 28, 0));
+    say("gemm-tiles", om_gemm8(&ctx, 20, 1 << 30, 128, q, q, nullptr, x, 1 << 30, 0));
     say("ok-gemm-no-rows", om_gemm8(&ctx, 0, 4, 4, nullptr, nullptr, nullptr, nullptr, 4, 0));
     say("ok-gemm-no-columns", om_gemm8(&ctx, 4, 0, 4, nullptr, nullptr, nullptr, nullptr, 4, 0));
 
@@ -69,6 +75,8 @@ int main() {
     say("gelu-null", om_gelu_fwd_x8(&ctx, x, x, nullptr, 1, 8));
     say("gelu-align", om_gelu_fwd_x8(&ctx, x, x, off, 1, 8));
     say("gelu-many", om_gelu_fwd_x8(&ctx, x, x, q, big, big));
+    say("gelu-narrow", om_gelu_fwd_x8(&ctx, x, x, q, (1 << 28) + 1, 1));
+    say("gelu-bwd-narrow", om_gelu_bwd_x8(&ctx, x, q, x, (1 << 28) + 1, 1, 0));
     say("gelu-bwd-null", om_gelu_bwd_x8(&ctx, nullptr, q, x, 1, 8, 0));
     say("gelu-bwd-align", om_gelu_bwd_x8(&ctx, x, off, x, 1, 8, 0));
     say("gelu-bwd-many", om_gelu_bwd_x8(&ctx, x, q, x, big, big, 0));
@@ -79,6 +87,9 @@ int main() {
     say("norm-cols", om_layernorm_fwd_x8(&ctx, x, x, x, x, q, x, 1, 0, 1e-5f));
     say("norm-null", om_layernorm_fwd_x8(&ctx, x, x, nullptr, x, q, x, 1, 8, 1e-5f));
     say("norm-align", om_layernorm_fwd_x8(&ctx, x, x, x, x, off, x, 1, 8, 1e-5f));
+    say("norm-many", om_layernorm_fwd_x8(&ctx, x, x, x, x, q, x, 1 << 26, 8, 1e-5f));
+    say("norm-many-wide", om_layernorm_fwd_x8(&ctx, x, x, x, x, q, x, 1 << 24, 1025, 1e-5f));
+    say("norm-bwd-many-wide", om_layernorm_bwd_x8(&ctx, x, q, x, x, x, x, x, 1 << 24, 8193, 0, 0));
     say("norm-bwd-cols", om_layernorm_bwd_x8(&ctx, x, q, x, x, x, x, x, 1, 0, 0, 0));
     say("norm-bwd-null", om_layernorm_bwd_x8(&ctx, x, nullptr, x, x, x, x, x, 1, 8, 0, 0));
     say("norm-bwd-align", om_layernorm_bwd_x8(&ctx, x, off, x, x, x, x, x, 1, 8, 0, 0));

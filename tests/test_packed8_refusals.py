@@ -25,7 +25,7 @@ def test_refusals(tmp_path):
     subprocess.run([hipcc, "-x", "hip", "--offload-arch=gfx950", "-std=c++17", "-O1", "-Wno-unused-result", MAIN, "-o", exe,
                     "-L", LIB, "-lom_hip", "-Wl,-rpath," + LIB], check=True, capture_output=True)
     out = subprocess.run([exe], check=True, capture_output=True, text=True, timeout=60).stdout.splitlines()
-    assert len(out) == 62, len(out)
+    assert len(out) == 72, len(out)
     for line in out:
         name, status, message = (line.split(" ", 2) + [""])[:3]
         assert "DEVICE" not in line
