@@ -92,7 +92,6 @@ def test_pack_special_values(dev):
     dev.call("om_pack8", X, 128, len(rows), 128, a, t)
     check_packed(read_packed(dev, a, *x.shape), x)
     check_packed(read_packed(dev, t, *x.shape[::-1]), np.ascontiguousarray(x.T))
-    assert np.array_equal(P.encode(x[:6]), P.encode(x[:6]))
     Y = dev.empty(x.shape)
     dev.call("om_unpack8", a, Y, 128, len(rows), 128, 0)
     assert np.array_equal(dev.get(Y), P.value(x).astype(np.float32), equal_nan=True)
@@ -151,7 +150,10 @@ def sum_bound(k, mag, extra=4):
 
 PRODUCTS = [(1, 1, 1), (3, 5, 7), (1, 300, 1000), (8, 70, 129), (16, 16, 4096), (17, 33, 640), (40, 100, 2000), (64, 64, 256),
             (65, 64, 128), (100, 130, 50), (128, 128, 128), (129, 257, 384), (300, 260, 1100), (512, 512, 513),
-            (1536, 384, 4096), (700, 900, 300), (2100, 2050, 130), (4096, 4100, 128)]
+            (1536, 384, 4096), (700, 900, 300), (2100, 2050, 130), (4096, 4100, 128),
+            # every tile with k in one part and in several
+            (777, 1000, 100), (9, 40, 9000), (17, 20, 5000), (17, 20, 16500), (33, 1537, 16500), (500, 2050, 2600),
+            (260, 1000, 9000), (70, 1000, 5000), (3503, 3501, 300)]
 
 
 @pytest.mark.parametrize("m,n,k", PRODUCTS)
@@ -245,7 +247,9 @@ def dw_case(dev, rng, rows, inp, out, g):
 DW = [(1, 1, 1), (2, 3, 5), (37, 20, 33), (127, 64, 64), (128, 128, 128), (129, 130, 257), (300, 77, 40), (1000, 384, 100),
       (4096, 384, 1536), (2500, 512, 2100), (640, 1000, 333), (64, 2048, 2304),
       # fewer than four columns of g, and rows just past whole blocks
-      (129, 20, 1), (257, 40, 2), (384, 33, 3), (130, 7, 1), (131, 9, 2), (3, 5, 2), (512, 140, 1), (300, 50, 5), (640, 64, 70)]
+      (129, 20, 1), (257, 40, 2), (384, 33, 3), (130, 7, 1), (131, 9, 2), (3, 5, 2), (512, 140, 1), (300, 50, 5), (640, 64, 70),
+      # every tile with the rows in one part and in several, the last of them short
+      (100, 1537, 1000), (2600, 260, 777), (5003, 777, 130), (9001, 130, 130), (5003, 1, 1), (9001, 260, 33), (9001, 33, 2)]
 
 
 @pytest.mark.parametrize("rows,inp,out", DW)
@@ -573,3 +577,122 @@ def test_two_contexts_at_once():
     ra, rb = A.read(), B.read()
     for k in Block.NAMES:
         assert np.array_equal(ra[k], wa[k]) and np.array_equal(rb[k], wb[k])
+
+
+# -------------------------------------------------------------------------------------------------- past 32-bit offsets
+class At:
+    """A place inside a device buffer."""
+
+    def __init__(self, buf, offset):
+        self.p = buf.data_ptr() + offset
+
+    def data_ptr(self):
+        return self.p
+
+
+def test_rows_far_apart(dev):
+    """Leading dimensions whose rows start past 2^32 values: what lies between them is not touched."""
+    rng = np.random.default_rng(12)
+    rows, cols, ld = 5, 200, 1 << 30
+    x = rng.normal(size=(rows, cols)).astype(np.float32)
+    X = dev.empty(((rows - 1) * ld + cols + 8,))
+    place = [At(X, 4 * r * ld) for r in range(rows)]
+    line = dev.empty((cols + 8,))
+
+    def row(r):
+        dev.call("om_copy", line, place[r], 4 * (cols + 8))
+        return dev.get(line)
+
+    for r in range(rows):
+        dev.call("om_fill", place[r], 9.0, cols + 8)
+        dev.call("om_copy", place[r], dev.put(x[r]), 4 * cols)
+    a, t = packed_buf(dev, rows, cols), packed_buf(dev, cols, rows)
+    dev.call("om_pack8", X, ld, rows, cols, a, t)
+    check_packed(read_packed(dev, a, rows, cols), x)
+    check_packed(read_packed(dev, t, cols, rows), np.ascontiguousarray(x.T))
+    dev.call("om_pack8", X, ld, rows, cols, a, None)
+    check_packed(read_packed(dev, a, rows, cols), x)
+    dev.call("om_unpack8", a, X, ld, rows, cols, 1)
+    v = P.value(x)
+    for r in range(rows):
+        assert np.array_equal(row(r), np.concatenate([x[r] + v[r].astype(np.float32), np.full(8, 9.0, np.float32)]))
+    B, bv = put_packed(dev, rng.normal(size=(cols, cols)).astype(np.float32))
+    dev.call("om_gemm8", rows, cols, cols, a, B, None, X, ld, 0)
+    for r in range(rows):
+        got = row(r)
+        assert (np.abs(got[:cols] - v[r] @ bv.T) <= sum_bound(cols, np.abs(v[r]) @ np.abs(bv).T)).all() and (got[cols:] == 9.0).all()
+
+
+def test_tensors_past_32_bits(dev):
+    """[66000, 65600]: more than 2^32 values, and codes past 2^32 bytes; the last rows are looked at."""
+    rng = np.random.default_rng(13)
+    rows, cols, n = 66000, 65600, 2
+    X, Q = dev.empty((rows, cols)), dev.empty((P.nbytes(rows, cols),), np.uint8)
+    x = rng.normal(size=(n, cols)).astype(np.float32)
+    last = At(X, 4 * (rows - n) * cols)
+    line = dev.empty((n, cols))
+
+    def fresh():
+        dev.call("om_fill", X, 1.0, rows * cols)
+        dev.call("om_copy", last, dev.put(x), 4 * n * cols)
+
+    def lines():
+        dev.call("om_copy", line, last, 4 * n * cols)
+        return dev.get(line)
+
+    def check_last():
+        S, T = P.strides(cols)
+        raw = dev.empty((n * (S + T),), np.uint8)
+        dev.call("om_copy", raw, At(Q, (rows - n) * S), n * S)
+        dev.call("om_copy", At(raw, n * S), At(Q, rows * S + (rows - n) * T), n * T)
+        return dev.get(raw)
+
+    fresh()
+    dev.call("om_pack8", X, cols, rows, cols, Q, None)
+    check_packed(check_last(), x)
+    dev.call("om_fill", X, 0.0, rows * cols)
+    dev.call("om_unpack8", Q, X, cols, rows, cols, 0)
+    v = P.value(x)
+    assert np.array_equal(lines(), v.astype(np.float32))
+
+    def beside(m, f=lambda u: u):  # m times rows of ones and then f of the last rows' values
+        return np.concatenate([np.repeat(m.sum(1)[:, None], rows - n, 1), m @ f(v).T], 1)
+
+    # as the second operand of a product, and as the packed input of a weight gradient
+    a = rng.normal(size=(20, cols)).astype(np.float32)
+    A, av = put_packed(dev, a)
+    Y = dev.empty((20, rows))
+    dev.call("om_gemm8", 20, rows, cols, A, Q, None, Y, rows, 0)
+    assert (np.abs(dev.get(Y) - beside(av)) <= sum_bound(cols, beside(np.abs(av), np.abs))).all()
+    g = rng.normal(size=(cols, 5)).astype(np.float32)
+    D = dev.empty((5, rows))
+    dev.call("om_linear_bwd_x8", dev.put(g), Q, None, None, D, None, cols, rows, 5, 0, 0, 0)
+    gd = g.astype(np.float64).T
+    assert (np.abs(dev.get(D) - beside(gd)) <= 3 * sum_bound(cols, beside(np.abs(gd), np.abs))).all()
+    # as many rows of a product, far into C
+    Z = dev.empty((rows, 70))
+    dev.call("om_gemm8", rows, 20, cols, Q, A, None, Z, 70, 0)
+    assert (np.abs(dev.get(Z)[:, :20].T - beside(av)) <= sum_bound(cols, beside(np.abs(av), np.abs))).all()
+    # GELU, in place, there and back
+    fresh()
+    Y1, L1 = dev.empty((n, cols)), dev.put(x)
+    dev.call("om_gelu_fwd", L1, Y1, n * cols)
+    dev.call("om_gelu_fwd_x8", X, X, Q, rows, cols)
+    assert np.array_equal(lines(), dev.get(Y1))
+    check_packed(check_last(), x)
+    fresh()
+    dev.call("om_gelu_bwd", L1, dev.put(v.astype(np.float32)), Y1, n * cols, 0)
+    dev.call("om_gelu_bwd_x8", X, Q, X, rows, cols, 0)
+    assert np.array_equal(lines(), dev.get(Y1))
+    # LayerNorm the same way: the last rows' bits are those of these rows alone
+    fresh()
+    ga, be = (rng.normal(size=cols).astype(np.float32) for _ in range(2))
+    GA, BE, R, R1, Q1 = dev.put(ga), dev.put(be), dev.empty((rows,)), dev.empty((n,)), packed_buf(dev, n, cols, 0)
+    dev.call("om_layernorm_fwd_x8", L1, GA, BE, Y1, Q1, R1, n, cols, 1e-5)
+    dev.call("om_layernorm_fwd_x8", X, GA, BE, X, Q, R, rows, cols, 1e-5)
+    assert np.array_equal(lines(), dev.get(Y1)) and np.array_equal(dev.get(R)[-n:], dev.get(R1))
+    assert np.array_equal(check_last(), dev.get(Q1))
+    fresh()
+    dev.call("om_layernorm_bwd_x8", L1, Q1, GA, R1, Y1, None, None, n, cols, 0, 0)
+    dev.call("om_layernorm_bwd_x8", X, Q, GA, R, X, None, None, rows, cols, 0, 0)
+    assert np.array_equal(lines(), dev.get(Y1))
