@@ -330,6 +330,22 @@ def test_weight_gradient_of_infinities_and_extremes(dev, rows, inp, out):
     assert (np.abs(got[rest] - want) <= lim).all()
 
 
+# column sums in one launch and in two, by single columns and by four
+@pytest.mark.parametrize("rows,cols", [(1, 1), (64, 300), (65, 17), (777, 333), (1024, 2048), (1025, 130), (1023, 2052), (64, 8193),
+                                       (4097, 768), (70, 16001)])
+def test_column_sums(dev, rows, cols):
+    rng = np.random.default_rng(rows + cols)
+    g, old = wide(rng, (rows, cols), -4, 4), rng.normal(size=cols).astype(np.float32)
+    want, size = g.astype(np.float64).sum(0), np.abs(g.astype(np.float64)).sum(0)
+    G = dev.put(g)
+    for acc in (0, 1):
+        B = dev.put(old)
+        dev.call("om_colsum", G, B, rows, cols, acc)
+        # a double sum rounded once, and one more addition where the old value is kept
+        ref = want + acc * old.astype(np.float64)
+        assert (np.abs(dev.get(B) - ref) <= EPS * (np.abs(ref) + acc * np.abs(want)) * 1.01 + 1e-14 * size).all()
+
+
 # ------------------------------------------------------------------------------------------------- GELU and LayerNorm
 @pytest.mark.parametrize("mode", [0, 1])
 @pytest.mark.parametrize("rows,cols", [(1, 1), (3, 130), (64, 256), (33, 1000), (700, 77), (5, 4096)])
