@@ -108,7 +108,7 @@ struct Stage {
     }
     // The scale dword that holds block blk's byte, of every row.
     __device__ __forceinline__ void load_scales(int blk, uint32_t lds, int wv) const {
-        if (wv < ROWS / 64) load_to_lds4(s + (blk & ~3), soff, lds + wv * 256);
+        if (wv < (ROWS + 63) / 64) load_to_lds4(s + (blk & ~3), soff, lds + wv * 256);
     }
 };
 
@@ -159,13 +159,15 @@ struct Out {
 };
 
 // A workgroup of WM x WN wavefronts computes BM x BN of C in stages of 128 k, two of them in LDS: the next one's loads are
-// issued as the current one begins. A lane's 16-byte piece g + 2 j (g = lane / 32) of a row feeds two MFMAs, which so see
+// issued as the current one begins. Products of few stages gain from more and smaller workgroups on a CU, not from more stages
+// in LDS (4096 x 1536 x 384: 128 x 64 with two stages and three workgroups a CU 11.3 us, with three and two 13.5, with six and
+// one 18.9). A lane's 16-byte piece g + 2 j (g = lane / 32) of a row feeds two MFMAs, which so see
 // k = 32 j + 16 g + 8 t + e in place of their own order, alike for both operands.
-template <int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(64 * WM * WN, 2) k_gemm8(Gemm8 p) {
+template <int BM, int BN, int WM, int WN, int WAVES>
+__global__ void __launch_bounds__(64 * WM * WN, WAVES) k_gemm8(Gemm8 p) {
     OM_LDS_POISON();
     constexpr int NW = WM * WN, MT = BM / WM / 32, NT = BN / WN / 32;
-    constexpr int STAGE = (BM + BN) * 132, AS = BM * 128, BS = AS + BN * 128, SS = BS + BM * 4;
+    constexpr int AS = BM * 128, BS = AS + BN * 128, SS = BS + (BM + 63) / 64 * 256, STAGE = SS + (BN + 63) / 64 * 256;
     __shared__ __attribute__((aligned(16))) char sh[2 * STAGE];
     const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -491,9 +493,9 @@ __global__ void __launch_bounds__(256) k_gemm8_join(Gemm8 p) {
 
 // A kernel's tile and what its workgroups take, in us, with `resident` of them on a CU at most: `fix` a round of those and
 // `each` a workgroup, and for a stage of kw blocks of k `alone` where a CU has one workgroup, `shared` a workgroup where it
-// has more; with every CU busy the clock falls and the caches fill, and a stage takes `chip` a workgroup and CU. Fitted to 5815
+// has more; with every CU busy the clock falls and the caches fill, and a stage takes `chip` a workgroup and CU. Fitted to 4080
 // (products) and 4611 (weight gradients) times over all kernels, splits of k from 1 to 16 and sizes from 1 to 16384; the
-// choice by them is 0.5 % behind the best of all those in the mean, 26 % at most.
+// choice by them is 0.8 % (0.5 %) behind the best of all those in the mean, 21 % (26 %) at most.
 struct Tile {
     int bm, bn, kw, resident;
     float fix, each, alone, shared, chip;
@@ -535,11 +537,9 @@ inline void split_blocks(int blocks, int kw, int splits, int &per, int &parts) {
     parts = blocks > per ? (blocks + per - 1) / per : 1;
 }
 
-constexpr Tile kTiles[] = {{256, 256, 1, 1, 8.0f, 0.4f, 2.27f, 0.4f, 3.2f},
-                           {128, 128, 1, 2, 0.0f, 2.0f, 0.856f, 0.45f, 0.86f},
-                           {64, 64, 1, 2, 0.53f, 1.91f, 0.305f, 0.271f, 0.264f},
-                           {32, 32, 1, 4, 0.44f, 0.48f, 0.184f, 0.102f, 0.069f},
-                           {32, 32, 2, 2, 0.0f, 1.26f, 0.246f, 0.203f, 0.201f}};
+constexpr Tile kTiles[] = {{256, 256, 1, 1, 5.26f, 0.32f, 2.484f, 0.44f, 3.11f}, {128, 128, 1, 2, 0.0f, 3.41f, 0.862f, 0.413f, 0.997f},
+                           {128, 64, 1, 3, 0.0f, 1.26f, 0.656f, 0.463f, 0.548f}, {64, 64, 1, 4, 0.0f, 0.56f, 0.485f, 0.3f, 0.272f},
+                           {32, 32, 1, 4, 0.28f, 0.63f, 0.197f, 0.096f, 0.1f},   {32, 32, 2, 2, 0.0f, 1.2f, 0.252f, 0.209f, 0.195f}};
 
 om_status gemm8(om_ctx *ctx, Gemm8 p) {
     // Up to 16 rows the thin kernel is the fastest (4 x 4096 x 4096: 5.6 us, the best of the others 8.2) until a wavefront has so
@@ -551,24 +551,25 @@ om_status gemm8(om_ctx *ctx, Gemm8 p) {
         hipLaunchKernelGGL((k_gemm8_thin<4, 4>), dim3((unsigned)(((int64_t)p.n + 15) / 16)), dim3(256), 0, ctx->stream, p);
         return OM_LAUNCH_CHECK(ctx, "om_gemm8");
     }
-    const Choice ch = choose(kTiles, ctx->num_cus, p.m, p.n, p.blocks, p.a.ldq, 2.46f, 0.89f);
+    const Choice ch = choose(kTiles, ctx->num_cus, p.m, p.n, p.blocks, p.a.ldq, 2.38f, 0.82f);
     OM_REQUIRE(ctx, ch.tile >= 0, "om_gemm8: k is more than a launch takes");
     const Tile &c = kTiles[ch.tile];
     p.tiles_m = (int)(((int64_t)p.m + c.bm - 1) / c.bm);
     p.tiles_n = (int)(((int64_t)p.n + c.bn - 1) / c.bn);
     split_blocks(p.blocks, c.kw, ch.splits, p.per, p.splits);
     const int64_t wgs = (int64_t)p.tiles_m * p.tiles_n * p.splits;
-    const int threads = ch.tile == 0 || ch.tile == 4 ? 512 : 256;
+    const int threads = ch.tile == 0 || ch.tile == 5 ? 512 : 256;
     OM_REQUIRE(ctx, launches(wgs, threads), "om_gemm8: %d x %d is more than a launch takes", p.m, p.n);
     if (om_status s = om::use_device(ctx)) return s;
     if (p.splits > 1)
         if (om_status s = om::scratch(ctx, sizeof(float) * (uint64_t)p.splits * (uint64_t)p.m * (uint64_t)p.n, &p.ws)) return s;
     auto go = [&](auto kern) { hipLaunchKernelGGL(kern, dim3((unsigned)wgs), dim3(threads), 0, ctx->stream, p); };
     switch (ch.tile) {
-        case 0: go(k_gemm8<256, 256, 2, 4>); break;
-        case 1: go(k_gemm8<128, 128, 2, 2>); break;
-        case 2: go(k_gemm8_few<64, 64, 1, 3>); break;
-        case 3: go(k_gemm8_few<32, 32, 1, 4>); break;
+        case 0: go(k_gemm8<256, 256, 2, 4, 2>); break;
+        case 1: go(k_gemm8<128, 128, 2, 2, 2>); break;
+        case 2: go(k_gemm8<128, 64, 2, 2, 3>); break;
+        case 3: go(k_gemm8<64, 64, 2, 2, 4>); break;
+        case 4: go(k_gemm8_few<32, 32, 1, 4>); break;
         default: go(k_gemm8_few<32, 32, 2, 4>); break;
     }
     if (p.splits > 1)
