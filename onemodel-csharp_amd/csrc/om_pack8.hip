@@ -12,6 +12,7 @@ namespace {
 
 using namespace om8;
 
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 constexpr int kThreads = 256;
 // Items of one wavefront in flight. Four give the same times on large tensors (61.7 and 61.6 us to pack 16384 x 4096) and take
 // longer on small ones (3.5 and 2.9 us for 64 x 256, 4.8 and 3.6 with GELU).
@@ -29,10 +30,10 @@ struct Item {
 // The wavefront's kUnroll neighbouring items: `load(u, item)` for each, then `mid()`, then `use(u, item)`. What mid does for
 // all of them at once (the reductions) is not held up by their conditions.
 template <bool PAIR, class Load, class Mid, class Use>
-__device__ __forceinline__ void each_item(int64_t rows, int64_t cols, int blocks, Load load, Mid mid, Use use) {
+__device__ __forceinline__ void each_item(uint32_t wg, int64_t rows, int64_t cols, int blocks, Load load, Mid mid, Use use) {
     const int lane = threadIdx.x & 63;
     const uint32_t segs = PAIR ? 1u : (uint32_t)(blocks + 1) / 2, total = PAIR ? (uint32_t)((rows + 1) / 2) : (uint32_t)rows * segs;
-    const uint32_t w = (blockIdx.x * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kUnroll;
+    const uint32_t w = (wg * (kThreads / 64) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6)) * kUnroll;
     uint32_t r = w / segs, k = w - r * segs;
     Item it[kUnroll];
 #pragma unroll
@@ -86,16 +87,76 @@ __device__ __forceinline__ void scales_of(const floatx4 (&v)[N], int (&s)[N]) {
 }
 
 template <bool PAIR>
+__device__ __forceinline__ void pack_rows(uint32_t wg, const float *__restrict__ x, int64_t ld, int64_t rows, int64_t cols,
+                                          int blocks, const Packed &p) {
+    floatx4 v[kUnroll] = {};
+    int s[kUnroll];
+    each_item<PAIR>(wg, rows, cols, blocks, [&](int u, const Item &it) { v[u] = take(x, ld, cols, it); },
+                    [&] { scales_of(v, s); },
+                    [&](int u, const Item &it) { put_block(p, it.row, it.blk, blocks, it.col, v[u], s[u]); });
+}
+template <bool PAIR>
 __global__ void __launch_bounds__(kThreads) k_pack8(const float *__restrict__ x, int64_t ld, int64_t rows, int64_t cols,
                                                     int blocks, Packed p) {
     OM_LDS_POISON();
-    floatx4 v[kUnroll] = {};
-    int s[kUnroll];
-    each_item<PAIR>(rows, cols, blocks, [&](int u, const Item &it) { v[u] = take(x, ld, cols, it); }, [&] { scales_of(v, s); },
-                    [&](int u, const Item &it) { put_block(p, it.row, it.blk, blocks, it.col, v[u], s[u]); });
+    pack_rows<PAIR>(blockIdx.x, x, ld, rows, cols, blocks, p);
 }
 
-// The transpose packed (and the tensor itself where ROWS): a workgroup takes 128 rows x 128 columns, so that both kinds
+// Both forms of a small tensor: the transpose by tiles of 128 rows x 32 columns, and from workgroup `tiles` on the rows, from a
+// reading of their own. Four times as many and smaller workgroups than one for 128 x 128 of both, and two barriers in place of
+// three: 777 x 1000 4.1 us and 5.1, 2304 x 768 4.7 and 5.4; at 4096 x 768 the second reading costs more (6.2 and 6.0 us), at
+// 16384 x 4096 half as much again (121 and 82). Thread t of a tile holds rows 4 (t / 8) .. + 3 of columns 4 (t % 8) .. + 3.
+constexpr int64_t kSmall = 1 << 21;
+template <bool PAIR>
+__global__ void __launch_bounds__(kThreads) k_pack8_small(const float *__restrict__ x, int64_t ld, int64_t rows, int64_t cols,
+                                                          int blocks, int rblocks, uint32_t tiles, int ctiles, Packed p, Packed t) {
+    OM_LDS_POISON();
+    if (blockIdx.x >= tiles) return pack_rows<PAIR>(blockIdx.x - tiles, x, ld, rows, cols, blocks, p);
+    __shared__ __attribute__((aligned(16))) uint32_t tops[4][32];
+    __shared__ __attribute__((aligned(16))) uint32_t tr[32 * 34];  // 34 to a column: the lanes that write meet on no bank
+    const int l = threadIdx.x & 7, g = threadIdx.x >> 3, w = threadIdx.x >> 6;
+    const int rb = (int)(blockIdx.x / ctiles), ct = (int)(blockIdx.x % ctiles);
+    const int64_t r0 = (int64_t)rb * 128 + 4 * g, c0 = (int64_t)ct * 32, c = c0 + 4 * l;
+    floatx4 v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) v[i] = r0 + i < rows ? load4(x + (r0 + i) * ld + c, cols - c) : floatx4{0.0f, 0.0f, 0.0f, 0.0f};
+    u32x4 top;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {  // over the eight lanes of the wavefront that have these columns
+        uint32_t m = top_of(v[0][e], v[1][e], v[2][e], v[3][e]);
+        m = max(m, lane_of16<kRotate8>(m));
+        auto o = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+        m = max(o[0], o[1]);
+        o = __builtin_amdgcn_permlane32_swap(m, m, false, false);
+        top[e] = max(o[0], o[1]);
+    }
+    if ((threadIdx.x & 56) == 0) *reinterpret_cast<u32x4 *>(&tops[w][4 * l]) = top;
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+        const u32x4 o = *reinterpret_cast<const u32x4 *>(&tops[q][4 * l]);
+#pragma unroll
+        for (int e = 0; e < 4; e++) top[e] = max(top[e], o[e]);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const int s = scale_byte(top[e]);
+        tr[(4 * l + e) * 34 + g] = encode4(floatx4{v[0][e], v[1][e], v[2][e], v[3][e]}, inverse_of(s));
+        if (g == e && c + e < cols) {
+            uint8_t *d = t.s + (c + e) * t.lds + rb;
+            d[0] = (uint8_t)s;
+            if (rb == rblocks - 1)
+                for (int z = 1; rb + z < t.lds; z++) d[z] = 0;
+        }
+    }
+    __syncthreads();
+    const int col = threadIdx.x >> 3, piece = threadIdx.x & 7;
+    if (c0 + col >= cols) return;
+    const u32x2 *s = reinterpret_cast<const u32x2 *>(tr + col * 34 + 4 * piece), a = s[0], b = s[1];
+    *reinterpret_cast<u32x4 *>(t.q + (c0 + col) * t.ldq + (int64_t)rb * 128 + 16 * piece) = u32x4{a[0], a[1], b[0], b[1]};
+}
+
+// The transpose of any tensor (and the tensor itself where ROWS): a workgroup takes 128 rows x 128 columns, so that both kinds
 // of blocks are whole. Thread t holds rows 4 (t / 32) .. + 3 of columns 4 (t % 32) .. + 3; sixteen wavefronts, since a small
 // tensor has few such tiles and its time is one tile's. Codes of the transpose go through LDS, four rows of a column in a
 // dword, so that they leave as whole 128-byte lines; dword g of a column stands at g ^ (column / 4), so that neither the
@@ -161,7 +222,7 @@ template <bool PAIR, bool ACC>
 __global__ void __launch_bounds__(kThreads) k_unpack8(Packed p, float *y, int64_t ld, int64_t rows, int64_t cols, int blocks) {
     OM_LDS_POISON();
     floatx4 v[kUnroll], old[kUnroll];
-    each_item<PAIR>(rows, cols, blocks,
+    each_item<PAIR>(blockIdx.x, rows, cols, blocks,
                     [&](int u, const Item &it) {
                         v[u] = value_of(p, it);
                         if constexpr (ACC) old[u] = take(y, ld, cols, it);
@@ -180,7 +241,7 @@ __global__ void __launch_bounds__(kThreads) k_gelu8(const float *x, float *y, in
     OM_LDS_POISON();
     floatx4 v[kUnroll] = {};
     int s[kUnroll];
-    each_item<PAIR>(rows, cols, blocks, [&](int u, const Item &it) { v[u] = take(x, cols, cols, it); },
+    each_item<PAIR>(blockIdx.x, rows, cols, blocks, [&](int u, const Item &it) { v[u] = take(x, cols, cols, it); },
                     [&] { scales_of(v, s); },
                     [&](int u, const Item &it) {
                         put_block(p, it.row, it.blk, blocks, it.col, v[u], s[u]);
@@ -195,7 +256,7 @@ __global__ void __launch_bounds__(kThreads) k_gelu8_bwd(const float *g, Packed p
                                                         int blocks) {
     OM_LDS_POISON();
     floatx4 h[kUnroll], gv[kUnroll], old[kUnroll];
-    each_item<PAIR>(rows, cols, blocks,
+    each_item<PAIR>(blockIdx.x, rows, cols, blocks,
                     [&](int u, const Item &it) {
                         h[u] = value_of(p, it);
                         gv[u] = take(g, cols, cols, it);
@@ -247,7 +308,14 @@ om_status om_pack8(om_ctx *ctx, const float *x, int ld_x, int rows, int cols, ui
             hipLaunchKernelGGL(k_pack8<decltype(pair)::value>, grid, dim3(kThreads), 0, ctx->stream, x, (int64_t)ld_x,
                                (int64_t)rows, (int64_t)cols, (int)cb, p);
         });
-    else if (x8)
+    else if (x8 && (int64_t)rows * cols <= kSmall) {
+        const int ct = (int)(((int64_t)cols + 31) / 32);
+        const uint32_t tiles = (uint32_t)(rb * ct);
+        walk(rows, cb, [&](auto pair, dim3 grid) {
+            hipLaunchKernelGGL(k_pack8_small<decltype(pair)::value>, dim3(grid.x + tiles), dim3(kThreads), 0, ctx->stream, x,
+                               (int64_t)ld_x, (int64_t)rows, (int64_t)cols, (int)cb, (int)rb, tiles, ct, p, t);
+        });
+    } else if (x8)
         hipLaunchKernelGGL(k_pack8_t<true>, dim3((unsigned)(rb * cb)), dim3(kTile), 0, ctx->stream, x, (int64_t)ld_x,
                            (int64_t)rows, (int64_t)cols, (int)rb, (int)cb, p, t);
     else

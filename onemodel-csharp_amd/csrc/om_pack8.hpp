@@ -70,6 +70,7 @@ __device__ __forceinline__ uint32_t lane_of16(uint32_t x) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, 0xF, 0xF, true);
 }
 constexpr int kSwap1 = 0xB1, kSwap2 = 0x4E, kHalfMirror = 0x141, kMirror = 0x140;  // quad_perm [1,0,3,2], [2,3,0,1]; rows of 16
+constexpr int kRotate8 = 0x128;  // of 16
 // Largest of 32 neighbouring lanes, in all of them: five steps on the vector pipe, four inside 16 lanes and one across.
 __device__ __forceinline__ uint32_t max32(uint32_t v) {
     v = max(v, lane_of16<kSwap1>(v));

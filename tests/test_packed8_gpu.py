@@ -48,7 +48,7 @@ def check_packed(raw, x):
 
 
 SHAPES = [(1, 1), (1, 128), (3, 5), (2, 129), (64, 256), (127, 127), (128, 128), (129, 130), (7, 512), (5, 513), (300, 77),
-          (33, 1000), (640, 384)]
+          (33, 1000), (640, 384), (4001, 1100), (1501, 1502), (20000, 130)]
 
 
 @pytest.mark.parametrize("rows,cols", SHAPES)
