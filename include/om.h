@@ -374,11 +374,13 @@ om_status om_layernorm_bwd_partials(om_ctx *ctx, const float *g, const float *x,
  * counterpart in the reference, whose tape keeps fp32). A packed tensor of [rows, cols] holds, for each block of 128
  * neighbouring values of a row, 8-bit floats (OCP e4m3) and one power of two: with e the least exponent from -127 on that
  * brings the block's largest finite |x| / 2^e to 448 or below, a code is x / 2^e rounded to nearest, ties to even (a relative
- * error of at most 2^-4, or 2^-10 2^e below 2^-6 2^e); infinities and NaN become NaN and leave the others alone.
+ * error of at most 2^-4, or 2^-10 2^e below 2^-6 2^e); infinities and NaN become NaN and leave the others alone. A value
+ * within 2^-5 of the largest float may round to 2^128, an infinity when it is used.
  * Layout: `rows` rows of codes of S = 128 ceil(cols / 128) bytes, zeros behind the last column, then `rows` rows of scale
  * bytes e + 127 of T = 4 ceil(S / 512) bytes, zeros behind the last block; om_pack8_bytes gives rows * (S + T), 0 where rows
  * or cols is not positive. Packed tensors start at multiples of 16 bytes (om_alloc's do). A block is 128 wide whatever cols
- * is, so a narrow tensor is best viewed as a wide one first.
+ * is, so a narrow tensor is best viewed as a wide one first. Sizes that a launch cannot hold (2^32 threads: packed tensors of
+ * 34 GB and more in practice) are refused, and so is k (rows of om_linear_bwd_x8) from 2^27 on.
  * Where an entry point says x8 its rows are packed; xt8 is the packed transpose, [cols, rows], whose blocks run along the
  * rows of x: a product takes each operand packed along the dimension it sums over. */
 uint64_t om_pack8_bytes(int rows, int cols);
@@ -394,7 +396,7 @@ om_status om_unpack8(om_ctx *ctx, const uint8_t *x8, float *y, int ld_y, int row
 om_status om_gemm8(om_ctx *ctx, int m, int n, int k, const uint8_t *a8, const uint8_t *b8, const float *bias, float *c,
                    int ldc, int acc);
 /* om_linear_bwd with the layer's input kept as xt8, the packed transpose of x [rows, in]: dw (+)= g^T x (every product
- * exact, sums fp32) and db (+)= fp64 column sums of g; dx (+)= g w is om_linear_bwd's. Each output may be NULL. */
+ * exact but for bits of g below 2^-126, sums fp32) and db (+)= fp64 column sums of g; dx (+)= g w is om_linear_bwd's. Each output may be NULL. */
 om_status om_linear_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *xt8, const float *w, float *dx, float *dw, float *db,
                            int rows, int in, int out, int acc_dx, int acc_dw, int acc_db);
 /* om_gelu_fwd over [rows, cols] that keeps its input packed, and its backward from that: dx (+)= g * gelu'(value of x8).

@@ -8,6 +8,10 @@
 // use), as their adder drops what is 2^-13 or so below its largest term. The conversion costs two to three vector
 // instructions an MFMA at 64 x 64 to 128 x 64 values a wavefront and runs beside it (16 k of both: 15.4 ns an MFMA alone,
 // 16.6 with six conversions to each).
+//
+// Bound: large products by the clock that the card keeps under matrix work (4096^3 107 to 111 us, 1240 to 1285 TFLOP/s; without
+// the loads 101, without the conversions 104; the library's bf16 product, which converts nothing and reads twice the bytes,
+// 105 to 112); small ones by the launch and one chain of loads, 4 to 6 us.
 #include "om_pack8.hpp"
 
 #include <cmath>
@@ -277,40 +281,38 @@ __global__ void __launch_bounds__(64 * WM * WN, WAVES) k_gemm8(Gemm8 p) {
     }
 }
 
-// Few tiles: the wavefronts of a workgroup share one tile of BM x BN and split k between them, four to a block of 128, so that
+// Few tiles: the wavefronts of a workgroup share one tile of 32 x 32 and split k between them, four to a block of 128, so that
 // every code is widened once and a stage of KW blocks goes round without a barrier inside it. D stages stand in LDS, and
-// one more in registers. Their sums meet in LDS and are added in order.
-template <int BM, int BN, int KW, int D>
+// one more in registers. Their sums meet in LDS and are added in order. (777 x 333 x 1000: 6.1 us, by 64 x 64 tiles 9.1; with a
+// block of its own to each wavefront and no barriers 5.9, and 20.0 in place of 15.4 at 1000 x 2000 x 2000.)
+template <int KW, int D>
 __global__ void __launch_bounds__(256 * KW, KW < 2 ? 2 : KW) k_gemm8_few(Gemm8 p) {
     OM_LDS_POISON();
     static_assert(4 % KW == 0, "a stage's scale bytes lie in one dword");
-    constexpr int NW = 4 * KW, MT = BM / 32, NT = BN / 32, BLOCK = (BM + BN) * 128;
-    constexpr int SS = KW * BLOCK, STAGE = SS + (BM + BN + 63) / 64 * 256;  // a scale load fills 64 dwords
-    constexpr int LD = BN + 1, OUT = NW * BM * LD * 4;
-    constexpr int LDS = D * STAGE > OUT ? D * STAGE : OUT, PER = (BM + BN) / 32;
+    constexpr int NW = 4 * KW, BLOCK = 64 * 128, SS = KW * BLOCK, STAGE = SS + 256;
+    constexpr int LD = 33, OUT = NW * 32 * LD * 4, LDS = D * STAGE > OUT ? D * STAGE : OUT, PER = 2;
     __shared__ __attribute__((aligned(16))) char sh[LDS];
     const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kb = wv >> 2, q = wv & 3;
     int split, tm, tn;
     tile_of(p.tiles_m, p.tiles_n, gridDim.x, split, tm, tn);
-    const int m0 = tm * BM, n0 = tn * BN;
-    // Rows 0 .. BM - 1 of a stage's block are A's, the others B's; this wavefront loads its quarter of block kb, eight rows of
+    const int m0 = 32 * tm, n0 = 32 * tn;
+    // Rows 0 .. 31 of a stage's block are A's, the others B's; this wavefront loads its quarter of block kb, eight rows of
     // one operand an instruction.
     const uint8_t *src[PER];
     uint32_t off[PER];
 #pragma unroll
     for (int i = 0; i < PER; i++) {
         const int r0 = 8 * (q * PER + i), r = r0 + (lane >> 3), piece = (lane ^ (r >> 1)) & 7;
-        const bool a = r0 < BM;
+        const bool a = r0 < 32;
         const Packed &o = a ? p.a : p.b;
         const int first = a ? m0 : n0, last = (a ? p.m : p.n) - 1 - first;
         src[i] = o.q + (int64_t)first * o.ldq;
-        off[i] = (uint32_t)min(a ? r : r - BM, last) * (uint32_t)o.ldq + 16 * piece;
+        off[i] = (uint32_t)min(a ? r : r - 32, last) * (uint32_t)o.ldq + 16 * piece;
     }
-    // scale bytes: 64 rows an instruction, A's and then B's
-    const int sr = min(wv * 64 + lane, BM + BN - 1);
-    const uint8_t *ssrc = sr < BM ? p.a.s + (int64_t)min(m0 + sr, p.m - 1) * p.a.lds
-                                  : p.b.s + (int64_t)min(n0 + sr - BM, p.n - 1) * p.b.lds;
+    // scale bytes: one instruction, A's rows and then B's
+    const uint8_t *ssrc = lane < 32 ? p.a.s + (int64_t)min(m0 + lane, p.m - 1) * p.a.lds
+                                    : p.b.s + (int64_t)min(n0 + lane - 32, p.n - 1) * p.b.lds;
     const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)sh;
     const int b0 = split * p.per, b1 = min(p.blocks, b0 + p.per), stages = (b1 - b0 + KW - 1) / KW;
     auto issue = [&](int st) {  // past the last stage the last one again, into a slot that nothing reads
@@ -318,38 +320,33 @@ __global__ void __launch_bounds__(256 * KW, KW < 2 ? 2 : KW) k_gemm8_few(Gemm8 p
         const int blk = min(b0 + min(st, stages - 1) * KW + kb, b1 - 1);
 #pragma unroll
         for (int i = 0; i < PER; i++) load_to_lds(src[i] + (int64_t)blk * 128, off[i], at + kb * BLOCK + (q * PER + i) * 1024);
-        if (wv * 64 < BM + BN) load_to_lds4(ssrc + (blk & ~3), at + SS + wv * 256);
+        if (wv == 0) load_to_lds4(ssrc + (blk & ~3), at + SS);
     };
-    floatx16 acc[MT][NT];
+    floatx16 acc[1][1];
 #pragma unroll
-    for (int i = 0; i < MT; i++)
-#pragma unroll
-        for (int j = 0; j < NT; j++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) acc[i][j][e] = 0.0f;
-    u32x4 raw[2][MT + NT], w[2][MT + NT];
-    uint32_t dw[2][MT + NT];
-    auto row_at = [&](int o) { return o < MT ? 32 * o + l32 : BM + 32 * (o - MT) + l32; };
+    for (int e = 0; e < 16; e++) acc[0][0][e] = 0.0f;
+    u32x4 raw[2][2], w[2][2];
+    uint32_t dw[2][2];
     auto read = [&](int h, int st, int o) {
         const char *cur = sh + (st % D) * STAGE;
-        dw[h][o] = *reinterpret_cast<const uint32_t *>(cur + SS + 4 * row_at(o));
-        raw[h][o] = *reinterpret_cast<const u32x4 *>(cur + kb * BLOCK + piece_at(row_at(o), 2 * q + g));
+        dw[h][o] = *reinterpret_cast<const uint32_t *>(cur + SS + 4 * (32 * o + l32));
+        raw[h][o] = *reinterpret_cast<const u32x4 *>(cur + kb * BLOCK + piece_at(32 * o + l32, 2 * q + g));
     };
     // Stage st from registers, the next one's codes read meanwhile, its own slot loaded anew. (Blocks past the last one hold
     // the last one's codes, which this wavefront drops.)
-    float sc[2][MT + NT];
+    float sc[2][2];
     auto turn = [&](int h, int st) {
         land<(D - 2) * PER>();
         issue(st + D);
 #pragma unroll
-        for (int o = 0; o < MT + NT; o++) read(h ^ 1, st + 1, o);
+        for (int o = 0; o < 2; o++) read(h ^ 1, st + 1, o);
         const int blk = b0 + st * KW + kb;
         if (blk < b1) {
-            half_chunk<MT, NT>(acc, w[0], w[1], [&](int o, int t) { return raw[h][o][2 + t]; }, [&](int o) { return sc[h][o]; },
+            half_chunk<1, 1>(acc, w[0], w[1], [&](int o, int t) { return raw[h][o][2 + t]; }, [&](int o) { return sc[h][o]; },
                                [](int) {});
 #pragma unroll
-            for (int o = 0; o < MT + NT; o++) sc[h ^ 1][o] = scale_in(dw[h ^ 1][o], blk + KW);
-            half_chunk<MT, NT>(acc, w[1], w[0], [&](int o, int t) { return raw[h ^ 1][o][t]; },
+            for (int o = 0; o < 2; o++) sc[h ^ 1][o] = scale_in(dw[h ^ 1][o], blk + KW);
+            half_chunk<1, 1>(acc, w[1], w[0], [&](int o, int t) { return raw[h ^ 1][o][t]; },
                                [&](int o) { return sc[h ^ 1][o]; }, [](int) {});
         }
     };
@@ -358,7 +355,7 @@ __global__ void __launch_bounds__(256 * KW, KW < 2 ? 2 : KW) k_gemm8_few(Gemm8 p
         for (int st = 0; st < D; st++) issue(st);
         land<(D - 1) * PER>();
 #pragma unroll
-        for (int o = 0; o < MT + NT; o++) {
+        for (int o = 0; o < 2; o++) {
             read(0, 0, o);
             sc[0][o] = scale_in(dw[0][o], b0 + kb);
             w[0][o] = widen8(raw[0][o][0], raw[0][o][1], sc[0][o]);
@@ -371,30 +368,24 @@ __global__ void __launch_bounds__(256 * KW, KW < 2 ? 2 : KW) k_gemm8_few(Gemm8 p
     land<0>();
     float *out = reinterpret_cast<float *>(sh);
 #pragma unroll
-    for (int i = 0; i < MT; i++)
-#pragma unroll
-        for (int j = 0; j < NT; j++)
-#pragma unroll
-            for (int e = 0; e < 16; e++)
-                out[(wv * BM + 32 * i + 8 * (e >> 2) + 4 * g + (e & 3)) * LD + 32 * j + l32] = acc[i][j][e];
+    for (int e = 0; e < 16; e++) out[(wv * 32 + 8 * (e >> 2) + 4 * g + (e & 3)) * LD + l32] = acc[0][0][e];
     __syncthreads();
     const Out to(p, split);
-    constexpr int EACH = BM * BN / (64 * NW);  // values a thread
-    static_assert(BM * BN % (64 * NW) == 0 && 64 * NW % BN == 0, "whole rows to a pass of the threads");
-    const int c = threadIdx.x % BN, col = n0 + c;
+    constexpr int EACH = 4 / KW;  // values a thread
+    const int c = threadIdx.x % 32, col = n0 + c;
     if (col >= p.n) return;
     const float bias = to.bias_of(col);
     float v[EACH];
 #pragma unroll
     for (int u = 0; u < EACH; u++) {
-        const int r = threadIdx.x / BN + u * (64 * NW / BN);
+        const int r = threadIdx.x / 32 + u * 8 * KW;
         v[u] = out[r * LD + c];
 #pragma unroll
-        for (int w = 1; w < NW; w++) v[u] += out[(w * BM + r) * LD + c];
+        for (int w = 1; w < NW; w++) v[u] += out[(w * 32 + r) * LD + c];
     }
 #pragma unroll
     for (int u = 0; u < EACH; u++) {
-        const int row = m0 + threadIdx.x / BN + u * (64 * NW / BN);
+        const int row = m0 + threadIdx.x / 32 + u * 8 * KW;
         if (row < p.m) to.put(row, col, v[u], bias);
     }
 }
@@ -569,8 +560,8 @@ om_status gemm8(om_ctx *ctx, Gemm8 p) {
         case 1: go(k_gemm8<128, 128, 2, 2, 2>); break;
         case 2: go(k_gemm8<128, 64, 2, 2, 3>); break;
         case 3: go(k_gemm8<64, 64, 2, 2, 4>); break;
-        case 4: go(k_gemm8_few<32, 32, 1, 4>); break;
-        default: go(k_gemm8_few<32, 32, 2, 4>); break;
+        case 4: go(k_gemm8_few<1, 4>); break;
+        default: go(k_gemm8_few<2, 4>); break;
     }
     if (p.splits > 1)
         hipLaunchKernelGGL(k_gemm8_join, dim3(om::grid1d((int64_t)p.m * p.n, 256, (int64_t)ctx->num_cus * 8)), dim3(256), 0,
@@ -580,10 +571,11 @@ om_status gemm8(om_ctx *ctx, Gemm8 p) {
 
 // ------------------------------------------------------------------------------------------------- weight gradient
 // dW = g^T x with x packed along the rows and g as it is. g is split into three bf16 parts that hold all of its bits (h + m +
-// l), a value of x is one part, so a product is three MFMAs (six with x in fp32) and as exact as those. A wavefront owns 32
-// rows of dW (columns of g) and all BN columns; it loads its g straight into fragments, 32 lanes to a row of g, and splits
-// them in registers. Sums that come out infinite or NaN (an infinite g, whose parts are NaN; a g that rounds up past bf16's
-// range) are formed again on the fp32 instruction.
+// l; parts below 2^-126, which only values below 2^-103 have, may count as zero), a value of x is one part, so a product is three MFMAs (six with x in fp32)
+// and as exact as those. A wavefront owns 32 rows of dW (columns of g) and all BN columns, so g is split once; 16384 x 4096 x
+// 4096 takes 1470 us, 1120 TFLOP/s of bf16 products and 85 to 90 % of the library's rate, with six vector instructions beside
+// each MFMA (64 x 128 by two such groups, x widened for both: 1490 us; 32 x 256: 1503). Sums that come out infinite or NaN (an
+// infinite g, whose parts are NaN; a g that rounds up past bf16's range) are formed again on the fp32 instruction.
 struct Dw8 {
     const float *g;         // [rows, m]
     Packed x;               // [n, rows]
@@ -611,55 +603,52 @@ __device__ __forceinline__ void split_rest(float r0, float r1, uint32_t &m, uint
     l = oms::pack2(r0 - __uint_as_float(m << 16), r1 - __uint_as_float(m & 0xFFFF0000u));
 }
 
-// A workgroup computes (32 MG) x (32 NT) of dW with MG groups of 4 KW wavefronts: wavefront (mg, kb, q) has 32 rows (columns
-// of g), all columns, and the q-th 32 k of every KW-th block of 128, so x is widened by MG wavefronts only and g is split
-// once. Both come through LDS, D stages of KW blocks and one more in registers, by loads of 16 bytes a lane (a dword a lane
-// into registers, as g's layout would have it, keeps the load path busy as long for a quarter of the data: 210 us against
-// 140 of products at 16384 x 768 x 2304). The next half's (16 k) splits and conversions stand between a half's MFMAs. At the end the wavefronts'
+// A workgroup computes 32 x (32 NT) of dW with four wavefronts: wavefront q has all of it over the q-th 32 k of every block of
+// 128. g and x come through LDS, D blocks and one more in registers, by loads of 16 bytes a lane (a dword a lane into registers,
+// as g's layout would have it, keeps the load path busy as long for a quarter of the data: 210 us against 140 of products at
+// 16384 x 768 x 2304). The next half's (16 k) splits and conversions stand between a half's MFMAs. At the end the wavefronts'
 // sums meet in LDS and are added in order.
-template <int NT, int MG, int KW, int D>
-__global__ void __launch_bounds__(256 * MG * KW, MG * KW < 4 ? 2 : 4) k_dw8(Dw8 p) {
+template <int NT, int D>
+__global__ void __launch_bounds__(256, 2) k_dw8(Dw8 p) {
     OM_LDS_POISON();
-    constexpr int NW = 4 * KW * MG, BM = 32 * MG, BN = 32 * NT, BLOCK = BN * 128, SS = KW * BLOCK;
-    constexpr int GS = SS + (BN + 63) / 64 * 256;  // a scale load fills 64 dwords
-    constexpr int STAGE = GS + NW * 4096, LD = BN + 1, OUT = NW * 32 * LD * 4, LDS = D * STAGE > OUT ? D * STAGE : OUT;
-    constexpr int PER = BN / 32 / MG, LOADS = PER + 4;
-    static_assert(BN % (32 * MG) == 0 && BN <= 64 * NW && 4 % KW == 0, "whole loads to each wavefront, scales by one of each");
+    constexpr int BN = 32 * NT, SS = BN * 128, GS = SS + (BN + 63) / 64 * 256;  // a scale load fills 64 dwords
+    constexpr int STAGE = GS + 4 * 4096, LD = BN + 1, OUT = 4 * 32 * LD * 4, LDS = D * STAGE > OUT ? D * STAGE : OUT;
+    constexpr int LOADS = NT + 4;
+    static_assert(BN <= 256, "scales by one load of each wavefront");
     __shared__ __attribute__((aligned(16))) char sh[LDS];
     const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
-    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), mg = wv / (4 * KW), kb = wv / 4 % KW, q = wv & 3;
+    const int q = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int split, tm, tn;
     tile_of(p.tiles_m, p.tiles_n, gridDim.x, split, tm, tn);
-    const int m0 = tm * BM + 32 * mg, n0 = tn * BN;
+    const int m0 = 32 * tm, n0 = tn * BN;
     // blocks of 128 rows, and (in the last split) the rows behind the last that is taken as one
-    const int b0 = split * p.per, b1 = min(p.full, b0 + p.per), count = max(b1 - b0, 0), stages = (count + KW - 1) / KW;
+    const int b0 = split * p.per, b1 = min(p.full, b0 + p.per), count = max(b1 - b0, 0);
     const bool tail = split == p.splits - 1 && p.full < p.blocks;
     const uint8_t *xq = p.x.q + (int64_t)n0 * p.x.ldq;
-    uint32_t off[PER];
+    uint32_t off[NT];
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-        const int r = 8 * ((q * MG + mg) * PER + i) + (lane >> 3), piece = (lane ^ (r >> 1)) & 7;
+    for (int i = 0; i < NT; i++) {
+        const int r = 8 * (q * NT + i) + (lane >> 3), piece = (lane ^ (r >> 1)) & 7;
         off[i] = (uint32_t)min(r, p.n - 1 - n0) * (uint32_t)p.x.ldq + 16 * piece;
     }
-    const uint8_t *xs = p.x.s + (int64_t)min(n0 + (wv * 64 + lane) % BN, p.n - 1) * p.x.lds;
+    const uint8_t *xs = p.x.s + (int64_t)min(n0 + (q * 64 + lane) % BN, p.n - 1) * p.x.lds;
     // g: this wavefront's own 32 rows x 32 columns of a stage, eight rows a load, four columns a lane. Columns past the last
     // four start there: column c then stands at c - (m - 4) of its four. (Of fewer than four columns the loads run on into
     // the next rows, which is why the last block is not loaded so then.)
     const int first4 = max(p.m - 4, 0), gc = min(m0 + l32, p.m - 1);
     const uint32_t goff = 4u * ((uint32_t)(lane >> 3) * (uint32_t)p.m + (uint32_t)min(m0 + 4 * (lane & 7), first4));
-    const int gat = GS + wv * 4096 + 2048 * g + 4 * ((l32 & ~3) + min(gc - min(m0 + (l32 & ~3), first4), 3));
+    const int gat = GS + q * 4096 + 2048 * g + 4 * ((l32 & ~3) + min(gc - min(m0 + (l32 & ~3), first4), 3));
     const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)sh;
     // Loads past the last block load that one again, into slots that nothing reads.
     auto issue = [&](int st) {
         const uint32_t at = base + (uint32_t)(st % D) * STAGE;
-        const int blk = b0 + min(min(st, stages - 1) * KW + kb, count - 1);
+        const int blk = b0 + min(st, count - 1);
 #pragma unroll
-        for (int i = 0; i < PER; i++)
-            load_to_lds(xq + (int64_t)blk * 128, off[i], at + kb * BLOCK + ((q * MG + mg) * PER + i) * 1024);
-        if (wv * 64 < BN) load_to_lds4(xs + (blk & ~3), at + SS + wv * 256);
+        for (int i = 0; i < NT; i++) load_to_lds(xq + (int64_t)blk * 128, off[i], at + (q * NT + i) * 1024);
+        if (q * 64 < BN) load_to_lds4(xs + (blk & ~3), at + SS + q * 256);
 #pragma unroll
         for (int i = 0; i < 4; i++)
-            load_to_lds(p.g + ((int64_t)blk * 128 + 32 * q + 8 * i) * p.m, goff, at + GS + wv * 4096 + i * 1024);
+            load_to_lds(p.g + ((int64_t)blk * 128 + 32 * q + 8 * i) * p.m, goff, at + GS + q * 4096 + i * 1024);
     };
     float raw[2][16];
     floatx16 acc[NT];
@@ -675,8 +664,8 @@ __global__ void __launch_bounds__(256 * MG * KW, MG * KW < 4 ? 2 : 4) k_dw8(Dw8 
         const char *cur = sh + (st % D) * STAGE;
 #pragma unroll
         for (int j = 0; j < NT; j++) {
-            sc[h][j] = scale_in(*reinterpret_cast<const uint32_t *>(cur + SS + 4 * (32 * j + l32)), b0 + st * KW + kb);
-            xr[h][j] = *reinterpret_cast<const u32x4 *>(cur + kb * BLOCK + piece_at(32 * j + l32, 2 * q + g));
+            sc[h][j] = scale_in(*reinterpret_cast<const uint32_t *>(cur + SS + 4 * (32 * j + l32)), b0 + st);
+            xr[h][j] = *reinterpret_cast<const u32x4 *>(cur + piece_at(32 * j + l32, 2 * q + g));
         }
 #pragma unroll
         for (int e = 0; e < 16; e++) raw[h][e] = *reinterpret_cast<const float *>(cur + gat + 128 * e);
@@ -721,11 +710,9 @@ __global__ void __launch_bounds__(256 * MG * KW, MG * KW < 4 ? 2 : 4) k_dw8(Dw8 
         land<(D - 2) * LOADS>();
         issue(st + D);
         read(h ^ 1, st + 1);
-        if (st * KW + kb < count) {
-            add_sums(h);
-            half(0, h);
-            half(1, h ^ 1);
-        }
+        add_sums(h);
+        half(0, h);
+        half(1, h ^ 1);
     };
     if (count > 0) {
 #pragma unroll
@@ -734,15 +721,14 @@ __global__ void __launch_bounds__(256 * MG * KW, MG * KW < 4 ? 2 : 4) k_dw8(Dw8 
         read(0, 0);
 #pragma unroll
         for (int v = 0; v < STEPS; v++) prepare(0, 0, v);
-        for (int st = 0; st < stages; st += 2) {
+        for (int st = 0; st < count; st += 2) {
             turn(0, st);
-            if (st + 1 < stages) turn(1, st + 1);
+            if (st + 1 < count) turn(1, st + 1);
         }
         land<0>();  // the loads past the last stage, too, before LDS is used again
     }
-    const bool rest = tail && kb == count % KW;
 #pragma unroll 1
-    for (int blk = rest ? p.full : p.blocks; blk < p.blocks; blk++) {  // the rows behind, straight from memory
+    for (int blk = tail ? p.full : p.blocks; blk < p.blocks; blk++) {  // the rows behind, straight from memory
 #pragma unroll
         for (int e = 0; e < 16; e++) {
             const int k = blk * 128 + 32 * q + 16 * g + e;
@@ -787,8 +773,8 @@ __global__ void __launch_bounds__(256 * MG * KW, MG * KW < 4 ? 2 : 4) k_dw8(Dw8 
                 }
             };
 #pragma unroll 1
-            for (int at = kb; at < count; at += KW) block(b0 + at);
-            if (rest)
+            for (int blk = b0; blk < b1; blk++) block(blk);
+            if (tail)
 #pragma unroll 1
                 for (int blk = p.full; blk < p.blocks; blk++) block(blk);
 #pragma unroll
@@ -800,12 +786,12 @@ __global__ void __launch_bounds__(256 * MG * KW, MG * KW < 4 ? 2 : 4) k_dw8(Dw8 
     if (sums) {
         cs += __shfl_xor(cs, 32, 64);
         double *shd = reinterpret_cast<double *>(sh);
-        if (g == 0) shd[wv * 32 + l32] = cs;
+        if (g == 0) shd[q * 32 + l32] = cs;
         __syncthreads();
         const int row = m0 + l32;
-        if (wv % (4 * KW) == 0 && g == 0 && row < p.m) {
+        if (q == 0 && g == 0 && row < p.m) {
 #pragma unroll
-            for (int i = 1; i < 4 * KW; i++) cs += shd[(wv + i) * 32 + l32];
+            for (int i = 1; i < 4; i++) cs += shd[i * 32 + l32];
             if (p.splits > 1) {
                 p.cs[(int64_t)split * p.m + row] = cs;
             } else {
@@ -819,10 +805,10 @@ __global__ void __launch_bounds__(256 * MG * KW, MG * KW < 4 ? 2 : 4) k_dw8(Dw8 
 #pragma unroll
     for (int j = 0; j < NT; j++)
 #pragma unroll
-        for (int e = 0; e < 16; e++) out[(wv * 32 + 8 * (e >> 2) + 4 * g + (e & 3)) * LD + 32 * j + l32] = acc[j][e];
+        for (int e = 0; e < 16; e++) out[(q * 32 + 8 * (e >> 2) + 4 * g + (e & 3)) * LD + 32 * j + l32] = acc[j][e];
     __syncthreads();
-    constexpr int STEP = 64 * NW / BN, EACH = BM / STEP;
-    static_assert(64 * NW % BN == 0 && BM % STEP == 0, "whole rows to a pass of the threads");
+    constexpr int STEP = 256 / BN, EACH = 32 / STEP;
+    static_assert(256 % BN == 0 && 32 % STEP == 0, "whole rows to a pass of the threads");
     const int c = threadIdx.x % BN, col = n0 + c;
     if (col >= p.n) return;
     const bool part = p.splits > 1;
@@ -830,11 +816,11 @@ __global__ void __launch_bounds__(256 * MG * KW, MG * KW < 4 ? 2 : 4) k_dw8(Dw8 
     const bool keep = !part && p.acc_dw;
 #pragma unroll 4
     for (int u = 0; u < EACH; u++) {
-        const int r = threadIdx.x / BN + u * STEP, row = tm * BM + r;
-        const float *s = out + (r / 32 * 4 * KW * 32 + r % 32) * LD + c;
+        const int r = threadIdx.x / BN + u * STEP, row = m0 + r;
+        const float *s = out + r * LD + c;
         float v = s[0];
 #pragma unroll
-        for (int w = 1; w < 4 * KW; w++) v += s[w * 32 * LD];
+        for (int w = 1; w < 4; w++) v += s[w * 32 * LD];
         if (row < p.m) {
             float *d = to + (int64_t)row * p.n + col;
             *d = keep ? *d + v : v;
@@ -887,9 +873,9 @@ om_status dw8(om_ctx *ctx, Dw8 p, int tile) {
         hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)p.tiles_m * p.tiles_n * p.splits)), dim3(256), 0, ctx->stream, p);
     };
     switch (tile) {
-        case 0: go(k_dw8<4, 1, 1, 2>); break;
-        case 1: go(k_dw8<2, 1, 1, 2>); break;
-        default: go(k_dw8<1, 1, 1, 3>); break;
+        case 0: go(k_dw8<4, 2>); break;
+        case 1: go(k_dw8<2, 2>); break;
+        default: go(k_dw8<1, 3>); break;
     }
     if (p.splits > 1)
         hipLaunchKernelGGL(k_dw8_join, dim3(om::grid1d((int64_t)p.m * p.n, 256, (int64_t)ctx->num_cus * 8)), dim3(256), 0,

