@@ -384,7 +384,7 @@ om_status om_layernorm_bwd_partials(om_ctx *ctx, const float *g, const float *x,
  * Where an entry point says x8 its rows are packed; xt8 is the packed transpose, [cols, rows], whose blocks run along the
  * rows of x: a product takes each operand packed along the dimension it sums over. */
 uint64_t om_pack8_bytes(int rows, int cols);
-/* x8 = x packed and xt8 = x^T packed, from one pass over x (rows of ld_x >= cols floats); either may be NULL, not both. */
+/* x8 = x packed and xt8 = x^T packed, in one launch (x: rows of ld_x >= cols floats); either may be NULL, not both. */
 om_status om_pack8(om_ctx *ctx, const float *x, int ld_x, int rows, int cols, uint8_t *x8, uint8_t *xt8);
 /* y[r][c] (+)= the packed value (rows of ld_y >= cols floats; what stands behind a row's cols values is left alone). */
 om_status om_unpack8(om_ctx *ctx, const uint8_t *x8, float *y, int ld_y, int rows, int cols, int acc);
@@ -396,7 +396,8 @@ om_status om_unpack8(om_ctx *ctx, const uint8_t *x8, float *y, int ld_y, int row
 om_status om_gemm8(om_ctx *ctx, int m, int n, int k, const uint8_t *a8, const uint8_t *b8, const float *bias, float *c,
                    int ldc, int acc);
 /* om_linear_bwd with the layer's input kept as xt8, the packed transpose of x [rows, in]: dw (+)= g^T x (every product
- * exact but for bits of g below 2^-126, sums fp32) and db (+)= fp64 column sums of g; dx (+)= g w is om_linear_bwd's. Each output may be NULL. */
+ * exact but for bits of g below 2^-126, sums fp32) and db (+)= fp64 column sums of g; dx (+)= g w is om_linear_bwd's. Each
+ * output may be NULL. */
 om_status om_linear_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *xt8, const float *w, float *dx, float *dw, float *db,
                            int rows, int in, int out, int acc_dx, int acc_dw, int acc_db);
 /* om_gelu_fwd over [rows, cols] that keeps its input packed, and its backward from that: dx (+)= g * gelu'(value of x8).
