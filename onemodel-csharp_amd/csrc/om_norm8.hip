@@ -11,6 +11,8 @@
 // block of 128. Rows past 16384 columns (backward: 8192, whose column sums need the registers) are read again for each pass.
 #include "om_pack8.hpp"
 
+#include <algorithm>
+#include <cmath>
 #include <type_traits>
 
 namespace {
@@ -110,13 +112,18 @@ __global__ void __launch_bounds__(256) k_ln8(const float *x, const float *__rest
 
 // A workgroup takes `chunk` rows: sixteen wavefronts a row each (NW = 1; eight past 512 columns, whose sums need the
 // registers), or four to a row (NW = 4). Every lane keeps the fp64 sums of its own columns and leaves them as one partial row
-// of the workgroup's (added over its wavefronts through LDS in order where several share the columns).
+// of the workgroup's (added over its wavefronts through LDS in order where several share the columns). A workgroup that is the only one leaves the sums themselves, out (+)= sum.
+struct Sums {
+    double *part;  // the partial rows, or null
+    float *out;
+    int acc;
+};
 template <int NW, int NV>
 constexpr int kBwdThreads = NW > 1 ? 256 : NV <= 2 ? 1024 : 512;
 template <int NW, int NV, bool ACC>
-__global__ void __launch_bounds__((kBwdThreads<NW, NV>)) k_ln8_bwd(const float *g, Packed p, const float *__restrict__ gamma,
-                                                             const float *__restrict__ rstd, float *dx, double *part_g,
-                                                             double *part_b, int64_t rows, int64_t cols, int chunk) {
+__global__ void __launch_bounds__((kBwdThreads<NW, NV>))
+    k_ln8_bwd(const float *g, Packed p, const float *__restrict__ gamma, const float *__restrict__ rstd, float *dx, Sums dgamma,
+              Sums dbeta, int64_t rows, int64_t cols, int chunk) {
     OM_LDS_POISON();
     constexpr int L = 64 * NW, WAVES = kBwdThreads<NW, NV> / 64, AT_ONCE = WAVES / NW;
     __shared__ float sh[4];
@@ -175,9 +182,12 @@ __global__ void __launch_bounds__((kBwdThreads<NW, NV>)) k_ln8_bwd(const float *
             }
         }
     }
-    auto leave = [&](double *part, const double (&sum)[4 * NV]) {
-        if (!part) return;
-        part += (int64_t)blockIdx.x * cols;
+    auto leave = [&](const Sums &to, const double (&sum)[4 * NV]) {
+        if (!to.part && !to.out) return;
+        auto put = [&](int64_t c, double v) {
+            if (to.part) to.part[(int64_t)blockIdx.x * cols + c] = v;
+            else to.out[c] = to.acc ? to.out[c] + (float)v : (float)v;
+        };
 #pragma unroll
         for (int i = 0; i < NV; i++) {
             if constexpr (NW == 1) {  // the wavefronts' sums of these 256 columns: value e of lane t at 64 e + t
@@ -190,17 +200,17 @@ __global__ void __launch_bounds__((kBwdThreads<NW, NV>)) k_ln8_bwd(const float *
                     double v = cs[64 * w + t];
 #pragma unroll
                     for (int k = 1; k < WAVES; k++) v += cs[256 * k + 64 * w + t];
-                    part[c] = v;
+                    put(c, v);
                 }
             } else {
 #pragma unroll
                 for (int e = 0; e < 4; e++)
-                    if (at(i) + e < cols) part[at(i) + e] = sum[4 * i + e];
+                    if (at(i) + e < cols) put(at(i) + e, sum[4 * i + e]);
             }
         }
     };
-    leave(part_g, sg);
-    leave(part_b, sb);
+    leave(dgamma, sg);
+    leave(dbeta, sb);
 }
 
 // dx alone for rows of any length: both passes over the row read it again.
@@ -280,6 +290,22 @@ void by_width(int64_t cols, int64_t kept, F f) {
 #undef OM_LN8
 }
 
+// Rows to a workgroup of the backward. Up to 1024 columns its eight or sixteen wavefronts take a row each and a CU holds one
+// workgroup, so 256 of them are one round (8192 x 384 12.1 us, 512 of them 15.3), and up to 32 (24) rows one alone saves the
+// second launch (24 x 384 6.2 us, 7.5 in three). Of longer rows a workgroup takes 0.7 to 2 us each, one after the other, and its
+// sums are a row to write, read and add: the two together are least about sqrt(rows / 32) (64 x 4096: 11.3 us by two, 28.4 by
+// sixteen; 4096 x 2048 25 us by eight, 29 by sixteen), with two workgroups a CU at most, or one past 4096 columns, of which a CU
+// holds no more (8192 x 8192: 145 us by 32 rows, 165 by 16).
+int rows_each(int64_t rows, int64_t cols, int cus) {
+    if (cols <= kOneWave) {
+        const int alone = cols <= 512 ? 32 : 24;
+        return rows <= alone ? alone : (int)std::max<int64_t>(8, (rows + cus - 1) / cus);
+    }
+    if (rows <= 2) return 2;
+    const int64_t most = cols > 4096 ? cus : 2 * cus;
+    return (int)std::max<int64_t>((rows + most - 1) / most, (int64_t)std::sqrt((double)rows / 32));
+}
+
 }  // namespace
 
 extern "C" {
@@ -313,11 +339,10 @@ om_status om_layernorm_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *xh8, c
     OM_REQUIRE(ctx, cols <= 65535 * 1024 && (cols <= kKeptBwd || launches(rows, 256)),
                "om_layernorm_bwd_x8: %d x %d is more than a launch takes", rows, cols);
     if (om_status s = om::use_device(ctx)) return s;
-    // chunks of rows: as many as two workgroups a CU, of at least 16 rows
-    const int64_t most = 2 * (int64_t)ctx->num_cus, even = (rows + most - 1) / most;
-    const int chunk = even < 16 ? 16 : (int)even, chunks = (int)(((int64_t)rows + chunk - 1) / chunk);
+    const int chunk = rows_each(rows, cols, ctx->num_cus), chunks = (int)(((int64_t)rows + chunk - 1) / chunk);
+    const bool one = chunks == 1 && cols <= kKeptBwd;
     double *pg = nullptr, *pb = nullptr;
-    if (dgamma || dbeta) {
+    if (!one && (dgamma || dbeta)) {
         float *scr;
         if (om_status s = om::scratch(ctx, sizeof(double) * 2ull * (uint64_t)chunks * (uint64_t)cols, &scr)) return s;
         double *base = reinterpret_cast<double *>(scr);
@@ -330,7 +355,8 @@ om_status om_layernorm_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *xh8, c
             constexpr int NW = decltype(nw)::value, NV = decltype(nv)::value;
             if constexpr (NV && 256 * NW * NV <= kKeptBwd) {
                 auto go = [&](auto kern) {
-                    hipLaunchKernelGGL(kern, dim3((unsigned)chunks), dim3(kBwdThreads<NW, NV>), 0, ctx->stream, g, p, gamma, rstd, dx, pg, pb,
+                    hipLaunchKernelGGL(kern, dim3((unsigned)chunks), dim3(kBwdThreads<NW, NV>), 0, ctx->stream, g, p, gamma, rstd, dx,
+                                       Sums{pg, one ? dgamma : nullptr, acc_params}, Sums{pb, one ? dbeta : nullptr, acc_params},
                                        (int64_t)rows, (int64_t)cols, chunk);
                 };
                 acc_dx ? go(k_ln8_bwd<NW, NV, true>) : go(k_ln8_bwd<NW, NV, false>);
@@ -346,6 +372,7 @@ om_status om_layernorm_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *xh8, c
             }
         });
     if (om_status s = OM_LAUNCH_CHECK(ctx, "om_layernorm_bwd_x8")) return s;
+    if (one) return OM_OK;
     if (dgamma && dbeta) return om::chunk_final(ctx, pg, chunks, cols, dgamma, acc_params, pb, dbeta);
     if (dgamma) return om::chunk_final(ctx, pg, chunks, cols, dgamma, acc_params);
     return dbeta ? om::chunk_final(ctx, pb, chunks, cols, dbeta, acc_params) : OM_OK;

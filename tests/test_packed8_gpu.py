@@ -399,7 +399,9 @@ def test_gelu_gradient_against_differences(dev):
 
 
 NORMS = [(1, 1), (1, 7), (3, 128), (5, 130), (64, 256), (33, 384), (130, 500), (70, 768), (9, 1023), (40, 1024), (21, 1025),
-         (17, 2047), (12, 3000), (600, 4096), (5, 5000), (3, 8192), (4, 8200), (2, 16384), (3, 20000)]
+         (17, 2047), (12, 3000), (600, 4096), (5, 5000), (3, 8192), (4, 8200), (2, 16384), (3, 20000),
+         # one workgroup, a few rows to each, and many
+         (24, 384), (32, 512), (33, 100), (25, 640), (64, 1100), (300, 2048), (100, 5000), (3000, 130), (2100, 1030), (9000, 64)]
 
 
 @pytest.mark.parametrize("rows,cols", NORMS)
