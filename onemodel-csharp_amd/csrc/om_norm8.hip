@@ -6,9 +6,10 @@
 // q = g gamma: dx = rstd (q - mean(q) - h mean(q h)), dgamma = sum of g h, dbeta = sum of g.
 //
 // Bound: HBM, 9 bytes a value each way (x or g 4, the packed rows 1, y or dx 4): 16384 x 4096 252 us both ways, 4.8 TB/s;
-// 4096 x 384 15.8 us, three launches near their latency. A row is read once and stays in registers:
-// one wavefront to a row of up to 1024, a workgroup to a longer one, four values a lane at a time, so that 32 lanes hold a
-// block of 128. Rows past 16384 columns (backward: 8192, whose column sums need the registers) are read again for each pass.
+// 4096 x 384 15.8 us, three launches near their latency. A row is read once and stays in registers: one wavefront to a row of up
+// to 1024 columns, then four, eight past 4096 and sixteen past 8192 (one row of 8192 forward 5.5 us by eight, 7.2 by four; 4096
+// rows of 16384 141 us by sixteen, 173 by four), four values a lane at a time, so that 32 lanes hold a block of 128. Rows past
+// 16384 columns (backward: 8192, whose column sums need the registers) are read again for each pass.
 #include "om_pack8.hpp"
 
 #include <algorithm>
@@ -43,15 +44,15 @@ __device__ __forceinline__ void put_codes(const Packed &p, int64_t row, int64_t 
     if ((threadIdx.x & 31) == 0) p.s[row * p.lds + blk] = (uint8_t)s;
 }
 
-// NW wavefronts to a row (4 / NW rows to a workgroup), NV quads of 64 NW lanes. NV = 0: any number, read again for each pass.
+// NW wavefronts to a row (of one, four rows to a workgroup), NV quads of 64 NW lanes. NV = 0: any number, read again for each pass.
 template <int NW, int NV>
-__global__ void __launch_bounds__(256) k_ln8(const float *x, const float *__restrict__ gamma, const float *__restrict__ beta,
+__global__ void __launch_bounds__(NW == 1 ? 256 : 64 * NW) k_ln8(const float *x, const float *__restrict__ gamma, const float *__restrict__ beta,
                                              float *y, Packed p, float *__restrict__ rstd, int64_t rows, int64_t cols,
                                              float eps, double inv_n) {
     OM_LDS_POISON();
-    __shared__ double sh[4];
+    __shared__ double sh[NW];
     constexpr int L = 64 * NW, KEEP = NV ? NV : 1;
-    const int64_t row = (int64_t)blockIdx.x * (4 / NW) + (NW == 1 ? threadIdx.x >> 6 : 0);
+    const int64_t row = NW == 1 ? (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
     if (row >= rows) return;  // whole rows leave; a row of more than one wavefront is its workgroup's only one
     const int t = threadIdx.x % L;
     const float *xr = x + row * cols;
@@ -119,14 +120,14 @@ struct Sums {
     int acc;
 };
 template <int NW, int NV>
-constexpr int kBwdThreads = NW > 1 ? 256 : NV <= 2 ? 1024 : 512;
+constexpr int kBwdThreads = NW > 1 ? 64 * NW : NV <= 2 ? 1024 : 512;
 template <int NW, int NV, bool ACC>
 __global__ void __launch_bounds__((kBwdThreads<NW, NV>))
     k_ln8_bwd(const float *g, Packed p, const float *__restrict__ gamma, const float *__restrict__ rstd, float *dx, Sums dgamma,
               Sums dbeta, int64_t rows, int64_t cols, int chunk) {
     OM_LDS_POISON();
     constexpr int L = 64 * NW, WAVES = kBwdThreads<NW, NV> / 64, AT_ONCE = WAVES / NW;
-    __shared__ float sh[4];
+    __shared__ float sh[NW];
     __shared__ double cs[NW == 1 ? WAVES * 256 : 1];
     const int t = threadIdx.x % L, w = threadIdx.x >> 6;
     const int64_t r0 = (int64_t)blockIdx.x * chunk, r1 = min(rows, r0 + chunk);
@@ -283,10 +284,10 @@ __global__ void __launch_bounds__(256) k_ln8_params_long(const float *__restrict
 constexpr int64_t kKeptFwd = 16384, kKeptBwd = 8192, kOneWave = 1024;  // kOneWave: a wavefront to a row
 template <class F>
 void by_width(int64_t cols, int64_t kept, F f) {
-    if (cols > kept) return f(std::integral_constant<int, 4>(), std::integral_constant<int, 0>());
+    if (cols > kept) return f(std::integral_constant<int, 16>(), std::integral_constant<int, 0>());
 #define OM_LN8(NW, NV) \
     if (cols <= 256 * NW * NV) return f(std::integral_constant<int, NW>(), std::integral_constant<int, NV>());
-    OM_LN8(1, 1) OM_LN8(1, 2) OM_LN8(1, 3) OM_LN8(1, 4) OM_LN8(4, 2) OM_LN8(4, 3) OM_LN8(4, 4) OM_LN8(4, 8) OM_LN8(4, 16)
+    OM_LN8(1, 1) OM_LN8(1, 2) OM_LN8(1, 3) OM_LN8(1, 4) OM_LN8(4, 2) OM_LN8(4, 3) OM_LN8(4, 4) OM_LN8(8, 4) OM_LN8(16, 4)
 #undef OM_LN8
 }
 
@@ -317,13 +318,13 @@ om_status om_layernorm_fwd_x8(om_ctx *ctx, const float *x, const float *gamma, c
     OM_REQUIRE(ctx, aligned16(xh8), "om_layernorm_fwd_x8: packed tensors start at multiples of 16 bytes");
     if (rows == 0) return OM_OK;
     OM_REQUIRE(ctx, x && gamma && beta && y && xh8 && rstd, "om_layernorm_fwd_x8: NULL pointer");
-    OM_REQUIRE(ctx, launches(cols <= kOneWave ? ((int64_t)rows + 3) / 4 : rows, 256),
+    OM_REQUIRE(ctx, cols <= kOneWave ? launches(((int64_t)rows + 3) / 4, 256) : launches(rows, 1024),
                "om_layernorm_fwd_x8: %d x %d is more than a launch takes", rows, cols);
     if (om_status s = om::use_device(ctx)) return s;
     const Packed p = packed(xh8, rows, cols);
     by_width(cols, kKeptFwd, [&](auto nw, auto nv) {
         constexpr int NW = decltype(nw)::value, NV = decltype(nv)::value;
-        hipLaunchKernelGGL((k_ln8<NW, NV>), dim3((unsigned)(((int64_t)rows * NW + 3) / 4)), dim3(256), 0, ctx->stream, x,
+        hipLaunchKernelGGL((k_ln8<NW, NV>), dim3((unsigned)(NW == 1 ? ((int64_t)rows + 3) / 4 : rows)), dim3(NW == 1 ? 256 : 64 * NW), 0, ctx->stream, x,
                            gamma, beta, y, p, rstd, (int64_t)rows, (int64_t)cols, eps, 1.0 / cols);
     });
     return OM_LAUNCH_CHECK(ctx, "om_layernorm_fwd_x8");
