@@ -272,12 +272,11 @@ __global__ void __launch_bounds__(1024) k_colsum_one(const float *__restrict__ g
         if (r0 + 4 * e < rows) a += (double)v[e];
     sub[w][t] = a;
     __syncthreads();
-    if (w >= 16) return;  // whole wavefronts; the others are a quarter of the barriers that follow
-    double s = 0.0;       // chunk w's sum
+    double s = 0.0;  // chunk w's sum
     if (w < chunks)
 #pragma unroll
         for (int q = 0; q < 4; q++) s += sub[4 * w + q][t];
-    sh[w][t] = s;
+    if (w < 16) sh[w][t] = s;
 #pragma unroll
     for (int o = 8; o > 0; o >>= 1) {
         __syncthreads();
