@@ -128,7 +128,7 @@ __global__ void __launch_bounds__((kBwdThreads<NW, NV>))
     OM_LDS_POISON();
     constexpr int L = 64 * NW, WAVES = kBwdThreads<NW, NV> / 64, AT_ONCE = WAVES / NW;
     __shared__ float sh[NW];
-    __shared__ double cs[NW == 1 ? WAVES * 256 : 1];
+    __shared__ double cs[NW == 1 ? 2 * NV * WAVES * 256 : 1];
     const int t = threadIdx.x % L, w = threadIdx.x >> 6;
     const int64_t r0 = (int64_t)blockIdx.x * chunk, r1 = min(rows, r0 + chunk);
     double sg[4 * NV], sb[4 * NV];
@@ -183,35 +183,37 @@ __global__ void __launch_bounds__((kBwdThreads<NW, NV>))
             }
         }
     }
-    auto leave = [&](const Sums &to, const double (&sum)[4 * NV]) {
-        if (!to.part && !to.out) return;
-        auto put = [&](int64_t c, double v) {
-            if (to.part) to.part[(int64_t)blockIdx.x * cols + c] = v;
-            else to.out[c] = to.acc ? to.out[c] + (float)v : (float)v;
-        };
-#pragma unroll
-        for (int i = 0; i < NV; i++) {
-            if constexpr (NW == 1) {  // the wavefronts' sums of these 256 columns: value e of lane t at 64 e + t
-                __syncthreads();
-#pragma unroll
-                for (int e = 0; e < 4; e++) cs[256 * w + 64 * e + t] = sum[4 * i + e];
-                __syncthreads();
-                const int64_t c = 256 * (int64_t)i + 4 * t + w;
-                if (w < 4 && c < cols) {
-                    double v = cs[64 * w + t];
-#pragma unroll
-                    for (int k = 1; k < WAVES; k++) v += cs[256 * k + 64 * w + t];
-                    put(c, v);
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (at(i) + e < cols) put(at(i) + e, sum[4 * i + e]);
-            }
-        }
+    auto put = [&](const Sums &to, int64_t c, double v) {
+        if (c >= cols) return;
+        if (to.part) to.part[(int64_t)blockIdx.x * cols + c] = v;
+        else if (to.out) to.out[c] = to.acc ? to.out[c] + (float)v : (float)v;
     };
-    leave(dgamma, sg);
-    leave(dbeta, sb);
+    if constexpr (NW == 1) {  // value e of quad i of lane t at 256 i + 64 e + t, a row of them to each wavefront
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                cs[(256 * w + 64 * e + t) + 256 * WAVES * i] = sg[4 * i + e];
+                cs[(256 * w + 64 * e + t) + 256 * WAVES * (NV + i)] = sb[4 * i + e];
+            }
+        __syncthreads();
+        for (int q = threadIdx.x; q < 512 * NV; q += 64 * WAVES) {
+            const double *from = cs + 256 * WAVES * (q >> 8) + (q & 255);
+            double v = from[0];
+#pragma unroll
+            for (int k = 1; k < WAVES; k++) v += from[256 * k];
+            const bool b = q >= 256 * NV;
+            put(b ? dbeta : dgamma, 256 * (int64_t)((q >> 8) - (b ? NV : 0)) + 4 * (q & 63) + ((q >> 6) & 3), v);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < NV; i++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                put(dgamma, at(i) + e, sg[4 * i + e]);
+                put(dbeta, at(i) + e, sb[4 * i + e]);
+            }
+    }
 }
 
 // dx alone for rows of any length: both passes over the row read it again.
@@ -293,7 +295,7 @@ void by_width(int64_t cols, int64_t kept, F f) {
 
 // Rows to a workgroup of the backward. Up to 1024 columns its eight or sixteen wavefronts take a row each and a CU holds one
 // workgroup, so 256 of them are one round (8192 x 384 12.1 us, 512 of them 15.3), and up to 32 (24) rows one alone saves the
-// second launch (24 x 384 6.2 us, 7.5 in three). Of longer rows a workgroup takes 0.7 to 2 us each, one after the other, and its
+// second launch (24 x 384 5.3 us, 6.6 in three). Of longer rows a workgroup takes 0.7 to 2 us each, one after the other, and its
 // sums are a row to write, read and add: the two together are least about sqrt(rows / 32) (64 x 4096: 11.3 us by two, 28.4 by
 // sixteen; 4096 x 2048 25 us by eight, 29 by sixteen), with two workgroups a CU at most, or one past 4096 columns, of which a CU
 // holds no more (8192 x 8192: 145 us by 32 rows, 165 by 16).
