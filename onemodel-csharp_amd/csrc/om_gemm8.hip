@@ -467,14 +467,27 @@ __global__ void __launch_bounds__(64 * NW) k_gemm8_thin(Gemm8 p) {
     to.put(r, col, v, to.bias_of(col));
 }
 
+// The sum of `parts` values `stride` apart, in order, eight loads in flight.
+template <class T>
+__device__ __forceinline__ T add_parts(const T *p, int64_t stride, int parts) {
+    T v = p[0];
+    for (int s0 = 1; s0 < parts; s0 += 8) {
+        T w[8];
+#pragma unroll
+        for (int u = 0; u < 8; u++) w[u] = s0 + u < parts ? p[(s0 + u) * stride] : T(0);
+#pragma unroll
+        for (int u = 0; u < 8; u++)
+            if (s0 + u < parts) v += w[u];
+    }
+    return v;
+}
+
 // Adds the splits' sums in order, then bias and C.
 __global__ void __launch_bounds__(256) k_gemm8_join(Gemm8 p) {
     OM_LDS_POISON();
     const int64_t total = (int64_t)p.m * p.n, step = (int64_t)gridDim.x * 256;
     for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
-        float v = p.ws[i];
-#pragma unroll 4
-        for (int s = 1; s < p.splits; s++) v += p.ws[s * total + i];
+        float v = add_parts(p.ws + i, total, p.splits);
         const int64_t row = i / p.n, col = i - row * p.n;
         if (p.bias) v = v + p.bias[col];
         float *c = p.c + row * p.ldc + col;
@@ -832,15 +845,12 @@ __global__ void __launch_bounds__(256) k_dw8_join(Dw8 p) {
     OM_LDS_POISON();
     const int64_t total = (int64_t)p.m * p.n, step = (int64_t)gridDim.x * 256, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
     for (int64_t i = at; i < total; i += step) {
-        float v = p.ws[i];
-#pragma unroll 4
-        for (int s = 1; s < p.splits; s++) v += p.ws[s * total + i];
+        const float v = add_parts(p.ws + i, total, p.splits);
         p.dw[i] = p.acc_dw ? p.dw[i] + v : v;
     }
     if (!p.db) return;
     for (int64_t i = at; i < p.m; i += step) {
-        double c = p.cs[i];
-        for (int s = 1; s < p.splits; s++) c += p.cs[(int64_t)s * p.m + i];
+        const double c = add_parts(p.cs + i, (int64_t)p.m, p.splits);
         p.db[i] = p.acc_db ? p.db[i] + (float)c : (float)c;
     }
 }
