@@ -498,8 +498,8 @@ __global__ void __launch_bounds__(256) k_gemm8_join(Gemm8 p) {
 // A kernel's tile and what its workgroups take, in us, with `resident` of them on a CU at most: `fix` a round of those and
 // `each` a workgroup, and for a stage of kw blocks of k `alone` where a CU has one workgroup, `shared` a workgroup where it
 // has more; with every CU busy the clock falls and the caches fill, and a stage takes `chip` a workgroup and CU. Fitted to 4080
-// (products) and 4611 (weight gradients) times over all kernels, splits of k from 1 to 16 and sizes from 1 to 16384; the
-// choice by them is 0.8 % (0.5 %) behind the best of all those in the mean, 21 % (26 %) at most.
+// (products) and 4383 (weight gradients) times over all kernels, splits of k and sizes from 1 to 16384; the choice by them is
+// 0.8 % (0.3 %) behind the best of all those in the mean, 11 % (9 %) at most.
 struct Tile {
     int bm, bn, kw, resident;
     float fix, each, alone, shared, chip;
@@ -507,19 +507,21 @@ struct Tile {
 struct Choice {
     int tile, splits;
 };
-// Splitting k costs a second launch that adds the parts, `join` us and `join_each` a million values.
+// Splitting k costs a second launch that adds the parts, `join` us and `join_each` a million values; `most` parts of `least` blocks
+// (weight gradients of few columns gain from up to 32 parts of two: 16384 x 64 x 64 11.5 us, 12.8 by 16 of four; products do not).
 template <int N>
-Choice choose(const Tile (&tiles)[N], int cus, int64_t m, int64_t n, int blocks, int64_t row_bytes, float join, float join_each) {
+Choice choose(const Tile (&tiles)[N], int cus, int64_t m, int64_t n, int blocks, int64_t row_bytes, float join, float join_each, int most,
+              int least) {
     Choice best = {-1, 1};
-    double least = 0.0;
+    double shortest = 0.0;
     // comparisons of one kernel or split: a number that is none of them leaves no choice
     const char *only_tile = om::tuning_env("OM_TILE8"), *only_splits = om::tuning_env("OM_SPLITS8");
     for (int t = 0; t < N; t++) {
         const Tile &c = tiles[t];
         if (only_tile && atoi(only_tile) != t) continue;
         if ((c.bm > c.bn ? c.bm : c.bn) * row_bytes > INT64_C(0xFFFFFFFF)) continue;  // offsets inside a tile: 32 bits
-        for (int s : {1, 2, 3, 4, 6, 8, 12, 16}) {
-            if (s > 1 && blocks < 4 * s) break;
+        for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
+            if (s > 1 && (s > most || blocks < least * s)) break;
             if (only_splits && atoi(only_splits) != s) continue;
             const int per = ((blocks + s - 1) / s + c.kw - 1) / c.kw * c.kw, parts = per ? (blocks + per - 1) / per : 1;
             const double wgs = (double)((m + c.bm - 1) / c.bm) * (double)((n + c.bn - 1) / c.bn) * parts;
@@ -527,8 +529,8 @@ Choice choose(const Tile (&tiles)[N], int cus, int64_t m, int64_t n, int blocks,
             double us = c.fix * rounds + c.each * load +
                         std::fmax(std::fmax(c.alone * rounds, c.shared * load), c.chip * wgs / cus) * stages;
             if (parts > 1) us += join + join_each * parts * (double)m * (double)n * 1e-6;
-            if (best.tile < 0 || us < least) {
-                least = us;
+            if (best.tile < 0 || us < shortest) {
+                shortest = us;
                 best = {t, s};
             }
         }
@@ -541,9 +543,9 @@ inline void split_blocks(int blocks, int kw, int splits, int &per, int &parts) {
     parts = blocks > per ? (blocks + per - 1) / per : 1;
 }
 
-constexpr Tile kTiles[] = {{256, 256, 1, 1, 5.26f, 0.32f, 2.484f, 0.44f, 3.11f}, {128, 128, 1, 2, 0.0f, 3.41f, 0.862f, 0.413f, 0.997f},
-                           {128, 64, 1, 3, 0.0f, 1.26f, 0.656f, 0.463f, 0.548f}, {64, 64, 1, 4, 0.0f, 0.56f, 0.485f, 0.3f, 0.272f},
-                           {32, 32, 1, 4, 0.28f, 0.63f, 0.197f, 0.096f, 0.1f},   {32, 32, 2, 2, 0.0f, 1.2f, 0.252f, 0.209f, 0.195f}};
+constexpr Tile kTiles[] = {{256, 256, 1, 1, 7.85f, 0.37f, 3.003f, 0.447f, 3.436f}, {128, 128, 1, 2, 0.0f, 3.0f, 0.925f, 0.413f, 1.005f},
+                           {128, 64, 1, 3, 0.0f, 1.09f, 0.61f, 0.513f, 0.436f},     {64, 64, 1, 4, 0.07f, 0.49f, 0.425f, 0.293f, 0.308f},
+                           {32, 32, 1, 4, 0.44f, 0.54f, 0.204f, 0.085f, 0.095f},    {32, 32, 2, 2, 0.0f, 1.22f, 0.214f, 0.155f, 0.188f}};
 
 om_status gemm8(om_ctx *ctx, Gemm8 p) {
     // Up to 16 rows the thin kernel is the fastest (4 x 4096 x 4096: 5.6 us, the best of the others 8.2) until a wavefront has so
@@ -555,7 +557,7 @@ om_status gemm8(om_ctx *ctx, Gemm8 p) {
         hipLaunchKernelGGL((k_gemm8_thin<4, 4>), dim3((unsigned)(((int64_t)p.n + 15) / 16)), dim3(256), 0, ctx->stream, p);
         return OM_LAUNCH_CHECK(ctx, "om_gemm8");
     }
-    const Choice ch = choose(kTiles, ctx->num_cus, p.m, p.n, p.blocks, p.a.ldq, 2.38f, 0.82f);
+    const Choice ch = choose(kTiles, ctx->num_cus, p.m, p.n, p.blocks, p.a.ldq, 1.96f, 1.06f, 16, 4);
     OM_REQUIRE(ctx, ch.tile >= 0, "om_gemm8: k is more than a launch takes");
     const Tile &c = kTiles[ch.tile];
     p.tiles_m = (int)(((int64_t)p.m + c.bm - 1) / c.bm);
@@ -841,27 +843,30 @@ __global__ void __launch_bounds__(256, 2) k_dw8(Dw8 p) {
     }
 }
 
-__global__ void __launch_bounds__(256) k_dw8_join(Dw8 p) {
+// Adds the parts in order: dW's, and by the workgroups from `tiles` on the column sums'.
+__global__ void __launch_bounds__(256) k_dw8_join(Dw8 p, unsigned tiles) {
     OM_LDS_POISON();
-    const int64_t total = (int64_t)p.m * p.n, step = (int64_t)gridDim.x * 256, at = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    for (int64_t i = at; i < total; i += step) {
+    if (blockIdx.x >= tiles) {
+        const int64_t i = (int64_t)(blockIdx.x - tiles) * 256 + threadIdx.x;
+        if (i >= p.m) return;
+        const float v = (float)add_parts(p.cs + i, (int64_t)p.m, p.splits);
+        p.db[i] = p.acc_db ? p.db[i] + v : v;
+        return;
+    }
+    const int64_t total = (int64_t)p.m * p.n, step = (int64_t)tiles * 256;
+    for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += step) {
         const float v = add_parts(p.ws + i, total, p.splits);
         p.dw[i] = p.acc_dw ? p.dw[i] + v : v;
     }
-    if (!p.db) return;
-    for (int64_t i = at; i < p.m; i += step) {
-        const double c = add_parts(p.cs + i, (int64_t)p.m, p.splits);
-        p.db[i] = p.acc_db ? p.db[i] + (float)c : (float)c;
-    }
 }
 
-constexpr Tile kTilesDw[] = {{32, 128, 1, 2, 0.77f, 1.63f, 0.76f, 0.696f, 0.72f},
-                             {32, 64, 1, 3, 0.71f, 0.62f, 0.563f, 0.463f, 0.471f},
-                             {32, 32, 1, 2, 0.0f, 0.84f, 0.523f, 0.38f, 0.375f}};
+constexpr Tile kTilesDw[] = {{32, 128, 1, 2, 0.78f, 1.56f, 0.817f, 0.702f, 0.648f},
+                             {32, 64, 1, 3, 0.61f, 0.64f, 0.572f, 0.459f, 0.46f},
+                             {32, 32, 1, 2, 0.0f, 0.91f, 0.519f, 0.465f, 0.375f}};
 
 // Chooses the kernel for p (its tile in `tile`) and fills in the tiles and splits.
 om_status plan_dw8(om_ctx *ctx, Dw8 &p, int &tile) {
-    const Choice ch = choose(kTilesDw, ctx->num_cus, p.m, p.n, p.blocks, p.x.ldq, 3.44f, 0.71f);
+    const Choice ch = choose(kTilesDw, ctx->num_cus, p.m, p.n, p.blocks, p.x.ldq, 2.63f, 1.0f, 32, 2);
     OM_REQUIRE(ctx, ch.tile >= 0 && p.rows <= INT32_MAX - 255 && p.m < 1 << 26,
                "om_linear_bwd_x8: rows=%d in=%d out=%d is more than a launch takes", p.rows, p.n, p.m);
     const Tile &c = kTilesDw[tile = ch.tile];
@@ -887,9 +892,10 @@ om_status dw8(om_ctx *ctx, Dw8 p, int tile) {
         case 1: go(k_dw8<2, 2>); break;
         default: go(k_dw8<1, 3>); break;
     }
-    if (p.splits > 1)
-        hipLaunchKernelGGL(k_dw8_join, dim3(om::grid1d((int64_t)p.m * p.n, 256, (int64_t)ctx->num_cus * 8)), dim3(256), 0,
-                           ctx->stream, p);
+    if (p.splits > 1) {
+        const unsigned tiles = om::grid1d((int64_t)p.m * p.n, 256, (int64_t)ctx->num_cus * 8), sums = p.db ? (p.m + 255) / 256 : 0;
+        hipLaunchKernelGGL(k_dw8_join, dim3(tiles + sums), dim3(256), 0, ctx->stream, p, tiles);
+    }
     return OM_LAUNCH_CHECK(ctx, "om_linear_bwd_x8");
 }
 
