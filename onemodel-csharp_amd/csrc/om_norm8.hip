@@ -6,7 +6,7 @@
 // q = g gamma: dx = rstd (q - mean(q) - h mean(q h)), dgamma = sum of g h, dbeta = sum of g.
 //
 // Bound: HBM, 9 bytes a value each way (x or g 4, the packed rows 1, y or dx 4): 16384 x 4096 252 us both ways, 4.8 TB/s;
-// 4096 x 384 15.8 us, three launches near their latency. A row is read once and stays in registers: one wavefront to a row of up
+// 4096 x 384 15.2 us, three launches near their latency. A row is read once and stays in registers: one wavefront to a row of up
 // to 1024 columns, then four, eight past 4096 and sixteen past 8192 (one row of 8192 forward 5.5 us by eight, 7.2 by four; 4096
 // rows of 16384 141 us by sixteen, 173 by four), four values a lane at a time, so that 32 lanes hold a block of 128. Rows past
 // 16384 columns (backward: 8192, whose column sums need the registers) are read again for each pass.
