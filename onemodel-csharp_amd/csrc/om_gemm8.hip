@@ -390,81 +390,97 @@ __global__ void __launch_bounds__(256 * KW, KW < 2 ? 2 : KW) k_gemm8_few(Gemm8 p
     }
 }
 
-// At most 16 rows of A: a workgroup computes 16 columns on v_mfma_f32_16x16x32_bf16, its NW wavefronts a share of k each.
-// Each wavefront goes through its blocks of 128 k alone, D of them on their way into its own part of LDS (whole 128-byte rows;
-// loaded straight into fragments, 64 bytes of 16 rows at a time, they take three times as long), so nothing meets before the
-// sums do. Bound: latency, then B's bytes.
-template <int NW, int D>
+// At most 16 MR rows of A: a workgroup computes 16 columns on v_mfma_f32_16x16x32_bf16, its NW wavefronts a share of k each.
+// Each wavefront goes through its blocks of 128 k alone, the next one on its way into its own part of LDS while this one is
+// multiplied (whole 128-byte rows; loaded straight into fragments, 64 bytes of 16 rows at a time, they take three times as
+// long), so nothing meets before the sums do. More wavefronts hide a block's latency better than more blocks in flight (17 x 2048
+// x 2048: eight 4.1 us, four with two blocks each 4.45) until a CU has several workgroups (17 x 8192 x 4096: eight 9.2, four 8.2).
+// Bound: latency, then B's bytes (16 x 4096 x 4096 5.2 us, 3.2 TB/s).
+template <int NW, int MR>
 __global__ void __launch_bounds__(64 * NW) k_gemm8_thin(Gemm8 p) {
     OM_LDS_POISON();
     typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-    constexpr int SLOT = 4096 + 256, LOADS = 5;
-    __shared__ __attribute__((aligned(16))) char sh[NW * D * SLOT];
+    constexpr int ROWS = 16 * (MR + 1), SCALES = (ROWS + 63) / 64, SLOT = ROWS * 128 + SCALES * 256;
+    constexpr int AT_B = MR * 2048, AT_S = ROWS * 128, OUT = NW * MR * 1024, LDS = NW * SLOT > OUT ? NW * SLOT : OUT;
+    __shared__ __attribute__((aligned(16))) char sh[LDS];
     const int lane = threadIdx.x & 63, row = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16;
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int per = (p.blocks + NW - 1) / NW, b0 = wv * per, b1 = min(p.blocks, b0 + per);
     // Rows and columns past the last one are the last one again; what they give is not stored.
-    uint32_t oa[2], ob[2];
+    uint32_t oa[2 * MR], ob[2];
 #pragma unroll
-    for (int i = 0; i < 2; i++) {
+    for (int i = 0; i < 2 * MR; i++) {
         const int r = 8 * i + (lane >> 3), piece = (lane ^ (r >> 1)) & 7;
         oa[i] = (uint32_t)min(r, p.m - 1) * (uint32_t)p.a.ldq + 16 * piece;
-        ob[i] = (uint32_t)min(r, p.n - 1 - n0) * (uint32_t)p.b.ldq + 16 * piece;
+        if (i < 2) ob[i] = (uint32_t)min(r, p.n - 1 - n0) * (uint32_t)p.b.ldq + 16 * piece;
     }
     const uint8_t *qb = p.b.q + (int64_t)n0 * p.b.ldq;
-    // scale dwords: 16 rows of A, then 16 of B, and those again
-    const uint8_t *ss = lane & 16 ? p.b.s + (int64_t)min(n0 + row, p.n - 1) * p.b.lds : p.a.s + (int64_t)min(row, p.m - 1) * p.a.lds;
-    char *mine = sh + wv * D * SLOT;
-    const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)mine;
-    auto issue = [&](int blk) {  // past the last block that one again, into a slot that nothing reads
-        const uint32_t at = base + (uint32_t)((blk - b0) % D) * SLOT;
-        const int k = min(blk, b1 - 1);
+    // scale dwords: A's rows, then B's, and B's again
+    const uint8_t *ss[SCALES];
 #pragma unroll
-        for (int i = 0; i < 2; i++) {
-            load_to_lds(p.a.q + (int64_t)k * 128, oa[i], at + 1024 * i);
-            load_to_lds(qb + (int64_t)k * 128, ob[i], at + 2048 + 1024 * i);
-        }
-        load_to_lds4(ss + (k & ~3), at + 4096);
+    for (int i = 0; i < SCALES; i++) {
+        const int r = 64 * i + lane;
+        ss[i] = r < 16 * MR ? p.a.s + (int64_t)min(r, p.m - 1) * p.a.lds : p.b.s + (int64_t)min(n0 + row, p.n - 1) * p.b.lds;
+    }
+    const char *mine = sh + wv * SLOT;
+    const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)sh + (uint32_t)wv * SLOT;
+    auto issue = [&](int k) {
+#pragma unroll
+        for (int i = 0; i < 2 * MR; i++) load_to_lds(p.a.q + (int64_t)k * 128, oa[i], at + 1024 * i);
+#pragma unroll
+        for (int i = 0; i < 2; i++) load_to_lds(qb + (int64_t)k * 128, ob[i], at + AT_B + 1024 * i);
+#pragma unroll
+        for (int i = 0; i < SCALES; i++) load_to_lds4(ss[i] + (k & ~3), at + AT_S + 256 * i);
     };
-    floatx4 acc = {0.0f, 0.0f, 0.0f, 0.0f};
+    floatx4 acc[MR];
+#pragma unroll
+    for (int i = 0; i < MR; i++) acc[i] = floatx4{0.0f, 0.0f, 0.0f, 0.0f};
     if (b0 < b1) {
-#pragma unroll
-        for (int i = 0; i < D; i++) issue(b0 + i);
+        issue(b0);
         for (int blk = b0; blk < b1; blk++) {
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"((D - 1) * LOADS) : "memory");
-            const char *cur = mine + (blk - b0) % D * SLOT;
-            u32x4 a[2], b[2];
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            u32x4 a[MR + 1][2];  // B's last
+            float f[MR + 1];
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                a[j] = *reinterpret_cast<const u32x4 *>(cur + piece_at(row, 4 * j + g));
-                b[j] = *reinterpret_cast<const u32x4 *>(cur + 2048 + piece_at(row, 4 * j + g));
+            for (int i = 0; i <= MR; i++) {
+#pragma unroll
+                for (int j = 0; j < 2; j++) a[i][j] = *reinterpret_cast<const u32x4 *>(mine + 2048 * i + piece_at(row, 4 * j + g));
+                f[i] = scale_in(*reinterpret_cast<const uint32_t *>(mine + AT_S + 4 * (16 * i + row)), blk);
             }
-            const float fa = scale_in(*reinterpret_cast<const uint32_t *>(cur + 4096 + 4 * row), blk);
-            const float fb = scale_in(*reinterpret_cast<const uint32_t *>(cur + 4096 + 64 + 4 * row), blk);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read, so the slot may be loaded again
-            issue(blk + D);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read, so the next may be loaded over it
+            if (blk + 1 < b1) issue(blk + 1);
 #pragma unroll
             for (int j = 0; j < 2; j++)
 #pragma unroll
-                for (int t = 0; t < 2; t++)
-                    acc = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                        __builtin_bit_cast(bf16x8, widen8(a[j][2 * t], a[j][2 * t + 1], fa)),
-                        __builtin_bit_cast(bf16x8, widen8(b[j][2 * t], b[j][2 * t + 1], fb)), acc, 0, 0, 0);
+                for (int t = 0; t < 2; t++) {
+                    const auto b = __builtin_bit_cast(bf16x8, widen8(a[MR][j][2 * t], a[MR][j][2 * t + 1], f[MR]));
+#pragma unroll
+                    for (int i = 0; i < MR; i++)
+                        acc[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                            __builtin_bit_cast(bf16x8, widen8(a[i][j][2 * t], a[i][j][2 * t + 1], f[i])), b, acc[i], 0, 0, 0);
+                }
         }
     }
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
     float *out = reinterpret_cast<float *>(sh);
 #pragma unroll
-    for (int e = 0; e < 4; e++) out[wv * 256 + (4 * g + e) * 16 + row] = acc[e];
-    __syncthreads();
-    const int r = threadIdx.x >> 4, col = n0 + (threadIdx.x & 15);
-    if (r >= p.m || col >= p.n) return;
-    float v = out[threadIdx.x];
+    for (int i = 0; i < MR; i++)
 #pragma unroll
-    for (int w = 1; w < NW; w++) v += out[256 * w + threadIdx.x];
+        for (int e = 0; e < 4; e++) out[(wv * MR + i) * 256 + (4 * g + e) * 16 + row] = acc[i][e];
+    __syncthreads();
     const Out to(p, 0);
-    to.put(r, col, v, to.bias_of(col));
+    const int col = n0 + (threadIdx.x & 15);
+    if (col >= p.n) return;
+    const float bias = to.bias_of(col);
+#pragma unroll
+    for (int i = threadIdx.x >> 4; i < 16 * MR; i += 4 * NW) {
+        if (i >= p.m) break;
+        const int at = 16 * i + (threadIdx.x & 15);
+        float v = out[at];
+#pragma unroll
+        for (int w = 1; w < NW; w++) v += out[256 * MR * w + at];
+        to.put(i, col, v, bias);
+    }
 }
 
 // The sum of `parts` values `stride` apart, in order, eight loads in flight.
@@ -548,13 +564,26 @@ constexpr Tile kTiles[] = {{256, 256, 1, 1, 7.85f, 0.37f, 3.003f, 0.447f, 3.436f
                            {32, 32, 1, 4, 0.44f, 0.54f, 0.204f, 0.085f, 0.095f},    {32, 32, 2, 2, 0.0f, 1.22f, 0.214f, 0.155f, 0.188f}};
 
 om_status gemm8(om_ctx *ctx, Gemm8 p) {
-    // Up to 16 rows the thin kernel is the fastest (4 x 4096 x 4096: 5.6 us, the best of the others 8.2) until a wavefront has so
-    // many blocks one after the other that a split of k is worth its second launch (16 x 16 x 16384: 10.5 and 7.8 us).
-    if (p.m <= 16 && p.blocks <= 64) {
-        OM_REQUIRE(ctx, launches(((int64_t)p.n + 15) / 16, 256), "om_gemm8: n=%d is more than a launch takes", p.n);
+    // Up to 64 rows the thin kernel is the fastest (17 x 2048 x 2048 4.0 us, the best of the others 6.0; 64 x 2048 x 2048 5.2 and
+    // 6.2) until a wavefront has so many blocks one after the other that the others, or a split of k, are (16 x 16 x 16384 10.5 us
+    // and 7.8, 40 x 256 x 8192 8.6 and 7.8, 64 x 4096 x 4096 9.2 and 8.5).
+    constexpr int kMostBlocks[] = {64, 64, 48, 24};
+    const int mr = (int)(((int64_t)p.m + 15) / 16);
+    if (mr <= 4 && p.blocks <= kMostBlocks[mr - 1]) {
+        const int64_t wgs = ((int64_t)p.n + 15) / 16;
+        const int nw = wgs <= ctx->num_cus ? 8 : 4;
+        OM_REQUIRE(ctx, launches(wgs, 64 * nw), "om_gemm8: n=%d is more than a launch takes", p.n);
         if (om_status s = om::use_device(ctx)) return s;
         p.splits = 1;
-        hipLaunchKernelGGL((k_gemm8_thin<4, 4>), dim3((unsigned)(((int64_t)p.n + 15) / 16)), dim3(256), 0, ctx->stream, p);
+        auto go = [&](auto eight, auto four) {
+            hipLaunchKernelGGL(nw == 8 ? eight : four, dim3((unsigned)wgs), dim3(64 * nw), 0, ctx->stream, p);
+        };
+        switch (mr) {
+            case 1: go(k_gemm8_thin<8, 1>, k_gemm8_thin<4, 1>); break;
+            case 2: go(k_gemm8_thin<8, 2>, k_gemm8_thin<4, 2>); break;
+            case 3: go(k_gemm8_thin<8, 3>, k_gemm8_thin<4, 3>); break;
+            default: go(k_gemm8_thin<8, 4>, k_gemm8_thin<4, 4>); break;
+        }
         return OM_LAUNCH_CHECK(ctx, "om_gemm8");
     }
     const Choice ch = choose(kTiles, ctx->num_cus, p.m, p.n, p.blocks, p.a.ldq, 1.96f, 1.06f, 16, 4);
