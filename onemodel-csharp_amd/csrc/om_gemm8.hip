@@ -281,111 +281,86 @@ __global__ void __launch_bounds__(64 * WM * WN, WAVES) k_gemm8(Gemm8 p) {
     }
 }
 
-// Few tiles: the wavefronts of a workgroup share one tile of 32 x 32 and split k between them, four to a block of 128, so that
-// every code is widened once and a stage of KW blocks goes round without a barrier inside it. D stages stand in LDS, and
-// one more in registers. Their sums meet in LDS and are added in order. (777 x 333 x 1000: 6.1 us, by 64 x 64 tiles 9.1; with a
-// block of its own to each wavefront and no barriers 5.9, and 20.0 in place of 15.4 at 1000 x 2000 x 2000.)
-template <int KW, int D>
-__global__ void __launch_bounds__(256 * KW, KW < 2 ? 2 : KW) k_gemm8_few(Gemm8 p) {
+// Few tiles: the NW wavefronts of a workgroup share one tile of 32 x 32 and take every NW-th block of 128 k each, alone: the next
+// block is on its way into a wavefront's own part of LDS while this one is multiplied, and nothing meets before the sums do, in
+// LDS and in order. (Four wavefronts on quarters of each block, with a barrier a block and four blocks in flight: 777 x 333 x 1000
+// 6.2 us, so 5.2; 4096 x 384 x 1536 13.9 and 11.3; 100 x 4096 x 4096 11.7 and 9.4.)
+template <int NW>
+__global__ void __launch_bounds__(64 * NW) k_gemm8_few(Gemm8 p) {
     OM_LDS_POISON();
-    static_assert(4 % KW == 0, "a stage's scale bytes lie in one dword");
-    constexpr int NW = 4 * KW, BLOCK = 64 * 128, SS = KW * BLOCK, STAGE = SS + 256;
-    constexpr int LD = 33, OUT = NW * 32 * LD * 4, LDS = D * STAGE > OUT ? D * STAGE : OUT, PER = 2;
+    constexpr int SLOT = 64 * 128 + 256, LD = 33, OUT = NW * 32 * LD * 4, LDS = NW * SLOT > OUT ? NW * SLOT : OUT;
     __shared__ __attribute__((aligned(16))) char sh[LDS];
     const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
-    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), kb = wv >> 2, q = wv & 3;
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int split, tm, tn;
     tile_of(p.tiles_m, p.tiles_n, gridDim.x, split, tm, tn);
     const int m0 = 32 * tm, n0 = 32 * tn;
-    // Rows 0 .. 31 of a stage's block are A's, the others B's; this wavefront loads its quarter of block kb, eight rows of
-    // one operand an instruction.
-    const uint8_t *src[PER];
-    uint32_t off[PER];
+    const int b0 = split * p.per, b1 = min(p.blocks, b0 + p.per);
+    // Rows 0 .. 31 of a block are A's, the others B's, eight a load; rows past the last one load it again, and what they give is
+    // not stored.
+    const uint8_t *qa = p.a.q + (int64_t)m0 * p.a.ldq, *qb = p.b.q + (int64_t)n0 * p.b.ldq;
+    uint32_t off[8];
 #pragma unroll
-    for (int i = 0; i < PER; i++) {
-        const int r0 = 8 * (q * PER + i), r = r0 + (lane >> 3), piece = (lane ^ (r >> 1)) & 7;
-        const bool a = r0 < 32;
-        const Packed &o = a ? p.a : p.b;
-        const int first = a ? m0 : n0, last = (a ? p.m : p.n) - 1 - first;
-        src[i] = o.q + (int64_t)first * o.ldq;
-        off[i] = (uint32_t)min(a ? r : r - 32, last) * (uint32_t)o.ldq + 16 * piece;
+    for (int i = 0; i < 8; i++) {
+        const int r = 8 * i + (lane >> 3), piece = (lane ^ (r >> 1)) & 7;
+        const bool a = i < 4;
+        off[i] = (uint32_t)min(a ? r : r - 32, (a ? p.m - m0 : p.n - n0) - 1) * (uint32_t)(a ? p.a.ldq : p.b.ldq) + 16 * piece;
     }
-    // scale bytes: one instruction, A's rows and then B's
-    const uint8_t *ssrc = lane < 32 ? p.a.s + (int64_t)min(m0 + lane, p.m - 1) * p.a.lds
-                                    : p.b.s + (int64_t)min(n0 + lane - 32, p.n - 1) * p.b.lds;
-    const uint32_t base = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)sh;
-    const int b0 = split * p.per, b1 = min(p.blocks, b0 + p.per), stages = (b1 - b0 + KW - 1) / KW;
-    auto issue = [&](int st) {  // past the last stage the last one again, into a slot that nothing reads
-        const uint32_t at = base + (uint32_t)(st % D) * STAGE;
-        const int blk = min(b0 + min(st, stages - 1) * KW + kb, b1 - 1);
+    const uint8_t *ss = g ? p.b.s + (int64_t)min(n0 + l32, p.n - 1) * p.b.lds : p.a.s + (int64_t)min(m0 + l32, p.m - 1) * p.a.lds;
+    const char *mine = sh + wv * SLOT;
+    const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)sh + (uint32_t)wv * SLOT;
+    auto issue = [&](int k) {
 #pragma unroll
-        for (int i = 0; i < PER; i++) load_to_lds(src[i] + (int64_t)blk * 128, off[i], at + kb * BLOCK + (q * PER + i) * 1024);
-        if (wv == 0) load_to_lds4(ssrc + (blk & ~3), at + SS);
+        for (int i = 0; i < 8; i++) load_to_lds((i < 4 ? qa : qb) + (int64_t)k * 128, off[i], at + 1024 * i);
+        load_to_lds4(ss + (k & ~3), at + 64 * 128);
     };
     floatx16 acc[1][1];
 #pragma unroll
     for (int e = 0; e < 16; e++) acc[0][0][e] = 0.0f;
-    u32x4 raw[2][2], w[2][2];
-    uint32_t dw[2][2];
-    auto read = [&](int h, int st, int o) {
-        const char *cur = sh + (st % D) * STAGE;
-        dw[h][o] = *reinterpret_cast<const uint32_t *>(cur + SS + 4 * (32 * o + l32));
-        raw[h][o] = *reinterpret_cast<const u32x4 *>(cur + kb * BLOCK + piece_at(32 * o + l32, 2 * q + g));
-    };
-    // Stage st from registers, the next one's codes read meanwhile, its own slot loaded anew. (Blocks past the last one hold
-    // the last one's codes, which this wavefront drops.)
-    float sc[2][2];
-    auto turn = [&](int h, int st) {
-        land<(D - 2) * PER>();
-        issue(st + D);
+    if (b0 + wv < b1) {
+        issue(b0 + wv);
+        for (int blk = b0 + wv; blk < b1; blk += NW) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            u32x4 raw[4][2], w[2][2];
+            float sc[2];
 #pragma unroll
-        for (int o = 0; o < 2; o++) read(h ^ 1, st + 1, o);
-        const int blk = b0 + st * KW + kb;
-        if (blk < b1) {
-            half_chunk<1, 1>(acc, w[0], w[1], [&](int o, int t) { return raw[h][o][2 + t]; }, [&](int o) { return sc[h][o]; },
-                               [](int) {});
+            for (int o = 0; o < 2; o++) {
+                sc[o] = scale_in(*reinterpret_cast<const uint32_t *>(mine + 64 * 128 + 4 * (32 * o + l32)), blk);
 #pragma unroll
-            for (int o = 0; o < 2; o++) sc[h ^ 1][o] = scale_in(dw[h ^ 1][o], blk + KW);
-            half_chunk<1, 1>(acc, w[1], w[0], [&](int o, int t) { return raw[h ^ 1][o][t]; },
-                               [&](int o) { return sc[h ^ 1][o]; }, [](int) {});
-        }
-    };
-    if (stages) {
+                for (int q = 0; q < 4; q++) raw[q][o] = *reinterpret_cast<const u32x4 *>(mine + piece_at(32 * o + l32, 2 * q + g));
+            }
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read, so the next may be loaded over it
+            if (blk + NW < b1) issue(blk + NW);
 #pragma unroll
-        for (int st = 0; st < D; st++) issue(st);
-        land<(D - 1) * PER>();
+            for (int o = 0; o < 2; o++) w[0][o] = widen8(raw[0][o][0], raw[0][o][1], sc[o]);
 #pragma unroll
-        for (int o = 0; o < 2; o++) {
-            read(0, 0, o);
-            sc[0][o] = scale_in(dw[0][o], b0 + kb);
-            w[0][o] = widen8(raw[0][o][0], raw[0][o][1], sc[0][o]);
-        }
-        for (int st = 0; st < stages; st += 2) {
-            turn(0, st);
-            if (st + 1 < stages) turn(1, st + 1);
+            for (int h = 0; h < 8; h++)  // (the last half converts its own codes again, for nothing)
+                half_chunk<1, 1>(acc, w[h & 1], w[(h & 1) ^ 1],
+                                 [&](int o, int t) { return raw[min(h + 1, 7) / 2][o][2 * (min(h + 1, 7) & 1) + t]; },
+                                 [&](int o) { return sc[o]; }, [](int) {});
         }
     }
-    land<0>();
+    __syncthreads();
     float *out = reinterpret_cast<float *>(sh);
 #pragma unroll
     for (int e = 0; e < 16; e++) out[(wv * 32 + 8 * (e >> 2) + 4 * g + (e & 3)) * LD + l32] = acc[0][0][e];
     __syncthreads();
     const Out to(p, split);
-    constexpr int EACH = 4 / KW;  // values a thread
+    constexpr int EACH = 16 / NW;  // values a thread
     const int c = threadIdx.x % 32, col = n0 + c;
     if (col >= p.n) return;
     const float bias = to.bias_of(col);
     float v[EACH];
 #pragma unroll
     for (int u = 0; u < EACH; u++) {
-        const int r = threadIdx.x / 32 + u * 8 * KW;
+        const int r = threadIdx.x / 32 + u * 2 * NW;
         v[u] = out[r * LD + c];
 #pragma unroll
         for (int w = 1; w < NW; w++) v[u] += out[(w * 32 + r) * LD + c];
     }
 #pragma unroll
     for (int u = 0; u < EACH; u++) {
-        const int row = m0 + threadIdx.x / 32 + u * 8 * KW;
+        const int row = m0 + threadIdx.x / 32 + u * 2 * NW;
         if (row < p.m) to.put(row, col, v[u], bias);
     }
 }
@@ -512,12 +487,12 @@ __global__ void __launch_bounds__(256) k_gemm8_join(Gemm8 p) {
 }
 
 // A kernel's tile and what its workgroups take, in us, with `resident` of them on a CU at most: `fix` a round of those and
-// `each` a workgroup, and for a stage of kw blocks of k `alone` where a CU has one workgroup, `shared` a workgroup where it
-// has more; with every CU busy the clock falls and the caches fill, and a stage takes `chip` a workgroup and CU. Fitted to 4080
-// (products) and 4383 (weight gradients) times over all kernels, splits of k and sizes from 1 to 16384; the choice by them is
-// 0.8 % (0.3 %) behind the best of all those in the mean, 11 % (9 %) at most.
+// `each` a workgroup, and for a block of k `alone` where a CU has one workgroup, `shared` a workgroup where it has more; with
+// every CU busy the clock falls and the caches fill, and a block takes `chip` a workgroup and CU. Fitted to 3402 (products) and
+// 4383 (weight gradients) times over all kernels, splits of k and sizes from 1 to 16384; the choice by them is 0.8 % (0.3 %)
+// behind the best of all those in the mean, 15 % (9 %) at most.
 struct Tile {
-    int bm, bn, kw, resident;
+    int bm, bn, resident;
     float fix, each, alone, shared, chip;
 };
 struct Choice {
@@ -539,11 +514,11 @@ Choice choose(const Tile (&tiles)[N], int cus, int64_t m, int64_t n, int blocks,
         for (int s : {1, 2, 3, 4, 6, 8, 12, 16, 24, 32}) {
             if (s > 1 && (s > most || blocks < least * s)) break;
             if (only_splits && atoi(only_splits) != s) continue;
-            const int per = ((blocks + s - 1) / s + c.kw - 1) / c.kw * c.kw, parts = per ? (blocks + per - 1) / per : 1;
+            const int per = (blocks + s - 1) / s, parts = per ? (blocks + per - 1) / per : 1;
             const double wgs = (double)((m + c.bm - 1) / c.bm) * (double)((n + c.bn - 1) / c.bn) * parts;
-            const double load = std::ceil(wgs / cus), rounds = std::ceil(load / c.resident), stages = per / c.kw;
+            const double load = std::ceil(wgs / cus), rounds = std::ceil(load / c.resident);
             double us = c.fix * rounds + c.each * load +
-                        std::fmax(std::fmax(c.alone * rounds, c.shared * load), c.chip * wgs / cus) * stages;
+                        std::fmax(std::fmax(c.alone * rounds, c.shared * load), c.chip * wgs / cus) * per;
             if (parts > 1) us += join + join_each * parts * (double)m * (double)n * 1e-6;
             if (best.tile < 0 || us < shortest) {
                 shortest = us;
@@ -553,15 +528,15 @@ Choice choose(const Tile (&tiles)[N], int cus, int64_t m, int64_t n, int blocks,
     }
     return best;
 }
-// Blocks of k to a split (whole stages, since a stage's scale bytes are one dword) and the splits that gives.
-inline void split_blocks(int blocks, int kw, int splits, int &per, int &parts) {
-    per = ((blocks + splits - 1) / splits + kw - 1) / kw * kw;
+// Blocks of k to a split and the splits that gives.
+inline void split_blocks(int blocks, int splits, int &per, int &parts) {
+    per = (blocks + splits - 1) / splits;
     parts = blocks > per ? (blocks + per - 1) / per : 1;
 }
 
-constexpr Tile kTiles[] = {{256, 256, 1, 1, 7.85f, 0.37f, 3.003f, 0.447f, 3.436f}, {128, 128, 1, 2, 0.0f, 3.0f, 0.925f, 0.413f, 1.005f},
-                           {128, 64, 1, 3, 0.0f, 1.09f, 0.61f, 0.513f, 0.436f},     {64, 64, 1, 4, 0.07f, 0.49f, 0.425f, 0.293f, 0.308f},
-                           {32, 32, 1, 4, 0.44f, 0.54f, 0.204f, 0.085f, 0.095f},    {32, 32, 2, 2, 0.0f, 1.22f, 0.214f, 0.155f, 0.188f}};
+constexpr Tile kTiles[] = {{256, 256, 1, 10.01f, 0.3f, 2.673f, 0.426f, 3.006f}, {128, 128, 2, 0.0f, 2.66f, 0.856f, 0.42f, 0.99f},
+                           {128, 64, 3, 0.0f, 1.27f, 0.669f, 0.436f, 0.504f},   {64, 64, 4, 0.07f, 0.52f, 0.497f, 0.293f, 0.24f},
+                           {32, 32, 4, 0.47f, 0.33f, 0.08f, 0.088f, 0.095f},    {32, 32, 2, 0.0f, 0.79f, 0.021f, 0.075f, 0.086f}};
 
 om_status gemm8(om_ctx *ctx, Gemm8 p) {
     // Up to 64 rows the thin kernel is the fastest (17 x 2048 x 2048 4.0 us, the best of the others 6.0; 64 x 2048 x 2048 5.2 and
@@ -586,12 +561,12 @@ om_status gemm8(om_ctx *ctx, Gemm8 p) {
         }
         return OM_LAUNCH_CHECK(ctx, "om_gemm8");
     }
-    const Choice ch = choose(kTiles, ctx->num_cus, p.m, p.n, p.blocks, p.a.ldq, 1.96f, 1.06f, 16, 4);
+    const Choice ch = choose(kTiles, ctx->num_cus, p.m, p.n, p.blocks, p.a.ldq, 2.5f, 0.69f, 16, 4);
     OM_REQUIRE(ctx, ch.tile >= 0, "om_gemm8: k is more than a launch takes");
     const Tile &c = kTiles[ch.tile];
     p.tiles_m = (int)(((int64_t)p.m + c.bm - 1) / c.bm);
     p.tiles_n = (int)(((int64_t)p.n + c.bn - 1) / c.bn);
-    split_blocks(p.blocks, c.kw, ch.splits, p.per, p.splits);
+    split_blocks(p.blocks, ch.splits, p.per, p.splits);
     const int64_t wgs = (int64_t)p.tiles_m * p.tiles_n * p.splits;
     const int threads = ch.tile == 0 || ch.tile == 5 ? 512 : 256;
     OM_REQUIRE(ctx, launches(wgs, threads), "om_gemm8: %d x %d is more than a launch takes", p.m, p.n);
@@ -604,8 +579,8 @@ om_status gemm8(om_ctx *ctx, Gemm8 p) {
         case 1: go(k_gemm8<128, 128, 2, 2, 2>); break;
         case 2: go(k_gemm8<128, 64, 2, 2, 3>); break;
         case 3: go(k_gemm8<64, 64, 2, 2, 4>); break;
-        case 4: go(k_gemm8_few<1, 4>); break;
-        default: go(k_gemm8_few<2, 4>); break;
+        case 4: go(k_gemm8_few<4>); break;
+        default: go(k_gemm8_few<8>); break;
     }
     if (p.splits > 1)
         hipLaunchKernelGGL(k_gemm8_join, dim3(om::grid1d((int64_t)p.m * p.n, 256, (int64_t)ctx->num_cus * 8)), dim3(256), 0,
@@ -889,9 +864,9 @@ __global__ void __launch_bounds__(256) k_dw8_join(Dw8 p, unsigned tiles) {
     }
 }
 
-constexpr Tile kTilesDw[] = {{32, 128, 1, 2, 0.78f, 1.56f, 0.817f, 0.702f, 0.648f},
-                             {32, 64, 1, 3, 0.61f, 0.64f, 0.572f, 0.459f, 0.46f},
-                             {32, 32, 1, 2, 0.0f, 0.91f, 0.519f, 0.465f, 0.375f}};
+constexpr Tile kTilesDw[] = {{32, 128, 2, 0.78f, 1.56f, 0.817f, 0.702f, 0.648f},
+                             {32, 64, 3, 0.61f, 0.64f, 0.572f, 0.459f, 0.46f},
+                             {32, 32, 2, 0.0f, 0.91f, 0.519f, 0.465f, 0.375f}};
 
 // Chooses the kernel for p (its tile in `tile`) and fills in the tiles and splits.
 om_status plan_dw8(om_ctx *ctx, Dw8 &p, int &tile) {
@@ -901,7 +876,7 @@ om_status plan_dw8(om_ctx *ctx, Dw8 &p, int &tile) {
     const Tile &c = kTilesDw[tile = ch.tile];
     p.tiles_m = (int)(((int64_t)p.m + c.bm - 1) / c.bm);
     p.tiles_n = (int)(((int64_t)p.n + c.bn - 1) / c.bn);
-    split_blocks(p.blocks, c.kw, ch.splits, p.per, p.splits);
+    split_blocks(p.blocks, ch.splits, p.per, p.splits);
     OM_REQUIRE(ctx, launches((int64_t)p.tiles_m * p.tiles_n * p.splits, 256),
                "om_linear_bwd_x8: in=%d out=%d is more than a launch takes", p.n, p.m);
     return OM_OK;
