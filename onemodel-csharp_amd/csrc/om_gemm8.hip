@@ -375,7 +375,8 @@ template <int NW, int MR>
 __global__ void __launch_bounds__(64 * NW) k_gemm8_thin(Gemm8 p) {
     OM_LDS_POISON();
     typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-    constexpr int ROWS = 16 * (MR + 1), SCALES = (ROWS + 63) / 64, SLOT = ROWS * 128 + SCALES * 256;
+    constexpr int ROWS = 16 * (MR + 1), SLOT = ROWS * 128 + 256;
+    static_assert(ROWS <= 64, "one load of scales");
     constexpr int AT_B = MR * 2048, AT_S = ROWS * 128, OUT = NW * MR * 1024, LDS = NW * SLOT > OUT ? NW * SLOT : OUT;
     __shared__ __attribute__((aligned(16))) char sh[LDS];
     const int lane = threadIdx.x & 63, row = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16;
@@ -391,12 +392,8 @@ __global__ void __launch_bounds__(64 * NW) k_gemm8_thin(Gemm8 p) {
     }
     const uint8_t *qb = p.b.q + (int64_t)n0 * p.b.ldq;
     // scale dwords: A's rows, then B's, and B's again
-    const uint8_t *ss[SCALES];
-#pragma unroll
-    for (int i = 0; i < SCALES; i++) {
-        const int r = 64 * i + lane;
-        ss[i] = r < 16 * MR ? p.a.s + (int64_t)min(r, p.m - 1) * p.a.lds : p.b.s + (int64_t)min(n0 + row, p.n - 1) * p.b.lds;
-    }
+    const uint8_t *ss =
+        lane < 16 * MR ? p.a.s + (int64_t)min(lane, p.m - 1) * p.a.lds : p.b.s + (int64_t)min(n0 + row, p.n - 1) * p.b.lds;
     const char *mine = sh + wv * SLOT;
     const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)sh + (uint32_t)wv * SLOT;
     auto issue = [&](int k) {
@@ -404,8 +401,7 @@ __global__ void __launch_bounds__(64 * NW) k_gemm8_thin(Gemm8 p) {
         for (int i = 0; i < 2 * MR; i++) load_to_lds(p.a.q + (int64_t)k * 128, oa[i], at + 1024 * i);
 #pragma unroll
         for (int i = 0; i < 2; i++) load_to_lds(qb + (int64_t)k * 128, ob[i], at + AT_B + 1024 * i);
-#pragma unroll
-        for (int i = 0; i < SCALES; i++) load_to_lds4(ss[i] + (k & ~3), at + AT_S + 256 * i);
+        load_to_lds4(ss + (k & ~3), at + AT_S);
     };
     floatx4 acc[MR];
 #pragma unroll
@@ -539,12 +535,12 @@ constexpr Tile kTiles[] = {{256, 256, 1, 10.01f, 0.3f, 2.673f, 0.426f, 3.006f}, 
                            {32, 32, 4, 0.47f, 0.33f, 0.08f, 0.088f, 0.095f},    {32, 32, 2, 0.0f, 0.79f, 0.021f, 0.075f, 0.086f}};
 
 om_status gemm8(om_ctx *ctx, Gemm8 p) {
-    // Up to 64 rows the thin kernel is the fastest (17 x 2048 x 2048 4.0 us, the best of the others 6.0; 64 x 2048 x 2048 5.2 and
-    // 6.2) until a wavefront has so many blocks one after the other that the others, or a split of k, are (16 x 16 x 16384 10.5 us
-    // and 7.8, 40 x 256 x 8192 8.6 and 7.8, 64 x 4096 x 4096 9.2 and 8.5).
-    constexpr int kMostBlocks[] = {64, 64, 48, 24};
+    // Up to 48 rows the thin kernel is the fastest (17 x 2048 x 2048 4.0 us, the best of the others 4.9; 40 x 2048 x 2048 4.6 and
+    // 5.0; 64 by such a kernel 5.3 and 5.0) until a wavefront has so many blocks one after the other that the others, or a split
+    // of k, are (16 x 64 x 12000 7.7 us and 6.6, 32 x 256 x 8192 7.3 and 6.9, 40 x 512 x 6000 6.9 and 6.8).
+    constexpr int kMostBlocks[] = {64, 48, 40};
     const int mr = (int)(((int64_t)p.m + 15) / 16);
-    if (mr <= 4 && p.blocks <= kMostBlocks[mr - 1]) {
+    if (mr <= 3 && p.blocks <= kMostBlocks[mr - 1]) {
         const int64_t wgs = ((int64_t)p.n + 15) / 16;
         const int nw = wgs <= ctx->num_cus ? 8 : 4;
         OM_REQUIRE(ctx, launches(wgs, 64 * nw), "om_gemm8: n=%d is more than a launch takes", p.n);
@@ -556,8 +552,7 @@ om_status gemm8(om_ctx *ctx, Gemm8 p) {
         switch (mr) {
             case 1: go(k_gemm8_thin<8, 1>, k_gemm8_thin<4, 1>); break;
             case 2: go(k_gemm8_thin<8, 2>, k_gemm8_thin<4, 2>); break;
-            case 3: go(k_gemm8_thin<8, 3>, k_gemm8_thin<4, 3>); break;
-            default: go(k_gemm8_thin<8, 4>, k_gemm8_thin<4, 4>); break;
+            default: go(k_gemm8_thin<8, 3>, k_gemm8_thin<4, 3>); break;
         }
         return OM_LAUNCH_CHECK(ctx, "om_gemm8");
     }

@@ -156,8 +156,8 @@ PRODUCTS = [(1, 1, 1), (3, 5, 7), (1, 300, 1000), (8, 70, 129), (16, 16, 4096), 
             (260, 1000, 9000), (70, 1000, 5000), (3503, 3501, 300), (6001, 2050, 300), (1537, 2050, 1300), (777, 1000, 9000),
             (1001, 4093, 100), (1001, 1000, 5000), (4099, 33, 16500), (4099, 33, 5000), (130, 1000, 9000), (130, 260, 9000),
             (4093, 4093, 520), (777, 333, 1000), (260, 500, 2000),
-            # up to 64 rows, four and eight wavefronts
-            (16, 4200, 300), (31, 257, 8192), (32, 5000, 200), (48, 4500, 700), (47, 30, 6100), (50, 300, 3000), (64, 4200, 130)]
+            # up to 48 rows, four and eight wavefronts, and past them
+            (16, 4200, 300), (31, 257, 8192), (32, 5000, 200), (48, 4500, 700), (47, 30, 5000), (47, 30, 6100), (50, 300, 3000), (64, 4200, 130)]
 
 
 @pytest.mark.parametrize("m,n,k", PRODUCTS)
