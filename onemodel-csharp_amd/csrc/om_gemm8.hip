@@ -11,7 +11,7 @@
 //
 // Bound: large products by the clock that the card keeps under matrix work (4096^3 107 to 111 us, 1240 to 1285 TFLOP/s; without
 // the loads 101, without the conversions 104; the library's bf16 product, which converts nothing and reads twice the bytes,
-// 105 to 112); small ones by the launch and one chain of loads, 4 to 6 us.
+// 105 to 112); small ones by the launch and one chain of loads, 3 to 6 us.
 #include "om_pack8.hpp"
 
 #include <cmath>
