@@ -485,8 +485,8 @@ __global__ void __launch_bounds__(256) k_gemm8_join(Gemm8 p) {
 // A kernel's tile and what its workgroups take, in us, with `resident` of them on a CU at most: `fix` a round of those and
 // `each` a workgroup, and for a block of k `alone` where a CU has one workgroup, `shared` a workgroup where it has more; with
 // every CU busy the clock falls and the caches fill, and a block takes `chip` a workgroup and CU. Fitted to 3402 (products) and
-// 4383 (weight gradients) times over all kernels, splits of k and sizes from 1 to 16384; the choice by them is 0.8 % (0.3 %)
-// behind the best of all those in the mean, 15 % (9 %) at most.
+// 5844 (weight gradients) times over all kernels, splits of k and sizes from 1 to 16384; the choice by them is 0.8 % (0.3 %)
+// behind the best of all those in the mean, 15 % (19 %) at most.
 struct Tile {
     int bm, bn, resident;
     float fix, each, alone, shared, chip;
@@ -594,7 +594,7 @@ struct Dw8 {
     const float *g;         // [rows, m]
     Packed x;               // [n, rows]
     int rows, m, n, blocks;
-    int full;               // blocks of 128 whole rows that are loaded four columns at a time
+    int full;               // pieces of 128 (k_dw8_few: 64) whole rows that are loaded four columns at a time
     float *dw, *db;
     int acc_dw, acc_db;
     int splits, per;
@@ -615,6 +615,73 @@ __device__ __forceinline__ void split_rest(float r0, float r1, uint32_t &m, uint
     m = oms::pack2(r0, r1);
     asm("" : "+v"(m));
     l = oms::pack2(r0 - __uint_as_float(m << 16), r1 - __uint_as_float(m & 0xFFFF0000u));
+}
+
+// t + the products of `count` rows from k0 on with this lane's column of x (codes cq, scales cx) and of g, on the fp32
+// instruction, two rows at a time.
+__device__ __forceinline__ floatx16 add_rows8(const Dw8 &p, const uint8_t *cq, const uint8_t *cx, int gc, int k0, int count, floatx16 t) {
+    const int g = (threadIdx.x >> 5) & 1;
+#pragma unroll 1
+    for (int end = min(k0 + count, p.rows); k0 < end; k0 += 2) {
+        const int k = min(k0 + g, p.rows - 1);
+        const bool in = k0 + g < p.rows;
+        const float x = decode4(cq[k], scale_of(cx[k >> 7]))[0], gv = p.g[(int64_t)k * p.m + gc];
+        t = __builtin_amdgcn_mfma_f32_32x32x2f32(in ? gv : 0.0f, in ? x : 0.0f, t, 0, 0, 0);
+    }
+    return t;
+}
+
+// The end of a workgroup whose NW wavefronts have a share of k each: their column sums and sums meet in LDS (at least NW * 32 *
+// (32 NT + 1) floats of it, free once all have come here) and are added in order.
+template <int NT, int NW>
+__device__ __forceinline__ void finish_dw8(const Dw8 &p, int split, int tn, int m0, int n0, const floatx16 (&acc)[NT], double cs, char *sh) {
+    constexpr int BN = 32 * NT, LD = BN + 1;
+    const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5, wv = threadIdx.x >> 6;
+    const bool sums = p.db && tn == 0;
+    __syncthreads();
+    if (sums) {
+        cs += __shfl_xor(cs, 32, 64);
+        double *shd = reinterpret_cast<double *>(sh);
+        if (g == 0) shd[wv * 32 + l32] = cs;
+        __syncthreads();
+        const int row = m0 + l32;
+        if (wv == 0 && g == 0 && row < p.m) {
+#pragma unroll
+            for (int i = 1; i < NW; i++) cs += shd[i * 32 + l32];
+            if (p.splits > 1) {
+                p.cs[(int64_t)split * p.m + row] = cs;
+            } else {
+                const float v = (float)cs;
+                p.db[row] = p.acc_db ? p.db[row] + v : v;
+            }
+        }
+        __syncthreads();
+    }
+    float *out = reinterpret_cast<float *>(sh);
+#pragma unroll
+    for (int j = 0; j < NT; j++)
+#pragma unroll
+        for (int e = 0; e < 16; e++) out[(wv * 32 + 8 * (e >> 2) + 4 * g + (e & 3)) * LD + 32 * j + l32] = acc[j][e];
+    __syncthreads();
+    constexpr int STEP = 64 * NW / BN, EACH = 32 / STEP;
+    static_assert(64 * NW % BN == 0 && 32 % STEP == 0, "whole rows to a pass of the threads");
+    const int c = threadIdx.x % BN, col = n0 + c;
+    if (col >= p.n) return;
+    const bool part = p.splits > 1;
+    float *to = part ? p.ws + (int64_t)split * p.m * p.n : p.dw;
+    const bool keep = !part && p.acc_dw;
+#pragma unroll 4
+    for (int u = 0; u < EACH; u++) {
+        const int r = threadIdx.x / BN + u * STEP, row = m0 + r;
+        const float *s = out + r * LD + c;
+        float v = s[0];
+#pragma unroll
+        for (int w = 1; w < NW; w++) v += s[w * 32 * LD];
+        if (row < p.m) {
+            float *d = to + (int64_t)row * p.n + col;
+            *d = keep ? *d + v : v;
+        }
+    }
 }
 
 // A workgroup computes 32 x (32 NT) of dW with four wavefronts: wavefront q has all of it over the q-th 32 k of every block of
@@ -777,15 +844,7 @@ __global__ void __launch_bounds__(256, 2) k_dw8(Dw8 p) {
             floatx16 t;
 #pragma unroll
             for (int e = 0; e < 16; e++) t[e] = 0.0f;
-            auto block = [&](int blk) {
-#pragma unroll 1
-                for (int k0 = blk * 128 + 32 * q, end = min(k0 + 32, p.rows); k0 < end; k0 += 2) {
-                    const int k = min(k0 + g, p.rows - 1);
-                    const bool in = k0 + g < p.rows;
-                    const float x = decode4(cq[k], scale_of(cx[blk]))[0], gv = p.g[(int64_t)k * p.m + gc];
-                    t = __builtin_amdgcn_mfma_f32_32x32x2f32(in ? gv : 0.0f, in ? x : 0.0f, t, 0, 0, 0);
-                }
-            };
+            auto block = [&](int blk) { t = add_rows8(p, cq, cx, gc, blk * 128 + 32 * q, 32, t); };
 #pragma unroll 1
             for (int blk = b0; blk < b1; blk++) block(blk);
             if (tail)
@@ -796,50 +855,133 @@ __global__ void __launch_bounds__(256, 2) k_dw8(Dw8 p) {
                 if (i == j) oms::take_beyond(acc[i], t);
         }
     }
-    __syncthreads();
-    if (sums) {
-        cs += __shfl_xor(cs, 32, 64);
-        double *shd = reinterpret_cast<double *>(sh);
-        if (g == 0) shd[q * 32 + l32] = cs;
-        __syncthreads();
-        const int row = m0 + l32;
-        if (q == 0 && g == 0 && row < p.m) {
+    finish_dw8<NT, 4>(p, split, tn, m0, n0, acc, cs, sh);
+}
+
+// The same for few tiles: 32 x 32 of dW, all of it to each of NW wavefronts, over every NW-th piece of 64 rows, alone: the next
+// piece of g and x is on its way into a wavefront's own part of LDS while this one is multiplied, and nothing meets before the
+// sums do. (300 x 300 x 300: 5.9 us, by the kernel above 6.6; 512 x 512 x 512 6.0 and 6.9; of more columns those above split g for
+// more of x.)
+template <int NW>
+__global__ void __launch_bounds__(64 * NW) k_dw8_few(Dw8 p) {
+    OM_LDS_POISON();
+    constexpr int SS = 2048, GS = SS + 256, SLOT = GS + 8192;  // x, its scales (a load fills 64 dwords), g
+    constexpr int OUT = NW * 32 * 33 * 4, LDS = NW * SLOT > OUT ? NW * SLOT : OUT, STEPS = 9;
+    __shared__ __attribute__((aligned(16))) char sh[LDS];
+    const int lane = threadIdx.x & 63, l32 = lane & 31, g = lane >> 5;
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    int split, tm, tn;
+    tile_of(p.tiles_m, p.tiles_n, gridDim.x, split, tm, tn);
+    const int m0 = 32 * tm, n0 = 32 * tn;
+    // pieces of 64 rows, and (in the last split) the rows behind the last that is taken as one
+    const int full = p.full, last = (p.rows + 63) / 64, c0 = 2 * split * p.per, c1 = min(full, c0 + 2 * p.per), count = max(c1 - c0, 0);
+    const bool tail = split == p.splits - 1 && full < last && wv == count % NW;
+    // x: 16 rows of 64 bytes a load, the four 16-byte pieces of a row permuted so that 16 neighbouring rows' equal pieces stand on
+    // distinct banks. g as above, eight rows a load.
+    const uint8_t *xq = p.x.q + (int64_t)n0 * p.x.ldq, *xs = p.x.s + (int64_t)min(n0 + l32, p.n - 1) * p.x.lds;
+    uint32_t off[2];
 #pragma unroll
-            for (int i = 1; i < 4; i++) cs += shd[i * 32 + l32];
-            if (p.splits > 1) {
-                p.cs[(int64_t)split * p.m + row] = cs;
-            } else {
-                const float v = (float)cs;
-                p.db[row] = p.acc_db ? p.db[row] + v : v;
+    for (int i = 0; i < 2; i++) {
+        const int r = 16 * i + (lane >> 2), piece = (lane ^ (r >> 2)) & 3;
+        off[i] = (uint32_t)min(r, p.n - 1 - n0) * (uint32_t)p.x.ldq + 16 * piece;
+    }
+    const int first4 = max(p.m - 4, 0), gc = min(m0 + l32, p.m - 1);
+    const uint32_t goff = 4u * ((uint32_t)(lane >> 3) * (uint32_t)p.m + (uint32_t)min(m0 + 4 * (lane & 7), first4));
+    const int gat = GS + 2048 * g + 4 * ((l32 & ~3) + min(gc - min(m0 + (l32 & ~3), first4), 3));
+    const char *mine = sh + wv * SLOT;
+    const uint32_t at = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) char *)sh + (uint32_t)wv * SLOT;
+    auto issue = [&](int c) {
+#pragma unroll
+        for (int i = 0; i < 2; i++) load_to_lds(xq + (int64_t)c * 64, off[i], at + 1024 * i);
+        load_to_lds4(xs + ((c >> 1) & ~3), at + SS);
+#pragma unroll
+        for (int i = 0; i < 8; i++) load_to_lds(p.g + ((int64_t)c * 64 + 8 * i) * p.m, goff, at + GS + i * 1024);
+    };
+    floatx16 acc[1];
+#pragma unroll
+    for (int e = 0; e < 16; e++) acc[0][e] = 0.0f;
+    const bool sums = p.db && tn == 0;
+    double cs = 0.0;
+    float raw[2][16], sc, left[2];
+    u32x4 xr[2], wa[2][3], wb[2];
+    // Step v of the operands of half h (16 rows) of a piece: four pairs of g in two steps each, then x.
+    auto prepare = [&](int h, int v) {
+        const int c = h >> 1, t = h & 1;
+        if (v == 8) {
+            wb[t] = widen8(xr[c][2 * t], xr[c][2 * t + 1], sc);
+        } else if (v % 2 == 0) {
+            left[0] = raw[c][8 * t + v];
+            left[1] = raw[c][8 * t + v + 1];
+            wa[t][0][v / 2] = split_first(left[0], left[1]);
+        } else {
+            uint32_t m, l;
+            split_rest(left[0], left[1], m, l);
+            wa[t][1][v / 2] = m;
+            wa[t][2][v / 2] = l;
+        }
+    };
+    auto multiply = [&] {  // the piece in registers
+        if (sums) {  // four chains
+            double part[4] = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+            for (int e = 0; e < 32; e++) part[e & 3] += (double)raw[e >> 4][e & 15];
+            cs += (part[0] + part[1]) + (part[2] + part[3]);
+        }
+#pragma unroll
+        for (int v = 0; v < STEPS; v++) prepare(0, v);
+#pragma unroll
+        for (int h = 0; h < 4; h++)
+#pragma unroll
+            for (int f = 0; f < 3; f++) {
+                acc[0] = oms::mma(wa[h & 1][2 - f], wb[h & 1], acc[0]);
+                if (h < 3)
+#pragma unroll
+                    for (int v = f * STEPS / 3; v < (f + 1) * STEPS / 3; v++) prepare(h + 1, v);
+                __builtin_amdgcn_sched_barrier(0);
             }
-        }
-        __syncthreads();
-    }
-    float *out = reinterpret_cast<float *>(sh);
+    };
+    if (wv < count) {
+        issue(c0 + wv);
+        for (int c = c0 + wv; c < c1; c += NW) {
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            sc = scale_in(*reinterpret_cast<const uint32_t *>(mine + SS + 4 * l32), c >> 1);
 #pragma unroll
-    for (int j = 0; j < NT; j++)
+            for (int q = 0; q < 2; q++) xr[q] = *reinterpret_cast<const u32x4 *>(mine + 64 * l32 + (((2 * q + g) ^ (l32 >> 2)) & 3) * 16);
 #pragma unroll
-        for (int e = 0; e < 16; e++) out[(q * 32 + 8 * (e >> 2) + 4 * g + (e & 3)) * LD + 32 * j + l32] = acc[j][e];
-    __syncthreads();
-    constexpr int STEP = 256 / BN, EACH = 32 / STEP;
-    static_assert(256 % BN == 0 && 32 % STEP == 0, "whole rows to a pass of the threads");
-    const int c = threadIdx.x % BN, col = n0 + c;
-    if (col >= p.n) return;
-    const bool part = p.splits > 1;
-    float *to = part ? p.ws + (int64_t)split * p.m * p.n : p.dw;
-    const bool keep = !part && p.acc_dw;
-#pragma unroll 4
-    for (int u = 0; u < EACH; u++) {
-        const int r = threadIdx.x / BN + u * STEP, row = m0 + r;
-        const float *s = out + r * LD + c;
-        float v = s[0];
-#pragma unroll
-        for (int w = 1; w < 4; w++) v += s[w * 32 * LD];
-        if (row < p.m) {
-            float *d = to + (int64_t)row * p.n + col;
-            *d = keep ? *d + v : v;
+            for (int e = 0; e < 32; e++) raw[e >> 4][e & 15] = *reinterpret_cast<const float *>(mine + gat + 4096 * (e >> 4) + 128 * (e & 15));
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // read, so the next may be loaded over it
+            if (c + NW < c1) issue(c + NW);
+            multiply();
         }
     }
+    const int64_t xcol = min(n0 + l32, p.n - 1);
+    const uint8_t *cq = p.x.q + xcol * p.x.ldq, *cx = p.x.s + xcol * p.x.lds;
+#pragma unroll 1
+    for (int c = tail ? full : last; c < last; c++) {  // the rows behind, straight from memory
+#pragma unroll
+        for (int e = 0; e < 32; e++) {
+            const int k = c * 64 + 32 * (e >> 4) + 16 * g + (e & 15);
+            const float v = p.g[(int64_t)min(k, p.rows - 1) * p.m + gc];
+            raw[e >> 4][e & 15] = k < p.rows ? v : 0.0f;
+        }
+#pragma unroll
+        for (int q = 0; q < 2; q++) xr[q] = *reinterpret_cast<const u32x4 *>(cq + (int64_t)c * 64 + 32 * q + 16 * g);
+        sc = scale_of(cx[c >> 1]);
+        multiply();
+    }
+    unsigned big = 0;
+#pragma unroll
+    for (int e = 0; e < 16; e++) oms::note(acc[0][e], big);
+    if (oms::beyond(big)) {  // this wavefront's k again
+        floatx16 t;
+#pragma unroll
+        for (int e = 0; e < 16; e++) t[e] = 0.0f;
+#pragma unroll 1
+        for (int c = c0 + wv; c < c1; c += NW) t = add_rows8(p, cq, cx, gc, c * 64, 64, t);
+        if (tail) t = add_rows8(p, cq, cx, gc, full * 64, (last - full) * 64, t);
+        oms::take_beyond(acc[0], t);
+    }
+    finish_dw8<1, NW>(p, split, tn, m0, n0, acc, cs, sh);
 }
 
 // Adds the parts in order: dW's, and by the workgroups from `tiles` on the column sums'.
@@ -859,20 +1001,23 @@ __global__ void __launch_bounds__(256) k_dw8_join(Dw8 p, unsigned tiles) {
     }
 }
 
-constexpr Tile kTilesDw[] = {{32, 128, 2, 0.78f, 1.56f, 0.817f, 0.702f, 0.648f},
-                             {32, 64, 3, 0.61f, 0.64f, 0.572f, 0.459f, 0.46f},
-                             {32, 32, 2, 0.0f, 0.91f, 0.519f, 0.465f, 0.375f}};
+constexpr Tile kTilesDw[] = {{32, 128, 2, 0.71f, 1.75f, 0.794f, 0.696f, 0.663f},
+                             {32, 64, 3, 0.83f, 0.65f, 0.525f, 0.429f, 0.456f},
+                             {32, 32, 2, 0.0f, 0.61f, 0.523f, 0.38f, 0.375f},
+                             {32, 32, 1, 0.3f, 0.55f, 0.31f, 0.314f, 0.348f}};
 
 // Chooses the kernel for p (its tile in `tile`) and fills in the tiles and splits.
 om_status plan_dw8(om_ctx *ctx, Dw8 &p, int &tile) {
-    const Choice ch = choose(kTilesDw, ctx->num_cus, p.m, p.n, p.blocks, p.x.ldq, 2.63f, 1.0f, 32, 2);
+    const Choice ch = choose(kTilesDw, ctx->num_cus, p.m, p.n, p.blocks, p.x.ldq, 2.14f, 0.92f, 32, 2);
     OM_REQUIRE(ctx, ch.tile >= 0 && p.rows <= INT32_MAX - 255 && p.m < 1 << 26,
                "om_linear_bwd_x8: rows=%d in=%d out=%d is more than a launch takes", p.rows, p.n, p.m);
     const Tile &c = kTilesDw[tile = ch.tile];
     p.tiles_m = (int)(((int64_t)p.m + c.bm - 1) / c.bm);
     p.tiles_n = (int)(((int64_t)p.n + c.bn - 1) / c.bn);
     split_blocks(p.blocks, ch.splits, p.per, p.splits);
-    OM_REQUIRE(ctx, launches((int64_t)p.tiles_m * p.tiles_n * p.splits, 256),
+    const int piece = tile == 3 ? 64 : 128;
+    p.full = p.m >= 4 ? p.rows / piece : p.rows > 3 ? (p.rows - 3) / piece : 0;  // four of fewer columns end up to three rows on
+    OM_REQUIRE(ctx, launches((int64_t)p.tiles_m * p.tiles_n * p.splits, tile == 3 ? 512 : 256),
                "om_linear_bwd_x8: in=%d out=%d is more than a launch takes", p.n, p.m);
     return OM_OK;
 }
@@ -884,12 +1029,13 @@ om_status dw8(om_ctx *ctx, Dw8 p, int tile) {
         p.cs = reinterpret_cast<double *>(p.ws + sums);
     }
     auto go = [&](auto kern) {
-        hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)p.tiles_m * p.tiles_n * p.splits)), dim3(256), 0, ctx->stream, p);
+        hipLaunchKernelGGL(kern, dim3((unsigned)((int64_t)p.tiles_m * p.tiles_n * p.splits)), dim3(tile == 3 ? 512 : 256), 0, ctx->stream, p);
     };
     switch (tile) {
         case 0: go(k_dw8<4, 2>); break;
         case 1: go(k_dw8<2, 2>); break;
-        default: go(k_dw8<1, 3>); break;
+        case 2: go(k_dw8<1, 3>); break;
+        default: go(k_dw8_few<8>); break;
     }
     if (p.splits > 1) {
         const unsigned tiles = om::grid1d((int64_t)p.m * p.n, 256, (int64_t)ctx->num_cus * 8), sums = p.db ? (p.m + 255) / 256 : 0;
@@ -935,7 +1081,6 @@ om_status om_linear_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *xt8, cons
         p.g = g;
         p.x = packed(xt8, in, rows);
         p.rows = rows, p.m = out, p.n = in, p.blocks = (int)blocks8(rows);
-        p.full = out >= 4 ? rows / 128 : rows > 3 ? (rows - 3) / 128 : 0;  // four of fewer columns end up to three rows on
         p.dw = dw, p.db = db, p.acc_dw = acc_dw, p.acc_db = acc_db;
         if (om_status s = plan_dw8(ctx, p, tile)) return s;
     }

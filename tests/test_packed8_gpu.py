@@ -253,7 +253,8 @@ DW = [(1, 1, 1), (2, 3, 5), (37, 20, 33), (127, 64, 64), (128, 128, 128), (129, 
       # fewer than four columns of g, and rows just past whole blocks
       (129, 20, 1), (257, 40, 2), (384, 33, 3), (130, 7, 1), (131, 9, 2), (3, 5, 2), (512, 140, 1), (300, 50, 5), (640, 64, 70),
       # every tile with the rows in one part and in several, the last of them short
-      (100, 1537, 1000), (2600, 260, 777), (5003, 777, 130), (9001, 130, 130), (5003, 1, 1), (9001, 260, 33), (9001, 33, 2)]
+      (100, 1537, 1000), (2600, 260, 777), (5003, 777, 130), (9001, 130, 130), (5003, 1, 1), (9001, 260, 33), (9001, 33, 2),
+      (2600, 1000, 260), (5003, 500, 1000), (9001, 1000, 500), (16390, 260, 500), (300, 300, 300), (1300, 33, 260), (16390, 20, 5)]
 
 
 @pytest.mark.parametrize("rows,inp,out", DW)
