@@ -145,14 +145,14 @@ __device__ __forceinline__ int wave_imax(int v) { return (int)(wave_umax((uint32
 __device__ __forceinline__ int wave_imin(int v) { return ~wave_imax(~v); }
 
 // 16 (or 4) bytes per lane from `src` (this lane's address) to LDS at byte address lds + 16 (4) * lane, without registers. m0
-// holds the address for this one instruction only; nothing else in these kernels reads it. Loads land in the order of
-// their issue; land<N>() waits until at most this wavefront's last N are in flight and its own LDS reads are done, then
-// meets the others.
+// holds the address for this one instruction only, which needs a wait state (s_nop 0) between the write and its read; nothing else
+// in these kernels reads it. Loads land in the order of their issue; land<N>() waits until at most this wavefront's last N are in
+// flight and its own LDS reads are done, then meets the others.
 __device__ __forceinline__ void load_to_lds(const void *src, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
 }
 __device__ __forceinline__ void load_to_lds4(const void *src, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
 }
 template <int N>
 __device__ __forceinline__ void land() {

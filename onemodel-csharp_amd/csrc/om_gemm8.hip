@@ -39,18 +39,18 @@ __device__ __forceinline__ u32x4 widen8(uint32_t w0, uint32_t w1, float scale) {
 }
 
 // 16 (or 4) bytes a lane from base (uniform) + off (this lane's) to LDS at byte address lds + 16 (4) * lane, without registers. m0
-// holds the address for this one instruction only; nothing else in these kernels reads it. Loads land in the order of their
-// issue; land<N>() waits until at most this wavefront's last N are in flight and its own LDS reads are done, then meets the
-// others.
+// holds the address for this one instruction only, which needs a wait state (s_nop 0) between the write and its read; nothing else
+// in these kernels reads it. Loads land in the order of their issue; land<N>() waits until at most this wavefront's last N are in
+// flight and its own LDS reads are done, then meets the others.
 __device__ __forceinline__ void load_to_lds(const void *base, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
 }
 __device__ __forceinline__ void load_to_lds4(const void *base, uint32_t off, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %2\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dword %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory", "m0");
 }
 // The same with an address to each lane.
 __device__ __forceinline__ void load_to_lds4(const void *src, uint32_t lds) {
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dword %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
 }
 template <int N>
 __device__ __forceinline__ void land() {

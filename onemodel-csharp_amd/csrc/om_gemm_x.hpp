@@ -436,11 +436,12 @@ __device__ __forceinline__ void dma_chunk(const float *src, int64_t ld, unsigned
     constexpr int CH = BKT / 4;  // float4 chunks per row
     // m0 is a reserved register: the compiler warns that it does not keep a value of its own in m0 across this
     // statement. That is safe here because nothing else in these kernels reads m0 (no LDS-direct or
-    // relative-indexing instructions in their assembly), so each load's m0 is the one set just before it.
+    // relative-indexing instructions in their assembly), so each load's m0 is the one set just before it. A load into LDS may
+    // read m0 one wait state after a scalar write of it at the earliest: s_nop 0, which the compiler cannot put in here.
 #pragma unroll
     for (int j = 0; j < INSTR / 4; j++) {
         const float *g = src + (int64_t)j * (256 / CH) * ld;
-        asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds + j * 4096u)
+        asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(g), "s"(lds + j * 4096u)
                      : "memory", "m0");
     }
 }
