@@ -341,7 +341,13 @@ om_status om_layernorm_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *xh8, c
     if (!dx && !dgamma && !dbeta) return OM_OK;
     OM_REQUIRE(ctx, cols <= 65535 * 1024 && (cols <= kKeptBwd || launches(rows, 256)),
                "om_layernorm_bwd_x8: %d x %d is more than a launch takes", rows, cols);
+    if (rows == 0 && acc_params) return OM_OK;
     if (om_status s = om::use_device(ctx)) return s;
+    if (rows == 0) {  // empty sums
+        if (dgamma)
+            if (om_status s = om_fill(ctx, dgamma, 0.0f, cols)) return s;
+        return dbeta ? om_fill(ctx, dbeta, 0.0f, cols) : OM_OK;
+    }
     const int chunk = rows_each(rows, cols, ctx->num_cus), chunks = (int)(((int64_t)rows + chunk - 1) / chunk);
     const bool one = chunks == 1 && cols <= kKeptBwd;
     double *pg = nullptr, *pb = nullptr;
@@ -353,27 +359,26 @@ om_status om_layernorm_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *xh8, c
         pb = dbeta ? base + (uint64_t)chunks * (uint64_t)cols : nullptr;
     }
     const Packed p = packed(xh8, rows, cols);
-    if (rows)
-        by_width(cols, kKeptBwd, [&](auto nw, auto nv) {
-            constexpr int NW = decltype(nw)::value, NV = decltype(nv)::value;
-            if constexpr (NV && 256 * NW * NV <= kKeptBwd) {
-                auto go = [&](auto kern) {
-                    hipLaunchKernelGGL(kern, dim3((unsigned)chunks), dim3(kBwdThreads<NW, NV>), 0, ctx->stream, g, p, gamma, rstd, dx,
-                                       Sums{pg, one ? dgamma : nullptr, acc_params}, Sums{pb, one ? dbeta : nullptr, acc_params},
-                                       (int64_t)rows, (int64_t)cols, chunk);
-                };
-                acc_dx ? go(k_ln8_bwd<NW, NV, true>) : go(k_ln8_bwd<NW, NV, false>);
-            } else if constexpr (!NV) {
-                auto go = [&](auto kern) {
-                    hipLaunchKernelGGL(kern, dim3((unsigned)rows), dim3(256), 0, ctx->stream, g, p, gamma, rstd, dx,
-                                       (int64_t)cols);
-                };
-                if (pg || pb)
-                    hipLaunchKernelGGL(k_ln8_params_long, dim3((unsigned)chunks, (unsigned)((cols + 1023) / 1024)), dim3(256),
-                                       0, ctx->stream, g, p, pg, pb, (int64_t)rows, (int64_t)cols, chunk);
-                if (dx) acc_dx ? go(k_ln8_dx_long<true>) : go(k_ln8_dx_long<false>);  // last: dx may be g
-            }
-        });
+    by_width(cols, kKeptBwd, [&](auto nw, auto nv) {
+        constexpr int NW = decltype(nw)::value, NV = decltype(nv)::value;
+        if constexpr (NV && 256 * NW * NV <= kKeptBwd) {
+            auto go = [&](auto kern) {
+                hipLaunchKernelGGL(kern, dim3((unsigned)chunks), dim3(kBwdThreads<NW, NV>), 0, ctx->stream, g, p, gamma, rstd, dx,
+                                   Sums{pg, one ? dgamma : nullptr, acc_params}, Sums{pb, one ? dbeta : nullptr, acc_params},
+                                   (int64_t)rows, (int64_t)cols, chunk);
+            };
+            acc_dx ? go(k_ln8_bwd<NW, NV, true>) : go(k_ln8_bwd<NW, NV, false>);
+        } else if constexpr (!NV) {
+            auto go = [&](auto kern) {
+                hipLaunchKernelGGL(kern, dim3((unsigned)rows), dim3(256), 0, ctx->stream, g, p, gamma, rstd, dx,
+                                   (int64_t)cols);
+            };
+            if (pg || pb)
+                hipLaunchKernelGGL(k_ln8_params_long, dim3((unsigned)chunks, (unsigned)((cols + 1023) / 1024)), dim3(256),
+                                   0, ctx->stream, g, p, pg, pb, (int64_t)rows, (int64_t)cols, chunk);
+            if (dx) acc_dx ? go(k_ln8_dx_long<true>) : go(k_ln8_dx_long<false>);  // last: dx may be g
+        }
+    });
     if (om_status s = OM_LAUNCH_CHECK(ctx, "om_layernorm_bwd_x8")) return s;
     if (one) return OM_OK;
     if (dgamma && dbeta) return om::chunk_final(ctx, pg, chunks, cols, dgamma, acc_params, pb, dbeta);
