@@ -293,8 +293,7 @@ __global__ void __launch_bounds__(1024) k_colsum_one(const float *__restrict__ g
 // 16 columns (a 128-byte line of partials) to a workgroup: group w of 16 lanes adds chunk partials c = w, w + 64, ..., eight
 // loads in flight before their adds, and the 64 groups' sums meet pairwise, w + 32 first: the additions of column_sum_wave's
 // first lane, in its order, with every line read whole (a wavefront to a column read 8 bytes of each: 8.3 us in place of
-// 4.6 for 256 chunks of 4096 columns). Used by every two-stage column reduction of the library (bias, LayerNorm and
-// convolution-bias gradients).
+// 4.6 for 256 chunks of 4096 columns).
 __global__ void __launch_bounds__(1024) om_k_chunk_final(const double *__restrict__ part, float *__restrict__ out,
                                                          const double *__restrict__ part2, float *__restrict__ out2,
                                                          int chunks, int cols, int acc) {
@@ -327,10 +326,28 @@ __global__ void __launch_bounds__(1024) om_k_chunk_final(const double *__restric
     }
 }
 
+// The same for few columns, a wavefront each.
+__global__ void __launch_bounds__(256) om_k_chunk_final_few(const double *__restrict__ part, float *__restrict__ out,
+                                                            const double *__restrict__ part2, float *__restrict__ out2,
+                                                            int chunks, int cols, int acc) {
+    OM_LDS_POISON();
+    const int col = (blockIdx.x * 256 + threadIdx.x) >> 6, lane = threadIdx.x & 63;
+    if (col >= cols) return;
+    omd::column_sum_wave(blockIdx.y ? part2 : part, blockIdx.y ? out2 : out, chunks, cols, col, acc, lane);
+}
+
+// The last stage of every two-stage column reduction of the library (bias, LayerNorm and convolution-bias gradients).
 om_status om::chunk_final(om_ctx *ctx, const double *part, int chunks, int cols, float *out, int acc,
                           const double *part2, float *out2) {
-    hipLaunchKernelGGL(om_k_chunk_final, dim3((unsigned)(((int64_t)cols + 15) / 16), part2 ? 2 : 1), dim3(1024), 0,
-                       om::cur_stream(ctx), part, out, part2, out2, chunks, cols, acc);
+    // Workgroups of 16 columns unless the only one is not full or a second one has four at most (om_colsum of 1000 chunks, us, by
+    // workgroups and by wavefronts: 1 column 8.8 and 7.2, 8 9.1 and 8.3, 16 9.0 and 9.6, 18 9.4 and 8.9, 22 9.2 and 9.6, 128 10.7
+    // and 13.8; of 64 chunks 1 column 6.1 and 5.6, 18 6.8 and 6.4, 64 6.7 and 6.6).
+    if (cols <= 20 && cols != 16)
+        hipLaunchKernelGGL(om_k_chunk_final_few, dim3((cols + 3) / 4, part2 ? 2 : 1), dim3(256), 0, om::cur_stream(ctx), part, out,
+                           part2, out2, chunks, cols, acc);
+    else
+        hipLaunchKernelGGL(om_k_chunk_final, dim3((unsigned)(((int64_t)cols + 15) / 16), part2 ? 2 : 1), dim3(1024), 0,
+                           om::cur_stream(ctx), part, out, part2, out2, chunks, cols, acc);
     return OM_LAUNCH_CHECK(ctx, "column reduction");
 }
 
@@ -680,8 +697,9 @@ om_status om_colsum(om_ctx *ctx, const float *g, float *db, int rows, int cols, 
     OM_REQUIRE(ctx, g && db && rows >= 0 && cols > 0, "om_colsum: bad arguments");
     if (rows == 0) return om_fill(ctx, db, 0.0f, accumulate ? 0 : cols);
     int chunks = (rows + kColChunk - 1) / kColChunk;
-    // One launch where it is the shorter (777 x 333 5.1 us and 6.6 in two, 1024 x 2048 5.4 and 6.1; 1024 x 4096 6.4 and 6.3,
-    // 64 x 16384 8.7 and 7.6).
+    // One launch where it is the shorter (launch behind launch with g in the caches: 777 x 333 5.1 us and 6.6 in two, 1024 x 2048
+    // 5.4 and 6.1; 1024 x 4096 6.4 and 6.3, 64 x 16384 8.7 and 7.6. The kernels alone by the profiler: 777 x 333 4.9 us, in two
+    // 4.2 + 2.6; with g read from HBM 10.4, in two 9.7 + 4.0).
     if (chunks <= 16 && cols <= 8192 && (int64_t)rows * cols <= 2 << 20) {
         hipLaunchKernelGGL(k_colsum_one, dim3((unsigned)(((int64_t)cols + 15) / 16)), dim3(1024), 0, om::cur_stream(ctx), g, rows,
                            cols, chunks, db, accumulate);
@@ -691,8 +709,10 @@ om_status om_colsum(om_ctx *ctx, const float *g, float *db, int rows, int cols, 
     om_status s = om::scratch(ctx, sizeof(double) * (uint64_t)chunks * cols, &scr);
     if (s) return s;
     double *part = reinterpret_cast<double *>(scr);
-    // wide loads from a million values on; below that fewer, longer workgroups cost 0.3 us of 7
-    if (cols >= 128 && (int64_t)rows * cols >= 1 << 20)
+    // Wide loads where each of their workgroups has all of its 256 columns (4096 x 256 6.2 us, single columns 6.8) from a million
+    // values on, and where it has not from three million on: before that their fewer, longer workgroups are the slower (4096 x
+    // 384 7.3 us and 6.9, 8192 x 128 7.3 and 6.7, 16384 x 192 7.6 and 7.5; 16320 x 257 7.7 and 11.0, 32768 x 128 8.1 and 8.2).
+    if (cols >= 128 && (int64_t)rows * cols >= (cols % 256 == 0 ? 1 << 20 : 3 << 20))
         hipLaunchKernelGGL(k_colsum_partial4, dim3((unsigned)(((int64_t)cols + 255) / 256), chunks), dim3(kBlock), 0,
                            om::cur_stream(ctx), g, rows, cols, part);
     else
