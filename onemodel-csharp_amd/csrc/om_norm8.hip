@@ -320,15 +320,18 @@ om_status om_layernorm_fwd_x8(om_ctx *ctx, const float *x, const float *gamma, c
     OM_REQUIRE(ctx, aligned16(xh8), "om_layernorm_fwd_x8: packed tensors start at multiples of 16 bytes");
     if (rows == 0) return OM_OK;
     OM_REQUIRE(ctx, x && gamma && beta && y && xh8 && rstd, "om_layernorm_fwd_x8: NULL pointer");
-    OM_REQUIRE(ctx, cols <= kOneWave ? launches(((int64_t)rows + 3) / 4, 256) : launches(rows, 1024),
-               "om_layernorm_fwd_x8: %d x %d is more than a launch takes", rows, cols);
-    if (om_status s = om::use_device(ctx)) return s;
     const Packed p = packed(xh8, rows, cols);
+    om_status status = OM_OK;
     by_width(cols, kKeptFwd, [&](auto nw, auto nv) {
-        constexpr int NW = decltype(nw)::value, NV = decltype(nv)::value;
-        hipLaunchKernelGGL((k_ln8<NW, NV>), dim3((unsigned)(NW == 1 ? ((int64_t)rows + 3) / 4 : rows)), dim3(NW == 1 ? 256 : 64 * NW), 0, ctx->stream, x,
-                           gamma, beta, y, p, rstd, (int64_t)rows, (int64_t)cols, eps, 1.0 / cols);
+        constexpr int NW = decltype(nw)::value, NV = decltype(nv)::value, threads = NW == 1 ? 256 : 64 * NW;
+        const int64_t groups = NW == 1 ? ((int64_t)rows + 3) / 4 : rows;
+        status = launches(groups, threads) ? om::use_device(ctx)
+                                           : om::fail(ctx, OM_E_ARG, "om_layernorm_fwd_x8: %d x %d is more than a launch takes", rows, cols);
+        if (status) return;
+        hipLaunchKernelGGL((k_ln8<NW, NV>), dim3((unsigned)groups), dim3(threads), 0, ctx->stream, x, gamma, beta, y, p, rstd,
+                           (int64_t)rows, (int64_t)cols, eps, 1.0 / cols);
     });
+    if (status) return status;
     return OM_LAUNCH_CHECK(ctx, "om_layernorm_fwd_x8");
 }
 
