@@ -1071,9 +1071,13 @@ om_status om_linear_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *xt8, cons
     OM_REQUIRE(ctx, rows == 0 || (g && (!dx || w) && (!dw || xt8)), "om_linear_bwd_x8: a needed tensor is NULL");
     if (!dx && !dw && !db) return OM_OK;
     if (rows == 0) {  // empty sums
-        if (dw && !acc_dw)
+        if (acc_dw) dw = nullptr;
+        if (acc_db) db = nullptr;
+        if (!dw && !db) return OM_OK;
+        if (om_status s = om::use_device(ctx)) return s;
+        if (dw)
             if (om_status s = om_fill(ctx, dw, 0.0f, (int64_t)in * out)) return s;
-        return db && !acc_db ? om_fill(ctx, db, 0.0f, out) : OM_OK;
+        return db ? om_fill(ctx, db, 0.0f, out) : OM_OK;
     }
     Dw8 p = {};
     int tile = 0;

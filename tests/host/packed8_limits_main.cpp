@@ -57,5 +57,12 @@ int main() {
     say("om_layernorm_bwd_x8-long", om_layernorm_bwd_x8(&ctx, x, q, x, x, x, x, x, 1 << 24, 8193, 0, 0));
     say("take-norm-bwd-wide", om_layernorm_bwd_x8(&ctx, x, q, x, x, x, x, x, 1, 65535 * 1024, 0, 0));
     say("om_layernorm_bwd_x8-wide", om_layernorm_bwd_x8(&ctx, x, q, x, x, x, x, x, 1, 65535 * 1024 + 1, 0, 0));
+
+    // no rows: outputs that are kept need no device, outputs that are zeroed need the context's own
+    say("ok-norm-no-rows", om_layernorm_bwd_x8(&ctx, nullptr, nullptr, nullptr, nullptr, nullptr, x, x, 0, 8, 0, 1));
+    say("take-norm-no-rows", om_layernorm_bwd_x8(&ctx, nullptr, nullptr, nullptr, nullptr, nullptr, x, x, 0, 8, 0, 0));
+    say("ok-linear-no-rows", om_linear_bwd_x8(&ctx, nullptr, nullptr, nullptr, nullptr, x, x, 0, 4, 4, 0, 1, 1));
+    say("take-linear-no-rows", om_linear_bwd_x8(&ctx, nullptr, nullptr, nullptr, nullptr, x, x, 0, 4, 4, 0, 0, 1));
+    say("take-linear-no-rows-db", om_linear_bwd_x8(&ctx, nullptr, nullptr, nullptr, nullptr, nullptr, x, 0, 4, 4, 0, 0, 0));
     return 0;
 }

@@ -58,3 +58,7 @@ def test_layernorm_forward(lines):
 
 def test_layernorm_backward(lines):
     _check([line for line in lines if "norm-bwd" in line[0] or line[0].startswith("om_layernorm_bwd")], "", 5)
+
+
+def test_no_rows(lines):
+    _check(lines, "no-rows", 5)
