@@ -379,8 +379,10 @@ om_status om_layernorm_bwd_partials(om_ctx *ctx, const float *g, const float *x,
  * Layout: `rows` rows of codes of S = 128 ceil(cols / 128) bytes, zeros behind the last column, then `rows` rows of scale
  * bytes e + 127 of T = 4 ceil(S / 512) bytes, zeros behind the last block; om_pack8_bytes gives rows * (S + T), 0 where rows
  * or cols is not positive. Packed tensors start at multiples of 16 bytes (om_alloc's do). A block is 128 wide whatever cols
- * is, so a narrow tensor is best viewed as a wide one first. Sizes that a launch cannot hold (2^32 threads: packed tensors of
- * 34 GB and more in practice) are refused, and so is k (rows of om_linear_bwd_x8) from 2^27 on.
+ * is, so a narrow tensor is best viewed as a wide one first. Sizes that a launch cannot hold (2^32 threads) are refused before
+ * anything is launched: packed tensors of 2^28 blocks (34 GB) and more, for a transpose 2^22 squares of 128 x 128 values; for
+ * LayerNorm more than 2^26 - 4 rows (2^24 - 1 past 1024 columns, 2^23 - 1 past 4096, 2^22 - 1 past 8192; its backward 2^24 - 1 rows
+ * past 8192 columns, and 65535 * 1024 columns); k, and the rows that a dw sums over, above 2^27 - 128; out above 2^26 - 1 for a dw.
  * Where an entry point says x8 its rows are packed; xt8 is the packed transpose, [cols, rows], whose blocks run along the
  * rows of x: a product takes each operand packed along the dimension it sums over. */
 uint64_t om_pack8_bytes(int rows, int cols);
@@ -395,9 +397,9 @@ om_status om_unpack8(om_ctx *ctx, const uint8_t *x8, float *y, int ld_y, int row
  * dx = om_gemm8(rows, in, out, g8, wt8), dw = om_gemm8(out, in, rows, gt8, xt8), db = om_colsum(g). */
 om_status om_gemm8(om_ctx *ctx, int m, int n, int k, const uint8_t *a8, const uint8_t *b8, const float *bias, float *c,
                    int ldc, int acc);
-/* om_linear_bwd with the layer's input kept as xt8, the packed transpose of x [rows, in]: dw (+)= g^T x (every product
- * exact but for bits of g below 2^-126, sums fp32) and db (+)= fp64 column sums of g; dx (+)= g w is om_linear_bwd's. Each
- * output may be NULL. */
+/* om_linear_bwd with the layer's input kept as xt8, the packed transpose of x [rows, in]: dw (+)= g^T x (every product exact
+ * but for bits of g and values of x below 2^-126, which may count as zero; sums fp32) and db (+)= fp64 column sums of g; dx (+)=
+ * g w is om_linear_bwd's. Each output may be NULL. */
 om_status om_linear_bwd_x8(om_ctx *ctx, const float *g, const uint8_t *xt8, const float *w, float *dx, float *dw, float *db,
                            int rows, int in, int out, int acc_dx, int acc_dw, int acc_db);
 /* om_gelu_fwd over [rows, cols] that keeps its input packed, and its backward from that: dx (+)= g * gelu'(value of x8).
