@@ -3,9 +3,11 @@
 //
 // Arithmetic. An e4m3 code times a power of two is a bf16 value (4 significand bits of 8), so the codes are widened in
 // registers, v_cvt_scalef32_pk_bf16_fp8 with the block's scale, and multiplied by v_mfma_f32_32x32x16_bf16: every product is
-// exact and sums are fp32 (2-norm error 1e-7 at k = 4096). The 8-bit matrix instructions have up to twice the rate, but do
-// not keep their sums: a 128-term dot product comes out 1.5e-5 off in the 2-norm (normal values; 5e-5 with all exponents in
-// use), as their adder drops what is 2^-13 or so below its largest term. The conversion costs two to three vector
+// exact and sums are fp32 (2-norm error 1e-7 at k = 4096). The 8-bit matrix instructions have up to twice the rate (bare
+// instructions, scaled 32x32x64 4590 TFLOP/s, bf16 32x32x16 2170), but do not keep their sums: a dot product comes out 1.2e-5 off
+// in the 2-norm over 32 terms, 1.5e-5 over 128 and over 4096 (normal values; 4e-5 to 5e-5 with all exponents in use), as if their
+// adder dropped what is 2^-13 or so below its largest term. That does not grow with k: to keep exact products and fp32 sums is a
+// choice, paid with up to half the rate of large products. The conversion costs two to three vector
 // instructions an MFMA at 64 x 64 to 128 x 64 values a wavefront and runs beside it (16 k of both: 15.4 ns an MFMA alone,
 // 16.6 with six conversions to each).
 //
@@ -801,8 +803,8 @@ __global__ void __launch_bounds__(256, 2) k_dw8(Dw8 p) {
 
 // The same for few tiles: 32 x 32 of dW, all of it to each of NW wavefronts, over every NW-th piece of 64 rows, alone: the next
 // piece of g and x is on its way into a wavefront's own part of LDS while this one is multiplied, and nothing meets before the
-// sums do. (300 x 300 x 300: 5.9 us, by the kernel above 6.6; 512 x 512 x 512 6.0 and 6.9; of more columns those above split g for
-// more of x.)
+// sums do. (300 x 300 x 300: 5.2 us, by the kernel above 6.1; 512 x 512 x 512 5.2 and 6.3; of more columns those above split g for
+// more of x: 1000 x 1000 x 1000 21.6, 13.4 by 32 x 128.)
 template <int NW>
 __global__ void __launch_bounds__(64 * NW) k_dw8_few(Dw8 p) {
     OM_LDS_POISON();
